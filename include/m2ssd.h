@@ -38,6 +38,9 @@ extern "C" {
 /* element types */
 #define M2_F32  0
 #define M2_BF16 1
+/* index types (token ids and targets only) */
+#define M2_I32  2
+#define M2_I64  3
 
 /* ---------------------------------------------------------------------------
  * chunk_cumsum: dt' = clip(softplus?(dt + dt_bias), dt_min, dt_max) (0 past
@@ -433,6 +436,124 @@ typedef struct {
     m2_causal_conv1d_update_args conv;
 } m2_skinny_gemm_norm_args;
 int m2_skinny_gemm_norm(const m2_skinny_gemm_norm_args* a, void* stream);
+
+/* ---------------------------------------------------------------------------
+ * embedding: out[n] = scale * weight[ids[n]], the products in float32, rounded
+ * once.  An id outside [0, vocab) reads nothing: its row becomes NaN.
+ * No counterpart operator in the reference (an array index,
+ * models/mamba2_lm.py:190).
+ * ------------------------------------------------------------------------- */
+typedef struct {
+    const void* ids;               /* [n], id_dtype (M2_I32 / M2_I64)           */
+    const void* weight;            /* [vocab, dim] at ldw, dtype                */
+    void*       out;               /* out [n, dim] at ldo, dtype                */
+    int64_t n, vocab, dim, ldw, ldo;
+    float   scale;
+    int32_t id_dtype, dtype;
+} m2_embedding_args;
+int m2_embedding(const m2_embedding_args* a, void* stream);
+
+/* ---------------------------------------------------------------------------
+ * embedding_grad: out[v] = scale * sum over {n : ids[n] == v} of grad[n], every
+ * row of out written once (zeros where no id names it), or, with accumulate,
+ * added into out at the rows that the ids name, the others untouched.  The sums
+ * are float32 over the n in order (by sorted ids): equal inputs give
+ * equal bits.  ids equal to padding_idx and ids outside [0, vocab) take no part.
+ * vocab < 2^27, n < 2^31.
+ * ------------------------------------------------------------------------- */
+typedef struct {
+    const void* ids;               /* [n], id_dtype (M2_I32 / M2_I64)           */
+    const void* grad;              /* [n, dim] at ldg, grad_dtype               */
+    void*       out;               /* out [vocab, dim] at ldo, out_dtype        */
+    int64_t n, vocab, dim, ldg, ldo;
+    int64_t padding_idx;           /* -1: none                                  */
+    float   scale;
+    int32_t id_dtype, grad_dtype, out_dtype, accumulate;
+    void*   workspace;
+    size_t  workspace_bytes;       /* >= m2_embedding_grad_workspace_size()     */
+} m2_embedding_grad_args;
+size_t m2_embedding_grad_workspace_size(const m2_embedding_grad_args* a);
+int m2_embedding_grad(const m2_embedding_grad_args* a, void* stream);
+
+/* ---------------------------------------------------------------------------
+ * linear_cross_entropy: the loss of a linear head over a vocabulary,
+ *   z[n, v] = x[n] . weight[v],  lse[n] = log sum_v exp(z[n, v]),
+ *   loss[n] = lse[n] - z[n, targets[n]]   (0 where targets[n] == ignore_index),
+ * in pieces of the vocabulary: the logits exist in registers only.  x of rows
+ * that are left out is not read.  A target outside [0, vocab) that is not
+ * ignore_index makes its loss NaN.  total (or NULL) takes the sum of the losses, over
+ * max(1, the number of rows kept) with mean.  float32 operands are multiplied as three bf16
+ * parts each (six products, about 2^-24 of each).  vocab, n < 2^30.
+ * No counterpart in the reference, whose models answer with logits
+ * (models/mamba2_lm.py:213-216).
+ * ------------------------------------------------------------------------- */
+typedef struct {
+    const void* x;                 /* [n, dim] at ldx, dtype                    */
+    const void* weight;            /* [vocab, dim] at ldw, dtype                */
+    const void* targets;           /* [n], target_dtype (M2_I32 / M2_I64)       */
+    float*      loss;              /* out [n]                                   */
+    float*      lse;               /* out [n] (0 where left out)                */
+    float*      total;             /* out [1] or NULL                           */
+    int64_t n, vocab, dim, ldx, ldw;
+    int64_t ignore_index;
+    int32_t dtype, target_dtype, mean;
+    void*   workspace;
+    size_t  workspace_bytes;
+} m2_linear_cross_entropy_args;
+size_t m2_linear_cross_entropy_workspace_size(const m2_linear_cross_entropy_args* a);
+int m2_linear_cross_entropy(const m2_linear_cross_entropy_args* a, void* stream);
+
+/* ---------------------------------------------------------------------------
+ * linear_cross_entropy_grad: with g[n] = grad_loss[n * grad_loss_stride], over
+ * max(1, the number of rows kept) with mean,
+ *   G[n, v] = g[n] (exp(z[n, v] - lse[n]) - [v == targets[n]]),
+ *   grad_x = G weight,  grad_weight = G^T x
+ * from the loss and lse that m2_linear_cross_entropy gave for the same inputs; the
+ * logits are computed again, a piece of the vocabulary at a time.  Rows of
+ * grad_x that are left out become 0.  Either output may be NULL.
+ * ------------------------------------------------------------------------- */
+typedef struct {
+    const void*  x;
+    const void*  weight;
+    const void*  targets;
+    const float* loss;             /* [n], as the forward gave it               */
+    const float* lse;              /* [n]                                       */
+    const float* grad_loss;        /* [n] at grad_loss_stride (0: one value)    */
+    void*        grad_x;           /* out [n, dim] contiguous, dtype, or NULL   */
+    void*        grad_weight;      /* out [vocab, dim] contiguous, dtype, or NULL */
+    int64_t n, vocab, dim, ldx, ldw;
+    int64_t ignore_index, grad_loss_stride;
+    int32_t dtype, target_dtype, mean;
+    void*   workspace;
+    size_t  workspace_bytes;
+} m2_linear_cross_entropy_grad_args;
+size_t m2_linear_cross_entropy_grad_workspace_size(const m2_linear_cross_entropy_grad_args* a);
+int m2_linear_cross_entropy_grad(const m2_linear_cross_entropy_grad_args* a, void* stream);
+
+/* ---------------------------------------------------------------------------
+ * clip_grad_norm: norm = sqrt(sum of the squares of every value of every
+ * tensor), summed in float64 in a fixed order; with clip, each
+ * out = min(1, max_norm / (norm + eps)) * in (float32, rounded once), which
+ * may be the tensor itself.  A norm that is not a number makes every output
+ * not a number.  `tensors` is a host array, read during the call.
+ * ------------------------------------------------------------------------- */
+typedef struct {
+    const void* in;                /* [n] contiguous, dtype                     */
+    void*       out;               /* out [n], the same dtype (read with clip)  */
+    int64_t     n;
+    int64_t     dtype;
+} m2_tensor_ref;
+typedef struct {
+    const m2_tensor_ref* tensors;  /* [count], host memory                      */
+    int64_t count;
+    float*  norm;                  /* out [1]                                   */
+    float   max_norm, eps;
+    int32_t clip;
+    void*   workspace;
+    size_t  workspace_bytes;
+} m2_clip_grad_norm_args;
+size_t m2_clip_grad_norm_workspace_size(const m2_clip_grad_norm_args* a);
+int m2_clip_grad_norm(const m2_clip_grad_norm_args* a, void* stream);
 
 /* ---------------------------------------------------------------------------
  * Testing hook, no counterpart in the reference: forces one of the kernel

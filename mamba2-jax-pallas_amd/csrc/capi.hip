@@ -79,6 +79,25 @@ M2_ENTRY(m2_causal_conv1d_update, m2_causal_conv1d_update_args, launch_causal_co
 M2_ENTRY(m2_rms_norm_gated, m2_rms_norm_gated_args, launch_rms_norm_gated)
 M2_ENTRY(m2_skinny_gemm, m2_skinny_gemm_args, launch_skinny_gemm)
 M2_ENTRY(m2_skinny_gemm_norm, m2_skinny_gemm_norm_args, launch_skinny_gemm_norm)
+M2_ENTRY(m2_embedding, m2_embedding_args, launch_embedding)
+M2_ENTRY(m2_embedding_grad, m2_embedding_grad_args, launch_embedding_grad)
+M2_ENTRY(m2_linear_cross_entropy, m2_linear_cross_entropy_args, launch_linear_ce)
+M2_ENTRY(m2_linear_cross_entropy_grad, m2_linear_cross_entropy_grad_args, launch_linear_ce_grad)
+M2_ENTRY(m2_clip_grad_norm, m2_clip_grad_norm_args, launch_clip_grad_norm)
+
+extern "C" size_t m2_embedding_grad_workspace_size(const m2_embedding_grad_args* a) {
+    return a ? m2::embedding_grad_workspace(*a) : 0;
+}
+extern "C" size_t m2_linear_cross_entropy_workspace_size(const m2_linear_cross_entropy_args* a) {
+    return a ? m2::linear_ce_workspace(*a) : 0;
+}
+extern "C" size_t m2_linear_cross_entropy_grad_workspace_size(
+    const m2_linear_cross_entropy_grad_args* a) {
+    return a ? m2::linear_ce_grad_workspace(*a) : 0;
+}
+extern "C" size_t m2_clip_grad_norm_workspace_size(const m2_clip_grad_norm_args* a) {
+    return a ? m2::clip_grad_norm_workspace(*a) : 0;
+}
 
 // ---------------------------------------------------------------------------
 // combined forward

@@ -1,0 +1,785 @@
+// linear_cross_entropy and its gradient: softmax cross entropy of a linear head
+// over a large vocabulary in pieces, without the logits ever being stored.
+//
+//   z[n, v] = x[n] . w[v];  loss[n] = log sum_v exp(z[n, v]) - z[n, t[n]]
+//   G[n, v] = g[n] (exp(z[n, v] - lse[n]) - [v == t[n]]);  dx = G w;  dw = G^T x
+//
+// Forward: the product runs in tiles (ce_gemm.h); each tile leaves, per token, the
+// maximum m of its logits but the target's and the sum s of their exponentials
+// below it (8 bytes for 256 logits), and the target's logit z_t where it holds it.  A
+// second kernel joins the tiles: loss = log(1 + s exp(m - z_t)), which keeps its
+// accuracy down to losses far below the step of the logits.
+// Backward: a piece of the vocabulary at a time, the same product again gives G in its
+// epilogue (rounded to bf16 once, relative error 2^-9 of each, as the result's own
+// rounding; float32 operands keep three bf16 planes of it), then dw of the piece and
+// the piece's part of dx, which float32 partial sums collect over pieces.  At
+// the target G is g expm1(-loss), not a difference of near-equal numbers.
+//
+// Tokens that are left out (ignore_index) are dropped at the start: the kept rows of x
+// are packed (zero-padded to whole K steps), so they cost nothing afterwards
+// and what stands in a row left out (a NaN, say) touches nothing.  The number of
+// kept tokens stays on the device; tiles past it end at once.
+//
+// Bound by the matrix units for more than a few hundred tokens (2 n V D operations
+// forward, 6 n V D backward with the logits computed again), by reading the
+// weights for few.
+#include "ce_gemm.h"
+
+namespace {
+
+using namespace m2ce;
+
+constexpr float LOG2E = 1.4426950408889634f;
+
+struct Tokens {              // in the workspace
+    int* idx;                // [np] row of x of each kept token
+    int* inv;                // [n] kept index of each row, -1: left out
+    int* tgt;                // [np] target, -1: outside the vocabulary
+    float* zt;               // [np] the target's logit (forward)
+    float* lse;              // [np] (backward, as the two below)
+    float* gf;               // [np] upstream gradient
+    float* gm;               // [np] G at the target
+    int* count;              // [1]; the 16 zero bytes of the padding lie behind it
+};
+
+// ---------------------------------------------------------------------------
+// which rows are kept, in order
+// ---------------------------------------------------------------------------
+__global__ void __launch_bounds__(1024) k_ce_compact(const void* targets, int64_t n, int64_t ignore, int t64,
+                                                     Tokens tk) {
+    __shared__ int wsum[16];
+    const int t = threadIdx.x, lane = t & 63, w = wave_id();
+    int base = 0;
+    constexpr int E = 8;
+    for (int64_t i0 = 0; i0 < n; i0 += 1024 * E) {
+        bool keep[E];
+        int mine = 0;
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+            const int64_t i = i0 + (int64_t)t * E + e;
+            keep[e] = false;
+            if (i < n) {
+                const int64_t v = t64 ? reinterpret_cast<const int64_t*>(targets)[i]
+                                      : (int64_t) reinterpret_cast<const int32_t*>(targets)[i];
+                keep[e] = v != ignore;
+            }
+            mine += keep[e];
+        }
+        int s = mine;
+#pragma unroll
+        for (int o = 1; o < 64; o <<= 1) {
+            const int u = __shfl_up(s, o);
+            if (lane >= o) s += u;
+        }
+        if (lane == 63) wsum[w] = s;
+        __syncthreads();
+        int at = base + s - mine, all = 0;
+#pragma unroll
+        for (int q = 0; q < 16; ++q) {
+            at += q < w ? wsum[q] : 0;
+            all += wsum[q];
+        }
+        base += all;
+        __syncthreads();
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+            const int64_t i = i0 + (int64_t)t * E + e;
+            if (i >= n) break;
+            tk.inv[i] = keep[e] ? at : -1;
+            if (keep[e]) tk.idx[at++] = (int)i;
+        }
+    }
+    if (t < 32) tk.count[t] = t == 0 ? base : 0;
+}
+
+// 8 consecutive elements of a row, zero past its end
+template <typename T> M2_DEV void load8(const T* row, int64_t c, int64_t dim, bool vec, float (&v)[8]) {
+    if (vec && c + 8 <= dim) {
+        if constexpr (sizeof(T) == 2) {
+            const u32x4 r = *reinterpret_cast<const u32x4*>(row + c);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) { v[2 * i] = bf16_lo(r[i]); v[2 * i + 1] = bf16_hi(r[i]); }
+        } else {
+            const f32x4 a = *reinterpret_cast<const f32x4*>(row + c), b = *reinterpret_cast<const f32x4*>(row + c + 4);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) { v[i] = a[i]; v[4 + i] = b[i]; }
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = c + i < dim ? to_f32(row[c + i]) : 0.f;
+    }
+}
+// v = h + m + l, each bf16 (an infinity or NaN stays in h alone)
+M2_DEV void split3(float v, float& h, float& m, float& l) {
+    h = (float)(bf16)v;
+    const float r = v - h;
+    const bool fin = fabsf(h) < __builtin_inff();
+    m = fin ? (float)(bf16)r : 0.f;
+    l = fin ? r - m : 0.f;
+}
+template <bool PLANES> M2_DEV void store8(bf16* p, int64_t plane, const float (&v)[8]) {
+    if constexpr (!PLANES) {
+        const u32x4 r = {pk_bf16(v[0], v[1]), pk_bf16(v[2], v[3]), pk_bf16(v[4], v[5]), pk_bf16(v[6], v[7])};
+        *reinterpret_cast<u32x4*>(p) = r;
+    } else {
+        float h[8], m[8], l[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) split3(v[i], h[i], m[i], l[i]);
+        store8<false>(p, 0, h);
+        store8<false>(p + plane, 0, m);
+        store8<false>(p + 2 * plane, 0, l);
+    }
+}
+
+struct PackArgs {
+    const void* src;
+    bf16* dst;
+    int64_t rows, dim, ld, dp, plane;
+    int vec;
+    // of the tokens
+    const void* targets;
+    const float* lse;
+    const float* loss;
+    const float* g;
+    int64_t gstride, vocab;
+    int t64, mean;
+};
+
+// Rows of src as bf16 (planes) with rows of dp elements, zeros behind dim: the weights
+// where they cannot be read in place, or the kept rows of x (TOK), with zero rows up to
+// the next whole K step, and what the epilogues need of each token.
+template <typename T, bool TOK>
+__global__ void __launch_bounds__(256) k_ce_pack(PackArgs a, Tokens tk) {
+    const int64_t r = (int64_t)blockIdx.x * 4 + wave_id();
+    const int lane = threadIdx.x & 63;
+    int64_t from = r;
+    if constexpr (TOK) {
+        const int count = *tk.count;
+        if (r >= ((count + 63) & ~63)) return;
+        from = r < count ? tk.idx[r] : -1;
+        if (lane == 0) {
+            int tg = -1;
+            float gf = 0.f, gm = 0.f, lse = 0.f;
+            if (from >= 0) {
+                const int64_t v = a.t64 ? reinterpret_cast<const int64_t*>(a.targets)[from]
+                                        : (int64_t) reinterpret_cast<const int32_t*>(a.targets)[from];
+                tg = v >= 0 && v < a.vocab ? (int)v : -1;
+                if (a.g) {
+                    gf = a.g[from * a.gstride] * (a.mean ? 1.f / (float)count : 1.f);
+                    lse = a.lse[from];
+                    const float l = a.loss[from];
+                    gm = gf * expm1f(-l);
+                    if (tg < 0) gf = l;                 // NaN: the row's gradients are too
+                }
+            }
+            tk.tgt[r] = tg;
+            if (a.g) { tk.lse[r] = lse; tk.gf[r] = gf; tk.gm[r] = gm; }
+            else tk.zt[r] = __builtin_nanf("");
+        }
+    } else {
+        if (r >= a.rows) return;
+    }
+    const T* src = static_cast<const T*>(a.src) + (from < 0 ? 0 : from) * a.ld;
+    bf16* dst = a.dst + r * a.dp;
+    for (int64_t c = lane * 8; c < a.dp; c += 512) {
+        float v[8];
+        if (from >= 0) {
+            load8(src, c, a.dim, a.vec, v);
+        } else {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) v[i] = 0.f;
+        }
+        store8<sizeof(T) == 4>(dst + c, a.plane, v);
+    }
+}
+
+// ---------------------------------------------------------------------------
+// epilogues.  A lane holds, of each 16x16 block, one n (lane & 15) and 4 consecutive
+// m (4 (lane >> 4) ..).
+// ---------------------------------------------------------------------------
+// m: vocabulary, n: token -> per token (max, sum of exp(z - max)) of the tile without the target
+struct EpiLse {
+    const int* tgt;
+    float* zt;
+    float2* part;        // [tm][np]
+    int64_t np;
+    int vocab;
+
+    template <class S>
+    M2_DEV void run(f32x4 (&acc)[S::FM][S::FN], char* smem, int m0, int n0, int wm, int wn, int lane, int count,
+                    int, int tm) const {
+        float2* red = reinterpret_cast<float2*>(smem);        // [WM][BN]
+        const int v0 = m0 + wm * S::FM * 16 + 4 * (lane >> 4);
+        const bool edge = m0 + S::BM > vocab;
+#pragma unroll
+        for (int j = 0; j < S::FN; ++j) {
+            const int nl = (wn * S::FN + j) * 16 + (lane & 15), n = n0 + nl;
+            const int t = n < count ? tgt[n] : -1;
+            float mx = -__builtin_inff();
+#pragma unroll
+            for (int i = 0; i < S::FM; ++i) {
+                const int v = v0 + 16 * i;
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    if (v + r == t) {
+                        zt[n] = acc[i][j][r];
+                        acc[i][j][r] = -__builtin_inff();
+                    }
+                    if (edge && v + r >= vocab) acc[i][j][r] = -__builtin_inff();
+                    mx = fmaxf(mx, acc[i][j][r]);
+                }
+            }
+            mx = fmaxf(mx, __shfl_xor(mx, 16));
+            mx = fmaxf(mx, __shfl_xor(mx, 32));
+            const float b = mx == -__builtin_inff() ? 0.f : mx;
+            float s = 0.f;
+#pragma unroll
+            for (int i = 0; i < S::FM; ++i)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) s += __builtin_amdgcn_exp2f((acc[i][j][r] - b) * LOG2E);
+            s += __shfl_xor(s, 16);
+            s += __shfl_xor(s, 32);
+            if (lane < 16) red[wm * S::BN + nl] = make_float2(mx, s);
+        }
+        __syncthreads();
+        const int t = threadIdx.x;
+        if (t < S::BN && n0 + t < count) {
+            float2 o = red[t];
+#pragma unroll
+            for (int q = 1; q < S::WM; ++q) {
+                const float2 u = red[q * S::BN + t];
+                const float m = fmaxf(o.x, u.x), b = m == -__builtin_inff() ? 0.f : m;
+                o.y = o.y * __builtin_amdgcn_exp2f((o.x - b) * LOG2E) + u.y * __builtin_amdgcn_exp2f((u.x - b) * LOG2E);
+                o.x = m;
+            }
+            part[(int64_t)tm * np + n0 + t] = o;
+        }
+    }
+};
+
+// m: vocabulary, n: token -> G, bf16 (three planes for float32 operands), zero past the
+// vocabulary and past the kept tokens
+struct EpiG {
+    const int* tgt;
+    const float* lse;
+    const float* gf;
+    const float* gm;
+    bf16* G;
+    int64_t ldg, plane;
+    int v_first, vocab;      // of the piece; of all
+
+    template <class S>
+    M2_DEV void run(f32x4 (&acc)[S::FM][S::FN], char* smem, int m0, int n0, int wm, int wn, int lane, int count,
+                    int, int) const {
+        const int mv = m0 + wm * S::FM * 16 + 4 * (lane >> 4);
+        const int lim = (count + 63) & ~63;
+#pragma unroll
+        for (int j = 0; j < S::FN; ++j) {
+            const int n = n0 + (wn * S::FN + j) * 16 + (lane & 15);
+            if (n >= lim) continue;
+            const bool on = n < count;
+            const int t = on ? tgt[n] - v_first : -1;
+            const float ls = on ? lse[n] : 0.f, g = on ? gf[n] : 0.f, gt = on ? gm[n] : 0.f;
+#pragma unroll
+            for (int i = 0; i < S::FM; ++i) {
+                const int m = mv + 16 * i;
+                float o[4];
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    const float p = g * __builtin_amdgcn_exp2f((acc[i][j][r] - ls) * LOG2E);
+                    o[r] = !on || v_first + m + r >= vocab ? 0.f : m + r == t ? gt : p;
+                }
+                bf16* d = G + (int64_t)n * ldg + m;
+                typedef uint32_t u2 __attribute__((ext_vector_type(2)));
+                if constexpr (S::TERMS == 1) {
+                    *reinterpret_cast<u2*>(d) = u2{pk_bf16(o[0], o[1]), pk_bf16(o[2], o[3])};
+                } else {
+                    float h[4], md[4], l[4];
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) split3(o[r], h[r], md[r], l[r]);
+                    *reinterpret_cast<u2*>(d) = u2{pk_bf16(h[0], h[1]), pk_bf16(h[2], h[3])};
+                    *reinterpret_cast<u2*>(d + plane) = u2{pk_bf16(md[0], md[1]), pk_bf16(md[2], md[3])};
+                    *reinterpret_cast<u2*>(d + 2 * plane) = u2{pk_bf16(l[0], l[1]), pk_bf16(l[2], l[3])};
+                }
+            }
+        }
+    }
+};
+
+// m: dim, n: token -> float32 partial sums of dx, one array per split, added to over the
+// pieces of the vocabulary
+struct EpiDx {
+    float* part;             // [splits][np][dp]
+    int64_t np, dp;
+    int add;
+
+    template <class S>
+    M2_DEV void run(f32x4 (&acc)[S::FM][S::FN], char*, int m0, int n0, int wm, int wn, int lane, int count,
+                    int split, int) const {
+        const int mv = m0 + wm * S::FM * 16 + 4 * (lane >> 4);
+#pragma unroll
+        for (int j = 0; j < S::FN; ++j) {
+            const int n = n0 + (wn * S::FN + j) * 16 + (lane & 15);
+            if (n >= count) continue;
+            float* d = part + ((int64_t)split * np + n) * dp;
+#pragma unroll
+            for (int i = 0; i < S::FM; ++i) {
+                const int m = mv + 16 * i;
+                if (m >= dp) continue;
+                f32x4 v = acc[i][j];
+                if (add) v += *reinterpret_cast<const f32x4*>(d + m);
+                *reinterpret_cast<f32x4*>(d + m) = v;
+            }
+        }
+    }
+};
+
+// m: dim, n: vocabulary -> rows of dw
+template <typename T> struct EpiDw {
+    T* dw;
+    int64_t dim;
+    int rows, vec;           // rows of the piece
+
+    template <class S>
+    M2_DEV void run(f32x4 (&acc)[S::FM][S::FN], char*, int m0, int n0, int wm, int wn, int lane, int, int,
+                    int) const {
+        const int mv = m0 + wm * S::FM * 16 + 4 * (lane >> 4);
+#pragma unroll
+        for (int j = 0; j < S::FN; ++j) {
+            const int n = n0 + (wn * S::FN + j) * 16 + (lane & 15);
+            if (n >= rows) continue;
+            T* d = dw + (int64_t)n * dim;
+#pragma unroll
+            for (int i = 0; i < S::FM; ++i) {
+                const int m = mv + 16 * i;
+                if (vec && m + 4 <= dim) {
+                    if constexpr (sizeof(T) == 2) {
+                        typedef uint32_t u2 __attribute__((ext_vector_type(2)));
+                        *reinterpret_cast<u2*>(d + m) =
+                            u2{pk_bf16(acc[i][j][0], acc[i][j][1]), pk_bf16(acc[i][j][2], acc[i][j][3])};
+                    } else {
+                        *reinterpret_cast<f32x4*>(d + m) = acc[i][j];
+                    }
+                } else {
+#pragma unroll
+                    for (int r = 0; r < 4; ++r)
+                        if (m + r < dim) d[m + r] = from_f32<T>(acc[i][j][r]);
+                }
+            }
+        }
+    }
+};
+
+// ---------------------------------------------------------------------------
+// joins
+// ---------------------------------------------------------------------------
+struct JoinArgs {
+    const float2* part;
+    int64_t np, n;
+    float* loss;
+    float* lse;
+    int tiles;
+};
+
+// 16 tokens per workgroup, 16 lanes each: lane q joins tiles q, q + 16, ...
+__global__ void __launch_bounds__(256) k_ce_join(JoinArgs a, Tokens tk) {
+    __shared__ float2 red[16][17];
+    const int tok = threadIdx.x & 15, q = threadIdx.x >> 4;
+    const int64_t n = (int64_t)blockIdx.x * 16 + tok;
+    const int k = n < a.n ? tk.inv[n] : -1;
+    float mx = -__builtin_inff(), s = 0.f;
+    if (k >= 0) {
+#pragma unroll 4
+        for (int i = q; i < a.tiles; i += 16) {
+            const float2 u = a.part[(int64_t)i * a.np + k];
+            const float m = fmaxf(mx, u.x), b = m == -__builtin_inff() ? 0.f : m;
+            s = s * __builtin_amdgcn_exp2f((mx - b) * LOG2E) + u.y * __builtin_amdgcn_exp2f((u.x - b) * LOG2E);
+            mx = m;
+        }
+    }
+    red[q][tok] = make_float2(mx, s);
+    __syncthreads();
+    if (q == 0 && n < a.n) {
+        float loss = 0.f, lse = 0.f;
+        if (k >= 0) {
+            for (int i = 1; i < 16; ++i) {
+                const float2 u = red[i][tok];
+                const float m = fmaxf(mx, u.x), b = m == -__builtin_inff() ? 0.f : m;
+                s = s * __builtin_amdgcn_exp2f((mx - b) * LOG2E) + u.y * __builtin_amdgcn_exp2f((u.x - b) * LOG2E);
+                mx = m;
+            }
+            // exp(loss) = 1 + the others' sum over exp(z_t)
+            const float zt = tk.zt[k], d = mx - zt;
+            const float e = __builtin_amdgcn_exp2f(-fabsf(d) * LOG2E);
+            loss = d <= 0.f ? log1pf(s * e) : d + logf(s + e);
+            lse = zt + loss;
+        }
+        a.loss[n] = loss;
+        a.lse[n] = lse;
+    }
+}
+
+// the losses' sum or mean, in a fixed order, in float64
+__global__ void __launch_bounds__(1024) k_ce_total(const float* loss, int64_t n, float* total, int mean,
+                                                   const int* count) {
+    __shared__ double red[16];
+    double s = 0;
+    for (int64_t i = threadIdx.x; i < n; i += 1024) s += loss[i];
+#pragma unroll
+    for (int o = 32; o >= 1; o >>= 1) s += __shfl_xor(s, o);
+    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = s;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        double all = 0;
+        for (int j = 0; j < 16; ++j) all += red[j];
+        *total = (float)(all / (mean ? max(*count, 1) : 1));
+    }
+}
+
+struct DxArgs {
+    const float* part;
+    void* dx;
+    int64_t n, np, dp, dim;
+    int splits, vec;
+};
+
+// dx of every row, 0 where it was left out: a wavefront per row and 512 columns
+template <typename T> __global__ void __launch_bounds__(256) k_ce_dx(DxArgs a, Tokens tk) {
+    const int64_t n = (int64_t)blockIdx.x * 4 + wave_id();
+    if (n >= a.n) return;
+    const int k = tk.inv[n];
+    T* d = static_cast<T*>(a.dx) + n * a.dim;
+    const int64_t c = (int64_t)blockIdx.y * 512 + (threadIdx.x & 63) * 8;
+    if (c >= a.dim) return;
+    float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+    if (k >= 0) {
+        const float* p = a.part + (int64_t)k * a.dp + c;
+#pragma unroll 4
+        for (int s = 0; s < a.splits; ++s, p += a.np * a.dp) {
+            const f32x4 x = *reinterpret_cast<const f32x4*>(p), y = *reinterpret_cast<const f32x4*>(p + 4);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) { v[i] += x[i]; v[4 + i] += y[i]; }
+        }
+    }
+    if (a.vec && c + 8 <= a.dim) {
+        if constexpr (sizeof(T) == 2) {
+            store8<false>(reinterpret_cast<bf16*>(d) + c, 0, v);
+        } else {
+            *reinterpret_cast<f32x4*>(d + c) = f32x4{v[0], v[1], v[2], v[3]};
+            *reinterpret_cast<f32x4*>(d + c + 4) = f32x4{v[4], v[5], v[6], v[7]};
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            if (c + i < a.dim) d[c + i] = from_f32<T>(v[i]);
+    }
+}
+
+// ---------------------------------------------------------------------------
+// plans
+// ---------------------------------------------------------------------------
+size_t align256(size_t v) { return (v + 255) & ~size_t(255); }
+bool al16(const void* p) { return ((uintptr_t)p & 15) == 0; }
+
+// What the two entry points share: sizes, the packed operands and the tokens' arrays.
+struct Common {
+    int64_t n, vocab, dim, np, dp;
+    bool f32, pack_w;
+    size_t idx, inv, tgt, count, x, w, at;
+};
+
+Common common(int64_t n, int64_t vocab, int64_t dim, int64_t ldw, const void* w, int dtype) {
+    Common c{};
+    c.n = n; c.vocab = vocab; c.dim = dim;
+    c.np = (n + 63) / 64 * 64;
+    c.dp = (dim + 63) / 64 * 64;
+    c.f32 = dtype == M2_F32;
+    // the weights are read in place where direct loads can: bf16 rows of whole 16-byte
+    // pieces (and offsets within a tile that fit 32 bits); else a copy in the workspace
+    c.pack_w = c.f32 || dim % 8 || ldw % 8 || !al16(w) || ldw > (1 << 22);
+    auto take = [&](size_t b) { const size_t r = c.at; c.at += align256(b); return r; };
+    c.idx = take(4 * (size_t)c.np);
+    c.inv = take(4 * (size_t)c.np);
+    c.tgt = take(4 * (size_t)c.np);
+    c.count = take(256);
+    const size_t planes = c.f32 ? 3 : 1;
+    c.x = take(2 * planes * (size_t)c.np * c.dp);
+    c.w = c.pack_w ? take(2 * planes * (size_t)vocab * c.dp) : c.at;
+    return c;
+}
+
+template <class S, class EPI> void launch(const Gemm& g, const EPI& e, hipStream_t s) {
+    hipLaunchKernelGGL((k_ce_gemm<S, EPI>), dim3((unsigned)(g.tm * g.tn * g.splits)), dim3(S::NT), 0, s, g, e);
+}
+inline int tiles(int64_t n, int t) { return (int)((n + t - 1) / t); }
+
+// Tiles of the product vocabulary x tokens by the number of tokens
+template <bool F32> struct Shapes {
+    static constexpr int T = F32 ? 6 : 1;
+    typedef Shape<256, 256, 2, 4, 2, false, false, T> Z256;
+    typedef Shape<128, 64, 4, 1, 3, false, false, T> Z64;
+    typedef Shape<128, 16, 4, 1, 4, false, false, T> Z16;
+    typedef Shape<256, 256, 2, 4, 2, true, false, T> X256;
+    typedef Shape<256, 64, 4, 1, 3, true, false, T> X64;
+    typedef Shape<256, 16, 4, 1, 3, true, false, T> X16;
+    typedef Shape<256, 256, 2, 4, 2, true, true, T> W256;
+};
+// tokens of a tile
+int tok_tile(int64_t n) { return n <= 16 ? 16 : n <= 64 ? 64 : 256; }
+int voc_tile(int64_t n) { return n <= 64 ? 128 : 256; }
+
+template <bool F32, class EPI> void launch_z(Gemm& g, int64_t rows, int64_t n, const EPI& e, hipStream_t s) {
+    typedef Shapes<F32> P;
+    g.tm = tiles(rows, voc_tile(n));
+    g.tn = tiles(n, tok_tile(n));
+    switch (tok_tile(n)) {
+        case 16: launch<typename P::Z16>(g, e, s); break;
+        case 64: launch<typename P::Z64>(g, e, s); break;
+        default: launch<typename P::Z256>(g, e, s);
+    }
+}
+
+int check_sizes(const char* who, int64_t n, int64_t vocab, int64_t dim, int64_t ldx, int64_t ldw, int dtype,
+                int tdtype) {
+    M2_REQUIRE(n >= 0 && n < (1 << 30) && vocab > 0 && vocab < (1 << 30) && dim > 0 && dim <= (1 << 20),
+               M2_ERR_INVALID, "%s: bad sizes (n %lld, vocab %lld, dim %lld)", who, (long long)n,
+               (long long)vocab, (long long)dim);
+    M2_REQUIRE(ldx >= dim && ldw >= dim, M2_ERR_INVALID, "%s: row strides", who);
+    M2_REQUIRE(dtype == M2_F32 || dtype == M2_BF16, M2_ERR_UNSUPPORTED, "%s: dtype %d", who, dtype);
+    M2_REQUIRE(tdtype == M2_I32 || tdtype == M2_I64, M2_ERR_UNSUPPORTED, "%s: target dtype %d", who, tdtype);
+    M2_REQUIRE((int64_t)tiles(vocab, 128) * tiles(n, 16) < (1ll << 28) || n > 64, M2_ERR_UNSUPPORTED,
+               "%s: too large", who);
+    M2_REQUIRE((int64_t)tiles(vocab, 256) * tiles(n, 256) < (1ll << 30), M2_ERR_UNSUPPORTED, "%s: too large", who);
+    return M2_OK;
+}
+
+struct FwdPlan {
+    Common c;
+    size_t zt, part, total;
+};
+FwdPlan fwd_plan(const m2_linear_cross_entropy_args& a) {
+    FwdPlan p{};
+    p.c = common(a.n, a.vocab, a.dim, a.ldw, a.weight, a.dtype);
+    auto take = [&](size_t b) { const size_t r = p.c.at; p.c.at += align256(b); return r; };
+    p.zt = take(4 * (size_t)p.c.np);
+    p.part = take(8 * (size_t)tiles(a.vocab, voc_tile(a.n)) * p.c.np);
+    p.total = p.c.at;
+    return p;
+}
+
+// G's workspace: 512 MB of it at most, in whole tiles of the vocabulary.  More
+// pieces cost launches and passes over the partial dx; less memory costs nothing else.
+constexpr int64_t G_BYTES = 512ll << 20;
+struct BwdPlan {
+    Common c;
+    int64_t piece;
+    int pieces, splits;
+    size_t lse, gf, gm, G, dx, total;
+};
+BwdPlan bwd_plan(const m2_linear_cross_entropy_grad_args& a) {
+    BwdPlan p{};
+    p.c = common(a.n, a.vocab, a.dim, a.ldw, a.weight, a.dtype);
+    auto take = [&](size_t b) { const size_t r = p.c.at; p.c.at += align256(b); return r; };
+    p.lse = take(4 * (size_t)p.c.np);
+    p.gf = take(4 * (size_t)p.c.np);
+    p.gm = take(4 * (size_t)p.c.np);
+    const int planes = p.c.f32 ? 3 : 1;
+    const int64_t all = (a.vocab + 255) / 256 * 256;
+    int64_t most = G_BYTES / (2 * planes * (p.c.np ? p.c.np : 64)) / 256 * 256;
+    if (most < 256) most = 256;
+    p.pieces = (int)((all + most - 1) / most);
+    p.piece = ((all / 256 + p.pieces - 1) / p.pieces) * 256;
+    p.pieces = (int)((all + p.piece - 1) / p.piece);
+    p.G = take(2 * planes * (size_t)(p.c.np ? p.c.np : 64) * p.piece);
+    // dx: K is the piece, split so that the tiles fill the CUs; a split costs a
+    // float32 array of dx, written and read once per piece
+    const int ncu = m2::cu_count();
+    const int64_t t = (int64_t)tiles(a.dim, 256) * tiles(a.n ? a.n : 1, tok_tile(a.n));
+    const int steps = (int)(p.piece / 64);
+    double best = 1e300;
+    p.splits = 1;
+    for (int s = 1; s <= 64 && s * 4 <= steps; ++s) {
+        const double rounds = (double)((t * s + ncu - 1) / ncu);
+        const double cost = rounds * ((double)steps / s + 12.0) + 0.02 * s * t;
+        if (cost < best) { best = cost; p.splits = s; }
+    }
+    p.dx = a.grad_x ? take(4 * (size_t)p.splits * p.c.np * p.c.dp) : 0;
+    p.total = p.c.at;
+    return p;
+}
+
+Tokens tokens(char* ws, const Common& c) {
+    Tokens t{};
+    t.idx = reinterpret_cast<int*>(ws + c.idx);
+    t.inv = reinterpret_cast<int*>(ws + c.inv);
+    t.tgt = reinterpret_cast<int*>(ws + c.tgt);
+    t.count = reinterpret_cast<int*>(ws + c.count);
+    return t;
+}
+
+template <typename T>
+void pack(char* ws, const Common& c, const void* x, int64_t ldx, const void* w, int64_t ldw, PackArgs a,
+          const Tokens& tk, int64_t ignore, hipStream_t s) {
+    hipLaunchKernelGGL(k_ce_compact, dim3(1), dim3(1024), 0, s, a.targets, c.n, ignore, a.t64, tk);
+    const int ev = 16 / (int)sizeof(T);
+    a.dim = c.dim; a.dp = c.dp;
+    a.src = x; a.ld = ldx; a.dst = reinterpret_cast<bf16*>(ws + c.x); a.rows = c.np; a.plane = c.np * c.dp;
+    a.vec = ldx % ev == 0 && al16(x);
+    hipLaunchKernelGGL((k_ce_pack<T, true>), dim3((unsigned)(c.np / 4)), dim3(256), 0, s, a, tk);
+    if (c.pack_w) {
+        a.src = w; a.ld = ldw; a.dst = reinterpret_cast<bf16*>(ws + c.w); a.rows = c.vocab;
+        a.plane = c.vocab * c.dp;
+        a.vec = ldw % ev == 0 && al16(w);
+        hipLaunchKernelGGL((k_ce_pack<T, false>), dim3((unsigned)((c.vocab + 3) / 4)), dim3(256), 0, s, a, tk);
+    }
+}
+
+Operand operand_w(char* ws, const Common& c, const void* w, int64_t ldw) {
+    if (c.pack_w) return Operand{reinterpret_cast<bf16*>(ws + c.w), c.dp, c.vocab * c.dp, 0, 0};
+    return Operand{static_cast<const bf16*>(w), ldw, 0, 0, 0};
+}
+
+template <bool F32> int run_fwd(const m2_linear_cross_entropy_args& a, const FwdPlan& p, hipStream_t s) {
+    typedef typename std::conditional<F32, float, bf16>::type T;
+    char* ws = static_cast<char*>(a.workspace);
+    const Common& c = p.c;
+    Tokens tk = tokens(ws, c);
+    tk.zt = reinterpret_cast<float*>(ws + p.zt);
+    PackArgs pa{};
+    pa.targets = a.targets; pa.vocab = a.vocab; pa.t64 = a.target_dtype == M2_I64;
+    pack<T>(ws, c, a.x, a.ldx, a.weight, a.ldw, pa, tk, a.ignore_index, s);
+    Gemm g{};
+    g.zeros = tk.count + 16; g.count = tk.count; g.splits = 1; g.tok_n = 1;
+    g.nk = (int)(c.dp / 64);
+    g.a = operand_w(ws, c, a.weight, a.ldw);
+    g.a.lim = (int)c.vocab;
+    g.a.klim = (int)(c.pack_w ? c.dp : c.dim);
+    g.b = Operand{reinterpret_cast<bf16*>(ws + c.x), c.dp, c.np * c.dp, (int)c.np, (int)c.dp};
+    EpiLse e{tk.tgt, tk.zt, reinterpret_cast<float2*>(ws + p.part), c.np, (int)c.vocab};
+    launch_z<F32>(g, c.vocab, c.n, e, s);
+    JoinArgs j{e.part, c.np, c.n, a.loss, a.lse, g.tm};
+    hipLaunchKernelGGL(k_ce_join, dim3((unsigned)((c.n + 15) / 16)), dim3(256), 0, s, j, tk);
+    if (a.total)
+        hipLaunchKernelGGL(k_ce_total, dim3(1), dim3(1024), 0, s, a.loss, c.n, a.total, a.mean, tk.count);
+    return m2::check_launch("linear_cross_entropy");
+}
+
+template <bool F32> int run_bwd(const m2_linear_cross_entropy_grad_args& a, const BwdPlan& p, hipStream_t s) {
+    typedef typename std::conditional<F32, float, bf16>::type T;
+    typedef Shapes<F32> P;
+    char* ws = static_cast<char*>(a.workspace);
+    const Common& c = p.c;
+    Tokens tk = tokens(ws, c);
+    tk.lse = reinterpret_cast<float*>(ws + p.lse);
+    tk.gf = reinterpret_cast<float*>(ws + p.gf);
+    tk.gm = reinterpret_cast<float*>(ws + p.gm);
+    PackArgs pa{};
+    pa.targets = a.targets; pa.vocab = a.vocab; pa.t64 = a.target_dtype == M2_I64;
+    pa.lse = a.lse; pa.loss = a.loss; pa.g = a.grad_loss; pa.gstride = a.grad_loss_stride; pa.mean = a.mean;
+    pack<T>(ws, c, a.x, a.ldx, a.weight, a.ldw, pa, tk, a.ignore_index, s);
+    const Operand w = operand_w(ws, c, a.weight, a.ldw);
+    bf16* G = reinterpret_cast<bf16*>(ws + p.G);
+    const int64_t gplane = c.np * p.piece;
+    Gemm g0{};
+    g0.zeros = tk.count + 16; g0.count = tk.count; g0.splits = 1;
+    float* dxp = reinterpret_cast<float*>(ws + p.dx);
+    const int wlim = (int)(c.pack_w ? c.dp : c.dim);
+    for (int q = 0; q < p.pieces; ++q) {
+        const int64_t v0 = q * p.piece;
+        const int64_t rows = c.vocab - v0 < p.piece ? c.vocab - v0 : p.piece;
+        // G of the piece
+        Gemm g = g0;
+        g.nk = (int)(c.dp / 64); g.tok_n = 1;
+        g.a = w;
+        g.a.p += v0 * w.ld;
+        g.a.lim = (int)rows;
+        g.a.klim = wlim;
+        g.b = Operand{reinterpret_cast<bf16*>(ws + c.x), c.dp, c.np * c.dp, (int)c.np, (int)c.dp};
+        EpiG eg{tk.tgt, tk.lse, tk.gf, tk.gm, G, p.piece, gplane, (int)v0, (int)c.vocab};
+        launch_z<F32>(g, (rows + 63) / 64 * 64, c.n, eg, s);
+        if (a.grad_x) {
+            Gemm d = g0;
+            d.nk = (int)((rows + 63) / 64); d.tok_n = 1; d.splits = p.splits;
+            d.a = w;
+            d.a.p += v0 * w.ld;
+            d.a.lim = wlim;
+            d.a.klim = (int)rows;
+            d.b = Operand{G, p.piece, gplane, (int)c.np, (int)p.piece};
+            d.tm = tiles(c.dim, 256);
+            d.tn = tiles(c.n, tok_tile(c.n));
+            EpiDx e{dxp, c.np, c.dp, q > 0};
+            switch (tok_tile(c.n)) {
+                case 16: launch<typename P::X16>(d, e, s); break;
+                case 64: launch<typename P::X64>(d, e, s); break;
+                default: launch<typename P::X256>(d, e, s);
+            }
+        }
+        if (a.grad_weight) {
+            Gemm d = g0;
+            d.nk = 0;
+            d.a = Operand{reinterpret_cast<bf16*>(ws + c.x), c.dp, c.np * c.dp, (int)c.dp, (int)c.np};
+            // rows of G past the last token tile are not there: its last row stands for
+            // them, against zero rows of x
+            d.b = Operand{G, p.piece, gplane, (int)p.piece, tiles(c.n, tok_tile(c.n)) * tok_tile(c.n)};
+            d.tm = tiles(c.dim, 256);
+            d.tn = tiles(rows, 256);
+            EpiDw<T> e{static_cast<T*>(a.grad_weight) + v0 * c.dim, c.dim, (int)rows,
+                       c.dim % 4 == 0 && al16(a.grad_weight)};
+            launch<typename P::W256>(d, e, s);
+        }
+    }
+    if (a.grad_x) {
+        DxArgs d{dxp, a.grad_x, c.n, c.np, c.dp, c.dim, p.splits, c.dim % 8 == 0 && al16(a.grad_x)};
+        hipLaunchKernelGGL((k_ce_dx<T>), dim3((unsigned)((c.n + 3) / 4), (unsigned)((c.dim + 511) / 512)),
+                           dim3(256), 0, s, d, tk);
+    }
+    return m2::check_launch("linear_cross_entropy_grad");
+}
+
+}  // namespace
+
+namespace m2 {
+
+size_t linear_ce_workspace(const m2_linear_cross_entropy_args& a) {
+    if (check_sizes("linear_cross_entropy", a.n, a.vocab, a.dim, a.ldx, a.ldw, a.dtype, a.target_dtype)) return 0;
+    return fwd_plan(a).total;
+}
+
+int launch_linear_ce(const m2_linear_cross_entropy_args& a, hipStream_t s) {
+    const char* who = "linear_cross_entropy";
+    if (int rc = check_sizes(who, a.n, a.vocab, a.dim, a.ldx, a.ldw, a.dtype, a.target_dtype)) return rc;
+    M2_REQUIRE(a.weight && (a.n == 0 || (a.x && a.targets && a.loss && a.lse)), M2_ERR_INVALID,
+               "%s: x, weight, targets, loss and lse are required", who);
+    const FwdPlan p = fwd_plan(a);
+    M2_REQUIRE(a.workspace && a.workspace_bytes >= p.total, M2_ERR_WORKSPACE,
+               "%s: workspace of %zu bytes needed, %zu given", who, p.total, a.workspace_bytes);
+    if (a.n == 0) {
+        if (!a.total) return M2_OK;
+        Tokens tk = tokens(static_cast<char*>(a.workspace), p.c);
+        hipLaunchKernelGGL(k_ce_compact, dim3(1), dim3(1024), 0, s, a.targets, (int64_t)0, a.ignore_index, 0, tk);
+        hipLaunchKernelGGL(k_ce_total, dim3(1), dim3(1024), 0, s, a.loss, (int64_t)0, a.total, a.mean, tk.count);
+        return check_launch(who);
+    }
+    return a.dtype == M2_F32 ? run_fwd<true>(a, p, s) : run_fwd<false>(a, p, s);
+}
+
+size_t linear_ce_grad_workspace(const m2_linear_cross_entropy_grad_args& a) {
+    if (check_sizes("linear_cross_entropy_grad", a.n, a.vocab, a.dim, a.ldx, a.ldw, a.dtype, a.target_dtype))
+        return 0;
+    return bwd_plan(a).total;
+}
+
+int launch_linear_ce_grad(const m2_linear_cross_entropy_grad_args& a, hipStream_t s) {
+    const char* who = "linear_cross_entropy_grad";
+    if (int rc = check_sizes(who, a.n, a.vocab, a.dim, a.ldx, a.ldw, a.dtype, a.target_dtype)) return rc;
+    M2_REQUIRE(a.n > 0, M2_ERR_INVALID, "%s: no tokens", who);
+    M2_REQUIRE(a.weight && a.x && a.targets && a.loss && a.lse && a.grad_loss && (a.grad_x || a.grad_weight),
+               M2_ERR_INVALID, "%s: x, weight, targets, loss, lse, grad_loss and an output are required", who);
+    M2_REQUIRE(a.grad_loss_stride >= 0, M2_ERR_INVALID, "%s: grad_loss stride", who);
+    const BwdPlan p = bwd_plan(a);
+    M2_REQUIRE(a.workspace && a.workspace_bytes >= p.total, M2_ERR_WORKSPACE,
+               "%s: workspace of %zu bytes needed, %zu given", who, p.total, a.workspace_bytes);
+    return a.dtype == M2_F32 ? run_bwd<true>(a, p, s) : run_bwd<false>(a, p, s);
+}
+
+}  // namespace m2

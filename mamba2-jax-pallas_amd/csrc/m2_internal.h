@@ -50,6 +50,18 @@ int launch_rms_norm_gated(const m2_rms_norm_gated_args& a, hipStream_t stream);
 int launch_skinny_gemm(const m2_skinny_gemm_args& a, hipStream_t stream);
 int launch_skinny_gemm_norm(const m2_skinny_gemm_norm_args& a, hipStream_t stream);
 
+// the vocabulary's operators (embedding.hip, linear_ce.hip, grad_norm.hip) and
+// the workspaces they need (0: bad sizes)
+int launch_embedding(const m2_embedding_args& a, hipStream_t stream);
+int launch_embedding_grad(const m2_embedding_grad_args& a, hipStream_t stream);
+size_t embedding_grad_workspace(const m2_embedding_grad_args& a);
+int launch_linear_ce(const m2_linear_cross_entropy_args& a, hipStream_t stream);
+size_t linear_ce_workspace(const m2_linear_cross_entropy_args& a);
+int launch_linear_ce_grad(const m2_linear_cross_entropy_grad_args& a, hipStream_t stream);
+size_t linear_ce_grad_workspace(const m2_linear_cross_entropy_grad_args& a);
+int launch_clip_grad_norm(const m2_clip_grad_norm_args& a, hipStream_t stream);
+size_t clip_grad_norm_workspace(const m2_clip_grad_norm_args& a);
+
 // chunk_state_varlen for bf16, head dim 64, dstate % 64 == 0, chunk_size % 32
 // == 0 (<= 256): one workgroup per (sequence, head, 64-column dstate block)
 bool varlen_states_fast_supported(const m2_chunk_state_varlen_args& a);

@@ -20,6 +20,8 @@ LIB_PATH = os.path.join(os.path.dirname(os.path.abspath(__file__)), "libm2ssd.so
 
 M2_F32 = 0
 M2_BF16 = 1
+M2_I32 = 2
+M2_I64 = 3
 ABI_VERSION = 5
 # bytes of the static scratch m2_ssd_combined_noalloc runs in (M2_NOALLOC_SCRATCH_BYTES)
 NOALLOC_SCRATCH_BYTES = 128 << 20
@@ -143,6 +145,45 @@ class SkinnyGemmNormArgs(ctypes.Structure):
                 ("conv_begin", _i64), ("conv", CausalConv1dUpdateArgs)]
 
 
+class EmbeddingArgs(ctypes.Structure):
+    _fields_ = [("ids", _c_p), ("weight", _c_p), ("out", _c_p), ("n", _i64), ("vocab", _i64),
+                ("dim", _i64), ("ldw", _i64), ("ldo", _i64), ("scale", _f32), ("id_dtype", _i32),
+                ("dtype", _i32)]
+
+
+class EmbeddingGradArgs(ctypes.Structure):
+    _fields_ = [("ids", _c_p), ("grad", _c_p), ("out", _c_p), ("n", _i64), ("vocab", _i64),
+                ("dim", _i64), ("ldg", _i64), ("ldo", _i64), ("padding_idx", _i64),
+                ("scale", _f32), ("id_dtype", _i32), ("grad_dtype", _i32), ("out_dtype", _i32),
+                ("accumulate", _i32), ("workspace", _c_p), ("workspace_bytes", ctypes.c_size_t)]
+
+
+class LinearCrossEntropyArgs(ctypes.Structure):
+    _fields_ = [("x", _c_p), ("weight", _c_p), ("targets", _c_p), ("loss", _c_p), ("lse", _c_p),
+                ("total", _c_p), ("n", _i64), ("vocab", _i64), ("dim", _i64), ("ldx", _i64),
+                ("ldw", _i64), ("ignore_index", _i64), ("dtype", _i32), ("target_dtype", _i32),
+                ("mean", _i32), ("workspace", _c_p), ("workspace_bytes", ctypes.c_size_t)]
+
+
+class LinearCrossEntropyGradArgs(ctypes.Structure):
+    _fields_ = [("x", _c_p), ("weight", _c_p), ("targets", _c_p), ("loss", _c_p), ("lse", _c_p),
+                ("grad_loss", _c_p), ("grad_x", _c_p), ("grad_weight", _c_p), ("n", _i64),
+                ("vocab", _i64), ("dim", _i64), ("ldx", _i64), ("ldw", _i64),
+                ("ignore_index", _i64), ("grad_loss_stride", _i64), ("dtype", _i32),
+                ("target_dtype", _i32), ("mean", _i32), ("workspace", _c_p),
+                ("workspace_bytes", ctypes.c_size_t)]
+
+
+class TensorRef(ctypes.Structure):
+    _fields_ = [("in_", _c_p), ("out", _c_p), ("n", _i64), ("dtype", _i64)]
+
+
+class ClipGradNormArgs(ctypes.Structure):
+    _fields_ = [("tensors", _c_p), ("count", _i64), ("norm", _c_p), ("max_norm", _f32),
+                ("eps", _f32), ("clip", _i32), ("workspace", _c_p),
+                ("workspace_bytes", ctypes.c_size_t)]
+
+
 # entry point name -> argument struct (every function declared in m2ssd.h)
 ENTRY_POINTS = {
     "m2_chunk_cumsum": ChunkCumsumArgs,
@@ -159,9 +200,23 @@ ENTRY_POINTS = {
     "m2_rms_norm_gated": RmsNormGatedArgs,
     "m2_skinny_gemm": SkinnyGemmArgs,
     "m2_skinny_gemm_norm": SkinnyGemmNormArgs,
+    "m2_embedding": EmbeddingArgs,
+    "m2_embedding_grad": EmbeddingGradArgs,
+    "m2_linear_cross_entropy": LinearCrossEntropyArgs,
+    "m2_linear_cross_entropy_grad": LinearCrossEntropyGradArgs,
+    "m2_clip_grad_norm": ClipGradNormArgs,
+}
+# workspace size functions of the entry points that take a workspace besides the
+# combined forward: name -> argument struct
+WORKSPACE_SIZES = {
+    "m2_embedding_grad_workspace_size": EmbeddingGradArgs,
+    "m2_linear_cross_entropy_workspace_size": LinearCrossEntropyArgs,
+    "m2_linear_cross_entropy_grad_workspace_size": LinearCrossEntropyGradArgs,
+    "m2_clip_grad_norm_workspace_size": ClipGradNormArgs,
 }
 OTHER_SYMBOLS = ("m2_ssd_combined_workspace_size", "m2_ssd_combined_plan", "m2_last_error", "m2_abi_version",
-                 "m2_set_dispatch_override", "m2_ssd_combined_noalloc_prepare")
+                 "m2_set_dispatch_override", "m2_ssd_combined_noalloc_prepare",
+                 *WORKSPACE_SIZES)
 
 # testing hook m2_set_dispatch_override: knob name -> (M2_KNOB_*, {choice: value})
 KNOBS = {
@@ -207,6 +262,10 @@ def load_library(path=LIB_PATH):
             fn = getattr(lib, name)
             fn.argtypes = [ctypes.POINTER(st), ctypes.c_void_p]
             fn.restype = ctypes.c_int
+        for name, st in WORKSPACE_SIZES.items():
+            fn = getattr(lib, name)
+            fn.argtypes = [ctypes.POINTER(st)]
+            fn.restype = ctypes.c_size_t
         lib.m2_ssd_combined_workspace_size.argtypes = [ctypes.POINTER(SsdCombinedArgs)]
         lib.m2_ssd_combined_workspace_size.restype = ctypes.c_size_t
         lib.m2_ssd_combined_plan.argtypes = [ctypes.POINTER(SsdCombinedArgs)]
@@ -236,6 +295,19 @@ def call(name, args, stream):
     rc = fn(ctypes.byref(args), stream)
     if rc != 0:
         raise M2Error(name, rc, load_library().m2_last_error().decode(errors="replace"))
+
+
+def call_with_workspace(name, args, device):
+    """Call entry point `name` on `device`'s current stream with a workspace of the
+    size that the library asks for (from torch's caching allocator, as a tensor of
+    that stream: it may be reused by later work there)."""
+    size = getattr(load_library(), name + "_workspace_size")(ctypes.byref(args))
+    if size == 0:
+        raise M2Error(name, -1, load_library().m2_last_error().decode(errors="replace"))
+    with torch.cuda.device(device):
+        ws = torch.empty(size, dtype=torch.uint8, device=device)
+        args.workspace, args.workspace_bytes = ws.data_ptr(), size
+        call(name, args, stream_of(device))
 
 
 # Bumped on every override change: results cached against the library's
@@ -278,6 +350,16 @@ def dtype_code(t, what):
         return _DTYPE_CODE[t.dtype]
     except KeyError:
         raise TypeError(f"{what}: dtype {t.dtype} is not supported (float32 or bfloat16)") from None
+
+
+_INDEX_CODE = {torch.int32: M2_I32, torch.int64: M2_I64}
+
+
+def index_code(t, what):
+    try:
+        return _INDEX_CODE[t.dtype]
+    except KeyError:
+        raise TypeError(f"{what}: dtype {t.dtype} is not supported (int32 or int64)") from None
 
 
 def torch_dtype(d):

@@ -1,0 +1,136 @@
+"""Embedding lookup on MI355X and its gradient by sorted tokens, as HIP kernels
+in libm2ssd.so (m2_embedding, m2_embedding_grad).
+
+No counterpart operator in the reference, whose lookup is an array index
+(models/mamba2_lm.py:190): the gradient of that index under autograd is a scatter-add of
+float atomics, whose order changes its result; this one sorts the tokens and
+gives equal bits for equal inputs.
+"""
+
+from __future__ import annotations
+
+import torch
+from torch.autograd.function import once_differentiable
+
+from .. import _lib as L
+
+
+def _flat_ids(ids):
+    L.index_code(ids, "ids")
+    return ids.reshape(-1).contiguous()
+
+
+def _rows(t, dim):
+    """t (..., dim) as rows (n, dim) with unit last stride (a view where it can be)."""
+    t = t.reshape(-1, dim)
+    if (t.shape[0] > 1 and t.stride(0) < dim) or (dim > 1 and t.stride(1) != 1):
+        t = t.contiguous()
+    return t
+
+
+def _stride(t, dim):
+    return t.stride(0) if t.shape[0] > 1 else dim
+
+
+def _lookup(ids, weight, scale):
+    dev = L.device_of(ids, weight)
+    L.require(weight.dim() == 2, f"weight.shape={tuple(weight.shape)}: expected (vocab, dim)")
+    code = L.dtype_code(weight, "weight")
+    flat = _flat_ids(ids)
+    vocab, dim = (int(s) for s in weight.shape)
+    L.require(vocab > 0 and dim > 0, f"weight.shape={tuple(weight.shape)}")
+    w = _rows(weight.detach(), dim)
+    out = torch.empty((*ids.shape, dim), dtype=weight.dtype, device=dev)
+    if flat.numel() == 0:
+        return out
+    args = L.EmbeddingArgs(ids=L.ptr(flat), weight=L.ptr(w), out=L.ptr(out), n=flat.numel(),
+                           vocab=vocab, dim=dim, ldw=_stride(w, dim), ldo=dim, scale=float(scale),
+                           id_dtype=L.index_code(flat, "ids"), dtype=code)
+    with torch.cuda.device(dev):
+        L.call("m2_embedding", args, L.stream_of(dev))
+    return out
+
+
+class _Embedding(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, ids, weight, scale, padding_idx):
+        ctx.save_for_backward(ids)
+        ctx.args = int(weight.shape[0]), float(scale), padding_idx, weight.dtype
+        return _lookup(ids, weight, scale)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, grad):
+        (ids,) = ctx.saved_tensors
+        vocab, scale, padding_idx, dtype = ctx.args
+        return None, embedding_grad(ids, grad, vocab, scale=scale, padding_idx=padding_idx,
+                                    dtype=dtype), None, None
+
+
+def _padding(padding_idx, vocab):
+    if padding_idx is None:
+        return None
+    p = int(padding_idx)
+    L.require(-vocab <= p < vocab, f"padding_idx={p} outside the vocabulary of {vocab}")
+    return p % vocab
+
+
+def embedding(ids, weight, scale=1.0, padding_idx=None):
+    """-> scale * weight[ids], shape (*ids.shape, dim), weight's dtype (the product
+    in float32, rounded once); differentiable in weight.
+
+    ids: int32 or int64, any shape.  weight (vocab, dim) float32 or bfloat16, rows
+    with a contiguous last dimension read in place.  An id outside the
+    vocabulary cannot be reported without waiting for the GPU: its row is NaN,
+    and it takes no part in the gradient.  padding_idx: an id whose gradient is left
+    out (its row is looked up like any other)."""
+    L.device_of(ids, weight)
+    L.require(weight.dim() == 2, f"weight.shape={tuple(weight.shape)}: expected (vocab, dim)")
+    padding_idx = _padding(padding_idx, int(weight.shape[0]))
+    if torch.is_grad_enabled() and weight.requires_grad:
+        return _Embedding.apply(ids, weight, scale, padding_idx)
+    return _lookup(ids, weight, scale)
+
+
+def embedding_grad(ids, grad, num_embeddings, scale=1.0, padding_idx=None, *, dtype=None, out=None):
+    """The gradient of ``embedding`` in its weight: (num_embeddings, dim), row v the
+    sum of scale * grad over the positions with ids == v, in their order
+    (float32 sums, rounded once; equal inputs give equal bits), zeros elsewhere.
+
+    ids: int32 or int64; grad (*ids.shape, dim) float32 or bfloat16.  dtype
+    (keyword only): float32 or bfloat16, default grad's.  out (keyword only): a
+    (num_embeddings, dim) float32 or bfloat16 tensor that the rows named by
+    ids are added into in place, the others left untouched, and that is returned: the
+    gradient of an embedding tied to the head, after the head's."""
+    dev = L.device_of(ids, grad, out)
+    vocab = int(num_embeddings)
+    L.require(0 < vocab < 2 ** 27, f"num_embeddings={vocab}")
+    L.require(grad.dim() == ids.dim() + 1 and tuple(grad.shape[:-1]) == tuple(ids.shape),
+              f"grad.shape={tuple(grad.shape)}: expected {tuple(ids.shape)} + (dim,)")
+    dim = int(grad.shape[-1])
+    L.require(dim > 0, "grad has no columns")
+    L.dtype_code(grad, "grad")
+    padding_idx = _padding(padding_idx, vocab)
+    flat = _flat_ids(ids)
+    g = _rows(grad.detach(), dim)
+    accumulate = out is not None
+    if accumulate:
+        L.require(dtype is None or out.dtype == dtype, "dtype and out disagree")
+        L.require(tuple(out.shape) == (vocab, dim) and (dim == 1 or out.stride(1) == 1)
+                  and (vocab == 1 or out.stride(0) >= dim),
+                  f"out must be ({vocab}, {dim}) with a contiguous last dimension")
+    else:
+        out = torch.empty((vocab, dim), dtype=L.torch_dtype(dtype) or grad.dtype, device=dev)
+    args = L.EmbeddingGradArgs(
+        ids=L.ptr(flat), grad=L.ptr(g), out=L.ptr(out), n=flat.numel(), vocab=vocab, dim=dim,
+        ldg=_stride(g, dim), ldo=_stride(out, dim),
+        padding_idx=-1 if padding_idx is None else padding_idx, scale=float(scale),
+        id_dtype=L.index_code(flat, "ids"), grad_dtype=L.dtype_code(g, "grad"),
+        out_dtype=L.dtype_code(out, "out"), accumulate=int(accumulate))
+    L.call_with_workspace("m2_embedding_grad", args, dev)
+    if accumulate:
+        torch.autograd.graph.increment_version(out)
+    return out
+
+
+__all__ = ["embedding", "embedding_grad"]

@@ -9,20 +9,21 @@
 // The gradient sorts (id, n) by id with a stable radix sort (equal ids keep the
 // order of n), walks the sorted list in pieces of up to 32 entries, one
 // workgroup each, with the sum of the current id's rows in registers, and
-// writes each row of the result once.  An id whose entries cross pieces
-// (frequent tokens) leaves one partial row per piece, which the workgroup of its
-// first piece's join adds in order: no float atomics, so equal inputs give
-// equal bits, and a token that is half of the batch is spread over as many
-// workgroups as any others.  The rows that no id names (most of a large
-// vocabulary) are zeroed by further workgroups of the same launch, from a bitmap
-// that the sort leaves: every byte of the result is written once.  Bound by
-// HBM: grad read once, the result written once.
+// writes each row that an id names once.  An id whose entries cross pieces
+// (frequent tokens) leaves one partial row per piece, which a second kernel
+// adds in order: no float atomics, so equal inputs give equal bits, and a token
+// that is half of the batch is spread over as many workgroups as any others.
+// The sort keeps one workgroup (of up to 16384 entries) or a few busy and is bound by
+// latencies; the rest of the chip meanwhile writes the zeros, which are most of a
+// large vocabulary's gradient.  The rows that ids name are written twice that way, at
+// most n rows; zeroing the others alone would have to wait for the sort.  Bound
+// by HBM: grad read once, the result written once and those rows again.
 #include "m2_internal.h"
 
 namespace {
 
 constexpr int SORT_THREADS = 256, SORT_ITEMS = 8, SORT_TILE = SORT_THREADS * SORT_ITEMS;
-constexpr int SMALL_THREADS = 1024, SMALL_ITEMS = 4, SMALL_N = SMALL_THREADS * SMALL_ITEMS;
+constexpr int SMALL_THREADS = 1024, SMALL_POS = 14, SMALL_N = 1 << SMALL_POS;
 constexpr int MAX_BINS = 512;
 
 M2_DEV int64_t load_id(const void* ids, int64_t i, int is64) {
@@ -116,9 +117,8 @@ struct SortArgs {
     int32_t* keys_out;
     int32_t* pos_out;
     int32_t* hist;               // [blocks][bins]
-    uint32_t* used;              // bitmap of the ids that take part
     int64_t vocab, padding;
-    int n, id64, shift, bits, nb, words;
+    int n, id64, shift, bits, nb;
 };
 
 M2_DEV int32_t key_of(const SortArgs& a, int i) {
@@ -126,12 +126,45 @@ M2_DEV int32_t key_of(const SortArgs& a, int i) {
     return id >= 0 && id < a.vocab && id != a.padding ? (int32_t)id : (int32_t)a.vocab;
 }
 
-__global__ void __launch_bounds__(SORT_THREADS) k_sort_hist(SortArgs a) {
+// Zeros of the result, written by the workgroups that a sort's launch has to spare: rows
+// [r0, r1), a contiguous range of bytes where the rows lie without gaps.
+struct FillArgs {
+    char* out;
+    int64_t r0, r1, ldo, row;    // bytes
+    int flat;                    // ldo == row, 16-byte aligned
+};
+constexpr int64_t FILL_BYTES = 64 << 10;     // of a workgroup, about
+
+M2_DEV void fill(const FillArgs& f, int block, int blocks) {
+    const u32x4 z = {0, 0, 0, 0};
+    if (f.flat) {
+        const int64_t b0 = f.r0 * f.row, n = (f.r1 - f.r0) * f.row / 16;
+        u32x4* p = reinterpret_cast<u32x4*>(f.out + b0);
+        const int64_t i0 = n * block / blocks, i1 = n * (block + 1) / blocks;
+#pragma unroll 4
+        for (int64_t i = i0 + threadIdx.x; i < i1; i += blockDim.x) p[i] = z;
+        // what 16-byte pieces leave of the last row
+        if (block == 0 && threadIdx.x < (int)(((f.r1 - f.r0) * f.row - n * 16) >> 1))
+            reinterpret_cast<uint16_t*>(p + n)[threadIdx.x] = 0;
+        return;
+    }
+    const int nw = blockDim.x >> 6, lane = threadIdx.x & 63;
+    for (int64_t r = f.r0 + (int64_t)block * nw + wave_id(); r < f.r1; r += (int64_t)blocks * nw) {
+        char* p = f.out + r * f.ldo;
+        // single elements (of 2 bytes) up to a 16-byte boundary and behind the last one
+        int64_t head = (16 - ((uintptr_t)p & 15)) & 15;
+        head = head < f.row ? head : f.row;
+        const int64_t vecs = (f.row - head) >> 4, tail = head + vecs * 16;
+        for (int64_t i = lane; i < vecs; i += 64) *reinterpret_cast<u32x4*>(p + head + i * 16) = z;
+        if (2 * lane < head) reinterpret_cast<uint16_t*>(p)[lane] = 0;
+        if (2 * lane < f.row - tail) reinterpret_cast<uint16_t*>(p + tail)[lane] = 0;
+    }
+}
+
+__global__ void __launch_bounds__(SORT_THREADS) k_sort_hist(SortArgs a, FillArgs f) {
     __shared__ int h[MAX_BINS];
     const int bins = 1 << a.bits, t = threadIdx.x, b = blockIdx.x;
-    if (!a.keys_in)
-        for (int64_t w = (int64_t)b * SORT_THREADS + t; w < a.words; w += (int64_t)a.nb * SORT_THREADS)
-            a.used[w] = 0;
+    if (b >= a.nb) return fill(f, b - a.nb, gridDim.x - a.nb);
     for (int d = t; d < bins; d += SORT_THREADS) h[d] = 0;
     __syncthreads();
 #pragma unroll
@@ -181,11 +214,12 @@ template <int NT> M2_DEV int block_excl(int v, int* tmp) {
     return base + s - v;
 }
 
-__global__ void __launch_bounds__(SORT_THREADS) k_sort_scatter(SortArgs a, int last) {
+__global__ void __launch_bounds__(SORT_THREADS) k_sort_scatter(SortArgs a, FillArgs f) {
     constexpr int NW = SORT_THREADS / 64;
     __shared__ int cnt[NW][MAX_BINS];
     __shared__ int tmp[NW];
     const int bins = 1 << a.bits, t = threadIdx.x, b = blockIdx.x, w = wave_id(), lane = t & 63;
+    if (b >= a.nb) return fill(f, b - a.nb, gridDim.x - a.nb);
     int32_t key[SORT_ITEMS], pos[SORT_ITEMS];
     int rank[SORT_ITEMS];
     const int base = b * SORT_TILE + w * 64 * SORT_ITEMS + lane;
@@ -238,35 +272,35 @@ __global__ void __launch_bounds__(SORT_THREADS) k_sort_scatter(SortArgs a, int l
         const int p = cnt[w][(key[j] >> a.shift) & (bins - 1)] + rank[j];
         a.keys_out[p] = key[j];
         a.pos_out[p] = pos[j];
-        if (last && key[j] < a.vocab) atomicOr(&a.used[key[j] >> 5], 1u << (key[j] & 31));
     }
 }
 
-// Up to SMALL_N entries: every pass in one workgroup, the list in LDS between
-// the passes (a.shift, a.bits: of every pass; passes in a.nb).
-__global__ void __launch_bounds__(SMALL_THREADS) k_sort_small(SortArgs a) {
+// Up to SMALL_N entries of a vocabulary below 2^18: every pass in one workgroup, the list
+// in LDS between the passes, an entry in one word (key, position).  a.bits: of
+// every pass; a.nb: the passes.  16384 entries take two passes over 16 words a thread.
+template <int IT>
+__global__ void __launch_bounds__(SMALL_THREADS) k_sort_small(SortArgs a, FillArgs f) {
     constexpr int NW = SMALL_THREADS / 64;
     __shared__ int cnt[NW][MAX_BINS];
-    __shared__ int32_t lk[SMALL_N], lp[SMALL_N];
+    __shared__ uint32_t list[SMALL_THREADS * IT];
     __shared__ int tmp[NW];
-    const int bins = 1 << a.bits, t = threadIdx.x, w = wave_id(), lane = t & 63;
-    for (int i = t; i < a.words; i += SMALL_THREADS) a.used[i] = 0;
-    const int base = w * 64 * SMALL_ITEMS + lane;
-    int32_t key[SMALL_ITEMS], pos[SMALL_ITEMS];
-    int rank[SMALL_ITEMS];
+    if (blockIdx.x > 0) return fill(f, blockIdx.x - 1, gridDim.x - 1);
+    const int bins = 1 << a.bits, t = threadIdx.x, w = wave_id();
+    const int base = w * 64 * IT + (t & 63);
+    uint32_t e[IT];
+    int rank[IT];
 #pragma unroll
-    for (int j = 0; j < SMALL_ITEMS; ++j) {
+    for (int j = 0; j < IT; ++j) {
         const int i = base + 64 * j;
-        key[j] = i < a.n ? key_of(a, i) : 0;
-        pos[j] = i;
+        e[j] = i < a.n ? (uint32_t)key_of(a, i) << SMALL_POS | (uint32_t)i : 0;
     }
     for (int pass = 0; pass < a.nb; ++pass) {
-        const int shift = pass * a.bits;
-        for (int d = t; d < NW * MAX_BINS; d += SMALL_THREADS) (&cnt[0][0])[d] = 0;
+        const int shift = SMALL_POS + pass * a.bits;
+        for (int d = t; d < NW * bins; d += SMALL_THREADS) cnt[d >> a.bits][d & (bins - 1)] = 0;
         __syncthreads();
 #pragma unroll
-        for (int j = 0; j < SMALL_ITEMS; ++j)
-            rank[j] = wave_rank((key[j] >> shift) & (bins - 1), base + 64 * j < a.n, a.bits, cnt[w]);
+        for (int j = 0; j < IT; ++j)
+            rank[j] = wave_rank((e[j] >> shift) & (bins - 1), base + 64 * j < a.n, a.bits, cnt[w]);
         __syncthreads();
         int tot = 0;
         if (t < bins)
@@ -282,27 +316,18 @@ __global__ void __launch_bounds__(SMALL_THREADS) k_sort_small(SortArgs a) {
             }
         __syncthreads();
 #pragma unroll
-        for (int j = 0; j < SMALL_ITEMS; ++j) {
-            if (base + 64 * j >= a.n) continue;
-            const int p = cnt[w][(key[j] >> shift) & (bins - 1)] + rank[j];
-            lk[p] = key[j];
-            lp[p] = pos[j];
-        }
+        for (int j = 0; j < IT; ++j)
+            if (base + 64 * j < a.n) list[cnt[w][(e[j] >> shift) & (bins - 1)] + rank[j]] = e[j];
         __syncthreads();
 #pragma unroll
-        for (int j = 0; j < SMALL_ITEMS; ++j) {
-            const int i = base + 64 * j;
-            if (i < a.n) { key[j] = lk[i]; pos[j] = lp[i]; }
-        }
+        for (int j = 0; j < IT; ++j) e[j] = list[base + 64 * j];
     }
 #pragma unroll
-    for (int j = 0; j < SMALL_ITEMS; ++j) {
+    for (int j = 0; j < IT; ++j) {
         const int i = base + 64 * j;
         if (i >= a.n) continue;
-        a.keys_out[i] = key[j];
-        a.pos_out[i] = pos[j];
-        // after the zeroing of `used` above: the passes' barriers lie between
-        if (key[j] < a.vocab) atomicOr(&a.used[key[j] >> 5], 1u << (key[j] & 31));
+        a.keys_out[i] = (int32_t)(e[j] >> SMALL_POS);
+        a.pos_out[i] = (int32_t)(e[j] & (SMALL_N - 1));
     }
 }
 
@@ -312,15 +337,13 @@ __global__ void __launch_bounds__(SMALL_THREADS) k_sort_small(SortArgs a) {
 struct ReduceArgs {
     const int32_t* keys;
     const int32_t* pos;
-    const uint32_t* used;
     const void* grad;
     void* out;
     float* part;             // [pieces][2][ldp]: of a row begun before the piece / left unfinished
     int64_t ldg, ldo, ldp, vocab;
     int n, piece, pieces;    // entries per piece
     int vecs, slabs;         // V-element pieces of a row, split over `slabs` workgroups
-    int cols;                // elements of a row
-    int nred, accumulate;    // workgroups that sum; the others zero rows
+    int nred, accumulate;
     float scale;
 };
 
@@ -340,41 +363,24 @@ M2_DEV void put_row(const ReduceArgs& a, int32_t key, int c, Vec<float, V> s) {
     o.store(p);
 }
 
-// Rows without an id become zero: whole 16-byte pieces, single elements at the ends
-// of a row that does not begin or end on one.
-template <typename TO> M2_DEV void zero_row(TO* p, int n, int t, int nt) {
-    constexpr int E = 16 / sizeof(TO);
-    int head = (int)((16 - ((uintptr_t)p & 15)) & 15) / (int)sizeof(TO);
-    head = head < n ? head : n;
-    const int vecs = (n - head) / E;
-    const u32x4 z = {0, 0, 0, 0};
-    for (int i = t; i < vecs; i += nt) *reinterpret_cast<u32x4*>(p + head + i * E) = z;
-    const int tail = head + vecs * E;
-    if (t < head) p[t] = (TO)0.f;
-    if (t < n - tail) p[tail + t] = (TO)0.f;
-}
+constexpr int MAX_PIECE = 32;
 
 template <typename T, typename TO, int V>
 __global__ void __launch_bounds__(512) k_embed_sum(ReduceArgs a) {
-    constexpr int UN = V == 1 ? 8 : 4;
-    const int t = threadIdx.x;
-    if ((int)blockIdx.x >= a.nred) {
-        // the rows of 32-bit words of the bitmap: a wavefront per row
-        const int nw = blockDim.x >> 6;
-        const int64_t stride = (int64_t)(gridDim.x - a.nred) * nw;
-        for (int64_t r = (int64_t)(blockIdx.x - a.nred) * nw + wave_id(); r < a.vocab; r += stride)
-            if (!((a.used[r >> 5] >> (r & 31)) & 1))
-                zero_row(static_cast<TO*>(a.out) + r * a.ldo, a.cols, t & 63, 64);
-        return;
-    }
+    constexpr int UN = 8;                 // rows in flight
+    const int t = threadIdx.x, lane = t & 63;
     const int p = blockIdx.x / a.slabs, slab = blockIdx.x % a.slabs;
     const int per = (a.vecs + a.slabs - 1) / a.slabs;
     const int c = slab * per + t;
     const bool on = t < per && c < a.vecs;
-    const int e0 = p * a.piece, e1 = min(a.n, e0 + a.piece);
-    const T* g = static_cast<const T*>(a.grad) + (int64_t)c * V;
-    int32_t key = a.keys[e0];
-    bool head = p > 0 && a.keys[e0 - 1] == key;      // the row began in an earlier piece
+    const int e0 = p * a.piece, cnt = min(a.n - e0, a.piece);
+    // the piece's entries, one a lane (every wavefront has them all)
+    const int q = e0 + min(lane, cnt - 1);
+    const int32_t keys = a.keys[q], pos = a.pos[q];
+    const int32_t before = p > 0 ? a.keys[e0 - 1] : -1, after = e0 + cnt < a.n ? a.keys[e0 + cnt] : -1;
+    const T* g = static_cast<const T*>(a.grad) + (int64_t)(on ? c : 0) * V;
+    int32_t key = __builtin_amdgcn_readlane(keys, 0);
+    bool head = before == key;            // the row began in an earlier piece
     Vec<float, V> s;
 #pragma unroll
     for (int i = 0; i < V; ++i) s.v[i] = 0.f;
@@ -383,31 +389,28 @@ __global__ void __launch_bounds__(512) k_embed_sum(ReduceArgs a) {
         if (!head && !more) put_row<TO, V>(a, key, c, s);
         else s.store(a.part + ((int64_t)p * 2 + (head ? 0 : 1)) * a.ldp + (int64_t)c * V);
     };
-    for (int e = e0; e < e1; e += UN) {
+    for (int e = 0; e < cnt; e += UN) {
         Vec<T, V> v[UN];
-        int32_t k[UN];
+        // past the piece's end: its last row again, not added
+#pragma unroll
+        for (int u = 0; u < UN; ++u)
+            v[u].load(g + (int64_t)__builtin_amdgcn_readlane(pos, min(e + u, cnt - 1)) * a.ldg);
 #pragma unroll
         for (int u = 0; u < UN; ++u) {
-            const int q = min(e + u, e1 - 1);
-            k[u] = a.keys[q];
-            if (on) v[u].load(g + (int64_t)a.pos[q] * a.ldg);
-        }
-#pragma unroll
-        for (int u = 0; u < UN; ++u) {
-            if (e + u >= e1) break;
-            if (k[u] != key) {
+            if (e + u >= cnt) break;
+            const int32_t k = __builtin_amdgcn_readlane(keys, e + u);
+            if (k != key) {
                 flush(false);
-                key = k[u];
+                key = k;
                 head = false;
 #pragma unroll
                 for (int i = 0; i < V; ++i) s.v[i] = 0.f;
             }
-            if (on)
 #pragma unroll
-                for (int i = 0; i < V; ++i) s.v[i] += v[u].v[i];
+            for (int i = 0; i < V; ++i) s.v[i] += v[u].v[i];
         }
     }
-    flush(e1 < a.n && a.keys[e1] == key);
+    flush(after == key);
 }
 
 // The rows that cross pieces: the piece in which such a row begins adds its
@@ -417,25 +420,35 @@ __global__ void __launch_bounds__(512) k_embed_join(ReduceArgs a) {
     const int p = blockIdx.x / a.slabs, slab = blockIdx.x % a.slabs, t = threadIdx.x;
     const int e0 = p * a.piece, e1 = min(a.n, e0 + a.piece);
     if (e1 >= a.n) return;
-    const int32_t key = a.keys[e1 - 1];
+    const int32_t key = a.keys[e1 - 1], first = a.keys[e0], before = p > 0 ? a.keys[e0 - 1] : -1;
     if (key >= a.vocab || a.keys[e1] != key) return;
-    if (a.keys[e0] == key && p > 0 && a.keys[e0 - 1] == key) return;      // begun before this piece
+    if (first == key && before == key) return;      // begun before this piece
     const int per = (a.vecs + a.slabs - 1) / a.slabs;
     const int c = slab * per + t;
+    // pieces p + 1 .. p + m begin with the row
+    int m = 0;
+    for (int q0 = p + 1; q0 < a.pieces; q0 += 64) {
+        const int64_t at = (int64_t)(q0 + (t & 63)) * a.piece;
+        const uint64_t same = __ballot(at < a.n && a.keys[at] == key);
+        const int run = ~same ? __ffsll((unsigned long long)~same) - 1 : 64;
+        m += run;
+        if (run < 64) break;
+    }
     if (t >= per || c >= a.vecs) return;
+    constexpr int UN = 8;
     Vec<float, V> s;
     s.load(a.part + ((int64_t)p * 2 + 1) * a.ldp + (int64_t)c * V);
-    int q = p + 1;
-    // piece q holds more of the row; the last such piece is the first that does not end in it
-    // before the list goes on with it
-    while (true) {
-        Vec<float, V> v;
-        v.load(a.part + (int64_t)q * 2 * a.ldp + (int64_t)c * V);
+    const float* from = a.part + (int64_t)(p + 1) * 2 * a.ldp + (int64_t)c * V;
+    for (int q = 0; q < m; q += UN) {
+        Vec<float, V> v[UN];
 #pragma unroll
-        for (int i = 0; i < V; ++i) s.v[i] += v.v[i];
-        const int64_t nx = (int64_t)(q + 1) * a.piece;
-        if (nx >= a.n || a.keys[nx] != key) break;
-        ++q;
+        for (int u = 0; u < UN; ++u) v[u].load(from + (int64_t)min(q + u, m - 1) * 2 * a.ldp);
+#pragma unroll
+        for (int u = 0; u < UN; ++u) {
+            if (q + u >= m) break;
+#pragma unroll
+            for (int i = 0; i < V; ++i) s.v[i] += v[u].v[i];
+        }
     }
     put_row<TO, V>(a, key, c, s);
 }
@@ -443,10 +456,10 @@ __global__ void __launch_bounds__(512) k_embed_join(ReduceArgs a) {
 size_t align256(size_t v) { return (v + 255) & ~size_t(255); }
 
 struct GradPlan {
-    int bits, passes, nb, piece, pieces, words;
+    int bits, passes, nb, piece, pieces;
     int64_t ldp;
     bool small;
-    size_t keys[2], pos[2], hist, used, part, total;
+    size_t keys[2], pos[2], hist, part, total;
 };
 
 GradPlan grad_plan(const m2_embedding_grad_args& a) {
@@ -455,21 +468,19 @@ GradPlan grad_plan(const m2_embedding_grad_args& a) {
     while ((1ll << kb) <= a.vocab) ++kb;          // keys 0 .. vocab
     p.passes = (kb + 8) / 9;
     p.bits = (kb + p.passes - 1) / p.passes;
-    p.small = a.n <= SMALL_N;
+    p.small = a.n <= SMALL_N && kb <= 32 - SMALL_POS;
     p.nb = (int)((a.n + SORT_TILE - 1) / SORT_TILE);
     // entries per piece: about 512 pieces, so that every CU has two, of 4 to 32
     // entries (longer pieces leave fewer partial rows, shorter ones more
     // workgroups to a small batch)
     int64_t e = a.n / 512;
-    p.piece = e < 4 ? 4 : e > 32 ? 32 : (int)e;
+    p.piece = e < 4 ? 4 : e > MAX_PIECE ? MAX_PIECE : (int)e;
     p.pieces = (int)((a.n + p.piece - 1) / p.piece);
-    p.words = (int)((a.vocab + 31) / 32);
     p.ldp = (a.dim + 7) / 8 * 8;
     size_t at = 0;
     auto take = [&](size_t bytes) { const size_t r = at; at += align256(bytes); return r; };
     for (int i = 0; i < 2; ++i) { p.keys[i] = take(4 * (size_t)a.n); p.pos[i] = take(4 * (size_t)a.n); }
     p.hist = take(4 * (size_t)p.nb << p.bits);
-    p.used = take(4 * (size_t)p.words);
     p.part = take((size_t)p.pieces * 2 * p.ldp * 4);
     p.total = at;
     return p;
@@ -485,8 +496,8 @@ int check_grad(const m2_embedding_grad_args& a) {
 }
 
 template <typename T, typename TO, int V>
-void launch_sums(const ReduceArgs& r, unsigned fill, int threads, hipStream_t s) {
-    hipLaunchKernelGGL((k_embed_sum<T, TO, V>), dim3(r.nred + fill), dim3(threads), 0, s, r);
+void launch_sums(const ReduceArgs& r, int threads, hipStream_t s) {
+    hipLaunchKernelGGL((k_embed_sum<T, TO, V>), dim3(r.nred), dim3(threads), 0, s, r);
     if (r.pieces > 1)
         hipLaunchKernelGGL((k_embed_join<TO, V>), dim3(r.nred), dim3(threads), 0, s, r);
 }
@@ -549,38 +560,55 @@ int launch_embedding_grad(const m2_embedding_grad_args& a, hipStream_t s) {
     char* ws = static_cast<char*>(a.workspace);
     auto at = [&](size_t o) { return reinterpret_cast<int32_t*>(ws + o); };
     SortArgs k{};
-    k.ids = a.ids; k.used = reinterpret_cast<uint32_t*>(ws + p.used); k.hist = at(p.hist);
+    k.ids = a.ids; k.hist = at(p.hist);
     k.vocab = a.vocab; k.padding = a.padding_idx; k.n = (int)a.n; k.id64 = a.id_dtype == M2_I64;
-    k.bits = p.bits; k.words = p.words;
+    k.bits = p.bits;
+    const int64_t osz = (int64_t)m2_dtype_size(a.out_dtype);
+    FillArgs f{static_cast<char*>(a.out), 0, 0, a.ldo * osz, a.dim * osz, 0};
+    f.flat = a.ldo == a.dim && al16(a.out);
+    // workgroups that write the zeros of rows r0 .. r1: a multiple of 16 rows keeps the next
+    // part of a flat range on a 16-byte boundary
+    const int parts = p.small ? 1 : 2 * p.passes;
+    auto zeros = [&](int i, int64_t most) -> unsigned {
+        if (a.accumulate) return 0;
+        f.r0 = a.vocab * i / parts / 16 * 16;
+        f.r1 = i + 1 == parts ? a.vocab : a.vocab * (i + 1) / parts / 16 * 16;
+        const int64_t b = ((f.r1 - f.r0) * f.row + FILL_BYTES - 1) / FILL_BYTES;
+        return (unsigned)(b < most ? b : most);
+    };
     int cur = 0;
     if (p.small) {
-        // one launch (also for n == 0, which only clears the bitmap)
+        // one launch (also for n == 0, which only writes the zeros)
         k.nb = p.passes;
         k.keys_out = at(p.keys[0]); k.pos_out = at(p.pos[0]);
-        hipLaunchKernelGGL(k_sort_small, dim3(1), dim3(SMALL_THREADS), 0, s, k);
+        const dim3 grid(1 + zeros(0, 8192)), thr(SMALL_THREADS);
+        if (a.n <= SMALL_THREADS) hipLaunchKernelGGL(k_sort_small<1>, grid, thr, 0, s, k, f);
+        else if (a.n <= 4 * SMALL_THREADS) hipLaunchKernelGGL(k_sort_small<4>, grid, thr, 0, s, k, f);
+        else hipLaunchKernelGGL(k_sort_small<16>, grid, thr, 0, s, k, f);
     } else {
         k.nb = p.nb;
         for (int pass = 0; pass < p.passes; ++pass) {
             k.shift = pass * p.bits;
             k.keys_out = at(p.keys[cur]); k.pos_out = at(p.pos[cur]);
-            hipLaunchKernelGGL(k_sort_hist, dim3(p.nb), dim3(SORT_THREADS), 0, s, k);
-            hipLaunchKernelGGL(k_sort_scatter, dim3(p.nb), dim3(SORT_THREADS), 0, s, k,
-                               (int)(pass == p.passes - 1));
+            unsigned z = zeros(2 * pass, 8192);
+            hipLaunchKernelGGL(k_sort_hist, dim3(p.nb + z), dim3(SORT_THREADS), 0, s, k, f);
+            z = zeros(2 * pass + 1, 8192);
+            hipLaunchKernelGGL(k_sort_scatter, dim3(p.nb + z), dim3(SORT_THREADS), 0, s, k, f);
             k.keys_in = k.keys_out; k.pos_in = k.pos_out;
             cur ^= 1;
         }
         cur ^= 1;
     }
     if (int rc = check_launch(who)) return rc;
+    if (a.n == 0) return M2_OK;
     const int gs = (int)m2_dtype_size(a.grad_dtype), os = (int)m2_dtype_size(a.out_dtype);
-    const int ev = gs == 2 ? 8 : 4;
     const bool vec = a.dim % 8 == 0 && a.ldg % 8 == 0 && a.ldo % 8 == 0 && al16(a.grad) && al16(a.out);
     ReduceArgs r{};
-    r.keys = at(p.keys[cur]); r.pos = at(p.pos[cur]); r.used = k.used;
+    r.keys = at(p.keys[cur]); r.pos = at(p.pos[cur]);
     r.grad = a.grad; r.out = a.out; r.part = reinterpret_cast<float*>(ws + p.part);
     r.ldg = a.ldg; r.ldo = a.ldo; r.ldp = p.ldp; r.vocab = a.vocab;
     r.n = (int)a.n; r.piece = p.piece; r.pieces = p.pieces; r.accumulate = a.accumulate;
-    r.scale = a.scale; r.cols = (int)a.dim;
+    r.scale = a.scale;
     const int V = vec ? 8 : 1;
     r.vecs = (int)(a.dim / V);
     r.slabs = (r.vecs + 511) / 512;
@@ -588,13 +616,10 @@ int launch_embedding_grad(const m2_embedding_grad_args& a, hipStream_t s) {
     const int threads = (per + 63) / 64 * 64;
     M2_REQUIRE((int64_t)p.pieces * r.slabs < (1ll << 30), M2_ERR_UNSUPPORTED, "%s: too large", who);
     r.nred = p.pieces * r.slabs;
-    const int64_t rows = (a.vocab + threads / 64 - 1) / (threads / 64);
-    const unsigned fill = a.accumulate ? 0u : (unsigned)(rows < 4096 ? rows : 4096);
-    if (r.nred + fill == 0) return M2_OK;
 #define M2_SUMS(T, TO)                                         \
     do {                                                       \
-        if (vec) launch_sums<T, TO, 8>(r, fill, threads, s);   \
-        else launch_sums<T, TO, 1>(r, fill, threads, s);       \
+        if (vec) launch_sums<T, TO, 8>(r, threads, s);   \
+        else launch_sums<T, TO, 1>(r, threads, s);       \
     } while (0)
     if (gs == 2 && os == 2) M2_SUMS(bf16, bf16);
     else if (gs == 2) M2_SUMS(bf16, float);

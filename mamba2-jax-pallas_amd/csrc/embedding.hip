@@ -20,6 +20,8 @@
 // by HBM: grad read once, the result written once and those rows again.
 #include "m2_internal.h"
 
+#include <type_traits>
+
 namespace {
 
 constexpr int SORT_THREADS = 256, SORT_ITEMS = 8, SORT_TILE = SORT_THREADS * SORT_ITEMS;
@@ -31,16 +33,17 @@ M2_DEV int64_t load_id(const void* ids, int64_t i, int is64) {
                 : (int64_t) reinterpret_cast<const int32_t*>(ids)[i];
 }
 
-// V consecutive elements as floats (one 16-byte access where V fills it)
+// V consecutive elements as floats (one access of at most 16 bytes at a time)
 template <typename T, int V> struct Vec {
     float v[V];
     M2_DEV void load(const T* p) {
         if constexpr (V == 1) {
             v[0] = to_f32(*p);
         } else if constexpr (sizeof(T) == 2) {
-            const u32x4 r = *reinterpret_cast<const u32x4*>(p);
+            typedef uint32_t Raw __attribute__((ext_vector_type(V / 2)));
+            const Raw r = *reinterpret_cast<const Raw*>(p);
 #pragma unroll
-            for (int i = 0; i < 4; ++i) { v[2 * i] = bf16_lo(r[i]); v[2 * i + 1] = bf16_hi(r[i]); }
+            for (int i = 0; i < V / 2; ++i) { v[2 * i] = bf16_lo(r[i]); v[2 * i + 1] = bf16_hi(r[i]); }
         } else {
 #pragma unroll
             for (int i = 0; i < V; i += 4) {
@@ -54,10 +57,11 @@ template <typename T, int V> struct Vec {
         if constexpr (V == 1) {
             *p = from_f32<T>(v[0]);
         } else if constexpr (sizeof(T) == 2) {
-            u32x4 r;
+            typedef uint32_t Raw __attribute__((ext_vector_type(V / 2)));
+            Raw r;
 #pragma unroll
-            for (int i = 0; i < 4; ++i) r[i] = pk_bf16(v[2 * i], v[2 * i + 1]);
-            *reinterpret_cast<u32x4*>(p) = r;
+            for (int i = 0; i < V / 2; ++i) r[i] = pk_bf16(v[2 * i], v[2 * i + 1]);
+            *reinterpret_cast<Raw*>(p) = r;
         } else {
 #pragma unroll
             for (int i = 0; i < V; i += 4) {
@@ -343,7 +347,7 @@ struct ReduceArgs {
     int64_t ldg, ldo, ldp, vocab;
     int n, piece, pieces;    // entries per piece
     int vecs, slabs;         // V-element pieces of a row, split over `slabs` workgroups
-    int nred, accumulate;
+    int accumulate;
     float scale;
 };
 
@@ -367,7 +371,6 @@ constexpr int MAX_PIECE = 32;
 
 template <typename T, typename TO, int V>
 __global__ void __launch_bounds__(512) k_embed_sum(ReduceArgs a) {
-    constexpr int UN = 8;                 // rows in flight
     const int t = threadIdx.x, lane = t & 63;
     const int p = blockIdx.x / a.slabs, slab = blockIdx.x % a.slabs;
     const int per = (a.vecs + a.slabs - 1) / a.slabs;
@@ -389,15 +392,13 @@ __global__ void __launch_bounds__(512) k_embed_sum(ReduceArgs a) {
         if (!head && !more) put_row<TO, V>(a, key, c, s);
         else s.store(a.part + ((int64_t)p * 2 + (head ? 0 : 1)) * a.ldp + (int64_t)c * V);
     };
-    for (int e = 0; e < cnt; e += UN) {
+    auto add = [&](int e, auto count) {
+        constexpr int UN = decltype(count)::value;
         Vec<T, V> v[UN];
-        // past the piece's end: its last row again, not added
 #pragma unroll
-        for (int u = 0; u < UN; ++u)
-            v[u].load(g + (int64_t)__builtin_amdgcn_readlane(pos, min(e + u, cnt - 1)) * a.ldg);
+        for (int u = 0; u < UN; ++u) v[u].load(g + (int64_t)__builtin_amdgcn_readlane(pos, e + u) * a.ldg);
 #pragma unroll
         for (int u = 0; u < UN; ++u) {
-            if (e + u >= cnt) break;
             const int32_t k = __builtin_amdgcn_readlane(keys, e + u);
             if (k != key) {
                 flush(false);
@@ -409,22 +410,28 @@ __global__ void __launch_bounds__(512) k_embed_sum(ReduceArgs a) {
 #pragma unroll
             for (int i = 0; i < V; ++i) s.v[i] += v[u].v[i];
         }
-    }
+    };
+    int e = 0;
+    for (; e + 8 <= cnt; e += 8) add(e, std::integral_constant<int, 8>());
+    if (e + 4 <= cnt) { add(e, std::integral_constant<int, 4>()); e += 4; }
+    for (; e < cnt; ++e) add(e, std::integral_constant<int, 1>());
     flush(after == key);
 }
 
 // The rows that cross pieces: the piece in which such a row begins adds its
 // partial rows in order.
+// A frequent token's partial rows are a chain of loads that one workgroup waits for:
+// narrow column parts and 16 rows in flight.
+constexpr int JOIN_THREADS = 256;
 template <typename TO, int V>
-__global__ void __launch_bounds__(512) k_embed_join(ReduceArgs a) {
+__global__ void __launch_bounds__(JOIN_THREADS) k_embed_join(ReduceArgs a) {
     const int p = blockIdx.x / a.slabs, slab = blockIdx.x % a.slabs, t = threadIdx.x;
     const int e0 = p * a.piece, e1 = min(a.n, e0 + a.piece);
     if (e1 >= a.n) return;
     const int32_t key = a.keys[e1 - 1], first = a.keys[e0], before = p > 0 ? a.keys[e0 - 1] : -1;
     if (key >= a.vocab || a.keys[e1] != key) return;
     if (first == key && before == key) return;      // begun before this piece
-    const int per = (a.vecs + a.slabs - 1) / a.slabs;
-    const int c = slab * per + t;
+    const int c = slab * JOIN_THREADS + t;
     // pieces p + 1 .. p + m begin with the row
     int m = 0;
     for (int q0 = p + 1; q0 < a.pieces; q0 += 64) {
@@ -434,22 +441,25 @@ __global__ void __launch_bounds__(512) k_embed_join(ReduceArgs a) {
         m += run;
         if (run < 64) break;
     }
-    if (t >= per || c >= a.vecs) return;
-    constexpr int UN = 8;
+    if (c >= a.vecs) return;
     Vec<float, V> s;
     s.load(a.part + ((int64_t)p * 2 + 1) * a.ldp + (int64_t)c * V);
     const float* from = a.part + (int64_t)(p + 1) * 2 * a.ldp + (int64_t)c * V;
-    for (int q = 0; q < m; q += UN) {
+    auto add = [&](auto count) {
+        constexpr int UN = decltype(count)::value;
         Vec<float, V> v[UN];
 #pragma unroll
-        for (int u = 0; u < UN; ++u) v[u].load(from + (int64_t)min(q + u, m - 1) * 2 * a.ldp);
+        for (int u = 0; u < UN; ++u) v[u].load(from + (int64_t)u * 2 * a.ldp);
 #pragma unroll
-        for (int u = 0; u < UN; ++u) {
-            if (q + u >= m) break;
+        for (int u = 0; u < UN; ++u)
 #pragma unroll
             for (int i = 0; i < V; ++i) s.v[i] += v[u].v[i];
-        }
-    }
+        from += (int64_t)UN * 2 * a.ldp;
+        m -= UN;
+    };
+    while (m >= 16) add(std::integral_constant<int, 16>());
+    while (m >= 4) add(std::integral_constant<int, 4>());
+    while (m > 0) add(std::integral_constant<int, 1>());
     put_row<TO, V>(a, key, c, s);
 }
 
@@ -497,9 +507,15 @@ int check_grad(const m2_embedding_grad_args& a) {
 
 template <typename T, typename TO, int V>
 void launch_sums(const ReduceArgs& r, int threads, hipStream_t s) {
-    hipLaunchKernelGGL((k_embed_sum<T, TO, V>), dim3(r.nred), dim3(threads), 0, s, r);
-    if (r.pieces > 1)
-        hipLaunchKernelGGL((k_embed_join<TO, V>), dim3(r.nred), dim3(threads), 0, s, r);
+    hipLaunchKernelGGL((k_embed_sum<T, TO, V>), dim3((unsigned)(r.pieces * r.slabs)), dim3(threads), 0, s, r);
+    if (r.pieces > 1) {
+        constexpr int JV = V == 1 ? 1 : 4;
+        ReduceArgs j = r;
+        j.vecs = r.vecs * (V / JV);
+        j.slabs = (j.vecs + JOIN_THREADS - 1) / JOIN_THREADS;
+        hipLaunchKernelGGL((k_embed_join<TO, JV>), dim3((unsigned)(r.pieces * j.slabs)), dim3(JOIN_THREADS), 0, s,
+                           j);
+    }
 }
 
 }  // namespace
@@ -614,8 +630,7 @@ int launch_embedding_grad(const m2_embedding_grad_args& a, hipStream_t s) {
     r.slabs = (r.vecs + 511) / 512;
     const int per = (r.vecs + r.slabs - 1) / r.slabs;
     const int threads = (per + 63) / 64 * 64;
-    M2_REQUIRE((int64_t)p.pieces * r.slabs < (1ll << 30), M2_ERR_UNSUPPORTED, "%s: too large", who);
-    r.nred = p.pieces * r.slabs;
+    M2_REQUIRE((int64_t)p.pieces * (a.dim / 256 + 1) < (1ll << 30), M2_ERR_UNSUPPORTED, "%s: too large", who);
 #define M2_SUMS(T, TO)                                         \
     do {                                                       \
         if (vec) launch_sums<T, TO, 8>(r, threads, s);   \

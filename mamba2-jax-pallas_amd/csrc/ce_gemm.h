@@ -2,14 +2,13 @@
 // (linear_ce.hip), with the epilogue as a template parameter: the logits of a tile
 // exist in its accumulators only.
 //
-// A tile is BM x BN, K in steps of 64 through a ring of ST LDS slots filled by
+// A tile is BM x BN, K in steps of BK (64 or 32) through a ring of ST LDS slots filled by
 // direct global -> LDS loads; WM x WN wavefronts, 16x16x32 MFMAs.  Each operand
 // is stored in global memory either with K contiguous ("row": A[m][k]) or with K strided
 // ("col": A[k][m]):
-//   row tile in LDS: [R][64], 128-byte rows whose 16-byte pieces are XOR-swizzled by
-//     the row (piece ^ (row & 7)); fragments by ds_read_b128, eight consecutive
-//     lanes on eight different pieces: no bank conflicts;
-//   col tile in LDS: [64][R], rows of 2 R bytes whose 32-byte pieces (the 16
+//   row tile in LDS: [R][BK], rows whose 16-byte pieces are XOR-swizzled by the row
+//     (swz); fragments by ds_read_b128, without bank conflicts;
+//   col tile in LDS: [BK][R], rows of 2 R bytes whose 32-byte pieces (the 16
 //     columns of one fragment) are XOR-swizzled by f(k) = k & 3 | (k >> 3 & 1) << 2;
 //     fragments by ds_read_b64_tr_b16, whose sixteen lanes read 4 k rows: the 8 rows that
 //     32 lanes touch lie on different banks.
@@ -43,12 +42,23 @@ struct Gemm {
 };
 
 // ---------------------------------------------------------------------------
-// global -> LDS
+// global -> LDS: R rows (columns) of BK of K
 // ---------------------------------------------------------------------------
-template <int R, bool TR, int NW> struct Loader {
-    static constexpr int INSTR = R / 8;                          // 1 KB each
+// 16-byte piece p of row r of a row tile lies at slot p ^ swz(r) of the row: 16 rows of one
+// piece fill all banks, and so do the quarters of 16 lanes that a ds_read_b128 takes
+// together (4 rows of two pieces each)
+template <int BK> M2_DEV int swz(int r) {
+    if constexpr (BK == 64) return r & 7;
+    const int b = (r >> 2) & 3;
+    return ((b ^ (b >> 1)) & 1) << 1 | b >> 1;
+}
+
+template <int R, bool TR, int NW, int BK> struct Loader {
+    static constexpr int BYTES = R * BK * 2;
+    static constexpr int INSTR = BYTES / 1024;                   // 1 KB each
     static constexpr int J = INSTR >= NW ? INSTR / NW : 1;       // per wavefront
-    static constexpr int BYTES = R * 128;
+    static constexpr int PP = BK / 8;                            // pieces of a row
+    static constexpr int PR = R / 8;                             // pieces of a k row
     uint32_t off[J];         // byte offset from the tile's base
     int m0;
 
@@ -59,12 +69,10 @@ template <int R, bool TR, int NW> struct Loader {
         for (int j = 0; j < J; ++j) {
             const int in = (w * J + j) % INSTR;
             if constexpr (!TR) {
-                int r = in * 8 + (lane >> 3);
-                const int c = (lane & 7) ^ (lane >> 3);
-                r = min(m0 + r, o.lim - 1) - m0;     // may be negative: tile past the end
-                off[j] = (uint32_t)((int64_t)r * o.ld * 2 + c * 16);
+                const int row = in * (64 / PP) + lane / PP;
+                const int c = (lane & (PP - 1)) ^ swz<BK>(row);
+                off[j] = (uint32_t)((int64_t)(min(m0 + row, o.lim - 1) - m0) * o.ld * 2 + c * 16);
             } else {
-                constexpr int PR = R / 8;            // 16-byte pieces of a k row
                 const int q = in * 64 + lane;
                 const int k = q / PR, c = q % PR;
                 const int f = (k & 3) | (((k >> 3) & 1) << 2);
@@ -74,87 +82,89 @@ template <int R, bool TR, int NW> struct Loader {
             }
         }
     }
-    // the tile of K step kt, plane pl, into LDS at `lds`
-    M2_DEV void issue(const Operand& o, const void* zeros, int kt, int pl, uint32_t lds, int w, int lane) const {
+    // K step kt of plane pl: where it begins
+    M2_DEV const bf16* base(const Operand& o, int kt, int pl) const {
+        if constexpr (!TR) return o.p + pl * o.plane + (int64_t)m0 * o.ld + (int64_t)kt * BK;
+        else return o.p + pl * o.plane + (int64_t)min(kt * BK, o.klim - 1) * o.ld + m0;
+    }
+    // load j of a step into the tile at LDS address `lds`; no branches: a row operand holds
+    // whole steps, a col operand's rows past the end are its last one
+    M2_DEV void piece(const Operand& o, const bf16* base, int kt, int j, uint32_t lds, int w, int lane) const {
+        const int in = (w * J + j) % INSTR;
         if constexpr (!TR) {
-            const bf16* base = o.p + pl * o.plane + (int64_t)m0 * o.ld + (int64_t)kt * 64;
-            if (kt * 64 + 64 <= o.klim) {
-#pragma unroll
-                for (int j = 0; j < J; ++j)
-                    dma16s(base, off[j], lds + ((w * J + j) % INSTR) * 1024);
-            } else {
-                const int c = (lane & 7) ^ (lane >> 3);
-                const bool ok = kt * 64 + c * 8 < o.klim;
-#pragma unroll
-                for (int j = 0; j < J; ++j)
-                    dma16(ok ? reinterpret_cast<const char*>(base) + off[j] : zeros,
-                          lds + ((w * J + j) % INSTR) * 1024);
-            }
+            dma16s(base, off[j], lds + in * 1024);
         } else {
-            const bf16* base = o.p + pl * o.plane + (int64_t)kt * 64 * o.ld + m0;
-            if (kt * 64 + 64 <= o.klim) {
+            const int k = (in * 64 + lane) / PR;
+            const int last = o.klim - 1 - min(kt * BK, o.klim - 1);
+            dma16s(base, off[j] - (uint32_t)max(k - last, 0) * (uint32_t)(o.ld * 2), lds + in * 1024);
+        }
+    }
+    // a whole step; a row operand's pieces past klim read zeros
+    M2_DEV void issue(const Operand& o, const void* zeros, int kt, int pl, uint32_t lds, int w, int lane) const {
+        const bf16* b = base(o, kt, pl);
+        if (TR || kt * BK + BK <= o.klim) {
 #pragma unroll
-                for (int j = 0; j < J; ++j)
-                    dma16s(base, off[j], lds + ((w * J + j) % INSTR) * 1024);
-            } else {
-                constexpr int PR = R / 8;
+            for (int j = 0; j < J; ++j) piece(o, b, kt, j, lds, w, lane);
+        } else {
 #pragma unroll
-                for (int j = 0; j < J; ++j) {
-                    const int k = (((w * J + j) % INSTR) * 64 + lane) / PR;
-                    const int64_t over = max(kt * 64 + k - (o.klim - 1), 0);
-                    dma16(reinterpret_cast<const char*>(base) + off[j] - over * o.ld * 2,
-                          lds + ((w * J + j) % INSTR) * 1024);
-                }
+            for (int j = 0; j < J; ++j) {
+                const int in = (w * J + j) % INSTR;
+                const int c = (lane & (PP - 1)) ^ swz<BK>(in * (64 / PP) + lane / PP);
+                dma16(kt * BK + c * 8 < o.klim ? reinterpret_cast<const char*>(b) + off[j] : zeros, lds + in * 1024);
             }
         }
     }
 };
 
 // ---------------------------------------------------------------------------
-// LDS -> fragments: F fragments of 16 rows from row r0 of the tile, K half kk
+// LDS -> fragments: F fragments of 16 rows from row r0 of the tile, 32 of K from 32 kk on
 // ---------------------------------------------------------------------------
-template <int R, bool TR, int F> struct Reader {
+template <int R, bool TR, int F, int BK> struct Reader {
     int x;
     M2_DEV void init(int r0, int lane) {
         if constexpr (!TR) {
-            x = (r0 + (lane & 15)) * 128;
+            x = (r0 + (lane & 15)) * BK * 2;
         } else {
             const int g = lane >> 4, r = (lane & 15) >> 2;
             const int f = r | ((g & 1) << 2);
             x = (8 * g + r) * (2 * R) + (lane & 3) * 8 + (((r0 >> 4) ^ f) << 5);
         }
     }
-    M2_DEV void read(const char* s, int kk, int lane, bf16x8 (&o)[F]) const {
+    M2_DEV bf16x8 one(const char* s, int kk, int lane, int i) const {
         if constexpr (!TR) {
-            const int sl = ((((lane >> 4) + 4 * kk) ^ (lane & 7)) << 4);
-            const char* p = s + x + sl;
-#pragma unroll
-            for (int i = 0; i < F; ++i) o[i] = *reinterpret_cast<const bf16x8*>(p + i * 2048);
+            const int sl = (((lane >> 4) + 4 * kk) ^ swz<BK>(lane & 15)) << 4;
+            return *reinterpret_cast<const bf16x8*>(s + x + sl + i * 32 * BK);
         } else {
-#pragma unroll
-            for (int i = 0; i < F; ++i) {
-                const char* p = s + (x ^ (i << 5)) + kk * 32 * 2 * R;
-                const bf16x4 lo = ds_read_tr(p), hi = ds_read_tr(p + 4 * 2 * R);
-                o[i] = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
-            }
+            const char* p = s + (x ^ (i << 5)) + kk * 32 * 2 * R;
+            const bf16x4 lo = ds_read_tr(p), hi = ds_read_tr(p + 4 * 2 * R);
+            return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
         }
+    }
+    M2_DEV void read(const char* s, int kk, int lane, bf16x8 (&o)[F]) const {
+#pragma unroll
+        for (int i = 0; i < F; ++i) o[i] = one(s, kk, lane, i);
     }
 };
 
-template <int BM_, int BN_, int WM_, int WN_, int ST_, bool ATR_, bool BTR_, int TERMS_> struct Shape {
-    static constexpr int BM = BM_, BN = BN_, WM = WM_, WN = WN_, ST = ST_, TERMS = TERMS_;
+template <int BM_, int BN_, int WM_, int WN_, int ST_, int BK_, bool ATR_, bool BTR_, int TERMS_> struct Shape {
+    static constexpr int BK = BK_, BM = BM_, BN = BN_, WM = WM_, WN = WN_, ST = ST_, TERMS = TERMS_;
     static constexpr bool ATR = ATR_, BTR = BTR_;
     static constexpr int NW = WM * WN, NT = NW * 64;
     static constexpr int FM = BM / WM / 16, FN = BN / WN / 16;
-    typedef Loader<BM, ATR, NW> LA;
-    typedef Loader<BN, BTR, NW> LB;
+    typedef Loader<BM, ATR, NW, BK> LA;
+    typedef Loader<BN, BTR, NW, BK> LB;
     static constexpr int SLOT = LA::BYTES + LB::BYTES;
     static constexpr int LDS = SLOT * ST;
     static constexpr int LOADS = LA::J + LB::J;
 };
 
+// The order of the products of the planes: (0,2) (2,0) (1,1) (0,1) (1,0) (0,0)
+template <int TERMS> M2_DEV int plane_a(int t) { return TERMS == 1 ? 0 : t == 1 ? 2 : (t == 2 || t == 4) ? 1 : 0; }
+template <int TERMS> M2_DEV int plane_b(int t) { return TERMS == 1 ? 0 : t == 0 ? 2 : (t == 2 || t == 3) ? 1 : 0; }
+
+// Few tokens: the operand of the vocabulary streams from HBM through a deep ring
 template <class S, class EPI>
-__global__ void __launch_bounds__(S::NT, S::NT >= 512 || 2 * S::LDS <= 160 * 1024 ? 2 : 1) k_ce_gemm(Gemm g, EPI epi) {
+__global__ void __launch_bounds__(S::NT, 2 * S::LDS <= 160 * 1024 ? 2 : 1) k_ce_stream(Gemm g, EPI epi) {
     __shared__ __align__(1024) char smem[S::LDS];
     const int lane = threadIdx.x & 63, w = wave_id();
     const int wm = w / S::WN, wn = w % S::WN;
@@ -180,18 +190,15 @@ __global__ void __launch_bounds__(S::NT, S::NT >= 512 || 2 * S::LDS <= 160 * 102
     const uint32_t lds0 = lds_addr(smem);
     int ikt = k0, iterm = 0, islot = 0;
     auto issue = [&]() {
-        // products in the order (0,2) (2,0) (1,1) (0,1) (1,0) (0,0)
-        const int pa = S::TERMS == 1 ? 0 : iterm == 1 ? 2 : (iterm == 2 || iterm == 4) ? 1 : 0;
-        const int pb = S::TERMS == 1 ? 0 : iterm == 0 ? 2 : (iterm == 2 || iterm == 3) ? 1 : 0;
         const uint32_t l = lds0 + islot * S::SLOT;
-        la.issue(g.a, g.zeros, ikt, pa, l, w, lane);
-        lb.issue(g.b, g.zeros, ikt, pb, l + S::LA::BYTES, w, lane);
+        la.issue(g.a, g.zeros, ikt, plane_a<S::TERMS>(iterm), l, w, lane);
+        lb.issue(g.b, g.zeros, ikt, plane_b<S::TERMS>(iterm), l + S::LA::BYTES, w, lane);
         if (++ikt == k1) { ikt = k0; ++iterm; }
         if (++islot == S::ST) islot = 0;
     };
 
-    Reader<S::BM, S::ATR, S::FM> ra;
-    Reader<S::BN, S::BTR, S::FN> rb;
+    Reader<S::BM, S::ATR, S::FM, S::BK> ra;
+    Reader<S::BN, S::BTR, S::FN, S::BK> rb;
     ra.init(wm * S::FM * 16, lane);
     rb.init(wn * S::FN * 16, lane);
 
@@ -226,8 +233,160 @@ __global__ void __launch_bounds__(S::NT, S::NT >= 512 || 2 * S::LDS <= 160 * 102
         }
         if (++slot == S::ST) slot = 0;
     }
-    lds_barrier();
-    epi.template run<S>(acc, smem, m0, n0, wm, wn, lane, count, split, tm);
+    epi.template run<S>(acc, m0, n0, wm, wn, lane, count, split, tm);
+}
+
+// Many tokens: persistent workgroups, each XCD with a contiguous range of the tiles
+// (neighbours share panels in its L2).  K in steps of 64, A through a ring of three slots, B of
+// two (all 160 KB for 256 x 256); the fragments of a half step (32 of K) are read while the half
+// step before multiplies, so the matrix units wait for neither LDS nor the
+// other wavefronts but once a step:
+//   half 0 of step i: multiply F0, read F1 (half 1 of step i), load A of step i + 2
+//   wait until step i + 1 has landed; barrier: everybody has read step i
+//   half 1 of step i: multiply F1, read F0 (half 0 of step i + 1), load B of step i + 2
+// so that both halves carry as many loads (all of them in one half leave too few cycles for
+// the 64 bytes a cycle that a CU takes in).  The loads run on into the next tile, whose first
+// steps arrive during the epilogue.
+template <class LD> struct Cursor {      // the step of an operand that is loaded next
+    LD ld;
+    int id, k, k0, k1, term;
+};
+
+template <class S, class EPI>
+__global__ void __launch_bounds__(S::NT, S::NT / 256) k_ce_tile(Gemm g, EPI epi) {
+    static_assert(S::BK == 64, "");
+    constexpr int B_AT = 3 * S::LA::BYTES;
+    __shared__ __align__(1024) char smem[B_AT + 2 * S::LB::BYTES];
+    const int lane = threadIdx.x & 63, w = wave_id();
+    const int wm = w / S::WN, wn = w % S::WN;
+    const int count = *g.count;
+    const int tn_all = g.tok_n ? min(g.tn, (((count + 63) & ~63) + S::BN - 1) / S::BN) : g.tn;
+    const int per = g.tm * tn_all, tiles = per * g.splits;
+    const int nk = g.nk ? g.nk : (count + 63) >> 6;
+    // this workgroup's place among its XCD's, and the XCD's tiles: as its share of the workgroups
+    const int xcd = blockIdx.x & 7, local = blockIdx.x >> 3;
+    const int nwg = gridDim.x, lw = (nwg - xcd + 7) >> 3;
+    const int before = xcd * (nwg >> 3) + min(xcd, nwg & 7);
+    const int t0 = (int)((int64_t)tiles * before / nwg) + local, t1 = (int)((int64_t)tiles * (before + lw) / nwg);
+    if (t0 >= t1) return;
+
+    auto place = [&](int id, int& tm, int& m0, int& n0, int& split) {
+        // 8 tiles of m beside each other, then the next n
+        split = id / per;
+        id -= split * per;
+        const int grp = id / (8 * tn_all), gm = min(8, g.tm - grp * 8), in = id - grp * 8 * tn_all;
+        tm = grp * 8 + in % gm;
+        m0 = tm * S::BM;
+        n0 = in / gm * S::BN;
+    };
+    auto first_step = [&](int split) { return (int)((int64_t)nk * split / g.splits); };
+    Cursor<typename S::LA> ca;
+    Cursor<typename S::LB> cb;
+    auto start = [&](auto& c, const Operand& o, bool is_a, int id) {
+        int tm, m0, n0, split;
+        place(id, tm, m0, n0, split);
+        c.id = id;
+        c.ld.init(o, is_a ? m0 : n0, w, lane);
+        c.k0 = c.k = first_step(split);
+        c.k1 = first_step(split + 1);
+        c.term = 0;
+    };
+    // past the last step the last tile's last step is loaded again (nobody reads it)
+    auto next = [&](auto& c, const Operand& o, bool is_a) {
+        if (++c.k < c.k1) return;
+        c.k = c.k0;
+        if (++c.term < S::TERMS) return;
+        if (c.id + lw < t1) start(c, o, is_a, c.id + lw);
+        else { c.k = c.k1 - 1; c.term = S::TERMS - 1; }
+    };
+    const uint32_t lds0 = lds_addr(smem);
+
+    Reader<S::BM, S::ATR, S::FM, 64> ra;
+    Reader<S::BN, S::BTR, S::FN, 64> rb;
+    ra.init(wm * S::FM * 16, lane);
+    rb.init(wn * S::FN * 16, lane);
+    f32x4 acc[S::FM][S::FN];
+    bf16x8 a0[S::FM], b0[S::FN], a1[S::FM], b1[S::FN];
+    int sa = 0, sb = 0;           // byte offsets of the slots of the current step
+    auto after = [](int slot) { return slot == 2 * S::LA::BYTES ? 0 : slot + S::LA::BYTES; };
+    if (nk > 0) {
+        start(ca, g.a, true, t0);
+        start(cb, g.b, false, t0);
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            ca.ld.issue(g.a, g.zeros, ca.k, plane_a<S::TERMS>(ca.term), lds0 + i * S::LA::BYTES, w, lane);
+            cb.ld.issue(g.b, g.zeros, cb.k, plane_b<S::TERMS>(cb.term), lds0 + B_AT + i * S::LB::BYTES, w, lane);
+            next(ca, g.a, true);
+            next(cb, g.b, false);
+        }
+        wait_vmem<S::LOADS>();
+        lds_barrier();
+        ra.read(smem, 0, lane, a0);
+        rb.read(smem + B_AT, 0, lane, b0);
+    }
+    constexpr int RD = S::FM + S::FN;
+    for (int id = t0; id < t1; id += lw) {
+        int tm, m0, n0, split;
+        place(id, tm, m0, n0, split);
+#pragma unroll
+        for (int i = 0; i < S::FM; ++i)
+#pragma unroll
+            for (int j = 0; j < S::FN; ++j) acc[i][j] = zero4();
+        const int steps = S::TERMS * (first_step(split + 1) - first_step(split));
+        for (int st = 0; st < steps; ++st) {
+            {
+                const char* pa = smem + sa;
+                const char* pb = smem + B_AT + sb;
+                const uint32_t l = lds0 + after(after(sa));
+                const bf16* from = ca.ld.base(g.a, ca.k, plane_a<S::TERMS>(ca.term));
+#pragma unroll
+                for (int i = 0; i < S::FM; ++i) {
+#pragma unroll
+                    for (int q = i * RD / S::FM; q < (i + 1) * RD / S::FM; ++q) {
+                        if (q < S::FN) b1[q] = rb.one(pb, 1, lane, q);
+                        else a1[q - S::FN] = ra.one(pa, 1, lane, q - S::FN);
+                    }
+#pragma unroll
+                    for (int q = i * S::LA::J / S::FM; q < (i + 1) * S::LA::J / S::FM; ++q)
+                        ca.ld.piece(g.a, from, ca.k, q, l, w, lane);
+#pragma unroll
+                    for (int j = 0; j < S::FN; ++j)
+                        acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a0[i], b0[j], acc[i][j], 0, 0, 0);
+                    __builtin_amdgcn_sched_barrier(0);
+                }
+                next(ca, g.a, true);
+            }
+            wait_vmem<S::LA::J>();
+            lds_barrier();
+            __builtin_amdgcn_sched_barrier(0);
+            {
+                const uint32_t l = lds0 + B_AT + sb;
+                sa = after(sa);
+                sb ^= S::LB::BYTES;
+                const char* pa = smem + sa;
+                const char* pb = smem + B_AT + sb;
+                const bf16* from = cb.ld.base(g.b, cb.k, plane_b<S::TERMS>(cb.term));
+#pragma unroll
+                for (int i = 0; i < S::FM; ++i) {
+#pragma unroll
+                    for (int q = i * RD / S::FM; q < (i + 1) * RD / S::FM; ++q) {
+                        if (q < S::FN) b0[q] = rb.one(pb, 0, lane, q);
+                        else a0[q - S::FN] = ra.one(pa, 0, lane, q - S::FN);
+                    }
+#pragma unroll
+                    for (int q = i * S::LB::J / S::FM; q < (i + 1) * S::LB::J / S::FM; ++q)
+                        cb.ld.piece(g.b, from, cb.k, q, l, w, lane);
+#pragma unroll
+                    for (int j = 0; j < S::FN; ++j)
+                        acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a1[i], b1[j], acc[i][j], 0, 0, 0);
+                    __builtin_amdgcn_sched_barrier(0);
+                }
+                next(cb, g.b, false);
+            }
+        }
+        epi.template run<S>(acc, m0, n0, wm, wn, lane, count, split, tm);
+    }
+    wait_vmem<0>();           // no load may land after the workgroup has ended
 }
 
 }  // namespace m2ce

@@ -197,62 +197,60 @@ __global__ void __launch_bounds__(256) k_ce_pack(PackArgs a, Tokens tk) {
 // epilogues.  A lane holds, of each 16x16 block, one n (lane & 15) and 4 consecutive
 // m (4 (lane >> 4) ..).
 // ---------------------------------------------------------------------------
-// m: vocabulary, n: token -> per token (max, sum of exp(z - max)) of the tile without the target
+// m: vocabulary, n: token -> per token (max, sum of exp(z - max)) without the target of the
+// BM / WM rows of the vocabulary that a row of wavefronts holds
 struct EpiLse {
     const int* tgt;
     float* zt;
-    float2* part;        // [tm][np]
+    float2* part;        // [tm * WM][np]
     int64_t np;
     int vocab;
 
     template <class S>
-    M2_DEV void run(f32x4 (&acc)[S::FM][S::FN], char* smem, int m0, int n0, int wm, int wn, int lane, int count,
-                    int, int tm) const {
-        float2* red = reinterpret_cast<float2*>(smem);        // [WM][BN]
+    M2_DEV void run(f32x4 (&acc)[S::FM][S::FN], int m0, int n0, int wm, int wn, int lane, int count, int, int tm) const {
         const int v0 = m0 + wm * S::FM * 16 + 4 * (lane >> 4);
-        const bool edge = m0 + S::BM > vocab;
+        const float ninf = -__builtin_inff();
+        if (m0 + S::BM > vocab) {
+#pragma unroll
+            for (int i = 0; i < S::FM; ++i)
+#pragma unroll
+                for (int r = 0; r < 4; ++r)
+                    if (v0 + 16 * i + r >= vocab)
+#pragma unroll
+                        for (int j = 0; j < S::FN; ++j) acc[i][j][r] = ninf;
+        }
 #pragma unroll
         for (int j = 0; j < S::FN; ++j) {
-            const int nl = (wn * S::FN + j) * 16 + (lane & 15), n = n0 + nl;
-            const int t = n < count ? tgt[n] : -1;
-            float mx = -__builtin_inff();
+            const int n = n0 + (wn * S::FN + j) * 16 + (lane & 15);
+            // the target's place among this lane's values, if it is there (few wavefronts
+            // have one: the others pay for one comparison)
+            const int d = n < count ? tgt[n] - v0 : -1;
+            if (__ballot(d >= 0 && d < 16 * S::FM && (d & 12) == 0)) {
 #pragma unroll
-            for (int i = 0; i < S::FM; ++i) {
-                const int v = v0 + 16 * i;
+                for (int i = 0; i < S::FM; ++i)
 #pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    if (v + r == t) {
-                        zt[n] = acc[i][j][r];
-                        acc[i][j][r] = -__builtin_inff();
-                    }
-                    if (edge && v + r >= vocab) acc[i][j][r] = -__builtin_inff();
-                    mx = fmaxf(mx, acc[i][j][r]);
-                }
+                    for (int r = 0; r < 4; ++r)
+                        if (d == 16 * i + r) {
+                            zt[n] = acc[i][j][r];
+                            acc[i][j][r] = ninf;
+                        }
             }
+            float mx = ninf;
+#pragma unroll
+            for (int i = 0; i < S::FM; ++i)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) mx = fmaxf(mx, acc[i][j][r]);
             mx = fmaxf(mx, __shfl_xor(mx, 16));
             mx = fmaxf(mx, __shfl_xor(mx, 32));
-            const float b = mx == -__builtin_inff() ? 0.f : mx;
+            const float b = mx == ninf ? 0.f : mx * -LOG2E;
             float s = 0.f;
 #pragma unroll
             for (int i = 0; i < S::FM; ++i)
 #pragma unroll
-                for (int r = 0; r < 4; ++r) s += __builtin_amdgcn_exp2f((acc[i][j][r] - b) * LOG2E);
+                for (int r = 0; r < 4; ++r) s += __builtin_amdgcn_exp2f(fmaf(acc[i][j][r], LOG2E, b));
             s += __shfl_xor(s, 16);
             s += __shfl_xor(s, 32);
-            if (lane < 16) red[wm * S::BN + nl] = make_float2(mx, s);
-        }
-        __syncthreads();
-        const int t = threadIdx.x;
-        if (t < S::BN && n0 + t < count) {
-            float2 o = red[t];
-#pragma unroll
-            for (int q = 1; q < S::WM; ++q) {
-                const float2 u = red[q * S::BN + t];
-                const float m = fmaxf(o.x, u.x), b = m == -__builtin_inff() ? 0.f : m;
-                o.y = o.y * __builtin_amdgcn_exp2f((o.x - b) * LOG2E) + u.y * __builtin_amdgcn_exp2f((u.x - b) * LOG2E);
-                o.x = m;
-            }
-            part[(int64_t)tm * np + n0 + t] = o;
+            if (lane < 16 && n < count) part[((int64_t)tm * S::WM + wm) * np + n] = make_float2(mx, s);
         }
     }
 };
@@ -269,7 +267,7 @@ struct EpiG {
     int v_first, vocab;      // of the piece; of all
 
     template <class S>
-    M2_DEV void run(f32x4 (&acc)[S::FM][S::FN], char* smem, int m0, int n0, int wm, int wn, int lane, int count,
+    M2_DEV void run(f32x4 (&acc)[S::FM][S::FN], int m0, int n0, int wm, int wn, int lane, int count,
                     int, int) const {
         const int mv = m0 + wm * S::FM * 16 + 4 * (lane >> 4);
         const int lim = (count + 63) & ~63;
@@ -314,7 +312,7 @@ struct EpiDx {
     int add;
 
     template <class S>
-    M2_DEV void run(f32x4 (&acc)[S::FM][S::FN], char*, int m0, int n0, int wm, int wn, int lane, int count,
+    M2_DEV void run(f32x4 (&acc)[S::FM][S::FN], int m0, int n0, int wm, int wn, int lane, int count,
                     int split, int) const {
         const int mv = m0 + wm * S::FM * 16 + 4 * (lane >> 4);
 #pragma unroll
@@ -341,7 +339,7 @@ template <typename T> struct EpiDw {
     int rows, vec;           // rows of the piece
 
     template <class S>
-    M2_DEV void run(f32x4 (&acc)[S::FM][S::FN], char*, int m0, int n0, int wm, int wn, int lane, int, int,
+    M2_DEV void run(f32x4 (&acc)[S::FM][S::FN], int m0, int n0, int wm, int wn, int lane, int, int,
                     int) const {
         const int mv = m0 + wm * S::FM * 16 + 4 * (lane >> 4);
 #pragma unroll
@@ -495,8 +493,9 @@ Common common(int64_t n, int64_t vocab, int64_t dim, int64_t ldw, const void* w,
     c.dp = (dim + 63) / 64 * 64;
     c.f32 = dtype == M2_F32;
     // the weights are read in place where direct loads can: bf16 rows of whole 16-byte
-    // pieces (and offsets within a tile that fit 32 bits); else a copy in the workspace
-    c.pack_w = c.f32 || dim % 8 || ldw % 8 || !al16(w) || ldw > (1 << 22);
+    // pieces (and offsets within a tile that fit 32 bits), of whole K steps where the
+    // tokens are many (k_ce_tile); else a copy in the workspace
+    c.pack_w = c.f32 || dim % (n <= 64 ? 8 : 64) || ldw % 8 || !al16(w) || ldw > (1 << 22);
     auto take = [&](size_t b) { const size_t r = c.at; c.at += align256(b); return r; };
     c.idx = take(4 * (size_t)c.np);
     c.inv = take(4 * (size_t)c.np);
@@ -509,24 +508,32 @@ Common common(int64_t n, int64_t vocab, int64_t dim, int64_t ldw, const void* w,
 }
 
 template <class S, class EPI> void launch(const Gemm& g, const EPI& e, hipStream_t s) {
-    hipLaunchKernelGGL((k_ce_gemm<S, EPI>), dim3((unsigned)(g.tm * g.tn * g.splits)), dim3(S::NT), 0, s, g, e);
+    const int64_t tiles = (int64_t)g.tm * g.tn * g.splits;
+    if constexpr (S::BN < 128) {
+        hipLaunchKernelGGL((k_ce_stream<S, EPI>), dim3((unsigned)tiles), dim3(S::NT), 0, s, g, e);
+    } else {
+        const int64_t ncu = m2::cu_count();
+        hipLaunchKernelGGL((k_ce_tile<S, EPI>), dim3((unsigned)(tiles < ncu ? tiles : ncu)), dim3(S::NT), 0, s, g, e);
+    }
 }
 inline int tiles(int64_t n, int t) { return (int)((n + t - 1) / t); }
 
 // Tiles of the product vocabulary x tokens by the number of tokens
 template <bool F32> struct Shapes {
     static constexpr int T = F32 ? 6 : 1;
-    typedef Shape<256, 256, 2, 4, 2, false, false, T> Z256;
-    typedef Shape<128, 64, 4, 1, 3, false, false, T> Z64;
-    typedef Shape<128, 16, 4, 1, 4, false, false, T> Z16;
-    typedef Shape<256, 256, 2, 4, 2, true, false, T> X256;
-    typedef Shape<256, 64, 4, 1, 3, true, false, T> X64;
-    typedef Shape<256, 16, 4, 1, 3, true, false, T> X16;
-    typedef Shape<256, 256, 2, 4, 2, true, true, T> W256;
+    typedef Shape<256, 256, 2, 4, 2, 64, false, false, T> Z256;
+    typedef Shape<128, 64, 4, 1, 3, 64, false, false, T> Z64;
+    typedef Shape<128, 16, 4, 1, 4, 64, false, false, T> Z16;
+    typedef Shape<256, 256, 2, 4, 2, 64, true, false, T> X256;
+    typedef Shape<256, 64, 4, 1, 3, 64, true, false, T> X64;
+    typedef Shape<256, 16, 4, 1, 3, 64, true, false, T> X16;
+    typedef Shape<256, 256, 2, 4, 2, 64, true, true, T> W256;
 };
 // tokens of a tile
 int tok_tile(int64_t n) { return n <= 16 ? 16 : n <= 64 ? 64 : 256; }
 int voc_tile(int64_t n) { return n <= 64 ? 128 : 256; }
+// rows of the vocabulary whose sums EpiLse leaves together
+int voc_part(int64_t n) { return n <= 64 ? 32 : 128; }
 
 template <bool F32, class EPI> void launch_z(Gemm& g, int64_t rows, int64_t n, const EPI& e, hipStream_t s) {
     typedef Shapes<F32> P;
@@ -562,7 +569,7 @@ FwdPlan fwd_plan(const m2_linear_cross_entropy_args& a) {
     p.c = common(a.n, a.vocab, a.dim, a.ldw, a.weight, a.dtype);
     auto take = [&](size_t b) { const size_t r = p.c.at; p.c.at += align256(b); return r; };
     p.zt = take(4 * (size_t)p.c.np);
-    p.part = take(8 * (size_t)tiles(a.vocab, voc_tile(a.n)) * p.c.np);
+    p.part = take(8 * (size_t)(voc_tile(a.n) / voc_part(a.n)) * tiles(a.vocab, voc_tile(a.n)) * p.c.np);
     p.total = p.c.at;
     return p;
 }
@@ -657,7 +664,7 @@ template <bool F32> int run_fwd(const m2_linear_cross_entropy_args& a, const Fwd
     g.b = Operand{reinterpret_cast<bf16*>(ws + c.x), c.dp, c.np * c.dp, (int)c.np, (int)c.dp};
     EpiLse e{tk.tgt, tk.zt, reinterpret_cast<float2*>(ws + p.part), c.np, (int)c.vocab};
     launch_z<F32>(g, c.vocab, c.n, e, s);
-    JoinArgs j{e.part, c.np, c.n, a.loss, a.lse, g.tm};
+    JoinArgs j{e.part, c.np, c.n, a.loss, a.lse, g.tm * (voc_tile(c.n) / voc_part(c.n))};
     hipLaunchKernelGGL(k_ce_join, dim3((unsigned)((c.n + 15) / 16)), dim3(256), 0, s, j, tk);
     if (a.total)
         hipLaunchKernelGGL(k_ce_total, dim3(1), dim3(1024), 0, s, a.loss, c.n, a.total, a.mean, tk.count);
@@ -699,7 +706,8 @@ template <bool F32> int run_bwd(const m2_linear_cross_entropy_grad_args& a, cons
         launch_z<F32>(g, (rows + 63) / 64 * 64, c.n, eg, s);
         if (a.grad_x) {
             Gemm d = g0;
-            d.nk = (int)((rows + 63) / 64); d.tok_n = 1; d.splits = p.splits;
+            d.nk = (int)((rows + 63) / 64); d.tok_n = 1;
+            d.splits = p.splits < d.nk ? p.splits : d.nk;     // a short last piece
             d.a = w;
             d.a.p += v0 * w.ld;
             d.a.lim = wlim;

@@ -37,9 +37,33 @@ struct Gemm {
     const void* zeros;   // 16 zero bytes
     const int* count;    // kept tokens (device)
     int nk;              // K steps of 64 (per plane product), 0: from count
-    int tm, tn, splits;
-    int tok_n;           // n is the token: tiles past the kept ones end at once
+    int tm, tn;
+    int tok_n;           // n is the token: tiles past the kept ones are left out
+    int splits;          // k_ce_stream: K in so many parts
+    int seg_nk;          // k_ce_tile with EPI::SEG: the K steps that deal() goes by
 };
+
+// k_ce_tile with EPI::SEG: as many whole tiles as fill the workgroups, and the rest of the tiles
+// cut in s parts of K each, so that few workgroups are idle in the end.  Parts of the same
+// K lie beside each other (they share panels).  Segment numbers: the tile of a whole
+// one; full + part * rest + (tile - full).
+struct Deal {
+    int full, rest, s;
+};
+__host__ __device__ inline Deal deal(int tiles, int nk, int nwg) {
+    Deal d;
+    d.full = tiles / nwg * nwg;
+    d.rest = tiles - d.full;
+    d.s = 1;
+    // a step takes about 1.4 us, writing and reading a segment of 256 KB the chip 0.11 us
+    // (whole numbers: the host sizes the workspace by the same)
+    int64_t best = INT64_MAX;
+    for (int s = 1; s <= 64 && s * 4 <= nk && d.rest * s <= 2 * nwg; ++s) {
+        const int64_t cost = (int64_t)140 * ((d.rest * s + nwg - 1) / nwg) * ((nk + s - 1) / s) + 11 * d.rest * s;
+        if (cost < best) { best = cost; d.s = s; }
+    }
+    return d;
+}
 
 // ---------------------------------------------------------------------------
 // global -> LDS: R rows (columns) of BK of K
@@ -236,7 +260,7 @@ __global__ void __launch_bounds__(S::NT, 2 * S::LDS <= 160 * 1024 ? 2 : 1) k_ce_
     epi.template run<S>(acc, m0, n0, wm, wn, lane, count, split, tm);
 }
 
-// Many tokens: persistent workgroups, each XCD with a contiguous range of the tiles
+// Many tokens: persistent workgroups (whole tiles, or with EPI::SEG segments of them), each XCD with a contiguous range of the tiles
 // (neighbours share panels in its L2).  K in steps of 64, A through a ring of three slots, B of
 // two (all 160 KB for 256 x 256); the fragments of a half step (32 of K) are read while the half
 // step before multiplies, so the matrix units wait for neither LDS nor the
@@ -247,9 +271,13 @@ __global__ void __launch_bounds__(S::NT, 2 * S::LDS <= 160 * 1024 ? 2 : 1) k_ce_
 // so that both halves carry as many loads (all of them in one half leave too few cycles for
 // the 64 bytes a cycle that a CU takes in).  The loads run on into the next tile, whose first
 // steps arrive during the epilogue.
+struct Work {                 // of a workgroup: its item i, a tile and its K steps
+    int i, tile, k0, k1, seg;
+};
 template <class LD> struct Cursor {      // the step of an operand that is loaded next
     LD ld;
-    int id, k, k0, k1, term;
+    Work at;
+    int k, term;
 };
 
 template <class S, class EPI>
@@ -261,43 +289,60 @@ __global__ void __launch_bounds__(S::NT, S::NT / 256) k_ce_tile(Gemm g, EPI epi)
     const int wm = w / S::WN, wn = w % S::WN;
     const int count = *g.count;
     const int tn_all = g.tok_n ? min(g.tn, (((count + 63) & ~63) + S::BN - 1) / S::BN) : g.tn;
-    const int per = g.tm * tn_all, tiles = per * g.splits;
+    const int tiles = g.tm * tn_all;
     const int nk = g.nk ? g.nk : (count + 63) >> 6;
-    // this workgroup's place among its XCD's, and the XCD's tiles: as its share of the workgroups
+    // this workgroup's place: those of an XCD beside each other
     const int xcd = blockIdx.x & 7, local = blockIdx.x >> 3;
     const int nwg = gridDim.x, lw = (nwg - xcd + 7) >> 3;
     const int before = xcd * (nwg >> 3) + min(xcd, nwg & 7);
-    const int t0 = (int)((int64_t)tiles * before / nwg) + local, t1 = (int)((int64_t)tiles * (before + lw) / nwg);
-    if (t0 >= t1) return;
-
-    auto place = [&](int id, int& tm, int& m0, int& n0, int& split) {
+    // whole tiles one workgroup after the other; each XCD a contiguous range, which its
+    // share of the workgroups gives
+    Deal dl{0, tiles, 1};
+    if constexpr (EPI::SEG) dl = deal(tiles, g.seg_nk, nwg);
+    const int f0 = dl.full / nwg * before + local, rounds = dl.full / nwg;
+    const int64_t cut = (int64_t)dl.rest * dl.s;
+    const int r0 = (int)(cut * before / nwg) + local, r1 = (int)(cut * (before + lw) / nwg);
+    auto work = [&](int i) {
+        if (EPI::SEG && i < rounds) return Work{i, f0 + i * lw, 0, nk, f0 + i * lw};
+        const int id = r0 + (i - rounds) * lw;
+        Work x{i, 0, 0, 0, dl.full + id};
+        if (id >= r1) return x;
+        const int part = EPI::SEG ? id / dl.rest : 0;
+        x.tile = dl.full + id - part * dl.rest;
+        x.k0 = EPI::SEG ? (int)((int64_t)nk * part / dl.s) : 0;
+        x.k1 = EPI::SEG ? (int)((int64_t)nk * (part + 1) / dl.s) : nk;
+        return x;
+    };
+    const int items = rounds + (r1 > r0 ? (r1 - r0 + lw - 1) / lw : 0);
+    if (items == 0) return;
+    auto place = [&](int id, int& tm, int& m0, int& n0) {
         // 8 tiles of m beside each other, then the next n
-        split = id / per;
-        id -= split * per;
         const int grp = id / (8 * tn_all), gm = min(8, g.tm - grp * 8), in = id - grp * 8 * tn_all;
         tm = grp * 8 + in % gm;
         m0 = tm * S::BM;
         n0 = in / gm * S::BN;
     };
-    auto first_step = [&](int split) { return (int)((int64_t)nk * split / g.splits); };
     Cursor<typename S::LA> ca;
     Cursor<typename S::LB> cb;
-    auto start = [&](auto& c, const Operand& o, bool is_a, int id) {
-        int tm, m0, n0, split;
-        place(id, tm, m0, n0, split);
-        c.id = id;
+    auto start = [&](auto& c, const Operand& o, bool is_a, const Work& x) {
+        int tm, m0, n0;
+        place(x.tile, tm, m0, n0);
         c.ld.init(o, is_a ? m0 : n0, w, lane);
-        c.k0 = c.k = first_step(split);
-        c.k1 = first_step(split + 1);
+        c.at = x;
+        c.k = x.k0;
         c.term = 0;
     };
     // past the last step the last tile's last step is loaded again (nobody reads it)
     auto next = [&](auto& c, const Operand& o, bool is_a) {
-        if (++c.k < c.k1) return;
-        c.k = c.k0;
+        if (++c.k < c.at.k1) return;
+        c.k = c.at.k0;
         if (++c.term < S::TERMS) return;
-        if (c.id + lw < t1) start(c, o, is_a, c.id + lw);
-        else { c.k = c.k1 - 1; c.term = S::TERMS - 1; }
+        for (int i = c.at.i + 1; i < items; ++i) {
+            const Work x = work(i);
+            if (x.k0 < x.k1) return start(c, o, is_a, x);
+        }
+        c.k = c.at.k1 - 1;
+        c.term = S::TERMS - 1;
     };
     const uint32_t lds0 = lds_addr(smem);
 
@@ -309,9 +354,12 @@ __global__ void __launch_bounds__(S::NT, S::NT / 256) k_ce_tile(Gemm g, EPI epi)
     bf16x8 a0[S::FM], b0[S::FN], a1[S::FM], b1[S::FN];
     int sa = 0, sb = 0;           // byte offsets of the slots of the current step
     auto after = [](int slot) { return slot == 2 * S::LA::BYTES ? 0 : slot + S::LA::BYTES; };
+    int first = 0;                // the first item that has steps (a short piece's parts may not)
+    while (first < items && nk > 0 && work(first).k0 >= work(first).k1) ++first;
+    if (first == items) return;
     if (nk > 0) {
-        start(ca, g.a, true, t0);
-        start(cb, g.b, false, t0);
+        start(ca, g.a, true, work(first));
+        start(cb, g.b, false, work(first));
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
             ca.ld.issue(g.a, g.zeros, ca.k, plane_a<S::TERMS>(ca.term), lds0 + i * S::LA::BYTES, w, lane);
@@ -325,14 +373,16 @@ __global__ void __launch_bounds__(S::NT, S::NT / 256) k_ce_tile(Gemm g, EPI epi)
         rb.read(smem + B_AT, 0, lane, b0);
     }
     constexpr int RD = S::FM + S::FN;
-    for (int id = t0; id < t1; id += lw) {
-        int tm, m0, n0, split;
-        place(id, tm, m0, n0, split);
+    for (int item = first; item < items; ++item) {
+        const Work wk = work(item);
+        if (EPI::SEG && wk.k0 >= wk.k1) continue;
+        int tm, m0, n0;
+        place(wk.tile, tm, m0, n0);
 #pragma unroll
         for (int i = 0; i < S::FM; ++i)
 #pragma unroll
             for (int j = 0; j < S::FN; ++j) acc[i][j] = zero4();
-        const int steps = S::TERMS * (first_step(split + 1) - first_step(split));
+        const int steps = S::TERMS * (wk.k1 - wk.k0);
         for (int st = 0; st < steps; ++st) {
             {
                 const char* pa = smem + sa;
@@ -356,7 +406,8 @@ __global__ void __launch_bounds__(S::NT, S::NT / 256) k_ce_tile(Gemm g, EPI epi)
                 }
                 next(ca, g.a, true);
             }
-            wait_vmem<S::LA::J>();
+            // (behind an epilogue they have: its stores need not have)
+            if (st > 0 || item == first) wait_vmem<S::LA::J>();
             lds_barrier();
             __builtin_amdgcn_sched_barrier(0);
             {
@@ -384,7 +435,9 @@ __global__ void __launch_bounds__(S::NT, S::NT / 256) k_ce_tile(Gemm g, EPI epi)
                 next(cb, g.b, false);
             }
         }
-        epi.template run<S>(acc, m0, n0, wm, wn, lane, count, split, tm);
+        // what is loaded so far (step 0 and 1 of the next tile) is there before any store
+        wait_vmem<0>();
+        epi.template run<S>(acc, m0, n0, wm, wn, lane, count, wk.seg, tm);
     }
     wait_vmem<0>();           // no load may land after the workgroup has ended
 }

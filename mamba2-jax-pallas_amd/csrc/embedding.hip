@@ -33,44 +33,47 @@ M2_DEV int64_t load_id(const void* ids, int64_t i, int is64) {
                 : (int64_t) reinterpret_cast<const int32_t*>(ids)[i];
 }
 
-// V consecutive elements as floats (one access of at most 16 bytes at a time)
+// V consecutive elements as floats, aligned as elements only
 template <typename T, int V> struct Vec {
     float v[V];
     M2_DEV void load(const T* p) {
         if constexpr (V == 1) {
             v[0] = to_f32(*p);
-        } else if constexpr (sizeof(T) == 2) {
-            typedef uint32_t Raw __attribute__((ext_vector_type(V / 2)));
-            const Raw r = *reinterpret_cast<const Raw*>(p);
+        } else if constexpr (sizeof(T) == 2 && V == 8) {
+            const u32x4 r = load16(p);
 #pragma unroll
-            for (int i = 0; i < V / 2; ++i) { v[2 * i] = bf16_lo(r[i]); v[2 * i + 1] = bf16_hi(r[i]); }
+            for (int i = 0; i < 4; ++i) { v[2 * i] = bf16_lo(r[i]); v[2 * i + 1] = bf16_hi(r[i]); }
+        } else if constexpr (sizeof(T) == 2) {
+#pragma unroll
+            for (int i = 0; i < V; ++i) v[i] = to_f32(p[i]);
         } else {
 #pragma unroll
             for (int i = 0; i < V; i += 4) {
-                const f32x4 r = *reinterpret_cast<const f32x4*>(p + i);
+                const u32x4 r = load16(p + i);
 #pragma unroll
-                for (int j = 0; j < 4; ++j) v[i + j] = r[j];
+                for (int j = 0; j < 4; ++j) v[i + j] = __uint_as_float(r[j]);
             }
         }
     }
     M2_DEV void store(T* p) const {
         if constexpr (V == 1) {
             *p = from_f32<T>(v[0]);
+        } else if constexpr (sizeof(T) == 2 && V == 8) {
+            store16(p, u32x4{pk_bf16(v[0], v[1]), pk_bf16(v[2], v[3]), pk_bf16(v[4], v[5]), pk_bf16(v[6], v[7])});
         } else if constexpr (sizeof(T) == 2) {
-            typedef uint32_t Raw __attribute__((ext_vector_type(V / 2)));
-            Raw r;
-#pragma unroll
-            for (int i = 0; i < V / 2; ++i) r[i] = pk_bf16(v[2 * i], v[2 * i + 1]);
-            *reinterpret_cast<Raw*>(p) = r;
+            typedef uint32_t Any __attribute__((ext_vector_type(2), aligned(2)));
+            *reinterpret_cast<Any*>(p) = Any{pk_bf16(v[0], v[1]), pk_bf16(v[2], v[3])};
         } else {
 #pragma unroll
-            for (int i = 0; i < V; i += 4) {
-                const f32x4 r = {v[i], v[i + 1], v[i + 2], v[i + 3]};
-                *reinterpret_cast<f32x4*>(p + i) = r;
-            }
+            for (int i = 0; i < V; i += 4)
+                store16(p + i, __builtin_bit_cast(u32x4, f32x4{v[i], v[i + 1], v[i + 2], v[i + 3]}));
         }
     }
 };
+// A row of cols elements in pieces of V (V == 1 where the row is shorter than 8): piece
+// c begins at column at(c); the last one ends with the row, and its first skip(c) elements
+// are its neighbour's too (computed twice, equal).
+template <int V> M2_DEV int piece_at(int c, int cols) { return min(c * V, cols - V); }
 
 // ---------------------------------------------------------------------------
 // lookup
@@ -80,7 +83,7 @@ struct EmbedArgs {
     const void* w;
     void* out;
     int64_t n, vocab, ldw, ldo;
-    int vecs;          // V-element pieces of a row
+    int cols, vecs;    // elements of a row, V-element pieces of it
     int parts;         // column parts of a row, 64 * UN pieces each
     float scale;
     int id64;
@@ -101,13 +104,13 @@ __global__ void __launch_bounds__(256) k_embedding(EmbedArgs a) {
     Vec<T, V> v[EMB_UN];
 #pragma unroll
     for (int u = 0; u < EMB_UN; ++u)
-        if (c0 + 64 * u < a.vecs) v[u].load(src + (int64_t)(c0 + 64 * u) * V);
+        if (c0 + 64 * u < a.vecs) v[u].load(src + piece_at<V>(c0 + 64 * u, a.cols));
 #pragma unroll
     for (int u = 0; u < EMB_UN; ++u) {
         if (c0 + 64 * u >= a.vecs) continue;
 #pragma unroll
         for (int i = 0; i < V; ++i) v[u].v[i] = ok ? v[u].v[i] * a.scale : __builtin_nanf("");
-        v[u].store(dst + (int64_t)(c0 + 64 * u) * V);
+        v[u].store(dst + piece_at<V>(c0 + 64 * u, a.cols));
     }
 }
 
@@ -346,16 +349,23 @@ struct ReduceArgs {
     float* part;             // [pieces][2][ldp]: of a row begun before the piece / left unfinished
     int64_t ldg, ldo, ldp, vocab;
     int n, piece, pieces;    // entries per piece
-    int vecs, slabs;         // V-element pieces of a row, split over `slabs` workgroups
+    int cols, vecs, slabs;   // elements of a row, V-element pieces of it, split over `slabs` workgroups
     int accumulate;
     float scale;
 };
 
 template <typename TO, int V>
 M2_DEV void put_row(const ReduceArgs& a, int32_t key, int c, Vec<float, V> s) {
-    TO* p = static_cast<TO*>(a.out) + (int64_t)key * a.ldo + (int64_t)c * V;
+    const int col = piece_at<V>(c, a.cols), skip = c * V - col;
+    TO* p = static_cast<TO*>(a.out) + (int64_t)key * a.ldo + col;
 #pragma unroll
     for (int i = 0; i < V; ++i) s.v[i] *= a.scale;
+    if (a.accumulate && skip) {          // the neighbour adds the others
+#pragma unroll
+        for (int i = 0; i < V; ++i)
+            if (i >= skip) p[i] = from_f32<TO>(s.v[i] + to_f32(p[i]));
+        return;
+    }
     Vec<TO, V> o;
     if (a.accumulate) {
         o.load(p);
@@ -381,7 +391,8 @@ __global__ void __launch_bounds__(512) k_embed_sum(ReduceArgs a) {
     const int q = e0 + min(lane, cnt - 1);
     const int32_t keys = a.keys[q], pos = a.pos[q];
     const int32_t before = p > 0 ? a.keys[e0 - 1] : -1, after = e0 + cnt < a.n ? a.keys[e0 + cnt] : -1;
-    const T* g = static_cast<const T*>(a.grad) + (int64_t)(on ? c : 0) * V;
+    const int col = piece_at<V>(on ? c : 0, a.cols);
+    const T* g = static_cast<const T*>(a.grad) + col;
     int32_t key = __builtin_amdgcn_readlane(keys, 0);
     bool head = before == key;            // the row began in an earlier piece
     Vec<float, V> s;
@@ -390,7 +401,7 @@ __global__ void __launch_bounds__(512) k_embed_sum(ReduceArgs a) {
     auto flush = [&](bool more) {
         if (!on || key >= a.vocab) return;
         if (!head && !more) put_row<TO, V>(a, key, c, s);
-        else s.store(a.part + ((int64_t)p * 2 + (head ? 0 : 1)) * a.ldp + (int64_t)c * V);
+        else s.store(a.part + ((int64_t)p * 2 + (head ? 0 : 1)) * a.ldp + col);
     };
     auto add = [&](int e, auto count) {
         constexpr int UN = decltype(count)::value;
@@ -443,8 +454,9 @@ __global__ void __launch_bounds__(JOIN_THREADS) k_embed_join(ReduceArgs a) {
     }
     if (c >= a.vecs) return;
     Vec<float, V> s;
-    s.load(a.part + ((int64_t)p * 2 + 1) * a.ldp + (int64_t)c * V);
-    const float* from = a.part + (int64_t)(p + 1) * 2 * a.ldp + (int64_t)c * V;
+    const int col = piece_at<V>(c, a.cols);
+    s.load(a.part + ((int64_t)p * 2 + 1) * a.ldp + col);
+    const float* from = a.part + (int64_t)(p + 1) * 2 * a.ldp + col;
     auto add = [&](auto count) {
         constexpr int UN = decltype(count)::value;
         Vec<float, V> v[UN];
@@ -511,7 +523,7 @@ void launch_sums(const ReduceArgs& r, int threads, hipStream_t s) {
     if (r.pieces > 1) {
         constexpr int JV = V == 1 ? 1 : 4;
         ReduceArgs j = r;
-        j.vecs = r.vecs * (V / JV);
+        j.vecs = (r.cols + JV - 1) / JV;
         j.slabs = (j.vecs + JOIN_THREADS - 1) / JOIN_THREADS;
         hipLaunchKernelGGL((k_embed_join<TO, JV>), dim3((unsigned)(r.pieces * j.slabs)), dim3(JOIN_THREADS), 0, s,
                            j);
@@ -535,10 +547,10 @@ int launch_embedding(const m2_embedding_args& a, hipStream_t s) {
     M2_REQUIRE(a.ldw >= a.dim && a.ldo >= a.dim, M2_ERR_INVALID, "%s: row strides", who);
     if (a.n == 0) return M2_OK;
     M2_REQUIRE(a.ids && a.weight && a.out, M2_ERR_INVALID, "%s: ids, weight and out are required", who);
-    const int es = (int)m2_dtype_size(a.dtype), ev = 16 / es;
-    const bool vec = a.dim % ev == 0 && a.ldw % ev == 0 && a.ldo % ev == 0 && al16(a.weight) && al16(a.out);
-    EmbedArgs k{a.ids, a.weight, a.out, a.n, a.vocab, a.ldw, a.ldo, 0, 0, a.scale, a.id_dtype == M2_I64};
-    k.vecs = (int)(vec ? a.dim / ev : a.dim);
+    const int ev = 16 / (int)m2_dtype_size(a.dtype);
+    const bool vec = a.dim >= ev;
+    EmbedArgs k{a.ids, a.weight, a.out, a.n, a.vocab, a.ldw, a.ldo, (int)a.dim, 0, 0, a.scale, a.id_dtype == M2_I64};
+    k.vecs = (int)(vec ? (a.dim + ev - 1) / ev : a.dim);
     k.parts = (k.vecs + 64 * EMB_UN - 1) / (64 * EMB_UN);
     const int64_t blocks = (a.n * k.parts + 3) / 4;
     M2_REQUIRE(blocks < (1ll << 31), M2_ERR_UNSUPPORTED, "%s: too many rows", who);
@@ -618,7 +630,7 @@ int launch_embedding_grad(const m2_embedding_grad_args& a, hipStream_t s) {
     if (int rc = check_launch(who)) return rc;
     if (a.n == 0) return M2_OK;
     const int gs = (int)m2_dtype_size(a.grad_dtype), os = (int)m2_dtype_size(a.out_dtype);
-    const bool vec = a.dim % 8 == 0 && a.ldg % 8 == 0 && a.ldo % 8 == 0 && al16(a.grad) && al16(a.out);
+    const bool vec = a.dim >= 8;
     ReduceArgs r{};
     r.keys = at(p.keys[cur]); r.pos = at(p.pos[cur]);
     r.grad = a.grad; r.out = a.out; r.part = reinterpret_cast<float*>(ws + p.part);
@@ -626,7 +638,8 @@ int launch_embedding_grad(const m2_embedding_grad_args& a, hipStream_t s) {
     r.n = (int)a.n; r.piece = p.piece; r.pieces = p.pieces; r.accumulate = a.accumulate;
     r.scale = a.scale;
     const int V = vec ? 8 : 1;
-    r.vecs = (int)(a.dim / V);
+    r.cols = (int)a.dim;
+    r.vecs = (int)((a.dim + V - 1) / V);
     r.slabs = (r.vecs + 511) / 512;
     const int per = (r.vecs + r.slabs - 1) / r.slabs;
     const int threads = (per + 63) / 64 * 64;

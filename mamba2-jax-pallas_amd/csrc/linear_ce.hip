@@ -93,16 +93,16 @@ __global__ void __launch_bounds__(1024) k_ce_compact(const void* targets, int64_
 }
 
 // 8 consecutive elements of a row, zero past its end
-template <typename T> M2_DEV void load8(const T* row, int64_t c, int64_t dim, bool vec, float (&v)[8]) {
-    if (vec && c + 8 <= dim) {
+template <typename T> M2_DEV void load8(const T* row, int64_t c, int64_t dim, float (&v)[8]) {
+    if (c + 8 <= dim) {
         if constexpr (sizeof(T) == 2) {
-            const u32x4 r = *reinterpret_cast<const u32x4*>(row + c);
+            const u32x4 r = load16(row + c);
 #pragma unroll
             for (int i = 0; i < 4; ++i) { v[2 * i] = bf16_lo(r[i]); v[2 * i + 1] = bf16_hi(r[i]); }
         } else {
-            const f32x4 a = *reinterpret_cast<const f32x4*>(row + c), b = *reinterpret_cast<const f32x4*>(row + c + 4);
+            const u32x4 a = load16(row + c), b = load16(row + c + 4);
 #pragma unroll
-            for (int i = 0; i < 4; ++i) { v[i] = a[i]; v[4 + i] = b[i]; }
+            for (int i = 0; i < 4; ++i) { v[i] = __uint_as_float(a[i]); v[4 + i] = __uint_as_float(b[i]); }
         }
     } else {
 #pragma unroll
@@ -135,7 +135,6 @@ struct PackArgs {
     const void* src;
     bf16* dst;
     int64_t rows, dim, ld, dp, plane;
-    int vec;
     // of the tokens
     const void* targets;
     const float* lse;
@@ -184,7 +183,7 @@ __global__ void __launch_bounds__(256) k_ce_pack(PackArgs a, Tokens tk) {
     for (int64_t c = lane * 8; c < a.dp; c += 512) {
         float v[8];
         if (from >= 0) {
-            load8(src, c, a.dim, a.vec, v);
+            load8(src, c, a.dim, v);
         } else {
 #pragma unroll
             for (int i = 0; i < 8; ++i) v[i] = 0.f;
@@ -200,6 +199,7 @@ __global__ void __launch_bounds__(256) k_ce_pack(PackArgs a, Tokens tk) {
 // m: vocabulary, n: token -> per token (max, sum of exp(z - max)) without the target of the
 // BM / WM rows of the vocabulary that a row of wavefronts holds
 struct EpiLse {
+    static constexpr bool SEG = false;
     const int* tgt;
     float* zt;
     float2* part;        // [tm * WM][np]
@@ -255,9 +255,58 @@ struct EpiLse {
     }
 };
 
+// Two fragments of 16 m beside each other, x and y: lane rows (16 lanes) 0 and 2 exchange
+// theirs of y for rows 1's and 3's of x, after which a lane holds 8 consecutive m from
+// pair_m on: (p, q)
+M2_DEV void pair_swap(uint32_t& p, uint32_t& q) {
+    const auto r = __builtin_amdgcn_permlane16_swap(p, q, false, false);
+    p = r[0];
+    q = r[1];
+}
+M2_DEV int pair_m(int lane) { return 16 * ((lane >> 4) & 1) + 8 * (lane >> 5); }
+M2_DEV void store_pair(bf16* d, const float (&x)[4], const float (&y)[4]) {
+    uint32_t a0 = pk_bf16(x[0], x[1]), a1 = pk_bf16(x[2], x[3]);
+    uint32_t b0 = pk_bf16(y[0], y[1]), b1 = pk_bf16(y[2], y[3]);
+    pair_swap(a0, b0);
+    pair_swap(a1, b1);
+    *reinterpret_cast<u32x4*>(d) = u32x4{a0, a1, b0, b1};
+}
+// the 32 values of m from m0 on (two fragments) of one n into a row of dim elements
+template <typename T>
+M2_DEV void store_row(T* row, int m0, int64_t dim, int lane, const f32x4& x, const f32x4& y) {
+    if constexpr (sizeof(T) == 2) {
+        // (the exchange is among the lanes of this n: all of them are here)
+        uint32_t p[4] = {pk_bf16(x[0], x[1]), pk_bf16(x[2], x[3]), pk_bf16(y[0], y[1]), pk_bf16(y[2], y[3])};
+        pair_swap(p[0], p[2]);
+        pair_swap(p[1], p[3]);
+        const int m = m0 + pair_m(lane);
+        if (m + 8 <= dim) {
+            store16(row + m, u32x4{p[0], p[1], p[2], p[3]});
+        } else {
+#pragma unroll
+            for (int r = 0; r < 8; ++r)
+                if (m + r < dim) reinterpret_cast<uint16_t*>(row)[m + r] = (uint16_t)(p[r >> 1] >> (16 * (r & 1)));
+        }
+    } else {
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+            const int m = m0 + 16 * e + 4 * (lane >> 4);
+            const f32x4& v = e ? y : x;
+            if (m + 4 <= dim) {
+                store16(row + m, __builtin_bit_cast(u32x4, v));
+            } else {
+#pragma unroll
+                for (int r = 0; r < 4; ++r)
+                    if (m + r < dim) row[m + r] = v[r];
+            }
+        }
+    }
+}
+
 // m: vocabulary, n: token -> G, bf16 (three planes for float32 operands), zero past the
 // vocabulary and past the kept tokens
 struct EpiG {
+    static constexpr bool SEG = false;
     const int* tgt;
     const float* lse;
     const float* gf;
@@ -267,53 +316,80 @@ struct EpiG {
     int v_first, vocab;      // of the piece; of all
 
     template <class S>
-    M2_DEV void run(f32x4 (&acc)[S::FM][S::FN], int m0, int n0, int wm, int wn, int lane, int count,
-                    int, int) const {
-        const int mv = m0 + wm * S::FM * 16 + 4 * (lane >> 4);
+    M2_DEV void run(f32x4 (&acc)[S::FM][S::FN], int m0, int n0, int wm, int wn, int lane, int count, int, int) const {
+        static_assert(S::FM % 2 == 0, "");
+        const int mw = m0 + wm * S::FM * 16, mv = mw + 4 * (lane >> 4);
         const int lim = (count + 63) & ~63;
+        // of the tokens, before the first store (a load behind it would wait for it)
+        int t[S::FN];
+        float ls[S::FN], g[S::FN], gt[S::FN];
+#pragma unroll
+        for (int j = 0; j < S::FN; ++j) {
+            const int n = n0 + (wn * S::FN + j) * 16 + (lane & 15);
+            const bool on = n < count;
+            t[j] = on ? tgt[n] - v_first : -1;
+            ls[j] = on ? lse[n] * -LOG2E : 0.f;
+            g[j] = on ? gf[n] : 0.f;
+            gt[j] = on ? gm[n] : 0.f;
+        }
+        // rows past the vocabulary: zeros, whatever x holds
+        const bool edge = v_first + m0 + S::BM > vocab;
 #pragma unroll
         for (int j = 0; j < S::FN; ++j) {
             const int n = n0 + (wn * S::FN + j) * 16 + (lane & 15);
             if (n >= lim) continue;
             const bool on = n < count;
-            const int t = on ? tgt[n] - v_first : -1;
-            const float ls = on ? lse[n] : 0.f, g = on ? gf[n] : 0.f, gt = on ? gm[n] : 0.f;
+            const int d = on ? t[j] - mv : -1;
+            const bool here = __ballot(d >= 0 && d < 16 * S::FM && (d & 12) == 0);
+            bf16* to = G + (int64_t)n * ldg + mw + pair_m(lane);
 #pragma unroll
-            for (int i = 0; i < S::FM; ++i) {
-                const int m = mv + 16 * i;
-                float o[4];
+            for (int i = 0; i < S::FM; i += 2) {
+                float o[2][4];
 #pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    const float p = g * __builtin_amdgcn_exp2f((acc[i][j][r] - ls) * LOG2E);
-                    o[r] = !on || v_first + m + r >= vocab ? 0.f : m + r == t ? gt : p;
-                }
-                bf16* d = G + (int64_t)n * ldg + m;
-                typedef uint32_t u2 __attribute__((ext_vector_type(2)));
+                for (int e = 0; e < 2; ++e)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) {
+                        const float p = g[j] * __builtin_amdgcn_exp2f(fmaf(acc[i + e][j][r], LOG2E, ls[j]));
+                        o[e][r] = on ? p : 0.f;
+                    }
+                if (here)
+#pragma unroll
+                    for (int e = 0; e < 2; ++e)
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) o[e][r] = d == 16 * (i + e) + r ? gt[j] : o[e][r];
+                if (edge)
+#pragma unroll
+                    for (int e = 0; e < 2; ++e)
+#pragma unroll
+                        for (int r = 0; r < 4; ++r)
+                            if (v_first + mv + 16 * (i + e) + r >= vocab) o[e][r] = 0.f;
                 if constexpr (S::TERMS == 1) {
-                    *reinterpret_cast<u2*>(d) = u2{pk_bf16(o[0], o[1]), pk_bf16(o[2], o[3])};
+                    store_pair(to + 16 * i, o[0], o[1]);
                 } else {
-                    float h[4], md[4], l[4];
+                    float h[2][4], md[2][4], l[2][4];
 #pragma unroll
-                    for (int r = 0; r < 4; ++r) split3(o[r], h[r], md[r], l[r]);
-                    *reinterpret_cast<u2*>(d) = u2{pk_bf16(h[0], h[1]), pk_bf16(h[2], h[3])};
-                    *reinterpret_cast<u2*>(d + plane) = u2{pk_bf16(md[0], md[1]), pk_bf16(md[2], md[3])};
-                    *reinterpret_cast<u2*>(d + 2 * plane) = u2{pk_bf16(l[0], l[1]), pk_bf16(l[2], l[3])};
+                    for (int e = 0; e < 2; ++e)
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) split3(o[e][r], h[e][r], md[e][r], l[e][r]);
+                    store_pair(to + 16 * i, h[0], h[1]);
+                    store_pair(to + 16 * i + plane, md[0], md[1]);
+                    store_pair(to + 16 * i + 2 * plane, l[0], l[1]);
                 }
             }
         }
     }
 };
 
-// m: dim, n: token -> float32 partial sums of dx, one array per split, added to over the
-// pieces of the vocabulary
-struct EpiDx {
+// m: dim, n: token -> float32 partial sums of dx, added to over the pieces of the vocabulary.
+// Few tokens (k_ce_stream): one array per split of K.
+struct EpiDxSplit {
     float* part;             // [splits][np][dp]
     int64_t np, dp;
     int add;
 
     template <class S>
-    M2_DEV void run(f32x4 (&acc)[S::FM][S::FN], int m0, int n0, int wm, int wn, int lane, int count,
-                    int split, int) const {
+    M2_DEV void run(f32x4 (&acc)[S::FM][S::FN], int m0, int n0, int wm, int wn, int lane, int count, int split,
+                    int) const {
         const int mv = m0 + wm * S::FM * 16 + 4 * (lane >> 4);
 #pragma unroll
         for (int j = 0; j < S::FN; ++j) {
@@ -331,39 +407,45 @@ struct EpiDx {
         }
     }
 };
+// Many (k_ce_tile): a segment as the lanes hold it, [wavefront][i][j][lane] of 4 values.
+struct EpiDxSeg {
+    static constexpr bool SEG = true;
+    float* part;             // [segments][BM * BN]
+    int add;
+
+    template <class S>
+    M2_DEV void run(f32x4 (&acc)[S::FM][S::FN], int, int, int wm, int wn, int lane, int, int seg, int) const {
+        f32x4* d = reinterpret_cast<f32x4*>(part) +
+                   ((int64_t)seg * S::NW + wm * S::WN + wn) * S::FM * S::FN * 64 + lane;
+        if (add) {
+#pragma unroll
+            for (int i = 0; i < S::FM; ++i)
+#pragma unroll
+                for (int j = 0; j < S::FN; ++j) acc[i][j] += d[(i * S::FN + j) * 64];
+        }
+#pragma unroll
+        for (int i = 0; i < S::FM; ++i)
+#pragma unroll
+            for (int j = 0; j < S::FN; ++j) d[(i * S::FN + j) * 64] = acc[i][j];
+    }
+};
 
 // m: dim, n: vocabulary -> rows of dw
 template <typename T> struct EpiDw {
+    static constexpr bool SEG = false;
     T* dw;
     int64_t dim;
-    int rows, vec;           // rows of the piece
+    int rows;                // rows of the piece
 
     template <class S>
-    M2_DEV void run(f32x4 (&acc)[S::FM][S::FN], int m0, int n0, int wm, int wn, int lane, int, int,
-                    int) const {
-        const int mv = m0 + wm * S::FM * 16 + 4 * (lane >> 4);
+    M2_DEV void run(f32x4 (&acc)[S::FM][S::FN], int m0, int n0, int wm, int wn, int lane, int, int, int) const {
 #pragma unroll
         for (int j = 0; j < S::FN; ++j) {
             const int n = n0 + (wn * S::FN + j) * 16 + (lane & 15);
             if (n >= rows) continue;
-            T* d = dw + (int64_t)n * dim;
 #pragma unroll
-            for (int i = 0; i < S::FM; ++i) {
-                const int m = mv + 16 * i;
-                if (vec && m + 4 <= dim) {
-                    if constexpr (sizeof(T) == 2) {
-                        typedef uint32_t u2 __attribute__((ext_vector_type(2)));
-                        *reinterpret_cast<u2*>(d + m) =
-                            u2{pk_bf16(acc[i][j][0], acc[i][j][1]), pk_bf16(acc[i][j][2], acc[i][j][3])};
-                    } else {
-                        *reinterpret_cast<f32x4*>(d + m) = acc[i][j];
-                    }
-                } else {
-#pragma unroll
-                    for (int r = 0; r < 4; ++r)
-                        if (m + r < dim) d[m + r] = from_f32<T>(acc[i][j][r]);
-                }
-            }
+            for (int i = 0; i < S::FM; i += 2)
+                store_row(dw + (int64_t)n * dim, m0 + (wm * S::FM + i) * 16, dim, lane, acc[i][j], acc[i + 1][j]);
         }
     }
 };
@@ -438,7 +520,7 @@ struct DxArgs {
     const float* part;
     void* dx;
     int64_t n, np, dp, dim;
-    int splits, vec;
+    int splits;
 };
 
 // dx of every row, 0 where it was left out: a wavefront per row and 512 columns
@@ -459,18 +541,63 @@ template <typename T> __global__ void __launch_bounds__(256) k_ce_dx(DxArgs a, T
             for (int i = 0; i < 4; ++i) { v[i] += x[i]; v[4 + i] += y[i]; }
         }
     }
-    if (a.vec && c + 8 <= a.dim) {
+    if (c + 8 <= a.dim) {
         if constexpr (sizeof(T) == 2) {
-            store8<false>(reinterpret_cast<bf16*>(d) + c, 0, v);
+            store16(d + c, u32x4{pk_bf16(v[0], v[1]), pk_bf16(v[2], v[3]), pk_bf16(v[4], v[5]), pk_bf16(v[6], v[7])});
         } else {
-            *reinterpret_cast<f32x4*>(d + c) = f32x4{v[0], v[1], v[2], v[3]};
-            *reinterpret_cast<f32x4*>(d + c + 4) = f32x4{v[4], v[5], v[6], v[7]};
+            store16(d + c, __builtin_bit_cast(u32x4, f32x4{v[0], v[1], v[2], v[3]}));
+            store16(d + c + 4, __builtin_bit_cast(u32x4, f32x4{v[4], v[5], v[6], v[7]}));
         }
     } else {
 #pragma unroll
         for (int i = 0; i < 8; ++i)
             if (c + i < a.dim) d[c + i] = from_f32<T>(v[i]);
     }
+}
+
+// The same from the segments of k_ce_tile, in their order: a wavefront for two fragments (32
+// columns) of 16 tokens; further workgroups zero the rows that were left out.
+struct DxSegArgs {
+    const float* part;
+    void* dx;
+    int64_t n, dim;
+    int tm, tn, seg_nk, nwg, nred;
+};
+template <typename T, class S> __global__ void __launch_bounds__(256) k_ce_dx_seg(DxSegArgs a, Tokens tk) {
+    const int lane = threadIdx.x & 63;
+    T* dx = static_cast<T*>(a.dx);
+    if ((int)blockIdx.x >= a.nred) {
+        for (int64_t r = (int64_t)(blockIdx.x - a.nred) * 4 + wave_id(); r < a.n; r += (int64_t)(gridDim.x - a.nred) * 4)
+            if (tk.inv[r] < 0)
+                for (int64_t c = lane; c < a.dim; c += 64) dx[r * a.dim + c] = from_f32<T>(0.f);
+        return;
+    }
+    const int count = *tk.count;
+    const int tn = min(a.tn, (((count + 63) & ~63) + S::BN - 1) / S::BN), tiles = a.tm * tn;
+    constexpr int PAIRS = S::FM / 2, PER = S::NW * PAIRS * S::FN;
+    int q = blockIdx.x * 4 + wave_id();
+    const int tile = q / PER;
+    q -= tile * PER;
+    if (tile >= tiles) return;
+    const int j = q % S::FN, i = q / S::FN % PAIRS * 2, w = q / S::FN / PAIRS;
+    // (the tile's place as in k_ce_tile)
+    const int grp = tile / (8 * tn), gm = min(8, a.tm - grp * 8), in = tile - grp * 8 * tn;
+    const int m0 = (grp * 8 + in % gm) * S::BM + (w / S::WN * S::FM + i) * 16;
+    const int n = in / gm * S::BN + (w % S::WN * S::FN + j) * 16 + (lane & 15);
+    if (n - (lane & 15) >= count || m0 >= a.dim) return;
+    const Deal d = deal(tiles, a.seg_nk, a.nwg);
+    constexpr int64_t SEG = (int64_t)S::NW * S::FM * S::FN * 64;
+    const f32x4* p = reinterpret_cast<const f32x4*>(a.part) + tile * SEG + (w * S::FM * S::FN + i * S::FN + j) * 64 + lane;
+    f32x4 x = p[0], y = p[S::FN * 64];
+    if (tile >= d.full) {
+#pragma unroll 8
+        for (int k = 1; k < d.s; ++k) {
+            p += d.rest * SEG;
+            x += p[0];
+            y += p[S::FN * 64];
+        }
+    }
+    if (n < count) store_row(dx + (int64_t)tk.idx[n] * a.dim, m0, a.dim, lane, x, y);
 }
 
 // ---------------------------------------------------------------------------
@@ -508,12 +635,13 @@ Common common(int64_t n, int64_t vocab, int64_t dim, int64_t ldw, const void* w,
 }
 
 template <class S, class EPI> void launch(const Gemm& g, const EPI& e, hipStream_t s) {
-    const int64_t tiles = (int64_t)g.tm * g.tn * g.splits;
+    const int64_t tiles = (int64_t)g.tm * g.tn;
     if constexpr (S::BN < 128) {
-        hipLaunchKernelGGL((k_ce_stream<S, EPI>), dim3((unsigned)tiles), dim3(S::NT), 0, s, g, e);
+        hipLaunchKernelGGL((k_ce_stream<S, EPI>), dim3((unsigned)(tiles * g.splits)), dim3(S::NT), 0, s, g, e);
     } else {
         const int64_t ncu = m2::cu_count();
-        hipLaunchKernelGGL((k_ce_tile<S, EPI>), dim3((unsigned)(tiles < ncu ? tiles : ncu)), dim3(S::NT), 0, s, g, e);
+        const unsigned nwg = (unsigned)(EPI::SEG ? g.splits : tiles < ncu ? tiles : ncu);
+        hipLaunchKernelGGL((k_ce_tile<S, EPI>), dim3(nwg), dim3(S::NT), 0, s, g, e);
     }
 }
 inline int tiles(int64_t n, int t) { return (int)((n + t - 1) / t); }
@@ -580,7 +708,7 @@ constexpr int64_t G_BYTES = 512ll << 20;
 struct BwdPlan {
     Common c;
     int64_t piece;
-    int pieces, splits;
+    int pieces, splits;      // of K for dx: parts (few tokens) or workgroups (many)
     size_t lse, gf, gm, G, dx, total;
 };
 BwdPlan bwd_plan(const m2_linear_cross_entropy_grad_args& a) {
@@ -598,11 +726,25 @@ BwdPlan bwd_plan(const m2_linear_cross_entropy_grad_args& a) {
     p.piece = ((all / 256 + p.pieces - 1) / p.pieces) * 256;
     p.pieces = (int)((all + p.piece - 1) / p.piece);
     p.G = take(2 * planes * (size_t)(p.c.np ? p.c.np : 64) * p.piece);
-    // dx: K is the piece, split so that the tiles fill the CUs; a split costs a
-    // float32 array of dx, written and read once per piece
+    // dx: K is the piece.  Many tokens: dealt out with the tiles (k_ce_tile), whose number
+    // depends on the tokens that are kept.  Few: split so that the tiles fill the CUs; a
+    // split costs a float32 array of dx, written and read once per piece
     const int ncu = m2::cu_count();
-    const int64_t t = (int64_t)tiles(a.dim, 256) * tiles(a.n ? a.n : 1, tok_tile(a.n));
-    const int steps = (int)(p.piece / 64);
+    const int tm = tiles(a.dim, 256), tn = tiles(a.n ? a.n : 1, tok_tile(a.n));
+    const int64_t t = (int64_t)tm * tn;
+    const int steps = (int)((a.vocab < p.piece ? a.vocab + 63 : p.piece) / 64);
+    if (a.n > 64) {
+        p.splits = ncu;
+        int64_t segs = 0;
+        for (int k = 1; k <= tn; ++k) {
+            const Deal d = deal(tm * k, steps, ncu);
+            const int64_t c = d.full + (int64_t)d.rest * d.s;
+            if (c > segs) segs = c;
+        }
+        p.dx = a.grad_x ? take(4 * 256 * 256 * (size_t)segs) : 0;
+        p.total = p.c.at;
+        return p;
+    }
     double best = 1e300;
     p.splits = 1;
     for (int s = 1; s <= 64 && s * 4 <= steps; ++s) {
@@ -628,15 +770,12 @@ template <typename T>
 void pack(char* ws, const Common& c, const void* x, int64_t ldx, const void* w, int64_t ldw, PackArgs a,
           const Tokens& tk, int64_t ignore, hipStream_t s) {
     hipLaunchKernelGGL(k_ce_compact, dim3(1), dim3(1024), 0, s, a.targets, c.n, ignore, a.t64, tk);
-    const int ev = 16 / (int)sizeof(T);
     a.dim = c.dim; a.dp = c.dp;
     a.src = x; a.ld = ldx; a.dst = reinterpret_cast<bf16*>(ws + c.x); a.rows = c.np; a.plane = c.np * c.dp;
-    a.vec = ldx % ev == 0 && al16(x);
     hipLaunchKernelGGL((k_ce_pack<T, true>), dim3((unsigned)(c.np / 4)), dim3(256), 0, s, a, tk);
     if (c.pack_w) {
         a.src = w; a.ld = ldw; a.dst = reinterpret_cast<bf16*>(ws + c.w); a.rows = c.vocab;
         a.plane = c.vocab * c.dp;
-        a.vec = ldw % ev == 0 && al16(w);
         hipLaunchKernelGGL((k_ce_pack<T, false>), dim3((unsigned)((c.vocab + 3) / 4)), dim3(256), 0, s, a, tk);
     }
 }
@@ -691,6 +830,7 @@ template <bool F32> int run_bwd(const m2_linear_cross_entropy_grad_args& a, cons
     g0.zeros = tk.count + 16; g0.count = tk.count; g0.splits = 1;
     float* dxp = reinterpret_cast<float*>(ws + p.dx);
     const int wlim = (int)(c.pack_w ? c.dp : c.dim);
+    DxSegArgs dxs{};
     for (int q = 0; q < p.pieces; ++q) {
         const int64_t v0 = q * p.piece;
         const int64_t rows = c.vocab - v0 < p.piece ? c.vocab - v0 : p.piece;
@@ -707,7 +847,7 @@ template <bool F32> int run_bwd(const m2_linear_cross_entropy_grad_args& a, cons
         if (a.grad_x) {
             Gemm d = g0;
             d.nk = (int)((rows + 63) / 64); d.tok_n = 1;
-            d.splits = p.splits < d.nk ? p.splits : d.nk;     // a short last piece
+            d.splits = p.splits;
             d.a = w;
             d.a.p += v0 * w.ld;
             d.a.lim = wlim;
@@ -715,11 +855,16 @@ template <bool F32> int run_bwd(const m2_linear_cross_entropy_grad_args& a, cons
             d.b = Operand{G, p.piece, gplane, (int)c.np, (int)p.piece};
             d.tm = tiles(c.dim, 256);
             d.tn = tiles(c.n, tok_tile(c.n));
-            EpiDx e{dxp, c.np, c.dp, q > 0};
-            switch (tok_tile(c.n)) {
-                case 16: launch<typename P::X16>(d, e, s); break;
-                case 64: launch<typename P::X64>(d, e, s); break;
-                default: launch<typename P::X256>(d, e, s);
+            if (c.n > 64) {
+                if (q == 0) dxs.seg_nk = d.nk;
+                d.seg_nk = dxs.seg_nk;
+                launch<typename P::X256>(d, EpiDxSeg{dxp, q > 0}, s);
+                dxs.tm = d.tm; dxs.tn = d.tn; dxs.nwg = p.splits;
+            } else {
+                if (d.splits > d.nk) d.splits = d.nk;             // a short last piece
+                const EpiDxSplit e{dxp, c.np, c.dp, q > 0};
+                if (c.n <= 16) launch<typename P::X16>(d, e, s);
+                else launch<typename P::X64>(d, e, s);
             }
         }
         if (a.grad_weight) {
@@ -731,13 +876,18 @@ template <bool F32> int run_bwd(const m2_linear_cross_entropy_grad_args& a, cons
             d.b = Operand{G, p.piece, gplane, (int)p.piece, tiles(c.n, tok_tile(c.n)) * tok_tile(c.n)};
             d.tm = tiles(c.dim, 256);
             d.tn = tiles(rows, 256);
-            EpiDw<T> e{static_cast<T*>(a.grad_weight) + v0 * c.dim, c.dim, (int)rows,
-                       c.dim % 4 == 0 && al16(a.grad_weight)};
+            EpiDw<T> e{static_cast<T*>(a.grad_weight) + v0 * c.dim, c.dim, (int)rows};
             launch<typename P::W256>(d, e, s);
         }
     }
-    if (a.grad_x) {
-        DxArgs d{dxp, a.grad_x, c.n, c.np, c.dp, c.dim, p.splits, c.dim % 8 == 0 && al16(a.grad_x)};
+    if (a.grad_x && c.n > 64) {
+        typedef typename P::X256 S;
+        dxs.part = dxp; dxs.dx = a.grad_x; dxs.n = c.n; dxs.dim = c.dim;
+        dxs.nred = dxs.tm * dxs.tn * (S::NW * S::FM * S::FN / 2 / 4);
+        const int zero = tiles(c.n, 64);
+        hipLaunchKernelGGL((k_ce_dx_seg<T, S>), dim3((unsigned)(dxs.nred + zero)), dim3(256), 0, s, dxs, tk);
+    } else if (a.grad_x) {
+        DxArgs d{dxp, a.grad_x, c.n, c.np, c.dp, c.dim, p.splits};
         hipLaunchKernelGGL((k_ce_dx<T>), dim3((unsigned)((c.n + 3) / 4), (unsigned)((c.dim + 511) / 512)),
                            dim3(256), 0, s, d, tk);
     }

@@ -179,6 +179,16 @@ M2_DEV void lds_barrier() {
 
 typedef __attribute__((__vector_size__(4 * sizeof(uint32_t)))) uint32_t u32x4;
 
+// 16 bytes at an address that need be aligned as its 2- or 4-byte elements only (rows of an odd
+// number of elements): the memory pipeline takes any address, and a wavefront's
+// run of 1 KB touches one cache line more than an aligned one.
+typedef uint32_t u32x4_any __attribute__((ext_vector_type(4), aligned(2)));
+M2_DEV u32x4 load16(const void* p) {
+    const u32x4_any v = *reinterpret_cast<const u32x4_any*>(p);
+    return u32x4{v[0], v[1], v[2], v[3]};
+}
+M2_DEV void store16(void* p, u32x4 v) { *reinterpret_cast<u32x4_any*>(p) = u32x4_any{v[0], v[1], v[2], v[3]}; }
+
 typedef __attribute__((__vector_size__(4 * sizeof(__bf16)))) __bf16 bf16x4;
 typedef __attribute__((address_space(3))) bf16x4 lds_bf16x4;
 

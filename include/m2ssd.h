@@ -499,7 +499,14 @@ typedef struct {
     int32_t dtype, target_dtype, mean;
     void*   workspace;
     size_t  workspace_bytes;
+    void*   saved;                 /* out, or NULL                              */
+    size_t  saved_bytes;           /* >= m2_linear_cross_entropy_saved_size()   */
 } m2_linear_cross_entropy_args;
+/* With saved, the forward leaves the operands as its kernels read them there (the kept
+ * rows of x; the weights where they are not read in place: float32, rows that
+ * are not whole 128-byte pieces), and the gradient given the same buffer for
+ * the same arguments does not prepare them again.  0: nothing to save (up to 64 rows). */
+size_t m2_linear_cross_entropy_saved_size(const m2_linear_cross_entropy_args* a);
 size_t m2_linear_cross_entropy_workspace_size(const m2_linear_cross_entropy_args* a);
 int m2_linear_cross_entropy(const m2_linear_cross_entropy_args* a, void* stream);
 
@@ -526,6 +533,8 @@ typedef struct {
     int32_t dtype, target_dtype, mean;
     void*   workspace;
     size_t  workspace_bytes;
+    void*   saved;                 /* as the forward left it, or NULL           */
+    size_t  saved_bytes;
 } m2_linear_cross_entropy_grad_args;
 size_t m2_linear_cross_entropy_grad_workspace_size(const m2_linear_cross_entropy_grad_args* a);
 int m2_linear_cross_entropy_grad(const m2_linear_cross_entropy_grad_args* a, void* stream);

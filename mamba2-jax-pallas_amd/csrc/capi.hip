@@ -91,6 +91,9 @@ extern "C" size_t m2_embedding_grad_workspace_size(const m2_embedding_grad_args*
 extern "C" size_t m2_linear_cross_entropy_workspace_size(const m2_linear_cross_entropy_args* a) {
     return a ? m2::linear_ce_workspace(*a) : 0;
 }
+extern "C" size_t m2_linear_cross_entropy_saved_size(const m2_linear_cross_entropy_args* a) {
+    return a ? m2::linear_ce_saved(*a) : 0;
+}
 extern "C" size_t m2_linear_cross_entropy_grad_workspace_size(
     const m2_linear_cross_entropy_grad_args* a) {
     return a ? m2::linear_ce_grad_workspace(*a) : 0;

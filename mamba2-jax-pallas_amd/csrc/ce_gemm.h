@@ -34,8 +34,8 @@ struct Operand {
 
 struct Gemm {
     Operand a, b;
-    const void* zeros;   // 16 zero bytes
-    const int* count;    // kept tokens (device)
+    const int* count;    // tokens that take part (device), or NULL: n
+    int n;
     int nk;              // K steps of 64 (per plane product), 0: from count
     int tm, tn;
     int tok_n;           // n is the token: tiles past the kept ones are left out
@@ -64,6 +64,8 @@ __host__ __device__ inline Deal deal(int tiles, int nk, int nwg) {
     }
     return d;
 }
+
+__device__ const uint32_t ZEROS[4] = {0, 0, 0, 0};      // what stands past a row's end
 
 // ---------------------------------------------------------------------------
 // global -> LDS: R rows (columns) of BK of K
@@ -124,7 +126,7 @@ template <int R, bool TR, int NW, int BK> struct Loader {
         }
     }
     // a whole step; a row operand's pieces past klim read zeros
-    M2_DEV void issue(const Operand& o, const void* zeros, int kt, int pl, uint32_t lds, int w, int lane) const {
+    M2_DEV void issue(const Operand& o, int kt, int pl, uint32_t lds, int w, int lane) const {
         const bf16* b = base(o, kt, pl);
         if (TR || kt * BK + BK <= o.klim) {
 #pragma unroll
@@ -134,7 +136,8 @@ template <int R, bool TR, int NW, int BK> struct Loader {
             for (int j = 0; j < J; ++j) {
                 const int in = (w * J + j) % INSTR;
                 const int c = (lane & (PP - 1)) ^ swz<BK>(in * (64 / PP) + lane / PP);
-                dma16(kt * BK + c * 8 < o.klim ? reinterpret_cast<const char*>(b) + off[j] : zeros, lds + in * 1024);
+                dma16(kt * BK + c * 8 < o.klim ? reinterpret_cast<const char*>(b) + off[j]
+                                               : reinterpret_cast<const char*>(ZEROS), lds + in * 1024);
             }
         }
     }
@@ -201,7 +204,7 @@ __global__ void __launch_bounds__(S::NT, 2 * S::LDS <= 160 * 1024 ? 2 : 1) k_ce_
     const int tm = grp * 8 + in % gm, tn = in / gm;
     const int m0 = tm * S::BM, n0 = tn * S::BN;
 
-    const int count = *g.count;
+    const int count = g.count ? *g.count : g.n;
     if (g.tok_n && n0 >= ((count + 63) & ~63)) return;
     const int nk = g.nk ? g.nk : (count + 63) >> 6;
     const int k0 = (int)((int64_t)nk * split / g.splits), k1 = (int)((int64_t)nk * (split + 1) / g.splits);
@@ -215,8 +218,8 @@ __global__ void __launch_bounds__(S::NT, 2 * S::LDS <= 160 * 1024 ? 2 : 1) k_ce_
     int ikt = k0, iterm = 0, islot = 0;
     auto issue = [&]() {
         const uint32_t l = lds0 + islot * S::SLOT;
-        la.issue(g.a, g.zeros, ikt, plane_a<S::TERMS>(iterm), l, w, lane);
-        lb.issue(g.b, g.zeros, ikt, plane_b<S::TERMS>(iterm), l + S::LA::BYTES, w, lane);
+        la.issue(g.a, ikt, plane_a<S::TERMS>(iterm), l, w, lane);
+        lb.issue(g.b, ikt, plane_b<S::TERMS>(iterm), l + S::LA::BYTES, w, lane);
         if (++ikt == k1) { ikt = k0; ++iterm; }
         if (++islot == S::ST) islot = 0;
     };
@@ -257,7 +260,7 @@ __global__ void __launch_bounds__(S::NT, 2 * S::LDS <= 160 * 1024 ? 2 : 1) k_ce_
         }
         if (++slot == S::ST) slot = 0;
     }
-    epi.template run<S>(acc, m0, n0, wm, wn, lane, count, split, tm);
+    epi.template run<S>(acc, smem, m0, n0, wm, wn, lane, count, split, tm);
 }
 
 // Many tokens: persistent workgroups (whole tiles, or with EPI::SEG segments of them), each XCD with a contiguous range of the tiles
@@ -287,7 +290,7 @@ __global__ void __launch_bounds__(S::NT, S::NT / 256) k_ce_tile(Gemm g, EPI epi)
     __shared__ __align__(1024) char smem[B_AT + 2 * S::LB::BYTES];
     const int lane = threadIdx.x & 63, w = wave_id();
     const int wm = w / S::WN, wn = w % S::WN;
-    const int count = *g.count;
+    const int count = g.count ? *g.count : g.n;
     const int tn_all = g.tok_n ? min(g.tn, (((count + 63) & ~63) + S::BN - 1) / S::BN) : g.tn;
     const int tiles = g.tm * tn_all;
     const int nk = g.nk ? g.nk : (count + 63) >> 6;
@@ -362,8 +365,8 @@ __global__ void __launch_bounds__(S::NT, S::NT / 256) k_ce_tile(Gemm g, EPI epi)
         start(cb, g.b, false, work(first));
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-            ca.ld.issue(g.a, g.zeros, ca.k, plane_a<S::TERMS>(ca.term), lds0 + i * S::LA::BYTES, w, lane);
-            cb.ld.issue(g.b, g.zeros, cb.k, plane_b<S::TERMS>(cb.term), lds0 + B_AT + i * S::LB::BYTES, w, lane);
+            ca.ld.issue(g.a, ca.k, plane_a<S::TERMS>(ca.term), lds0 + i * S::LA::BYTES, w, lane);
+            cb.ld.issue(g.b, cb.k, plane_b<S::TERMS>(cb.term), lds0 + B_AT + i * S::LB::BYTES, w, lane);
             next(ca, g.a, true);
             next(cb, g.b, false);
         }
@@ -437,7 +440,7 @@ __global__ void __launch_bounds__(S::NT, S::NT / 256) k_ce_tile(Gemm g, EPI epi)
         }
         // what is loaded so far (step 0 and 1 of the next tile) is there before any store
         wait_vmem<0>();
-        epi.template run<S>(acc, m0, n0, wm, wn, lane, count, wk.seg, tm);
+        epi.template run<S>(acc, nullptr, m0, n0, wm, wn, lane, count, wk.seg, tm);
     }
     wait_vmem<0>();           // no load may land after the workgroup has ended
 }

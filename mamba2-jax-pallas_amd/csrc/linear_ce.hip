@@ -39,8 +39,12 @@ struct Tokens {              // in the workspace
     float* lse;              // [np] (backward, as the two below)
     float* gf;               // [np] upstream gradient
     float* gm;               // [np] G at the target
-    int* count;              // [1]; the 16 zero bytes of the padding lie behind it
+    int* count;              // [1]
 };
+
+M2_DEV int64_t load_target(const void* targets, int t64, int64_t i) {
+    return t64 ? reinterpret_cast<const int64_t*>(targets)[i] : (int64_t) reinterpret_cast<const int32_t*>(targets)[i];
+}
 
 // ---------------------------------------------------------------------------
 // which rows are kept, in order
@@ -59,9 +63,7 @@ __global__ void __launch_bounds__(1024) k_ce_compact(const void* targets, int64_
             const int64_t i = i0 + (int64_t)t * E + e;
             keep[e] = false;
             if (i < n) {
-                const int64_t v = t64 ? reinterpret_cast<const int64_t*>(targets)[i]
-                                      : (int64_t) reinterpret_cast<const int32_t*>(targets)[i];
-                keep[e] = v != ignore;
+                keep[e] = load_target(targets, t64, i) != ignore;
             }
             mine += keep[e];
         }
@@ -89,7 +91,7 @@ __global__ void __launch_bounds__(1024) k_ce_compact(const void* targets, int64_
             if (keep[e]) tk.idx[at++] = (int)i;
         }
     }
-    if (t < 32) tk.count[t] = t == 0 ? base : 0;
+    if (t == 0) *tk.count = base;
 }
 
 // 8 consecutive elements of a row, zero past its end
@@ -140,39 +142,67 @@ struct PackArgs {
     const float* lse;
     const float* loss;
     const float* g;
-    int64_t gstride, vocab;
+    int64_t gstride, vocab, n, ignore;
     int t64, mean;
 };
 
+// what the epilogues of the backward need of kept token r, row `from` of the inputs (-1: none)
+M2_DEV void token_grads(const PackArgs& a, const Tokens& tk, int64_t r, int64_t from, int tgt, int count) {
+    float gf = 0.f, gm = 0.f, lse = 0.f;
+    if (from >= 0) {
+        gf = a.g[from * a.gstride] * (a.mean ? 1.f / (float)count : 1.f);
+        lse = a.lse[from];
+        const float l = a.loss[from];
+        gm = gf * expm1f(-l);
+        if (tgt < 0) gf = l;                 // NaN: the row's gradients are too
+    }
+    tk.lse[r] = lse;
+    tk.gf[r] = gf;
+    tk.gm[r] = gm;
+}
+// the same where the forward left the packed operands
+__global__ void __launch_bounds__(256) k_ce_tokens(PackArgs a, Tokens tk) {
+    const int64_t r = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    const int count = *tk.count;
+    if (r < ((count + 63) & ~63)) token_grads(a, tk, r, r < count ? tk.idx[r] : -1, tk.tgt[r], count);
+}
+
 // Rows of src as bf16 (planes) with rows of dp elements, zeros behind dim: the weights
 // where they cannot be read in place, or the kept rows of x (TOK), with zero rows up to
-// the next whole K step, and what the epilogues need of each token.
+// the next whole K step, and what the epilogues need of each token.  Up to 64 tokens
+// every wavefront finds the kept ones by itself (k_ce_compact does for more).
 template <typename T, bool TOK>
 __global__ void __launch_bounds__(256) k_ce_pack(PackArgs a, Tokens tk) {
     const int64_t r = (int64_t)blockIdx.x * 4 + wave_id();
     const int lane = threadIdx.x & 63;
     int64_t from = r;
     if constexpr (TOK) {
-        const int count = *tk.count;
+        int count;
+        if (a.n <= 64) {
+            const bool keep = lane < a.n && load_target(a.targets, a.t64, lane) != a.ignore;
+            const uint64_t all = __ballot(keep);
+            const int at = __popcll(all & ((1ull << lane) - 1));
+            const uint64_t mine = __ballot(keep && at == r);
+            from = mine ? __ffsll((unsigned long long)mine) - 1 : -1;
+            count = __popcll(all);
+            if (r == 0) {
+                if (lane < a.n) tk.inv[lane] = keep ? at : -1;
+                if (keep) tk.idx[at] = lane;
+                if (lane == 0) *tk.count = count;
+            }
+        } else {
+            count = *tk.count;
+            from = r < count ? tk.idx[r] : -1;
+        }
         if (r >= ((count + 63) & ~63)) return;
-        from = r < count ? tk.idx[r] : -1;
         if (lane == 0) {
             int tg = -1;
-            float gf = 0.f, gm = 0.f, lse = 0.f;
             if (from >= 0) {
-                const int64_t v = a.t64 ? reinterpret_cast<const int64_t*>(a.targets)[from]
-                                        : (int64_t) reinterpret_cast<const int32_t*>(a.targets)[from];
+                const int64_t v = load_target(a.targets, a.t64, from);
                 tg = v >= 0 && v < a.vocab ? (int)v : -1;
-                if (a.g) {
-                    gf = a.g[from * a.gstride] * (a.mean ? 1.f / (float)count : 1.f);
-                    lse = a.lse[from];
-                    const float l = a.loss[from];
-                    gm = gf * expm1f(-l);
-                    if (tg < 0) gf = l;                 // NaN: the row's gradients are too
-                }
             }
             tk.tgt[r] = tg;
-            if (a.g) { tk.lse[r] = lse; tk.gf[r] = gf; tk.gm[r] = gm; }
+            if (a.g) token_grads(a, tk, r, from, tg, count);
             else tk.zt[r] = __builtin_nanf("");
         }
     } else {
@@ -196,18 +226,41 @@ __global__ void __launch_bounds__(256) k_ce_pack(PackArgs a, Tokens tk) {
 // epilogues.  A lane holds, of each 16x16 block, one n (lane & 15) and 4 consecutive
 // m (4 (lane >> 4) ..).
 // ---------------------------------------------------------------------------
-// m: vocabulary, n: token -> per token (max, sum of exp(z - max)) without the target of the
-// BM / WM rows of the vocabulary that a row of wavefronts holds
+// a running maximum and the sum of exp(z - maximum)
+struct LogSum {
+    float mx = -__builtin_inff(), s = 0.f;
+    M2_DEV void add(float2 u) {
+        const float m = fmaxf(mx, u.x), b = m == -__builtin_inff() ? 0.f : m;
+        s = s * __builtin_amdgcn_exp2f((mx - b) * LOG2E) + u.y * __builtin_amdgcn_exp2f((u.x - b) * LOG2E);
+        mx = m;
+    }
+    // exp(loss) = 1 + the others' sum over exp(z_t)
+    M2_DEV float loss(float zt) const {
+        const float d = mx - zt, e = __builtin_amdgcn_exp2f(-fabsf(d) * LOG2E);
+        return d <= 0.f ? log1pf(s * e) : d + logf(s + e);
+    }
+};
+// m: vocabulary, n: token -> per token (max, sum of exp(z - max)) without the target: of a tile
+// (k_ce_stream), or of the BM / WM rows of the vocabulary that a row of wavefronts holds
+// (k_ce_tile, whose LDS is full)
 struct EpiLse {
     static constexpr bool SEG = false;
-    const int* tgt;
+    const int* tgt;          // of the kept tokens, or NULL: the caller's targets
+    const void* targets;
+    int64_t ignore;
     float* zt;
-    float2* part;        // [tm * WM][np]
+    float2* part;            // [parts][np]
     int64_t np;
-    int vocab;
+    int vocab, t64;
+
+    M2_DEV int target(int n) const {
+        if (tgt) return tgt[n];
+        const int64_t v = load_target(targets, t64, n);
+        return v >= 0 && v < vocab && v != ignore ? (int)v : -1;
+    }
 
     template <class S>
-    M2_DEV void run(f32x4 (&acc)[S::FM][S::FN], int m0, int n0, int wm, int wn, int lane, int count, int, int tm) const {
+    M2_DEV void run(f32x4 (&acc)[S::FM][S::FN], char* smem, int m0, int n0, int wm, int wn, int lane, int count, int, int tm) const {
         const int v0 = m0 + wm * S::FM * 16 + 4 * (lane >> 4);
         const float ninf = -__builtin_inff();
         if (m0 + S::BM > vocab) {
@@ -224,7 +277,7 @@ struct EpiLse {
             const int n = n0 + (wn * S::FN + j) * 16 + (lane & 15);
             // the target's place among this lane's values, if it is there (few wavefronts
             // have one: the others pay for one comparison)
-            const int d = n < count ? tgt[n] - v0 : -1;
+            const int d = n < count ? target(n) - v0 : -1;
             if (__ballot(d >= 0 && d < 16 * S::FM && (d & 12) == 0)) {
 #pragma unroll
                 for (int i = 0; i < S::FM; ++i)
@@ -250,7 +303,21 @@ struct EpiLse {
                 for (int r = 0; r < 4; ++r) s += __builtin_amdgcn_exp2f(fmaf(acc[i][j][r], LOG2E, b));
             s += __shfl_xor(s, 16);
             s += __shfl_xor(s, 32);
-            if (lane < 16 && n < count) part[((int64_t)tm * S::WM + wm) * np + n] = make_float2(mx, s);
+            if constexpr (S::BN < 128) {
+                if (lane < 16) reinterpret_cast<float2*>(smem)[wm * S::BN + n - n0] = make_float2(mx, s);
+            } else {
+                if (lane < 16 && n < count) part[((int64_t)tm * S::WM + wm) * np + n] = make_float2(mx, s);
+            }
+        }
+        if constexpr (S::BN < 128) {
+            __syncthreads();
+            const int t = threadIdx.x;
+            if (t < S::BN && n0 + t < count) {
+                LogSum o = {};
+#pragma unroll
+                for (int q = 0; q < S::WM; ++q) o.add(reinterpret_cast<const float2*>(smem)[q * S::BN + t]);
+                part[(int64_t)tm * np + n0 + t] = make_float2(o.mx, o.s);
+            }
         }
     }
 };
@@ -316,7 +383,7 @@ struct EpiG {
     int v_first, vocab;      // of the piece; of all
 
     template <class S>
-    M2_DEV void run(f32x4 (&acc)[S::FM][S::FN], int m0, int n0, int wm, int wn, int lane, int count, int, int) const {
+    M2_DEV void run(f32x4 (&acc)[S::FM][S::FN], char* smem, int m0, int n0, int wm, int wn, int lane, int count, int, int) const {
         static_assert(S::FM % 2 == 0, "");
         const int mw = m0 + wm * S::FM * 16, mv = mw + 4 * (lane >> 4);
         const int lim = (count + 63) & ~63;
@@ -388,7 +455,7 @@ struct EpiDxSplit {
     int add;
 
     template <class S>
-    M2_DEV void run(f32x4 (&acc)[S::FM][S::FN], int m0, int n0, int wm, int wn, int lane, int count, int split,
+    M2_DEV void run(f32x4 (&acc)[S::FM][S::FN], char* smem, int m0, int n0, int wm, int wn, int lane, int count, int split,
                     int) const {
         const int mv = m0 + wm * S::FM * 16 + 4 * (lane >> 4);
 #pragma unroll
@@ -414,7 +481,7 @@ struct EpiDxSeg {
     int add;
 
     template <class S>
-    M2_DEV void run(f32x4 (&acc)[S::FM][S::FN], int, int, int wm, int wn, int lane, int, int seg, int) const {
+    M2_DEV void run(f32x4 (&acc)[S::FM][S::FN], char* smem, int, int, int wm, int wn, int lane, int, int seg, int) const {
         f32x4* d = reinterpret_cast<f32x4*>(part) +
                    ((int64_t)seg * S::NW + wm * S::WN + wn) * S::FM * S::FN * 64 + lane;
         if (add) {
@@ -438,7 +505,7 @@ template <typename T> struct EpiDw {
     int rows;                // rows of the piece
 
     template <class S>
-    M2_DEV void run(f32x4 (&acc)[S::FM][S::FN], int m0, int n0, int wm, int wn, int lane, int, int, int) const {
+    M2_DEV void run(f32x4 (&acc)[S::FM][S::FN], char* smem, int m0, int n0, int wm, int wn, int lane, int, int, int) const {
 #pragma unroll
         for (int j = 0; j < S::FN; ++j) {
             const int n = n0 + (wn * S::FN + j) * 16 + (lane & 15);
@@ -458,45 +525,76 @@ struct JoinArgs {
     int64_t np, n;
     float* loss;
     float* lse;
-    int tiles;
+    int parts;
 };
 
-// 16 tokens per workgroup, 16 lanes each: lane q joins tiles q, q + 16, ...
+// 16 tokens per workgroup, 16 lanes each: lane q joins parts q, q + 16, ...
 __global__ void __launch_bounds__(256) k_ce_join(JoinArgs a, Tokens tk) {
     __shared__ float2 red[16][17];
     const int tok = threadIdx.x & 15, q = threadIdx.x >> 4;
     const int64_t n = (int64_t)blockIdx.x * 16 + tok;
     const int k = n < a.n ? tk.inv[n] : -1;
-    float mx = -__builtin_inff(), s = 0.f;
+    LogSum o;
     if (k >= 0) {
 #pragma unroll 4
-        for (int i = q; i < a.tiles; i += 16) {
-            const float2 u = a.part[(int64_t)i * a.np + k];
-            const float m = fmaxf(mx, u.x), b = m == -__builtin_inff() ? 0.f : m;
-            s = s * __builtin_amdgcn_exp2f((mx - b) * LOG2E) + u.y * __builtin_amdgcn_exp2f((u.x - b) * LOG2E);
-            mx = m;
-        }
+        for (int i = q; i < a.parts; i += 16) o.add(a.part[(int64_t)i * a.np + k]);
     }
-    red[q][tok] = make_float2(mx, s);
+    red[q][tok] = make_float2(o.mx, o.s);
     __syncthreads();
     if (q == 0 && n < a.n) {
         float loss = 0.f, lse = 0.f;
         if (k >= 0) {
-            for (int i = 1; i < 16; ++i) {
-                const float2 u = red[i][tok];
-                const float m = fmaxf(mx, u.x), b = m == -__builtin_inff() ? 0.f : m;
-                s = s * __builtin_amdgcn_exp2f((mx - b) * LOG2E) + u.y * __builtin_amdgcn_exp2f((u.x - b) * LOG2E);
-                mx = m;
-            }
-            // exp(loss) = 1 + the others' sum over exp(z_t)
-            const float zt = tk.zt[k], d = mx - zt;
-            const float e = __builtin_amdgcn_exp2f(-fabsf(d) * LOG2E);
-            loss = d <= 0.f ? log1pf(s * e) : d + logf(s + e);
+            for (int i = 1; i < 16; ++i) o.add(red[i][tok]);
+            const float zt = tk.zt[k];
+            loss = o.loss(zt);
             lse = zt + loss;
         }
         a.loss[n] = loss;
         a.lse[n] = lse;
     }
+}
+
+// Up to 64 tokens, none of them dropped before the product: one workgroup, 16 to 64 lanes a
+// token, which also adds the losses up
+__global__ void __launch_bounds__(1024) k_ce_join_few(JoinArgs a, EpiLse e, float* total, int mean) {
+    __shared__ float2 red[1024];
+    const int w = a.n <= 16 ? 16 : a.n <= 32 ? 32 : 64;
+    const int t = threadIdx.x, tok = t & (w - 1), q = t / w, lanes = 1024 / w;
+    LogSum o;
+    if (tok < a.n) {
+#pragma unroll 4
+        for (int i = q; i < a.parts; i += lanes) o.add(a.part[(int64_t)i * a.np + tok]);
+    }
+    red[t] = make_float2(o.mx, o.s);
+    __syncthreads();
+    // 4 lanes of the first wavefronts join the lanes' sums, the first of them the four
+    if (q < 4) {
+        o = LogSum();
+        for (int i = q; i < lanes; i += 4) o.add(red[i * w + tok]);
+    }
+    __syncthreads();
+    if (q < 4) red[t] = make_float2(o.mx, o.s);
+    __syncthreads();
+    if (t >= 64) return;
+    float loss = 0.f, lse = 0.f;
+    bool kept = false;
+    if (t < a.n) {              // q == 0
+        for (int i = 1; i < 4; ++i) o.add(red[i * w + tok]);
+        kept = load_target(e.targets, e.t64, t) != e.ignore;
+        if (kept) {
+            const float zt = e.target(t) >= 0 ? e.zt[t] : __builtin_nanf("");
+            loss = o.loss(zt);
+            lse = zt + loss;
+        }
+        a.loss[t] = loss;
+        a.lse[t] = lse;
+    }
+    if (!total) return;
+    double s = loss;
+#pragma unroll
+    for (int k = 32; k >= 1; k >>= 1) s += __shfl_xor(s, k);
+    const int count = __popcll(__ballot(kept));
+    if (t == 0) *total = (float)(s / (mean ? max(count, 1) : 1));
 }
 
 // the losses' sum or mean, in a fixed order, in float64
@@ -627,7 +725,7 @@ Common common(int64_t n, int64_t vocab, int64_t dim, int64_t ldw, const void* w,
     c.idx = take(4 * (size_t)c.np);
     c.inv = take(4 * (size_t)c.np);
     c.tgt = take(4 * (size_t)c.np);
-    c.count = take(256);
+    c.count = take(4);
     const size_t planes = c.f32 ? 3 : 1;
     c.x = take(2 * planes * (size_t)c.np * c.dp);
     c.w = c.pack_w ? take(2 * planes * (size_t)vocab * c.dp) : c.at;
@@ -660,8 +758,8 @@ template <bool F32> struct Shapes {
 // tokens of a tile
 int tok_tile(int64_t n) { return n <= 16 ? 16 : n <= 64 ? 64 : 256; }
 int voc_tile(int64_t n) { return n <= 64 ? 128 : 256; }
-// rows of the vocabulary whose sums EpiLse leaves together
-int voc_part(int64_t n) { return n <= 64 ? 32 : 128; }
+// parts of a tile whose sums EpiLse leaves apart
+int tile_parts(int64_t n) { return n <= 64 ? 1 : 2; }
 
 template <bool F32, class EPI> void launch_z(Gemm& g, int64_t rows, int64_t n, const EPI& e, hipStream_t s) {
     typedef Shapes<F32> P;
@@ -690,15 +788,18 @@ int check_sizes(const char* who, int64_t n, int64_t vocab, int64_t dim, int64_t 
 
 struct FwdPlan {
     Common c;
+    bool direct;             // x read in place, nothing packed: few tokens
     size_t zt, part, total;
 };
 FwdPlan fwd_plan(const m2_linear_cross_entropy_args& a) {
     FwdPlan p{};
     p.c = common(a.n, a.vocab, a.dim, a.ldw, a.weight, a.dtype);
-    auto take = [&](size_t b) { const size_t r = p.c.at; p.c.at += align256(b); return r; };
+    p.direct = a.n <= 64 && !p.c.pack_w && a.ldx % 8 == 0 && al16(a.x);
+    size_t at = p.direct || a.saved ? 0 : p.c.at;
+    auto take = [&](size_t b) { const size_t r = at; at += align256(b); return r; };
     p.zt = take(4 * (size_t)p.c.np);
-    p.part = take(8 * (size_t)(voc_tile(a.n) / voc_part(a.n)) * tiles(a.vocab, voc_tile(a.n)) * p.c.np);
-    p.total = p.c.at;
+    p.part = take(8 * (size_t)tile_parts(a.n) * tiles(a.vocab, voc_tile(a.n)) * p.c.np);
+    p.total = at ? at : 256;
     return p;
 }
 
@@ -714,7 +815,8 @@ struct BwdPlan {
 BwdPlan bwd_plan(const m2_linear_cross_entropy_grad_args& a) {
     BwdPlan p{};
     p.c = common(a.n, a.vocab, a.dim, a.ldw, a.weight, a.dtype);
-    auto take = [&](size_t b) { const size_t r = p.c.at; p.c.at += align256(b); return r; };
+    size_t at = a.saved ? 0 : p.c.at;
+    auto take = [&](size_t b) { const size_t r = at; at += align256(b); return r; };
     p.lse = take(4 * (size_t)p.c.np);
     p.gf = take(4 * (size_t)p.c.np);
     p.gm = take(4 * (size_t)p.c.np);
@@ -742,7 +844,7 @@ BwdPlan bwd_plan(const m2_linear_cross_entropy_grad_args& a) {
             if (c > segs) segs = c;
         }
         p.dx = a.grad_x ? take(4 * 256 * 256 * (size_t)segs) : 0;
-        p.total = p.c.at;
+        p.total = at;
         return p;
     }
     double best = 1e300;
@@ -753,7 +855,7 @@ BwdPlan bwd_plan(const m2_linear_cross_entropy_grad_args& a) {
         if (cost < best) { best = cost; p.splits = s; }
     }
     p.dx = a.grad_x ? take(4 * (size_t)p.splits * p.c.np * p.c.dp) : 0;
-    p.total = p.c.at;
+    p.total = at;
     return p;
 }
 
@@ -769,7 +871,8 @@ Tokens tokens(char* ws, const Common& c) {
 template <typename T>
 void pack(char* ws, const Common& c, const void* x, int64_t ldx, const void* w, int64_t ldw, PackArgs a,
           const Tokens& tk, int64_t ignore, hipStream_t s) {
-    hipLaunchKernelGGL(k_ce_compact, dim3(1), dim3(1024), 0, s, a.targets, c.n, ignore, a.t64, tk);
+    a.n = c.n; a.ignore = ignore;
+    if (c.n > 64) hipLaunchKernelGGL(k_ce_compact, dim3(1), dim3(1024), 0, s, a.targets, c.n, ignore, a.t64, tk);
     a.dim = c.dim; a.dp = c.dp;
     a.src = x; a.ld = ldx; a.dst = reinterpret_cast<bf16*>(ws + c.x); a.rows = c.np; a.plane = c.np * c.dp;
     hipLaunchKernelGGL((k_ce_pack<T, true>), dim3((unsigned)(c.np / 4)), dim3(256), 0, s, a, tk);
@@ -788,22 +891,37 @@ Operand operand_w(char* ws, const Common& c, const void* w, int64_t ldw) {
 template <bool F32> int run_fwd(const m2_linear_cross_entropy_args& a, const FwdPlan& p, hipStream_t s) {
     typedef typename std::conditional<F32, float, bf16>::type T;
     char* ws = static_cast<char*>(a.workspace);
+    char* cm = a.saved ? static_cast<char*>(a.saved) : ws;
     const Common& c = p.c;
-    Tokens tk = tokens(ws, c);
-    tk.zt = reinterpret_cast<float*>(ws + p.zt);
-    PackArgs pa{};
-    pa.targets = a.targets; pa.vocab = a.vocab; pa.t64 = a.target_dtype == M2_I64;
-    pack<T>(ws, c, a.x, a.ldx, a.weight, a.ldw, pa, tk, a.ignore_index, s);
+    const int t64 = a.target_dtype == M2_I64;
+    float* zt = reinterpret_cast<float*>(ws + p.zt);
+    EpiLse e{nullptr, a.targets, a.ignore_index, zt, reinterpret_cast<float2*>(ws + p.part), c.np, (int)c.vocab, t64};
     Gemm g{};
-    g.zeros = tk.count + 16; g.count = tk.count; g.splits = 1; g.tok_n = 1;
+    g.tok_n = 1; g.splits = 1;
     g.nk = (int)(c.dp / 64);
-    g.a = operand_w(ws, c, a.weight, a.ldw);
+    JoinArgs j{e.part, c.np, c.n, a.loss, a.lse, 0};
+    if (p.direct) {
+        g.n = (int)c.n;
+        g.a = Operand{static_cast<const bf16*>(a.weight), a.ldw, 0, (int)c.vocab, (int)c.dim};
+        g.b = Operand{static_cast<const bf16*>(a.x), a.ldx, 0, (int)c.n, (int)c.dim};
+        launch_z<F32>(g, c.vocab, c.n, e, s);
+        j.parts = g.tm;
+        hipLaunchKernelGGL(k_ce_join_few, dim3(1), dim3(1024), 0, s, j, e, a.total, a.mean);
+        return m2::check_launch("linear_cross_entropy");
+    }
+    Tokens tk = tokens(cm, c);
+    tk.zt = zt;
+    PackArgs pa{};
+    pa.targets = a.targets; pa.vocab = a.vocab; pa.t64 = t64;
+    pack<T>(cm, c, a.x, a.ldx, a.weight, a.ldw, pa, tk, a.ignore_index, s);
+    g.count = tk.count;
+    g.a = operand_w(cm, c, a.weight, a.ldw);
     g.a.lim = (int)c.vocab;
     g.a.klim = (int)(c.pack_w ? c.dp : c.dim);
-    g.b = Operand{reinterpret_cast<bf16*>(ws + c.x), c.dp, c.np * c.dp, (int)c.np, (int)c.dp};
-    EpiLse e{tk.tgt, tk.zt, reinterpret_cast<float2*>(ws + p.part), c.np, (int)c.vocab};
+    g.b = Operand{reinterpret_cast<bf16*>(cm + c.x), c.dp, c.np * c.dp, (int)c.np, (int)c.dp};
+    e.tgt = tk.tgt;
     launch_z<F32>(g, c.vocab, c.n, e, s);
-    JoinArgs j{e.part, c.np, c.n, a.loss, a.lse, g.tm * (voc_tile(c.n) / voc_part(c.n))};
+    j.parts = g.tm * tile_parts(c.n);
     hipLaunchKernelGGL(k_ce_join, dim3((unsigned)((c.n + 15) / 16)), dim3(256), 0, s, j, tk);
     if (a.total)
         hipLaunchKernelGGL(k_ce_total, dim3(1), dim3(1024), 0, s, a.loss, c.n, a.total, a.mean, tk.count);
@@ -814,20 +932,22 @@ template <bool F32> int run_bwd(const m2_linear_cross_entropy_grad_args& a, cons
     typedef typename std::conditional<F32, float, bf16>::type T;
     typedef Shapes<F32> P;
     char* ws = static_cast<char*>(a.workspace);
+    char* cm = a.saved ? static_cast<char*>(a.saved) : ws;
     const Common& c = p.c;
-    Tokens tk = tokens(ws, c);
+    Tokens tk = tokens(cm, c);
     tk.lse = reinterpret_cast<float*>(ws + p.lse);
     tk.gf = reinterpret_cast<float*>(ws + p.gf);
     tk.gm = reinterpret_cast<float*>(ws + p.gm);
     PackArgs pa{};
     pa.targets = a.targets; pa.vocab = a.vocab; pa.t64 = a.target_dtype == M2_I64;
     pa.lse = a.lse; pa.loss = a.loss; pa.g = a.grad_loss; pa.gstride = a.grad_loss_stride; pa.mean = a.mean;
-    pack<T>(ws, c, a.x, a.ldx, a.weight, a.ldw, pa, tk, a.ignore_index, s);
-    const Operand w = operand_w(ws, c, a.weight, a.ldw);
+    if (a.saved) hipLaunchKernelGGL(k_ce_tokens, dim3((unsigned)((c.np + 255) / 256)), dim3(256), 0, s, pa, tk);
+    else pack<T>(cm, c, a.x, a.ldx, a.weight, a.ldw, pa, tk, a.ignore_index, s);
+    const Operand w = operand_w(cm, c, a.weight, a.ldw);
     bf16* G = reinterpret_cast<bf16*>(ws + p.G);
     const int64_t gplane = c.np * p.piece;
     Gemm g0{};
-    g0.zeros = tk.count + 16; g0.count = tk.count; g0.splits = 1;
+    g0.count = tk.count; g0.splits = 1;
     float* dxp = reinterpret_cast<float*>(ws + p.dx);
     const int wlim = (int)(c.pack_w ? c.dp : c.dim);
     DxSegArgs dxs{};
@@ -841,7 +961,7 @@ template <bool F32> int run_bwd(const m2_linear_cross_entropy_grad_args& a, cons
         g.a.p += v0 * w.ld;
         g.a.lim = (int)rows;
         g.a.klim = wlim;
-        g.b = Operand{reinterpret_cast<bf16*>(ws + c.x), c.dp, c.np * c.dp, (int)c.np, (int)c.dp};
+        g.b = Operand{reinterpret_cast<bf16*>(cm + c.x), c.dp, c.np * c.dp, (int)c.np, (int)c.dp};
         EpiG eg{tk.tgt, tk.lse, tk.gf, tk.gm, G, p.piece, gplane, (int)v0, (int)c.vocab};
         launch_z<F32>(g, (rows + 63) / 64 * 64, c.n, eg, s);
         if (a.grad_x) {
@@ -870,7 +990,7 @@ template <bool F32> int run_bwd(const m2_linear_cross_entropy_grad_args& a, cons
         if (a.grad_weight) {
             Gemm d = g0;
             d.nk = 0;
-            d.a = Operand{reinterpret_cast<bf16*>(ws + c.x), c.dp, c.np * c.dp, (int)c.dp, (int)c.np};
+            d.a = Operand{reinterpret_cast<bf16*>(cm + c.x), c.dp, c.np * c.dp, (int)c.dp, (int)c.np};
             // rows of G past the last token tile are not there: its last row stands for
             // them, against zero rows of x
             d.b = Operand{G, p.piece, gplane, (int)p.piece, tiles(c.n, tok_tile(c.n)) * tok_tile(c.n)};
@@ -898,6 +1018,11 @@ template <bool F32> int run_bwd(const m2_linear_cross_entropy_grad_args& a, cons
 
 namespace m2 {
 
+size_t linear_ce_saved(const m2_linear_cross_entropy_args& a) {
+    if (check_sizes("linear_cross_entropy", a.n, a.vocab, a.dim, a.ldx, a.ldw, a.dtype, a.target_dtype)) return 0;
+    return a.n <= 64 ? 0 : common(a.n, a.vocab, a.dim, a.ldw, a.weight, a.dtype).at;
+}
+
 size_t linear_ce_workspace(const m2_linear_cross_entropy_args& a) {
     if (check_sizes("linear_cross_entropy", a.n, a.vocab, a.dim, a.ldx, a.ldw, a.dtype, a.target_dtype)) return 0;
     return fwd_plan(a).total;
@@ -911,11 +1036,11 @@ int launch_linear_ce(const m2_linear_cross_entropy_args& a, hipStream_t s) {
     const FwdPlan p = fwd_plan(a);
     M2_REQUIRE(a.workspace && a.workspace_bytes >= p.total, M2_ERR_WORKSPACE,
                "%s: workspace of %zu bytes needed, %zu given", who, p.total, a.workspace_bytes);
+    M2_REQUIRE(!a.saved || (a.n > 64 && a.saved_bytes >= p.c.at), M2_ERR_WORKSPACE,
+               "%s: saved of %zu bytes needed (none for up to 64 rows), %zu given", who, a.n > 64 ? p.c.at : 0,
+               a.saved_bytes);
     if (a.n == 0) {
-        if (!a.total) return M2_OK;
-        Tokens tk = tokens(static_cast<char*>(a.workspace), p.c);
-        hipLaunchKernelGGL(k_ce_compact, dim3(1), dim3(1024), 0, s, a.targets, (int64_t)0, a.ignore_index, 0, tk);
-        hipLaunchKernelGGL(k_ce_total, dim3(1), dim3(1024), 0, s, a.loss, (int64_t)0, a.total, a.mean, tk.count);
+        if (a.total) hipLaunchKernelGGL(k_ce_total, dim3(1), dim3(1024), 0, s, a.loss, (int64_t)0, a.total, 0, nullptr);
         return check_launch(who);
     }
     return a.dtype == M2_F32 ? run_fwd<true>(a, p, s) : run_fwd<false>(a, p, s);
@@ -935,6 +1060,9 @@ int launch_linear_ce_grad(const m2_linear_cross_entropy_grad_args& a, hipStream_
                M2_ERR_INVALID, "%s: x, weight, targets, loss, lse, grad_loss and an output are required", who);
     M2_REQUIRE(a.grad_loss_stride >= 0, M2_ERR_INVALID, "%s: grad_loss stride", who);
     const BwdPlan p = bwd_plan(a);
+    M2_REQUIRE(!a.saved || (a.n > 64 && a.saved_bytes >= p.c.at), M2_ERR_WORKSPACE,
+               "%s: saved of %zu bytes needed (none for up to 64 rows), %zu given", who, a.n > 64 ? p.c.at : 0,
+               a.saved_bytes);
     M2_REQUIRE(a.workspace && a.workspace_bytes >= p.total, M2_ERR_WORKSPACE,
                "%s: workspace of %zu bytes needed, %zu given", who, p.total, a.workspace_bytes);
     return a.dtype == M2_F32 ? run_bwd<true>(a, p, s) : run_bwd<false>(a, p, s);

@@ -57,6 +57,7 @@ int launch_embedding_grad(const m2_embedding_grad_args& a, hipStream_t stream);
 size_t embedding_grad_workspace(const m2_embedding_grad_args& a);
 int launch_linear_ce(const m2_linear_cross_entropy_args& a, hipStream_t stream);
 size_t linear_ce_workspace(const m2_linear_cross_entropy_args& a);
+size_t linear_ce_saved(const m2_linear_cross_entropy_args& a);
 int launch_linear_ce_grad(const m2_linear_cross_entropy_grad_args& a, hipStream_t stream);
 size_t linear_ce_grad_workspace(const m2_linear_cross_entropy_grad_args& a);
 int launch_clip_grad_norm(const m2_clip_grad_norm_args& a, hipStream_t stream);

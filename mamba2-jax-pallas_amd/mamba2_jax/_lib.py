@@ -162,7 +162,8 @@ class LinearCrossEntropyArgs(ctypes.Structure):
     _fields_ = [("x", _c_p), ("weight", _c_p), ("targets", _c_p), ("loss", _c_p), ("lse", _c_p),
                 ("total", _c_p), ("n", _i64), ("vocab", _i64), ("dim", _i64), ("ldx", _i64),
                 ("ldw", _i64), ("ignore_index", _i64), ("dtype", _i32), ("target_dtype", _i32),
-                ("mean", _i32), ("workspace", _c_p), ("workspace_bytes", ctypes.c_size_t)]
+                ("mean", _i32), ("workspace", _c_p), ("workspace_bytes", ctypes.c_size_t),
+                ("saved", _c_p), ("saved_bytes", ctypes.c_size_t)]
 
 
 class LinearCrossEntropyGradArgs(ctypes.Structure):
@@ -171,7 +172,8 @@ class LinearCrossEntropyGradArgs(ctypes.Structure):
                 ("vocab", _i64), ("dim", _i64), ("ldx", _i64), ("ldw", _i64),
                 ("ignore_index", _i64), ("grad_loss_stride", _i64), ("dtype", _i32),
                 ("target_dtype", _i32), ("mean", _i32), ("workspace", _c_p),
-                ("workspace_bytes", ctypes.c_size_t)]
+                ("workspace_bytes", ctypes.c_size_t), ("saved", _c_p),
+                ("saved_bytes", ctypes.c_size_t)]
 
 
 class TensorRef(ctypes.Structure):
@@ -211,6 +213,7 @@ ENTRY_POINTS = {
 WORKSPACE_SIZES = {
     "m2_embedding_grad_workspace_size": EmbeddingGradArgs,
     "m2_linear_cross_entropy_workspace_size": LinearCrossEntropyArgs,
+    "m2_linear_cross_entropy_saved_size": LinearCrossEntropyArgs,
     "m2_linear_cross_entropy_grad_workspace_size": LinearCrossEntropyGradArgs,
     "m2_clip_grad_norm_workspace_size": ClipGradNormArgs,
 }
@@ -297,14 +300,33 @@ def call(name, args, stream):
         raise M2Error(name, rc, load_library().m2_last_error().decode(errors="replace"))
 
 
+_get_device = getattr(torch._C, "_cuda_getDevice", None)
+_HERE = contextlib.nullcontext()
+
+
+def on_device(device):
+    """torch.cuda.device(device), without its cost where that is the current device already."""
+    if _get_device is not None and _get_device() == device.index:
+        return _HERE
+    return torch.cuda.device(device)
+
+
+def size_of(name, args):
+    """The bytes that size function `name` asks for."""
+    fn = _fns.get(name)
+    if fn is None:
+        fn = _fns[name] = getattr(load_library(), name)
+    return fn(ctypes.byref(args))
+
+
 def call_with_workspace(name, args, device):
     """Call entry point `name` on `device`'s current stream with a workspace of the
     size that the library asks for (from torch's caching allocator, as a tensor of
     that stream: it may be reused by later work there)."""
-    size = getattr(load_library(), name + "_workspace_size")(ctypes.byref(args))
+    size = size_of(name + "_workspace_size", args)
     if size == 0:
         raise M2Error(name, -1, load_library().m2_last_error().decode(errors="replace"))
-    with torch.cuda.device(device):
+    with on_device(device):
         ws = torch.empty(size, dtype=torch.uint8, device=device)
         args.workspace, args.workspace_bytes = ws.data_ptr(), size
         call(name, args, stream_of(device))

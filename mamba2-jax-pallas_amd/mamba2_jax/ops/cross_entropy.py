@@ -14,59 +14,66 @@ import torch
 from torch.autograd.function import once_differentiable
 
 from .. import _lib as L
-from .embedding import _rows, _stride
+from .embedding import _dense, _rows, _stride
 
 REDUCTIONS = ("mean", "sum", "none")
+
+
+def _forward(x, weight, targets, ignore_index, reduction, save):
+    """-> (per-position losses, lse, their reduction or None, contiguous targets, what the
+    gradient need not prepare again or None)"""
+    dev, dim = x.device, x.shape[-1]
+    xr, w, t = _rows(x, dim), _rows(weight, dim), _dense(targets)
+    loss = torch.empty(targets.shape, dtype=torch.float32, device=dev)
+    lse = torch.empty(targets.shape, dtype=torch.float32, device=dev)
+    total = None if reduction == "none" else torch.empty((), dtype=torch.float32, device=dev)
+    args = L.LinearCrossEntropyArgs(
+        xr.data_ptr(), w.data_ptr(), t.data_ptr(), loss.data_ptr(), lse.data_ptr(), L.ptr(total),
+        t.numel(), w.shape[0], dim, _stride(xr, dim), _stride(w, dim), int(ignore_index),
+        L.dtype_code(w, "weight"), L.index_code(t, "targets"), int(reduction == "mean"))
+    saved = None
+    if save:
+        size = L.size_of("m2_linear_cross_entropy_saved_size", args)
+        if size:
+            saved = torch.empty(size, dtype=torch.uint8, device=dev)
+            args.saved, args.saved_bytes = saved.data_ptr(), size
+    L.call_with_workspace("m2_linear_cross_entropy", args, dev)
+    return loss, lse, total, t, saved
 
 
 class _LinearCrossEntropy(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, targets, ignore_index, reduction):
-        dev = x.device
-        dim = int(x.shape[-1])
-        xr, w = _rows(x.detach(), dim), _rows(weight.detach(), dim)
-        t = targets.reshape(-1).contiguous()
-        n, vocab = t.numel(), int(w.shape[0])
-        loss = torch.empty(targets.shape, dtype=torch.float32, device=dev)
-        lse = torch.empty_like(loss)
-        total = None if reduction == "none" else torch.empty((), dtype=torch.float32, device=dev)
-        args = L.LinearCrossEntropyArgs(
-            x=L.ptr(xr), weight=L.ptr(w), targets=L.ptr(t), loss=L.ptr(loss), lse=L.ptr(lse),
-            total=L.ptr(total), n=n, vocab=vocab, dim=dim, ldx=_stride(xr, dim),
-            ldw=_stride(w, dim), ignore_index=int(ignore_index), dtype=L.dtype_code(w, "weight"),
-            target_dtype=L.index_code(t, "targets"), mean=int(reduction == "mean"))
-        L.call_with_workspace("m2_linear_cross_entropy", args, dev)
+        loss, lse, total, t, saved = _forward(x, weight, targets, ignore_index, reduction, True)
         # the per-token losses are the result where nothing is reduced: what the backward
         # reads is then a copy, which the caller's in-place changes do not reach
-        kept = loss.clone() if total is None and (ctx.needs_input_grad[0] or ctx.needs_input_grad[1]) \
-            else loss
-        ctx.save_for_backward(x, weight, t, kept, lse)
+        ctx.save_for_backward(x, weight, t, loss.clone() if total is None else loss, lse, saved)
         ctx.args = int(ignore_index), reduction
         return loss if total is None else total
 
     @staticmethod
     @once_differentiable
     def backward(ctx, grad):
-        x, weight, t, loss, lse = ctx.saved_tensors
+        x, weight, t, loss, lse, saved = ctx.saved_tensors
         ignore_index, reduction = ctx.args
         want_x, want_w = ctx.needs_input_grad[:2]
-        dev, dim = x.device, int(x.shape[-1])
+        dev, dim = x.device, x.shape[-1]
         dx = torch.empty(x.shape, dtype=x.dtype, device=dev) if want_x else None
         dw = torch.empty(weight.shape, dtype=weight.dtype, device=dev) if want_w else None
-        if t.numel() == 0:
+        n = t.numel()
+        if n == 0:
             return dx, None if dw is None else dw.zero_(), None, None, None
         xr, w = _rows(x, dim), _rows(weight, dim)
         g = grad.reshape(-1)
         if g.dtype != torch.float32:
             g = g.float()
         args = L.LinearCrossEntropyGradArgs(
-            x=L.ptr(xr), weight=L.ptr(w), targets=L.ptr(t), loss=L.ptr(loss), lse=L.ptr(lse),
-            grad_loss=L.ptr(g), grad_x=L.ptr(dx), grad_weight=L.ptr(dw), n=t.numel(),
-            vocab=int(w.shape[0]), dim=dim, ldx=_stride(xr, dim), ldw=_stride(w, dim),
-            ignore_index=ignore_index,
-            grad_loss_stride=0 if reduction != "none" else int(g.stride(0)),
-            dtype=L.dtype_code(w, "weight"), target_dtype=L.index_code(t, "targets"),
-            mean=int(reduction == "mean"))
+            xr.data_ptr(), w.data_ptr(), t.data_ptr(), loss.data_ptr(), lse.data_ptr(), g.data_ptr(),
+            L.ptr(dx), L.ptr(dw), n, w.shape[0], dim, _stride(xr, dim), _stride(w, dim),
+            ignore_index, 0 if reduction != "none" else g.stride(0), L.dtype_code(w, "weight"),
+            L.index_code(t, "targets"), int(reduction == "mean"))
+        if saved is not None:
+            args.saved, args.saved_bytes = saved.data_ptr(), saved.numel()
         L.call_with_workspace("m2_linear_cross_entropy_grad", args, dev)
         return dx, dw, None, None, None
 
@@ -87,20 +94,25 @@ def linear_cross_entropy(x, weight, targets, ignore_index=-100, reduction="mean"
     the logits again, at most 512 MB of their gradient at a time: bfloat16
     operands round it to bfloat16 before its products with weight and x (float32
     sums, each result rounded once); float32 operands are multiplied as three
-    bfloat16 parts each, accurate to about 2^-24 of each product."""
-    dev = L.device_of(x, weight, targets)
-    L.require(reduction in REDUCTIONS, f"reduction={reduction!r}: one of {REDUCTIONS}")
+    bfloat16 parts each, accurate to about 2^-24 of each product.  Between the two the
+    graph holds the positions' losses and what the kernels read: a packed
+    copy of x's kept rows, and of weight where it cannot be read in place (float32, as
+    three bfloat16 parts: 1.5 times weight; a dim that 64 does not divide)."""
+    L.device_of(x, weight, targets)
+    L.require(reduction in REDUCTIONS, lambda: f"reduction={reduction!r}: one of {REDUCTIONS}")
     L.require(weight.dim() == 2 and x.dim() >= 1 and x.shape[-1] == weight.shape[1],
-              f"x.shape={tuple(x.shape)}, weight.shape={tuple(weight.shape)}: expected (..., dim) "
-              "and (vocab, dim)")
-    L.require(tuple(targets.shape) == tuple(x.shape[:-1]),
-              f"targets.shape={tuple(targets.shape)}: expected {tuple(x.shape[:-1])}")
-    L.require(weight.shape[0] > 0 and weight.shape[1] > 0, f"weight.shape={tuple(weight.shape)}")
+              lambda: f"x.shape={tuple(x.shape)}, weight.shape={tuple(weight.shape)}: expected "
+                      "(..., dim) and (vocab, dim)")
+    L.require(targets.shape == x.shape[:-1],
+              lambda: f"targets.shape={tuple(targets.shape)}: expected {tuple(x.shape[:-1])}")
+    L.require(weight.shape[0] > 0 and weight.shape[1] > 0, lambda: f"weight.shape={tuple(weight.shape)}")
     L.index_code(targets, "targets")
     if L.dtype_code(x, "x") != L.dtype_code(weight, "weight"):
         raise TypeError(f"x is {x.dtype} and weight {weight.dtype}: they must be the same")
-    del dev
-    return _LinearCrossEntropy.apply(x, weight, targets, ignore_index, reduction)
+    if (x.requires_grad or weight.requires_grad) and torch.is_grad_enabled():
+        return _LinearCrossEntropy.apply(x, weight, targets, ignore_index, reduction)
+    loss, _, total, _, _ = _forward(x, weight, targets, ignore_index, reduction, False)
+    return loss if total is None else total
 
 
 __all__ = ["linear_cross_entropy"]

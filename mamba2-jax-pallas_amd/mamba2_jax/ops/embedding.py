@@ -15,14 +15,10 @@ from torch.autograd.function import once_differentiable
 from .. import _lib as L
 
 
-def _flat_ids(ids):
-    L.index_code(ids, "ids")
-    return ids.reshape(-1).contiguous()
-
-
 def _rows(t, dim):
     """t (..., dim) as rows (n, dim) with unit last stride (a view where it can be)."""
-    t = t.reshape(-1, dim)
+    if t.dim() != 2:
+        t = t.reshape(-1, dim)
     if (t.shape[0] > 1 and t.stride(0) < dim) or (dim > 1 and t.stride(1) != 1):
         t = t.contiguous()
     return t
@@ -32,22 +28,22 @@ def _stride(t, dim):
     return t.stride(0) if t.shape[0] > 1 else dim
 
 
-def _lookup(ids, weight, scale):
-    dev = L.device_of(ids, weight)
-    L.require(weight.dim() == 2, f"weight.shape={tuple(weight.shape)}: expected (vocab, dim)")
-    code = L.dtype_code(weight, "weight")
-    flat = _flat_ids(ids)
-    vocab, dim = (int(s) for s in weight.shape)
-    L.require(vocab > 0 and dim > 0, f"weight.shape={tuple(weight.shape)}")
-    w = _rows(weight.detach(), dim)
+def _dense(t):
+    return t if t.is_contiguous() else t.contiguous()
+
+
+def _lookup(dev, ids, weight, scale):
+    code, id_code = L.dtype_code(weight, "weight"), L.index_code(ids, "ids")
+    vocab, dim = weight.shape
+    L.require(vocab > 0 and dim > 0, lambda: f"weight.shape={tuple(weight.shape)}")
+    ids, w = _dense(ids), _rows(weight, dim)
     out = torch.empty((*ids.shape, dim), dtype=weight.dtype, device=dev)
-    if flat.numel() == 0:
-        return out
-    args = L.EmbeddingArgs(ids=L.ptr(flat), weight=L.ptr(w), out=L.ptr(out), n=flat.numel(),
-                           vocab=vocab, dim=dim, ldw=_stride(w, dim), ldo=dim, scale=float(scale),
-                           id_dtype=L.index_code(flat, "ids"), dtype=code)
-    with torch.cuda.device(dev):
-        L.call("m2_embedding", args, L.stream_of(dev))
+    n = ids.numel()
+    if n:
+        args = L.EmbeddingArgs(ids.data_ptr(), w.data_ptr(), out.data_ptr(), n, vocab, dim,
+                               _stride(w, dim), dim, scale, id_code, code)
+        with L.on_device(dev):
+            L.call("m2_embedding", args, L.stream_of(dev))
     return out
 
 
@@ -55,8 +51,8 @@ class _Embedding(torch.autograd.Function):
     @staticmethod
     def forward(ctx, ids, weight, scale, padding_idx):
         ctx.save_for_backward(ids)
-        ctx.args = int(weight.shape[0]), float(scale), padding_idx, weight.dtype
-        return _lookup(ids, weight, scale)
+        ctx.args = int(weight.shape[0]), scale, padding_idx, weight.dtype
+        return _lookup(weight.device, ids, weight, scale)
 
     @staticmethod
     @once_differentiable
@@ -84,12 +80,13 @@ def embedding(ids, weight, scale=1.0, padding_idx=None):
     vocabulary cannot be reported without waiting for the GPU: its row is NaN,
     and it takes no part in the gradient.  padding_idx: an id whose gradient is left
     out (its row is looked up like any other)."""
-    L.device_of(ids, weight)
-    L.require(weight.dim() == 2, f"weight.shape={tuple(weight.shape)}: expected (vocab, dim)")
-    padding_idx = _padding(padding_idx, int(weight.shape[0]))
-    if torch.is_grad_enabled() and weight.requires_grad:
+    dev = L.device_of(ids, weight)
+    L.require(weight.dim() == 2, lambda: f"weight.shape={tuple(weight.shape)}: expected (vocab, dim)")
+    padding_idx = _padding(padding_idx, weight.shape[0])
+    scale = float(scale)
+    if weight.requires_grad and torch.is_grad_enabled():
         return _Embedding.apply(ids, weight, scale, padding_idx)
-    return _lookup(ids, weight, scale)
+    return _lookup(dev, ids, weight, scale)
 
 
 def embedding_grad(ids, grad, num_embeddings, scale=1.0, padding_idx=None, *, dtype=None, out=None):
@@ -104,29 +101,26 @@ def embedding_grad(ids, grad, num_embeddings, scale=1.0, padding_idx=None, *, dt
     gradient of an embedding tied to the head, after the head's."""
     dev = L.device_of(ids, grad, out)
     vocab = int(num_embeddings)
-    L.require(0 < vocab < 2 ** 27, f"num_embeddings={vocab}")
-    L.require(grad.dim() == ids.dim() + 1 and tuple(grad.shape[:-1]) == tuple(ids.shape),
-              f"grad.shape={tuple(grad.shape)}: expected {tuple(ids.shape)} + (dim,)")
-    dim = int(grad.shape[-1])
+    L.require(0 < vocab < 2 ** 27, lambda: f"num_embeddings={vocab}")
+    L.require(grad.dim() == ids.dim() + 1 and grad.shape[:-1] == ids.shape,
+              lambda: f"grad.shape={tuple(grad.shape)}: expected {tuple(ids.shape)} + (dim,)")
+    dim = grad.shape[-1]
     L.require(dim > 0, "grad has no columns")
-    L.dtype_code(grad, "grad")
+    grad_code, id_code = L.dtype_code(grad, "grad"), L.index_code(ids, "ids")
     padding_idx = _padding(padding_idx, vocab)
-    flat = _flat_ids(ids)
-    g = _rows(grad.detach(), dim)
+    ids, g = _dense(ids), _rows(grad, dim)
     accumulate = out is not None
     if accumulate:
         L.require(dtype is None or out.dtype == dtype, "dtype and out disagree")
-        L.require(tuple(out.shape) == (vocab, dim) and (dim == 1 or out.stride(1) == 1)
+        L.require(out.shape == (vocab, dim) and (dim == 1 or out.stride(1) == 1)
                   and (vocab == 1 or out.stride(0) >= dim),
                   f"out must be ({vocab}, {dim}) with a contiguous last dimension")
     else:
         out = torch.empty((vocab, dim), dtype=L.torch_dtype(dtype) or grad.dtype, device=dev)
     args = L.EmbeddingGradArgs(
-        ids=L.ptr(flat), grad=L.ptr(g), out=L.ptr(out), n=flat.numel(), vocab=vocab, dim=dim,
-        ldg=_stride(g, dim), ldo=_stride(out, dim),
-        padding_idx=-1 if padding_idx is None else padding_idx, scale=float(scale),
-        id_dtype=L.index_code(flat, "ids"), grad_dtype=L.dtype_code(g, "grad"),
-        out_dtype=L.dtype_code(out, "out"), accumulate=int(accumulate))
+        ids.data_ptr(), g.data_ptr(), out.data_ptr(), ids.numel(), vocab, dim, _stride(g, dim),
+        _stride(out, dim), -1 if padding_idx is None else padding_idx, float(scale), id_code,
+        grad_code, L.dtype_code(out, "out"), int(accumulate))
     L.call_with_workspace("m2_embedding_grad", args, dev)
     if accumulate:
         torch.autograd.graph.increment_version(out)

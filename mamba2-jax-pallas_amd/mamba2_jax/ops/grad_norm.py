@@ -5,7 +5,8 @@ training path.
 
 from __future__ import annotations
 
-import ctypes
+from array import array
+from itertools import chain
 
 import torch
 
@@ -17,17 +18,15 @@ def _dense(t):
     return t.is_contiguous() or torch.empty_like(t, device="meta").stride() == t.stride()
 
 
-def _run(tensors, outs, max_norm, eps):
-    dev = L.device_of(*tensors)
-    refs = (L.TensorRef * len(tensors))()
-    flat = []
-    for i, t in enumerate(tensors):
-        flat += (t.data_ptr(), 0 if outs is None else outs[i].data_ptr(), t.numel(),
-                 L.dtype_code(t, f"tensor {i}"))
-    ctypes.memmove(refs, (ctypes.c_int64 * len(flat))(*flat), ctypes.sizeof(refs))
+def _run(dev, tensors, outs, max_norm, eps):
+    # a table of m2_tensor_ref (in, out, n, dtype), built without a Python loop over its rows
+    ins = [t.data_ptr() for t in tensors]
+    codes = [L.dtype_code(t, "a tensor") for t in tensors]
+    to = [0] * len(ins) if outs is None else [t.data_ptr() for t in outs]
+    refs = array("q", chain.from_iterable(zip(ins, to, [t.numel() for t in tensors], codes)))
     norm = torch.empty((), dtype=torch.float32, device=dev)
-    args = L.ClipGradNormArgs(tensors=ctypes.addressof(refs), count=len(tensors), norm=norm.data_ptr(),
-                              max_norm=max_norm, eps=eps, clip=int(outs is not None))
+    args = L.ClipGradNormArgs(refs.buffer_info()[0], len(ins), norm.data_ptr(), max_norm, eps,
+                              int(outs is not None))
     L.call_with_workspace("m2_clip_grad_norm", args, dev)
     return norm
 
@@ -36,9 +35,10 @@ def global_norm(tensors):
     """The square root of the sum of the squares of all values of all tensors (float32
     or bfloat16, on one GPU), a float32 scalar on the GPU; summed in float64 in
     a fixed order."""
-    tensors = [t.detach() if _dense(t) else t.detach().contiguous() for t in tensors]
+    tensors = list(tensors)
     L.require(len(tensors) > 0, "global_norm: no tensors")
-    return _run(tensors, None, 0.0, 0.0)
+    dev = L.device_of(*tensors)
+    return _run(dev, [t if _dense(t) else t.detach().contiguous() for t in tensors], None, 0.0, 0.0)
 
 
 def clip_grad_norm(grads, max_norm, *, out=None, eps=1e-6):
@@ -52,24 +52,26 @@ def clip_grad_norm(grads, max_norm, *, out=None, eps=1e-6):
     returned; out=grads clips in place (and writes nothing where the norm is within
     max_norm).  By default the results are new tensors and grads stay as they
     are.  max_norm must not be negative."""
-    grads = [g.detach() for g in grads]
+    grads = list(grads)
     L.require(len(grads) > 0, "clip_grad_norm: no gradients")
     max_norm, eps = float(max_norm), float(eps)
-    L.require(max_norm >= 0 and eps >= 0, f"max_norm={max_norm}, eps={eps}: must not be negative")
+    L.require(max_norm >= 0 and eps >= 0, lambda: f"max_norm={max_norm}, eps={eps}: must not be negative")
     if out is None:
-        grads = [g if _dense(g) else g.contiguous() for g in grads]
-        outs = [torch.empty_like(g) for g in grads]
+        dev = L.device_of(*grads)
+        grads = [g if _dense(g) else g.detach().contiguous() for g in grads]
+        outs = [torch.empty_like(g, requires_grad=False) for g in grads]
     else:
         outs = list(out)
-        L.require(len(outs) == len(grads), f"out holds {len(outs)} tensors for {len(grads)} gradients")
+        L.require(len(outs) == len(grads),
+                  lambda: f"out holds {len(outs)} tensors for {len(grads)} gradients")
+        dev = L.device_of(*grads, *outs)
         for i, (g, o) in enumerate(zip(grads, outs)):
-            L.require(o.shape == g.shape and o.dtype == g.dtype
-                      and (o.is_contiguous() and g.is_contiguous()
-                           or o.stride() == g.stride() and _dense(o)),
-                      lambda: f"out[{i}] must have the shape, dtype and strides of its gradient, "
-                              "without gaps")
-        L.device_of(*grads, *outs)
-    norm = _run(grads, outs, max_norm, eps)
+            if not (o.shape == g.shape and o.dtype == g.dtype
+                    and (o.is_contiguous() and g.is_contiguous()
+                         or o.stride() == g.stride() and _dense(o))):
+                raise L.M2ShapeError(f"out[{i}] must have the shape, dtype and strides of its "
+                                     "gradient, without gaps")
+    norm = _run(dev, grads, outs, max_norm, eps)
     if out is not None:
         torch.autograd.graph.increment_version(outs)
     return outs, norm

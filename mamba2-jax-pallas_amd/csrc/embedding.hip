@@ -18,6 +18,10 @@
 // large vocabulary's gradient.  The rows that ids name are written twice that way, at
 // most n rows; zeroing the others alone would have to wait for the sort.  Bound
 // by HBM: grad read once, the result written once and those rows again.
+//
+// Up to 256 entries need neither sort nor partial rows: one launch, in which every entry
+// looks for its id among the others and the first of an id adds up all of them, while
+// further workgroups write the zeros of the rows that no id names.
 #include "m2_internal.h"
 
 #include <type_traits>
@@ -475,6 +479,94 @@ __global__ void __launch_bounds__(JOIN_THREADS) k_embed_join(ReduceArgs a) {
     put_row<TO, V>(a, key, c, s);
 }
 
+// ---------------------------------------------------------------------------
+// few entries: the whole gradient in one launch
+// ---------------------------------------------------------------------------
+constexpr int FEW_N = 256, FEW_THREADS = 256, FEW_ROWS = 4096;
+struct FewArgs {
+    const void* ids;
+    int64_t padding;
+    int64_t row_bytes, ld_bytes;
+    int id64, nred, rows;    // workgroups that sum; rows that one of the others zeroes
+};
+
+template <typename T, typename TO, int V>
+__global__ void __launch_bounds__(FEW_THREADS) k_embed_few(ReduceArgs a, FewArgs f) {
+    __shared__ uint8_t named[FEW_ROWS];
+    const int t = threadIdx.x, lane = t & 63;
+    auto key_at = [&](int i) {
+        const int64_t id = load_id(f.ids, i, f.id64);
+        return id >= 0 && id < a.vocab && id != f.padding ? (int32_t)id : -1;
+    };
+    if ((int)blockIdx.x >= f.nred) {
+        const int64_t r0 = (int64_t)(blockIdx.x - f.nred) * f.rows;
+        const int rows = (int)min((int64_t)f.rows, a.vocab - r0);
+        for (int i = t; i < rows; i += FEW_THREADS) named[i] = 0;
+        __syncthreads();
+        if (t < a.n) {
+            const int64_t r = key_at(t) - r0;
+            if (r >= 0 && r < rows) named[r] = 1;
+        }
+        __syncthreads();
+        // 16-byte pieces, the last one of a row ends with it; rows shorter than that by their
+        // 2-byte elements
+        char* out = static_cast<char*>(a.out) + r0 * f.ld_bytes;
+        const int bytes = f.row_bytes < 16 ? 2 : 16;
+        const uint32_t per = (uint32_t)((f.row_bytes + bytes - 1) / bytes);
+        const uint32_t all = per * rows;
+        for (uint32_t i = t; i < all; i += FEW_THREADS) {
+            const uint32_t r = i / per, c = i - r * per;
+            if (named[r]) continue;
+            char* p = out + r * f.ld_bytes + min((int64_t)c * bytes, f.row_bytes - bytes);
+            if (bytes == 16) store16(p, u32x4{0, 0, 0, 0});
+            else *reinterpret_cast<uint16_t*>(p) = 0;
+        }
+        return;
+    }
+    const int e = blockIdx.x / a.slabs, slab = blockIdx.x % a.slabs;
+    const int32_t key = key_at(e);
+    if (key < 0) return;
+    uint64_t same[FEW_N / 64];            // entries with this id
+#pragma unroll
+    for (int j = 0; j < FEW_N / 64; ++j) {
+        const int i = 64 * j + lane;
+        same[j] = __ballot(i < a.n && key_at(i) == key);
+    }
+    // an earlier entry has it: that one's workgroup adds them all
+#pragma unroll
+    for (int j = 0; j < FEW_N / 64; ++j)
+        if (64 * j <= e && (same[j] & ((e >> 6) == j ? (1ull << (e & 63)) - 1 : ~0ull))) return;
+    const int c = slab * FEW_THREADS + t;
+    if (c >= a.vecs) return;
+    const T* g = static_cast<const T*>(a.grad) + piece_at<V>(c, a.cols);
+    Vec<float, V> s;
+#pragma unroll
+    for (int i = 0; i < V; ++i) s.v[i] = 0.f;
+#pragma unroll
+    for (int j = 0; j < FEW_N / 64; ++j) {
+        uint64_t m = same[j];
+        while (m) {
+            constexpr int UN = 4;
+            Vec<T, V> v[UN];
+            int k = 0;
+#pragma unroll
+            for (int u = 0; u < UN; ++u)
+                if (m) {
+                    const int at = 64 * j + __ffsll((unsigned long long)m) - 1;
+                    m &= m - 1;
+                    v[u].load(g + (int64_t)at * a.ldg);
+                    k = u + 1;
+                }
+#pragma unroll
+            for (int u = 0; u < UN; ++u)
+                if (u < k)
+#pragma unroll
+                    for (int i = 0; i < V; ++i) s.v[i] += v[u].v[i];
+        }
+    }
+    put_row<TO, V>(a, key, c, s);
+}
+
 size_t align256(size_t v) { return (v + 255) & ~size_t(255); }
 
 struct GradPlan {
@@ -567,8 +659,7 @@ int launch_embedding(const m2_embedding_args& a, hipStream_t s) {
 
 size_t embedding_grad_workspace(const m2_embedding_grad_args& a) {
     if (check_grad(a)) return 0;
-    const size_t n = grad_plan(a).total;
-    return n ? n : 256;
+    return a.n <= FEW_N ? 256 : grad_plan(a).total;
 }
 
 int launch_embedding_grad(const m2_embedding_grad_args& a, hipStream_t s) {
@@ -582,9 +673,35 @@ int launch_embedding_grad(const m2_embedding_grad_args& a, hipStream_t s) {
     M2_REQUIRE(a.out && (a.n == 0 || (a.ids && a.grad)), M2_ERR_INVALID, "%s: ids, grad and out are required",
                who);
     const GradPlan p = grad_plan(a);
-    M2_REQUIRE(a.workspace && a.workspace_bytes >= (p.total ? p.total : 256), M2_ERR_WORKSPACE,
-               "%s: workspace of %zu bytes needed, %zu given", who, p.total, a.workspace_bytes);
+    const size_t need = embedding_grad_workspace(a);
+    M2_REQUIRE(a.workspace && a.workspace_bytes >= need, M2_ERR_WORKSPACE,
+               "%s: workspace of %zu bytes needed, %zu given", who, need, a.workspace_bytes);
     if (a.n == 0 && a.accumulate) return M2_OK;
+    if (a.n <= FEW_N) {
+        ReduceArgs r{};
+        const bool vec = a.dim >= 8;
+        const int64_t osz = (int64_t)m2_dtype_size(a.out_dtype);
+        r.grad = a.grad; r.out = a.out; r.ldg = a.ldg; r.ldo = a.ldo; r.vocab = a.vocab;
+        r.n = (int)a.n; r.cols = (int)a.dim; r.accumulate = a.accumulate; r.scale = a.scale;
+        r.vecs = (int)(vec ? (a.dim + 7) / 8 : a.dim);
+        r.slabs = (r.vecs + FEW_THREADS - 1) / FEW_THREADS;
+        FewArgs f{a.ids, a.padding_idx, a.dim * osz, a.ldo * osz, a.id_dtype == M2_I64, (int)a.n * r.slabs, 0};
+        const int64_t rows = (FILL_BYTES + f.row_bytes - 1) / f.row_bytes;
+        f.rows = (int)(rows < FEW_ROWS ? rows : FEW_ROWS);
+        const int64_t zero = a.accumulate ? 0 : (a.vocab + f.rows - 1) / f.rows;
+        const dim3 grid((unsigned)(f.nred + zero)), thr(FEW_THREADS);
+#define M2_FEW(T, TO)                                                                              \
+    do {                                                                                           \
+        if (vec) hipLaunchKernelGGL((k_embed_few<T, TO, 8>), grid, thr, 0, s, r, f);               \
+        else hipLaunchKernelGGL((k_embed_few<T, TO, 1>), grid, thr, 0, s, r, f);                   \
+    } while (0)
+        if (a.grad_dtype == M2_BF16 && a.out_dtype == M2_BF16) M2_FEW(bf16, bf16);
+        else if (a.grad_dtype == M2_BF16) M2_FEW(bf16, float);
+        else if (a.out_dtype == M2_BF16) M2_FEW(float, bf16);
+        else M2_FEW(float, float);
+#undef M2_FEW
+        return check_launch(who);
+    }
     char* ws = static_cast<char*>(a.workspace);
     auto at = [&](size_t o) { return reinterpret_cast<int32_t*>(ws + o); };
     SortArgs k{};
@@ -606,7 +723,7 @@ int launch_embedding_grad(const m2_embedding_grad_args& a, hipStream_t s) {
     };
     int cur = 0;
     if (p.small) {
-        // one launch (also for n == 0, which only writes the zeros)
+        // one launch
         k.nb = p.passes;
         k.keys_out = at(p.keys[0]); k.pos_out = at(p.pos[0]);
         const dim3 grid(1 + zeros(0, 8192)), thr(SMALL_THREADS);
@@ -628,7 +745,6 @@ int launch_embedding_grad(const m2_embedding_grad_args& a, hipStream_t s) {
         cur ^= 1;
     }
     if (int rc = check_launch(who)) return rc;
-    if (a.n == 0) return M2_OK;
     const int gs = (int)m2_dtype_size(a.grad_dtype), os = (int)m2_dtype_size(a.out_dtype);
     const bool vec = a.dim >= 8;
     ReduceArgs r{};

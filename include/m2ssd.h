@@ -491,8 +491,8 @@ typedef struct {
     const void* x;                 /* [n, dim] at ldx, dtype                    */
     const void* weight;            /* [vocab, dim] at ldw, dtype                */
     const void* targets;           /* [n], target_dtype (M2_I32 / M2_I64)       */
-    float*      loss;              /* out [n]                                   */
-    float*      lse;               /* out [n] (0 where left out)                */
+    float*      loss;              /* out [n], or NULL with total               */
+    float*      lse;               /* out [n] (0 where left out) or NULL        */
     float*      total;             /* out [1] or NULL                           */
     int64_t n, vocab, dim, ldx, ldw;
     int64_t ignore_index;
@@ -502,10 +502,11 @@ typedef struct {
     void*   saved;                 /* out, or NULL                              */
     size_t  saved_bytes;           /* >= m2_linear_cross_entropy_saved_size()   */
 } m2_linear_cross_entropy_args;
-/* With saved, the forward leaves the operands as its kernels read them there (the kept
- * rows of x; the weights where they are not read in place: float32, rows that
- * are not whole 128-byte pieces), and the gradient given the same buffer for
- * the same arguments does not prepare them again.  0: nothing to save (up to 64 rows). */
+/* With saved, the forward leaves there what the gradient reads: which rows are kept, their
+ * lse and loss, and the operands as its kernels read them (the kept rows of x; the weights where
+ * they are not read in place: float32, rows that are not whole 128-byte pieces).
+ * The gradient given the same buffer for the same arguments needs neither x, targets,
+ * loss nor lse. */
 size_t m2_linear_cross_entropy_saved_size(const m2_linear_cross_entropy_args* a);
 size_t m2_linear_cross_entropy_workspace_size(const m2_linear_cross_entropy_args* a);
 int m2_linear_cross_entropy(const m2_linear_cross_entropy_args* a, void* stream);

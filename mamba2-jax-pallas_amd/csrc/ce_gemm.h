@@ -9,7 +9,8 @@
 //   row tile in LDS: [R][BK], rows whose 16-byte pieces are XOR-swizzled by the row
 //     (swz); fragments by ds_read_b128, without bank conflicts;
 //   col tile in LDS: [BK][R], rows of 2 R bytes whose 32-byte pieces (the 16
-//     columns of one fragment) are XOR-swizzled by f(k) = k & 3 | (k >> 3 & 1) << 2;
+//     columns of one fragment) are XOR-swizzled by f(k) = k & 3 | (k >> 3 & 1) << 2 (as far
+//     as R has pieces);
 //     fragments by ds_read_b64_tr_b16, whose sixteen lanes read 4 k rows: the 8 rows that
 //     32 lanes touch lie on different banks.
 // The swizzle is applied to the global address of each lane, since a direct
@@ -101,7 +102,7 @@ template <int R, bool TR, int NW, int BK> struct Loader {
             } else {
                 const int q = in * 64 + lane;
                 const int k = q / PR, c = q % PR;
-                const int f = (k & 3) | (((k >> 3) & 1) << 2);
+                const int f = ((k & 3) | (((k >> 3) & 1) << 2)) & (R / 16 - 1);
                 int m = ((((c >> 1) ^ f) << 1) | (c & 1)) * 8;
                 m = min(m0 + m, o.lim - 8) - m0;
                 off[j] = (uint32_t)((int64_t)k * o.ld * 2 + m * 2);
@@ -153,7 +154,7 @@ template <int R, bool TR, int F, int BK> struct Reader {
             x = (r0 + (lane & 15)) * BK * 2;
         } else {
             const int g = lane >> 4, r = (lane & 15) >> 2;
-            const int f = r | ((g & 1) << 2);
+            const int f = (r | ((g & 1) << 2)) & (R / 16 - 1);
             x = (8 * g + r) * (2 * R) + (lane & 3) * 8 + (((r0 >> 4) ^ f) << 5);
         }
     }

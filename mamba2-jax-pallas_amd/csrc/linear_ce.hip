@@ -31,15 +31,14 @@ using namespace m2ce;
 
 constexpr float LOG2E = 1.4426950408889634f;
 
-struct Tokens {              // in the workspace
-    int* idx;                // [np] row of x of each kept token
+struct Tokens {              // of the kept tokens: in the workspace, or saved for the gradient
+    int* idx;                // [np] row of x of each
     int* inv;                // [n] kept index of each row, -1: left out
     int* tgt;                // [np] target, -1: outside the vocabulary
+    float* lse;              // [np]
+    float* em1;              // [np] expm1(-loss): G at the target
+    int* count;              // [2] their number; workgroups of k_ce_join that are done
     float* zt;               // [np] the target's logit (forward)
-    float* lse;              // [np] (backward, as the two below)
-    float* gf;               // [np] upstream gradient
-    float* gm;               // [np] G at the target
-    int* count;              // [1]
 };
 
 M2_DEV int64_t load_target(const void* targets, int t64, int64_t i) {
@@ -91,7 +90,7 @@ __global__ void __launch_bounds__(1024) k_ce_compact(const void* targets, int64_
             if (keep[e]) tk.idx[at++] = (int)i;
         }
     }
-    if (t == 0) *tk.count = base;
+    if (t < 2) tk.count[t] = t == 0 ? base : 0;
 }
 
 // 8 consecutive elements of a row, zero past its end
@@ -139,71 +138,61 @@ struct PackArgs {
     int64_t rows, dim, ld, dp, plane;
     // of the tokens
     const void* targets;
-    const float* lse;
+    const float* lse;        // given to a gradient that finds nothing saved
     const float* loss;
-    const float* g;
-    int64_t gstride, vocab, n, ignore;
-    int t64, mean;
+    int64_t vocab, n, ignore;
+    int t64;
 };
-
-// what the epilogues of the backward need of kept token r, row `from` of the inputs (-1: none)
-M2_DEV void token_grads(const PackArgs& a, const Tokens& tk, int64_t r, int64_t from, int tgt, int count) {
-    float gf = 0.f, gm = 0.f, lse = 0.f;
-    if (from >= 0) {
-        gf = a.g[from * a.gstride] * (a.mean ? 1.f / (float)count : 1.f);
-        lse = a.lse[from];
-        const float l = a.loss[from];
-        gm = gf * expm1f(-l);
-        if (tgt < 0) gf = l;                 // NaN: the row's gradients are too
-    }
-    tk.lse[r] = lse;
-    tk.gf[r] = gf;
-    tk.gm[r] = gm;
-}
-// the same where the forward left the packed operands
-__global__ void __launch_bounds__(256) k_ce_tokens(PackArgs a, Tokens tk) {
-    const int64_t r = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    const int count = *tk.count;
-    if (r < ((count + 63) & ~63)) token_grads(a, tk, r, r < count ? tk.idx[r] : -1, tk.tgt[r], count);
-}
+constexpr int64_t PACK_FINDS = 1024;     // up to so many tokens the packing finds the kept ones itself
 
 // Rows of src as bf16 (planes) with rows of dp elements, zeros behind dim: the weights
 // where they cannot be read in place, or the kept rows of x (TOK), with zero rows up to
-// the next whole K step, and what the epilogues need of each token.  Up to 64 tokens
-// every wavefront finds the kept ones by itself (k_ce_compact does for more).
+// the next whole K step.  Up to PACK_FINDS tokens a wavefront for each row counts
+// the kept ones before it, and 64 more write the zero rows; beyond, k_ce_compact has found them.
 template <typename T, bool TOK>
 __global__ void __launch_bounds__(256) k_ce_pack(PackArgs a, Tokens tk) {
-    const int64_t r = (int64_t)blockIdx.x * 4 + wave_id();
+    int64_t r = (int64_t)blockIdx.x * 4 + wave_id();
     const int lane = threadIdx.x & 63;
     int64_t from = r;
     if constexpr (TOK) {
-        int count;
-        if (a.n <= 64) {
-            const bool keep = lane < a.n && load_target(a.targets, a.t64, lane) != a.ignore;
-            const uint64_t all = __ballot(keep);
-            const int at = __popcll(all & ((1ull << lane) - 1));
-            const uint64_t mine = __ballot(keep && at == r);
-            from = mine ? __ffsll((unsigned long long)mine) - 1 : -1;
-            count = __popcll(all);
-            if (r == 0) {
-                if (lane < a.n) tk.inv[lane] = keep ? at : -1;
-                if (keep) tk.idx[at] = lane;
-                if (lane == 0) *tk.count = count;
+        if (a.n <= PACK_FINDS) {
+            if (r >= a.n + 64) return;
+            int before = 0;
+            const int64_t end = min(r, a.n);
+#pragma unroll 4
+            for (int64_t i = 0; i < end; i += 64)
+                before += __popcll(__ballot(i + lane < end && load_target(a.targets, a.t64, i + lane) != a.ignore));
+            if (r >= a.n) {                   // before: all of them
+                if (r == a.n && lane < 2) tk.count[lane] = lane == 0 ? before : 0;
+                r += before - a.n;
+                if (r >= ((before + 63) & ~63)) return;
+                from = -1;
+            } else {
+                const bool keep = load_target(a.targets, a.t64, r) != a.ignore;
+                if (lane == 0) {
+                    tk.inv[r] = keep ? before : -1;
+                    if (keep) tk.idx[before] = (int)r;
+                }
+                if (!keep) return;
+                r = before;
             }
         } else {
-            count = *tk.count;
+            const int count = *tk.count;
+            if (r >= ((count + 63) & ~63)) return;
             from = r < count ? tk.idx[r] : -1;
         }
-        if (r >= ((count + 63) & ~63)) return;
         if (lane == 0) {
             int tg = -1;
             if (from >= 0) {
                 const int64_t v = load_target(a.targets, a.t64, from);
                 tg = v >= 0 && v < a.vocab ? (int)v : -1;
+                if (a.loss) {
+                    tk.lse[r] = a.lse[from];
+                    tk.em1[r] = expm1f(-a.loss[from]);
+                }
             }
             tk.tgt[r] = tg;
-            if (a.g) token_grads(a, tk, r, from, tg, count);
-            else tk.zt[r] = __builtin_nanf("");
+            if (tk.zt) tk.zt[r] = __builtin_nanf("");
         }
     } else {
         if (r >= a.rows) return;
@@ -374,13 +363,13 @@ M2_DEV void store_row(T* row, int m0, int64_t dim, int lane, const f32x4& x, con
 // vocabulary and past the kept tokens
 struct EpiG {
     static constexpr bool SEG = false;
-    const int* tgt;
-    const float* lse;
-    const float* gf;
-    const float* gm;
+    Tokens tk;
+    const float* up;         // upstream gradient
     bf16* G;
     int64_t ldg, plane;
+    int64_t ups;             // its stride (0: one value)
     int v_first, vocab;      // of the piece; of all
+    int mean;
 
     template <class S>
     M2_DEV void run(f32x4 (&acc)[S::FM][S::FN], char* smem, int m0, int n0, int wm, int wn, int lane, int count, int, int) const {
@@ -390,14 +379,17 @@ struct EpiG {
         // of the tokens, before the first store (a load behind it would wait for it)
         int t[S::FN];
         float ls[S::FN], g[S::FN], gt[S::FN];
+        const float scale = mean ? 1.f / (float)count : 1.f;
 #pragma unroll
         for (int j = 0; j < S::FN; ++j) {
             const int n = n0 + (wn * S::FN + j) * 16 + (lane & 15);
             const bool on = n < count;
-            t[j] = on ? tgt[n] - v_first : -1;
-            ls[j] = on ? lse[n] * -LOG2E : 0.f;
-            g[j] = on ? gf[n] : 0.f;
-            gt[j] = on ? gm[n] : 0.f;
+            t[j] = on ? tk.tgt[n] : 0;
+            ls[j] = on ? tk.lse[n] * -LOG2E : 0.f;
+            g[j] = on ? up[ups ? tk.idx[n] * ups : 0] * scale : 0.f;
+            gt[j] = on ? g[j] * tk.em1[n] : 0.f;
+            if (t[j] < 0) g[j] = __builtin_nanf("");       // a target outside the vocabulary
+            t[j] -= v_first;
         }
         // rows past the vocabulary: zeros, whatever x holds
         const bool edge = v_first + m0 + S::BM > vocab;
@@ -523,40 +515,85 @@ template <typename T> struct EpiDw {
 struct JoinArgs {
     const float2* part;
     int64_t np, n;
-    float* loss;
-    float* lse;
-    int parts;
+    float* loss;             // of every position, or NULL
+    float* lse;              // the same
+    float* total;            // or NULL
+    double* sums;            // of each workgroup
+    int parts, mean;
 };
 
-// 16 tokens per workgroup, 16 lanes each: lane q joins parts q, q + 16, ...
-__global__ void __launch_bounds__(256) k_ce_join(JoinArgs a, Tokens tk) {
-    __shared__ float2 red[16][17];
-    const int tok = threadIdx.x & 15, q = threadIdx.x >> 4;
+// 16 tokens per workgroup, 64 lanes each: lane q joins parts q, q + 64, ...  The losses are added
+// up in float64, those of a workgroup first, then by the last one to be done the workgroups' in
+// their order: which one is last changes nothing.
+__global__ void __launch_bounds__(1024) k_ce_join(JoinArgs a, Tokens tk) {
+    __shared__ float2 red[64][17];
+    __shared__ bool last;
+    __shared__ double wsum[16];
+    const int t = threadIdx.x, tok = t & 15, q = t >> 4;
     const int64_t n = (int64_t)blockIdx.x * 16 + tok;
     const int k = n < a.n ? tk.inv[n] : -1;
     LogSum o;
     if (k >= 0) {
 #pragma unroll 4
-        for (int i = q; i < a.parts; i += 16) o.add(a.part[(int64_t)i * a.np + k]);
+        for (int i = q; i < a.parts; i += 64) o.add(a.part[(int64_t)i * a.np + k]);
     }
     red[q][tok] = make_float2(o.mx, o.s);
     __syncthreads();
-    if (q == 0 && n < a.n) {
+    if (q < 8) {
+        o = LogSum();
+#pragma unroll
+        for (int i = q; i < 64; i += 8) o.add(red[i][tok]);
+    }
+    __syncthreads();
+    if (q < 8) red[q][tok] = make_float2(o.mx, o.s);
+    __syncthreads();
+    if (t < 16) {
         float loss = 0.f, lse = 0.f;
         if (k >= 0) {
-            for (int i = 1; i < 16; ++i) o.add(red[i][tok]);
+            o = LogSum();
+#pragma unroll
+            for (int i = 0; i < 8; ++i) o.add(red[i][tok]);
             const float zt = tk.zt[k];
             loss = o.loss(zt);
             lse = zt + loss;
+            tk.lse[k] = lse;
+            tk.em1[k] = expm1f(-loss);
         }
-        a.loss[n] = loss;
-        a.lse[n] = lse;
+        if (n < a.n) {
+            if (a.loss) a.loss[n] = loss;
+            if (a.lse) a.lse[n] = lse;
+        }
+        double s = loss;
+#pragma unroll
+        for (int e = 8; e >= 1; e >>= 1) s += __shfl_xor(s, e);
+        if (t == 0) {
+            last = false;
+            if (a.total) {
+                a.sums[blockIdx.x] = s;
+                last = __hip_atomic_fetch_add(tk.count + 1, 1, __ATOMIC_ACQ_REL, __HIP_MEMORY_SCOPE_AGENT) ==
+                       (int)gridDim.x - 1;
+            }
+        }
+    }
+    __syncthreads();
+    if (!last) return;
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "agent");
+    double s = 0;
+    for (int i = t; i < (int)gridDim.x; i += 1024) s += a.sums[i];
+#pragma unroll
+    for (int e = 32; e >= 1; e >>= 1) s += __shfl_xor(s, e);
+    if ((t & 63) == 0) wsum[t >> 6] = s;
+    __syncthreads();
+    if (t == 0) {
+        s = 0;
+        for (int i = 0; i < 16; ++i) s += wsum[i];
+        *a.total = (float)(s / (a.mean ? max(*tk.count, 1) : 1));
     }
 }
 
 // Up to 64 tokens, none of them dropped before the product: one workgroup, 16 to 64 lanes a
 // token, which also adds the losses up
-__global__ void __launch_bounds__(1024) k_ce_join_few(JoinArgs a, EpiLse e, float* total, int mean) {
+__global__ void __launch_bounds__(1024) k_ce_join_few(JoinArgs a, EpiLse e) {
     __shared__ float2 red[1024];
     const int w = a.n <= 16 ? 16 : a.n <= 32 ? 32 : 64;
     const int t = threadIdx.x, tok = t & (w - 1), q = t / w, lanes = 1024 / w;
@@ -586,33 +623,18 @@ __global__ void __launch_bounds__(1024) k_ce_join_few(JoinArgs a, EpiLse e, floa
             loss = o.loss(zt);
             lse = zt + loss;
         }
-        a.loss[t] = loss;
-        a.lse[t] = lse;
+        if (a.loss) a.loss[t] = loss;
+        if (a.lse) a.lse[t] = lse;
     }
-    if (!total) return;
+    if (!a.total) return;
     double s = loss;
 #pragma unroll
     for (int k = 32; k >= 1; k >>= 1) s += __shfl_xor(s, k);
     const int count = __popcll(__ballot(kept));
-    if (t == 0) *total = (float)(s / (mean ? max(count, 1) : 1));
+    if (t == 0) *a.total = (float)(s / (a.mean ? max(count, 1) : 1));
 }
 
-// the losses' sum or mean, in a fixed order, in float64
-__global__ void __launch_bounds__(1024) k_ce_total(const float* loss, int64_t n, float* total, int mean,
-                                                   const int* count) {
-    __shared__ double red[16];
-    double s = 0;
-    for (int64_t i = threadIdx.x; i < n; i += 1024) s += loss[i];
-#pragma unroll
-    for (int o = 32; o >= 1; o >>= 1) s += __shfl_xor(s, o);
-    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = s;
-    __syncthreads();
-    if (threadIdx.x == 0) {
-        double all = 0;
-        for (int j = 0; j < 16; ++j) all += red[j];
-        *total = (float)(all / (mean ? max(*count, 1) : 1));
-    }
-}
+__global__ void k_ce_nothing(float* total) { *total = 0.f; }      // of no tokens
 
 struct DxArgs {
     const float* part;
@@ -704,34 +726,6 @@ template <typename T, class S> __global__ void __launch_bounds__(256) k_ce_dx_se
 size_t align256(size_t v) { return (v + 255) & ~size_t(255); }
 bool al16(const void* p) { return ((uintptr_t)p & 15) == 0; }
 
-// What the two entry points share: sizes, the packed operands and the tokens' arrays.
-struct Common {
-    int64_t n, vocab, dim, np, dp;
-    bool f32, pack_w;
-    size_t idx, inv, tgt, count, x, w, at;
-};
-
-Common common(int64_t n, int64_t vocab, int64_t dim, int64_t ldw, const void* w, int dtype) {
-    Common c{};
-    c.n = n; c.vocab = vocab; c.dim = dim;
-    c.np = (n + 63) / 64 * 64;
-    c.dp = (dim + 63) / 64 * 64;
-    c.f32 = dtype == M2_F32;
-    // the weights are read in place where direct loads can: bf16 rows of whole 16-byte
-    // pieces (and offsets within a tile that fit 32 bits), of whole K steps where the
-    // tokens are many (k_ce_tile); else a copy in the workspace
-    c.pack_w = c.f32 || dim % (n <= 64 ? 8 : 64) || ldw % 8 || !al16(w) || ldw > (1 << 22);
-    auto take = [&](size_t b) { const size_t r = c.at; c.at += align256(b); return r; };
-    c.idx = take(4 * (size_t)c.np);
-    c.inv = take(4 * (size_t)c.np);
-    c.tgt = take(4 * (size_t)c.np);
-    c.count = take(4);
-    const size_t planes = c.f32 ? 3 : 1;
-    c.x = take(2 * planes * (size_t)c.np * c.dp);
-    c.w = c.pack_w ? take(2 * planes * (size_t)vocab * c.dp) : c.at;
-    return c;
-}
-
 template <class S, class EPI> void launch(const Gemm& g, const EPI& e, hipStream_t s) {
     const int64_t tiles = (int64_t)g.tm * g.tn;
     if constexpr (S::BN < 128) {
@@ -754,18 +748,54 @@ template <bool F32> struct Shapes {
     typedef Shape<256, 64, 4, 1, 3, 64, true, false, T> X64;
     typedef Shape<256, 16, 4, 1, 3, 64, true, false, T> X16;
     typedef Shape<256, 256, 2, 4, 2, 64, true, true, T> W256;
+    typedef Shape<128, 64, 4, 1, 3, 64, true, true, T> W64;
 };
-// tokens of a tile
-int tok_tile(int64_t n) { return n <= 16 ? 16 : n <= 64 ? 64 : 256; }
-int voc_tile(int64_t n) { return n <= 64 ? 128 : 256; }
+// Tokens of a tile of the logits.  The tiles of 256 x 256 run at three times the rate of those of
+// 128 x 64, but where they leave more than half of the CUs without one, the small ones
+// are faster: 300 x 4000 x 333 f32, loss and gradients: 235 against 122 us.
+bool fills(int64_t m, int64_t n) { return 2 * (int64_t)tiles(m, 256) * tiles(n, 256) > m2::cu_count(); }
+int z_tile(int64_t n, int64_t vocab) { return n <= 16 ? 16 : n <= 64 || !fills(vocab, n) ? 64 : 256; }
+int z_rows(int z) { return z < 256 ? 128 : 256; }
 // parts of a tile whose sums EpiLse leaves apart
-int tile_parts(int64_t n) { return n <= 64 ? 1 : 2; }
+int z_parts(int z) { return z < 256 ? 1 : 2; }
 
-template <bool F32, class EPI> void launch_z(Gemm& g, int64_t rows, int64_t n, const EPI& e, hipStream_t s) {
+// What the two entry points share: sizes, the packed operands and the tokens' arrays.
+struct Common {
+    int64_t n, vocab, dim, np, dp;
+    bool f32, pack_w;
+    size_t idx, inv, tgt, lse, em1, count, x, w, at;
+    int z;                   // tokens of a tile of the logits
+};
+
+Common common(int64_t n, int64_t vocab, int64_t dim, int64_t ldw, const void* w, int dtype) {
+    Common c{};
+    c.n = n; c.vocab = vocab; c.dim = dim;
+    c.np = (n + 63) / 64 * 64;
+    c.dp = (dim + 63) / 64 * 64;
+    c.f32 = dtype == M2_F32;
+    c.z = z_tile(n, vocab);
+    // the weights are read in place where direct loads can: bf16 rows of whole 16-byte
+    // pieces (and offsets within a tile that fit 32 bits), of whole K steps for k_ce_tile; else
+    // a copy in the workspace
+    c.pack_w = c.f32 || dim % (c.z < 256 ? 8 : 64) || ldw % 8 || !al16(w) || ldw > (1 << 22);
+    auto take = [&](size_t b) { const size_t r = c.at; c.at += align256(b); return r; };
+    c.idx = take(4 * (size_t)c.np);
+    c.inv = take(4 * (size_t)c.np);
+    c.tgt = take(4 * (size_t)c.np);
+    c.lse = take(4 * (size_t)c.np);
+    c.em1 = take(4 * (size_t)c.np);
+    c.count = take(8);
+    const size_t planes = c.f32 ? 3 : 1;
+    c.x = take(2 * planes * (size_t)c.np * c.dp);
+    c.w = c.pack_w ? take(2 * planes * (size_t)vocab * c.dp) : c.at;
+    return c;
+}
+
+template <bool F32, class EPI> void launch_z(Gemm& g, int z, int64_t rows, int64_t n, const EPI& e, hipStream_t s) {
     typedef Shapes<F32> P;
-    g.tm = tiles(rows, voc_tile(n));
-    g.tn = tiles(n, tok_tile(n));
-    switch (tok_tile(n)) {
+    g.tm = tiles(rows, z_rows(z));
+    g.tn = tiles(n, z);
+    switch (z) {
         case 16: launch<typename P::Z16>(g, e, s); break;
         case 64: launch<typename P::Z64>(g, e, s); break;
         default: launch<typename P::Z256>(g, e, s);
@@ -789,16 +819,17 @@ int check_sizes(const char* who, int64_t n, int64_t vocab, int64_t dim, int64_t 
 struct FwdPlan {
     Common c;
     bool direct;             // x read in place, nothing packed: few tokens
-    size_t zt, part, total;
+    size_t zt, part, sums, total;
 };
 FwdPlan fwd_plan(const m2_linear_cross_entropy_args& a) {
     FwdPlan p{};
     p.c = common(a.n, a.vocab, a.dim, a.ldw, a.weight, a.dtype);
-    p.direct = a.n <= 64 && !p.c.pack_w && a.ldx % 8 == 0 && al16(a.x);
+    p.direct = a.n <= 64 && !a.saved && !p.c.pack_w && a.ldx % 8 == 0 && al16(a.x);
     size_t at = p.direct || a.saved ? 0 : p.c.at;
     auto take = [&](size_t b) { const size_t r = at; at += align256(b); return r; };
     p.zt = take(4 * (size_t)p.c.np);
-    p.part = take(8 * (size_t)tile_parts(a.n) * tiles(a.vocab, voc_tile(a.n)) * p.c.np);
+    p.part = take(8 * (size_t)z_parts(p.c.z) * tiles(a.vocab, z_rows(p.c.z)) * p.c.np);
+    p.sums = take(8 * (size_t)tiles(a.n, 16));
     p.total = at ? at : 256;
     return p;
 }
@@ -809,17 +840,15 @@ constexpr int64_t G_BYTES = 512ll << 20;
 struct BwdPlan {
     Common c;
     int64_t piece;
-    int pieces, splits;      // of K for dx: parts (few tokens) or workgroups (many)
-    size_t lse, gf, gm, G, dx, total;
+    int pieces;
+    int x, splits;           // dx: tokens of a tile; parts of K (few tokens) or workgroups (many)
+    size_t G, dx, total;
 };
 BwdPlan bwd_plan(const m2_linear_cross_entropy_grad_args& a) {
     BwdPlan p{};
     p.c = common(a.n, a.vocab, a.dim, a.ldw, a.weight, a.dtype);
     size_t at = a.saved ? 0 : p.c.at;
     auto take = [&](size_t b) { const size_t r = at; at += align256(b); return r; };
-    p.lse = take(4 * (size_t)p.c.np);
-    p.gf = take(4 * (size_t)p.c.np);
-    p.gm = take(4 * (size_t)p.c.np);
     const int planes = p.c.f32 ? 3 : 1;
     const int64_t all = (a.vocab + 255) / 256 * 256;
     int64_t most = G_BYTES / (2 * planes * (p.c.np ? p.c.np : 64)) / 256 * 256;
@@ -832,21 +861,26 @@ BwdPlan bwd_plan(const m2_linear_cross_entropy_grad_args& a) {
     // depends on the tokens that are kept.  Few: split so that the tiles fill the CUs; a
     // split costs a float32 array of dx, written and read once per piece
     const int ncu = m2::cu_count();
-    const int tm = tiles(a.dim, 256), tn = tiles(a.n ? a.n : 1, tok_tile(a.n));
-    const int64_t t = (int64_t)tm * tn;
     const int steps = (int)((a.vocab < p.piece ? a.vocab + 63 : p.piece) / 64);
+    const int tm = tiles(a.dim, 256);
+    p.x = a.n <= 16 ? 16 : 64;
     if (a.n > 64) {
+        const int tn = tiles(a.n, 256);
         p.splits = ncu;
-        int64_t segs = 0;
+        int64_t segs = 0, all_segs = 0;
         for (int k = 1; k <= tn; ++k) {
             const Deal d = deal(tm * k, steps, ncu);
-            const int64_t c = d.full + (int64_t)d.rest * d.s;
-            if (c > segs) segs = c;
+            all_segs = d.full + (int64_t)d.rest * d.s;
+            if (all_segs > segs) segs = all_segs;
         }
-        p.dx = a.grad_x ? take(4 * 256 * 256 * (size_t)segs) : 0;
-        p.total = at;
-        return p;
+        if (2 * all_segs > ncu) {             // else the smaller tiles, as for the logits
+            p.x = 256;
+            p.dx = a.grad_x ? take(4 * 256 * 256 * (size_t)segs) : 0;
+            p.total = at;
+            return p;
+        }
     }
+    const int64_t t = (int64_t)tm * tiles(a.n ? a.n : 1, p.x);
     double best = 1e300;
     p.splits = 1;
     for (int s = 1; s <= 64 && s * 4 <= steps; ++s) {
@@ -864,6 +898,8 @@ Tokens tokens(char* ws, const Common& c) {
     t.idx = reinterpret_cast<int*>(ws + c.idx);
     t.inv = reinterpret_cast<int*>(ws + c.inv);
     t.tgt = reinterpret_cast<int*>(ws + c.tgt);
+    t.lse = reinterpret_cast<float*>(ws + c.lse);
+    t.em1 = reinterpret_cast<float*>(ws + c.em1);
     t.count = reinterpret_cast<int*>(ws + c.count);
     return t;
 }
@@ -872,10 +908,11 @@ template <typename T>
 void pack(char* ws, const Common& c, const void* x, int64_t ldx, const void* w, int64_t ldw, PackArgs a,
           const Tokens& tk, int64_t ignore, hipStream_t s) {
     a.n = c.n; a.ignore = ignore;
-    if (c.n > 64) hipLaunchKernelGGL(k_ce_compact, dim3(1), dim3(1024), 0, s, a.targets, c.n, ignore, a.t64, tk);
+    const bool finds = c.n <= PACK_FINDS;
+    if (!finds) hipLaunchKernelGGL(k_ce_compact, dim3(1), dim3(1024), 0, s, a.targets, c.n, ignore, a.t64, tk);
     a.dim = c.dim; a.dp = c.dp;
     a.src = x; a.ld = ldx; a.dst = reinterpret_cast<bf16*>(ws + c.x); a.rows = c.np; a.plane = c.np * c.dp;
-    hipLaunchKernelGGL((k_ce_pack<T, true>), dim3((unsigned)(c.np / 4)), dim3(256), 0, s, a, tk);
+    hipLaunchKernelGGL((k_ce_pack<T, true>), dim3((unsigned)((finds ? c.n + 67 : c.np) / 4)), dim3(256), 0, s, a, tk);
     if (c.pack_w) {
         a.src = w; a.ld = ldw; a.dst = reinterpret_cast<bf16*>(ws + c.w); a.rows = c.vocab;
         a.plane = c.vocab * c.dp;
@@ -899,14 +936,14 @@ template <bool F32> int run_fwd(const m2_linear_cross_entropy_args& a, const Fwd
     Gemm g{};
     g.tok_n = 1; g.splits = 1;
     g.nk = (int)(c.dp / 64);
-    JoinArgs j{e.part, c.np, c.n, a.loss, a.lse, 0};
+    JoinArgs j{e.part, c.np, c.n, a.loss, a.lse, a.total, reinterpret_cast<double*>(ws + p.sums), 0, a.mean};
     if (p.direct) {
         g.n = (int)c.n;
         g.a = Operand{static_cast<const bf16*>(a.weight), a.ldw, 0, (int)c.vocab, (int)c.dim};
         g.b = Operand{static_cast<const bf16*>(a.x), a.ldx, 0, (int)c.n, (int)c.dim};
-        launch_z<F32>(g, c.vocab, c.n, e, s);
+        launch_z<F32>(g, c.z, c.vocab, c.n, e, s);
         j.parts = g.tm;
-        hipLaunchKernelGGL(k_ce_join_few, dim3(1), dim3(1024), 0, s, j, e, a.total, a.mean);
+        hipLaunchKernelGGL(k_ce_join_few, dim3(1), dim3(1024), 0, s, j, e);
         return m2::check_launch("linear_cross_entropy");
     }
     Tokens tk = tokens(cm, c);
@@ -920,11 +957,9 @@ template <bool F32> int run_fwd(const m2_linear_cross_entropy_args& a, const Fwd
     g.a.klim = (int)(c.pack_w ? c.dp : c.dim);
     g.b = Operand{reinterpret_cast<bf16*>(cm + c.x), c.dp, c.np * c.dp, (int)c.np, (int)c.dp};
     e.tgt = tk.tgt;
-    launch_z<F32>(g, c.vocab, c.n, e, s);
-    j.parts = g.tm * tile_parts(c.n);
-    hipLaunchKernelGGL(k_ce_join, dim3((unsigned)((c.n + 15) / 16)), dim3(256), 0, s, j, tk);
-    if (a.total)
-        hipLaunchKernelGGL(k_ce_total, dim3(1), dim3(1024), 0, s, a.loss, c.n, a.total, a.mean, tk.count);
+    launch_z<F32>(g, c.z, c.vocab, c.n, e, s);
+    j.parts = g.tm * z_parts(c.z);
+    hipLaunchKernelGGL(k_ce_join, dim3((unsigned)tiles(c.n, 16)), dim3(1024), 0, s, j, tk);
     return m2::check_launch("linear_cross_entropy");
 }
 
@@ -935,14 +970,10 @@ template <bool F32> int run_bwd(const m2_linear_cross_entropy_grad_args& a, cons
     char* cm = a.saved ? static_cast<char*>(a.saved) : ws;
     const Common& c = p.c;
     Tokens tk = tokens(cm, c);
-    tk.lse = reinterpret_cast<float*>(ws + p.lse);
-    tk.gf = reinterpret_cast<float*>(ws + p.gf);
-    tk.gm = reinterpret_cast<float*>(ws + p.gm);
     PackArgs pa{};
     pa.targets = a.targets; pa.vocab = a.vocab; pa.t64 = a.target_dtype == M2_I64;
-    pa.lse = a.lse; pa.loss = a.loss; pa.g = a.grad_loss; pa.gstride = a.grad_loss_stride; pa.mean = a.mean;
-    if (a.saved) hipLaunchKernelGGL(k_ce_tokens, dim3((unsigned)((c.np + 255) / 256)), dim3(256), 0, s, pa, tk);
-    else pack<T>(cm, c, a.x, a.ldx, a.weight, a.ldw, pa, tk, a.ignore_index, s);
+    pa.lse = a.lse; pa.loss = a.loss;
+    if (!a.saved) pack<T>(cm, c, a.x, a.ldx, a.weight, a.ldw, pa, tk, a.ignore_index, s);
     const Operand w = operand_w(cm, c, a.weight, a.ldw);
     bf16* G = reinterpret_cast<bf16*>(ws + p.G);
     const int64_t gplane = c.np * p.piece;
@@ -962,8 +993,8 @@ template <bool F32> int run_bwd(const m2_linear_cross_entropy_grad_args& a, cons
         g.a.lim = (int)rows;
         g.a.klim = wlim;
         g.b = Operand{reinterpret_cast<bf16*>(cm + c.x), c.dp, c.np * c.dp, (int)c.np, (int)c.dp};
-        EpiG eg{tk.tgt, tk.lse, tk.gf, tk.gm, G, p.piece, gplane, (int)v0, (int)c.vocab};
-        launch_z<F32>(g, (rows + 63) / 64 * 64, c.n, eg, s);
+        const EpiG eg{tk, a.grad_loss, G, p.piece, gplane, a.grad_loss_stride, (int)v0, (int)c.vocab, a.mean};
+        launch_z<F32>(g, c.z, (rows + 63) / 64 * 64, c.n, eg, s);
         if (a.grad_x) {
             Gemm d = g0;
             d.nk = (int)((rows + 63) / 64); d.tok_n = 1;
@@ -974,8 +1005,8 @@ template <bool F32> int run_bwd(const m2_linear_cross_entropy_grad_args& a, cons
             d.a.klim = (int)rows;
             d.b = Operand{G, p.piece, gplane, (int)c.np, (int)p.piece};
             d.tm = tiles(c.dim, 256);
-            d.tn = tiles(c.n, tok_tile(c.n));
-            if (c.n > 64) {
+            d.tn = tiles(c.n, p.x);
+            if (p.x == 256) {
                 if (q == 0) dxs.seg_nk = d.nk;
                 d.seg_nk = dxs.seg_nk;
                 launch<typename P::X256>(d, EpiDxSeg{dxp, q > 0}, s);
@@ -983,7 +1014,7 @@ template <bool F32> int run_bwd(const m2_linear_cross_entropy_grad_args& a, cons
             } else {
                 if (d.splits > d.nk) d.splits = d.nk;             // a short last piece
                 const EpiDxSplit e{dxp, c.np, c.dp, q > 0};
-                if (c.n <= 16) launch<typename P::X16>(d, e, s);
+                if (p.x == 16) launch<typename P::X16>(d, e, s);
                 else launch<typename P::X64>(d, e, s);
             }
         }
@@ -991,16 +1022,20 @@ template <bool F32> int run_bwd(const m2_linear_cross_entropy_grad_args& a, cons
             Gemm d = g0;
             d.nk = 0;
             d.a = Operand{reinterpret_cast<bf16*>(cm + c.x), c.dp, c.np * c.dp, (int)c.dp, (int)c.np};
-            // rows of G past the last token tile are not there: its last row stands for
-            // them, against zero rows of x
-            d.b = Operand{G, p.piece, gplane, (int)p.piece, tiles(c.n, tok_tile(c.n)) * tok_tile(c.n)};
-            d.tm = tiles(c.dim, 256);
-            d.tn = tiles(rows, 256);
+            // rows of G past a tile of 16 tokens are not there: its last row stands for them,
+            // against zero rows of x
+            d.b = Operand{G, p.piece, gplane, (int)p.piece, c.z == 16 ? 16 : (int)c.np};
             EpiDw<T> e{static_cast<T*>(a.grad_weight) + v0 * c.dim, c.dim, (int)rows};
-            launch<typename P::W256>(d, e, s);
+            if (fills(c.dim, rows)) {
+                d.tm = tiles(c.dim, 256); d.tn = tiles(rows, 256);
+                launch<typename P::W256>(d, e, s);
+            } else {
+                d.tm = tiles(c.dim, 128); d.tn = tiles(rows, 64);
+                launch<typename P::W64>(d, e, s);
+            }
         }
     }
-    if (a.grad_x && c.n > 64) {
+    if (a.grad_x && p.x == 256) {
         typedef typename P::X256 S;
         dxs.part = dxp; dxs.dx = a.grad_x; dxs.n = c.n; dxs.dim = c.dim;
         dxs.nred = dxs.tm * dxs.tn * (S::NW * S::FM * S::FN / 2 / 4);
@@ -1020,7 +1055,7 @@ namespace m2 {
 
 size_t linear_ce_saved(const m2_linear_cross_entropy_args& a) {
     if (check_sizes("linear_cross_entropy", a.n, a.vocab, a.dim, a.ldx, a.ldw, a.dtype, a.target_dtype)) return 0;
-    return a.n <= 64 ? 0 : common(a.n, a.vocab, a.dim, a.ldw, a.weight, a.dtype).at;
+    return common(a.n, a.vocab, a.dim, a.ldw, a.weight, a.dtype).at;
 }
 
 size_t linear_ce_workspace(const m2_linear_cross_entropy_args& a) {
@@ -1031,16 +1066,15 @@ size_t linear_ce_workspace(const m2_linear_cross_entropy_args& a) {
 int launch_linear_ce(const m2_linear_cross_entropy_args& a, hipStream_t s) {
     const char* who = "linear_cross_entropy";
     if (int rc = check_sizes(who, a.n, a.vocab, a.dim, a.ldx, a.ldw, a.dtype, a.target_dtype)) return rc;
-    M2_REQUIRE(a.weight && (a.n == 0 || (a.x && a.targets && a.loss && a.lse)), M2_ERR_INVALID,
-               "%s: x, weight, targets, loss and lse are required", who);
+    M2_REQUIRE(a.weight && (a.n == 0 || (a.x && a.targets)) && (a.loss || a.total), M2_ERR_INVALID,
+               "%s: x, weight, targets and loss or total are required", who);
     const FwdPlan p = fwd_plan(a);
     M2_REQUIRE(a.workspace && a.workspace_bytes >= p.total, M2_ERR_WORKSPACE,
                "%s: workspace of %zu bytes needed, %zu given", who, p.total, a.workspace_bytes);
-    M2_REQUIRE(!a.saved || (a.n > 64 && a.saved_bytes >= p.c.at), M2_ERR_WORKSPACE,
-               "%s: saved of %zu bytes needed (none for up to 64 rows), %zu given", who, a.n > 64 ? p.c.at : 0,
-               a.saved_bytes);
+    M2_REQUIRE(!a.saved || a.saved_bytes >= p.c.at, M2_ERR_WORKSPACE, "%s: saved of %zu bytes needed, %zu given",
+               who, p.c.at, a.saved_bytes);
     if (a.n == 0) {
-        if (a.total) hipLaunchKernelGGL(k_ce_total, dim3(1), dim3(1024), 0, s, a.loss, (int64_t)0, a.total, 0, nullptr);
+        if (a.total) hipLaunchKernelGGL(k_ce_nothing, dim3(1), dim3(1), 0, s, a.total);
         return check_launch(who);
     }
     return a.dtype == M2_F32 ? run_fwd<true>(a, p, s) : run_fwd<false>(a, p, s);
@@ -1056,13 +1090,14 @@ int launch_linear_ce_grad(const m2_linear_cross_entropy_grad_args& a, hipStream_
     const char* who = "linear_cross_entropy_grad";
     if (int rc = check_sizes(who, a.n, a.vocab, a.dim, a.ldx, a.ldw, a.dtype, a.target_dtype)) return rc;
     M2_REQUIRE(a.n > 0, M2_ERR_INVALID, "%s: no tokens", who);
-    M2_REQUIRE(a.weight && a.x && a.targets && a.loss && a.lse && a.grad_loss && (a.grad_x || a.grad_weight),
-               M2_ERR_INVALID, "%s: x, weight, targets, loss, lse, grad_loss and an output are required", who);
+    M2_REQUIRE(a.weight && a.grad_loss && (a.grad_x || a.grad_weight), M2_ERR_INVALID,
+               "%s: weight, grad_loss and an output are required", who);
+    M2_REQUIRE(a.saved || (a.x && a.targets && a.loss && a.lse), M2_ERR_INVALID,
+               "%s: saved, or x, targets, loss and lse are required", who);
     M2_REQUIRE(a.grad_loss_stride >= 0, M2_ERR_INVALID, "%s: grad_loss stride", who);
     const BwdPlan p = bwd_plan(a);
-    M2_REQUIRE(!a.saved || (a.n > 64 && a.saved_bytes >= p.c.at), M2_ERR_WORKSPACE,
-               "%s: saved of %zu bytes needed (none for up to 64 rows), %zu given", who, a.n > 64 ? p.c.at : 0,
-               a.saved_bytes);
+    M2_REQUIRE(!a.saved || a.saved_bytes >= p.c.at, M2_ERR_WORKSPACE, "%s: saved of %zu bytes needed, %zu given",
+               who, p.c.at, a.saved_bytes);
     M2_REQUIRE(a.workspace && a.workspace_bytes >= p.total, M2_ERR_WORKSPACE,
                "%s: workspace of %zu bytes needed, %zu given", who, p.total, a.workspace_bytes);
     return a.dtype == M2_F32 ? run_bwd<true>(a, p, s) : run_bwd<false>(a, p, s);

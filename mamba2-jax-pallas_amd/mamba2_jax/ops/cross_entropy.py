@@ -20,62 +20,65 @@ REDUCTIONS = ("mean", "sum", "none")
 
 
 def _forward(x, weight, targets, ignore_index, reduction, save):
-    """-> (per-position losses, lse, their reduction or None, contiguous targets, what the
-    gradient need not prepare again or None)"""
+    """-> (the reduction, or the per-position losses; what the gradient reads, or None)"""
     dev, dim = x.device, x.shape[-1]
     xr, w, t = _rows(x, dim), _rows(weight, dim), _dense(targets)
-    loss = torch.empty(targets.shape, dtype=torch.float32, device=dev)
-    lse = torch.empty(targets.shape, dtype=torch.float32, device=dev)
-    total = None if reduction == "none" else torch.empty((), dtype=torch.float32, device=dev)
+    none = reduction == "none"
+    out = torch.empty(targets.shape if none else (), dtype=torch.float32, device=dev)
     args = L.LinearCrossEntropyArgs(
-        xr.data_ptr(), w.data_ptr(), t.data_ptr(), loss.data_ptr(), lse.data_ptr(), L.ptr(total),
-        t.numel(), w.shape[0], dim, _stride(xr, dim), _stride(w, dim), int(ignore_index),
-        L.dtype_code(w, "weight"), L.index_code(t, "targets"), int(reduction == "mean"))
+        xr.data_ptr(), w.data_ptr(), t.data_ptr(), out.data_ptr() if none else 0, 0,
+        0 if none else out.data_ptr(), t.numel(), w.shape[0], dim, _stride(xr, dim),
+        _stride(w, dim), ignore_index, L.dtype_code(w, "weight"), L.index_code(t, "targets"),
+        int(reduction == "mean"))
+    if none and not t.numel():
+        return out, None
     saved = None
     if save:
         size = L.size_of("m2_linear_cross_entropy_saved_size", args)
-        if size:
-            saved = torch.empty(size, dtype=torch.uint8, device=dev)
-            args.saved, args.saved_bytes = saved.data_ptr(), size
+        saved = torch.empty(size, dtype=torch.uint8, device=dev)
+        args.saved, args.saved_bytes = saved.data_ptr(), size
     L.call_with_workspace("m2_linear_cross_entropy", args, dev)
-    return loss, lse, total, t, saved
+    return out, saved
+
+
+def _backward(ctx, grad):
+    weight, saved = ctx.saved_tensors
+    shape, n, ignore_index, reduction, index_code = ctx.args
+    want_x, want_w = ctx.needs_input_grad[:2]
+    dev, dim = weight.device, weight.shape[1]
+    dx = torch.empty(shape, dtype=weight.dtype, device=dev) if want_x else None
+    dw = torch.empty(weight.shape, dtype=weight.dtype, device=dev) if want_w else None
+    if n == 0:
+        return dx, None if dw is None else dw.zero_(), None, None, None
+    w = _rows(weight, dim)
+    g = grad.reshape(-1) if grad.dim() != 1 else grad
+    if g.dtype != torch.float32:
+        g = g.float()
+    args = L.LinearCrossEntropyGradArgs(
+        0, w.data_ptr(), 0, 0, 0, g.data_ptr(), L.ptr(dx), L.ptr(dw), n, w.shape[0], dim, dim,
+        _stride(w, dim), ignore_index, 0 if reduction != "none" else g.stride(0),
+        L.dtype_code(w, "weight"), index_code, int(reduction == "mean"))
+    args.saved, args.saved_bytes = saved.data_ptr(), saved.numel()
+    L.call_with_workspace("m2_linear_cross_entropy_grad", args, dev)
+    return dx, dw, None, None, None
+
+
+_backward_once = once_differentiable(_backward)
 
 
 class _LinearCrossEntropy(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, targets, ignore_index, reduction):
-        loss, lse, total, t, saved = _forward(x, weight, targets, ignore_index, reduction, True)
-        # the per-token losses are the result where nothing is reduced: what the backward
-        # reads is then a copy, which the caller's in-place changes do not reach
-        ctx.save_for_backward(x, weight, t, loss.clone() if total is None else loss, lse, saved)
-        ctx.args = int(ignore_index), reduction
-        return loss if total is None else total
+        out, saved = _forward(x, weight, targets, ignore_index, reduction, True)
+        # (x is not read again: its kept rows are in `saved`)
+        ctx.save_for_backward(weight, saved)
+        ctx.args = x.shape, targets.numel(), ignore_index, reduction, L.index_code(targets, "targets")
+        return out
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, grad):
-        x, weight, t, loss, lse, saved = ctx.saved_tensors
-        ignore_index, reduction = ctx.args
-        want_x, want_w = ctx.needs_input_grad[:2]
-        dev, dim = x.device, x.shape[-1]
-        dx = torch.empty(x.shape, dtype=x.dtype, device=dev) if want_x else None
-        dw = torch.empty(weight.shape, dtype=weight.dtype, device=dev) if want_w else None
-        n = t.numel()
-        if n == 0:
-            return dx, None if dw is None else dw.zero_(), None, None, None
-        xr, w = _rows(x, dim), _rows(weight, dim)
-        g = grad.reshape(-1)
-        if g.dtype != torch.float32:
-            g = g.float()
-        args = L.LinearCrossEntropyGradArgs(
-            xr.data_ptr(), w.data_ptr(), t.data_ptr(), loss.data_ptr(), lse.data_ptr(), g.data_ptr(),
-            L.ptr(dx), L.ptr(dw), n, w.shape[0], dim, _stride(xr, dim), _stride(w, dim),
-            ignore_index, 0 if reduction != "none" else g.stride(0), L.dtype_code(w, "weight"),
-            L.index_code(t, "targets"), int(reduction == "mean"))
-        if saved is not None:
-            args.saved, args.saved_bytes = saved.data_ptr(), saved.numel()
-        L.call_with_workspace("m2_linear_cross_entropy_grad", args, dev)
-        return dx, dw, None, None, None
+        # (once_differentiable's own bookkeeping only where a second derivative is recorded)
+        return (_backward_once if torch.is_grad_enabled() else _backward)(ctx, grad)
 
 
 def linear_cross_entropy(x, weight, targets, ignore_index=-100, reduction="mean"):
@@ -95,9 +98,9 @@ def linear_cross_entropy(x, weight, targets, ignore_index=-100, reduction="mean"
     operands round it to bfloat16 before its products with weight and x (float32
     sums, each result rounded once); float32 operands are multiplied as three
     bfloat16 parts each, accurate to about 2^-24 of each product.  Between the two the
-    graph holds the positions' losses and what the kernels read: a packed
-    copy of x's kept rows, and of weight where it cannot be read in place (float32, as
-    three bfloat16 parts: 1.5 times weight; a dim that 64 does not divide)."""
+    graph holds what the kernels read: a packed copy of x's kept rows, and of weight
+    where it cannot be read in place (float32, as three bfloat16 parts: 1.5 times
+    weight; a dim that 64 does not divide)."""
     L.device_of(x, weight, targets)
     L.require(reduction in REDUCTIONS, lambda: f"reduction={reduction!r}: one of {REDUCTIONS}")
     L.require(weight.dim() == 2 and x.dim() >= 1 and x.shape[-1] == weight.shape[1],
@@ -109,10 +112,10 @@ def linear_cross_entropy(x, weight, targets, ignore_index=-100, reduction="mean"
     L.index_code(targets, "targets")
     if L.dtype_code(x, "x") != L.dtype_code(weight, "weight"):
         raise TypeError(f"x is {x.dtype} and weight {weight.dtype}: they must be the same")
+    ignore_index = int(ignore_index)
     if (x.requires_grad or weight.requires_grad) and torch.is_grad_enabled():
         return _LinearCrossEntropy.apply(x, weight, targets, ignore_index, reduction)
-    loss, _, total, _, _ = _forward(x, weight, targets, ignore_index, reduction, False)
-    return loss if total is None else total
+    return _forward(x, weight, targets, ignore_index, reduction, False)[0]
 
 
 __all__ = ["linear_cross_entropy"]

@@ -50,19 +50,23 @@ struct Gemm {
 // one; full + part * rest + (tile - full).
 struct Deal {
     int full, rest, s;
+    int64_t cost;            // 5 ns
 };
-__host__ __device__ inline Deal deal(int tiles, int nk, int nwg) {
+// bn: the tile's n, 256 or 128
+__host__ __device__ inline Deal deal(int tiles, int nk, int nwg, int bn) {
+    // a step takes about 1.4 us (0.85 us), writing and reading a segment of 256 KB the chip
+    // 0.11 us (whole numbers: the host sizes the workspace by the same)
+    const int step = bn == 256 ? 280 : 170, seg = bn == 256 ? 22 : 11;
     Deal d;
     d.full = tiles / nwg * nwg;
     d.rest = tiles - d.full;
     d.s = 1;
-    // a step takes about 1.4 us, writing and reading a segment of 256 KB the chip 0.11 us
-    // (whole numbers: the host sizes the workspace by the same)
-    int64_t best = INT64_MAX;
-    for (int s = 1; s <= 64 && s * 4 <= nk && d.rest * s <= 2 * nwg; ++s) {
-        const int64_t cost = (int64_t)140 * ((d.rest * s + nwg - 1) / nwg) * ((nk + s - 1) / s) + 11 * d.rest * s;
-        if (cost < best) { best = cost; d.s = s; }
+    d.cost = INT64_MAX;
+    for (int s = 1; s <= 64 && (s == 1 || (s * 4 <= nk && d.rest * s <= 2 * nwg)); ++s) {
+        const int64_t cost = (int64_t)step * ((d.rest * s + nwg - 1) / nwg) * ((nk + s - 1) / s) + (int64_t)seg * d.rest * s;
+        if (cost < d.cost) { d.cost = cost; d.s = s; }
     }
+    d.cost += (int64_t)(d.full / nwg) * nk * step + (int64_t)seg * d.full;
     return d;
 }
 
@@ -301,8 +305,8 @@ __global__ void __launch_bounds__(S::NT, S::NT / 256) k_ce_tile(Gemm g, EPI epi)
     const int before = xcd * (nwg >> 3) + min(xcd, nwg & 7);
     // whole tiles one workgroup after the other; each XCD a contiguous range, which its
     // share of the workgroups gives
-    Deal dl{0, tiles, 1};
-    if constexpr (EPI::SEG) dl = deal(tiles, g.seg_nk, nwg);
+    Deal dl{0, tiles, 1, 0};
+    if constexpr (EPI::SEG) dl = deal(tiles, g.seg_nk, nwg, S::BN);
     const int f0 = dl.full / nwg * before + local, rounds = dl.full / nwg;
     const int64_t cut = (int64_t)dl.rest * dl.s;
     const int r0 = (int)(cut * before / nwg) + local, r1 = (int)(cut * (before + lw) / nwg);

@@ -2,38 +2,56 @@
 // times min(1, max_norm / (norm + eps)).
 //
 // Bound by HBM: every tensor is read for the norm and read again and written for the
-// result (the scale is not known before the last value is).  The tensors
-// travel as a table in the kernel's arguments, up to 96 per launch; a
-// launch's workgroups share its elements evenly whatever the tensors' sizes
-// (pieces of 16384 elements, a contiguous range of pieces per workgroup), so one large
-// embedding and a hundred small vectors take one pass.  The squares
-// are summed in float64 per thread (the vector units do that well
-// above the rate at which HBM brings the values in): no square overflows and long
-// sums lose nothing, and the order is fixed, so equal inputs give equal
-// bits.  The second pass walks the pieces in the opposite order: what the first pass read
-// last is still in the 256 MB last-level cache.
+// result (the scale is not known before the last value is).  The tensors' table goes to
+// the workspace through kernel arguments, 136 at a time (a copy from the host would
+// neither be captured into a graph nor run without waiting); then one launch
+// reads everything and one scales it, so that one large embedding and a hundred small
+// vectors take one pass.  The workgroups share the tensors' pieces of 16 KB evenly,
+// a contiguous range each.  The squares are summed in float64 per thread (the vector
+// units do that well above the rate at which HBM brings the values in): no square
+// overflows and long sums lose nothing, and the order is fixed, so equal inputs give equal
+// bits.  Every workgroup of the second pass adds the first one's sums up by itself,
+// and walks its pieces in the opposite order: what the first pass read last is still in the
+// 256 MB last-level cache.
 #include "m2_internal.h"
 
 namespace {
 
 constexpr int NT = 256;               // threads of a workgroup
-constexpr int MAXT = 96;              // tensors per launch (the table stays below 4 KB)
-constexpr int PIECE = 16384;          // elements
-constexpr int MAXWG = 2048;           // workgroups per launch
+constexpr int BATCH = 136;            // table entries that travel with one launch (below 4 KB)
+constexpr int PIECE_BYTES = 16 << 10;
+constexpr int MAXWG = 2048;           // 8 workgroups on each CU
 
-struct Table {
-    const void* in[MAXT];
-    void* out[MAXT];
-    int64_t n[MAXT];
-    int first[MAXT + 1];              // first piece of each tensor
-    uint8_t bf[MAXT];
+struct Entry {
+    const void* in;
+    void* out;
+    int64_t n;
+    int64_t first;                    // number of pieces before this tensor
+    int64_t bf;
+};
+struct Batch {
+    const void* in[BATCH];
+    void* out[BATCH];
+    int64_t n[BATCH];                 // ~n: bf16
+    uint32_t first[BATCH];            // behind base
+    int64_t base;
     int count;
 };
-
 struct PassArgs {
-    double* part;                     // this launch's partial sums
-    const float* norm;                // [norm, scale] (second pass)
+    const Entry* table;
+    int64_t count, pieces;
+    double* part;                     // sums of the first pass, one a workgroup
+    float* norm;                      // out
+    float max_norm, eps;
+    int parts;
 };
+
+__global__ void __launch_bounds__(256) k_table(Batch b, Entry* to) {
+    const int i = threadIdx.x;
+    if (i >= b.count) return;
+    const int64_t n = b.n[i];
+    to[i] = Entry{b.in[i], b.out[i], n < 0 ? ~n : n, b.base + b.first[i], n < 0};
+}
 
 M2_DEV double block_sum(double v, double* red) {
 #pragma unroll
@@ -41,19 +59,24 @@ M2_DEV double block_sum(double v, double* red) {
     if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
     __syncthreads();
     double s = 0;
-    for (int j = 0; j < (int)(blockDim.x >> 6); ++j) s += red[j];
+#pragma unroll
+    for (int j = 0; j < NT / 64; ++j) s += red[j];
     __syncthreads();
     return s;
 }
 
-// The tensor that piece p belongs to
-M2_DEV int find(const Table& tb, int p) {
-    int lo = 0, hi = tb.count - 1;
-    while (lo < hi) {
-        const int m = (lo + hi + 1) >> 1;
-        if (tb.first[m] <= p) lo = m; else hi = m - 1;
-    }
-    return lo;
+// The tensor that piece p belongs to: the number of tensors that begin at or before it
+M2_DEV int64_t find(const PassArgs& a, int64_t p, int* red) {
+    int c = 0;
+    for (int64_t i = threadIdx.x; i < a.count; i += NT) c += a.table[i].first <= p;
+#pragma unroll
+    for (int o = 32; o >= 1; o >>= 1) c += __shfl_xor(c, o);
+    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = c;
+    __syncthreads();
+    int s = 0;
+#pragma unroll
+    for (int j = 0; j < NT / 64; ++j) s += red[j];
+    return __builtin_amdgcn_readfirstlane(s - 1);
 }
 
 // Elements [i0, i1) of a tensor: single ones up to a 16-byte boundary of `p`, whole
@@ -73,19 +96,22 @@ M2_DEV void walk(const void* p, int es, int64_t i0, int64_t i1, F1 f1, FV fv) {
     if (tail + t < i1) f1(tail + t);
 }
 
-__global__ void __launch_bounds__(NT) k_sumsq(Table tb, PassArgs a) {
+__global__ void __launch_bounds__(NT) k_sumsq(PassArgs a) {
     __shared__ double red[NT / 64];
-    const int np = tb.first[tb.count];
-    const int per = (np + gridDim.x - 1) / gridDim.x;
-    const int p0 = blockIdx.x * per, p1 = min(np, p0 + per);
+    __shared__ int found[NT / 64];
+    const int64_t p0 = a.pieces * blockIdx.x / gridDim.x, p1 = a.pieces * (blockIdx.x + 1) / gridDim.x;
     double s = 0;
-    int ti = p0 < p1 ? find(tb, p0) : 0;
-    for (int p = p0; p < p1; ++p) {
-        while (p >= tb.first[ti + 1]) ++ti;
-        const int64_t i0 = (int64_t)(p - tb.first[ti]) * PIECE;
-        const int64_t i1 = min(tb.n[ti], i0 + PIECE);
-        if (tb.bf[ti]) {
-            const bf16* x = static_cast<const bf16*>(tb.in[ti]);
+    int64_t ti = find(a, p0, found);
+    Entry e = a.table[ti];
+    int64_t end = ti + 1 < a.count ? a.table[ti + 1].first : a.pieces;
+    for (int64_t p = p0; p < p1; ++p) {
+        if (p >= end) {
+            e = a.table[++ti];
+            end = ti + 1 < a.count ? a.table[ti + 1].first : a.pieces;
+        }
+        if (e.bf) {
+            const int64_t i0 = (p - e.first) * (PIECE_BYTES / 2), i1 = min(e.n, i0 + PIECE_BYTES / 2);
+            const bf16* x = static_cast<const bf16*>(e.in);
             walk<8>(x, 2, i0, i1,
                     [&](int64_t i) { const double v = (float)x[i]; s = fma(v, v, s); },
                     [&](int64_t i) {
@@ -98,7 +124,8 @@ __global__ void __launch_bounds__(NT) k_sumsq(Table tb, PassArgs a) {
                         }
                     });
         } else {
-            const float* x = static_cast<const float*>(tb.in[ti]);
+            const int64_t i0 = (p - e.first) * (PIECE_BYTES / 4), i1 = min(e.n, i0 + PIECE_BYTES / 4);
+            const float* x = static_cast<const float*>(e.in);
             walk<4>(x, 4, i0, i1, [&](int64_t i) { const double v = x[i]; s = fma(v, v, s); },
                     [&](int64_t i) {
                         const f32x4 r = *reinterpret_cast<const f32x4*>(x + i);
@@ -111,75 +138,67 @@ __global__ void __launch_bounds__(NT) k_sumsq(Table tb, PassArgs a) {
     if (threadIdx.x == 0) a.part[blockIdx.x] = s;
 }
 
-// norm and the factor, in `out` (caller) and `ws` = [norm, factor]
-__global__ void __launch_bounds__(1024) k_norm(const double* part, int n, float max_norm, float eps,
-                                               float* out, float* ws) {
-    __shared__ double red[16];
+// the norm, from the workgroups' sums in a fixed order
+M2_DEV float norm_of(const PassArgs& a, double* red) {
     double s = 0;
-    for (int i = threadIdx.x; i < n; i += 1024) s += part[i];
-    s = block_sum(s, red);
-    if (threadIdx.x == 0) {
-        const float norm = (float)sqrt(s);
-        const float c = max_norm / (norm + eps);
-        *out = norm;
-        ws[0] = norm;
-        ws[1] = c >= 1.f ? 1.f : c;          // a norm that is not a number stays one here
-    }
+    for (int i = threadIdx.x; i < a.parts; i += NT) s += a.part[i];
+    return (float)sqrt(block_sum(s, red));
+}
+__global__ void __launch_bounds__(NT) k_norm(PassArgs a) {
+    __shared__ double red[NT / 64];
+    const float norm = norm_of(a, red);
+    if (threadIdx.x == 0) *a.norm = norm;
 }
 
-__global__ void __launch_bounds__(NT) k_scale(Table tb, PassArgs a) {
-    const float c = a.norm[1];
-    const int np = tb.first[tb.count];
-    const int per = (np + gridDim.x - 1) / gridDim.x;
+__global__ void __launch_bounds__(NT) k_scale(PassArgs a) {
+    __shared__ double red[NT / 64];
+    __shared__ int found[NT / 64];
+    const float norm = norm_of(a, red);
+    if (blockIdx.x == 0 && threadIdx.x == 0) *a.norm = norm;
+    float c = a.max_norm / (norm + a.eps);
+    c = c >= 1.f ? 1.f : c;                    // a norm that is not a number stays one here
     // the opposite order of k_sumsq
     const int b = gridDim.x - 1 - blockIdx.x;
-    const int p0 = b * per, p1 = min(np, p0 + per);
-    int ti = p0 < p1 ? find(tb, p1 - 1) : 0;
-    for (int p = p1 - 1; p >= p0; --p) {
-        while (p < tb.first[ti]) --ti;
-        if (c == 1.f && tb.in[ti] == tb.out[ti]) continue;      // in place, nothing to do
-        const int64_t i0 = (int64_t)(p - tb.first[ti]) * PIECE;
-        const int64_t i1 = min(tb.n[ti], i0 + PIECE);
+    const int64_t p0 = a.pieces * b / gridDim.x, p1 = a.pieces * (b + 1) / gridDim.x;
+    if (p0 >= p1) return;
+    int64_t ti = find(a, p1 - 1, found);
+    Entry e = a.table[ti];
+    for (int64_t p = p1 - 1; p >= p0; --p) {
+        if (p < e.first) e = a.table[--ti];
+        if (c == 1.f && e.in == e.out) continue;      // in place, nothing to do
         // input and output on the same 16-byte phase: whole pieces of both
-        const bool same = (((uintptr_t)tb.in[ti] ^ (uintptr_t)tb.out[ti]) & 15) == 0;
-        if (tb.bf[ti]) {
-            const bf16* x = static_cast<const bf16*>(tb.in[ti]);
-            bf16* y = static_cast<bf16*>(tb.out[ti]);
+        const bool same = (((uintptr_t)e.in ^ (uintptr_t)e.out) & 15) == 0;
+        if (e.bf) {
+            const int64_t i0 = (p - e.first) * (PIECE_BYTES / 2), i1 = min(e.n, i0 + PIECE_BYTES / 2);
+            const bf16* x = static_cast<const bf16*>(e.in);
+            bf16* y = static_cast<bf16*>(e.out);
             walk<8>(x, 2, i0, i1, [&](int64_t i) { y[i] = (bf16)((float)x[i] * c); },
                     [&](int64_t i) {
                         const u32x4 r = *reinterpret_cast<const u32x4*>(x + i);
                         u32x4 o;
 #pragma unroll
                         for (int j = 0; j < 4; ++j) o[j] = pk_bf16(bf16_lo(r[j]) * c, bf16_hi(r[j]) * c);
-                        if (same) {
-                            *reinterpret_cast<u32x4*>(y + i) = o;
-                        } else {
-                            const uint16_t* q = reinterpret_cast<const uint16_t*>(&o);
-#pragma unroll
-                            for (int j = 0; j < 8; ++j) reinterpret_cast<uint16_t*>(y)[i + j] = q[j];
-                        }
+                        if (same) *reinterpret_cast<u32x4*>(y + i) = o;
+                        else store16(y + i, o);
                     });
         } else {
-            const float* x = static_cast<const float*>(tb.in[ti]);
-            float* y = static_cast<float*>(tb.out[ti]);
+            const int64_t i0 = (p - e.first) * (PIECE_BYTES / 4), i1 = min(e.n, i0 + PIECE_BYTES / 4);
+            const float* x = static_cast<const float*>(e.in);
+            float* y = static_cast<float*>(e.out);
             walk<4>(x, 4, i0, i1, [&](int64_t i) { y[i] = x[i] * c; },
                     [&](int64_t i) {
                         f32x4 r = *reinterpret_cast<const f32x4*>(x + i);
 #pragma unroll
                         for (int j = 0; j < 4; ++j) r[j] *= c;
-                        if (same) {
-                            *reinterpret_cast<f32x4*>(y + i) = r;
-                        } else {
-#pragma unroll
-                            for (int j = 0; j < 4; ++j) y[i + j] = r[j];
-                        }
+                        if (same) *reinterpret_cast<f32x4*>(y + i) = r;
+                        else store16(y + i, __builtin_bit_cast(u32x4, r));
                     });
         }
     }
 }
 
-// workspace: [norm, factor] in 256 bytes, then the partial sums of each launch
-size_t need(int64_t count) { return 256 + (size_t)((count + MAXT - 1) / MAXT + 1) * MAXWG * 8; }
+// workspace: the first pass's sums, then the table
+size_t need(int64_t count) { return MAXWG * 8 + (size_t)count * sizeof(Entry) + 256; }
 
 }  // namespace
 
@@ -191,27 +210,6 @@ size_t clip_grad_norm_workspace(const m2_clip_grad_norm_args& a) {
         return 0;
     }
     return need(a.count);
-}
-
-// fills the table from tensor i on (tensors without elements are passed over);
-// returns the number of pieces
-static int64_t fill(const m2_clip_grad_norm_args& a, int64_t& i, Table& tb) {
-    tb.count = 0;
-    int64_t np = 0;
-    for (; i < a.count && tb.count < MAXT; ++i) {
-        const m2_tensor_ref& r = a.tensors[i];
-        if (r.n == 0) continue;
-        const int64_t k = (r.n + PIECE - 1) / PIECE;
-        if (np + k >= (1ll << 31) - 1) break;
-        tb.in[tb.count] = r.in;
-        tb.out[tb.count] = r.out;
-        tb.n[tb.count] = r.n;
-        tb.bf[tb.count] = r.dtype == M2_BF16;
-        tb.first[tb.count++] = (int)np;
-        np += k;
-    }
-    tb.first[tb.count] = (int)np;
-    return np;
 }
 
 int launch_clip_grad_norm(const m2_clip_grad_norm_args& a, hipStream_t s) {
@@ -232,26 +230,36 @@ int launch_clip_grad_norm(const m2_clip_grad_norm_args& a, hipStream_t s) {
                                      (!a.clip || (r.out && (uintptr_t)r.out % es == 0)))),
                    M2_ERR_INVALID, "%s: tensor %lld: bad pointer or size", who, (long long)i);
     }
-    float* nw = static_cast<float*>(a.workspace);
-    double* part = reinterpret_cast<double*>(static_cast<char*>(a.workspace) + 256);
-    Table tb;
-    int64_t parts = 0;
-    for (int64_t i = 0; i < a.count;) {
-        const int64_t np = fill(a, i, tb);
-        if (np == 0) break;
-        const unsigned grid = (unsigned)(np < MAXWG ? np : MAXWG);
-        hipLaunchKernelGGL(k_sumsq, dim3(grid), dim3(NT), 0, s, tb, PassArgs{part + parts, nullptr});
-        parts += grid;
+    PassArgs p{};
+    p.part = static_cast<double*>(a.workspace);
+    Entry* table = reinterpret_cast<Entry*>(static_cast<char*>(a.workspace) + MAXWG * 8);
+    p.table = table; p.norm = a.norm; p.max_norm = a.max_norm; p.eps = a.eps;
+    // tensors without elements are passed over
+    Batch b;
+    b.count = 0;
+    auto send = [&]() {
+        hipLaunchKernelGGL(k_table, dim3(1), dim3(256), 0, s, b, table + p.count);
+        p.count += b.count;
+        b.count = 0;
+    };
+    for (int64_t i = 0; i < a.count; ++i) {
+        const m2_tensor_ref& r = a.tensors[i];
+        if (r.n == 0) continue;
+        const int64_t per = r.dtype == M2_BF16 ? PIECE_BYTES / 2 : PIECE_BYTES / 4;
+        if (b.count == BATCH || (b.count && p.pieces - b.base > (int64_t)UINT32_MAX)) send();
+        if (b.count == 0) b.base = p.pieces;
+        const int k = b.count++;
+        b.in[k] = r.in;
+        b.out[k] = r.out;
+        b.n[k] = r.dtype == M2_BF16 ? ~r.n : r.n;
+        b.first[k] = (uint32_t)(p.pieces - b.base);
+        p.pieces += (r.n + per - 1) / per;
     }
-    hipLaunchKernelGGL(k_norm, dim3(1), dim3(1024), 0, s, part, (int)parts, a.max_norm, a.eps, a.norm, nw);
-    if (a.clip) {
-        for (int64_t i = 0; i < a.count;) {
-            const int64_t np = fill(a, i, tb);
-            if (np == 0) break;
-            const unsigned grid = (unsigned)(np < MAXWG ? np : MAXWG);
-            hipLaunchKernelGGL(k_scale, dim3(grid), dim3(NT), 0, s, tb, PassArgs{nullptr, nw});
-        }
-    }
+    if (b.count) send();
+    p.parts = (int)(p.pieces < MAXWG ? p.pieces : MAXWG);
+    if (p.parts) hipLaunchKernelGGL(k_sumsq, dim3(p.parts), dim3(NT), 0, s, p);
+    if (a.clip && p.parts) hipLaunchKernelGGL(k_scale, dim3(p.parts), dim3(NT), 0, s, p);
+    else hipLaunchKernelGGL(k_norm, dim3(1), dim3(NT), 0, s, p);
     return check_launch(who);
 }
 

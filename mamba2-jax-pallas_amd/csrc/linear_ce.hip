@@ -705,7 +705,7 @@ template <typename T, class S> __global__ void __launch_bounds__(256) k_ce_dx_se
     const int m0 = (grp * 8 + in % gm) * S::BM + (w / S::WN * S::FM + i) * 16;
     const int n = in / gm * S::BN + (w % S::WN * S::FN + j) * 16 + (lane & 15);
     if (n - (lane & 15) >= count || m0 >= a.dim) return;
-    const Deal d = deal(tiles, a.seg_nk, a.nwg);
+    const Deal d = deal(tiles, a.seg_nk, a.nwg, S::BN);
     constexpr int64_t SEG = (int64_t)S::NW * S::FM * S::FN * 64;
     const f32x4* p = reinterpret_cast<const f32x4*>(a.part) + tile * SEG + (w * S::FM * S::FN + i * S::FN + j) * 64 + lane;
     f32x4 x = p[0], y = p[S::FN * 64];
@@ -745,6 +745,7 @@ template <bool F32> struct Shapes {
     typedef Shape<128, 64, 4, 1, 3, 64, false, false, T> Z64;
     typedef Shape<128, 16, 4, 1, 4, 64, false, false, T> Z16;
     typedef Shape<256, 256, 2, 4, 2, 64, true, false, T> X256;
+    typedef Shape<256, 128, 2, 4, 2, 64, true, false, T> X128;
     typedef Shape<256, 64, 4, 1, 3, 64, true, false, T> X64;
     typedef Shape<256, 16, 4, 1, 3, 64, true, false, T> X16;
     typedef Shape<256, 256, 2, 4, 2, 64, true, true, T> W256;
@@ -865,20 +866,21 @@ BwdPlan bwd_plan(const m2_linear_cross_entropy_grad_args& a) {
     const int tm = tiles(a.dim, 256);
     p.x = a.n <= 16 ? 16 : 64;
     if (a.n > 64) {
-        const int tn = tiles(a.n, 256);
         p.splits = ncu;
+        p.x = deal(tm * tiles(a.n, 256), steps, ncu, 256).cost <= deal(tm * tiles(a.n, 128), steps, ncu, 128).cost ? 256
+                                                                                                           : 128;
         int64_t segs = 0, all_segs = 0;
-        for (int k = 1; k <= tn; ++k) {
-            const Deal d = deal(tm * k, steps, ncu);
+        for (int k = 1; k <= tiles(a.n, p.x); ++k) {
+            const Deal d = deal(tm * k, steps, ncu, p.x);
             all_segs = d.full + (int64_t)d.rest * d.s;
             if (all_segs > segs) segs = all_segs;
         }
-        if (2 * all_segs > ncu) {             // else the smaller tiles, as for the logits
-            p.x = 256;
-            p.dx = a.grad_x ? take(4 * 256 * 256 * (size_t)segs) : 0;
+        if (2 * all_segs > ncu) {
+            p.dx = a.grad_x ? take(4 * 256 * (size_t)p.x * segs) : 0;
             p.total = at;
             return p;
         }
+        p.x = 64;                             // too few: the smaller tiles, as for the logits
     }
     const int64_t t = (int64_t)tm * tiles(a.n ? a.n : 1, p.x);
     double best = 1e300;
@@ -1006,10 +1008,11 @@ template <bool F32> int run_bwd(const m2_linear_cross_entropy_grad_args& a, cons
             d.b = Operand{G, p.piece, gplane, (int)c.np, (int)p.piece};
             d.tm = tiles(c.dim, 256);
             d.tn = tiles(c.n, p.x);
-            if (p.x == 256) {
+            if (p.x >= 128) {
                 if (q == 0) dxs.seg_nk = d.nk;
                 d.seg_nk = dxs.seg_nk;
-                launch<typename P::X256>(d, EpiDxSeg{dxp, q > 0}, s);
+                if (p.x == 256) launch<typename P::X256>(d, EpiDxSeg{dxp, q > 0}, s);
+                else launch<typename P::X128>(d, EpiDxSeg{dxp, q > 0}, s);
                 dxs.tm = d.tm; dxs.tn = d.tn; dxs.nwg = p.splits;
             } else {
                 if (d.splits > d.nk) d.splits = d.nk;             // a short last piece
@@ -1035,12 +1038,12 @@ template <bool F32> int run_bwd(const m2_linear_cross_entropy_grad_args& a, cons
             }
         }
     }
-    if (a.grad_x && p.x == 256) {
-        typedef typename P::X256 S;
+    if (a.grad_x && p.x >= 128) {
         dxs.part = dxp; dxs.dx = a.grad_x; dxs.n = c.n; dxs.dim = c.dim;
-        dxs.nred = dxs.tm * dxs.tn * (S::NW * S::FM * S::FN / 2 / 4);
-        const int zero = tiles(c.n, 64);
-        hipLaunchKernelGGL((k_ce_dx_seg<T, S>), dim3((unsigned)(dxs.nred + zero)), dim3(256), 0, s, dxs, tk);
+        dxs.nred = dxs.tm * dxs.tn * (256 * p.x / (32 * 16) / 4);
+        const dim3 grid((unsigned)(dxs.nred + tiles(c.n, 64))), thr(256);
+        if (p.x == 256) hipLaunchKernelGGL((k_ce_dx_seg<T, typename P::X256>), grid, thr, 0, s, dxs, tk);
+        else hipLaunchKernelGGL((k_ce_dx_seg<T, typename P::X128>), grid, thr, 0, s, dxs, tk);
     } else if (a.grad_x) {
         DxArgs d{dxp, a.grad_x, c.n, c.np, c.dp, c.dim, p.splits};
         hipLaunchKernelGGL((k_ce_dx<T>), dim3((unsigned)((c.n + 3) / 4), (unsigned)((c.dim + 511) / 512)),

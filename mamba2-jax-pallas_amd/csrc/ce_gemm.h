@@ -17,8 +17,8 @@
 // load writes LDS linearly.
 //
 // float32 operands come as three bf16 planes (v = p0 + p1 + p2 exactly but for
-// the last bits) and K runs six times: the products p_i q_j with i + j <= 2, the small
-// ones first; what is left out is 2^-24 of the product.
+// the last bits); the products p_i q_j with i + j <= 2 are added up, the small ones
+// first; what is left out is 2^-24 of the product.
 #pragma once
 
 #include "m2_internal.h"
@@ -52,11 +52,9 @@ struct Deal {
     int full, rest, s;
     int64_t cost;            // 5 ns
 };
-// bn: the tile's n, 256 or 128
-__host__ __device__ inline Deal deal(int tiles, int nk, int nwg, int bn) {
-    // a step takes about 1.4 us (0.85 us), writing and reading a segment of 256 KB the chip
-    // 0.11 us (whole numbers: the host sizes the workspace by the same)
-    const int step = bn == 256 ? 280 : 170, seg = bn == 256 ? 22 : 11;
+// step: the time of one, seg: of writing and reading a segment by the whole chip, in 5 ns
+// (whole numbers: the host sizes the workspace by the same)
+__host__ __device__ inline Deal deal(int tiles, int nk, int nwg, int step, int seg) {
     Deal d;
     d.full = tiles / nwg * nwg;
     d.rest = tiles - d.full;
@@ -188,11 +186,11 @@ template <int BM_, int BN_, int WM_, int WN_, int ST_, int BK_, bool ATR_, bool 
     static constexpr int SLOT = LA::BYTES + LB::BYTES;
     static constexpr int LDS = SLOT * ST;
     static constexpr int LOADS = LA::J + LB::J;
+    // what deal() goes by: 1.4 us a step of 256 x 256 (as measured), 0.85 us of 256 x 128; six
+    // products 4.5 us of 256 x 128, 1.5 us of 128 x 64; a segment of 256 KB 0.11 us
+    static constexpr int STEP = TERMS == 1 ? (BN == 256 ? 280 : 170) : BN == 128 ? 900 : BN == 64 ? 300 : 100;
+    static constexpr int SEG = BM * BN * 22 / 65536 + 1;
 };
-
-// The order of the products of the planes: (0,2) (2,0) (1,1) (0,1) (1,0) (0,0)
-template <int TERMS> M2_DEV int plane_a(int t) { return TERMS == 1 ? 0 : t == 1 ? 2 : (t == 2 || t == 4) ? 1 : 0; }
-template <int TERMS> M2_DEV int plane_b(int t) { return TERMS == 1 ? 0 : t == 0 ? 2 : (t == 2 || t == 3) ? 1 : 0; }
 
 // Few tokens: the operand of the vocabulary streams from HBM through a deep ring
 template <class S, class EPI>
@@ -213,19 +211,19 @@ __global__ void __launch_bounds__(S::NT, 2 * S::LDS <= 160 * 1024 ? 2 : 1) k_ce_
     if (g.tok_n && n0 >= ((count + 63) & ~63)) return;
     const int nk = g.nk ? g.nk : (count + 63) >> 6;
     const int k0 = (int)((int64_t)nk * split / g.splits), k1 = (int)((int64_t)nk * (split + 1) / g.splits);
-    const int total = (k1 - k0) * S::TERMS;
+    const int total = k1 - k0;
 
     typename S::LA la;
     typename S::LB lb;
     la.init(g.a, m0, w, lane);
     lb.init(g.b, n0, w, lane);
     const uint32_t lds0 = lds_addr(smem);
-    int ikt = k0, iterm = 0, islot = 0;
+    int ikt = k0, islot = 0;
     auto issue = [&]() {
         const uint32_t l = lds0 + islot * S::SLOT;
-        la.issue(g.a, ikt, plane_a<S::TERMS>(iterm), l, w, lane);
-        lb.issue(g.b, ikt, plane_b<S::TERMS>(iterm), l + S::LA::BYTES, w, lane);
-        if (++ikt == k1) { ikt = k0; ++iterm; }
+        la.issue(g.a, ikt, 0, l, w, lane);
+        lb.issue(g.b, ikt, 0, l + S::LA::BYTES, w, lane);
+        ++ikt;
         if (++islot == S::ST) islot = 0;
     };
 
@@ -268,6 +266,68 @@ __global__ void __launch_bounds__(S::NT, 2 * S::LDS <= 160 * 1024 ? 2 : 1) k_ce_
     epi.template run<S>(acc, smem, m0, n0, wm, wn, lane, count, split, tm);
 }
 
+struct Work {                 // of a workgroup: its item i, a tile and its K steps of 64
+    int i, tile, k0, k1, seg;
+};
+// The tiles and segments of a workgroup of the persistent kernels: whole tiles one workgroup
+// after the other, each XCD a contiguous range, which its share of the workgroups gives.
+template <class S, class EPI> struct Schedule {
+    int tm_all, tn_all, nk, full, rest, s, f0, rounds, r0, r1, lw, items;
+
+    M2_DEV void init(const Gemm& g, int count) {
+        tm_all = g.tm;
+        tn_all = g.tok_n ? min(g.tn, (((count + 63) & ~63) + S::BN - 1) / S::BN) : g.tn;
+        nk = g.nk ? g.nk : (count + 63) >> 6;
+        const int tiles = g.tm * tn_all;
+        const int xcd = blockIdx.x & 7, local = blockIdx.x >> 3, nwg = gridDim.x;
+        lw = (nwg - xcd + 7) >> 3;
+        const int before = xcd * (nwg >> 3) + min(xcd, nwg & 7);
+        full = 0; rest = tiles; s = 1;
+        if constexpr (EPI::SEG) {
+            const Deal d = deal(tiles, g.seg_nk, nwg, S::STEP, S::SEG);
+            full = d.full; rest = d.rest; s = d.s;
+        }
+        f0 = full / nwg * before + local;
+        rounds = full / nwg;
+        const int64_t cut = (int64_t)rest * s;
+        r0 = (int)(cut * before / nwg) + local;
+        r1 = (int)(cut * (before + lw) / nwg);
+        items = rounds + (r1 > r0 ? (r1 - r0 + lw - 1) / lw : 0);
+    }
+    M2_DEV Work work(int i) const {
+        if (EPI::SEG && i < rounds) return Work{i, f0 + i * lw, 0, nk, f0 + i * lw};
+        const int id = r0 + (i - rounds) * lw;
+        const int part = EPI::SEG ? id / rest : 0;
+        Work x{i, full + id - part * rest, 0, nk, full + id};
+        if constexpr (EPI::SEG) {
+            x.k0 = (int)((int64_t)nk * part / s);
+            x.k1 = (int)((int64_t)nk * (part + 1) / s);
+        }
+        return x;
+    }
+    // the first item from i on that has steps (a short piece's parts may not), or items
+    M2_DEV int with_steps(int i) const {
+        if constexpr (EPI::SEG)
+            for (; i < items; ++i) {
+                const Work x = work(i);
+                if (x.k0 < x.k1) break;
+            }
+        return i;
+    }
+    // 8 tiles of m beside each other, then the next n
+    M2_DEV void place(int tile, int& tm, int& m0, int& n0) const {
+        const int grp = tile / (8 * tn_all), gm = min(8, tm_all - grp * 8), in = tile - grp * 8 * tn_all;
+        tm = grp * 8 + in % gm;
+        m0 = tm * S::BM;
+        n0 = in / gm * S::BN;
+    }
+};
+template <class LD> struct Cursor {      // the step of an operand that is loaded next
+    LD ld;
+    Work at;
+    int k;
+};
+
 // Many tokens: persistent workgroups (whole tiles, or with EPI::SEG segments of them), each XCD with a contiguous range of the tiles
 // (neighbours share panels in its L2).  K in steps of 64, A through a ring of three slots, B of
 // two (all 160 KB for 256 x 256); the fragments of a half step (32 of K) are read while the half
@@ -279,78 +339,33 @@ __global__ void __launch_bounds__(S::NT, 2 * S::LDS <= 160 * 1024 ? 2 : 1) k_ce_
 // so that both halves carry as many loads (all of them in one half leave too few cycles for
 // the 64 bytes a cycle that a CU takes in).  The loads run on into the next tile, whose first
 // steps arrive during the epilogue.
-struct Work {                 // of a workgroup: its item i, a tile and its K steps
-    int i, tile, k0, k1, seg;
-};
-template <class LD> struct Cursor {      // the step of an operand that is loaded next
-    LD ld;
-    Work at;
-    int k, term;
-};
-
 template <class S, class EPI>
 __global__ void __launch_bounds__(S::NT, S::NT / 256) k_ce_tile(Gemm g, EPI epi) {
-    static_assert(S::BK == 64, "");
+    static_assert(S::BK == 64 && S::TERMS == 1, "");
     constexpr int B_AT = 3 * S::LA::BYTES;
     __shared__ __align__(1024) char smem[B_AT + 2 * S::LB::BYTES];
     const int lane = threadIdx.x & 63, w = wave_id();
     const int wm = w / S::WN, wn = w % S::WN;
     const int count = g.count ? *g.count : g.n;
-    const int tn_all = g.tok_n ? min(g.tn, (((count + 63) & ~63) + S::BN - 1) / S::BN) : g.tn;
-    const int tiles = g.tm * tn_all;
-    const int nk = g.nk ? g.nk : (count + 63) >> 6;
-    // this workgroup's place: those of an XCD beside each other
-    const int xcd = blockIdx.x & 7, local = blockIdx.x >> 3;
-    const int nwg = gridDim.x, lw = (nwg - xcd + 7) >> 3;
-    const int before = xcd * (nwg >> 3) + min(xcd, nwg & 7);
-    // whole tiles one workgroup after the other; each XCD a contiguous range, which its
-    // share of the workgroups gives
-    Deal dl{0, tiles, 1, 0};
-    if constexpr (EPI::SEG) dl = deal(tiles, g.seg_nk, nwg, S::BN);
-    const int f0 = dl.full / nwg * before + local, rounds = dl.full / nwg;
-    const int64_t cut = (int64_t)dl.rest * dl.s;
-    const int r0 = (int)(cut * before / nwg) + local, r1 = (int)(cut * (before + lw) / nwg);
-    auto work = [&](int i) {
-        if (EPI::SEG && i < rounds) return Work{i, f0 + i * lw, 0, nk, f0 + i * lw};
-        const int id = r0 + (i - rounds) * lw;
-        Work x{i, 0, 0, 0, dl.full + id};
-        if (id >= r1) return x;
-        const int part = EPI::SEG ? id / dl.rest : 0;
-        x.tile = dl.full + id - part * dl.rest;
-        x.k0 = EPI::SEG ? (int)((int64_t)nk * part / dl.s) : 0;
-        x.k1 = EPI::SEG ? (int)((int64_t)nk * (part + 1) / dl.s) : nk;
-        return x;
-    };
-    const int items = rounds + (r1 > r0 ? (r1 - r0 + lw - 1) / lw : 0);
-    if (items == 0) return;
-    auto place = [&](int id, int& tm, int& m0, int& n0) {
-        // 8 tiles of m beside each other, then the next n
-        const int grp = id / (8 * tn_all), gm = min(8, g.tm - grp * 8), in = id - grp * 8 * tn_all;
-        tm = grp * 8 + in % gm;
-        m0 = tm * S::BM;
-        n0 = in / gm * S::BN;
-    };
+    Schedule<S, EPI> sc;
+    sc.init(g, count);
+    const int first = sc.nk > 0 ? sc.with_steps(0) : 0;
+    if (first >= sc.items) return;
     Cursor<typename S::LA> ca;
     Cursor<typename S::LB> cb;
-    auto start = [&](auto& c, const Operand& o, bool is_a, const Work& x) {
+    auto start = [&](auto& c, const Operand& o, bool is_a, int item) {
         int tm, m0, n0;
-        place(x.tile, tm, m0, n0);
+        c.at = sc.work(item);
+        sc.place(c.at.tile, tm, m0, n0);
         c.ld.init(o, is_a ? m0 : n0, w, lane);
-        c.at = x;
-        c.k = x.k0;
-        c.term = 0;
+        c.k = c.at.k0;
     };
     // past the last step the last tile's last step is loaded again (nobody reads it)
     auto next = [&](auto& c, const Operand& o, bool is_a) {
         if (++c.k < c.at.k1) return;
-        c.k = c.at.k0;
-        if (++c.term < S::TERMS) return;
-        for (int i = c.at.i + 1; i < items; ++i) {
-            const Work x = work(i);
-            if (x.k0 < x.k1) return start(c, o, is_a, x);
-        }
-        c.k = c.at.k1 - 1;
-        c.term = S::TERMS - 1;
+        const int i = sc.with_steps(c.at.i + 1);
+        if (i < sc.items) start(c, o, is_a, i);
+        else c.k = c.at.k1 - 1;
     };
     const uint32_t lds0 = lds_addr(smem);
 
@@ -362,16 +377,13 @@ __global__ void __launch_bounds__(S::NT, S::NT / 256) k_ce_tile(Gemm g, EPI epi)
     bf16x8 a0[S::FM], b0[S::FN], a1[S::FM], b1[S::FN];
     int sa = 0, sb = 0;           // byte offsets of the slots of the current step
     auto after = [](int slot) { return slot == 2 * S::LA::BYTES ? 0 : slot + S::LA::BYTES; };
-    int first = 0;                // the first item that has steps (a short piece's parts may not)
-    while (first < items && nk > 0 && work(first).k0 >= work(first).k1) ++first;
-    if (first == items) return;
-    if (nk > 0) {
-        start(ca, g.a, true, work(first));
-        start(cb, g.b, false, work(first));
+    if (sc.nk > 0) {
+        start(ca, g.a, true, first);
+        start(cb, g.b, false, first);
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-            ca.ld.issue(g.a, ca.k, plane_a<S::TERMS>(ca.term), lds0 + i * S::LA::BYTES, w, lane);
-            cb.ld.issue(g.b, cb.k, plane_b<S::TERMS>(cb.term), lds0 + B_AT + i * S::LB::BYTES, w, lane);
+            ca.ld.issue(g.a, ca.k, 0, lds0 + i * S::LA::BYTES, w, lane);
+            cb.ld.issue(g.b, cb.k, 0, lds0 + B_AT + i * S::LB::BYTES, w, lane);
             next(ca, g.a, true);
             next(cb, g.b, false);
         }
@@ -381,22 +393,21 @@ __global__ void __launch_bounds__(S::NT, S::NT / 256) k_ce_tile(Gemm g, EPI epi)
         rb.read(smem + B_AT, 0, lane, b0);
     }
     constexpr int RD = S::FM + S::FN;
-    for (int item = first; item < items; ++item) {
-        const Work wk = work(item);
-        if (EPI::SEG && wk.k0 >= wk.k1) continue;
+    for (int item = first; item < sc.items; item = sc.with_steps(item + 1)) {
+        const Work wk = sc.work(item);
         int tm, m0, n0;
-        place(wk.tile, tm, m0, n0);
+        sc.place(wk.tile, tm, m0, n0);
 #pragma unroll
         for (int i = 0; i < S::FM; ++i)
 #pragma unroll
             for (int j = 0; j < S::FN; ++j) acc[i][j] = zero4();
-        const int steps = S::TERMS * (wk.k1 - wk.k0);
+        const int steps = wk.k1 - wk.k0;
         for (int st = 0; st < steps; ++st) {
             {
                 const char* pa = smem + sa;
                 const char* pb = smem + B_AT + sb;
                 const uint32_t l = lds0 + after(after(sa));
-                const bf16* from = ca.ld.base(g.a, ca.k, plane_a<S::TERMS>(ca.term));
+                const bf16* from = ca.ld.base(g.a, ca.k, 0);
 #pragma unroll
                 for (int i = 0; i < S::FM; ++i) {
 #pragma unroll
@@ -424,7 +435,7 @@ __global__ void __launch_bounds__(S::NT, S::NT / 256) k_ce_tile(Gemm g, EPI epi)
                 sb ^= S::LB::BYTES;
                 const char* pa = smem + sa;
                 const char* pb = smem + B_AT + sb;
-                const bf16* from = cb.ld.base(g.b, cb.k, plane_b<S::TERMS>(cb.term));
+                const bf16* from = cb.ld.base(g.b, cb.k, 0);
 #pragma unroll
                 for (int i = 0; i < S::FM; ++i) {
 #pragma unroll
@@ -445,6 +456,129 @@ __global__ void __launch_bounds__(S::NT, S::NT / 256) k_ce_tile(Gemm g, EPI epi)
         }
         // what is loaded so far (step 0 and 1 of the next tile) is there before any store
         wait_vmem<0>();
+        epi.template run<S>(acc, nullptr, m0, n0, wm, wn, lane, count, wk.seg, tm);
+    }
+    wait_vmem<0>();           // no load may land after the workgroup has ended
+}
+
+// float32 operands, any number of tokens: persistent workgroups, steps of 32 of K through ST
+// slots that hold the three planes of both operands: each plane is loaded once for the
+// products it takes part in (loading the pair of planes of one product after the
+// other moves twice as much and takes six times as many steps, whose latency is
+// what bounds a few tiles).  B's fragments of a step and those of one row of A's stay in
+// registers; the row after it is read while this one multiplies.  The last row of a step
+// multiplies behind the step's barrier, while the next step's first fragments are read
+// and the slot is filled again.
+template <class S, class EPI>
+__global__ void __launch_bounds__(S::NT, S::NT / 256) k_ce_planes(Gemm g, EPI epi) {
+    static_assert(S::BK == 32 && S::TERMS == 6 && S::FM % 2 == 0, "");
+    constexpr int PA = S::LA::BYTES, PB = S::LB::BYTES, SLOT = 3 * (PA + PB), LOADS = 3 * S::LOADS;
+    __shared__ __align__(1024) char smem[SLOT * S::ST];
+    const int lane = threadIdx.x & 63, w = wave_id();
+    const int wm = w / S::WN, wn = w % S::WN;
+    const int count = g.count ? *g.count : g.n;
+    Schedule<S, EPI> sc;
+    sc.init(g, count);
+    const int first = sc.nk > 0 ? sc.with_steps(0) : 0;
+    if (first >= sc.items) return;
+    Cursor<typename S::LA> c;
+    typename S::LB lb;
+    auto start = [&](int item) {
+        int tm, m0, n0;
+        c.at = sc.work(item);
+        sc.place(c.at.tile, tm, m0, n0);
+        c.ld.init(g.a, m0, w, lane);
+        lb.init(g.b, n0, w, lane);
+        c.k = 2 * c.at.k0;
+    };
+    // past the last step the last tile's last step is loaded again (nobody reads it)
+    auto next = [&]() {
+        if (++c.k < 2 * c.at.k1) return;
+        const int i = sc.with_steps(c.at.i + 1);
+        if (i < sc.items) start(i);
+        else c.k = 2 * c.at.k1 - 1;
+    };
+    // load q of a step's LOADS
+    auto load = [&](int q, uint32_t l) {
+        constexpr int J = S::LA::J, K = S::LB::J;
+        if (q < 3 * J) c.ld.piece(g.a, c.ld.base(g.a, c.k, q / J), c.k, q % J, l + q / J * PA, w, lane);
+        else lb.piece(g.b, lb.base(g.b, c.k, (q - 3 * J) / K), c.k, (q - 3 * J) % K, l + 3 * PA + (q - 3 * J) / K * PB, w, lane);
+    };
+    const uint32_t lds0 = lds_addr(smem);
+    Reader<S::BM, S::ATR, S::FM, 32> ra;
+    Reader<S::BN, S::BTR, S::FN, 32> rb;
+    ra.init(wm * S::FM * 16, lane);
+    rb.init(wn * S::FN * 16, lane);
+    f32x4 acc[S::FM][S::FN];
+    bf16x8 a[2][3], b0[3][S::FN], b1[3][S::FN];
+    int slot = 0;                 // byte offset of the current step's
+    if (sc.nk > 0) {
+        start(first);
+#pragma unroll
+        for (int i = 0; i < S::ST; ++i) {
+#pragma unroll
+            for (int q = 0; q < LOADS; ++q) load(q, lds0 + i * SLOT);
+            next();
+        }
+        wait_vmem<(S::ST - 1) * LOADS>();
+        lds_barrier();
+#pragma unroll
+        for (int p = 0; p < 3; ++p) {
+            rb.read(smem + 3 * PA + p * PB, 0, lane, b0[p]);
+            a[0][p] = ra.one(smem + p * PA, 0, lane, 0);
+        }
+    }
+    // the small products first
+    constexpr int PI[6] = {0, 2, 1, 0, 1, 0}, PJ[6] = {2, 0, 1, 1, 0, 0};
+    auto step = [&](const bf16x8(&b)[3][S::FN], bf16x8(&nb)[3][S::FN]) {
+        const char* s0 = smem + slot;
+        const uint32_t l = lds0 + slot;
+        slot = slot == (S::ST - 1) * SLOT ? 0 : slot + SLOT;
+        const char* s1 = smem + slot;
+#pragma unroll
+        for (int i = 0; i < S::FM; ++i) {
+            const bool last = i == S::FM - 1;
+            if (!last) {
+#pragma unroll
+                for (int p = 0; p < 3; ++p) a[(i + 1) & 1][p] = ra.one(s0 + p * PA, 0, lane, i + 1);
+            } else {
+                wait_vmem<(S::ST - 2) * LOADS>();
+                lds_barrier();
+                __builtin_amdgcn_sched_barrier(0);
+            }
+#pragma unroll
+            for (int t = 0; t < 6; ++t) {
+                if (last) {
+                    constexpr int RD = 3 * S::FN + 3;
+#pragma unroll
+                    for (int q = t * RD / 6; q < (t + 1) * RD / 6; ++q) {
+                        if (q < 3 * S::FN) nb[q / S::FN][q % S::FN] = rb.one(s1 + 3 * PA + q / S::FN * PB, 0, lane, q % S::FN);
+                        else a[0][q - 3 * S::FN] = ra.one(s1 + (q - 3 * S::FN) * PA, 0, lane, 0);
+                    }
+#pragma unroll
+                    for (int q = t * LOADS / 6; q < (t + 1) * LOADS / 6; ++q) load(q, l);
+                }
+#pragma unroll
+                for (int j = 0; j < S::FN; ++j)
+                    acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a[i & 1][PI[t]], b[PJ[t]][j], acc[i][j], 0, 0, 0);
+                if (last) __builtin_amdgcn_sched_barrier(0);
+            }
+            __builtin_amdgcn_sched_barrier(0);
+        }
+        next();
+    };
+    for (int item = first; item < sc.items; item = sc.with_steps(item + 1)) {
+        const Work wk = sc.work(item);
+        int tm, m0, n0;
+        sc.place(wk.tile, tm, m0, n0);
+#pragma unroll
+        for (int i = 0; i < S::FM; ++i)
+#pragma unroll
+            for (int j = 0; j < S::FN; ++j) acc[i][j] = zero4();
+        for (int k = wk.k0; k < wk.k1; ++k) {
+            step(b0, b1);
+            step(b1, b0);
+        }
         epi.template run<S>(acc, nullptr, m0, n0, wm, wn, lane, count, wk.seg, tm);
     }
     wait_vmem<0>();           // no load may land after the workgroup has ended

@@ -231,7 +231,7 @@ struct LogSum {
 };
 // m: vocabulary, n: token -> per token (max, sum of exp(z - max)) without the target: of a tile
 // (k_ce_stream), or of the BM / WM rows of the vocabulary that a row of wavefronts holds
-// (k_ce_tile, whose LDS is full)
+// (the others, whose LDS is full)
 struct EpiLse {
     static constexpr bool SEG = false;
     const int* tgt;          // of the kept tokens, or NULL: the caller's targets
@@ -292,13 +292,13 @@ struct EpiLse {
                 for (int r = 0; r < 4; ++r) s += __builtin_amdgcn_exp2f(fmaf(acc[i][j][r], LOG2E, b));
             s += __shfl_xor(s, 16);
             s += __shfl_xor(s, 32);
-            if constexpr (S::BN < 128) {
+            if constexpr (S::BN < 128 && S::TERMS == 1) {
                 if (lane < 16) reinterpret_cast<float2*>(smem)[wm * S::BN + n - n0] = make_float2(mx, s);
             } else {
                 if (lane < 16 && n < count) part[((int64_t)tm * S::WM + wm) * np + n] = make_float2(mx, s);
             }
         }
-        if constexpr (S::BN < 128) {
+        if constexpr (S::BN < 128 && S::TERMS == 1) {
             __syncthreads();
             const int t = threadIdx.x;
             if (t < S::BN && n0 + t < count) {
@@ -705,7 +705,7 @@ template <typename T, class S> __global__ void __launch_bounds__(256) k_ce_dx_se
     const int m0 = (grp * 8 + in % gm) * S::BM + (w / S::WN * S::FM + i) * 16;
     const int n = in / gm * S::BN + (w % S::WN * S::FN + j) * 16 + (lane & 15);
     if (n - (lane & 15) >= count || m0 >= a.dim) return;
-    const Deal d = deal(tiles, a.seg_nk, a.nwg, S::BN);
+    const Deal d = deal(tiles, a.seg_nk, a.nwg, S::STEP, S::SEG);
     constexpr int64_t SEG = (int64_t)S::NW * S::FM * S::FN * 64;
     const f32x4* p = reinterpret_cast<const f32x4*>(a.part) + tile * SEG + (w * S::FM * S::FN + i * S::FN + j) * 64 + lane;
     f32x4 x = p[0], y = p[S::FN * 64];
@@ -728,37 +728,59 @@ bool al16(const void* p) { return ((uintptr_t)p & 15) == 0; }
 
 template <class S, class EPI> void launch(const Gemm& g, const EPI& e, hipStream_t s) {
     const int64_t tiles = (int64_t)g.tm * g.tn;
-    if constexpr (S::BN < 128) {
+    if constexpr (S::TERMS == 1 && S::BN < 128) {
         hipLaunchKernelGGL((k_ce_stream<S, EPI>), dim3((unsigned)(tiles * g.splits)), dim3(S::NT), 0, s, g, e);
     } else {
         const int64_t ncu = m2::cu_count();
         const unsigned nwg = (unsigned)(EPI::SEG ? g.splits : tiles < ncu ? tiles : ncu);
-        hipLaunchKernelGGL((k_ce_tile<S, EPI>), dim3(nwg), dim3(S::NT), 0, s, g, e);
+        if constexpr (S::TERMS == 1) hipLaunchKernelGGL((k_ce_tile<S, EPI>), dim3(nwg), dim3(S::NT), 0, s, g, e);
+        else hipLaunchKernelGGL((k_ce_planes<S, EPI>), dim3(nwg), dim3(S::NT), 0, s, g, e);
     }
 }
 inline int tiles(int64_t n, int t) { return (int)((n + t - 1) / t); }
 
-// Tiles of the product vocabulary x tokens by the number of tokens
+// Tiles of the logits (Z), of dx (X) and of dw (W); the number is a tile's n
 template <bool F32> struct Shapes {
-    static constexpr int T = F32 ? 6 : 1;
-    typedef Shape<256, 256, 2, 4, 2, 64, false, false, T> Z256;
-    typedef Shape<128, 64, 4, 1, 3, 64, false, false, T> Z64;
-    typedef Shape<128, 16, 4, 1, 4, 64, false, false, T> Z16;
-    typedef Shape<256, 256, 2, 4, 2, 64, true, false, T> X256;
-    typedef Shape<256, 128, 2, 4, 2, 64, true, false, T> X128;
-    typedef Shape<256, 64, 4, 1, 3, 64, true, false, T> X64;
-    typedef Shape<256, 16, 4, 1, 3, 64, true, false, T> X16;
-    typedef Shape<256, 256, 2, 4, 2, 64, true, true, T> W256;
-    typedef Shape<128, 64, 4, 1, 3, 64, true, true, T> W64;
+    typedef Shape<256, 256, 2, 4, 2, 64, false, false, 1> Z256;
+    typedef Shape<128, 64, 4, 1, 3, 64, false, false, 1> Z64;
+    typedef Shape<128, 16, 4, 1, 4, 64, false, false, 1> Z16;
+    typedef Shape<256, 256, 2, 4, 2, 64, true, false, 1> X256;
+    typedef Shape<256, 128, 2, 4, 2, 64, true, false, 1> X128;
+    typedef Shape<256, 64, 4, 1, 3, 64, true, false, 1> X64;
+    typedef Shape<256, 16, 4, 1, 3, 64, true, false, 1> X16;
+    typedef Shape<256, 256, 2, 4, 2, 64, true, true, 1> W256;
+    typedef Shape<128, 64, 4, 1, 3, 64, true, true, 1> W64;
 };
-// Tokens of a tile of the logits.  The tiles of 256 x 256 run at three times the rate of those of
-// 128 x 64, but where they leave more than half of the CUs without one, the small ones
-// are faster: 300 x 4000 x 333 f32, loss and gradients: 235 against 122 us.
+template <> struct Shapes<true> {
+    typedef Shape<256, 128, 4, 2, 2, 32, false, false, 6> Z128;
+    typedef Shape<128, 64, 4, 2, 4, 32, false, false, 6> Z64;
+    typedef Shape<128, 16, 4, 1, 4, 32, false, false, 6> Z16;
+    typedef Shape<256, 128, 4, 2, 2, 32, true, false, 6> X128;
+    typedef Shape<128, 64, 4, 2, 4, 32, true, false, 6> X64;
+    typedef Shape<128, 16, 4, 1, 4, 32, true, false, 6> X16;
+    typedef Shape<256, 128, 4, 2, 2, 32, true, true, 6> W128;
+    typedef Shape<128, 64, 4, 2, 4, 32, true, true, 6> W64;
+};
+
+// Tokens of a tile of the logits.  bf16: the tiles of 256 x 256 run at three times the rate of
+// those of 128 x 64, but where they leave more than half of the CUs without one, the
+// small ones are faster.  float32: 256 x 128 and 128 x 64 alike, by rounds over the CUs.
 bool fills(int64_t m, int64_t n) { return 2 * (int64_t)tiles(m, 256) * tiles(n, 256) > m2::cu_count(); }
-int z_tile(int64_t n, int64_t vocab) { return n <= 16 ? 16 : n <= 64 || !fills(vocab, n) ? 64 : 256; }
-int z_rows(int z) { return z < 256 ? 128 : 256; }
+bool large_planes(int64_t m, int64_t n) {
+    typedef Shapes<true>::Z128 L;
+    typedef Shapes<true>::Z64 S;
+    const int64_t ncu = m2::cu_count();
+    return L::STEP * (((int64_t)tiles(m, L::BM) * tiles(n, L::BN) + ncu - 1) / ncu) <=
+           S::STEP * (((int64_t)tiles(m, S::BM) * tiles(n, S::BN) + ncu - 1) / ncu);
+}
+int z_tile(int64_t n, int64_t vocab, bool f32) {
+    if (n <= 16) return 16;
+    if (f32) return n > 64 && large_planes(vocab, n) ? 128 : 64;
+    return n <= 64 || !fills(vocab, n) ? 64 : 256;
+}
+int z_rows(int z) { return z < 128 ? 128 : 256; }
 // parts of a tile whose sums EpiLse leaves apart
-int z_parts(int z) { return z < 256 ? 1 : 2; }
+int z_parts(int z, bool f32) { return f32 ? 4 : z < 256 ? 1 : 2; }
 
 // What the two entry points share: sizes, the packed operands and the tokens' arrays.
 struct Common {
@@ -774,7 +796,7 @@ Common common(int64_t n, int64_t vocab, int64_t dim, int64_t ldw, const void* w,
     c.np = (n + 63) / 64 * 64;
     c.dp = (dim + 63) / 64 * 64;
     c.f32 = dtype == M2_F32;
-    c.z = z_tile(n, vocab);
+    c.z = z_tile(n, vocab, c.f32);
     // the weights are read in place where direct loads can: bf16 rows of whole 16-byte
     // pieces (and offsets within a tile that fit 32 bits), of whole K steps for k_ce_tile; else
     // a copy in the workspace
@@ -799,7 +821,9 @@ template <bool F32, class EPI> void launch_z(Gemm& g, int z, int64_t rows, int64
     switch (z) {
         case 16: launch<typename P::Z16>(g, e, s); break;
         case 64: launch<typename P::Z64>(g, e, s); break;
-        default: launch<typename P::Z256>(g, e, s);
+        default:
+            if constexpr (F32) launch<typename P::Z128>(g, e, s);
+            else launch<typename P::Z256>(g, e, s);
     }
 }
 
@@ -829,7 +853,7 @@ FwdPlan fwd_plan(const m2_linear_cross_entropy_args& a) {
     size_t at = p.direct || a.saved ? 0 : p.c.at;
     auto take = [&](size_t b) { const size_t r = at; at += align256(b); return r; };
     p.zt = take(4 * (size_t)p.c.np);
-    p.part = take(8 * (size_t)z_parts(p.c.z) * tiles(a.vocab, z_rows(p.c.z)) * p.c.np);
+    p.part = take(8 * (size_t)z_parts(p.c.z, p.c.f32) * tiles(a.vocab, z_rows(p.c.z)) * p.c.np);
     p.sums = take(8 * (size_t)tiles(a.n, 16));
     p.total = at ? at : 256;
     return p;
@@ -864,24 +888,42 @@ BwdPlan bwd_plan(const m2_linear_cross_entropy_grad_args& a) {
     const int ncu = m2::cu_count();
     const int steps = (int)((a.vocab < p.piece ? a.vocab + 63 : p.piece) / 64);
     const int tm = tiles(a.dim, 256);
-    p.x = a.n <= 16 ? 16 : 64;
-    if (a.n > 64) {
-        p.splits = ncu;
-        p.x = deal(tm * tiles(a.n, 256), steps, ncu, 256).cost <= deal(tm * tiles(a.n, 128), steps, ncu, 128).cost ? 256
-                                                                                                           : 128;
-        int64_t segs = 0, all_segs = 0;
-        for (int k = 1; k <= tiles(a.n, p.x); ++k) {
-            const Deal d = deal(tm * k, steps, ncu, p.x);
+    // with the shape S: what its plan costs, and the most segments over the numbers of kept tokens
+    auto cost = [&](auto shape) {
+        typedef decltype(shape) S;
+        return deal(tiles(a.dim, S::BM) * tiles(a.n ? a.n : 1, S::BN), steps, ncu, S::STEP, S::SEG).cost;
+    };
+    int64_t all_segs = 0;
+    auto take_segs = [&](auto shape) {
+        typedef decltype(shape) S;
+        int64_t segs = 0;
+        for (int k = 1; k <= tiles(a.n ? a.n : 1, S::BN); ++k) {
+            const Deal d = deal(tiles(a.dim, S::BM) * k, steps, ncu, S::STEP, S::SEG);
             all_segs = d.full + (int64_t)d.rest * d.s;
             if (all_segs > segs) segs = all_segs;
         }
+        p.x = S::BN;
+        p.splits = ncu;
+        return 4 * (size_t)S::BM * S::BN * segs;
+    };
+    if (p.c.f32) {
+        typedef Shapes<true> P;
+        const size_t b = a.n <= 16 ? take_segs(P::X16())
+                         : a.n > 64 && cost(P::X128()) <= cost(P::X64()) ? take_segs(P::X128()) : take_segs(P::X64());
+        p.dx = a.grad_x ? take(b) : 0;
+        p.total = at;
+        return p;
+    }
+    if (a.n > 64) {
+        typedef Shapes<false> P;
+        const size_t b = cost(P::X256()) <= cost(P::X128()) ? take_segs(P::X256()) : take_segs(P::X128());
         if (2 * all_segs > ncu) {
-            p.dx = a.grad_x ? take(4 * 256 * (size_t)p.x * segs) : 0;
+            p.dx = a.grad_x ? take(b) : 0;
             p.total = at;
             return p;
         }
-        p.x = 64;                             // too few: the smaller tiles, as for the logits
     }
+    p.x = a.n <= 16 ? 16 : 64;                // few: the smaller tiles, as for the logits
     const int64_t t = (int64_t)tm * tiles(a.n ? a.n : 1, p.x);
     double best = 1e300;
     p.splits = 1;
@@ -960,7 +1002,7 @@ template <bool F32> int run_fwd(const m2_linear_cross_entropy_args& a, const Fwd
     g.b = Operand{reinterpret_cast<bf16*>(cm + c.x), c.dp, c.np * c.dp, (int)c.np, (int)c.dp};
     e.tgt = tk.tgt;
     launch_z<F32>(g, c.z, c.vocab, c.n, e, s);
-    j.parts = g.tm * z_parts(c.z);
+    j.parts = g.tm * z_parts(c.z, F32);
     hipLaunchKernelGGL(k_ce_join, dim3((unsigned)tiles(c.n, 16)), dim3(1024), 0, s, j, tk);
     return m2::check_launch("linear_cross_entropy");
 }
@@ -1006,20 +1048,29 @@ template <bool F32> int run_bwd(const m2_linear_cross_entropy_grad_args& a, cons
             d.a.lim = wlim;
             d.a.klim = (int)rows;
             d.b = Operand{G, p.piece, gplane, (int)c.np, (int)p.piece};
-            d.tm = tiles(c.dim, 256);
             d.tn = tiles(c.n, p.x);
-            if (p.x >= 128) {
-                if (q == 0) dxs.seg_nk = d.nk;
-                d.seg_nk = dxs.seg_nk;
-                if (p.x == 256) launch<typename P::X256>(d, EpiDxSeg{dxp, q > 0}, s);
-                else launch<typename P::X128>(d, EpiDxSeg{dxp, q > 0}, s);
-                dxs.tm = d.tm; dxs.tn = d.tn; dxs.nwg = p.splits;
+            if (q == 0) dxs.seg_nk = d.nk;
+            d.seg_nk = dxs.seg_nk;
+            const EpiDxSeg seg{dxp, q > 0};
+            auto go = [&](auto shape, const auto& e) {
+                typedef decltype(shape) S;
+                d.tm = tiles(c.dim, S::BM);
+                launch<S>(d, e, s);
+            };
+            if constexpr (F32) {
+                if (p.x == 128) go(typename P::X128(), seg);
+                else if (p.x == 64) go(typename P::X64(), seg);
+                else go(typename P::X16(), seg);
+            } else if (p.x >= 128) {
+                if (p.x == 256) go(typename P::X256(), seg);
+                else go(typename P::X128(), seg);
             } else {
                 if (d.splits > d.nk) d.splits = d.nk;             // a short last piece
                 const EpiDxSplit e{dxp, c.np, c.dp, q > 0};
-                if (p.x == 16) launch<typename P::X16>(d, e, s);
-                else launch<typename P::X64>(d, e, s);
+                if (p.x == 16) go(typename P::X16(), e);
+                else go(typename P::X64(), e);
             }
+            dxs.tm = d.tm; dxs.tn = d.tn; dxs.nwg = p.splits;
         }
         if (a.grad_weight) {
             Gemm d = g0;
@@ -1029,22 +1080,37 @@ template <bool F32> int run_bwd(const m2_linear_cross_entropy_grad_args& a, cons
             // against zero rows of x
             d.b = Operand{G, p.piece, gplane, (int)p.piece, c.z == 16 ? 16 : (int)c.np};
             EpiDw<T> e{static_cast<T*>(a.grad_weight) + v0 * c.dim, c.dim, (int)rows};
-            if (fills(c.dim, rows)) {
-                d.tm = tiles(c.dim, 256); d.tn = tiles(rows, 256);
-                launch<typename P::W256>(d, e, s);
+            auto go = [&](auto shape) {
+                typedef decltype(shape) S;
+                d.tm = tiles(c.dim, S::BM); d.tn = tiles(rows, S::BN);
+                launch<S>(d, e, s);
+            };
+            if constexpr (F32) {
+                if (large_planes(c.dim, rows)) go(typename P::W128());
+                else go(typename P::W64());
             } else {
-                d.tm = tiles(c.dim, 128); d.tn = tiles(rows, 64);
-                launch<typename P::W64>(d, e, s);
+                if (fills(c.dim, rows)) go(typename P::W256());
+                else go(typename P::W64());
             }
         }
     }
-    if (a.grad_x && p.x >= 128) {
-        dxs.part = dxp; dxs.dx = a.grad_x; dxs.n = c.n; dxs.dim = c.dim;
-        dxs.nred = dxs.tm * dxs.tn * (256 * p.x / (32 * 16) / 4);
-        const dim3 grid((unsigned)(dxs.nred + tiles(c.n, 64))), thr(256);
-        if (p.x == 256) hipLaunchKernelGGL((k_ce_dx_seg<T, typename P::X256>), grid, thr, 0, s, dxs, tk);
-        else hipLaunchKernelGGL((k_ce_dx_seg<T, typename P::X128>), grid, thr, 0, s, dxs, tk);
-    } else if (a.grad_x) {
+    if (!a.grad_x) return m2::check_launch("linear_cross_entropy_grad");
+    if (F32 || p.x >= 128) {
+        auto go = [&](auto shape) {
+            typedef decltype(shape) S;
+            dxs.part = dxp; dxs.dx = a.grad_x; dxs.n = c.n; dxs.dim = c.dim;
+            dxs.nred = (dxs.tm * dxs.tn * (S::NW * S::FM / 2 * S::FN) + 3) / 4;
+            hipLaunchKernelGGL((k_ce_dx_seg<T, S>), dim3((unsigned)(dxs.nred + tiles(c.n, 64))), dim3(256), 0, s, dxs, tk);
+        };
+        if constexpr (F32) {
+            if (p.x == 128) go(typename P::X128());
+            else if (p.x == 64) go(typename P::X64());
+            else go(typename P::X16());
+        } else {
+            if (p.x == 256) go(typename P::X256());
+            else go(typename P::X128());
+        }
+    } else {
         DxArgs d{dxp, a.grad_x, c.n, c.np, c.dp, c.dim, p.splits};
         hipLaunchKernelGGL((k_ce_dx<T>), dim3((unsigned)((c.n + 3) / 4), (unsigned)((c.dim + 511) / 512)),
                            dim3(256), 0, s, d, tk);

@@ -37,14 +37,14 @@ struct Gemm {
     Operand a, b;
     const int* count;    // tokens that take part (device), or NULL: n
     int n;
-    int nk;              // K steps of 64 (per plane product), 0: from count
+    int nk;              // K steps of 64, 0: from count
     int tm, tn;
     int tok_n;           // n is the token: tiles past the kept ones are left out
     int splits;          // k_ce_stream: K in so many parts
-    int seg_nk;          // k_ce_tile with EPI::SEG: the K steps that deal() goes by
+    int seg_nk;          // persistent kernels with EPI::SEG: the K steps that deal() goes by
 };
 
-// k_ce_tile with EPI::SEG: as many whole tiles as fill the workgroups, and the rest of the tiles
+// Persistent kernels with EPI::SEG: as many whole tiles as fill the workgroups, and the rest of the tiles
 // cut in s parts of K each, so that few workgroups are idle in the end.  Parts of the same
 // K lie beside each other (they share panels).  Segment numbers: the tile of a whole
 // one; full + part * rest + (tile - full).
@@ -192,7 +192,8 @@ template <int BM_, int BN_, int WM_, int WN_, int ST_, int BK_, bool ATR_, bool 
     static constexpr int SEG = BM * BN * 22 / 65536 + 1;
 };
 
-// Few tokens: the operand of the vocabulary streams from HBM through a deep ring
+// bf16, few tokens (or tiles): the operand of the vocabulary streams from HBM through a deep
+// ring, two workgroups a CU.  16 tokens over 50288 x 2560: 257 MB in 45 us, 5.7 TB/s.
 template <class S, class EPI>
 __global__ void __launch_bounds__(S::NT, 2 * S::LDS <= 160 * 1024 ? 2 : 1) k_ce_stream(Gemm g, EPI epi) {
     __shared__ __align__(1024) char smem[S::LDS];
@@ -328,17 +329,22 @@ template <class LD> struct Cursor {      // the step of an operand that is loade
     int k;
 };
 
-// Many tokens: persistent workgroups (whole tiles, or with EPI::SEG segments of them), each XCD with a contiguous range of the tiles
-// (neighbours share panels in its L2).  K in steps of 64, A through a ring of three slots, B of
-// two (all 160 KB for 256 x 256); the fragments of a half step (32 of K) are read while the half
-// step before multiplies, so the matrix units wait for neither LDS nor the
-// other wavefronts but once a step:
+// bf16, many tokens.  K in steps of 64, A through a ring of three slots, B of two (all
+// 160 KB for 256 x 256); the fragments of a half step (32 of K) are read while the half step
+// before multiplies, so the matrix units wait for neither LDS nor the other
+// wavefronts but once a step:
 //   half 0 of step i: multiply F0, read F1 (half 1 of step i), load A of step i + 2
 //   wait until step i + 1 has landed; barrier: everybody has read step i
 //   half 1 of step i: multiply F1, read F0 (half 0 of step i + 1), load B of step i + 2
 // so that both halves carry as many loads (all of them in one half leave too few cycles for
 // the 64 bytes a cycle that a CU takes in).  The loads run on into the next tile, whose first
 // steps arrive during the epilogue.
+// 8192 x 50288 x 2560 with EpiLse: 1.55 ms, 1.36 PFLOP/s (a library product of these sizes 1.75 ms).
+// The matrix units are busy in 70 % of the cycles, at the 1.82 GHz that the card's power leaves
+// them (with 59 % busy it ran at 1.9 GHz): what is left to gain in cycles the clock
+// takes back.  Measured and dropped: steps of 32 through a ring of four (a barrier twice
+// as often, half cache lines: 12 % slower), one contiguous round of tiles over all XCDs
+// (5 % slower: less of a panel stays in an XCD's L2).
 template <class S, class EPI>
 __global__ void __launch_bounds__(S::NT, S::NT / 256) k_ce_tile(Gemm g, EPI epi) {
     static_assert(S::BK == 64 && S::TERMS == 1, "");
@@ -468,7 +474,8 @@ __global__ void __launch_bounds__(S::NT, S::NT / 256) k_ce_tile(Gemm g, EPI epi)
 // what bounds a few tiles).  B's fragments of a step and those of one row of A's stay in
 // registers; the row after it is read while this one multiplies.  The last row of a step
 // multiplies behind the step's barrier, while the next step's first fragments are read
-// and the slot is filled again.
+// and the slot is filled again.  1024 x 50288 x 768, a quarter of the tokens left out: dw in
+// 305 us, 1.17 PFLOP/s of the six products (pair by pair 428 us).
 template <class S, class EPI>
 __global__ void __launch_bounds__(S::NT, S::NT / 256) k_ce_planes(Gemm g, EPI epi) {
     static_assert(S::BK == 32 && S::TERMS == 6 && S::FM % 2 == 0, "");

@@ -4,7 +4,7 @@
 //
 // The lookup is a gather of whole rows: a wavefront per (row, column part), 16 bytes a
 // lane, bound by HBM for many rows and by two dependent loads (id, row) for
-// few.
+// few: 16384 x 2560 bf16 25 us, 16 rows 2.8 us of GPU time in a call of 9.5.
 //
 // The gradient sorts (id, n) by id with a stable radix sort (equal ids keep the
 // order of n), walks the sorted list in pieces of up to 32 entries, one
@@ -21,7 +21,8 @@
 //
 // Up to 256 entries need neither sort nor partial rows: one launch, in which every entry
 // looks for its id among the others and the first of an id adds up all of them, while
-// further workgroups write the zeros of the rows that no id names.
+// further workgroups write the zeros of the rows that no id names (64 x 512 bf16 over 8000:
+// 12.4 us a call, 17.5 with sort and join).
 #include "m2_internal.h"
 
 #include <type_traits>

@@ -4,11 +4,11 @@
 //   z[n, v] = x[n] . w[v];  loss[n] = log sum_v exp(z[n, v]) - z[n, t[n]]
 //   G[n, v] = g[n] (exp(z[n, v] - lse[n]) - [v == t[n]]);  dx = G w;  dw = G^T x
 //
-// Forward: the product runs in tiles (ce_gemm.h); each tile leaves, per token, the
-// maximum m of its logits but the target's and the sum s of their exponentials
-// below it (8 bytes for 256 logits), and the target's logit z_t where it holds it.  A
-// second kernel joins the tiles: loss = log(1 + s exp(m - z_t)), which keeps its
-// accuracy down to losses far below the step of the logits.
+// Forward: the product runs in tiles (ce_gemm.h); each leaves, per token and 128 logits, the
+// maximum m of the logits but the target's and the sum s of their exponentials
+// below it (8 bytes), and the target's logit z_t where it holds it.  A second kernel
+// joins them: loss = log(1 + s exp(m - z_t)), which keeps its accuracy down to
+// losses far below the step of the logits.
 // Backward: a piece of the vocabulary at a time, the same product again gives G in its
 // epilogue (rounded to bf16 once, relative error 2^-9 of each, as the result's own
 // rounding; float32 operands keep three bf16 planes of it), then dw of the piece and
@@ -18,11 +18,16 @@
 // Tokens that are left out (ignore_index) are dropped at the start: the kept rows of x
 // are packed (zero-padded to whole K steps), so they cost nothing afterwards
 // and what stands in a row left out (a NaN, say) touches nothing.  The number of
-// kept tokens stays on the device; tiles past it end at once.
+// kept tokens stays on the device, where the tiles are dealt out by it.  Only
+// the scoring of up to 64 bf16 tokens reads x in place: every token is a column of its
+// own there, and the join passes over those left out.
 //
 // Bound by the matrix units for more than a few hundred tokens (2 n V D operations
 // forward, 6 n V D backward with the logits computed again), by reading the
-// weights for few.
+// weights for few.  bf16, 50288 x 2560: 16 tokens scored in 56 us (4.6 TB/s of weights), 4096
+// in 0.81 ms (1.30 PFLOP/s), loss and gradients of 8192 in 6.65 ms (1.27 PFLOP/s with the
+// logits computed twice).  Keeping the logits would save a quarter of the
+// latter and hold 1.6 GB instead of at most 512 MB of G.
 #include "ce_gemm.h"
 
 namespace {

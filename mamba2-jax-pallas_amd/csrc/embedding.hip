@@ -144,8 +144,13 @@ struct FillArgs {
     char* out;
     int64_t r0, r1, ldo, row;    // bytes
     int flat;                    // ldo == row, 16-byte aligned
+    int nt;                      // past the caches
 };
-constexpr int64_t FILL_BYTES = 64 << 10;     // of a workgroup, about
+// Non-temporal zeros leave grad where its producer put it, in the 256 MB cache that they would
+// fill, but run at HBM's rate, others at the cache's: 16384 x 2560 bf16 over 50288 (grad a
+// third of the result) 82 us against 101, 2047 x 768 f32 over 50277 (a 25th) 46 against
+// 34; the two meet at about an eighth.  Bytes of a workgroup: 64 KB with, 256 KB without.
+constexpr int64_t FILL_BYTES = 64 << 10;
 
 M2_DEV void fill(const FillArgs& f, int block, int blocks) {
     const u32x4 z = {0, 0, 0, 0};
@@ -153,8 +158,13 @@ M2_DEV void fill(const FillArgs& f, int block, int blocks) {
         const int64_t b0 = f.r0 * f.row, n = (f.r1 - f.r0) * f.row / 16;
         u32x4* p = reinterpret_cast<u32x4*>(f.out + b0);
         const int64_t i0 = n * block / blocks, i1 = n * (block + 1) / blocks;
+        if (f.nt) {
 #pragma unroll 4
-        for (int64_t i = i0 + threadIdx.x; i < i1; i += blockDim.x) p[i] = z;
+            for (int64_t i = i0 + threadIdx.x; i < i1; i += blockDim.x) __builtin_nontemporal_store(z, p + i);
+        } else {
+#pragma unroll 4
+            for (int64_t i = i0 + threadIdx.x; i < i1; i += blockDim.x) p[i] = z;
+        }
         // what 16-byte pieces leave of the last row
         if (block == 0 && threadIdx.x < (int)(((f.r1 - f.r0) * f.row - n * 16) >> 1))
             reinterpret_cast<uint16_t*>(p + n)[threadIdx.x] = 0;
@@ -710,7 +720,9 @@ int launch_embedding_grad(const m2_embedding_grad_args& a, hipStream_t s) {
     k.vocab = a.vocab; k.padding = a.padding_idx; k.n = (int)a.n; k.id64 = a.id_dtype == M2_I64;
     k.bits = p.bits;
     const int64_t osz = (int64_t)m2_dtype_size(a.out_dtype);
-    FillArgs f{static_cast<char*>(a.out), 0, 0, a.ldo * osz, a.dim * osz, 0};
+    FillArgs f{static_cast<char*>(a.out), 0, 0, a.ldo * osz, a.dim * osz, 0, 0};
+    f.nt = 8 * a.n * (int64_t)m2_dtype_size(a.grad_dtype) >= a.vocab * osz;
+    const int64_t fill_bytes = f.nt ? FILL_BYTES : 4 * FILL_BYTES;
     f.flat = a.ldo == a.dim && al16(a.out);
     // workgroups that write the zeros of rows r0 .. r1: a multiple of 16 rows keeps the next
     // part of a flat range on a 16-byte boundary
@@ -719,7 +731,7 @@ int launch_embedding_grad(const m2_embedding_grad_args& a, hipStream_t s) {
         if (a.accumulate) return 0;
         f.r0 = a.vocab * i / parts / 16 * 16;
         f.r1 = i + 1 == parts ? a.vocab : a.vocab * (i + 1) / parts / 16 * 16;
-        const int64_t b = ((f.r1 - f.r0) * f.row + FILL_BYTES - 1) / FILL_BYTES;
+        const int64_t b = ((f.r1 - f.r0) * f.row + fill_bytes - 1) / fill_bytes;
         return (unsigned)(b < most ? b : most);
     };
     int cur = 0;

@@ -12,8 +12,8 @@
 // overflows and long sums lose nothing, and the order is fixed, so equal inputs give equal
 // bits.  Every workgroup of the second pass adds the first one's sums up by itself,
 // and walks its pieces in the opposite order: what the first pass read last is still in the
-// 256 MB last-level cache.  130m float32 gradients (515 MB, 218 tensors): 330 us; 1.3b bf16
-// (2.7 GB): 1.55 ms, 5.2 TB/s of the three transfers.
+// 256 MB last-level cache.  130m float32 gradients (515 MB, 218 tensors): 300 us; 1.3b bf16
+// (2.7 GB): 1.5 ms, 5.4 TB/s of the three transfers.
 #include "m2_internal.h"
 
 namespace {
@@ -151,7 +151,8 @@ __global__ void __launch_bounds__(NT) k_norm(PassArgs a) {
     if (threadIdx.x == 0) *a.norm = norm;
 }
 
-__global__ void __launch_bounds__(NT) k_scale(PassArgs a) {
+// PAST: the results past the caches
+template <bool PAST> __global__ void __launch_bounds__(NT) k_scale(PassArgs a) {
     __shared__ double red[NT / 64];
     __shared__ int found[NT / 64];
     const float norm = norm_of(a, red);
@@ -179,8 +180,9 @@ __global__ void __launch_bounds__(NT) k_scale(PassArgs a) {
                         u32x4 o;
 #pragma unroll
                         for (int j = 0; j < 4; ++j) o[j] = pk_bf16(bf16_lo(r[j]) * c, bf16_hi(r[j]) * c);
-                        if (same) *reinterpret_cast<u32x4*>(y + i) = o;
-                        else store16(y + i, o);
+                        if (!same) store16(y + i, o);
+                        else if constexpr (PAST) __builtin_nontemporal_store(o, reinterpret_cast<u32x4*>(y + i));
+                        else *reinterpret_cast<u32x4*>(y + i) = o;
                     });
         } else {
             const int64_t i0 = (p - e.first) * (PIECE_BYTES / 4), i1 = min(e.n, i0 + PIECE_BYTES / 4);
@@ -191,8 +193,9 @@ __global__ void __launch_bounds__(NT) k_scale(PassArgs a) {
                         f32x4 r = *reinterpret_cast<const f32x4*>(x + i);
 #pragma unroll
                         for (int j = 0; j < 4; ++j) r[j] *= c;
-                        if (same) *reinterpret_cast<f32x4*>(y + i) = r;
-                        else store16(y + i, __builtin_bit_cast(u32x4, r));
+                        if (!same) store16(y + i, __builtin_bit_cast(u32x4, r));
+                        else if constexpr (PAST) __builtin_nontemporal_store(r, reinterpret_cast<f32x4*>(y + i));
+                        else *reinterpret_cast<f32x4*>(y + i) = r;
                     });
         }
     }
@@ -259,7 +262,11 @@ int launch_clip_grad_norm(const m2_clip_grad_norm_args& a, hipStream_t s) {
     if (b.count) send();
     p.parts = (int)(p.pieces < MAXWG ? p.pieces : MAXWG);
     if (p.parts) hipLaunchKernelGGL(k_sumsq, dim3(p.parts), dim3(NT), 0, s, p);
-    if (a.clip && p.parts) hipLaunchKernelGGL(k_scale, dim3(p.parts), dim3(NT), 0, s, p);
+    // tensors and results that do not both fit the last-level cache: the results go past it, and
+    // what the first pass read stays (515 MB: 352 to 317 us; 2.7 GB: 1586 to 1542)
+    const bool past = p.pieces > (128 << 20) / PIECE_BYTES;
+    if (a.clip && p.parts && past) hipLaunchKernelGGL(k_scale<true>, dim3(p.parts), dim3(NT), 0, s, p);
+    else if (a.clip && p.parts) hipLaunchKernelGGL(k_scale<false>, dim3(p.parts), dim3(NT), 0, s, p);
     else hipLaunchKernelGGL(k_norm, dim3(1), dim3(NT), 0, s, p);
     return check_launch(who);
 }

@@ -13,19 +13,43 @@ import torch
 from .. import _lib as L
 
 
+# (maps of these cost half as much per tensor as a loop that calls the methods, and a
+# model has hundreds of tensors)
+_ptr, _numel, _contiguous = torch.Tensor.data_ptr, torch.Tensor.numel, torch.Tensor.is_contiguous
+_CODES = {torch.float32: L.M2_F32, torch.bfloat16: L.M2_BF16}
+
+
 def _dense(t):
     """True when t's elements fill one block of memory, in any order of dimensions."""
     return t.is_contiguous() or torch.empty_like(t, device="meta").stride() == t.stride()
 
 
+def _device(tensors):
+    """The common GPU device of the tensors."""
+    try:
+        devices = set(map(torch.Tensor.get_device, tensors))
+    except TypeError:
+        devices = ()
+    if len(devices) == 1 and -1 not in devices:
+        return tensors[0].device
+    return L.device_of(*tensors)          # says what is wrong
+
+
+def _gathered(tensors):
+    if all(map(_contiguous, tensors)):
+        return tensors
+    return [t if _dense(t) else t.detach().contiguous() for t in tensors]
+
+
 def _run(dev, tensors, outs, max_norm, eps):
-    # a table of m2_tensor_ref (in, out, n, dtype), built without a Python loop over its rows
-    ins = [t.data_ptr() for t in tensors]
-    codes = [L.dtype_code(t, "a tensor") for t in tensors]
-    to = [0] * len(ins) if outs is None else [t.data_ptr() for t in outs]
-    refs = array("q", chain.from_iterable(zip(ins, to, [t.numel() for t in tensors], codes)))
+    # a table of m2_tensor_ref (in, out, n, dtype)
+    codes = [_CODES.get(t.dtype) for t in tensors]
+    if None in codes:
+        L.dtype_code(tensors[codes.index(None)], "a tensor")      # raises
+    to = [0] * len(tensors) if outs is None else map(_ptr, outs)
+    refs = array("q", chain.from_iterable(zip(map(_ptr, tensors), to, map(_numel, tensors), codes)))
     norm = torch.empty((), dtype=torch.float32, device=dev)
-    args = L.ClipGradNormArgs(refs.buffer_info()[0], len(ins), norm.data_ptr(), max_norm, eps,
+    args = L.ClipGradNormArgs(refs.buffer_info()[0], len(tensors), norm.data_ptr(), max_norm, eps,
                               int(outs is not None))
     L.call_with_workspace("m2_clip_grad_norm", args, dev)
     return norm
@@ -37,8 +61,8 @@ def global_norm(tensors):
     a fixed order."""
     tensors = list(tensors)
     L.require(len(tensors) > 0, "global_norm: no tensors")
-    dev = L.device_of(*tensors)
-    return _run(dev, [t if _dense(t) else t.detach().contiguous() for t in tensors], None, 0.0, 0.0)
+    dev = _device(tensors)
+    return _run(dev, _gathered(tensors), None, 0.0, 0.0)
 
 
 def clip_grad_norm(grads, max_norm, *, out=None, eps=1e-6):
@@ -57,20 +81,23 @@ def clip_grad_norm(grads, max_norm, *, out=None, eps=1e-6):
     max_norm, eps = float(max_norm), float(eps)
     L.require(max_norm >= 0 and eps >= 0, lambda: f"max_norm={max_norm}, eps={eps}: must not be negative")
     if out is None:
-        dev = L.device_of(*grads)
-        grads = [g if _dense(g) else g.detach().contiguous() for g in grads]
+        dev = _device(grads)
+        grads = _gathered(grads)
         outs = [torch.empty_like(g, requires_grad=False) for g in grads]
     else:
         outs = list(out)
         L.require(len(outs) == len(grads),
                   lambda: f"out holds {len(outs)} tensors for {len(grads)} gradients")
-        dev = L.device_of(*grads, *outs)
-        for i, (g, o) in enumerate(zip(grads, outs)):
-            if not (o.shape == g.shape and o.dtype == g.dtype
-                    and (o.is_contiguous() and g.is_contiguous()
-                         or o.stride() == g.stride() and _dense(o))):
-                raise L.M2ShapeError(f"out[{i}] must have the shape, dtype and strides of its "
-                                     "gradient, without gaps")
+        dev = _device(grads + outs)
+        if not ([g.shape for g in grads] == [o.shape for o in outs]
+                and [g.dtype for g in grads] == [o.dtype for o in outs]
+                and all(map(_contiguous, grads)) and all(map(_contiguous, outs))):
+            for i, (g, o) in enumerate(zip(grads, outs)):
+                if not (o.shape == g.shape and o.dtype == g.dtype
+                        and (o.is_contiguous() and g.is_contiguous()
+                             or o.stride() == g.stride() and _dense(o))):
+                    raise L.M2ShapeError(f"out[{i}] must have the shape, dtype and strides of its "
+                                         "gradient, without gaps")
     norm = _run(dev, grads, outs, max_norm, eps)
     if out is not None:
         torch.autograd.graph.increment_version(outs)

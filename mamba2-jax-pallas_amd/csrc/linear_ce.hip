@@ -865,7 +865,8 @@ FwdPlan fwd_plan(const m2_linear_cross_entropy_args& a) {
 }
 
 // G's workspace: 512 MB of it at most, in whole tiles of the vocabulary.  More
-// pieces cost launches and passes over the partial dx; less memory costs nothing else.
+// pieces cost launches and passes over the partial dx (8192 x 50288 x 2560: with 192 MB 6.92 ms
+// against 6.66, with 1 GB 6.67).
 constexpr int64_t G_BYTES = 512ll << 20;
 struct BwdPlan {
     Common c;

@@ -46,8 +46,8 @@ def _backward(ctx, grad):
     shape, n, ignore_index, reduction, index_code = ctx.args
     want_x, want_w = ctx.needs_input_grad[:2]
     dev, dim = weight.device, weight.shape[1]
-    dx = torch.empty(shape, dtype=weight.dtype, device=dev) if want_x else None
-    dw = torch.empty(weight.shape, dtype=weight.dtype, device=dev) if want_w else None
+    dx = weight.new_empty(shape) if want_x else None
+    dw = weight.new_empty(weight.shape) if want_w else None
     if n == 0:
         return dx, None if dw is None else dw.zero_(), None, None, None
     w = _rows(weight, dim)
@@ -101,13 +101,15 @@ def linear_cross_entropy(x, weight, targets, ignore_index=-100, reduction="mean"
     graph holds what the kernels read: a packed copy of x's kept rows, and of weight
     where it cannot be read in place (float32, as three bfloat16 parts: 1.5 times
     weight; a dim that 64 does not divide)."""
-    L.device_of(x, weight, targets)
+    L.device_of_two(x, weight)
+    L.device_of_two(x, targets)
+    shape = x.shape
     L.require(reduction in REDUCTIONS, lambda: f"reduction={reduction!r}: one of {REDUCTIONS}")
-    L.require(weight.dim() == 2 and x.dim() >= 1 and x.shape[-1] == weight.shape[1],
-              lambda: f"x.shape={tuple(x.shape)}, weight.shape={tuple(weight.shape)}: expected "
+    L.require(weight.dim() == 2 and shape and shape[-1] == weight.shape[1],
+              lambda: f"x.shape={tuple(shape)}, weight.shape={tuple(weight.shape)}: expected "
                       "(..., dim) and (vocab, dim)")
-    L.require(targets.shape == x.shape[:-1],
-              lambda: f"targets.shape={tuple(targets.shape)}: expected {tuple(x.shape[:-1])}")
+    L.require(targets.shape == shape[:-1],
+              lambda: f"targets.shape={tuple(targets.shape)}: expected {tuple(shape[:-1])}")
     L.require(weight.shape[0] > 0 and weight.shape[1] > 0, lambda: f"weight.shape={tuple(weight.shape)}")
     L.index_code(targets, "targets")
     if L.dtype_code(x, "x") != L.dtype_code(weight, "weight"):

@@ -35,9 +35,10 @@ def _dense(t):
 def _lookup(dev, ids, weight, scale):
     code, id_code = L.dtype_code(weight, "weight"), L.index_code(ids, "ids")
     vocab, dim = weight.shape
-    L.require(vocab > 0 and dim > 0, lambda: f"weight.shape={tuple(weight.shape)}")
+    if not (vocab and dim):
+        raise L.M2ShapeError(f"weight.shape={tuple(weight.shape)}")
     ids, w = _dense(ids), _rows(weight, dim)
-    out = torch.empty((*ids.shape, dim), dtype=weight.dtype, device=dev)
+    out = w.new_empty((*ids.shape, dim))
     n = ids.numel()
     if n:
         args = L.EmbeddingArgs(ids.data_ptr(), w.data_ptr(), out.data_ptr(), n, vocab, dim,
@@ -80,9 +81,11 @@ def embedding(ids, weight, scale=1.0, padding_idx=None):
     vocabulary cannot be reported without waiting for the GPU: its row is NaN,
     and it takes no part in the gradient.  padding_idx: an id whose gradient is left
     out (its row is looked up like any other)."""
-    dev = L.device_of(ids, weight)
-    L.require(weight.dim() == 2, lambda: f"weight.shape={tuple(weight.shape)}: expected (vocab, dim)")
-    padding_idx = _padding(padding_idx, weight.shape[0])
+    dev = L.device_of_two(weight, ids)
+    if weight.dim() != 2:
+        raise L.M2ShapeError(f"weight.shape={tuple(weight.shape)}: expected (vocab, dim)")
+    if padding_idx is not None:
+        padding_idx = _padding(padding_idx, weight.shape[0])
     scale = float(scale)
     if weight.requires_grad and torch.is_grad_enabled():
         return _Embedding.apply(ids, weight, scale, padding_idx)
@@ -99,7 +102,7 @@ def embedding_grad(ids, grad, num_embeddings, scale=1.0, padding_idx=None, *, dt
     (num_embeddings, dim) float32 or bfloat16 tensor that the rows named by
     ids are added into in place, the others left untouched, and that is returned: the
     gradient of an embedding tied to the head, after the head's."""
-    dev = L.device_of(ids, grad, out)
+    dev = L.device_of_two(grad, ids) if out is None else L.device_of(ids, grad, out)
     vocab = int(num_embeddings)
     L.require(0 < vocab < 2 ** 27, lambda: f"num_embeddings={vocab}")
     L.require(grad.dim() == ids.dim() + 1 and grad.shape[:-1] == ids.shape,
@@ -116,7 +119,7 @@ def embedding_grad(ids, grad, num_embeddings, scale=1.0, padding_idx=None, *, dt
                   and (vocab == 1 or out.stride(0) >= dim),
                   f"out must be ({vocab}, {dim}) with a contiguous last dimension")
     else:
-        out = torch.empty((vocab, dim), dtype=L.torch_dtype(dtype) or grad.dtype, device=dev)
+        out = g.new_empty((vocab, dim), dtype=None if dtype is None else L.torch_dtype(dtype))
     args = L.EmbeddingGradArgs(
         ids.data_ptr(), g.data_ptr(), out.data_ptr(), ids.numel(), vocab, dim, _stride(g, dim),
         _stride(out, dim), -1 if padding_idx is None else padding_idx, float(scale), id_code,

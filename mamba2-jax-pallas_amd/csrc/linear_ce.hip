@@ -10,8 +10,8 @@
 // joins them: loss = log(1 + s exp(m - z_t)), which keeps its accuracy down to
 // losses far below the step of the logits.
 // Backward: a piece of the vocabulary at a time, the same product again gives G in its
-// epilogue (rounded to bf16 once, relative error 2^-9 of each, as the result's own
-// rounding; float32 operands keep three bf16 planes of it), then dw of the piece and
+// epilogue (rounded to bf16 once, as the results are; what that takes from the target's is
+// given back, lost_of; float32 operands keep three bf16 planes of it), then dw of the piece and
 // the piece's part of dx, which float32 partial sums collect over pieces.  At
 // the target G is g expm1(-loss), not a difference of near-equal numbers.
 //
@@ -44,6 +44,7 @@ struct Tokens {              // of the kept tokens: in the workspace, or saved f
     float* em1;              // [np] expm1(-loss): G at the target
     int* count;              // [2] their number; workgroups of k_ce_join that are done
     float* zt;               // [np] the target's logit (forward)
+    float* lost;             // [np] what bf16 takes from G at the target (backward, EpiG)
 };
 
 M2_DEV int64_t load_target(const void* targets, int t64, int64_t i) {
@@ -364,17 +365,36 @@ M2_DEV void store_row(T* row, int m0, int64_t dim, int lane, const f32x4& x, con
     }
 }
 
+// The upstream gradient of the kept tokens' losses.
+struct Up {
+    const float* g;
+    int64_t stride;          // 0: one value
+    int mean;
+    M2_DEV float of(const Tokens& tk, int n, int count) const {
+        return g[stride ? tk.idx[n] * stride : 0] * (mean ? 1.f / (float)count : 1.f);
+    }
+};
+// What bf16 takes from G at the target, where most of a row's weight is, is up to 2^-8 of it
+// and the same for every column.  dx gets it back: 1.66e-3 off, as one rounding alone, where it
+// was 2.0 to 3.7e-3.  So does dw of up to 64 kept tokens; more average it out (2.2e-3 at
+// 320, 1.8e-3 at 4000), and frequent targets would make it cost (256 tokens over 20000
+// x 1024: 60 us of 145).
+M2_DEV float lost_of(const Tokens& tk, int n) { return tk.tgt[n] >= 0 ? tk.lost[n] : 0.f; }
+M2_DEV f32x4 load4(const bf16* p) {          // 8-byte aligned
+    typedef uint32_t u2 __attribute__((ext_vector_type(2)));
+    const u2 v = *reinterpret_cast<const u2*>(p);
+    return f32x4{bf16_lo(v[0]), bf16_hi(v[0]), bf16_lo(v[1]), bf16_hi(v[1])};
+}
+
 // m: vocabulary, n: token -> G, bf16 (three planes for float32 operands), zero past the
 // vocabulary and past the kept tokens
 struct EpiG {
     static constexpr bool SEG = false;
     Tokens tk;
-    const float* up;         // upstream gradient
+    Up up;
     bf16* G;
     int64_t ldg, plane;
-    int64_t ups;             // its stride (0: one value)
     int v_first, vocab;      // of the piece; of all
-    int mean;
 
     template <class S>
     M2_DEV void run(f32x4 (&acc)[S::FM][S::FN], char* smem, int m0, int n0, int wm, int wn, int lane, int count, int, int) const {
@@ -384,14 +404,13 @@ struct EpiG {
         // of the tokens, before the first store (a load behind it would wait for it)
         int t[S::FN];
         float ls[S::FN], g[S::FN], gt[S::FN];
-        const float scale = mean ? 1.f / (float)count : 1.f;
 #pragma unroll
         for (int j = 0; j < S::FN; ++j) {
             const int n = n0 + (wn * S::FN + j) * 16 + (lane & 15);
             const bool on = n < count;
             t[j] = on ? tk.tgt[n] : 0;
             ls[j] = on ? tk.lse[n] * -LOG2E : 0.f;
-            g[j] = on ? up[ups ? tk.idx[n] * ups : 0] * scale : 0.f;
+            g[j] = on ? up.of(tk, n, count) : 0.f;
             gt[j] = on ? g[j] * tk.em1[n] : 0.f;
             if (t[j] < 0) g[j] = __builtin_nanf("");       // a target outside the vocabulary
             t[j] -= v_first;
@@ -404,7 +423,9 @@ struct EpiG {
             if (n >= lim) continue;
             const bool on = n < count;
             const int d = on ? t[j] - mv : -1;
-            const bool here = __ballot(d >= 0 && d < 16 * S::FM && (d & 12) == 0);
+            const bool mine = d >= 0 && d < 16 * S::FM && (d & 12) == 0, here = __ballot(mine);
+            if (S::TERMS == 1 && mine)
+                tk.lost[n] = fabsf(gt[j]) < __builtin_inff() ? gt[j] - (float)(bf16)gt[j] : 0.f;
             bf16* to = G + (int64_t)n * ldg + mw + pair_m(lane);
 #pragma unroll
             for (int i = 0; i < S::FM; i += 2) {
@@ -497,19 +518,51 @@ struct EpiDxSeg {
 // m: dim, n: vocabulary -> rows of dw
 template <typename T> struct EpiDw {
     static constexpr bool SEG = false;
+    static constexpr int FEW = 64;           // up to so many kept tokens get back what G lost
     T* dw;
-    int64_t dim;
-    int rows;                // rows of the piece
+    int64_t dim, dp;
+    const bf16* x;           // packed, rows of dp
+    Tokens tk;
+    int v_first, rows;       // of the piece
 
     template <class S>
-    M2_DEV void run(f32x4 (&acc)[S::FM][S::FN], char* smem, int m0, int n0, int wm, int wn, int lane, int, int, int) const {
+    M2_DEV void run(f32x4 (&acc)[S::FM][S::FN], char* smem, int m0, int n0, int wm, int wn, int lane, int count, int,
+                    int) const {
+        const int mw = m0 + wm * S::FM * 16, nw = n0 + wn * S::FN * 16;
+        if constexpr (sizeof(T) == 2) {
+            // one more product for each token whose target is one of this wavefront's: its row of x
+            // against what G lost there (whose own rounding is 2^-8 of that)
+            if (count <= FEW) {
+                const int t = lane < count ? tk.tgt[lane] - v_first - nw : -1;
+                for (uint64_t hit = __ballot(t >= 0 && t < 16 * S::FN); hit; hit &= hit - 1) {
+                    const int k = __ffsll((unsigned long long)hit) - 1;
+                    const int at = __builtin_amdgcn_readlane(t, k);
+                    // K is this token alone: the first element of the first 16 lanes
+                    const bf16 zero = (bf16)0.f, r = (bf16)tk.lost[k];
+                    bf16x8 b = {lane == (at & 15) ? r : zero, zero, zero, zero, zero, zero, zero, zero};
+                    bf16x8 a = {zero, zero, zero, zero, zero, zero, zero, zero};
+                    bf16 v[S::FM];
+#pragma unroll
+                    for (int i = 0; i < S::FM; ++i)
+                        v[i] = x[(int64_t)k * dp + min((int64_t)mw + 16 * i + (lane & 15), dp - 1)];
+#pragma unroll
+                    for (int j = 0; j < S::FN; ++j)
+                        if (at >> 4 == j)
+#pragma unroll
+                            for (int i = 0; i < S::FM; ++i) {
+                                a[0] = lane < 16 ? v[i] : zero;
+                                acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, acc[i][j], 0, 0, 0);
+                            }
+                }
+            }
+        }
 #pragma unroll
         for (int j = 0; j < S::FN; ++j) {
-            const int n = n0 + (wn * S::FN + j) * 16 + (lane & 15);
+            const int n = nw + 16 * j + (lane & 15);
             if (n >= rows) continue;
 #pragma unroll
             for (int i = 0; i < S::FM; i += 2)
-                store_row(dw + (int64_t)n * dim, m0 + (wm * S::FM + i) * 16, dim, lane, acc[i][j], acc[i + 1][j]);
+                store_row(dw + (int64_t)n * dim, mw + 16 * i, dim, lane, acc[i][j], acc[i + 1][j]);
         }
     }
 };
@@ -643,40 +696,40 @@ __global__ void k_ce_nothing(float* total) { *total = 0.f; }      // of no token
 
 struct DxArgs {
     const float* part;
-    void* dx;
-    int64_t n, np, dp, dim;
+    bf16* dx;
+    const bf16* w;           // the weights, rows of ldw
+    int64_t n, np, dp, dim, ldw;
     int splits;
 };
 
 // dx of every row, 0 where it was left out: a wavefront per row and 512 columns
-template <typename T> __global__ void __launch_bounds__(256) k_ce_dx(DxArgs a, Tokens tk) {
+__global__ void __launch_bounds__(256) k_ce_dx(DxArgs a, Tokens tk) {
     const int64_t n = (int64_t)blockIdx.x * 4 + wave_id();
     if (n >= a.n) return;
     const int k = tk.inv[n];
-    T* d = static_cast<T*>(a.dx) + n * a.dim;
+    bf16* d = a.dx + n * a.dim;
     const int64_t c = (int64_t)blockIdx.y * 512 + (threadIdx.x & 63) * 8;
     if (c >= a.dim) return;
-    float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+    f32x4 x = zero4(), y = zero4();
     if (k >= 0) {
+        const float r = lost_of(tk, k);
+        const bf16* w = a.w + max(tk.tgt[k], 0) * a.ldw + c;
+        x = r * load4(w);
+        y = r * load4(w + 4);
         const float* p = a.part + (int64_t)k * a.dp + c;
 #pragma unroll 4
         for (int s = 0; s < a.splits; ++s, p += a.np * a.dp) {
-            const f32x4 x = *reinterpret_cast<const f32x4*>(p), y = *reinterpret_cast<const f32x4*>(p + 4);
-#pragma unroll
-            for (int i = 0; i < 4; ++i) { v[i] += x[i]; v[4 + i] += y[i]; }
+            x += *reinterpret_cast<const f32x4*>(p);
+            y += *reinterpret_cast<const f32x4*>(p + 4);
         }
     }
+    const u32x4 o = {pk_bf16(x[0], x[1]), pk_bf16(x[2], x[3]), pk_bf16(y[0], y[1]), pk_bf16(y[2], y[3])};
     if (c + 8 <= a.dim) {
-        if constexpr (sizeof(T) == 2) {
-            store16(d + c, u32x4{pk_bf16(v[0], v[1]), pk_bf16(v[2], v[3]), pk_bf16(v[4], v[5]), pk_bf16(v[6], v[7])});
-        } else {
-            store16(d + c, __builtin_bit_cast(u32x4, f32x4{v[0], v[1], v[2], v[3]}));
-            store16(d + c + 4, __builtin_bit_cast(u32x4, f32x4{v[4], v[5], v[6], v[7]}));
-        }
+        store16(d + c, o);
     } else {
 #pragma unroll
         for (int i = 0; i < 8; ++i)
-            if (c + i < a.dim) d[c + i] = from_f32<T>(v[i]);
+            if (c + i < a.dim) reinterpret_cast<uint16_t*>(d)[c + i] = (uint16_t)(o[i >> 1] >> (16 * (i & 1)));
     }
 }
 
@@ -685,7 +738,8 @@ template <typename T> __global__ void __launch_bounds__(256) k_ce_dx(DxArgs a, T
 struct DxSegArgs {
     const float* part;
     void* dx;
-    int64_t n, dim;
+    const bf16* w;           // the weights, rows of ldw
+    int64_t n, dim, ldw;
     int tm, tn, seg_nk, nwg, nred;
 };
 template <typename T, class S> __global__ void __launch_bounds__(256) k_ce_dx_seg(DxSegArgs a, Tokens tk) {
@@ -710,10 +764,19 @@ template <typename T, class S> __global__ void __launch_bounds__(256) k_ce_dx_se
     const int m0 = (grp * 8 + in % gm) * S::BM + (w / S::WN * S::FM + i) * 16;
     const int n = in / gm * S::BN + (w % S::WN * S::FN + j) * 16 + (lane & 15);
     if (n - (lane & 15) >= count || m0 >= a.dim) return;
+    f32x4 x = zero4(), y = zero4();
+    if (sizeof(T) == 2 && n < count) {
+        const float r = lost_of(tk, n);
+        const int m = m0 + 4 * (lane >> 4);
+        const bf16* w = a.w + max(tk.tgt[n], 0) * a.ldw + m;
+        if (m < a.dim) x = r * load4(w);
+        if (m + 16 < a.dim) y = r * load4(w + 16);
+    }
     const Deal d = deal(tiles, a.seg_nk, a.nwg, S::STEP, S::SEG);
     constexpr int64_t SEG = (int64_t)S::NW * S::FM * S::FN * 64;
     const f32x4* p = reinterpret_cast<const f32x4*>(a.part) + tile * SEG + (w * S::FM * S::FN + i * S::FN + j) * 64 + lane;
-    f32x4 x = p[0], y = p[S::FN * 64];
+    x += p[0];
+    y += p[S::FN * 64];
     if (tile >= d.full) {
 #pragma unroll 8
         for (int k = 1; k < d.s; ++k) {
@@ -873,7 +936,7 @@ struct BwdPlan {
     int64_t piece;
     int pieces;
     int x, splits;           // dx: tokens of a tile; parts of K (few tokens) or workgroups (many)
-    size_t G, dx, total;
+    size_t G, dx, lost, total;
 };
 BwdPlan bwd_plan(const m2_linear_cross_entropy_grad_args& a) {
     BwdPlan p{};
@@ -887,6 +950,7 @@ BwdPlan bwd_plan(const m2_linear_cross_entropy_grad_args& a) {
     p.pieces = (int)((all + most - 1) / most);
     p.piece = ((all / 256 + p.pieces - 1) / p.pieces) * 256;
     p.pieces = (int)((all + p.piece - 1) / p.piece);
+    p.lost = take(4 * (size_t)p.c.np);
     p.G = take(2 * planes * (size_t)(p.c.np ? p.c.np : 64) * p.piece);
     // dx: K is the piece.  Many tokens: dealt out with the tiles (k_ce_tile), whose number
     // depends on the tokens that are kept.  Few: split so that the tiles fill the CUs; a
@@ -1020,6 +1084,7 @@ template <bool F32> int run_bwd(const m2_linear_cross_entropy_grad_args& a, cons
     char* cm = a.saved ? static_cast<char*>(a.saved) : ws;
     const Common& c = p.c;
     Tokens tk = tokens(cm, c);
+    tk.lost = reinterpret_cast<float*>(ws + p.lost);
     PackArgs pa{};
     pa.targets = a.targets; pa.vocab = a.vocab; pa.t64 = a.target_dtype == M2_I64;
     pa.lse = a.lse; pa.loss = a.loss;
@@ -1031,6 +1096,7 @@ template <bool F32> int run_bwd(const m2_linear_cross_entropy_grad_args& a, cons
     g0.count = tk.count; g0.splits = 1;
     float* dxp = reinterpret_cast<float*>(ws + p.dx);
     const int wlim = (int)(c.pack_w ? c.dp : c.dim);
+    const Up up{a.grad_loss, a.grad_loss_stride, a.mean};
     DxSegArgs dxs{};
     for (int q = 0; q < p.pieces; ++q) {
         const int64_t v0 = q * p.piece;
@@ -1043,7 +1109,7 @@ template <bool F32> int run_bwd(const m2_linear_cross_entropy_grad_args& a, cons
         g.a.lim = (int)rows;
         g.a.klim = wlim;
         g.b = Operand{reinterpret_cast<bf16*>(cm + c.x), c.dp, c.np * c.dp, (int)c.np, (int)c.dp};
-        const EpiG eg{tk, a.grad_loss, G, p.piece, gplane, a.grad_loss_stride, (int)v0, (int)c.vocab, a.mean};
+        const EpiG eg{tk, up, G, p.piece, gplane, (int)v0, (int)c.vocab};
         launch_z<F32>(g, c.z, (rows + 63) / 64 * 64, c.n, eg, s);
         if (a.grad_x) {
             Gemm d = g0;
@@ -1085,7 +1151,7 @@ template <bool F32> int run_bwd(const m2_linear_cross_entropy_grad_args& a, cons
             // rows of G past a tile of 16 tokens are not there: its last row stands for them,
             // against zero rows of x
             d.b = Operand{G, p.piece, gplane, (int)p.piece, c.z == 16 ? 16 : (int)c.np};
-            EpiDw<T> e{static_cast<T*>(a.grad_weight) + v0 * c.dim, c.dim, (int)rows};
+            const EpiDw<T> e{static_cast<T*>(a.grad_weight) + v0 * c.dim, c.dim, c.dp, d.a.p, tk, (int)v0, (int)rows};
             auto go = [&](auto shape) {
                 typedef decltype(shape) S;
                 d.tm = tiles(c.dim, S::BM); d.tn = tiles(rows, S::BN);
@@ -1101,25 +1167,24 @@ template <bool F32> int run_bwd(const m2_linear_cross_entropy_grad_args& a, cons
         }
     }
     if (!a.grad_x) return m2::check_launch("linear_cross_entropy_grad");
-    if (F32 || p.x >= 128) {
-        auto go = [&](auto shape) {
-            typedef decltype(shape) S;
-            dxs.part = dxp; dxs.dx = a.grad_x; dxs.n = c.n; dxs.dim = c.dim;
-            dxs.nred = (dxs.tm * dxs.tn * (S::NW * S::FM / 2 * S::FN) + 3) / 4;
-            hipLaunchKernelGGL((k_ce_dx_seg<T, S>), dim3((unsigned)(dxs.nred + tiles(c.n, 64))), dim3(256), 0, s, dxs, tk);
-        };
-        if constexpr (F32) {
-            if (p.x == 128) go(typename P::X128());
-            else if (p.x == 64) go(typename P::X64());
-            else go(typename P::X16());
-        } else {
-            if (p.x == 256) go(typename P::X256());
-            else go(typename P::X128());
-        }
+    auto reduce = [&](auto shape) {
+        typedef decltype(shape) S;
+        dxs.part = dxp; dxs.dx = a.grad_x; dxs.n = c.n; dxs.dim = c.dim;
+        dxs.w = w.p; dxs.ldw = w.ld;
+        dxs.nred = (dxs.tm * dxs.tn * (S::NW * S::FM / 2 * S::FN) + 3) / 4;
+        hipLaunchKernelGGL((k_ce_dx_seg<T, S>), dim3((unsigned)(dxs.nred + tiles(c.n, 64))), dim3(256), 0, s, dxs, tk);
+    };
+    if constexpr (F32) {
+        if (p.x == 128) reduce(typename P::X128());
+        else if (p.x == 64) reduce(typename P::X64());
+        else reduce(typename P::X16());
+    } else if (p.x >= 128) {
+        if (p.x == 256) reduce(typename P::X256());
+        else reduce(typename P::X128());
     } else {
-        DxArgs d{dxp, a.grad_x, c.n, c.np, c.dp, c.dim, p.splits};
-        hipLaunchKernelGGL((k_ce_dx<T>), dim3((unsigned)((c.n + 3) / 4), (unsigned)((c.dim + 511) / 512)),
-                           dim3(256), 0, s, d, tk);
+        const DxArgs d{dxp, static_cast<bf16*>(a.grad_x), w.p, c.n, c.np, c.dp, c.dim, w.ld, p.splits};
+        hipLaunchKernelGGL(k_ce_dx, dim3((unsigned)((c.n + 3) / 4), (unsigned)((c.dim + 511) / 512)), dim3(256), 0, s, d,
+                           tk);
     }
     return m2::check_launch("linear_cross_entropy_grad");
 }

@@ -376,7 +376,7 @@ struct Up {
 };
 // What bf16 takes from G at the target, where most of a row's weight is, is up to 2^-8 of it
 // and the same for every column.  dx gets it back: 1.66e-3 off, as one rounding alone, where it
-// was 2.0 to 3.7e-3.  So does dw of up to 64 kept tokens; more average it out (2.2e-3 at
+// was 2.0 to 3.7e-3.  So does dw of up to 64 kept tokens (of 512); more average it out (2.2e-3 at
 // 320, 1.8e-3 at 4000), and frequent targets would make it cost (256 tokens over 20000
 // x 1024: 60 us of 145).
 M2_DEV float lost_of(const Tokens& tk, int n) { return tk.tgt[n] >= 0 ? tk.lost[n] : 0.f; }
@@ -515,10 +515,11 @@ struct EpiDxSeg {
     }
 };
 
-// m: dim, n: vocabulary -> rows of dw
-template <typename T> struct EpiDw {
+// m: dim, n: vocabulary -> rows of dw.  BACK: up to FEW kept tokens get back what G lost (a kernel of
+// its own: the registers cost the main loop a tenth of its rate)
+template <typename T, bool BACK> struct EpiDw {
     static constexpr bool SEG = false;
-    static constexpr int FEW = 64;           // up to so many kept tokens get back what G lost
+    static constexpr int FEW = 64;
     T* dw;
     int64_t dim, dp;
     const bf16* x;           // packed, rows of dp
@@ -529,7 +530,7 @@ template <typename T> struct EpiDw {
     M2_DEV void run(f32x4 (&acc)[S::FM][S::FN], char* smem, int m0, int n0, int wm, int wn, int lane, int count, int,
                     int) const {
         const int mw = m0 + wm * S::FM * 16, nw = n0 + wn * S::FN * 16;
-        if constexpr (sizeof(T) == 2) {
+        if constexpr (BACK) {
             // one more product for each token whose target is one of this wavefront's: its row of x
             // against what G lost there (whose own rounding is 2^-8 of that)
             if (count <= FEW) {
@@ -1151,11 +1152,14 @@ template <bool F32> int run_bwd(const m2_linear_cross_entropy_grad_args& a, cons
             // rows of G past a tile of 16 tokens are not there: its last row stands for them,
             // against zero rows of x
             d.b = Operand{G, p.piece, gplane, (int)p.piece, c.z == 16 ? 16 : (int)c.np};
-            const EpiDw<T> e{static_cast<T*>(a.grad_weight) + v0 * c.dim, c.dim, c.dp, d.a.p, tk, (int)v0, (int)rows};
             auto go = [&](auto shape) {
                 typedef decltype(shape) S;
                 d.tm = tiles(c.dim, S::BM); d.tn = tiles(rows, S::BN);
-                launch<S>(d, e, s);
+                T* dw = static_cast<T*>(a.grad_weight) + v0 * c.dim;
+                // (how many of n tokens are kept only the device knows: with more than 512 they
+                // are hardly ever as few as that)
+                if (!F32 && c.n <= 512) launch<S>(d, EpiDw<T, !F32>{dw, c.dim, c.dp, d.a.p, tk, (int)v0, (int)rows}, s);
+                else launch<S>(d, EpiDw<T, false>{dw, c.dim, c.dp, d.a.p, tk, (int)v0, (int)rows}, s);
             };
             if constexpr (F32) {
                 if (large_planes(c.dim, rows)) go(typename P::W128());

@@ -198,3 +198,45 @@ def test_weight_changed_before_the_gradient_is_refused():
     with torch.no_grad():
         xg.zero_()
     assert torch.equal(torch.autograd.grad(loss, xg)[0], want)
+
+
+@pytest.mark.parametrize("n", [3, 60, 300, 700])
+def test_ce_target_is_not_rounded(n):
+    """bfloat16: G at the target, most of a row's weight, rounds by up to 2^-8 of it in every column
+    alike, which dx (and dw of up to 64 tokens) gets back.  What is left are roundings of
+    either sign, each at most 2^-8 of its term: their sum over a row's columns with the
+    results' signs exceeds 6 times the root of the sum of their squares' bounds once in
+    3e7 rows (Hoeffding), where the one lost would be 2^-8 of the sum of all.  (The results' own
+    roundings have either sign where a row is a sum of several: dw of three tokens is nearly
+    one row of x times a number, whose roundings all depend on that number.)"""
+    announce("ce target", n)
+    dim, vocab, up = 2048, 1500, 1.0038          # 1.0038: a rounding of nearly half a step
+    g = gen(39, n)
+    w = (torch.randn((vocab, dim), generator=g, device=DEV) / dim ** 0.5).to(torch.bfloat16)
+    x = torch.randn((n, dim), generator=g, device=DEV).to(torch.bfloat16)
+    t = torch.randperm(vocab, generator=g, device=DEV)[:n]
+    xg, wg = x.clone().requires_grad_(), w.clone().requires_grad_()
+    loss = ops.linear_cross_entropy(xg, wg, t, reduction="sum")
+    dx, dw = torch.autograd.grad(loss, (xg, wg), torch.tensor(up, device=DEV))
+    X, W = x.double(), w.double()
+    z = X @ W.t()
+    G = torch.softmax(z, 1)
+    G[torch.arange(n, device=DEV), t] -= 1
+    G *= float(torch.tensor(up))
+    rounded = G.clone()
+    rounded[torch.arange(n, device=DEV), t] = 0              # the target's is not
+    e = 1e-4                                                 # the logits' and lse's errors, relative to a term
+    ub = 2.0 ** -8
+
+    def check(got, a, b, c, what):
+        ref = a @ b
+        s = ((got.double() - ref) * ref.sign()).sum(1).abs()
+        bound = 6 * ub * ((ref ** 2).sum(1).sqrt() + ((c ** 2) @ (b ** 2)).sum(1).sqrt()) \
+            + (e + ub ** 2) * (a.abs() @ b.abs()).sum(1)
+        print(f"  {what}: worst {float((s / bound).max()):.3f} of the bound", flush=True)
+        assert bool((s <= bound).all())
+        lost = ub * 0.9 * ref.abs().sum(1)
+        assert bool((lost > 2 * bound).all()), "the bound would not notice"
+    check(dx, G, W, rounded, "dx")
+    if n == 60:
+        check(dw[t], G.t()[t], X, rounded.t()[t], "dw")

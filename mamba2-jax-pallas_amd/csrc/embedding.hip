@@ -13,8 +13,7 @@
 // (frequent tokens) leaves one partial row per piece, which a second kernel
 // adds in order: no float atomics, so equal inputs give equal bits, and a token
 // that is half of the batch is spread over as many workgroups as any others.
-// The sort keeps one workgroup (of up to 16384 entries) or a few busy and is bound by
-// latencies; the rest of the chip meanwhile writes the zeros, which are most of a
+// The sort keeps one workgroup (of up to 16384 entries) or a few busy; the rest of the chip meanwhile writes the zeros, which are most of a
 // large vocabulary's gradient.  The rows that ids name are written twice that way, at
 // most n rows; zeroing the others alone would have to wait for the sort.  Bound
 // by HBM: grad read once, the result written once and those rows again.
@@ -201,22 +200,41 @@ __global__ void __launch_bounds__(SORT_THREADS) k_sort_hist(SortArgs a, FillArgs
     for (int d = t; d < bins; d += SORT_THREADS) a.hist[b * bins + d] = h[d];
 }
 
-// The place of an entry among the entries of its wavefront with the same
-// digit, and their number so far: lanes with equal digits find each other by
-// one ballot per bit; the first of them advances the wavefront's counter.
-M2_DEV int wave_rank(int digit, bool on, int bits, int* cnt) {
-    const int lane = threadIdx.x & 63;
-    uint64_t peers = __ballot(on);
-    for (int b = 0; b < bits; ++b) {
-        const bool one = (digit >> b) & 1;
-        const uint64_t m = __ballot(one);
-        peers &= one ? m : ~m;
+// The lanes with this lane's digit of BITS bits, by one ballot per bit (lanes that are not `on`
+// are nobody's).
+template <int BITS> M2_DEV uint64_t wave_peers(int digit, bool on) {
+    const uint64_t all = __ballot(on);
+    uint32_t lo = (uint32_t)all, hi = (uint32_t)(all >> 32);
+#pragma unroll
+    for (int b = 0; b < BITS; ++b) {
+        const int one = (digit << (31 - b)) >> 31;          // 0 or all bits
+        const uint64_t m = __ballot(one != 0);
+        lo &= ~((uint32_t)m ^ (uint32_t)one);
+        hi &= ~((uint32_t)(m >> 32) ^ (uint32_t)one);
     }
-    const int leader = __ffsll((unsigned long long)peers) - 1;
-    int old = 0;
-    if (on && lane == leader) old = atomicAdd(&cnt[digit], __popcll(peers));
-    old = __shfl(old, leader < 0 ? 0 : leader);
-    return old + __popcll(peers & ((1ull << lane) - 1));
+    return (uint64_t)hi << 32 | lo;
+}
+// The places of a thread's IT entries among those of their wavefront with the same digit, in
+// the order of j and of the lanes; their numbers are left in cnt.  Three passes, so that
+// the LDS accesses of all entries are under way together.
+template <int BITS, int IT, typename D, typename ON>
+M2_DEV void wave_ranks(D digit, ON on, int* cnt, int (&rank)[IT]) {
+    const int lane = threadIdx.x & 63;
+    const uint64_t below = (1ull << lane) - 1;
+    int first[IT];
+#pragma unroll
+    for (int j = 0; j < IT; ++j) {
+        const uint64_t peers = wave_peers<BITS>(digit(j), on(j));
+        first[j] = peers ? __ffsll((unsigned long long)peers) - 1 : 0;
+        rank[j] = __popcll(peers & below);
+        // the first of the lanes counts them all
+        if (on(j) && rank[j] == 0) rank[j] = atomicAdd(&cnt[digit(j)], __popcll(peers)) << 6;
+    }
+#pragma unroll
+    for (int j = 0; j < IT; ++j) {
+        const int base = __shfl(rank[j], first[j]) >> 6;
+        rank[j] = base + (lane == first[j] ? 0 : rank[j]);
+    }
 }
 
 // Exclusive prefix sums of v over the workgroup's NT threads, in thread order
@@ -253,9 +271,8 @@ __global__ void __launch_bounds__(SORT_THREADS) k_sort_scatter(SortArgs a, FillA
     }
     for (int d = t; d < NW * MAX_BINS; d += SORT_THREADS) (&cnt[0][0])[d] = 0;
     __syncthreads();
-#pragma unroll
-    for (int j = 0; j < SORT_ITEMS; ++j)
-        rank[j] = wave_rank((key[j] >> a.shift) & (bins - 1), base + 64 * j < a.n, a.bits, cnt[w]);
+    wave_ranks<9, SORT_ITEMS>([&](int j) { return (key[j] >> a.shift) & (bins - 1); },
+                              [&](int j) { return base + 64 * j < a.n; }, cnt[w], rank);
     __syncthreads();
     // where each (digit, wavefront) of this block begins: the entries of smaller digits in
     // all blocks, of this digit in earlier blocks and in earlier wavefronts.  Thread t
@@ -298,31 +315,34 @@ __global__ void __launch_bounds__(SORT_THREADS) k_sort_scatter(SortArgs a, FillA
 }
 
 // Up to SMALL_N entries of a vocabulary below 2^18: every pass in one workgroup, the list
-// in LDS between the passes, an entry in one word (key, position).  a.bits: of
-// every pass; a.nb: the passes.  16384 entries take two passes over 16 words a thread.
-template <int IT>
+// in LDS between the passes, an entry in one word (key, position).  a.nb passes of BITS bits;
+// 16384 entries are 16 words a thread.  One workgroup on one CU, bound by its vector
+// instructions (the ballots): 26 us at 16384 entries of 16 bits, 5 at 1000; the whole
+// gradient of 8192 x 64 takes 24.5 us (32.5 with 16 words a thread), of 16384 x 64 43, and
+// of 20000 x 64 by the sort over many workgroups 45.
+template <int IT, int BITS>
 __global__ void __launch_bounds__(SMALL_THREADS) k_sort_small(SortArgs a, FillArgs f) {
     constexpr int NW = SMALL_THREADS / 64;
     __shared__ int cnt[NW][MAX_BINS];
     __shared__ uint32_t list[SMALL_THREADS * IT];
     __shared__ int tmp[NW];
     if (blockIdx.x > 0) return fill(f, blockIdx.x - 1, gridDim.x - 1);
-    const int bins = 1 << a.bits, t = threadIdx.x, w = wave_id();
+    constexpr int bins = 1 << BITS;
+    const int t = threadIdx.x, w = wave_id();
     const int base = w * 64 * IT + (t & 63);
     uint32_t e[IT];
     int rank[IT];
 #pragma unroll
     for (int j = 0; j < IT; ++j) {
         const int i = base + 64 * j;
-        e[j] = i < a.n ? (uint32_t)key_of(a, i) << SMALL_POS | (uint32_t)i : 0;
+        e[j] = (uint32_t)key_of(a, min(i, a.n - 1)) << SMALL_POS | (uint32_t)i;      // used below n
     }
     for (int pass = 0; pass < a.nb; ++pass) {
-        const int shift = SMALL_POS + pass * a.bits;
-        for (int d = t; d < NW * bins; d += SMALL_THREADS) cnt[d >> a.bits][d & (bins - 1)] = 0;
+        const int shift = SMALL_POS + pass * BITS;
+        for (int d = t; d < NW * bins; d += SMALL_THREADS) cnt[d >> BITS][d & (bins - 1)] = 0;
         __syncthreads();
-#pragma unroll
-        for (int j = 0; j < IT; ++j)
-            rank[j] = wave_rank((e[j] >> shift) & (bins - 1), base + 64 * j < a.n, a.bits, cnt[w]);
+        wave_ranks<BITS, IT>([&](int j) { return (int)(e[j] >> shift) & (bins - 1); },
+                             [&](int j) { return base + 64 * j < a.n; }, cnt[w], rank);
         __syncthreads();
         int tot = 0;
         if (t < bins)
@@ -740,9 +760,21 @@ int launch_embedding_grad(const m2_embedding_grad_args& a, hipStream_t s) {
         k.nb = p.passes;
         k.keys_out = at(p.keys[0]); k.pos_out = at(p.pos[0]);
         const dim3 grid(1 + zeros(0, 8192)), thr(SMALL_THREADS);
-        if (a.n <= SMALL_THREADS) hipLaunchKernelGGL(k_sort_small<1>, grid, thr, 0, s, k, f);
-        else if (a.n <= 4 * SMALL_THREADS) hipLaunchKernelGGL(k_sort_small<4>, grid, thr, 0, s, k, f);
-        else hipLaunchKernelGGL(k_sort_small<16>, grid, thr, 0, s, k, f);
+        auto sort = [&](auto bits) {
+            constexpr int B = decltype(bits)::value;
+            auto run = [&](auto kernel) { hipLaunchKernelGGL(kernel, grid, thr, 0, s, k, f); };
+            if (a.n <= SMALL_THREADS) run(k_sort_small<1, B>);
+            else if (a.n <= 2 * SMALL_THREADS) run(k_sort_small<2, B>);
+            else if (a.n <= 4 * SMALL_THREADS) run(k_sort_small<4, B>);
+            else if (a.n <= 8 * SMALL_THREADS) run(k_sort_small<8, B>);
+            else if (a.n <= 12 * SMALL_THREADS) run(k_sort_small<12, B>);
+            else run(k_sort_small<16, B>);
+        };
+        // bits and words a thread as constants: the ballots are most of the time, and those of
+        // absent bits and entries cost as much
+        if (p.bits <= 7) sort(std::integral_constant<int, 7>());
+        else if (p.bits == 8) sort(std::integral_constant<int, 8>());
+        else sort(std::integral_constant<int, 9>());
     } else {
         k.nb = p.nb;
         for (int pass = 0; pass < p.passes; ++pass) {

@@ -240,3 +240,18 @@ def test_ce_target_is_not_rounded(n):
     check(dx, G, W, rounded, "dx")
     if n == 60:
         check(dw[t], G.t()[t], X, rounded.t()[t], "dw")
+
+
+@pytest.mark.parametrize("vocab", [1, 126, 255, 511, 512, 16383, 20000, 65535, 65536, 262142])
+@pytest.mark.parametrize("n", [1023, 2047, 2048, 2049, 4097, 8191, 8192, 8193, 12288, 12289, 16383])
+def test_embedding_grad_sorts(n, vocab):
+    """Whole numbers, whose sums are exact: every entry is added once, to its row."""
+    announce("embedding_grad sorts", n, vocab)
+    g = gen(35, n, vocab)
+    ids = make_ids(n, vocab, "any" if n & 1 else "zipf", g)
+    ids[n // 3] = vocab
+    ids[n // 2] = -1
+    grad = torch.randint(-100, 101, (n, 4), generator=g, device=DEV).float()
+    want = torch.zeros(vocab + 1, 4, dtype=torch.float64, device=DEV)
+    want.index_add_(0, torch.where((ids < 0) | (ids > vocab), vocab, ids).long(), grad.double())
+    assert torch.equal(ops.embedding_grad(ids, grad, vocab).double(), want[:vocab])

@@ -265,9 +265,9 @@ __global__ void __launch_bounds__(SORT_THREADS) k_sort_scatter(SortArgs a, FillA
     const int base = b * SORT_TILE + w * 64 * SORT_ITEMS + lane;
 #pragma unroll
     for (int j = 0; j < SORT_ITEMS; ++j) {
-        const int i = base + 64 * j;
-        key[j] = i < a.n ? (a.keys_in ? a.keys_in[i] : key_of(a, i)) : 0;
-        pos[j] = i < a.n && a.pos_in ? a.pos_in[i] : i;
+        const int i = base + 64 * j, at = min(i, a.n - 1);      // used below n
+        key[j] = a.keys_in ? a.keys_in[at] : key_of(a, at);
+        pos[j] = a.pos_in ? a.pos_in[at] : i;
     }
     for (int d = t; d < NW * MAX_BINS; d += SORT_THREADS) (&cnt[0][0])[d] = 0;
     __syncthreads();
@@ -284,6 +284,7 @@ __global__ void __launch_bounds__(SORT_THREADS) k_sort_scatter(SortArgs a, FillA
         const int d = t * D + k;
         tot[k] = before[k] = 0;
         if (d < bins)
+#pragma unroll 8
             for (int q = 0; q < a.nb; ++q) {
                 const int c = a.hist[q * bins + d];
                 tot[k] += c;
@@ -319,7 +320,7 @@ __global__ void __launch_bounds__(SORT_THREADS) k_sort_scatter(SortArgs a, FillA
 // 16384 entries are 16 words a thread.  One workgroup on one CU, bound by its vector
 // instructions (the ballots): 26 us at 16384 entries of 16 bits, 5 at 1000; the whole
 // gradient of 8192 x 64 takes 24.5 us (32.5 with 16 words a thread), of 16384 x 64 43, and
-// of 20000 x 64 by the sort over many workgroups 45.
+// of 20000 x 64 by the sort over many workgroups 41.
 template <int IT, int BITS>
 __global__ void __launch_bounds__(SMALL_THREADS) k_sort_small(SortArgs a, FillArgs f) {
     constexpr int NW = SMALL_THREADS / 64;

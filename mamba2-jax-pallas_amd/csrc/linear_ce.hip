@@ -370,14 +370,24 @@ struct Up {
     const float* g;
     int64_t stride;          // 0: one value
     int mean;
+    // of a token, in G; of all, where they have one value: dx and dw are multiplied by it behind
+    // their products and G is softmax - onehot alone.  Its bf16 at the target is then
+    // that of -1 + p, nearly exact for a small p, where the same value times 1 / count is off by
+    // the same up to 2^-8 in every row of dw that has a target (dw of 241 tokens over
+    // 1762: 2.4e-3 off, 2.0e-3 so; 1.7e-3 is the result's own rounding).
     M2_DEV float of(const Tokens& tk, int n, int count) const {
-        return g[stride ? tk.idx[n] * stride : 0] * (mean ? 1.f / (float)count : 1.f);
+        return stride ? g[tk.idx[n] * stride] * (mean ? 1.f / (float)count : 1.f) : 1.f;
+    }
+    M2_DEV float all(int count) const {
+        if (stride || count == 0) return 1.f;
+        // (a scalar load: a vector load would wait for the loads of the next tile)
+        return *(const __attribute__((address_space(4))) float*)(uintptr_t)g * (mean ? 1.f / (float)count : 1.f);
     }
 };
 // What bf16 takes from G at the target, where most of a row's weight is, is up to 2^-8 of it
 // and the same for every column.  dx gets it back: 1.66e-3 off, as one rounding alone, where it
-// was 2.0 to 3.7e-3.  So does dw of up to 64 kept tokens (of 512); more average it out (2.2e-3 at
-// 320, 1.8e-3 at 4000), and frequent targets would make it cost (256 tokens over 20000
+// was 2.0 to 3.7e-3.  So does dw of up to 64 kept tokens (of 512); more average it out (2.0e-3 at
+// 320, 1.7e-3 at 4000), and frequent targets would make it cost (256 tokens over 20000
 // x 1024: 60 us of 145).
 M2_DEV float lost_of(const Tokens& tk, int n) { return tk.tgt[n] >= 0 ? tk.lost[n] : 0.f; }
 M2_DEV f32x4 load4(const bf16* p) {          // 8-byte aligned
@@ -524,12 +534,14 @@ template <typename T, bool BACK> struct EpiDw {
     int64_t dim, dp;
     const bf16* x;           // packed, rows of dp
     Tokens tk;
+    Up up;
     int v_first, rows;       // of the piece
 
     template <class S>
     M2_DEV void run(f32x4 (&acc)[S::FM][S::FN], char* smem, int m0, int n0, int wm, int wn, int lane, int count, int,
                     int) const {
         const int mw = m0 + wm * S::FM * 16, nw = n0 + wn * S::FN * 16;
+        const float all = up.all(count);
         if constexpr (BACK) {
             // one more product for each token whose target is one of this wavefront's: its row of x
             // against what G lost there (whose own rounding is 2^-8 of that)
@@ -563,7 +575,7 @@ template <typename T, bool BACK> struct EpiDw {
             if (n >= rows) continue;
 #pragma unroll
             for (int i = 0; i < S::FM; i += 2)
-                store_row(dw + (int64_t)n * dim, mw + 16 * i, dim, lane, acc[i][j], acc[i + 1][j]);
+                store_row(dw + (int64_t)n * dim, mw + 16 * i, dim, lane, all * acc[i][j], all * acc[i + 1][j]);
         }
     }
 };
@@ -701,6 +713,7 @@ struct DxArgs {
     const bf16* w;           // the weights, rows of ldw
     int64_t n, np, dp, dim, ldw;
     int splits;
+    Up up;
 };
 
 // dx of every row, 0 where it was left out: a wavefront per row and 512 columns
@@ -723,6 +736,9 @@ __global__ void __launch_bounds__(256) k_ce_dx(DxArgs a, Tokens tk) {
             x += *reinterpret_cast<const f32x4*>(p);
             y += *reinterpret_cast<const f32x4*>(p + 4);
         }
+        const float all = a.up.all(*tk.count);
+        x *= all;
+        y *= all;
     }
     const u32x4 o = {pk_bf16(x[0], x[1]), pk_bf16(x[2], x[3]), pk_bf16(y[0], y[1]), pk_bf16(y[2], y[3])};
     if (c + 8 <= a.dim) {
@@ -742,6 +758,7 @@ struct DxSegArgs {
     const bf16* w;           // the weights, rows of ldw
     int64_t n, dim, ldw;
     int tm, tn, seg_nk, nwg, nred;
+    Up up;
 };
 template <typename T, class S> __global__ void __launch_bounds__(256) k_ce_dx_seg(DxSegArgs a, Tokens tk) {
     const int lane = threadIdx.x & 63;
@@ -786,7 +803,8 @@ template <typename T, class S> __global__ void __launch_bounds__(256) k_ce_dx_se
             y += p[S::FN * 64];
         }
     }
-    if (n < count) store_row(dx + (int64_t)tk.idx[n] * a.dim, m0, a.dim, lane, x, y);
+    const float all = a.up.all(count);
+    if (n < count) store_row(dx + (int64_t)tk.idx[n] * a.dim, m0, a.dim, lane, all * x, all * y);
 }
 
 // ---------------------------------------------------------------------------
@@ -1099,6 +1117,7 @@ template <bool F32> int run_bwd(const m2_linear_cross_entropy_grad_args& a, cons
     const int wlim = (int)(c.pack_w ? c.dp : c.dim);
     const Up up{a.grad_loss, a.grad_loss_stride, a.mean};
     DxSegArgs dxs{};
+    dxs.up = up;
     for (int q = 0; q < p.pieces; ++q) {
         const int64_t v0 = q * p.piece;
         const int64_t rows = c.vocab - v0 < p.piece ? c.vocab - v0 : p.piece;
@@ -1158,8 +1177,8 @@ template <bool F32> int run_bwd(const m2_linear_cross_entropy_grad_args& a, cons
                 T* dw = static_cast<T*>(a.grad_weight) + v0 * c.dim;
                 // (how many of n tokens are kept only the device knows: with more than 512 they
                 // are hardly ever as few as that)
-                if (!F32 && c.n <= 512) launch<S>(d, EpiDw<T, !F32>{dw, c.dim, c.dp, d.a.p, tk, (int)v0, (int)rows}, s);
-                else launch<S>(d, EpiDw<T, false>{dw, c.dim, c.dp, d.a.p, tk, (int)v0, (int)rows}, s);
+                if (!F32 && c.n <= 512) launch<S>(d, EpiDw<T, !F32>{dw, c.dim, c.dp, d.a.p, tk, up, (int)v0, (int)rows}, s);
+                else launch<S>(d, EpiDw<T, false>{dw, c.dim, c.dp, d.a.p, tk, up, (int)v0, (int)rows}, s);
             };
             if constexpr (F32) {
                 if (large_planes(c.dim, rows)) go(typename P::W128());
@@ -1186,7 +1205,7 @@ template <bool F32> int run_bwd(const m2_linear_cross_entropy_grad_args& a, cons
         if (p.x == 256) reduce(typename P::X256());
         else reduce(typename P::X128());
     } else {
-        const DxArgs d{dxp, static_cast<bf16*>(a.grad_x), w.p, c.n, c.np, c.dp, c.dim, w.ld, p.splits};
+        const DxArgs d{dxp, static_cast<bf16*>(a.grad_x), w.p, c.n, c.np, c.dp, c.dim, w.ld, p.splits, up};
         hipLaunchKernelGGL(k_ce_dx, dim3((unsigned)((c.n + 3) / 4), (unsigned)((c.dim + 511) / 512)), dim3(256), 0, s, d,
                            tk);
     }

@@ -255,3 +255,56 @@ def test_embedding_grad_sorts(n, vocab):
     want = torch.zeros(vocab + 1, 4, dtype=torch.float64, device=DEV)
     want.index_add_(0, torch.where((ids < 0) | (ids > vocab), vocab, ids).long(), grad.double())
     assert torch.equal(ops.embedding_grad(ids, grad, vocab).double(), want[:vocab])
+
+
+@pytest.mark.parametrize("n", [60, 700])
+def test_ce_target_each_loss(n):
+    """The same for a gradient of each loss, which G holds: dx gets back what rounding takes from
+    G at the target (the bound of test_ce_target's docstring: roundings of either sign)."""
+    announce("ce target, each loss", n)
+    dim, vocab = 2048, 1500
+    g = gen(40, n)
+    w = (torch.randn((vocab, dim), generator=g, device=DEV) / dim ** 0.5).to(torch.bfloat16)
+    x = torch.randn((n, dim), generator=g, device=DEV).to(torch.bfloat16)
+    t = torch.randint(0, vocab, (n,), generator=g, device=DEV)
+    up = torch.full((n,), 1.0038, device=DEV)
+    xg = x.clone().requires_grad_()
+    dx, = torch.autograd.grad(ops.linear_cross_entropy(xg, w, t, reduction="none"), xg, up)
+    G = torch.softmax(x.double() @ w.double().t(), 1)
+    G[torch.arange(n, device=DEV), t] -= 1
+    G *= up.double()[:, None]
+    rounded = G.clone()
+    rounded[torch.arange(n, device=DEV), t] = 0
+    W, ub = w.double(), 2.0 ** -8
+    ref = G @ W
+    s = ((dx.double() - ref) * ref.sign()).sum(1).abs()
+    bound = 6 * ub * ((ref ** 2).sum(1).sqrt() + ((rounded ** 2) @ (W ** 2)).sum(1).sqrt()) \
+        + (1e-4 + ub ** 2) * (G.abs() @ W.abs()).sum(1)
+    assert bool((s <= bound).all())
+    assert bool((0.9 * ub * ref.abs().sum(1) > 2 * bound).all()), "the bound would not notice"
+
+
+@pytest.mark.parametrize("n", [484, 600, 1210])
+@pytest.mark.parametrize("how", ["mean", "sum"])
+def test_ce_dw_one_gradient(n, how):
+    """bfloat16, one gradient for all losses: it is not part of what G rounds.  With zero
+    weights every logit is 0 and softmax 1 / 4096; rows of x cancel in pairs, so a target's row
+    of dw is its row of x times -up, up to 2^-12 by the rounding of -1 + 1 / 4096.  One
+    rounding of the result is left (2^-8), and float32's of sums over the tokens."""
+    announce("ce dw one gradient", n, how)
+    vocab, dim = 4096, 264
+    up = 1.0351 * (n if how == "mean" else 1)          # of each loss 1.0351: a rounding of nearly half a step
+    g = gen(41, n)
+    half = torch.randn((n // 2, dim), generator=g, device=DEV).to(torch.bfloat16)
+    x = torch.cat([half, -half])
+    w = torch.zeros((vocab, dim), device=DEV, dtype=torch.bfloat16, requires_grad=True)
+    t = torch.randperm(vocab, generator=g, device=DEV)[:n]
+    dw, = torch.autograd.grad(ops.linear_cross_entropy(x, w, t, reduction=how), w, torch.tensor(up, device=DEV))
+    each = float(torch.tensor(up)) / (n if how == "mean" else 1)
+    ref = torch.zeros((vocab, dim), dtype=torch.float64, device=DEV)
+    ref[t] = -each * x.double()
+    small = (n + 8) * 2.0 ** -24 * each * (x.double().abs().sum(0) / vocab)
+    tol = ref.abs() * (2.0 ** -8 + 2.0 ** -12 + 2.0 ** -16) + small
+    assert bool(((dw.double() - ref).abs() <= tol).all())
+    once = torch.tensor(each * (1 - 1 / vocab), device=DEV).bfloat16().double()      # rounded before x
+    assert bool((((-once * x.double()).bfloat16().double() - ref[t]).abs() > tol[t]).any()), "would not be noticed"

@@ -936,7 +936,10 @@ struct FwdPlan {
 FwdPlan fwd_plan(const m2_linear_cross_entropy_args& a) {
     FwdPlan p{};
     p.c = common(a.n, a.vocab, a.dim, a.ldw, a.weight, a.dtype);
-    p.direct = a.n <= 64 && !a.saved && !p.c.pack_w && a.ldx % 8 == 0 && al16(a.x);
+    // (the kernel's offsets within a tile are of 32 bits: rows that lie further apart, the last
+    // positions of long prompts, are packed, with 64-bit addresses)
+    p.direct = a.n <= 64 && !a.saved && !p.c.pack_w && a.ldx % 8 == 0 && al16(a.x) &&
+               a.ldx <= (1ll << 30) / (a.n > 1 ? a.n - 1 : 1);
     size_t at = p.direct || a.saved ? 0 : p.c.at;
     auto take = [&](size_t b) { const size_t r = at; at += align256(b); return r; };
     p.zt = take(4 * (size_t)p.c.np);

@@ -1,0 +1,28 @@
+"""What the vocabulary's operators once answered wrongly or refused too late, as far as it shows without
+a GPU."""
+
+import ctypes
+
+import pytest
+
+from mamba2_jax import _lib as L
+
+SCORE = dict(x=4096, weight=4096, targets=4096, loss=4096, n=16, vocab=50288, dim=2560, ldx=2560, ldw=2560,
+             ignore_index=-100, dtype=L.M2_BF16, target_dtype=L.M2_I64)
+
+
+def score_workspace(**over):
+    a = L.LinearCrossEntropyArgs(**{**SCORE, **over})
+    return L.load_library().m2_linear_cross_entropy_workspace_size(ctypes.byref(a))
+
+
+@pytest.mark.parametrize("n,near,far", [(16, 2560 * 1024, 2560 * 65536), (64, 2560 * 1024, 2560 * 16384),
+                                        (2, 2 ** 30, 2 ** 30 + 8), (64, 2 ** 30 // 63 // 8 * 8, 2 ** 31 // 63 // 8 * 8)])
+def test_far_rows_of_x_are_packed(n, near, far):
+    """Few tokens are scored with x read in place, whose offsets have 32 bits; rows that lie
+    further apart are packed first, into a workspace that is larger by them."""
+    packed = 2 * 64 * 2560
+    direct = score_workspace(n=n)
+    assert score_workspace(n=n, ldx=near) == direct
+    assert score_workspace(n=n, ldx=far) >= direct + packed
+    assert score_workspace(n=n, ldx=2 ** 60) >= direct + packed

@@ -264,7 +264,7 @@ __global__ void __launch_bounds__(S::NT, 2 * S::LDS <= 160 * 1024 ? 2 : 1) k_ce_
         }
         if (++slot == S::ST) slot = 0;
     }
-    epi.template run<S>(acc, smem, m0, n0, wm, wn, lane, count, split, tm);
+    epi.template run<S>(acc, m0, n0, wm, wn, lane, count, split, tm);
 }
 
 struct Work {                 // of a workgroup: its item i, a tile and its K steps of 64
@@ -462,7 +462,7 @@ __global__ void __launch_bounds__(S::NT, S::NT / 256) k_ce_tile(Gemm g, EPI epi)
         }
         // what is loaded so far (step 0 and 1 of the next tile) is there before any store
         wait_vmem<0>();
-        epi.template run<S>(acc, nullptr, m0, n0, wm, wn, lane, count, wk.seg, tm);
+        epi.template run<S>(acc, m0, n0, wm, wn, lane, count, wk.seg, tm);
     }
     wait_vmem<0>();           // no load may land after the workgroup has ended
 }
@@ -586,7 +586,7 @@ __global__ void __launch_bounds__(S::NT, S::NT / 256) k_ce_planes(Gemm g, EPI ep
             step(b0, b1);
             step(b1, b0);
         }
-        epi.template run<S>(acc, nullptr, m0, n0, wm, wn, lane, count, wk.seg, tm);
+        epi.template run<S>(acc, m0, n0, wm, wn, lane, count, wk.seg, tm);
     }
     wait_vmem<0>();           // no load may land after the workgroup has ended
 }

@@ -255,7 +255,10 @@ struct EpiLse {
     }
 
     template <class S>
-    M2_DEV void run(f32x4 (&acc)[S::FM][S::FN], char* smem, int m0, int n0, int wm, int wn, int lane, int count, int, int tm) const {
+    M2_DEV void run(f32x4 (&acc)[S::FM][S::FN], int m0, int n0, int wm, int wn, int lane, int count, int, int tm) const {
+        // (LDS of their own: the operands' ring may still be read by other wavefronts)
+        constexpr bool JOIN = S::BN < 128 && S::TERMS == 1;
+        __shared__ float2 sums[JOIN ? S::WM * S::BN : 1];
         const int v0 = m0 + wm * S::FM * 16 + 4 * (lane >> 4);
         const float ninf = -__builtin_inff();
         if (m0 + S::BM > vocab) {
@@ -298,19 +301,19 @@ struct EpiLse {
                 for (int r = 0; r < 4; ++r) s += __builtin_amdgcn_exp2f(fmaf(acc[i][j][r], LOG2E, b));
             s += __shfl_xor(s, 16);
             s += __shfl_xor(s, 32);
-            if constexpr (S::BN < 128 && S::TERMS == 1) {
-                if (lane < 16) reinterpret_cast<float2*>(smem)[wm * S::BN + n - n0] = make_float2(mx, s);
+            if constexpr (JOIN) {
+                if (lane < 16) sums[wm * S::BN + n - n0] = make_float2(mx, s);
             } else {
                 if (lane < 16 && n < count) part[((int64_t)tm * S::WM + wm) * np + n] = make_float2(mx, s);
             }
         }
-        if constexpr (S::BN < 128 && S::TERMS == 1) {
+        if constexpr (JOIN) {
             __syncthreads();
             const int t = threadIdx.x;
             if (t < S::BN && n0 + t < count) {
                 LogSum o = {};
 #pragma unroll
-                for (int q = 0; q < S::WM; ++q) o.add(reinterpret_cast<const float2*>(smem)[q * S::BN + t]);
+                for (int q = 0; q < S::WM; ++q) o.add(sums[q * S::BN + t]);
                 part[(int64_t)tm * np + n0 + t] = make_float2(o.mx, o.s);
             }
         }
@@ -407,7 +410,7 @@ struct EpiG {
     int v_first, vocab;      // of the piece; of all
 
     template <class S>
-    M2_DEV void run(f32x4 (&acc)[S::FM][S::FN], char* smem, int m0, int n0, int wm, int wn, int lane, int count, int, int) const {
+    M2_DEV void run(f32x4 (&acc)[S::FM][S::FN], int m0, int n0, int wm, int wn, int lane, int count, int, int) const {
         static_assert(S::FM % 2 == 0, "");
         const int mw = m0 + wm * S::FM * 16, mv = mw + 4 * (lane >> 4);
         const int lim = (count + 63) & ~63;
@@ -483,7 +486,7 @@ struct EpiDxSplit {
     int add;
 
     template <class S>
-    M2_DEV void run(f32x4 (&acc)[S::FM][S::FN], char* smem, int m0, int n0, int wm, int wn, int lane, int count, int split,
+    M2_DEV void run(f32x4 (&acc)[S::FM][S::FN], int m0, int n0, int wm, int wn, int lane, int count, int split,
                     int) const {
         const int mv = m0 + wm * S::FM * 16 + 4 * (lane >> 4);
 #pragma unroll
@@ -509,7 +512,7 @@ struct EpiDxSeg {
     int add;
 
     template <class S>
-    M2_DEV void run(f32x4 (&acc)[S::FM][S::FN], char* smem, int, int, int wm, int wn, int lane, int, int seg, int) const {
+    M2_DEV void run(f32x4 (&acc)[S::FM][S::FN], int, int, int wm, int wn, int lane, int, int seg, int) const {
         f32x4* d = reinterpret_cast<f32x4*>(part) +
                    ((int64_t)seg * S::NW + wm * S::WN + wn) * S::FM * S::FN * 64 + lane;
         if (add) {
@@ -538,7 +541,7 @@ template <typename T, bool BACK> struct EpiDw {
     int v_first, rows;       // of the piece
 
     template <class S>
-    M2_DEV void run(f32x4 (&acc)[S::FM][S::FN], char* smem, int m0, int n0, int wm, int wn, int lane, int count, int,
+    M2_DEV void run(f32x4 (&acc)[S::FM][S::FN], int m0, int n0, int wm, int wn, int lane, int count, int,
                     int) const {
         const int mw = m0 + wm * S::FM * 16, nw = n0 + wn * S::FN * 16;
         const float all = up.all(count);

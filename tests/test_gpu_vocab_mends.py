@@ -26,3 +26,18 @@ def test_score_rows_far_apart(n, apart, dtype):
     loss = ops.linear_cross_entropy(far, w, t, reduction="none")
     within(loss, r.loss, r.loss_tol, "loss")
     assert not bool(loss[t == IGN].any())
+
+
+@pytest.mark.parametrize("n", [1, 16, 17, 64])
+@pytest.mark.parametrize("dim", [64, 192, 256, 320, 448, 576, 832, 2560])
+def test_score_last_step_in_each_slot(n, dim):
+    """Few tokens: the wavefronts of a tile put their sums together in LDS that no operand lies in,
+    whichever slot of the ring (of four up to 16 tokens, of three beyond) the last K step
+    is in.  16 runs of more tiles than the card has CUs, equal to the bit."""
+    announce("last step in each slot", n, dim)
+    x, w, t = ce_inputs(n, 128 * 300, dim, "bf16", key=51)
+    r = Ref(x, w, t, torch.ones(n, device=DEV, dtype=torch.float64))
+    loss = ops.linear_cross_entropy(x, w, t, reduction="none")
+    within(loss, r.loss, r.loss_tol, "loss")
+    for _ in range(15):
+        assert torch.equal(ops.linear_cross_entropy(x, w, t, reduction="none"), loss)

@@ -2,11 +2,14 @@
 a GPU."""
 
 import ctypes
+import os
+import re
 
 import pytest
 
 from mamba2_jax import _lib as L
 
+CSRC = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(L.__file__))), "csrc")
 SCORE = dict(x=4096, weight=4096, targets=4096, loss=4096, n=16, vocab=50288, dim=2560, ldx=2560, ldw=2560,
              ignore_index=-100, dtype=L.M2_BF16, target_dtype=L.M2_I64)
 
@@ -26,3 +29,12 @@ def test_far_rows_of_x_are_packed(n, near, far):
     assert score_workspace(n=n, ldx=near) == direct
     assert score_workspace(n=n, ldx=far) >= direct + packed
     assert score_workspace(n=n, ldx=2 ** 60) >= direct + packed
+
+
+def test_epilogues_do_not_see_the_ring():
+    """Behind the last K step no barrier says that every wavefront has read its operands, so an
+    epilogue must not write to the ring that holds them: it is not given it.  (A race cannot be
+    shown by running it.)"""
+    with open(os.path.join(CSRC, "ce_gemm.h")) as f:
+        calls = re.findall(r"epi\.template run<S>\(([^;]*)\);", f.read())
+    assert len(calls) == 3 and not any("smem" in c or "lds" in c for c in calls)

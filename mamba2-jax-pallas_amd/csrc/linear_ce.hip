@@ -45,7 +45,9 @@ struct Tokens {              // of the kept tokens: in the workspace, or saved f
     int* count;              // [2] their number; workgroups of k_ce_join that are done
     float* zt;               // [np] the target's logit (forward)
     float* lost;             // [np] what bf16 takes from G at the target (backward, EpiG)
+    int* first;              // [vocab] the first kept token with this target, or NONE
 };
+constexpr int NONE = 0x7fffffff;
 
 M2_DEV int64_t load_target(const void* targets, int t64, int64_t i) {
     return t64 ? reinterpret_cast<const int64_t*>(targets)[i] : (int64_t) reinterpret_cast<const int32_t*>(targets)[i];
@@ -148,8 +150,10 @@ struct PackArgs {
     const float* loss;
     int64_t vocab, n, ignore;
     int t64;
+    int row_blocks;          // further workgroups clear tk.first
 };
 constexpr int64_t PACK_FINDS = 1024;     // up to so many tokens the packing finds the kept ones itself
+constexpr int CLEAR = 2048;              // entries of Tokens::first that one workgroup clears
 
 // Rows of src as bf16 (planes) with rows of dp elements, zeros behind dim: the weights
 // where they cannot be read in place, or the kept rows of x (TOK), with zero rows up to
@@ -161,6 +165,11 @@ __global__ void __launch_bounds__(256) k_ce_pack(PackArgs a, Tokens tk) {
     const int lane = threadIdx.x & 63;
     int64_t from = r;
     if constexpr (TOK) {
+        if ((int)blockIdx.x >= a.row_blocks) {
+            const int64_t v0 = (int64_t)(blockIdx.x - a.row_blocks) * CLEAR;
+            for (int64_t v = v0 + threadIdx.x; v < min(v0 + CLEAR, a.vocab); v += 256) tk.first[v] = NONE;
+            return;
+        }
         if (a.n <= PACK_FINDS) {
             if (r >= a.n + 64) return;
             int before = 0;
@@ -388,11 +397,13 @@ struct Up {
     }
 };
 // What bf16 takes from G at the target, where most of a row's weight is, is up to 2^-8 of it
-// and the same for every column.  dx gets it back: 1.66e-3 off, as one rounding alone, where it
-// was 2.0 to 3.7e-3.  So does dw of up to 64 kept tokens (of 512); more average it out (2.0e-3 at
-// 320, 1.7e-3 at 4000), and frequent targets would make it cost (256 tokens over 20000
-// x 1024: 60 us of 145).
+// and the same for every column.  dx and dw get it back in float32: dx is 1.66e-3 off, as one
+// rounding alone, where it was 2.0 to 3.7e-3, dw of 300 tokens over 32003 x 1001 1.44e-3 (1.71)
 M2_DEV float lost_of(const Tokens& tk, int n) { return tk.tgt[n] >= 0 ? tk.lost[n] : 0.f; }
+M2_DEV float lost_at(float gt) {
+    const float r = gt - (float)(bf16)gt;
+    return fabsf(r) < __builtin_inff() ? r : 0.f;         // (an infinity or NaN is G itself)
+}
 M2_DEV f32x4 load4(const bf16* p) {          // 8-byte aligned
     typedef uint32_t u2 __attribute__((ext_vector_type(2)));
     const u2 v = *reinterpret_cast<const u2*>(p);
@@ -438,7 +449,7 @@ struct EpiG {
             const int d = on ? t[j] - mv : -1;
             const bool mine = d >= 0 && d < 16 * S::FM && (d & 12) == 0, here = __ballot(mine);
             if (S::TERMS == 1 && mine)
-                tk.lost[n] = fabsf(gt[j]) < __builtin_inff() ? gt[j] - (float)(bf16)gt[j] : 0.f;
+                tk.lost[n] = lost_at(gt[j]);
             bf16* to = G + (int64_t)n * ldg + mw + pair_m(lane);
 #pragma unroll
             for (int i = 0; i < S::FM; i += 2) {
@@ -528,48 +539,35 @@ struct EpiDxSeg {
     }
 };
 
-// m: dim, n: vocabulary -> rows of dw.  BACK: up to FEW kept tokens get back what G lost (a kernel of
-// its own: the registers cost the main loop a tenth of its rate)
-template <typename T, bool BACK> struct EpiDw {
+// m: dim, n: vocabulary -> rows of dw, with what G lost at the targets (bf16: back, k_ce_back)
+template <typename T> struct EpiDw {
     static constexpr bool SEG = false;
-    static constexpr int FEW = 64;
     T* dw;
     int64_t dim, dp;
-    const bf16* x;           // packed, rows of dp
-    Tokens tk;
+    const float* back;       // [np][dp], the rows of the first token of each target
+    const int* first;        // of the piece
     Up up;
-    int v_first, rows;       // of the piece
+    int rows;                // of the piece
 
     template <class S>
-    M2_DEV void run(f32x4 (&acc)[S::FM][S::FN], int m0, int n0, int wm, int wn, int lane, int count, int,
-                    int) const {
+    M2_DEV void run(f32x4 (&acc)[S::FM][S::FN], int m0, int n0, int wm, int wn, int lane, int count, int, int) const {
         const int mw = m0 + wm * S::FM * 16, nw = n0 + wn * S::FN * 16;
         const float all = up.all(count);
-        if constexpr (BACK) {
-            // one more product for each token whose target is one of this wavefront's: its row of x
-            // against what G lost there (whose own rounding is 2^-8 of that)
-            if (count <= FEW) {
-                const int t = lane < count ? tk.tgt[lane] - v_first - nw : -1;
-                for (uint64_t hit = __ballot(t >= 0 && t < 16 * S::FN); hit; hit &= hit - 1) {
-                    const int k = __ffsll((unsigned long long)hit) - 1;
-                    const int at = __builtin_amdgcn_readlane(t, k);
-                    // K is this token alone: the first element of the first 16 lanes
-                    const bf16 zero = (bf16)0.f, r = (bf16)tk.lost[k];
-                    bf16x8 b = {lane == (at & 15) ? r : zero, zero, zero, zero, zero, zero, zero, zero};
-                    bf16x8 a = {zero, zero, zero, zero, zero, zero, zero, zero};
-                    bf16 v[S::FM];
+        if constexpr (sizeof(T) == 2) {
+            int k[S::FN];
 #pragma unroll
-                    for (int i = 0; i < S::FM; ++i)
-                        v[i] = x[(int64_t)k * dp + min((int64_t)mw + 16 * i + (lane & 15), dp - 1)];
+            for (int j = 0; j < S::FN; ++j) {
+                const int n = nw + 16 * j + (lane & 15);
+                k[j] = n < rows ? first[n] : NONE;
+            }
 #pragma unroll
-                    for (int j = 0; j < S::FN; ++j)
-                        if (at >> 4 == j)
+            for (int j = 0; j < S::FN; ++j) {
+                if (k[j] == NONE) continue;
+                const int m = mw + 4 * (lane >> 4);
+                const float* b = back + k[j] * dp + m;
 #pragma unroll
-                            for (int i = 0; i < S::FM; ++i) {
-                                a[0] = lane < 16 ? v[i] : zero;
-                                acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, acc[i][j], 0, 0, 0);
-                            }
-                }
+                for (int i = 0; i < S::FM; ++i)
+                    if (m + 16 * i < dp) acc[i][j] += *reinterpret_cast<const f32x4*>(b + 16 * i);
             }
         }
 #pragma unroll
@@ -582,6 +580,103 @@ template <typename T, bool BACK> struct EpiDw {
         }
     }
 };
+
+// ---------------------------------------------------------------------------
+// what G lost at the targets, for dw
+// ---------------------------------------------------------------------------
+struct BackArgs {
+    const bf16* x;           // packed, rows of dp
+    float* back;             // out [np][dp]
+    int64_t dp;
+    int v_first, rows;       // of the piece
+};
+// Of each target of the piece: lost[n] x[n] summed over its tokens among 64, in their order, into the row
+// of the first of them: a wavefront for a token and 512 columns.  (One product more for
+// each token in dw's epilogue, as matrix instructions, costs the main loop its registers and
+// leaves a frequent target to one wavefront.)  1230 kept of 2048 tokens x 768 over 50288: 7 us here, 9 in
+// k_ce_back_join, of 485 with the gradient.
+__global__ void __launch_bounds__(256) k_ce_back(BackArgs a, Tokens tk) {
+    const int n = blockIdx.x * 4 + wave_id(), lane = threadIdx.x & 63;
+    if (n >= *tk.count) return;
+    const int t = tk.tgt[n] - a.v_first, n0 = n & ~63;
+    if (t < 0 || t >= a.rows) return;
+    // (past the kept tokens stands -1 up to the next multiple of 64)
+    uint64_t same = __ballot(tk.tgt[n0 + lane] - a.v_first == t);
+    const float lost = tk.lost[n0 + lane];
+    if (n0 + __ffsll((unsigned long long)same) - 1 != n) return;
+    if (blockIdx.y == 0 && lane == 0) atomicMin(tk.first + a.v_first + t, n);
+    const int64_t c = (int64_t)blockIdx.y * 512 + lane * 8;
+    float s[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+    while (same) {
+        constexpr int UN = 4;
+        u32x4 v[UN];
+        float l[UN];
+        int k = 0;
+#pragma unroll
+        for (int u = 0; u < UN; ++u)
+            if (same) {
+                const int at = __ffsll((unsigned long long)same) - 1;
+                same &= same - 1;
+                l[u] = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(lost), at));
+                v[u] = *reinterpret_cast<const u32x4*>(a.x + (n0 + at) * a.dp + min(c, a.dp - 8));
+                k = u + 1;
+            }
+#pragma unroll
+        for (int u = 0; u < UN; ++u)
+            if (u < k)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    s[2 * i] = fmaf(l[u], bf16_lo(v[u][i]), s[2 * i]);
+                    s[2 * i + 1] = fmaf(l[u], bf16_hi(v[u][i]), s[2 * i + 1]);
+                }
+    }
+    if (c >= a.dp) return;
+    f32x4* d = reinterpret_cast<f32x4*>(a.back + n * a.dp + c);
+    d[0] = f32x4{s[0], s[1], s[2], s[3]};
+    d[1] = f32x4{s[4], s[5], s[6], s[7]};
+}
+// More than 64 tokens: the first token of a target adds the rows of the later 64s, in their order.
+__global__ void __launch_bounds__(256) k_ce_back_join(BackArgs a, Tokens tk) {
+    const int n = blockIdx.x * 4 + wave_id(), lane = threadIdx.x & 63, count = *tk.count;
+    if (n >= count) return;
+    const int tgt = tk.tgt[n];
+    if (tgt < a.v_first || tgt - a.v_first >= a.rows || tk.first[tgt] != n) return;
+    const int64_t c = min((int64_t)blockIdx.y * 512 + lane * 8, a.dp - 8);      // (not stored twice)
+    f32x4 x = zero4(), y = zero4();
+    bool any = false;
+    constexpr int UN = 8;
+    for (int i0 = (n | 63) + 1; i0 < count; i0 += 64 * UN) {
+        uint64_t same[UN];
+#pragma unroll
+        for (int u = 0; u < UN; ++u) {
+            const int i = i0 + 64 * u + lane;
+            same[u] = __ballot(i < count && tk.tgt[i] == tgt);
+        }
+        f32x4 v[UN], w[UN];
+#pragma unroll
+        for (int u = 0; u < UN; ++u)
+            if (same[u]) {
+                const f32x4* p = reinterpret_cast<const f32x4*>(
+                    a.back + (int64_t)(i0 + 64 * u + __ffsll((unsigned long long)same[u]) - 1) * a.dp + c);
+                v[u] = p[0];
+                w[u] = p[1];
+            }
+#pragma unroll
+        for (int u = 0; u < UN; ++u)
+            if (same[u]) {
+                x += v[u];
+                y += w[u];
+                any = true;
+            }
+    }
+    if (!any) return;
+    f32x4* d = reinterpret_cast<f32x4*>(a.back + (int64_t)n * a.dp + c);
+    x += d[0];
+    y += d[1];
+    if ((int64_t)blockIdx.y * 512 + lane * 8 >= a.dp) return;
+    d[0] = x;
+    d[1] = y;
+}
 
 // ---------------------------------------------------------------------------
 // joins
@@ -876,7 +971,7 @@ int z_parts(int z, bool f32) { return f32 ? 4 : z < 256 ? 1 : 2; }
 struct Common {
     int64_t n, vocab, dim, np, dp;
     bool f32, pack_w;
-    size_t idx, inv, tgt, lse, em1, count, x, w, at;
+    size_t idx, inv, tgt, lse, em1, count, first, x, w, at;
     int z;                   // tokens of a tile of the logits
 };
 
@@ -898,6 +993,7 @@ Common common(int64_t n, int64_t vocab, int64_t dim, int64_t ldw, const void* w,
     c.lse = take(4 * (size_t)c.np);
     c.em1 = take(4 * (size_t)c.np);
     c.count = take(8);
+    c.first = c.f32 ? c.at : take(4 * (size_t)vocab);
     const size_t planes = c.f32 ? 3 : 1;
     c.x = take(2 * planes * (size_t)c.np * c.dp);
     c.w = c.pack_w ? take(2 * planes * (size_t)vocab * c.dp) : c.at;
@@ -961,7 +1057,7 @@ struct BwdPlan {
     int64_t piece;
     int pieces;
     int x, splits;           // dx: tokens of a tile; parts of K (few tokens) or workgroups (many)
-    size_t G, dx, lost, total;
+    size_t G, dx, lost, back, total;
 };
 BwdPlan bwd_plan(const m2_linear_cross_entropy_grad_args& a) {
     BwdPlan p{};
@@ -976,6 +1072,7 @@ BwdPlan bwd_plan(const m2_linear_cross_entropy_grad_args& a) {
     p.piece = ((all / 256 + p.pieces - 1) / p.pieces) * 256;
     p.pieces = (int)((all + p.piece - 1) / p.piece);
     p.lost = take(4 * (size_t)p.c.np);
+    p.back = p.c.f32 || !a.grad_weight ? 0 : take(4 * (size_t)p.c.np * p.c.dp);
     p.G = take(2 * planes * (size_t)(p.c.np ? p.c.np : 64) * p.piece);
     // dx: K is the piece.  Many tokens: dealt out with the tiles (k_ce_tile), whose number
     // depends on the tokens that are kept.  Few: split so that the tiles fill the CUs; a
@@ -1040,18 +1137,21 @@ Tokens tokens(char* ws, const Common& c) {
     t.lse = reinterpret_cast<float*>(ws + c.lse);
     t.em1 = reinterpret_cast<float*>(ws + c.em1);
     t.count = reinterpret_cast<int*>(ws + c.count);
+    t.first = reinterpret_cast<int*>(ws + c.first);
     return t;
 }
 
 template <typename T>
 void pack(char* ws, const Common& c, const void* x, int64_t ldx, const void* w, int64_t ldw, PackArgs a,
-          const Tokens& tk, int64_t ignore, hipStream_t s) {
+          const Tokens& tk, int64_t ignore, bool grad, hipStream_t s) {
     a.n = c.n; a.ignore = ignore;
     const bool finds = c.n <= PACK_FINDS;
     if (!finds) hipLaunchKernelGGL(k_ce_compact, dim3(1), dim3(1024), 0, s, a.targets, c.n, ignore, a.t64, tk);
     a.dim = c.dim; a.dp = c.dp;
     a.src = x; a.ld = ldx; a.dst = reinterpret_cast<bf16*>(ws + c.x); a.rows = c.np; a.plane = c.np * c.dp;
-    hipLaunchKernelGGL((k_ce_pack<T, true>), dim3((unsigned)((finds ? c.n + 67 : c.np) / 4)), dim3(256), 0, s, a, tk);
+    a.row_blocks = (int)((finds ? c.n + 67 : c.np) / 4);
+    const int clear = grad && !c.f32 ? tiles(c.vocab, CLEAR) : 0;
+    hipLaunchKernelGGL((k_ce_pack<T, true>), dim3((unsigned)(a.row_blocks + clear)), dim3(256), 0, s, a, tk);
     if (c.pack_w) {
         a.src = w; a.ld = ldw; a.dst = reinterpret_cast<bf16*>(ws + c.w); a.rows = c.vocab;
         a.plane = c.vocab * c.dp;
@@ -1089,7 +1189,7 @@ template <bool F32> int run_fwd(const m2_linear_cross_entropy_args& a, const Fwd
     tk.zt = zt;
     PackArgs pa{};
     pa.targets = a.targets; pa.vocab = a.vocab; pa.t64 = t64;
-    pack<T>(cm, c, a.x, a.ldx, a.weight, a.ldw, pa, tk, a.ignore_index, s);
+    pack<T>(cm, c, a.x, a.ldx, a.weight, a.ldw, pa, tk, a.ignore_index, a.saved != nullptr, s);
     g.count = tk.count;
     g.a = operand_w(cm, c, a.weight, a.ldw);
     g.a.lim = (int)c.vocab;
@@ -1113,7 +1213,7 @@ template <bool F32> int run_bwd(const m2_linear_cross_entropy_grad_args& a, cons
     PackArgs pa{};
     pa.targets = a.targets; pa.vocab = a.vocab; pa.t64 = a.target_dtype == M2_I64;
     pa.lse = a.lse; pa.loss = a.loss;
-    if (!a.saved) pack<T>(cm, c, a.x, a.ldx, a.weight, a.ldw, pa, tk, a.ignore_index, s);
+    if (!a.saved) pack<T>(cm, c, a.x, a.ldx, a.weight, a.ldw, pa, tk, a.ignore_index, true, s);
     const Operand w = operand_w(cm, c, a.weight, a.ldw);
     bf16* G = reinterpret_cast<bf16*>(ws + p.G);
     const int64_t gplane = c.np * p.piece;
@@ -1171,6 +1271,13 @@ template <bool F32> int run_bwd(const m2_linear_cross_entropy_grad_args& a, cons
             dxs.tm = d.tm; dxs.tn = d.tn; dxs.nwg = p.splits;
         }
         if (a.grad_weight) {
+            const BackArgs back{reinterpret_cast<const bf16*>(cm + c.x), reinterpret_cast<float*>(ws + p.back), c.dp,
+                                (int)v0, (int)rows};
+            if constexpr (!F32) {
+                const dim3 grid((unsigned)(c.np / 4), (unsigned)((c.dp + 511) / 512));
+                hipLaunchKernelGGL(k_ce_back, grid, dim3(256), 0, s, back, tk);
+                if (c.n > 64) hipLaunchKernelGGL(k_ce_back_join, grid, dim3(256), 0, s, back, tk);
+            }
             Gemm d = g0;
             d.nk = 0;
             d.a = Operand{reinterpret_cast<bf16*>(cm + c.x), c.dp, c.np * c.dp, (int)c.dp, (int)c.np};
@@ -1181,10 +1288,7 @@ template <bool F32> int run_bwd(const m2_linear_cross_entropy_grad_args& a, cons
                 typedef decltype(shape) S;
                 d.tm = tiles(c.dim, S::BM); d.tn = tiles(rows, S::BN);
                 T* dw = static_cast<T*>(a.grad_weight) + v0 * c.dim;
-                // (how many of n tokens are kept only the device knows: with more than 512 they
-                // are hardly ever as few as that)
-                if (!F32 && c.n <= 512) launch<S>(d, EpiDw<T, !F32>{dw, c.dim, c.dp, d.a.p, tk, up, (int)v0, (int)rows}, s);
-                else launch<S>(d, EpiDw<T, false>{dw, c.dim, c.dp, d.a.p, tk, up, (int)v0, (int)rows}, s);
+                launch<S>(d, EpiDw<T>{dw, c.dim, c.dp, back.back, tk.first + v0, up, (int)rows}, s);
             };
             if constexpr (F32) {
                 if (large_planes(c.dim, rows)) go(typename P::W128());

@@ -6,7 +6,7 @@ import torch
 
 from gpu_util import announce
 from mamba2_jax import ops
-from test_gpu_vocab import DEV, DT, IGN, Ref, ce_inputs, within
+from test_gpu_vocab import DEV, DT, F, IGN, Ref, ce_inputs, gen, make_ids, u, within
 
 pytestmark = pytest.mark.gpu
 
@@ -41,3 +41,56 @@ def test_score_last_step_in_each_slot(n, dim):
     within(loss, r.loss, r.loss_tol, "loss")
     for _ in range(15):
         assert torch.equal(ops.linear_cross_entropy(x, w, t, reduction="none"), loss)
+
+
+def dw_tolerance(x, w, t, up):
+    """(dw, its tolerance) of test_gpu_vocab's Ref, in which G at the target is not rounded to
+    bfloat16: what that would take from it is added in float32, off by the roundings of its products
+    and sums."""
+    r = Ref(x, w, t, up)
+    kept = t != IGN
+    X, tt = x.double()[kept], t[kept]
+    z = X @ w.double().t()
+    G = up[kept] * torch.expm1(z.gather(1, tt[:, None])[:, 0] - torch.logsumexp(z, 1))
+    half = u(torch.bfloat16)
+    at = torch.zeros_like(r.dw).index_add_(0, tt, G.abs()[:, None] * X.abs())
+    count = torch.bincount(tt, minlength=len(w)).double()[:, None]
+    # what an unmended dw would be
+    lost = torch.zeros_like(r.dw).index_add_(0, tt, (G.float().bfloat16().double() - G)[:, None] * X)
+    return r.dw, r.dw_tol - half * at + half * (count + 8) * F * at, r.dw + lost
+
+
+# tokens, kept, vocabulary, width, how the targets fall, one gradient of all losses or one of each
+DW = [(500, 60, 5000, 136, "any", "each"), (600, 60, 5000, 136, "any", "each"), (40, 40, 3000, 64, "any", "each"),
+      (64, 64, 3000, 700, "same", "each"), (65, 65, 3000, 72, "same", "each"), (700, 700, 5000, 128, "zipf", "each"),
+      (700, 600, 20000, 264, "zipf", "one"), (1500, 1500, 900, 64, "same", "each"),
+      (2100, 1300, 4000, 96, "same", "one"), (3000, 2500, 5000, 1001, "zipf", "each"),
+      (5000, 4400, 60011, 72, "zipf", "each")]
+
+
+@pytest.mark.parametrize("n,kept,vocab,dim,how,up", DW)
+def test_dw_gets_back_what_the_target_lost(n, kept, vocab, dim, how, up):
+    """bfloat16: dw of any number of tokens, of targets that many share, over several pieces of
+    the vocabulary (the last case), whatever share of the tokens is kept."""
+    announce("dw's target", n, kept, vocab, dim, how, up)
+    g = gen(52, n, kept, vocab)
+    w = (torch.randn((vocab, dim), generator=g, device=DEV) / dim ** 0.5).to(torch.bfloat16)
+    x = torch.randn((n, dim), generator=g, device=DEV).to(torch.bfloat16)
+    t = make_ids(n, vocab, how, g)
+    if vocab == 60011:
+        t[::7] = vocab - 1 - torch.arange(len(t[::7]), device=DEV) % 5
+    t[torch.randperm(n, generator=g, device=DEV)[:n - kept]] = IGN
+    if up == "one":
+        ups = torch.full((n,), 0.7, device=DEV)
+        arg, reduction = torch.tensor(0.7, device=DEV), "sum"
+    else:
+        ups = arg = torch.rand(n, generator=g, device=DEV) + 0.5
+        reduction = "none"
+    wg = w.clone().requires_grad_()
+    loss = ops.linear_cross_entropy(x, wg, t, reduction=reduction)
+    dw, = torch.autograd.grad(loss, wg, arg, retain_graph=True)
+    want, tol, unmended = dw_tolerance(x, w, t, ups.double())
+    within(dw, want, tol, "dw")
+    assert torch.equal(torch.autograd.grad(loss, wg, arg)[0], dw)
+    if up == "each":
+        assert bool(((unmended.to(torch.bfloat16).double() - want).abs() > tol).any()), "would not be noticed"

@@ -238,10 +238,16 @@ struct LogSum {
         s = s * __builtin_amdgcn_exp2f((mx - b) * LOG2E) + u.y * __builtin_amdgcn_exp2f((u.x - b) * LOG2E);
         mx = m;
     }
-    // exp(loss) = 1 + the others' sum over exp(z_t)
-    M2_DEV float loss(float zt) const {
+    // (loss, lse): exp(loss) = 1 + the others' sum over exp(z_t).  lse from the larger of maximum
+    // and z_t on: z_t + loss would keep z_t's roundings where it lies far below the others
+    M2_DEV float2 with_target(float zt) const {
         const float d = mx - zt, e = __builtin_amdgcn_exp2f(-fabsf(d) * LOG2E);
-        return d <= 0.f ? log1pf(s * e) : d + logf(s + e);
+        if (d <= 0.f) {
+            const float l = log1pf(s * e);
+            return make_float2(l, zt + l);
+        }
+        const float l = logf(s + e);
+        return make_float2(d + l, mx + l);
     }
 };
 // m: vocabulary, n: token -> per token (max, sum of exp(z - max)) without the target: of a tile
@@ -723,8 +729,9 @@ __global__ void __launch_bounds__(1024) k_ce_join(JoinArgs a, Tokens tk) {
 #pragma unroll
             for (int i = 0; i < 8; ++i) o.add(red[i][tok]);
             const float zt = tk.zt[k];
-            loss = o.loss(zt);
-            lse = zt + loss;
+            const float2 r = o.with_target(zt);
+            loss = r.x;
+            lse = r.y;
             tk.lse[k] = lse;
             tk.em1[k] = expm1f(-loss);
         }
@@ -789,8 +796,9 @@ __global__ void __launch_bounds__(1024) k_ce_join_few(JoinArgs a, EpiLse e) {
         kept = load_target(e.targets, e.t64, t) != e.ignore;
         if (kept) {
             const float zt = e.target(t) >= 0 ? e.zt[t] : __builtin_nanf("");
-            loss = o.loss(zt);
-            lse = zt + loss;
+            const float2 r = o.with_target(zt);
+            loss = r.x;
+            lse = r.y;
         }
         if (a.loss) a.loss[t] = loss;
         if (a.lse) a.lse[t] = lse;

@@ -7,6 +7,7 @@ import torch
 from gpu_util import announce
 from mamba2_jax import ops
 from test_gpu_vocab import DEV, DT, F, IGN, Ref, ce_inputs, gen, make_ids, u, within
+from test_gpu_vocab_sizes import _bwd, _fwd
 
 pytestmark = pytest.mark.gpu
 
@@ -94,3 +95,40 @@ def test_dw_gets_back_what_the_target_lost(n, kept, vocab, dim, how, up):
     assert torch.equal(torch.autograd.grad(loss, wg, arg)[0], dw)
     if up == "each":
         assert bool(((unmended.to(torch.bfloat16).double() - want).abs() > tol).any()), "would not be noticed"
+
+
+def far_below(n, dtype):
+    """Inputs whose targets' logits are -10000 and the others of the order of ten (exact in bfloat16)."""
+    g = gen(53, n)
+    w = torch.randint(-8, 9, (300, 64), generator=g, device=DEV) / 16.0
+    x = torch.randint(-8, 9, (n, 64), generator=g, device=DEV) / 4.0
+    w[:, 0], x[:, 0] = 0.0, 100.0
+    t = torch.randint(0, 40, (n,), generator=g, device=DEV)
+    w[:40] = 0.0
+    w[:40, 0] = -100.0
+    return x.to(DT[dtype]), w.to(DT[dtype]), t
+
+
+@pytest.mark.parametrize("n", [9, 40, 300])
+@pytest.mark.parametrize("saved", [False, True])
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+def test_lse_of_targets_far_below(n, saved, dtype):
+    """lse does not depend on how far below the others the target lies.  The logits are exact (multiples
+    of 1 / 64 below 1024 in size, as are all their partial sums), so its error is a rounding
+    each for the exponentials' arguments, the maximum and the result, and those of a sum of 300."""
+    announce("lse far below", n, saved, dtype)
+    x, w, t = far_below(n, dtype)
+    loss, lse, total, buf = _fwd(x, w, t, saved=saved)
+    z = x.double() @ w.double().t()
+    want = torch.logsumexp(z, 1)
+    top = z[:, 40:].abs().max()
+    tol = F * (100 + 8 * top)
+    within(lse, want, tol.expand(n), "lse")
+    assert tol < 1e4 * F / 2, "would not be noticed"
+    # the softmax in float32's gradient: dw of the rows that are nobody's target
+    if dtype == "f32":
+        _, dw = _bwd(x, w, t, loss, lse, buf, mean=0)
+        p = 1.5 * torch.softmax(z, 1)[:, 40:]
+        ref, mag = p.t() @ x.double(), p.t() @ x.abs().double()
+        e = 1.05 * (2 * tol + 8 * F * (top + 8)) + (6 * (n / 4 + 32) + 16) * F
+        within(dw[40:], ref, e * mag + F * ref.abs() + 1e-42, "dw")

@@ -239,8 +239,11 @@ struct LogSum {
         mx = m;
     }
     // (loss, lse): exp(loss) = 1 + the others' sum over exp(z_t).  lse from the larger of maximum
-    // and z_t on: z_t + loss would keep z_t's roundings where it lies far below the others
+    // and z_t on: z_t + loss would keep z_t's roundings where it lies far below the others.  A target's logit
+    // of -inf has loss inf and the others' lse; a logit of +inf, the target's or not (s is
+    // NaN then), no softmax: an overflow is not a perfect prediction.
     M2_DEV float2 with_target(float zt) const {
+        if (zt == __builtin_inff()) return make_float2(__builtin_nanf(""), __builtin_nanf(""));
         const float d = mx - zt, e = __builtin_amdgcn_exp2f(-fabsf(d) * LOG2E);
         if (d <= 0.f) {
             const float l = log1pf(s * e);

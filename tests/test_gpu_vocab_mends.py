@@ -132,3 +132,46 @@ def test_lse_of_targets_far_below(n, saved, dtype):
         ref, mag = p.t() @ x.double(), p.t() @ x.abs().double()
         e = 1.05 * (2 * tol + 8 * F * (top + 8)) + (6 * (n / 4 + 32) + 16) * F
         within(dw[40:], ref, e * mag + F * ref.abs() + 1e-42, "dw")
+
+
+@pytest.mark.parametrize("n", [5, 40, 300])
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("where", ["target", "other"])
+@pytest.mark.parametrize("sign", [1, -1])
+def test_infinite_logits(n, dtype, where, sign):
+    """A logit of +inf has no softmax: NaN, as exp(z - max) gives it.  One of -inf has none of it: loss inf
+    if it is the target's, and gradients that are finite all the same."""
+    announce("infinite logits", n, dtype, where, sign)
+    x, w, t = ce_inputs(n, 300, 64, dtype, key=54)
+    t = torch.arange(n, device=DEV) % 299
+    t[1] = 299
+    x[:, 0], w[:, 0] = 0.0, 0.0
+    row = 1 if where == "target" else 3                 # its logit of weight row 299 is infinite
+    x[row, 0], w[299, 0] = sign * 2.0 ** 100, 2.0 ** 100
+    xg, wg = x.clone().requires_grad_(), w.clone().requires_grad_()
+    saved = ops.linear_cross_entropy(xg, wg, t, reduction="none")
+    alone = ops.linear_cross_entropy(x, w, t, reduction="none")
+    dx, dw = torch.autograd.grad(saved.sum(), (xg, wg))
+    z = x.double() @ w.double().t()
+    z[row, 299] = sign * float("inf")
+    p = torch.exp(z - z.max(1, keepdim=True).values)
+    p /= p.sum(1, keepdim=True)
+    rest = torch.arange(n, device=DEV) != row
+    for loss in (saved.detach(), alone):
+        if sign > 0:
+            assert bool(loss[row].isnan())
+        elif where == "target":
+            assert float(loss[row]) == float("inf")
+        assert bool(loss[rest].isfinite().all())
+        assert bool(ops.linear_cross_entropy(x, w, t).isnan()) == (sign > 0)
+    assert bool(dx[rest].isfinite().all())
+    if sign > 0:
+        assert bool(dx[row].isnan().all()) and bool(dw.isnan().all())
+        return
+    G = p - torch.nn.functional.one_hot(t, 300)
+    # G's rounding and the result's; the logits' error, 6 (64 / 4 + 16) F of at most 20, twice
+    lim = 2.0 ** -11 + (2.0 ** -7 if dtype == "bf16" else 0.0)
+    want = G @ w.double()
+    assert bool(((dx.double() - want).abs() <= lim * (G.abs() @ w.abs().double()) + 1e-30).all())
+    want = G.t().contiguous() @ x.double()
+    assert bool(((dw.double() - want).abs() <= lim * (G.abs().t().contiguous() @ x.abs().double()) + 1e-30).all())

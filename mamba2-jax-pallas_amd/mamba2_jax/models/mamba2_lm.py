@@ -32,6 +32,7 @@ import torch
 
 from ..modules.mamba2 import (MixerDims, _lecun_normal, block_step_fusable, mamba2_block_forward,
                               mamba2_block_step, mamba2_block_step_fused)
+from .. import _lib as L
 from ..ops import linear
 from ..ops.cross_entropy import linear_cross_entropy
 from ..ops.embedding import embedding
@@ -389,11 +390,17 @@ class Mamba2LMHeadModel:
         0.  reduction: "none" the positions' losses (batch, seqlen), "mean" (over the
         positions kept; its exponential is the perplexity) or "sum" a scalar.  The final norm
         is rounded to the head's dtype once and the head multiplies it with float32
-        sums.  The layers take no gradients; a head that requires one gets it."""
+        sums.  The layers and the embedding take no gradients; a head of its own that requires
+        one gets it.  A head tied to an embedding that requires one is refused (the head's
+        part alone would be wrong): score under torch.no_grad(), or detach the weights."""
+        w = params["lm_head_weight"]
+        L.require(not (torch.is_grad_enabled() and w.requires_grad
+                       and w.data_ptr() == params["embedding"]["weight"].data_ptr()),
+                  "score: lm_head_weight requires a gradient and is tied to the embedding, which "
+                  "takes none (use torch.no_grad(), or detach it)")
         if targets is None:
             targets = torch.full_like(input_ids, ignore_index)
             targets[:, :-1] = input_ids[:, 1:]
-        w = params["lm_head_weight"]
         with torch.no_grad():
             res, out = self._layers(params, embedding(input_ids, params["embedding"]["weight"]))
             src, resid = (res.float(), None) if out is None else (out, res)

@@ -6,8 +6,10 @@ import os
 import re
 
 import pytest
+import torch
 
 from mamba2_jax import _lib as L
+from mamba2_jax.models import Mamba2Config, Mamba2LMHeadModel
 
 CSRC = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(L.__file__))), "csrc")
 SCORE = dict(x=4096, weight=4096, targets=4096, loss=4096, n=16, vocab=50288, dim=2560, ldx=2560, ldw=2560,
@@ -38,3 +40,20 @@ def test_epilogues_do_not_see_the_ring():
     with open(os.path.join(CSRC, "ce_gemm.h")) as f:
         calls = re.findall(r"epi\.template run<S>\(([^;]*)\);", f.read())
     assert len(calls) == 3 and not any("smem" in c or "lds" in c for c in calls)
+
+
+def test_score_refuses_a_tied_head_that_learns():
+    """Its gradient would be the head's part alone, without the embedding's.  (On the CPU: what is
+    not refused is stopped by the missing GPU.)"""
+    model = Mamba2LMHeadModel(Mamba2Config(d_model=64, n_layer=1, vocab_size=32, headdim=32, d_state=16))
+    ids = torch.zeros((1, 4), dtype=torch.long)
+    table = torch.zeros((32, 64)).requires_grad_()
+    tied = {"embedding": {"weight": table}, "lm_head_weight": table}
+    for head in (table, table.view(32, 64)):
+        with pytest.raises(L.M2ShapeError, match="tied"):
+            model.score({**tied, "lm_head_weight": head}, ids)
+    own = table.detach().clone().requires_grad_()
+    for params, grad in ((tied, False), ({**tied, "lm_head_weight": table.detach()}, True),
+                         ({**tied, "lm_head_weight": own}, True)):
+        with torch.set_grad_enabled(grad), pytest.raises(ValueError, match="no CPU path"):
+            model.score(params, ids)

@@ -31,6 +31,10 @@ namespace {
 constexpr int SORT_THREADS = 256, SORT_ITEMS = 8, SORT_TILE = SORT_THREADS * SORT_ITEMS;
 constexpr int SMALL_THREADS = 1024, SMALL_POS = 14, SMALL_N = 1 << SMALL_POS;
 constexpr int MAX_BINS = 512;
+// Workgroups of a pass over many entries: each counts, then moves, a contiguous run of tiles.  Every
+// one of them adds up the counts of all, which is half a gigabyte read from the L2 at most; with a
+// workgroup for each tile it would grow with the square of the entries.
+constexpr int SORT_BLOCKS = 512;
 
 M2_DEV int64_t load_id(const void* ids, int64_t i, int is64) {
     return is64 ? reinterpret_cast<const int64_t*>(ids)[i]
@@ -130,6 +134,10 @@ struct SortArgs {
     int32_t* hist;               // [blocks][bins]
     int64_t vocab, padding;
     int n, id64, shift, bits, nb;
+    int tiles;                   // of SORT_TILE entries
+
+    // of workgroup b: [tile(b), tile(b + 1))
+    M2_DEV int tile(int b) const { return (int)((int64_t)tiles * b / nb); }
 };
 
 M2_DEV int32_t key_of(const SortArgs& a, int i) {
@@ -188,12 +196,14 @@ __global__ void __launch_bounds__(SORT_THREADS) k_sort_hist(SortArgs a, FillArgs
     if (b >= a.nb) return fill(f, b - a.nb, gridDim.x - a.nb);
     for (int d = t; d < bins; d += SORT_THREADS) h[d] = 0;
     __syncthreads();
+    for (int tile = a.tile(b); tile < a.tile(b + 1); ++tile) {
 #pragma unroll
-    for (int j = 0; j < SORT_ITEMS; ++j) {
-        const int i = b * SORT_TILE + j * SORT_THREADS + t;
-        if (i < a.n) {
-            const int32_t k = a.keys_in ? a.keys_in[i] : key_of(a, i);
-            atomicAdd(&h[(k >> a.shift) & (bins - 1)], 1);
+        for (int j = 0; j < SORT_ITEMS; ++j) {
+            const int i = tile * SORT_TILE + j * SORT_THREADS + t;
+            if (i < a.n) {
+                const int32_t k = a.keys_in ? a.keys_in[i] : key_of(a, i);
+                atomicAdd(&h[(k >> a.shift) & (bins - 1)], 1);
+            }
         }
     }
     __syncthreads();
@@ -262,56 +272,69 @@ __global__ void __launch_bounds__(SORT_THREADS) k_sort_scatter(SortArgs a, FillA
     if (b >= a.nb) return fill(f, b - a.nb, gridDim.x - a.nb);
     int32_t key[SORT_ITEMS], pos[SORT_ITEMS];
     int rank[SORT_ITEMS];
-    const int base = b * SORT_TILE + w * 64 * SORT_ITEMS + lane;
+    int tile = a.tile(b), base = 0;
+    const int end = a.tile(b + 1);
+    auto load = [&]() {
+        base = tile * SORT_TILE + w * 64 * SORT_ITEMS + lane;
 #pragma unroll
-    for (int j = 0; j < SORT_ITEMS; ++j) {
-        const int i = base + 64 * j, at = min(i, a.n - 1);      // used below n
-        key[j] = a.keys_in ? a.keys_in[at] : key_of(a, at);
-        pos[j] = a.pos_in ? a.pos_in[at] : i;
-    }
-    for (int d = t; d < NW * MAX_BINS; d += SORT_THREADS) (&cnt[0][0])[d] = 0;
-    __syncthreads();
-    wave_ranks<9, SORT_ITEMS>([&](int j) { return (key[j] >> a.shift) & (bins - 1); },
-                              [&](int j) { return base + 64 * j < a.n; }, cnt[w], rank);
-    __syncthreads();
-    // where each (digit, wavefront) of this block begins: the entries of smaller digits in
-    // all blocks, of this digit in earlier blocks and in earlier wavefronts.  Thread t
-    // owns digits D t .. D t + D - 1 (a fixed order for the prefix sum).
+        for (int j = 0; j < SORT_ITEMS; ++j) {
+            const int i = base + 64 * j, at = min(i, a.n - 1);      // used below n
+            key[j] = a.keys_in ? a.keys_in[at] : key_of(a, at);
+            pos[j] = a.pos_in ? a.pos_in[at] : i;
+        }
+    };
+    load();
+    // where each digit of this block begins: the entries of smaller digits in all blocks and
+    // of this digit in earlier blocks.  Thread t owns digits D t .. D t + D - 1 (a fixed order
+    // for the prefix sum).
     constexpr int D = MAX_BINS / SORT_THREADS;
-    int tot[D], before[D], mine = 0;
+    int next[D], tot[D], mine = 0;
 #pragma unroll
     for (int k = 0; k < D; ++k) {
         const int d = t * D + k;
-        tot[k] = before[k] = 0;
+        tot[k] = next[k] = 0;
         if (d < bins)
 #pragma unroll 8
             for (int q = 0; q < a.nb; ++q) {
                 const int c = a.hist[q * bins + d];
                 tot[k] += c;
-                before[k] += q < b ? c : 0;
+                next[k] += q < b ? c : 0;
             }
         mine += tot[k];
     }
     int start = block_excl<SORT_THREADS>(mine, tmp);
 #pragma unroll
     for (int k = 0; k < D; ++k) {
-        const int d = t * D + k;
-        int s = start + before[k];
-#pragma unroll
-        for (int q = 0; q < NW; ++q) {
-            const int c = cnt[q][d];
-            cnt[q][d] = s;
-            s += c;
-        }
+        next[k] += start;
         start += tot[k];
     }
-    __syncthreads();
+    for (;;) {
+        for (int d = t; d < NW * MAX_BINS; d += SORT_THREADS) (&cnt[0][0])[d] = 0;
+        __syncthreads();
+        wave_ranks<9, SORT_ITEMS>([&](int j) { return (key[j] >> a.shift) & (bins - 1); },
+                                  [&](int j) { return base + 64 * j < a.n; }, cnt[w], rank);
+        __syncthreads();
+        // where each (digit, wavefront) of this tile begins
 #pragma unroll
-    for (int j = 0; j < SORT_ITEMS; ++j) {
-        if (base + 64 * j >= a.n) continue;
-        const int p = cnt[w][(key[j] >> a.shift) & (bins - 1)] + rank[j];
-        a.keys_out[p] = key[j];
-        a.pos_out[p] = pos[j];
+        for (int k = 0; k < D; ++k) {
+#pragma unroll
+            for (int q = 0; q < NW; ++q) {
+                const int c = cnt[q][t * D + k];
+                cnt[q][t * D + k] = next[k];
+                next[k] += c;
+            }
+        }
+        __syncthreads();
+#pragma unroll
+        for (int j = 0; j < SORT_ITEMS; ++j) {
+            if (base + 64 * j >= a.n) continue;
+            const int p = cnt[w][(key[j] >> a.shift) & (bins - 1)] + rank[j];
+            a.keys_out[p] = key[j];
+            a.pos_out[p] = pos[j];
+        }
+        if (++tile >= end) return;
+        load();
+        __syncthreads();             // everybody has its places
     }
 }
 
@@ -602,7 +625,7 @@ __global__ void __launch_bounds__(FEW_THREADS) k_embed_few(ReduceArgs a, FewArgs
 size_t align256(size_t v) { return (v + 255) & ~size_t(255); }
 
 struct GradPlan {
-    int bits, passes, nb, piece, pieces;
+    int bits, passes, tiles, nb, piece, pieces;
     int64_t ldp;
     bool small;
     size_t keys[2], pos[2], hist, part, total;
@@ -615,7 +638,8 @@ GradPlan grad_plan(const m2_embedding_grad_args& a) {
     p.passes = (kb + 8) / 9;
     p.bits = (kb + p.passes - 1) / p.passes;
     p.small = a.n <= SMALL_N && kb <= 32 - SMALL_POS;
-    p.nb = (int)((a.n + SORT_TILE - 1) / SORT_TILE);
+    p.tiles = (int)((a.n + SORT_TILE - 1) / SORT_TILE);
+    p.nb = p.tiles < SORT_BLOCKS ? p.tiles : SORT_BLOCKS;
     // entries per piece: about 512 pieces, so that every CU has two, of 4 to 32
     // entries (longer pieces leave fewer partial rows, shorter ones more
     // workgroups to a small batch)
@@ -778,6 +802,7 @@ int launch_embedding_grad(const m2_embedding_grad_args& a, hipStream_t s) {
         else sort(std::integral_constant<int, 9>());
     } else {
         k.nb = p.nb;
+        k.tiles = p.tiles;
         for (int pass = 0; pass < p.passes; ++pass) {
             k.shift = pass * p.bits;
             k.keys_out = at(p.keys[cur]); k.pos_out = at(p.pos[cur]);

@@ -175,3 +175,23 @@ def test_infinite_logits(n, dtype, where, sign):
     assert bool(((dx.double() - want).abs() <= lim * (G.abs() @ w.abs().double()) + 1e-30).all())
     want = G.t().contiguous() @ x.double()
     assert bool(((dw.double() - want).abs() <= lim * (G.abs().t().contiguous() @ x.abs().double()) + 1e-30).all())
+
+
+@pytest.mark.parametrize("n,vocab", [(512 * 2048, 3000), (512 * 2048 + 1, 300000), (1025 * 2048 - 7, 70000),
+                                     (5_000_011, 2 ** 26)])
+def test_embedding_grad_of_many_entries(n, vocab):
+    """More tiles than the sort has workgroups.  Whole numbers, whose sums are exact."""
+    announce("many entries", n, vocab)
+    g = gen(55, n)
+    ids = make_ids(n, vocab, "any" if n & 1 else "zipf", g)
+    ids[n // 3], ids[n // 2] = vocab, -1
+    grad = torch.randint(-3, 4, (n, 2), generator=g, device=DEV).float()
+    want = torch.zeros(vocab + 1, 2, dtype=torch.float64, device=DEV)
+    want.index_add_(0, torch.where((ids < 0) | (ids > vocab), vocab, ids), grad.double())
+    assert torch.equal(ops.embedding_grad(ids, grad, vocab).double(), want[:vocab])
+    # the order of a token's entries is theirs: (2^24 + 1) - 2^24 is 0 in float32 (four entries a token:
+    # none is summed in two parts, which begin at multiples of four)
+    k = n // 4
+    ids = torch.arange(4 * k, device=DEV) % k
+    vals = torch.tensor([2.0 ** 24, 1.0, -(2.0 ** 24), 0.0], device=DEV)[torch.arange(4 * k, device=DEV) // k]
+    assert not bool(ops.embedding_grad(ids, vals[:, None], k).any())

@@ -57,3 +57,14 @@ def test_score_refuses_a_tied_head_that_learns():
                          ({**tied, "lm_head_weight": own}, True)):
         with torch.set_grad_enabled(grad), pytest.raises(ValueError, match="no CPU path"):
             model.score(params, ids)
+
+
+@pytest.mark.parametrize("n", [20000, 2 ** 21, 2 ** 30])
+def test_embedding_grad_counts_are_bounded(n):
+    """The sort of many entries reads its workgroups' counts in every workgroup: there are at most 512
+    of them (1 MB of counts), or the work would grow with the square of the entries."""
+    a = L.EmbeddingGradArgs(n=n, vocab=2 ** 20, dim=8, ldg=8, ldo=8, padding_idx=-1, scale=1.0, id_dtype=L.M2_I64,
+                            grad_dtype=L.M2_BF16, out_dtype=L.M2_F32)
+    size = L.load_library().m2_embedding_grad_workspace_size(ctypes.byref(a))
+    rest = 16 * n + (n // 32 + 1) * 2 * 8 * 4           # keys and places, partial rows
+    assert rest <= size <= rest + 2 ** 20 + 4096

@@ -662,6 +662,8 @@ int check_grad(const m2_embedding_grad_args& a) {
                    a.dim < (1ll << 30),
                M2_ERR_INVALID, "%s: bad sizes (n %lld, vocab %lld, dim %lld)", who, (long long)a.n,
                (long long)a.vocab, (long long)a.dim);
+    M2_REQUIRE(a.n <= FEW_N || (int64_t)grad_plan(a).pieces * (a.dim / 256 + 1) < (1ll << 30), M2_ERR_UNSUPPORTED,
+               "%s: too large (n %lld, dim %lld)", who, (long long)a.n, (long long)a.dim);
     return M2_OK;
 }
 
@@ -830,7 +832,6 @@ int launch_embedding_grad(const m2_embedding_grad_args& a, hipStream_t s) {
     r.slabs = (r.vecs + 511) / 512;
     const int per = (r.vecs + r.slabs - 1) / r.slabs;
     const int threads = (per + 63) / 64 * 64;
-    M2_REQUIRE((int64_t)p.pieces * (a.dim / 256 + 1) < (1ll << 30), M2_ERR_UNSUPPORTED, "%s: too large", who);
 #define M2_SUMS(T, TO)                                         \
     do {                                                       \
         if (vec) launch_sums<T, TO, 8>(r, threads, s);   \

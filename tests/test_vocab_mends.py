@@ -68,3 +68,15 @@ def test_embedding_grad_counts_are_bounded(n):
     size = L.load_library().m2_embedding_grad_workspace_size(ctypes.byref(a))
     rest = 16 * n + (n // 32 + 1) * 2 * 8 * 4           # keys and places, partial rows
     assert rest <= size <= rest + 2 ** 20 + 4096
+
+
+def test_embedding_grad_refuses_before_it_writes():
+    """More rows than a launch takes: refused with the size, before anything is launched (a launch
+    without a GPU would answer with another error)."""
+    lib = L.load_library()
+    a = L.EmbeddingGradArgs(ids=4096, grad=4096, out=4096, n=2 ** 31 - 5000, vocab=1000, dim=4096, ldg=4096, ldo=4096,
+                            padding_idx=-1, scale=1.0, id_dtype=L.M2_I64, grad_dtype=L.M2_BF16, out_dtype=L.M2_F32,
+                            workspace=4096, workspace_bytes=2 ** 62)
+    assert lib.m2_embedding_grad_workspace_size(ctypes.byref(a)) == 0
+    assert lib.m2_embedding_grad(ctypes.byref(a), None) == -2
+    assert "too large" in lib.m2_last_error().decode()

@@ -46,6 +46,8 @@ struct Tokens {              // of the kept tokens: in the workspace, or saved f
     float* zt;               // [np] the target's logit (forward)
     float* lost;             // [np] what bf16 takes from G at the target (backward, EpiG)
     int* first;              // [vocab] the first kept token with this target, or NONE
+    unsigned long long* runs;    // [vocab][run_words] which 64s of kept tokens have this target
+    int run_words;
 };
 constexpr int NONE = 0x7fffffff;
 
@@ -153,7 +155,7 @@ struct PackArgs {
     int row_blocks;          // further workgroups clear tk.first
 };
 constexpr int64_t PACK_FINDS = 1024;     // up to so many tokens the packing finds the kept ones itself
-constexpr int CLEAR = 2048;              // entries of Tokens::first that one workgroup clears
+constexpr int CLEAR = 2048;              // entries of Tokens::first and rows of Tokens::runs that one workgroup clears
 
 // Rows of src as bf16 (planes) with rows of dp elements, zeros behind dim: the weights
 // where they cannot be read in place, or the kept rows of x (TOK), with zero rows up to
@@ -167,7 +169,9 @@ __global__ void __launch_bounds__(256) k_ce_pack(PackArgs a, Tokens tk) {
     if constexpr (TOK) {
         if ((int)blockIdx.x >= a.row_blocks) {
             const int64_t v0 = (int64_t)(blockIdx.x - a.row_blocks) * CLEAR;
-            for (int64_t v = v0 + threadIdx.x; v < min(v0 + CLEAR, a.vocab); v += 256) tk.first[v] = NONE;
+            const int64_t v1 = min(v0 + CLEAR, a.vocab);
+            for (int64_t v = v0 + threadIdx.x; v < v1; v += 256) tk.first[v] = NONE;
+            for (int64_t i = v0 * tk.run_words + threadIdx.x; i < v1 * tk.run_words; i += 256) tk.runs[i] = 0;
             return;
         }
         if (a.n <= PACK_FINDS) {
@@ -613,7 +617,11 @@ __global__ void __launch_bounds__(256) k_ce_back(BackArgs a, Tokens tk) {
     uint64_t same = __ballot(tk.tgt[n0 + lane] - a.v_first == t);
     const float lost = tk.lost[n0 + lane];
     if (n0 + __ffsll((unsigned long long)same) - 1 != n) return;
-    if (blockIdx.y == 0 && lane == 0) atomicMin(tk.first + a.v_first + t, n);
+    if (blockIdx.y == 0 && lane == 0) {
+        const int64_t v = a.v_first + t;
+        atomicMin(tk.first + v, n);
+        atomicOr(tk.runs + v * tk.run_words + (n >> 12), 1ull << ((n >> 6) & 63));
+    }
     const int64_t c = (int64_t)blockIdx.y * 512 + lane * 8;
     float s[8] = {0, 0, 0, 0, 0, 0, 0, 0};
     while (same) {
@@ -653,30 +661,38 @@ __global__ void __launch_bounds__(256) k_ce_back_join(BackArgs a, Tokens tk) {
     const int64_t c = min((int64_t)blockIdx.y * 512 + lane * 8, a.dp - 8);      // (not stored twice)
     f32x4 x = zero4(), y = zero4();
     bool any = false;
-    constexpr int UN = 8;
-    for (int i0 = (n | 63) + 1; i0 < count; i0 += 64 * UN) {
-        uint64_t same[UN];
+    const unsigned long long* runs = tk.runs + (int64_t)tgt * tk.run_words;
+    for (int word = n >> 12; word < tk.run_words; ++word) {
+        uint64_t m = runs[word];
+        if (word == n >> 12) m &= m - 1;             // n's own
+        while (m) {
+            constexpr int UN = 8;
+            int run[UN], t[UN], k = 0;
 #pragma unroll
-        for (int u = 0; u < UN; ++u) {
-            const int i = i0 + 64 * u + lane;
-            same[u] = __ballot(i < count && tk.tgt[i] == tgt);
+            for (int u = 0; u < UN; ++u)
+                if (m) {
+                    run[u] = (word << 12) + ((__ffsll((unsigned long long)m) - 1) << 6);
+                    m &= m - 1;
+                    t[u] = tk.tgt[run[u] + lane];
+                    k = u + 1;
+                }
+            f32x4 v[UN], w[UN];
+#pragma unroll
+            for (int u = 0; u < UN; ++u)
+                if (u < k) {
+                    const int i = run[u] + __ffsll((unsigned long long)__ballot(t[u] == tgt)) - 1;
+                    const f32x4* p = reinterpret_cast<const f32x4*>(a.back + i * a.dp + c);
+                    v[u] = p[0];
+                    w[u] = p[1];
+                }
+#pragma unroll
+            for (int u = 0; u < UN; ++u)
+                if (u < k) {
+                    x += v[u];
+                    y += w[u];
+                }
+            any = true;
         }
-        f32x4 v[UN], w[UN];
-#pragma unroll
-        for (int u = 0; u < UN; ++u)
-            if (same[u]) {
-                const f32x4* p = reinterpret_cast<const f32x4*>(
-                    a.back + (int64_t)(i0 + 64 * u + __ffsll((unsigned long long)same[u]) - 1) * a.dp + c);
-                v[u] = p[0];
-                w[u] = p[1];
-            }
-#pragma unroll
-        for (int u = 0; u < UN; ++u)
-            if (same[u]) {
-                x += v[u];
-                y += w[u];
-                any = true;
-            }
     }
     if (!any) return;
     f32x4* d = reinterpret_cast<f32x4*>(a.back + (int64_t)n * a.dp + c);
@@ -982,7 +998,8 @@ int z_parts(int z, bool f32) { return f32 ? 4 : z < 256 ? 1 : 2; }
 struct Common {
     int64_t n, vocab, dim, np, dp;
     bool f32, pack_w;
-    size_t idx, inv, tgt, lse, em1, count, first, x, w, at;
+    size_t idx, inv, tgt, lse, em1, count, first, runs, x, w, at;
+    int run_words;
     int z;                   // tokens of a tile of the logits
 };
 
@@ -1004,7 +1021,10 @@ Common common(int64_t n, int64_t vocab, int64_t dim, int64_t ldw, const void* w,
     c.lse = take(4 * (size_t)c.np);
     c.em1 = take(4 * (size_t)c.np);
     c.count = take(8);
+    // (bf16's gradient: 4 bytes and a bit for each 64 tokens a row of the vocabulary)
+    c.run_words = (int)((n + 4095) / 4096);
     c.first = c.f32 ? c.at : take(4 * (size_t)vocab);
+    c.runs = c.f32 ? c.at : take(8 * (size_t)vocab * c.run_words);
     const size_t planes = c.f32 ? 3 : 1;
     c.x = take(2 * planes * (size_t)c.np * c.dp);
     c.w = c.pack_w ? take(2 * planes * (size_t)vocab * c.dp) : c.at;
@@ -1149,6 +1169,8 @@ Tokens tokens(char* ws, const Common& c) {
     t.em1 = reinterpret_cast<float*>(ws + c.em1);
     t.count = reinterpret_cast<int*>(ws + c.count);
     t.first = reinterpret_cast<int*>(ws + c.first);
+    t.runs = reinterpret_cast<unsigned long long*>(ws + c.runs);
+    t.run_words = c.run_words;
     return t;
 }
 

@@ -606,8 +606,8 @@ struct BackArgs {
 // Of each target of the piece: lost[n] x[n] summed over its tokens among 64, in their order, into the row
 // of the first of them: a wavefront for a token and 512 columns.  (One product more for
 // each token in dw's epilogue, as matrix instructions, costs the main loop its registers and
-// leaves a frequent target to one wavefront.)  1230 kept of 2048 tokens x 768 over 50288: 7 us here, 9 in
-// k_ce_back_join, of 485 with the gradient.
+// leaves a frequent target to one wavefront.)  1230 kept of 2048 tokens x 768 over 50288: 7 us here, 7 in
+// k_ce_back_join, of 484 with the gradient.
 __global__ void __launch_bounds__(256) k_ce_back(BackArgs a, Tokens tk) {
     const int n = blockIdx.x * 4 + wave_id(), lane = threadIdx.x & 63;
     if (n >= *tk.count) return;
@@ -652,7 +652,8 @@ __global__ void __launch_bounds__(256) k_ce_back(BackArgs a, Tokens tk) {
     d[0] = f32x4{s[0], s[1], s[2], s[3]};
     d[1] = f32x4{s[4], s[5], s[6], s[7]};
 }
-// More than 64 tokens: the first token of a target adds the rows of the later 64s, in their order.
+// More than 64 tokens: the first token of a target adds the rows of the later 64s, in their order.  (Found by
+// going through all tokens' targets instead of the bits: 104 us for 8192 x 50288 x 2560, 34 so.)
 __global__ void __launch_bounds__(256) k_ce_back_join(BackArgs a, Tokens tk) {
     const int n = blockIdx.x * 4 + wave_id(), lane = threadIdx.x & 63, count = *tk.count;
     if (n >= count) return;
@@ -1003,7 +1004,8 @@ struct Common {
     int z;                   // tokens of a tile of the logits
 };
 
-Common common(int64_t n, int64_t vocab, int64_t dim, int64_t ldw, const void* w, int dtype) {
+// grad: with what only a gradient reads
+Common common(int64_t n, int64_t vocab, int64_t dim, int64_t ldw, const void* w, int dtype, bool grad) {
     Common c{};
     c.n = n; c.vocab = vocab; c.dim = dim;
     c.np = (n + 63) / 64 * 64;
@@ -1023,8 +1025,8 @@ Common common(int64_t n, int64_t vocab, int64_t dim, int64_t ldw, const void* w,
     c.count = take(8);
     // (bf16's gradient: 4 bytes and a bit for each 64 tokens a row of the vocabulary)
     c.run_words = (int)((n + 4095) / 4096);
-    c.first = c.f32 ? c.at : take(4 * (size_t)vocab);
-    c.runs = c.f32 ? c.at : take(8 * (size_t)vocab * c.run_words);
+    c.first = c.f32 || !grad ? c.at : take(4 * (size_t)vocab);
+    c.runs = c.f32 || !grad ? c.at : take(8 * (size_t)vocab * c.run_words);
     const size_t planes = c.f32 ? 3 : 1;
     c.x = take(2 * planes * (size_t)c.np * c.dp);
     c.w = c.pack_w ? take(2 * planes * (size_t)vocab * c.dp) : c.at;
@@ -1065,7 +1067,7 @@ struct FwdPlan {
 };
 FwdPlan fwd_plan(const m2_linear_cross_entropy_args& a) {
     FwdPlan p{};
-    p.c = common(a.n, a.vocab, a.dim, a.ldw, a.weight, a.dtype);
+    p.c = common(a.n, a.vocab, a.dim, a.ldw, a.weight, a.dtype, a.saved != nullptr);
     // (the kernel's offsets within a tile are of 32 bits: rows that lie further apart, the last
     // positions of long prompts, are packed, with 64-bit addresses)
     p.direct = a.n <= 64 && !a.saved && !p.c.pack_w && a.ldx % 8 == 0 && al16(a.x) &&
@@ -1092,7 +1094,7 @@ struct BwdPlan {
 };
 BwdPlan bwd_plan(const m2_linear_cross_entropy_grad_args& a) {
     BwdPlan p{};
-    p.c = common(a.n, a.vocab, a.dim, a.ldw, a.weight, a.dtype);
+    p.c = common(a.n, a.vocab, a.dim, a.ldw, a.weight, a.dtype, true);
     size_t at = a.saved ? 0 : p.c.at;
     auto take = [&](size_t b) { const size_t r = at; at += align256(b); return r; };
     const int planes = p.c.f32 ? 3 : 1;
@@ -1361,7 +1363,7 @@ namespace m2 {
 
 size_t linear_ce_saved(const m2_linear_cross_entropy_args& a) {
     if (check_sizes("linear_cross_entropy", a.n, a.vocab, a.dim, a.ldx, a.ldw, a.dtype, a.target_dtype)) return 0;
-    return common(a.n, a.vocab, a.dim, a.ldw, a.weight, a.dtype).at;
+    return common(a.n, a.vocab, a.dim, a.ldw, a.weight, a.dtype, true).at;
 }
 
 size_t linear_ce_workspace(const m2_linear_cross_entropy_args& a) {

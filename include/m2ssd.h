@@ -439,7 +439,7 @@ int m2_skinny_gemm_norm(const m2_skinny_gemm_norm_args* a, void* stream);
 
 /* ---------------------------------------------------------------------------
  * embedding: out[n] = scale * weight[ids[n]], the products in float32, rounded
- * once.  An id outside [0, vocab) reads nothing: its row becomes NaN.
+ * once.  An id outside [0, vocab) makes its row NaN.
  * No counterpart operator in the reference (an array index,
  * models/mamba2_lm.py:190).
  * ------------------------------------------------------------------------- */
@@ -454,12 +454,12 @@ typedef struct {
 int m2_embedding(const m2_embedding_args* a, void* stream);
 
 /* ---------------------------------------------------------------------------
- * embedding_grad: out[v] = scale * sum over {n : ids[n] == v} of grad[n], every
- * row of out written once (zeros where no id names it), or, with accumulate,
- * added into out at the rows that the ids name, the others untouched.  The sums
+ * embedding_grad: out[v] = scale * sum over {n : ids[n] == v} of grad[n] (zeros
+ * where no id names v; with more than 256 entries the others are zeroed first too), or, with
+ * accumulate, added into out at the rows that the ids name, the others untouched.  The sums
  * are float32 over the n in order (by sorted ids): equal inputs give
  * equal bits.  ids equal to padding_idx and ids outside [0, vocab) take no part.
- * vocab < 2^27, n < 2^31.
+ * vocab < 2^27, n < 2^31 - 4096, n (dim / 256 + 1) < 2^35.
  * ------------------------------------------------------------------------- */
 typedef struct {
     const void* ids;               /* [n], id_dtype (M2_I32 / M2_I64)           */
@@ -479,9 +479,9 @@ int m2_embedding_grad(const m2_embedding_grad_args* a, void* stream);
  * linear_cross_entropy: the loss of a linear head over a vocabulary,
  *   z[n, v] = x[n] . weight[v],  lse[n] = log sum_v exp(z[n, v]),
  *   loss[n] = lse[n] - z[n, targets[n]]   (0 where targets[n] == ignore_index),
- * in pieces of the vocabulary: the logits exist in registers only.  x of rows
- * that are left out is not read.  A target outside [0, vocab) that is not
- * ignore_index makes its loss NaN.  total (or NULL) takes the sum of the losses, over
+ * in pieces of the vocabulary: the logits exist in registers only.  What x holds in rows
+ * that are left out reaches nothing (the rows must be readable).  A target outside [0, vocab)
+ * that is not ignore_index makes its loss NaN, and so does a logit of +inf or NaN.  total (or NULL) takes the sum of the losses, over
  * max(1, the number of rows kept) with mean.  float32 operands are multiplied as three bf16
  * parts each (six products, about 2^-24 of each).  vocab, n < 2^30.
  * No counterpart in the reference, whose models answer with logits

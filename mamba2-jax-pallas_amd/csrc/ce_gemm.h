@@ -193,7 +193,9 @@ template <int BM_, int BN_, int WM_, int WN_, int ST_, int BK_, bool ATR_, bool 
 };
 
 // bf16, few tokens (or tiles): the operand of the vocabulary streams from HBM through a deep
-// ring, two workgroups a CU.  16 tokens over 50288 x 2560: 257 MB in 45 us, 5.7 TB/s.
+// ring, two workgroups a CU where two rings of the shape fit its LDS (the logits' and dw's do,
+// dx's tiles of 256 columns do not).  16 tokens over 50288 x 2560: 257 MB in 51 us, 5.0 TB/s (38
+// where a part of the weights is in the last-level cache).
 template <class S, class EPI>
 __global__ void __launch_bounds__(S::NT, 2 * S::LDS <= 160 * 1024 ? 2 : 1) k_ce_stream(Gemm g, EPI epi) {
     __shared__ __align__(1024) char smem[S::LDS];

@@ -106,7 +106,7 @@ __global__ void __launch_bounds__(256) k_embedding(EmbedArgs a) {
     if (row >= a.n) return;
     const int c0 = (int)(work % a.parts) * 64 * EMB_UN + (threadIdx.x & 63);
     const int64_t id = load_id(a.ids, row, a.id64);
-    const bool ok = id >= 0 && id < a.vocab;
+    const bool ok = id >= 0 && id < a.vocab;             // if not, row 0 is read and NaN written
     const T* src = static_cast<const T*>(a.w) + (ok ? id : 0) * a.ldw;
     T* dst = static_cast<T*>(a.out) + row * a.ldo;
     Vec<T, V> v[EMB_UN];

@@ -11,8 +11,8 @@
 // losses far below the step of the logits.
 // Backward: a piece of the vocabulary at a time, the same product again gives G in its
 // epilogue (rounded to bf16 once, as the results are; what that takes from the target's is
-// given back, lost_of; float32 operands keep three bf16 planes of it), then dw of the piece and
-// the piece's part of dx, which float32 partial sums collect over pieces.  At
+// given back in float32, lost_of; float32 operands keep three bf16 planes of it), then dw of the
+// piece and the piece's part of dx, which float32 partial sums collect over pieces.  At
 // the target G is g expm1(-loss), not a difference of near-equal numbers.
 //
 // Tokens that are left out (ignore_index) are dropped at the start: the kept rows of x
@@ -25,9 +25,9 @@
 // Bound by the matrix units for more than a few hundred tokens (2 n V D operations
 // forward, 6 n V D backward with the logits computed again), by reading the
 // weights for few.  bf16, 50288 x 2560: 16 tokens scored in 56 us (4.6 TB/s of weights), 4096
-// in 0.81 ms (1.30 PFLOP/s), loss and gradients of 8192 in 6.65 ms (1.27 PFLOP/s with the
+// in 0.80 to 0.83 ms (1.3 PFLOP/s), loss and gradients of 8192 in 6.8 ms (1.24 PFLOP/s with the
 // logits computed twice).  Keeping the logits would save a quarter of the
-// latter and hold 1.6 GB instead of at most 512 MB of G.
+// latter and hold 1.6 GB instead of 512 MB of G.
 #include "ce_gemm.h"
 
 namespace {
@@ -396,10 +396,8 @@ struct Up {
     int64_t stride;          // 0: one value
     int mean;
     // of a token, in G; of all, where they have one value: dx and dw are multiplied by it behind
-    // their products and G is softmax - onehot alone.  Its bf16 at the target is then
-    // that of -1 + p, nearly exact for a small p, where the same value times 1 / count is off by
-    // the same up to 2^-8 in every row of dw that has a target (dw of 241 tokens over
-    // 1762: 2.4e-3 off, 2.0e-3 so; 1.7e-3 is the result's own rounding).
+    // their products and G is softmax - onehot alone, whose bf16 is nearly exact at a
+    // target of small probability.
     M2_DEV float of(const Tokens& tk, int n, int count) const {
         return stride ? g[tk.idx[n] * stride] * (mean ? 1.f / (float)count : 1.f) : 1.f;
     }
@@ -1081,7 +1079,8 @@ FwdPlan fwd_plan(const m2_linear_cross_entropy_args& a) {
     return p;
 }
 
-// G's workspace: 512 MB of it at most, in whole tiles of the vocabulary.  More
+// G's workspace: 512 MB of it, or one tile of the vocabulary (256 rows) for all tokens where that
+// is more (from a million bf16 tokens, 350000 of float32, on).  More
 // pieces cost launches and passes over the partial dx (8192 x 50288 x 2560: with 192 MB 6.92 ms
 // against 6.66, with 1 GB 6.67).
 constexpr int64_t G_BYTES = 512ll << 20;

@@ -93,11 +93,15 @@ def linear_cross_entropy(x, weight, targets, ignore_index=-100, reduction="mean"
 
     reduction: "mean" (over the positions kept; 0 where there are none) and "sum"
     return a scalar, "none" the per-position losses in targets' shape.  Sums, the softmax's
-    maximum and sum and the loss are float32 or wider.  The gradient computes
-    the logits again, at most 512 MB of their gradient at a time: bfloat16
-    operands round it to bfloat16 before its products with weight and x (float32
-    sums, each result rounded once); float32 operands are multiplied as three
-    bfloat16 parts each, accurate to about 2^-24 of each product.  Between the two the
+    maximum and sum and the loss are float32 or wider.  A logit of +inf or NaN makes
+    its loss and gradients NaN; a target's of -inf has loss inf and the
+    gradient of softmax - onehot.  The gradient computes the logits again, 512 MB of their
+    gradient at a time (or 256 rows of the vocabulary for all tokens, where that is more: a million
+    tokens in bfloat16): bfloat16 operands round it to bfloat16 before its products with weight
+    and x (float32 sums, each result rounded once), and what that takes from the
+    targets' is added in float32, through a float32 row for each token; float32 operands are
+    multiplied as three bfloat16 parts each, accurate to about 2^-24 of each product (an
+    infinity among them gives NaN).  Between the two the
     graph holds what the kernels read: a packed copy of x's kept rows, and of weight
     where it cannot be read in place (float32, as three bfloat16 parts: 1.5 times
     weight; a dim that 64 does not divide)."""

@@ -13,8 +13,8 @@
 // (frequent tokens) leaves one partial row per piece, which a second kernel
 // adds in order: no float atomics, so equal inputs give equal bits, and a token
 // that is half of the batch is spread over as many workgroups as any others.
-// The sort keeps one workgroup (of up to 16384 entries) or a few busy; the rest of the chip meanwhile writes the zeros, which are most of a
-// large vocabulary's gradient.  The rows that ids name are written twice that way, at
+// The sort keeps one workgroup (of up to 16384 entries) or some (512 at most) busy; the rest of the
+// chip meanwhile writes the zeros, which are most of a large vocabulary's gradient.  The rows that ids name are written twice that way, at
 // most n rows; zeroing the others alone would have to wait for the sort.  Bound
 // by HBM: grad read once, the result written once and those rows again.
 //

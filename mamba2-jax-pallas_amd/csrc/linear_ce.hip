@@ -152,10 +152,10 @@ struct PackArgs {
     const float* loss;
     int64_t vocab, n, ignore;
     int t64;
-    int row_blocks;          // further workgroups clear tk.first
+    int row_blocks;          // further workgroups clear tk.first and tk.runs
 };
 constexpr int64_t PACK_FINDS = 1024;     // up to so many tokens the packing finds the kept ones itself
-constexpr int CLEAR = 2048;              // entries of Tokens::first and rows of Tokens::runs that one workgroup clears
+constexpr int CLEAR = 2048;              // rows of the vocabulary that one workgroup clears them for
 
 // Rows of src as bf16 (planes) with rows of dp elements, zeros behind dim: the weights
 // where they cannot be read in place, or the kept rows of x (TOK), with zero rows up to
@@ -243,9 +243,9 @@ struct LogSum {
         mx = m;
     }
     // (loss, lse): exp(loss) = 1 + the others' sum over exp(z_t).  lse from the larger of maximum
-    // and z_t on: z_t + loss would keep z_t's roundings where it lies far below the others.  A target's logit
-    // of -inf has loss inf and the others' lse; a logit of +inf, the target's or not (s is
-    // NaN then), no softmax: an overflow is not a perfect prediction.
+    // and z_t on: z_t + loss would keep z_t's roundings where it lies far below the others.  A
+    // target's logit of -inf has loss inf and the others' lse; a logit of +inf, the target's or
+    // not (s is NaN then), no softmax: an overflow is not a perfect prediction.
     M2_DEV float2 with_target(float zt) const {
         if (zt == __builtin_inff()) return make_float2(__builtin_nanf(""), __builtin_nanf(""));
         const float d = mx - zt, e = __builtin_amdgcn_exp2f(-fabsf(d) * LOG2E);

@@ -566,6 +566,84 @@ size_t m2_clip_grad_norm_workspace_size(const m2_clip_grad_norm_args* a);
 int m2_clip_grad_norm(const m2_clip_grad_norm_args* a, void* stream);
 
 /* ---------------------------------------------------------------------------
+ * gated_linear_recurrence: of every batch row and channel
+ *   log a[t] = A sigmoid(r[t]),  h[t] = a[t] h[t-1] + sqrt(1 - a[t]^2) sigmoid(i[t]) x[t]
+ * with h[-1] = initial_states (0 without), A <= 0 and finite; float32, out = h rounded once.
+ * With seq_idx the state is cleared before a position whose entry is not negative and differs from the
+ * one before it; a position with a negative entry is padding: out is 0 there, the state passes it
+ * unchanged, and what x, r and i hold there (they must be readable) reaches nothing.
+ * final_states is the state behind the last position.  x, r and i are addressed through their strides of
+ * batch and time (elements; channels are contiguous), e.g. as slices of one projection's output.
+ * span_states (or NULL) takes the states that enter every M2_RECURRENCE_SPAN positions, which
+ * the gradient reads.
+ * No counterpart in the reference, whose only recurrence is the SSD's (ops/ssd_naive.py:220-322).
+ * ------------------------------------------------------------------------- */
+#define M2_RECURRENCE_SPAN 64
+typedef struct {
+    const void*    x;              /* [b, L, d] at the strides below, dtype     */
+    const void*    r;              /* the same: the decay's gate                */
+    const void*    i;              /* the same: the input's gate                */
+    const float*   A;              /* [d]                                       */
+    const float*   initial_states; /* [b, d] or NULL                            */
+    const int32_t* seq_idx;        /* [b, L] contiguous, or NULL                */
+    void*          out;            /* out [b, L, d] contiguous, dtype           */
+    float*         final_states;   /* out [b, d] or NULL                        */
+    float*         span_states;    /* out [b, ceil(L / span), d] or NULL        */
+    int64_t batch, seqlen, dim;
+    int64_t x_stride_batch, x_stride_time, r_stride_batch, r_stride_time, i_stride_batch, i_stride_time;
+    int32_t dtype;
+} m2_gated_recurrence_args;
+int m2_gated_recurrence(const m2_gated_recurrence_args* a, void* stream);
+
+/* ---------------------------------------------------------------------------
+ * gated_linear_recurrence_grad: from the gradients of out and of final_states those of x, r,
+ * i, A (summed over the batch in order) and initial_states; the states are computed again from
+ * span_states.  The gradients of padding are 0.  Where a[t] is 1 the root has no slope: its part is
+ * taken as 0.
+ * ------------------------------------------------------------------------- */
+typedef struct {
+    const void*    x;
+    const void*    r;
+    const void*    i;
+    const float*   A;
+    const int32_t* seq_idx;
+    const float*   span_states;    /* as the forward left them                  */
+    const void*    grad_out;       /* [b, L, d] at the strides below, dtype     */
+    const float*   grad_final_states;   /* [b, d] or NULL                       */
+    void*          grad_x;         /* out [b, L, d] contiguous, dtype           */
+    void*          grad_r;
+    void*          grad_i;
+    float*         grad_A;         /* out [d]                                   */
+    float*         grad_initial_states; /* out [b, d] or NULL                   */
+    int64_t batch, seqlen, dim;
+    int64_t x_stride_batch, x_stride_time, r_stride_batch, r_stride_time, i_stride_batch, i_stride_time;
+    int64_t grad_out_stride_batch, grad_out_stride_time;
+    int32_t dtype;
+    void*   workspace;
+    size_t  workspace_bytes;
+} m2_gated_recurrence_grad_args;
+size_t m2_gated_recurrence_grad_workspace_size(const m2_gated_recurrence_grad_args* a);
+int m2_gated_recurrence_grad(const m2_gated_recurrence_grad_args* a, void* stream);
+
+/* ---------------------------------------------------------------------------
+ * gated_linear_recurrence_update: one position of every batch row, new_state = h, out = h
+ * rounded once; new_state may be state.
+ * ------------------------------------------------------------------------- */
+typedef struct {
+    const void*  x;                /* [b, d] at x_stride_batch, dtype           */
+    const void*  r;
+    const void*  i;
+    const float* A;                /* [d]                                       */
+    const float* state;            /* [b, d]                                    */
+    float*       new_state;        /* out [b, d]                                */
+    void*        out;              /* out [b, d], dtype                         */
+    int64_t batch, dim;
+    int64_t x_stride_batch, r_stride_batch, i_stride_batch;
+    int32_t dtype;
+} m2_gated_recurrence_update_args;
+int m2_gated_recurrence_update(const m2_gated_recurrence_update_args* a, void* stream);
+
+/* ---------------------------------------------------------------------------
  * Testing hook, no counterpart in the reference: forces one of the kernel
  * choices the library otherwise makes from the shape, process-wide, so that a
  * test can run every path on one shape (production code never calls it; no

@@ -84,6 +84,9 @@ M2_ENTRY(m2_embedding_grad, m2_embedding_grad_args, launch_embedding_grad)
 M2_ENTRY(m2_linear_cross_entropy, m2_linear_cross_entropy_args, launch_linear_ce)
 M2_ENTRY(m2_linear_cross_entropy_grad, m2_linear_cross_entropy_grad_args, launch_linear_ce_grad)
 M2_ENTRY(m2_clip_grad_norm, m2_clip_grad_norm_args, launch_clip_grad_norm)
+M2_ENTRY(m2_gated_recurrence, m2_gated_recurrence_args, launch_gated_recurrence)
+M2_ENTRY(m2_gated_recurrence_grad, m2_gated_recurrence_grad_args, launch_gated_recurrence_grad)
+M2_ENTRY(m2_gated_recurrence_update, m2_gated_recurrence_update_args, launch_gated_recurrence_update)
 
 extern "C" size_t m2_embedding_grad_workspace_size(const m2_embedding_grad_args* a) {
     return a ? m2::embedding_grad_workspace(*a) : 0;
@@ -100,6 +103,9 @@ extern "C" size_t m2_linear_cross_entropy_grad_workspace_size(
 }
 extern "C" size_t m2_clip_grad_norm_workspace_size(const m2_clip_grad_norm_args* a) {
     return a ? m2::clip_grad_norm_workspace(*a) : 0;
+}
+extern "C" size_t m2_gated_recurrence_grad_workspace_size(const m2_gated_recurrence_grad_args* a) {
+    return a ? m2::gated_recurrence_grad_workspace(*a) : 0;
 }
 
 // ---------------------------------------------------------------------------

@@ -63,6 +63,12 @@ size_t linear_ce_grad_workspace(const m2_linear_cross_entropy_grad_args& a);
 int launch_clip_grad_norm(const m2_clip_grad_norm_args& a, hipStream_t stream);
 size_t clip_grad_norm_workspace(const m2_clip_grad_norm_args& a);
 
+// the gated linear recurrence (gated_recurrence.hip)
+int launch_gated_recurrence(const m2_gated_recurrence_args& a, hipStream_t stream);
+int launch_gated_recurrence_grad(const m2_gated_recurrence_grad_args& a, hipStream_t stream);
+size_t gated_recurrence_grad_workspace(const m2_gated_recurrence_grad_args& a);
+int launch_gated_recurrence_update(const m2_gated_recurrence_update_args& a, hipStream_t stream);
+
 // chunk_state_varlen for bf16, head dim 64, dstate % 64 == 0, chunk_size % 32
 // == 0 (<= 256): one workgroup per (sequence, head, 64-column dstate block)
 bool varlen_states_fast_supported(const m2_chunk_state_varlen_args& a);

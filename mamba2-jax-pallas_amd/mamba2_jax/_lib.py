@@ -186,6 +186,32 @@ class ClipGradNormArgs(ctypes.Structure):
                 ("workspace_bytes", ctypes.c_size_t)]
 
 
+class GatedRecurrenceArgs(ctypes.Structure):
+    _fields_ = [("x", _c_p), ("r", _c_p), ("i", _c_p), ("A", _c_p), ("initial_states", _c_p),
+                ("seq_idx", _c_p), ("out", _c_p), ("final_states", _c_p), ("span_states", _c_p),
+                ("batch", _i64), ("seqlen", _i64), ("dim", _i64), ("x_stride_batch", _i64),
+                ("x_stride_time", _i64), ("r_stride_batch", _i64), ("r_stride_time", _i64),
+                ("i_stride_batch", _i64), ("i_stride_time", _i64), ("dtype", _i32)]
+
+
+class GatedRecurrenceGradArgs(ctypes.Structure):
+    _fields_ = [("x", _c_p), ("r", _c_p), ("i", _c_p), ("A", _c_p), ("seq_idx", _c_p),
+                ("span_states", _c_p), ("grad_out", _c_p), ("grad_final_states", _c_p),
+                ("grad_x", _c_p), ("grad_r", _c_p), ("grad_i", _c_p), ("grad_A", _c_p),
+                ("grad_initial_states", _c_p), ("batch", _i64), ("seqlen", _i64), ("dim", _i64),
+                ("x_stride_batch", _i64), ("x_stride_time", _i64), ("r_stride_batch", _i64),
+                ("r_stride_time", _i64), ("i_stride_batch", _i64), ("i_stride_time", _i64),
+                ("grad_out_stride_batch", _i64), ("grad_out_stride_time", _i64), ("dtype", _i32),
+                ("workspace", _c_p), ("workspace_bytes", ctypes.c_size_t)]
+
+
+class GatedRecurrenceUpdateArgs(ctypes.Structure):
+    _fields_ = [("x", _c_p), ("r", _c_p), ("i", _c_p), ("A", _c_p), ("state", _c_p),
+                ("new_state", _c_p), ("out", _c_p), ("batch", _i64), ("dim", _i64),
+                ("x_stride_batch", _i64), ("r_stride_batch", _i64), ("i_stride_batch", _i64),
+                ("dtype", _i32)]
+
+
 # entry point name -> argument struct (every function declared in m2ssd.h)
 ENTRY_POINTS = {
     "m2_chunk_cumsum": ChunkCumsumArgs,
@@ -207,6 +233,9 @@ ENTRY_POINTS = {
     "m2_linear_cross_entropy": LinearCrossEntropyArgs,
     "m2_linear_cross_entropy_grad": LinearCrossEntropyGradArgs,
     "m2_clip_grad_norm": ClipGradNormArgs,
+    "m2_gated_recurrence": GatedRecurrenceArgs,
+    "m2_gated_recurrence_grad": GatedRecurrenceGradArgs,
+    "m2_gated_recurrence_update": GatedRecurrenceUpdateArgs,
 }
 # workspace size functions of the entry points that take a workspace besides the
 # combined forward: name -> argument struct
@@ -216,7 +245,10 @@ WORKSPACE_SIZES = {
     "m2_linear_cross_entropy_saved_size": LinearCrossEntropyArgs,
     "m2_linear_cross_entropy_grad_workspace_size": LinearCrossEntropyGradArgs,
     "m2_clip_grad_norm_workspace_size": ClipGradNormArgs,
+    "m2_gated_recurrence_grad_workspace_size": GatedRecurrenceGradArgs,
 }
+# positions between two of the states that the recurrence leaves its gradient (M2_RECURRENCE_SPAN)
+RECURRENCE_SPAN = 64
 OTHER_SYMBOLS = ("m2_ssd_combined_workspace_size", "m2_ssd_combined_plan", "m2_last_error", "m2_abi_version",
                  "m2_set_dispatch_override", "m2_ssd_combined_noalloc_prepare",
                  *WORKSPACE_SIZES)

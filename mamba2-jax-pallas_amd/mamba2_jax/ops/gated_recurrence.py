@@ -1,0 +1,185 @@
+"""The gated linear recurrence over time on MI355X, its gradient and its single step, as
+HIP kernels in libm2ssd.so (m2_gated_recurrence, m2_gated_recurrence_grad,
+m2_gated_recurrence_update).
+
+    log a_t = A sigmoid(r_t)
+    h_t = a_t h_{t-1} + sqrt(1 - a_t^2) sigmoid(i_t) x_t
+
+No counterpart operator in the reference, whose only recurrence is the SSD's
+(ops/ssd_naive.py:220-322), a state of headdim x dstate values with one decay for each head;
+here a channel is a state of its own with its own decay, and the two gates come
+straight from the projections that make them.
+"""
+
+from __future__ import annotations
+
+import torch
+from torch.autograd.function import once_differentiable
+
+from .. import _lib as L
+
+
+def _strided(t):
+    """t with contiguous channels (a copy where they are not)."""
+    return t if t.stride(-1) == 1 or t.shape[-1] == 1 else t.contiguous()
+
+
+def _f32(t):
+    """t as a contiguous float32 tensor (a view where it can be), or None."""
+    if t is None:
+        return None
+    if t.dtype != torch.float32:
+        t = t.float()
+    return t if t.is_contiguous() else t.contiguous()
+
+
+def _forward(x, r, i, A, initial_states, seq_idx, want_final, save):
+    """-> (out, the final states or None, what the gradient reads)"""
+    dev = x.device
+    batch, seqlen, dim = x.shape
+    x, r, i = _strided(x), _strided(r), _strided(i)
+    A, h0 = _f32(A), _f32(initial_states)
+    out = torch.empty((batch, seqlen, dim), dtype=x.dtype, device=dev)
+    final = torch.empty((batch, dim), dtype=torch.float32, device=dev) if want_final else None
+    spans = torch.empty((batch, -(-seqlen // L.RECURRENCE_SPAN), dim), dtype=torch.float32, device=dev) \
+        if save else None
+    args = L.GatedRecurrenceArgs(
+        x.data_ptr(), r.data_ptr(), i.data_ptr(), A.data_ptr(), L.ptr(h0), L.ptr(seq_idx),
+        out.data_ptr(), L.ptr(final), L.ptr(spans), batch, seqlen, dim, x.stride(0), x.stride(1),
+        r.stride(0), r.stride(1), i.stride(0), i.stride(1), L.dtype_code(x, "x"))
+    with L.on_device(dev):
+        L.call("m2_gated_recurrence", args, L.stream_of(dev))
+    return out, final, (x, r, i, A, seq_idx, spans)
+
+
+def _backward(ctx, grad, grad_final=None):
+    x, r, i, A, seq_idx, spans = ctx.saved_tensors
+    a_dtype, h0_dtype = ctx.dtypes
+    batch, seqlen, dim = x.shape
+    dev = x.device
+    has_h0 = h0_dtype is not None
+    if batch == 0 or seqlen == 0:
+        dh0 = None
+        if has_h0:
+            dh0 = torch.zeros((batch, dim), dtype=h0_dtype, device=dev) if grad_final is None \
+                else grad_final.to(h0_dtype)
+        return x.new_zeros(x.shape), x.new_zeros(x.shape), x.new_zeros(x.shape), \
+            torch.zeros(dim, dtype=a_dtype, device=dev), dh0, None, None
+    g = x.new_zeros(x.shape) if grad is None else _strided(grad)
+    gf = _f32(grad_final)
+    dx, dr, di = (torch.empty((batch, seqlen, dim), dtype=x.dtype, device=dev) for _ in range(3))
+    dA = torch.empty(dim, dtype=torch.float32, device=dev)
+    dh0 = torch.empty((batch, dim), dtype=torch.float32, device=dev) if has_h0 else None
+    args = L.GatedRecurrenceGradArgs(
+        x.data_ptr(), r.data_ptr(), i.data_ptr(), A.data_ptr(), L.ptr(seq_idx), spans.data_ptr(),
+        g.data_ptr(), L.ptr(gf), dx.data_ptr(), dr.data_ptr(), di.data_ptr(), dA.data_ptr(),
+        L.ptr(dh0), batch, seqlen, dim, x.stride(0), x.stride(1), r.stride(0), r.stride(1),
+        i.stride(0), i.stride(1), g.stride(0), g.stride(1), L.dtype_code(x, "x"))
+    L.call_with_workspace("m2_gated_recurrence_grad", args, dev)
+    if a_dtype != torch.float32:
+        dA = dA.to(a_dtype)
+    if has_h0 and h0_dtype != torch.float32:
+        dh0 = dh0.to(h0_dtype)
+    return dx, dr, di, dA, dh0, None, None
+
+
+_backward_once = once_differentiable(_backward)
+
+
+class _GatedRecurrence(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, r, i, A, initial_states, seq_idx, want_final):
+        ctx.set_materialize_grads(False)
+        out, final, saved = _forward(x, r, i, A, initial_states, seq_idx, want_final, True)
+        ctx.save_for_backward(*saved)
+        ctx.dtypes = A.dtype, None if initial_states is None else initial_states.dtype
+        return (out, final) if want_final else out
+
+    @staticmethod
+    def backward(ctx, grad, grad_final=None):
+        return (_backward_once if torch.is_grad_enabled() else _backward)(ctx, grad, grad_final)
+
+
+def _check_gates(x, r, i, A, shape):
+    L.require(shape[-1] > 0, lambda: f"x.shape={tuple(shape)}: no channels")
+    L.require(r.shape == shape and i.shape == shape,
+              lambda: f"r.shape={tuple(r.shape)}, i.shape={tuple(i.shape)}: expected x's {tuple(shape)}")
+    L.require(A.shape == shape[-1:], lambda: f"A.shape={tuple(A.shape)}: expected ({shape[-1]},)")
+    code = L.dtype_code(x, "x")
+    if r.dtype != x.dtype or i.dtype != x.dtype:
+        raise TypeError(f"x is {x.dtype}, r {r.dtype} and i {i.dtype}: they must be the same")
+    L.dtype_code(A, "A")
+    return code
+
+
+def gated_linear_recurrence(x, r, i, A, initial_states=None, seq_idx=None, return_final_states=False):
+    """-> h (batch, seqlen, dim), x's dtype, and with return_final_states (h, final states (batch,
+    dim) float32), of
+
+        log a_t = A sigmoid(r_t),  h_t = a_t h_{t-1} + sqrt(1 - a_t^2) sigmoid(i_t) x_t
+
+    for every channel; differentiable in x, r, i, A and initial_states.
+
+    x, r, i (batch, seqlen, dim), all bfloat16 or all float32: views whose channels are
+    contiguous (slices of one projection's output, say) are read in place.  A (dim,), finite and <= 0 (a
+    positive one gives NaN), float32 or bfloat16.  initial_states (batch, dim): h_{-1}, zeros by
+    default.  seq_idx (batch, seqlen) int32 or int64 (of int32's range): where an entry differs from the one before it a new
+    sequence begins, with a state of zero (the first goes on from initial_states); a negative
+    entry is padding: h is 0 there, the state passes it unchanged, its
+    gradients are 0 and what the inputs hold there (a NaN, say) reaches nothing.  The final
+    states are those behind the last position.
+
+    Gates, states and sums are float32 (a state and the gradient that comes back to it never
+    leave it between two positions); h and the gradients are rounded once.  Between the two the graph holds x, r, i and
+    the states that enter every 64 positions.  Where a_t is 1 the root has no slope, and its part
+    of the gradient is taken as 0.  Equal inputs give equal bits."""
+    dev = L.device_of(x, r, i, A, initial_states, seq_idx)
+    shape = x.shape
+    L.require(len(shape) == 3, lambda: f"x.shape={tuple(shape)}: expected (batch, seqlen, dim)")
+    _check_gates(x, r, i, A, shape)
+    if initial_states is not None:
+        L.require(initial_states.shape == (shape[0], shape[2]),
+                  lambda: f"initial_states.shape={tuple(initial_states.shape)}: expected {(shape[0], shape[2])}")
+        L.dtype_code(initial_states, "initial_states")
+    if seq_idx is not None:
+        L.require(seq_idx.shape == shape[:2],
+                  lambda: f"seq_idx.shape={tuple(seq_idx.shape)}: expected {tuple(shape[:2])}")
+        L.index_code(seq_idx, "seq_idx")
+        seq_idx = seq_idx.to(torch.int32).contiguous()
+    want_final = bool(return_final_states)
+    if torch.is_grad_enabled() and (x.requires_grad or r.requires_grad or i.requires_grad or A.requires_grad
+                                    or (initial_states is not None and initial_states.requires_grad)):
+        return _GatedRecurrence.apply(x, r, i, A, initial_states, seq_idx, want_final)
+    out, final, _ = _forward(x, r, i, A, initial_states, seq_idx, want_final, False)
+    return (out, final) if want_final else out
+
+
+def gated_linear_recurrence_update(state, x, r, i, A, *, inplace=False):
+    """One step of ``gated_linear_recurrence`` -> (new_state (batch, dim) float32, h (batch, dim),
+    x's dtype).
+
+    state (batch, dim); x, r, i (batch, dim), all bfloat16 or all float32, rows with contiguous
+    channels read in place; A (dim,).  The caller's state is left untouched, unless inplace=True (keyword
+    only) and it is float32 and contiguous: it is then updated and returned.
+    Takes no gradients."""
+    dev = L.device_of(state, x, r, i, A)
+    shape = x.shape
+    L.require(len(shape) == 2, lambda: f"x.shape={tuple(shape)}: expected (batch, dim)")
+    L.require(state.shape == shape, lambda: f"state.shape={tuple(state.shape)}: expected {tuple(shape)}")
+    code = _check_gates(x, r, i, A, shape)
+    L.dtype_code(state, "state")
+    src = _f32(state)
+    new = src if inplace and src is state else torch.empty(shape, dtype=torch.float32, device=dev)
+    x, r, i, A = _strided(x), _strided(r), _strided(i), _f32(A)
+    out = torch.empty(shape, dtype=x.dtype, device=dev)
+    args = L.GatedRecurrenceUpdateArgs(
+        x.data_ptr(), r.data_ptr(), i.data_ptr(), A.data_ptr(), src.data_ptr(), new.data_ptr(),
+        out.data_ptr(), shape[0], shape[1], x.stride(0), r.stride(0), i.stride(0), code)
+    with L.on_device(dev):
+        L.call("m2_gated_recurrence_update", args, L.stream_of(dev))
+    if new is state:
+        torch.autograd.graph.increment_version(new)
+    return new, out
+
+
+__all__ = ["gated_linear_recurrence", "gated_linear_recurrence_update"]

@@ -644,6 +644,53 @@ typedef struct {
 int m2_gated_recurrence_update(const m2_gated_recurrence_update_args* a, void* stream);
 
 /* ---------------------------------------------------------------------------
+ * gated_linear: the first half of a gated feed-forward block,
+ *   g[n, f] = x[n] . weight[f],  v[n, f] = x[n] . weight[hidden + f],  out = act(g) v,
+ * float32 sums, rounded once; act(g) = g sigmoid(g) (M2_SILU) or gelu's tanh form (M2_GELU).  float32
+ * operands are multiplied as three bf16 parts each (six products, about 2^-24 of each; an infinity
+ * among them gives NaN).  With saved (m2_gated_linear_saved_size bytes, 16-byte aligned) g and v
+ * are left there for the gradient, in dtype.  n < 2^30, hidden dim < 2^30.
+ * No counterpart in the reference, whose blocks have a mixer alone (models/mamba2_lm.py:196-211).
+ * ------------------------------------------------------------------------- */
+#define M2_SILU 0
+#define M2_GELU 1
+typedef struct {
+    const void* x;                 /* [n, dim] at ldx, dtype                    */
+    const void* weight;            /* [2 hidden, dim] at ldw, dtype             */
+    void*       out;               /* out [n, hidden] contiguous, dtype         */
+    int64_t n, dim, hidden, ldx, ldw;
+    int32_t dtype, activation;
+    void*   workspace;
+    size_t  workspace_bytes;
+    void*   saved;                 /* out, or NULL                              */
+    size_t  saved_bytes;
+} m2_gated_linear_args;
+size_t m2_gated_linear_saved_size(const m2_gated_linear_args* a);
+size_t m2_gated_linear_workspace_size(const m2_gated_linear_args* a);
+int m2_gated_linear(const m2_gated_linear_args* a, void* stream);
+
+/* ---------------------------------------------------------------------------
+ * gated_linear_grad: with d = grad_out, dv = d act(g), dg = d v act'(g) (bf16 operands: rounded to
+ * bf16 once),
+ *   grad_x = dg weight[:hidden] + dv weight[hidden:],  grad_weight = [dg | dv]^T x
+ * from what the forward left in saved for the same arguments.  Either output may be NULL.
+ * ------------------------------------------------------------------------- */
+typedef struct {
+    const void* x;
+    const void* weight;
+    const void* saved;             /* as the forward left it                    */
+    const void* grad_out;          /* [n, hidden] at ldg, dtype                 */
+    void*       grad_x;            /* out [n, dim] contiguous, dtype, or NULL   */
+    void*       grad_weight;       /* out [2 hidden, dim] contiguous, or NULL   */
+    int64_t n, dim, hidden, ldx, ldw, ldg;
+    int32_t dtype, activation;
+    void*   workspace;
+    size_t  workspace_bytes;
+} m2_gated_linear_grad_args;
+size_t m2_gated_linear_grad_workspace_size(const m2_gated_linear_grad_args* a);
+int m2_gated_linear_grad(const m2_gated_linear_grad_args* a, void* stream);
+
+/* ---------------------------------------------------------------------------
  * Testing hook, no counterpart in the reference: forces one of the kernel
  * choices the library otherwise makes from the shape, process-wide, so that a
  * test can run every path on one shape (production code never calls it; no

@@ -86,6 +86,8 @@ M2_ENTRY(m2_linear_cross_entropy_grad, m2_linear_cross_entropy_grad_args, launch
 M2_ENTRY(m2_clip_grad_norm, m2_clip_grad_norm_args, launch_clip_grad_norm)
 M2_ENTRY(m2_gated_recurrence, m2_gated_recurrence_args, launch_gated_recurrence)
 M2_ENTRY(m2_gated_recurrence_grad, m2_gated_recurrence_grad_args, launch_gated_recurrence_grad)
+M2_ENTRY(m2_gated_linear, m2_gated_linear_args, launch_gated_linear)
+M2_ENTRY(m2_gated_linear_grad, m2_gated_linear_grad_args, launch_gated_linear_grad)
 M2_ENTRY(m2_gated_recurrence_update, m2_gated_recurrence_update_args, launch_gated_recurrence_update)
 
 extern "C" size_t m2_embedding_grad_workspace_size(const m2_embedding_grad_args* a) {
@@ -106,6 +108,15 @@ extern "C" size_t m2_clip_grad_norm_workspace_size(const m2_clip_grad_norm_args*
 }
 extern "C" size_t m2_gated_recurrence_grad_workspace_size(const m2_gated_recurrence_grad_args* a) {
     return a ? m2::gated_recurrence_grad_workspace(*a) : 0;
+}
+extern "C" size_t m2_gated_linear_saved_size(const m2_gated_linear_args* a) {
+    return a ? m2::gated_linear_saved(*a) : 0;
+}
+extern "C" size_t m2_gated_linear_workspace_size(const m2_gated_linear_args* a) {
+    return a ? m2::gated_linear_workspace(*a) : 0;
+}
+extern "C" size_t m2_gated_linear_grad_workspace_size(const m2_gated_linear_grad_args* a) {
+    return a ? m2::gated_linear_grad_workspace(*a) : 0;
 }
 
 // ---------------------------------------------------------------------------

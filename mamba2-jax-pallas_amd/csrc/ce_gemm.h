@@ -1,6 +1,6 @@
 // Tiled bf16 matrix product D[m, n] = sum_k A[m, k] B[n, k] of the vocabulary's loss
-// (linear_ce.hip), with the epilogue as a template parameter: the logits of a tile
-// exist in its accumulators only.
+// (linear_ce.hip) and of the gated feed-forward product (gated_linear.hip), with the epilogue as a template
+// parameter: the logits, or the two products, of a tile exist in its accumulators only.
 //
 // A tile is BM x BN, K in steps of BK (64 or 32) through a ring of ST LDS slots filled by
 // direct global -> LDS loads; WM x WN wavefronts, 16x16x32 MFMAs.  Each operand
@@ -25,12 +25,103 @@
 
 namespace m2ce {
 
+// ---------------------------------------------------------------------------
+// rows in and out
+// ---------------------------------------------------------------------------
+// 8 consecutive elements of a row, zero past its end
+template <typename T> M2_DEV void load8(const T* row, int64_t c, int64_t dim, float (&v)[8]) {
+    if (c + 8 <= dim) {
+        if constexpr (sizeof(T) == 2) {
+            const u32x4 r = load16(row + c);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) { v[2 * i] = bf16_lo(r[i]); v[2 * i + 1] = bf16_hi(r[i]); }
+        } else {
+            const u32x4 a = load16(row + c), b = load16(row + c + 4);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) { v[i] = __uint_as_float(a[i]); v[4 + i] = __uint_as_float(b[i]); }
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = c + i < dim ? to_f32(row[c + i]) : 0.f;
+    }
+}
+// v = h + m + l, each bf16 (an infinity or NaN stays in h alone)
+M2_DEV void split3(float v, float& h, float& m, float& l) {
+    h = (float)(bf16)v;
+    const float r = v - h;
+    const bool fin = fabsf(h) < __builtin_inff();
+    m = fin ? (float)(bf16)r : 0.f;
+    l = fin ? r - m : 0.f;
+}
+template <bool PLANES> M2_DEV void store8(bf16* p, int64_t plane, const float (&v)[8]) {
+    if constexpr (!PLANES) {
+        const u32x4 r = {pk_bf16(v[0], v[1]), pk_bf16(v[2], v[3]), pk_bf16(v[4], v[5]), pk_bf16(v[6], v[7])};
+        *reinterpret_cast<u32x4*>(p) = r;
+    } else {
+        float h[8], m[8], l[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) split3(v[i], h[i], m[i], l[i]);
+        store8<false>(p, 0, h);
+        store8<false>(p + plane, 0, m);
+        store8<false>(p + 2 * plane, 0, l);
+    }
+}
+
+// Two fragments of 16 m beside each other, x and y: lane rows (16 lanes) 0 and 2 exchange
+// theirs of y for rows 1's and 3's of x, after which a lane holds 8 consecutive m from
+// pair_m on: (p, q)
+M2_DEV void pair_swap(uint32_t& p, uint32_t& q) {
+    const auto r = __builtin_amdgcn_permlane16_swap(p, q, false, false);
+    p = r[0];
+    q = r[1];
+}
+M2_DEV int pair_m(int lane) { return 16 * ((lane >> 4) & 1) + 8 * (lane >> 5); }
+M2_DEV void store_pair(bf16* d, const float (&x)[4], const float (&y)[4]) {
+    uint32_t a0 = pk_bf16(x[0], x[1]), a1 = pk_bf16(x[2], x[3]);
+    uint32_t b0 = pk_bf16(y[0], y[1]), b1 = pk_bf16(y[2], y[3]);
+    pair_swap(a0, b0);
+    pair_swap(a1, b1);
+    *reinterpret_cast<u32x4*>(d) = u32x4{a0, a1, b0, b1};
+}
+// the 32 values of m from m0 on (two fragments) of one n into a row of dim elements
+template <typename T>
+M2_DEV void store_row(T* row, int m0, int64_t dim, int lane, const f32x4& x, const f32x4& y) {
+    if constexpr (sizeof(T) == 2) {
+        // (the exchange is among the lanes of this n: all of them are here)
+        uint32_t p[4] = {pk_bf16(x[0], x[1]), pk_bf16(x[2], x[3]), pk_bf16(y[0], y[1]), pk_bf16(y[2], y[3])};
+        pair_swap(p[0], p[2]);
+        pair_swap(p[1], p[3]);
+        const int m = m0 + pair_m(lane);
+        if (m + 8 <= dim) {
+            store16(row + m, u32x4{p[0], p[1], p[2], p[3]});
+        } else {
+#pragma unroll
+            for (int r = 0; r < 8; ++r)
+                if (m + r < dim) reinterpret_cast<uint16_t*>(row)[m + r] = (uint16_t)(p[r >> 1] >> (16 * (r & 1)));
+        }
+    } else {
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+            const int m = m0 + 16 * e + 4 * (lane >> 4);
+            const f32x4& v = e ? y : x;
+            if (m + 4 <= dim) {
+                store16(row + m, __builtin_bit_cast(u32x4, v));
+            } else {
+#pragma unroll
+                for (int r = 0; r < 4; ++r)
+                    if (m + r < dim) row[m + r] = v[r];
+            }
+        }
+    }
+}
+
 struct Operand {
     const bf16* p;
     int64_t ld;          // elements between rows (row: of m; col: of k)
     int64_t plane;       // elements between the planes of a float32 operand
     int lim;             // valid m (row: rows past it read the last one; col: columns, a multiple of 8)
     int klim;            // valid k (row: pieces past it read zeros; col: rows past it read the last one)
+    int pair;            // of a paired row operand: rows between the two halves
 };
 
 struct Gemm {
@@ -82,7 +173,11 @@ template <int BK> M2_DEV int swz(int r) {
     return ((b ^ (b >> 1)) & 1) << 1 | b >> 1;
 }
 
-template <int R, bool TR, int NW, int BK> struct Loader {
+// PAIR (row operands): the tile's rows are 16 of one half of the matrix and the same 16 of the other
+// half, in turn, so that a wavefront's accumulators hold both of each pair; m0 counts the rows
+// of both, lim those of a half.
+template <int R, bool TR, int NW, int BK, bool PAIR = false> struct Loader {
+    static_assert(!(TR && PAIR), "");
     static constexpr int BYTES = R * BK * 2;
     static constexpr int INSTR = BYTES / 1024;                   // 1 KB each
     static constexpr int J = INSTR >= NW ? INSTR / NW : 1;       // per wavefront
@@ -93,11 +188,16 @@ template <int R, bool TR, int NW, int BK> struct Loader {
 
     // m0: first row (column) of the tile
     M2_DEV void init(const Operand& o, int m0_, int w, int lane) {
-        m0 = m0_;
+        m0 = PAIR ? m0_ / 2 : m0_;
 #pragma unroll
         for (int j = 0; j < J; ++j) {
             const int in = (w * J + j) % INSTR;
-            if constexpr (!TR) {
+            if constexpr (PAIR) {
+                const int row = in * (64 / PP) + lane / PP;
+                const int c = (lane & (PP - 1)) ^ swz<BK>(row);
+                const int f = min(m0 + (row >> 5) * 16 + (row & 15), o.lim - 1) - m0;
+                off[j] = (uint32_t)((int64_t)(f + ((row >> 4) & 1) * o.pair) * o.ld * 2 + c * 16);
+            } else if constexpr (!TR) {
                 const int row = in * (64 / PP) + lane / PP;
                 const int c = (lane & (PP - 1)) ^ swz<BK>(row);
                 off[j] = (uint32_t)((int64_t)(min(m0 + row, o.lim - 1) - m0) * o.ld * 2 + c * 16);
@@ -176,12 +276,13 @@ template <int R, bool TR, int F, int BK> struct Reader {
     }
 };
 
-template <int BM_, int BN_, int WM_, int WN_, int ST_, int BK_, bool ATR_, bool BTR_, int TERMS_> struct Shape {
+template <int BM_, int BN_, int WM_, int WN_, int ST_, int BK_, bool ATR_, bool BTR_, int TERMS_, bool PAIR_ = false>
+struct Shape {
     static constexpr int BK = BK_, BM = BM_, BN = BN_, WM = WM_, WN = WN_, ST = ST_, TERMS = TERMS_;
     static constexpr bool ATR = ATR_, BTR = BTR_;
     static constexpr int NW = WM * WN, NT = NW * 64;
     static constexpr int FM = BM / WM / 16, FN = BN / WN / 16;
-    typedef Loader<BM, ATR, NW, BK> LA;
+    typedef Loader<BM, ATR, NW, BK, PAIR_> LA;
     typedef Loader<BN, BTR, NW, BK> LB;
     static constexpr int SLOT = LA::BYTES + LB::BYTES;
     static constexpr int LDS = SLOT * ST;
@@ -592,5 +693,24 @@ __global__ void __launch_bounds__(S::NT, S::NT / 256) k_ce_planes(Gemm g, EPI ep
     }
     wait_vmem<0>();           // no load may land after the workgroup has ended
 }
+
+// ---------------------------------------------------------------------------
+// launches
+// ---------------------------------------------------------------------------
+inline size_t align256(size_t v) { return (v + 255) & ~size_t(255); }
+inline bool al16(const void* p) { return ((uintptr_t)p & 15) == 0; }
+
+template <class S, class EPI> void launch(const Gemm& g, const EPI& e, hipStream_t s) {
+    const int64_t tiles = (int64_t)g.tm * g.tn;
+    if constexpr (S::TERMS == 1 && S::BN < 128) {
+        hipLaunchKernelGGL((k_ce_stream<S, EPI>), dim3((unsigned)(tiles * g.splits)), dim3(S::NT), 0, s, g, e);
+    } else {
+        const int64_t ncu = m2::cu_count();
+        const unsigned nwg = (unsigned)(EPI::SEG ? g.splits : tiles < ncu ? tiles : ncu);
+        if constexpr (S::TERMS == 1) hipLaunchKernelGGL((k_ce_tile<S, EPI>), dim3(nwg), dim3(S::NT), 0, s, g, e);
+        else hipLaunchKernelGGL((k_ce_planes<S, EPI>), dim3(nwg), dim3(S::NT), 0, s, g, e);
+    }
+}
+inline int tiles(int64_t n, int t) { return (int)((n + t - 1) / t); }
 
 }  // namespace m2ce

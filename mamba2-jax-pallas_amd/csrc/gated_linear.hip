@@ -1,0 +1,686 @@
+// The gated feed-forward product and its gradient:
+//
+//   [g | v] = x W^T (W: the gate's F rows, then the values'),  h = act(g) v
+//   dv = dh act(g), dg = dh v act'(g);  dx = [dg | dv] W;  dW = [dg | dv]^T x
+//
+// act(g) = g sigmoid(u), u = g (silu) or 2 c (g + k g^3), c = sqrt(2 / pi), k = 0.044715 (gelu's tanh form).
+//
+// Forward: the product runs in the tiles of ce_gemm.h, whose rows are 16 of the gate and
+// the same 16 of the values in turn (PAIR): a lane's accumulators hold g and v of the same place, and
+// the epilogue stores h alone (and, for a gradient, g and v in the operands' type: to compute them again
+// would take a third of the gradient's operations, to keep them costs their bytes twice).  Up to 64 tokens
+// whose rows a lane can load in 16-byte pieces run k_glu_few, bound by reading W once.
+// Backward: k_glu_dz makes dz = [dg | dv] (bf16, or three planes of it for float32), then two
+// products read it: dx with K over W's rows, dW with K over the tokens.  Tiles that would leave CUs idle in the
+// last round are cut along K into float32 parts (deal), which k_glu_join adds up.
+//
+// Operands that direct loads cannot take in place (float32, widths that 64 does not divide, unaligned
+// rows) are packed first: rows padded with zeros, the gate's and the values' to whole 64s.
+#include "ce_gemm.h"
+
+namespace {
+
+using namespace m2ce;
+
+constexpr float LOG2E = 1.4426950408889634f;
+
+// act(g) and, for SLOPE, its derivative
+template <bool SLOPE> M2_DEV float act(float g, int gelu, float& slope) {
+    constexpr float C2 = 1.5957691216057308f, K = 0.044715f;
+    // (bounded: past +-100, +-20 of gelu, the sigmoid is 0 or 1 and its slope 0, not 0 inf)
+    const float lim = gelu ? 20.f : 100.f, b = __builtin_amdgcn_fmed3f(g, -lim, lim);
+    const float u = gelu ? C2 * b * fmaf(K * b, b, 1.f) : b;
+    const float s = __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(u * -LOG2E));
+    if constexpr (SLOPE) {
+        const float du = gelu ? C2 * fmaf(3.f * K * b, b, 1.f) : 1.f;
+        slope = g != g ? g : fmaf(b * s * (1.f - s), du, s);
+    }
+    return g * s;
+}
+
+// four consecutive values of a row of dim elements
+template <typename T> M2_DEV void store_quad(T* row, int m, int64_t dim, const f32x4& v) {
+    if (m + 4 <= dim) {
+        if constexpr (sizeof(T) == 2) {
+            typedef uint32_t any __attribute__((ext_vector_type(2), aligned(2)));
+            *reinterpret_cast<any*>(row + m) = any{pk_bf16(v[0], v[1]), pk_bf16(v[2], v[3])};
+        } else {
+            store16(row + m, __builtin_bit_cast(u32x4, v));
+        }
+    } else {
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+            if (m + r < dim) row[m + r] = from_f32<T>(v[r]);
+    }
+}
+
+// ---------------------------------------------------------------------------
+// forward
+// ---------------------------------------------------------------------------
+// m: pairs of the hidden size, n: token -> h, and z = [g | v] with rows of 2 fp
+template <typename T> struct EpiGlu {
+    static constexpr bool SEG = false;
+    T* h;
+    T* z;                    // or NULL
+    int64_t hidden, fp;
+    int gelu;
+
+    template <class S>
+    M2_DEV void run(f32x4 (&acc)[S::FM][S::FN], int m0, int n0, int wm, int wn, int lane, int count, int, int) const {
+        static_assert(S::FM % 2 == 0, "");
+        constexpr bool WIDE = S::FM % 4 == 0;
+        const int f0 = m0 / 2 + wm * S::FM * 8;
+#pragma unroll
+        for (int j = 0; j < S::FN; ++j) {
+            const int n = n0 + (wn * S::FN + j) * 16 + (lane & 15);
+            if (n >= count) continue;
+            T* to = h + (int64_t)n * hidden;
+            T* gr = z + (int64_t)n * 2 * fp;
+#pragma unroll
+            for (int i = 0; i < S::FM; i += WIDE ? 4 : 2) {
+                const int f = f0 + 8 * i;
+                f32x4 o[WIDE ? 2 : 1];
+#pragma unroll
+                for (int e = 0; e < (WIDE ? 2 : 1); ++e)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) {
+                        float slope;
+                        o[e][r] = act<false>(acc[i + 2 * e][j][r], gelu, slope) * acc[i + 2 * e + 1][j][r];
+                    }
+                if constexpr (WIDE) {
+                    store_row(to, f, hidden, lane, o[0], o[1]);
+                    if (z) {
+                        store_row(gr, f, hidden, lane, acc[i][j], acc[i + 2][j]);
+                        store_row(gr + fp, f, hidden, lane, acc[i + 1][j], acc[i + 3][j]);
+                    }
+                } else {
+                    const int q = f + 4 * (lane >> 4);
+                    store_quad(to, q, hidden, o[0]);
+                    if (z) {
+                        store_quad(gr, q, hidden, acc[i][j]);
+                        store_quad(gr + fp, q, hidden, acc[i + 1][j]);
+                    }
+                }
+            }
+        }
+    }
+};
+
+// 8 consecutive k of a row as matrix operands: bf16, or a float32's three planes
+template <typename T> struct Few;
+template <> struct Few<bf16> {
+    bf16x8 v;
+    M2_DEV void load(const bf16* p, bool in) {
+        const bf16x8 zero = {};
+        v = *reinterpret_cast<const bf16x8*>(p);
+        if (!in) v = zero;
+    }
+    static M2_DEV f32x4 mma(const Few& a, const Few& b, f32x4 c) {
+        return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a.v, b.v, c, 0, 0, 0);
+    }
+};
+template <> struct Few<float> {
+    u32x4 lo, hi;
+    M2_DEV void load(const float* p, bool in) {
+        const u32x4 zero = {};
+        lo = reinterpret_cast<const u32x4*>(p)[0];
+        hi = reinterpret_cast<const u32x4*>(p)[1];
+        if (!in) lo = hi = zero;
+    }
+    M2_DEV void planes(bf16x8 (&p)[3]) const {
+        float h[8], m[8], l[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) split3(__uint_as_float(i < 4 ? lo[i & 3] : hi[i & 3]), h[i], m[i], l[i]);
+        auto pack = [](const float(&f)[8]) {
+            return as_bf16x8(pk_bf16(f[0], f[1]), pk_bf16(f[2], f[3]), pk_bf16(f[4], f[5]), pk_bf16(f[6], f[7]));
+        };
+        p[0] = pack(h); p[1] = pack(m); p[2] = pack(l);
+    }
+    static M2_DEV f32x4 mma(const Few& a, const Few& b, f32x4 c) {
+        bf16x8 x[3], y[3];
+        a.planes(x);
+        b.planes(y);
+        constexpr int PI[6] = {0, 2, 1, 0, 1, 0}, PJ[6] = {2, 0, 1, 1, 0, 0};      // the small products first
+#pragma unroll
+        for (int t = 0; t < 6; ++t) c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(x[PI[t]], y[PJ[t]], c, 0, 0, 0);
+        return c;
+    }
+};
+
+struct FewArgs {
+    const void *x, *w;
+    void *h, *z;
+    int64_t ldx, ldw, fp;
+    int n, dim, hidden, gelu;
+};
+// Up to 16 MT tokens: a workgroup takes 8 of the hidden size, its NW wavefronts split K and meet in LDS.
+// The 16 rows of a matrix operand are the 8 of the gate and the 8 of the values, so that lanes
+// l and l + 32 hold g and v of the same place; every weight is read once, x comes from the cache.
+template <typename T, int MT, int NW>
+__global__ void __launch_bounds__(NW * 64) k_glu_few(FewArgs a) {
+    constexpr int U = sizeof(T) == 2 ? (MT > 2 ? 4 : 8) : MT > 2 ? 2 : 4;    // steps of 32 whose loads are issued together
+    __shared__ f32x4 red[NW][MT][64];
+    const int lane = threadIdx.x & 63, w = wave_id();
+    const int f0 = blockIdx.x * 8, row = lane & 15, kq = (lane >> 4) * 8;
+    const T* wr = static_cast<const T*>(a.w) +
+                  ((int64_t)(row >> 3) * a.hidden + min(f0 + (row & 7), a.hidden - 1)) * a.ldw;
+    const T* xr[MT];
+#pragma unroll
+    for (int t = 0; t < MT; ++t) xr[t] = static_cast<const T*>(a.x) + (int64_t)min(16 * t + row, a.n - 1) * a.ldx;
+    const int steps = (a.dim + 31) / 32, per = (steps + NW - 1) / NW;
+    const int s1 = min(steps, (w + 1) * per);
+    f32x4 acc[MT];
+#pragma unroll
+    for (int t = 0; t < MT; ++t) acc[t] = zero4();
+    for (int s = w * per; s < s1; s += U) {
+        Few<T> fw[U], fx[U][MT];
+#pragma unroll
+        for (int q = 0; q < U; ++q) {
+            const int k = (s + q) * 32 + kq;
+            const bool in = s + q < s1 && k < a.dim;
+            const int at = in ? k : 0;
+            fw[q].load(wr + at, in);
+#pragma unroll
+            for (int t = 0; t < MT; ++t) fx[q][t].load(xr[t] + at, in);
+        }
+#pragma unroll
+        for (int q = 0; q < U; ++q)
+#pragma unroll
+            for (int t = 0; t < MT; ++t) acc[t] = Few<T>::mma(fw[q], fx[q][t], acc[t]);
+    }
+#pragma unroll
+    for (int t = 0; t < MT; ++t) red[w][t][lane] = acc[t];
+    __syncthreads();
+#pragma unroll
+    for (int t = w; t < MT; t += NW) {
+        f32x4 v = red[0][t][lane];
+#pragma unroll
+        for (int u = 1; u < NW; ++u) v += red[u][t][lane];
+        f32x4 o, other;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            other[r] = __shfl_xor(v[r], 32);
+            float slope;
+            o[r] = act<false>(v[r], a.gelu, slope) * other[r];
+        }
+        const int n = 16 * t + (lane & 15), f = f0 + 4 * ((lane >> 4) & 1);
+        if (lane >= 32 || n >= a.n) continue;
+        store_quad(static_cast<T*>(a.h) + (int64_t)n * a.hidden, f, a.hidden, o);
+        if (a.z) {
+            T* z = static_cast<T*>(a.z) + (int64_t)n * 2 * a.fp;
+            store_quad(z, f, a.hidden, v);
+            store_quad(z + a.fp, f, a.hidden, other);
+        }
+    }
+}
+
+// ---------------------------------------------------------------------------
+// packing, dz
+// ---------------------------------------------------------------------------
+// rows of src as bf16 (planes) with rows of dp elements, zeros behind dim and in the rows that src lacks: row j
+// is src's j, or with `half` the j-th of the first `valid` rows, and half + j the j-th of the other `valid`
+struct PackArgs {
+    const void* src;
+    bf16* dst;
+    int64_t rows, dim, ld, dp, plane, half, valid;
+};
+template <typename T> __global__ void __launch_bounds__(256) k_glu_pack(PackArgs a) {
+    const int64_t r = (int64_t)blockIdx.x * 4 + wave_id();
+    if (r >= a.rows) return;
+    const int lane = threadIdx.x & 63;
+    const int second = a.half && r >= a.half;
+    const int64_t j = second ? r - a.half : r;
+    const bool in = j < a.valid;
+    const T* src = static_cast<const T*>(a.src) + (in ? j + (second ? a.valid : 0) : 0) * a.ld;
+    for (int64_t c = lane * 8; c < a.dp; c += 512) {
+        float v[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+        if (in) load8(src, c, a.dim, v);
+        store8<sizeof(T) == 4>(a.dst + r * a.dp + c, a.plane, v);
+    }
+}
+
+struct DzArgs {
+    const void *z, *dh;
+    bf16* dz;                // [np][2 fp], zeros past n and past hidden
+    int64_t n, np, hidden, fp, ldg, plane;
+    int gelu;
+};
+template <typename T> __global__ void __launch_bounds__(256) k_glu_dz(DzArgs a) {
+    const int64_t per = a.fp / 8, id = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    const int64_t n = id / per, c = (id - n * per) * 8;
+    if (n >= a.np) return;
+    float dg[8] = {0, 0, 0, 0, 0, 0, 0, 0}, dv[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+    if (n < a.n && c < a.hidden) {
+        float g[8], v[8], up[8];
+        const T* z = static_cast<const T*>(a.z) + n * 2 * a.fp;
+        load8(z, c, a.fp, g);
+        load8(z + a.fp, c, a.fp, v);
+        load8(static_cast<const T*>(a.dh) + n * a.ldg, c, a.hidden, up);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            float slope;
+            const float s = act<true>(g[i], a.gelu, slope);
+            // (past the hidden size z holds anything)
+            dv[i] = c + i < a.hidden ? up[i] * s : 0.f;
+            dg[i] = c + i < a.hidden ? up[i] * v[i] * slope : 0.f;
+        }
+    }
+    bf16* to = a.dz + n * 2 * a.fp + c;
+    store8<sizeof(T) == 4>(to, a.plane, dg);
+    store8<sizeof(T) == 4>(to + a.fp, a.plane, dv);
+}
+
+// ---------------------------------------------------------------------------
+// the gradients' products
+// ---------------------------------------------------------------------------
+// where the rows (n) of a product go: the n-th, or with `half` the first `valid` of either half
+template <typename T> struct Out {
+    T* p;
+    int64_t dim;
+    int half, valid;
+    M2_DEV T* row(int n) const {
+        const int second = half && n >= half, j = second ? n - half : n;
+        return j < valid ? p + (int64_t)(second ? j + valid : j) * dim : nullptr;
+    }
+};
+// m: columns, n: rows.  A whole tile is stored; the parts of one that deal() cut as the lanes hold them,
+// [part][wavefront][i][j][lane] of 4 values.
+template <typename T> struct EpiOut {
+    static constexpr bool SEG = true;
+    Out<T> out;
+    float* part;
+    int full;                // tiles that are whole
+
+    template <class S>
+    M2_DEV void run(f32x4 (&acc)[S::FM][S::FN], int m0, int n0, int wm, int wn, int lane, int, int seg, int) const {
+        static_assert(S::FM % 2 == 0, "");
+        if (seg >= full) {
+            f32x4* d = reinterpret_cast<f32x4*>(part) +
+                       ((int64_t)(seg - full) * S::NW + wm * S::WN + wn) * S::FM * S::FN * 64 + lane;
+#pragma unroll
+            for (int i = 0; i < S::FM; ++i)
+#pragma unroll
+                for (int j = 0; j < S::FN; ++j) d[(i * S::FN + j) * 64] = acc[i][j];
+            return;
+        }
+        const int mw = m0 + wm * S::FM * 16, nw = n0 + wn * S::FN * 16;
+#pragma unroll
+        for (int j = 0; j < S::FN; ++j) {
+            T* to = out.row(nw + 16 * j + (lane & 15));
+            if (!to) continue;
+#pragma unroll
+            for (int i = 0; i < S::FM; i += 2) store_row(to, mw + 16 * i, out.dim, lane, acc[i][j], acc[i + 1][j]);
+        }
+    }
+};
+// the parts of the cut tiles, in their order: a wavefront for two fragments (32 columns) of 16 rows
+struct JoinArgs {
+    const float* part;
+    int tm, tn, full, rest, s;
+};
+template <typename T, class S> __global__ void __launch_bounds__(256) k_glu_join(JoinArgs a, Out<T> out) {
+    const int lane = threadIdx.x & 63;
+    constexpr int PAIRS = S::FM / 2, PER = S::NW * PAIRS * S::FN;
+    int q = blockIdx.x * 4 + wave_id();
+    const int t = q / PER;
+    q -= t * PER;
+    if (t >= a.rest) return;
+    const int j = q % S::FN, i = q / S::FN % PAIRS * 2, w = q / S::FN / PAIRS;
+    // (the tile's place as in the product's kernel)
+    const int tile = a.full + t;
+    const int grp = tile / (8 * a.tn), gm = min(8, a.tm - grp * 8), in = tile - grp * 8 * a.tn;
+    const int m0 = (grp * 8 + in % gm) * S::BM + (w / S::WN * S::FM + i) * 16;
+    T* to = out.row(in / gm * S::BN + (w % S::WN * S::FN + j) * 16 + (lane & 15));
+    constexpr int64_t TILE = (int64_t)S::NW * S::FM * S::FN * 64;
+    const f32x4* p = reinterpret_cast<const f32x4*>(a.part) + t * TILE + (w * S::FM * S::FN + i * S::FN + j) * 64 + lane;
+    f32x4 x = p[0], y = p[S::FN * 64];
+#pragma unroll 8
+    for (int k = 1; k < a.s; ++k) {
+        p += a.rest * TILE;
+        x += p[0];
+        y += p[S::FN * 64];
+    }
+    if (to) store_row(to, m0, out.dim, lane, x, y);
+}
+
+// few tokens (k_ce_stream): one array of dx for each split of K, [splits][np][dp]
+struct EpiSplit {
+    static constexpr bool SEG = false;
+    float* part;
+    int64_t np, dp;
+
+    template <class S>
+    M2_DEV void run(f32x4 (&acc)[S::FM][S::FN], int m0, int n0, int wm, int wn, int lane, int count, int split,
+                    int) const {
+        const int mv = m0 + wm * S::FM * 16 + 4 * (lane >> 4);
+#pragma unroll
+        for (int j = 0; j < S::FN; ++j) {
+            const int n = n0 + (wn * S::FN + j) * 16 + (lane & 15);
+            if (n >= count) continue;
+            float* d = part + ((int64_t)split * np + n) * dp;
+#pragma unroll
+            for (int i = 0; i < S::FM; ++i)
+                if (mv + 16 * i < dp) *reinterpret_cast<f32x4*>(d + mv + 16 * i) = acc[i][j];
+        }
+    }
+};
+__global__ void __launch_bounds__(64) k_glu_sum(const float* part, bf16* dx, int64_t np, int64_t dp, int64_t dim,
+                                                int splits) {
+    const int64_t n = blockIdx.y, c = ((int64_t)blockIdx.x * 64 + threadIdx.x) * 4;
+    if (c >= dim) return;
+    f32x4 v = zero4();
+    const float* p = part + n * dp + c;
+#pragma unroll 8
+    for (int s = 0; s < splits; ++s) v += *reinterpret_cast<const f32x4*>(p + s * np * dp);
+    store_quad(dx + n * dim, (int)c, dim, v);
+}
+
+// ---------------------------------------------------------------------------
+// plans
+// ---------------------------------------------------------------------------
+template <bool F32> struct Shapes {
+    typedef Shape<256, 256, 2, 4, 2, 64, false, false, 1, true> Z256;
+    typedef Shape<128, 64, 4, 1, 3, 64, false, false, 1, true> Z64;
+    typedef Shape<128, 16, 4, 1, 4, 64, false, false, 1, true> Z16;
+    typedef Shape<256, 256, 2, 4, 2, 64, true, false, 1> X256;
+    typedef Shape<256, 128, 2, 4, 2, 64, true, false, 1> X128;
+    typedef Shape<256, 64, 4, 1, 3, 64, true, false, 1> X64;
+    typedef Shape<256, 16, 4, 1, 3, 64, true, false, 1> X16;
+    typedef Shape<256, 256, 2, 4, 2, 64, true, true, 1> W256;
+    typedef Shape<256, 128, 2, 4, 2, 64, true, true, 1> W128;
+};
+template <> struct Shapes<true> {
+    typedef Shape<256, 128, 4, 2, 2, 32, false, false, 6, true> Z256;
+    typedef Shape<128, 64, 4, 2, 4, 32, false, false, 6, true> Z64;
+    typedef Shape<128, 16, 4, 1, 4, 32, false, false, 6, true> Z16;
+    typedef Shape<256, 128, 4, 2, 2, 32, true, false, 6> X256;
+    typedef Shape<128, 64, 4, 2, 4, 32, true, false, 6> X128;
+    typedef Shape<256, 128, 4, 2, 2, 32, true, true, 6> W256;
+    typedef Shape<128, 64, 4, 2, 4, 32, true, true, 6> W128;
+};
+
+// The rounds of tiles over the CUs that a shape takes, in 5 ns: the small shapes are slower a step, but
+// fewer of the CUs stay without a tile
+template <class S> int64_t rounds(int64_t m, int64_t n) {
+    const int64_t ncu = m2::cu_count();
+    return S::STEP * (((int64_t)tiles(m, S::BM) * tiles(n, S::BN) + ncu - 1) / ncu);
+}
+
+// What both entry points share: how the operands are read
+struct Common {
+    int64_t n, np, dim, hidden, dp, fp;
+    bool f32, pack_x, pack_w;
+    size_t x, w, at;
+};
+// rows: K runs along the rows of both (the gradients) or along dim only
+Common common(int64_t n, int64_t dim, int64_t hidden, int64_t ldx, int64_t ldw, const void* x, const void* w, int dtype,
+              bool rows) {
+    Common c{};
+    c.n = n; c.dim = dim; c.hidden = hidden;
+    c.np = (n + 63) / 64 * 64;
+    c.dp = (dim + 63) / 64 * 64;
+    c.fp = (hidden + 63) / 64 * 64;
+    c.f32 = dtype == M2_F32;
+    // in place: bf16 rows of whole 128-byte pieces, whose offsets within a tile fit 32 bits
+    auto direct = [&](const void* p, int64_t ld, int64_t apart) {
+        return !c.f32 && dim % 64 == 0 && ld % 8 == 0 && al16(p) && ld <= (1 << 22) && ld * (apart + 256) < (1ll << 31);
+    };
+    c.pack_x = !direct(x, ldx, 0);
+    c.pack_w = !direct(w, ldw, hidden) || (rows && hidden % 64);
+    auto take = [&](size_t b) { const size_t r = c.at; c.at += align256(b); return r; };
+    const size_t planes = c.f32 ? 3 : 1;
+    c.x = c.pack_x ? take(2 * planes * (size_t)c.np * c.dp) : c.at;
+    c.w = c.pack_w ? take(2 * planes * (size_t)2 * c.fp * c.dp) : c.at;
+    return c;
+}
+
+template <typename T> Operand operand_x(char* ws, const Common& c, const void* x, int64_t ldx, hipStream_t s) {
+    if (!c.pack_x) return Operand{static_cast<const bf16*>(x), ldx, 0, (int)c.n, (int)c.dim};
+    bf16* to = reinterpret_cast<bf16*>(ws + c.x);
+    const PackArgs a{x, to, c.np, c.dim, ldx, c.dp, c.np * c.dp, 0, c.n};
+    hipLaunchKernelGGL(k_glu_pack<T>, dim3((unsigned)((c.np + 3) / 4)), dim3(256), 0, s, a);
+    return Operand{to, c.dp, c.np * c.dp, (int)c.np, (int)c.dp};
+}
+template <typename T> Operand operand_w(char* ws, const Common& c, const void* w, int64_t ldw, hipStream_t s) {
+    if (!c.pack_w) return Operand{static_cast<const bf16*>(w), ldw, 0, (int)c.hidden, (int)c.dim, (int)c.hidden};
+    bf16* to = reinterpret_cast<bf16*>(ws + c.w);
+    const PackArgs a{w, to, 2 * c.fp, c.dim, ldw, c.dp, 2 * c.fp * c.dp, c.fp, c.hidden};
+    hipLaunchKernelGGL(k_glu_pack<T>, dim3((unsigned)(2 * c.fp / 4)), dim3(256), 0, s, a);
+    return Operand{to, c.dp, 2 * c.fp * c.dp, (int)c.fp, (int)c.dp, (int)c.fp};
+}
+
+int check_sizes(const char* who, int64_t n, int64_t dim, int64_t hidden, int64_t ldx, int64_t ldw, int dtype,
+                int activation) {
+    M2_REQUIRE(n >= 0 && n < (1 << 30) && dim > 0 && dim <= (1 << 20) && hidden > 0 && hidden < (1 << 28), M2_ERR_INVALID,
+               "%s: bad sizes (n %lld, dim %lld, hidden %lld)", who, (long long)n, (long long)dim, (long long)hidden);
+    M2_REQUIRE(ldx >= dim && ldw >= dim, M2_ERR_INVALID, "%s: row strides", who);
+    M2_REQUIRE(dtype == M2_F32 || dtype == M2_BF16, M2_ERR_UNSUPPORTED, "%s: dtype %d", who, dtype);
+    M2_REQUIRE(activation == M2_SILU || activation == M2_GELU, M2_ERR_UNSUPPORTED, "%s: activation %d", who, activation);
+    // (offsets between the halves of a tile's rows; counts of tiles)
+    M2_REQUIRE((hidden + 64) * ((dim + 63) / 64 * 64) < (1ll << 30) &&
+                   (int64_t)tiles(2 * hidden, 128) * tiles(n, 16) < (1ll << 30),
+               M2_ERR_UNSUPPORTED, "%s: too large", who);
+    return M2_OK;
+}
+
+// 16-byte pieces along K that a lane loads by itself
+bool few(const m2_gated_linear_args& a) {
+    const int64_t e = 8, es = a.dtype == M2_F32 ? 4 : 2;
+    return a.n <= 64 && a.dim % e == 0 && a.ldx * es % 16 == 0 && a.ldw * es % 16 == 0 && al16(a.x) && al16(a.weight);
+}
+
+template <typename T> void run_few(const m2_gated_linear_args& a, hipStream_t s) {
+    const FewArgs k{a.x, a.weight, a.out, a.saved, a.ldx, a.ldw, (a.hidden + 63) / 64 * 64,
+                    (int)a.n, (int)a.dim, (int)a.hidden, a.activation == M2_GELU};
+    const unsigned wgs = (unsigned)((a.hidden + 7) / 8);
+    auto go = [&](auto mt) {
+        constexpr int MT = decltype(mt)::value;
+        // enough wavefronts for ~2048 over the chip
+        if (wgs >= 512) hipLaunchKernelGGL((k_glu_few<T, MT, 4>), dim3(wgs), dim3(256), 0, s, k);
+        else hipLaunchKernelGGL((k_glu_few<T, MT, 8>), dim3(wgs), dim3(512), 0, s, k);
+    };
+    if (a.n <= 16) go(std::integral_constant<int, 1>());
+    else if (a.n <= 32) go(std::integral_constant<int, 2>());
+    else go(std::integral_constant<int, 4>());
+}
+
+template <bool F32> int run_fwd(const m2_gated_linear_args& a, const Common& c, hipStream_t s) {
+    typedef typename std::conditional<F32, float, bf16>::type T;
+    typedef Shapes<F32> P;
+    char* ws = static_cast<char*>(a.workspace);
+    Gemm g{};
+    g.n = (int)c.n; g.splits = 1;
+    g.nk = (int)(c.dp / 64);
+    g.b = operand_x<T>(ws, c, a.x, a.ldx, s);
+    g.a = operand_w<T>(ws, c, a.weight, a.ldw, s);
+    const EpiGlu<T> e{static_cast<T*>(a.out), static_cast<T*>(a.saved), c.hidden, c.fp, a.activation == M2_GELU};
+    auto go = [&](auto shape) {
+        typedef decltype(shape) S;
+        g.tm = tiles(2 * ((c.hidden + 15) / 16 * 16), S::BM);
+        g.tn = tiles(c.n, S::BN);
+        launch<S>(g, e, s);
+    };
+    if (c.n <= 16) go(typename P::Z16());
+    else if (c.n <= 64 || rounds<typename P::Z64>(2 * c.hidden, c.n) < rounds<typename P::Z256>(2 * c.hidden, c.n)) go(typename P::Z64());
+    else go(typename P::Z256());
+    return m2::check_launch("gated_linear");
+}
+
+struct BwdPlan {
+    Common c;
+    size_t dz, part, total;
+    int x;                   // dx: 0 the large tiles, 1 the small, 64 / 16 k_ce_stream's
+    int w;                   // dW: the same
+    int splits;
+};
+template <class S> Deal deal_of(int64_t m, int64_t n, int64_t k) {
+    return deal(tiles(m, S::BM) * tiles(n, S::BN), (int)(k / 64), m2::cu_count(), S::STEP, S::SEG);
+}
+template <bool F32> BwdPlan plan_bwd(const m2_gated_linear_grad_args& a) {
+    typedef Shapes<F32> P;
+    BwdPlan p{};
+    p.c = common(a.n, a.dim, a.hidden, a.ldx, a.ldw, a.x, a.weight, a.dtype, true);
+    const Common& c = p.c;
+    size_t at = c.at;
+    auto take = [&](size_t b) { const size_t r = at; at += align256(b); return r; };
+    p.dz = take(2 * (size_t)(F32 ? 3 : 1) * c.np * 2 * c.fp);
+    // (the two products run one after the other and share the parts' buffer)
+    size_t need = 0;
+    auto parts = [&](const Deal& d, size_t tile) {
+        const size_t b = d.s > 1 ? 4 * tile * d.rest * d.s : 0;
+        if (b > need) need = b;
+    };
+    auto choose = [&](auto large, auto small, int64_t m, int64_t n, int64_t k) {
+        typedef decltype(large) A;
+        typedef decltype(small) B;
+        const Deal da = deal_of<A>(m, n, k), db = deal_of<B>(m, n, k);
+        if (da.cost <= db.cost) { parts(da, (size_t)A::BM * A::BN); return 0; }
+        parts(db, (size_t)B::BM * B::BN);
+        return 1;
+    };
+    if (a.grad_x) {
+        if (!F32 && c.n <= 64) {
+            // as many parts of K as fill the CUs; a part costs a float32 array of dx, written and read once
+            p.x = c.n <= 16 ? 16 : 64;
+            const int ncu = m2::cu_count(), steps = (int)(2 * c.fp / 64), t = tiles(c.dim, 256);
+            double best = 1e300;
+            p.splits = 1;
+            for (int s = 1; s <= 64 && s * 4 <= steps; ++s) {
+                const double cost = (double)((t * s + ncu - 1) / ncu) * ((double)steps / s + 12.0) + 0.02 * s * t;
+                if (cost < best) { best = cost; p.splits = s; }
+            }
+            need = 4 * (size_t)p.splits * c.np * c.dp;
+        } else {
+            p.x = choose(typename P::X256(), typename P::X128(), c.dim, c.n, 2 * c.fp);
+        }
+    }
+    if (a.grad_weight) p.w = choose(typename P::W256(), typename P::W128(), c.dim, 2 * c.fp, c.np);
+    p.part = take(need);
+    p.total = at;
+    return p;
+}
+
+template <bool F32> int run_bwd(const m2_gated_linear_grad_args& a, const BwdPlan& p, hipStream_t s) {
+    typedef typename std::conditional<F32, float, bf16>::type T;
+    typedef Shapes<F32> P;
+    char* ws = static_cast<char*>(a.workspace);
+    const Common& c = p.c;
+    bf16* dz = reinterpret_cast<bf16*>(ws + p.dz);
+    float* part = reinterpret_cast<float*>(ws + p.part);
+    const int64_t plane = c.np * 2 * c.fp;
+    const DzArgs d{a.saved, a.grad_out, dz, c.n, c.np, c.hidden, c.fp, a.ldg, plane, a.activation == M2_GELU};
+    hipLaunchKernelGGL(k_glu_dz<T>, dim3((unsigned)((c.np * (c.fp / 8) + 255) / 256)), dim3(256), 0, s, d);
+    auto product = [&](auto shape, Gemm g, int64_t m, int64_t n, int64_t k, const Out<T>& out) {
+        typedef decltype(shape) S;
+        g.tm = tiles(m, S::BM);
+        g.tn = tiles(n, S::BN);
+        g.nk = g.seg_nk = (int)(k / 64);
+        g.splits = m2::cu_count();
+        const Deal dl = deal_of<S>(m, n, k);
+        const EpiOut<T> e{out, part, dl.s > 1 ? dl.full : g.tm * g.tn};
+        launch<S>(g, e, s);
+        if (dl.s > 1) {
+            const JoinArgs j{part, g.tm, g.tn, dl.full, dl.rest, dl.s};
+            const int64_t waves = (int64_t)dl.rest * (S::NW * S::FM / 2 * S::FN);
+            hipLaunchKernelGGL((k_glu_join<T, S>), dim3((unsigned)((waves + 3) / 4)), dim3(256), 0, s, j, out);
+        }
+    };
+    if (a.grad_x) {
+        Gemm g{};
+        g.n = (int)c.n;
+        g.a = operand_w<T>(ws, c, a.weight, a.ldw, s);
+        g.a.lim = g.a.klim;                  // read by columns
+        g.a.klim = (int)(2 * c.fp);
+        g.b = Operand{dz, 2 * c.fp, plane, (int)c.np, (int)(2 * c.fp)};
+        const Out<T> out{static_cast<T*>(a.grad_x), c.dim, 0, (int)c.n};
+        if (p.x > 1) {
+            if constexpr (!F32) {
+                g.tm = tiles(c.dim, 256);
+                g.tn = 1;
+                g.nk = (int)(2 * c.fp / 64);
+                g.splits = p.splits;
+                const EpiSplit e{part, c.np, c.dp};
+                if (p.x == 16) launch<typename P::X16>(g, e, s);
+                else launch<typename P::X64>(g, e, s);
+                hipLaunchKernelGGL(k_glu_sum, dim3((unsigned)((c.dim + 255) / 256), (unsigned)c.n), dim3(64), 0, s, part,
+                                   static_cast<bf16*>(a.grad_x), c.np, c.dp, c.dim, p.splits);
+            }
+        } else if (p.x == 0) {
+            product(typename P::X256(), g, c.dim, c.n, 2 * c.fp, out);
+        } else {
+            product(typename P::X128(), g, c.dim, c.n, 2 * c.fp, out);
+        }
+    }
+    if (a.grad_weight) {
+        Gemm g{};
+        g.n = (int)(2 * c.fp);
+        g.a = operand_x<T>(ws, c, a.x, a.ldx, s);
+        g.a.klim = g.a.lim;                  // read by columns; zero rows of dz stand against the repeated last row
+        g.a.lim = (int)c.dp;
+        g.b = Operand{dz, 2 * c.fp, plane, (int)(2 * c.fp), (int)c.np};
+        const Out<T> out{static_cast<T*>(a.grad_weight), c.dim, (int)c.fp, (int)c.hidden};
+        if (p.w == 0) product(typename P::W256(), g, c.dim, 2 * c.fp, c.np, out);
+        else product(typename P::W128(), g, c.dim, 2 * c.fp, c.np, out);
+    }
+    return m2::check_launch("gated_linear_grad");
+}
+
+}  // namespace
+
+namespace m2 {
+
+size_t gated_linear_saved(const m2_gated_linear_args& a) {
+    if (check_sizes("gated_linear", a.n, a.dim, a.hidden, a.ldx, a.ldw, a.dtype, a.activation)) return 0;
+    const size_t b = m2_dtype_size(a.dtype) * (size_t)a.n * 2 * ((a.hidden + 63) / 64 * 64);
+    return b ? b : 256;
+}
+
+size_t gated_linear_workspace(const m2_gated_linear_args& a) {
+    if (check_sizes("gated_linear", a.n, a.dim, a.hidden, a.ldx, a.ldw, a.dtype, a.activation)) return 0;
+    if (few(a)) return 256;
+    const size_t b = common(a.n, a.dim, a.hidden, a.ldx, a.ldw, a.x, a.weight, a.dtype, false).at;
+    return b ? b : 256;
+}
+
+int launch_gated_linear(const m2_gated_linear_args& a, hipStream_t s) {
+    const char* who = "gated_linear";
+    if (int rc = check_sizes(who, a.n, a.dim, a.hidden, a.ldx, a.ldw, a.dtype, a.activation)) return rc;
+    M2_REQUIRE(a.n == 0 || (a.x && a.weight && a.out), M2_ERR_INVALID, "%s: x, weight and out are required", who);
+    M2_REQUIRE(!a.saved || a.saved_bytes >= gated_linear_saved(a), M2_ERR_WORKSPACE,
+               "%s: saved of %zu bytes needed, %zu given", who, gated_linear_saved(a), a.saved_bytes);
+    if (a.n == 0) return M2_OK;
+    if (few(a)) {
+        if (a.dtype == M2_F32) run_few<float>(a, s);
+        else run_few<bf16>(a, s);
+        return check_launch(who);
+    }
+    const Common c = common(a.n, a.dim, a.hidden, a.ldx, a.ldw, a.x, a.weight, a.dtype, false);
+    M2_REQUIRE(c.at == 0 || (a.workspace && a.workspace_bytes >= c.at), M2_ERR_WORKSPACE,
+               "%s: workspace of %zu bytes needed, %zu given", who, c.at, a.workspace_bytes);
+    return c.f32 ? run_fwd<true>(a, c, s) : run_fwd<false>(a, c, s);
+}
+
+static BwdPlan plan(const m2_gated_linear_grad_args& a) {
+    return a.dtype == M2_F32 ? plan_bwd<true>(a) : plan_bwd<false>(a);
+}
+
+size_t gated_linear_grad_workspace(const m2_gated_linear_grad_args& a) {
+    if (check_sizes("gated_linear_grad", a.n, a.dim, a.hidden, a.ldx, a.ldw, a.dtype, a.activation)) return 0;
+    const size_t b = plan(a).total;
+    return b ? b : 256;
+}
+
+int launch_gated_linear_grad(const m2_gated_linear_grad_args& a, hipStream_t s) {
+    const char* who = "gated_linear_grad";
+    if (int rc = check_sizes(who, a.n, a.dim, a.hidden, a.ldx, a.ldw, a.dtype, a.activation)) return rc;
+    M2_REQUIRE(a.n > 0, M2_ERR_INVALID, "%s: no tokens", who);
+    M2_REQUIRE(a.ldg >= a.hidden, M2_ERR_INVALID, "%s: row strides", who);
+    M2_REQUIRE(a.x && a.weight && a.saved && a.grad_out && (a.grad_x || a.grad_weight), M2_ERR_INVALID,
+               "%s: x, weight, saved, grad_out and an output are required", who);
+    const BwdPlan p = plan(a);
+    M2_REQUIRE(a.workspace && a.workspace_bytes >= p.total, M2_ERR_WORKSPACE,
+               "%s: workspace of %zu bytes needed, %zu given", who, p.total, a.workspace_bytes);
+    return a.dtype == M2_F32 ? run_bwd<true>(a, p, s) : run_bwd<false>(a, p, s);
+}
+
+}  // namespace m2

@@ -103,45 +103,6 @@ __global__ void __launch_bounds__(1024) k_ce_compact(const void* targets, int64_
     if (t < 2) tk.count[t] = t == 0 ? base : 0;
 }
 
-// 8 consecutive elements of a row, zero past its end
-template <typename T> M2_DEV void load8(const T* row, int64_t c, int64_t dim, float (&v)[8]) {
-    if (c + 8 <= dim) {
-        if constexpr (sizeof(T) == 2) {
-            const u32x4 r = load16(row + c);
-#pragma unroll
-            for (int i = 0; i < 4; ++i) { v[2 * i] = bf16_lo(r[i]); v[2 * i + 1] = bf16_hi(r[i]); }
-        } else {
-            const u32x4 a = load16(row + c), b = load16(row + c + 4);
-#pragma unroll
-            for (int i = 0; i < 4; ++i) { v[i] = __uint_as_float(a[i]); v[4 + i] = __uint_as_float(b[i]); }
-        }
-    } else {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = c + i < dim ? to_f32(row[c + i]) : 0.f;
-    }
-}
-// v = h + m + l, each bf16 (an infinity or NaN stays in h alone)
-M2_DEV void split3(float v, float& h, float& m, float& l) {
-    h = (float)(bf16)v;
-    const float r = v - h;
-    const bool fin = fabsf(h) < __builtin_inff();
-    m = fin ? (float)(bf16)r : 0.f;
-    l = fin ? r - m : 0.f;
-}
-template <bool PLANES> M2_DEV void store8(bf16* p, int64_t plane, const float (&v)[8]) {
-    if constexpr (!PLANES) {
-        const u32x4 r = {pk_bf16(v[0], v[1]), pk_bf16(v[2], v[3]), pk_bf16(v[4], v[5]), pk_bf16(v[6], v[7])};
-        *reinterpret_cast<u32x4*>(p) = r;
-    } else {
-        float h[8], m[8], l[8];
-#pragma unroll
-        for (int i = 0; i < 8; ++i) split3(v[i], h[i], m[i], l[i]);
-        store8<false>(p, 0, h);
-        store8<false>(p + plane, 0, m);
-        store8<false>(p + 2 * plane, 0, l);
-    }
-}
-
 struct PackArgs {
     const void* src;
     bf16* dst;
@@ -341,54 +302,6 @@ struct EpiLse {
         }
     }
 };
-
-// Two fragments of 16 m beside each other, x and y: lane rows (16 lanes) 0 and 2 exchange
-// theirs of y for rows 1's and 3's of x, after which a lane holds 8 consecutive m from
-// pair_m on: (p, q)
-M2_DEV void pair_swap(uint32_t& p, uint32_t& q) {
-    const auto r = __builtin_amdgcn_permlane16_swap(p, q, false, false);
-    p = r[0];
-    q = r[1];
-}
-M2_DEV int pair_m(int lane) { return 16 * ((lane >> 4) & 1) + 8 * (lane >> 5); }
-M2_DEV void store_pair(bf16* d, const float (&x)[4], const float (&y)[4]) {
-    uint32_t a0 = pk_bf16(x[0], x[1]), a1 = pk_bf16(x[2], x[3]);
-    uint32_t b0 = pk_bf16(y[0], y[1]), b1 = pk_bf16(y[2], y[3]);
-    pair_swap(a0, b0);
-    pair_swap(a1, b1);
-    *reinterpret_cast<u32x4*>(d) = u32x4{a0, a1, b0, b1};
-}
-// the 32 values of m from m0 on (two fragments) of one n into a row of dim elements
-template <typename T>
-M2_DEV void store_row(T* row, int m0, int64_t dim, int lane, const f32x4& x, const f32x4& y) {
-    if constexpr (sizeof(T) == 2) {
-        // (the exchange is among the lanes of this n: all of them are here)
-        uint32_t p[4] = {pk_bf16(x[0], x[1]), pk_bf16(x[2], x[3]), pk_bf16(y[0], y[1]), pk_bf16(y[2], y[3])};
-        pair_swap(p[0], p[2]);
-        pair_swap(p[1], p[3]);
-        const int m = m0 + pair_m(lane);
-        if (m + 8 <= dim) {
-            store16(row + m, u32x4{p[0], p[1], p[2], p[3]});
-        } else {
-#pragma unroll
-            for (int r = 0; r < 8; ++r)
-                if (m + r < dim) reinterpret_cast<uint16_t*>(row)[m + r] = (uint16_t)(p[r >> 1] >> (16 * (r & 1)));
-        }
-    } else {
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-            const int m = m0 + 16 * e + 4 * (lane >> 4);
-            const f32x4& v = e ? y : x;
-            if (m + 4 <= dim) {
-                store16(row + m, __builtin_bit_cast(u32x4, v));
-            } else {
-#pragma unroll
-                for (int r = 0; r < 4; ++r)
-                    if (m + r < dim) row[m + r] = v[r];
-            }
-        }
-    }
-}
 
 // The upstream gradient of the kept tokens' losses.
 struct Up {
@@ -934,22 +847,6 @@ template <typename T, class S> __global__ void __launch_bounds__(256) k_ce_dx_se
 // ---------------------------------------------------------------------------
 // plans
 // ---------------------------------------------------------------------------
-size_t align256(size_t v) { return (v + 255) & ~size_t(255); }
-bool al16(const void* p) { return ((uintptr_t)p & 15) == 0; }
-
-template <class S, class EPI> void launch(const Gemm& g, const EPI& e, hipStream_t s) {
-    const int64_t tiles = (int64_t)g.tm * g.tn;
-    if constexpr (S::TERMS == 1 && S::BN < 128) {
-        hipLaunchKernelGGL((k_ce_stream<S, EPI>), dim3((unsigned)(tiles * g.splits)), dim3(S::NT), 0, s, g, e);
-    } else {
-        const int64_t ncu = m2::cu_count();
-        const unsigned nwg = (unsigned)(EPI::SEG ? g.splits : tiles < ncu ? tiles : ncu);
-        if constexpr (S::TERMS == 1) hipLaunchKernelGGL((k_ce_tile<S, EPI>), dim3(nwg), dim3(S::NT), 0, s, g, e);
-        else hipLaunchKernelGGL((k_ce_planes<S, EPI>), dim3(nwg), dim3(S::NT), 0, s, g, e);
-    }
-}
-inline int tiles(int64_t n, int t) { return (int)((n + t - 1) / t); }
-
 // Tiles of the logits (Z), of dx (X) and of dw (W); the number is a tile's n
 template <bool F32> struct Shapes {
     typedef Shape<256, 256, 2, 4, 2, 64, false, false, 1> Z256;

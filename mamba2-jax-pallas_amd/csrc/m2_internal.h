@@ -69,6 +69,13 @@ int launch_gated_recurrence_grad(const m2_gated_recurrence_grad_args& a, hipStre
 size_t gated_recurrence_grad_workspace(const m2_gated_recurrence_grad_args& a);
 int launch_gated_recurrence_update(const m2_gated_recurrence_update_args& a, hipStream_t stream);
 
+// the gated feed-forward product (gated_linear.hip)
+int launch_gated_linear(const m2_gated_linear_args& a, hipStream_t stream);
+size_t gated_linear_saved(const m2_gated_linear_args& a);
+size_t gated_linear_workspace(const m2_gated_linear_args& a);
+int launch_gated_linear_grad(const m2_gated_linear_grad_args& a, hipStream_t stream);
+size_t gated_linear_grad_workspace(const m2_gated_linear_grad_args& a);
+
 // chunk_state_varlen for bf16, head dim 64, dstate % 64 == 0, chunk_size % 32
 // == 0 (<= 256): one workgroup per (sequence, head, 64-column dstate block)
 bool varlen_states_fast_supported(const m2_chunk_state_varlen_args& a);

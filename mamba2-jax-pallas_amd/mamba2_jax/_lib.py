@@ -212,6 +212,20 @@ class GatedRecurrenceUpdateArgs(ctypes.Structure):
                 ("dtype", _i32)]
 
 
+class GatedLinearArgs(ctypes.Structure):
+    _fields_ = [("x", _c_p), ("weight", _c_p), ("out", _c_p), ("n", _i64), ("dim", _i64),
+                ("hidden", _i64), ("ldx", _i64), ("ldw", _i64), ("dtype", _i32),
+                ("activation", _i32), ("workspace", _c_p), ("workspace_bytes", ctypes.c_size_t),
+                ("saved", _c_p), ("saved_bytes", ctypes.c_size_t)]
+
+
+class GatedLinearGradArgs(ctypes.Structure):
+    _fields_ = [("x", _c_p), ("weight", _c_p), ("saved", _c_p), ("grad_out", _c_p),
+                ("grad_x", _c_p), ("grad_weight", _c_p), ("n", _i64), ("dim", _i64),
+                ("hidden", _i64), ("ldx", _i64), ("ldw", _i64), ("ldg", _i64), ("dtype", _i32),
+                ("activation", _i32), ("workspace", _c_p), ("workspace_bytes", ctypes.c_size_t)]
+
+
 # entry point name -> argument struct (every function declared in m2ssd.h)
 ENTRY_POINTS = {
     "m2_chunk_cumsum": ChunkCumsumArgs,
@@ -236,6 +250,8 @@ ENTRY_POINTS = {
     "m2_gated_recurrence": GatedRecurrenceArgs,
     "m2_gated_recurrence_grad": GatedRecurrenceGradArgs,
     "m2_gated_recurrence_update": GatedRecurrenceUpdateArgs,
+    "m2_gated_linear": GatedLinearArgs,
+    "m2_gated_linear_grad": GatedLinearGradArgs,
 }
 # workspace size functions of the entry points that take a workspace besides the
 # combined forward: name -> argument struct
@@ -246,7 +262,12 @@ WORKSPACE_SIZES = {
     "m2_linear_cross_entropy_grad_workspace_size": LinearCrossEntropyGradArgs,
     "m2_clip_grad_norm_workspace_size": ClipGradNormArgs,
     "m2_gated_recurrence_grad_workspace_size": GatedRecurrenceGradArgs,
+    "m2_gated_linear_saved_size": GatedLinearArgs,
+    "m2_gated_linear_workspace_size": GatedLinearArgs,
+    "m2_gated_linear_grad_workspace_size": GatedLinearGradArgs,
 }
+# activations of the gated feed-forward product (M2_SILU, M2_GELU)
+ACTIVATIONS = {"silu": 0, "gelu": 1}
 # positions between two of the states that the recurrence leaves its gradient (M2_RECURRENCE_SPAN)
 RECURRENCE_SPAN = 64
 OTHER_SYMBOLS = ("m2_ssd_combined_workspace_size", "m2_ssd_combined_plan", "m2_last_error", "m2_abi_version",

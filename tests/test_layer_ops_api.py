@@ -14,7 +14,8 @@ from mamba2_jax import ops
 HEADER = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "include", "m2ssd.h")
 STRUCTS = {"GatedRecurrenceArgs": "m2_gated_recurrence_args",
            "GatedRecurrenceGradArgs": "m2_gated_recurrence_grad_args",
-           "GatedRecurrenceUpdateArgs": "m2_gated_recurrence_update_args"}
+           "GatedRecurrenceUpdateArgs": "m2_gated_recurrence_update_args",
+           "GatedLinearArgs": "m2_gated_linear_args", "GatedLinearGradArgs": "m2_gated_linear_grad_args"}
 
 
 def test_struct_layout_matches_header(tmp_path):
@@ -83,6 +84,58 @@ def test_gated_recurrence_update_refusals():
     for p in ("x", "r", "i", "A", "state", "new_state", "out"):
         refused(name, mk(**{p: None}), -1, "required")
     assert L.load_library().m2_gated_recurrence_update(ctypes.byref(mk(batch=0, x=None)), None) == 0
+
+
+def test_gated_linear_refusals():
+    ok = dict(x=4096, weight=4096, out=4096, n=100, dim=60, hidden=30, ldx=60, ldw=60, dtype=L.M2_BF16,
+              activation=L.ACTIVATIONS["silu"])
+    mk = lambda **k: L.GatedLinearArgs(**{**ok, **k})
+    lib = L.load_library()
+    name = "m2_gated_linear"
+    need = lib.m2_gated_linear_workspace_size(ctypes.byref(mk()))
+    saved = lib.m2_gated_linear_saved_size(ctypes.byref(mk()))
+    assert need > 0 and saved == 100 * 2 * 64 * 2
+    far = dict(ldx=1 << 22, ldw=1 << 22)
+    for bad in (dict(n=-1), dict(n=1 << 30), dict(dim=0), dict(dim=1 << 21), dict(hidden=0), dict(hidden=1 << 28)):
+        assert lib.m2_gated_linear_workspace_size(ctypes.byref(mk(**{**far, **bad}))) == 0
+        assert lib.m2_gated_linear_saved_size(ctypes.byref(mk(**{**far, **bad}))) == 0
+        refused(name, mk(**{**far, **bad}), -1, "bad sizes")
+    refused(name, mk(ldx=59), -1, "row strides")
+    refused(name, mk(ldw=59), -1, "row strides")
+    refused(name, mk(dtype=L.M2_I64), -2, "dtype")
+    refused(name, mk(activation=2), -2, "activation")
+    refused(name, mk(dim=1 << 16, ldx=1 << 16, ldw=1 << 16, hidden=1 << 14), -2, "too large")
+    for p in ("x", "weight", "out"):
+        refused(name, mk(**{p: None}), -1, "required")
+    refused(name, mk(workspace=4096, workspace_bytes=need - 1), -4, "workspace")
+    refused(name, mk(workspace_bytes=need), -4, "workspace")
+    refused(name, mk(workspace=4096, workspace_bytes=need, saved=4096, saved_bytes=saved - 1), -4, "saved")
+    assert lib.m2_gated_linear(ctypes.byref(mk(n=0, x=None)), None) == 0
+    okg = {k: v for k, v in ok.items() if k != "out"} | dict(saved=4096, grad_out=4096, grad_x=4096, grad_weight=4096,
+                                                            ldg=30)
+    mg = lambda **k: L.GatedLinearGradArgs(**{**okg, **k})
+    name = "m2_gated_linear_grad"
+    need = lib.m2_gated_linear_grad_workspace_size(ctypes.byref(mg()))
+    assert need > 0
+    refused(name, mg(n=0), -1, "no tokens")
+    refused(name, mg(ldg=29), -1, "row strides")
+    for p in ("x", "weight", "saved", "grad_out"):
+        refused(name, mg(**{p: None}), -1, "required")
+    refused(name, mg(grad_x=None, grad_weight=None), -1, "required")
+    refused(name, mg(workspace=4096, workspace_bytes=need - 1), -4, "workspace")
+
+
+def test_gated_linear_shape_refusals():
+    x, w = _fake(3, 8), _fake(12, 8)
+    for args in ((x[0, 0], w), (x, w[0]), (x, w[:, :7]), (x, w[:11]), (x, w[:0]), (x[:, :0], w[:, :0]), (x, w, "relu")):
+        with pytest.raises(L.M2ShapeError):
+            ops.gated_linear(*args)
+    with pytest.raises(TypeError):
+        ops.gated_linear(x.bfloat16(), w)
+    with pytest.raises(TypeError):
+        ops.gated_linear(x.half(), w.half())
+    with pytest.raises(ValueError):
+        ops.gated_linear(torch.zeros(3, 8), torch.zeros(12, 8))
 
 
 def test_python_refuses_cpu_tensors():

@@ -573,12 +573,13 @@ int m2_clip_grad_norm(const m2_clip_grad_norm_args* a, void* stream);
  * one before it; a position with a negative entry is padding: out is 0 there, the state passes it
  * unchanged, and what x, r and i hold there (they must be readable) reaches nothing.
  * final_states is the state behind the last position.  x, r and i are addressed through their strides of
- * batch and time (elements; channels are contiguous), e.g. as slices of one projection's output.
+ * batch and time (elements; channels are contiguous; of time 0, or dim to 2^20), e.g. as slices of one
+ * projection's output.  dim <= 2^20.
  * span_states (or NULL) takes the states that enter every M2_RECURRENCE_SPAN positions, which
  * the gradient reads.
  * No counterpart in the reference, whose only recurrence is the SSD's (ops/ssd_naive.py:220-322).
  * ------------------------------------------------------------------------- */
-#define M2_RECURRENCE_SPAN 64
+#define M2_RECURRENCE_SPAN 32
 typedef struct {
     const void*    x;              /* [b, L, d] at the strides below, dtype     */
     const void*    r;              /* the same: the decay's gate                */
@@ -592,7 +593,10 @@ typedef struct {
     int64_t batch, seqlen, dim;
     int64_t x_stride_batch, x_stride_time, r_stride_batch, r_stride_time, i_stride_batch, i_stride_time;
     int32_t dtype;
+    void*   workspace;
+    size_t  workspace_bytes;
 } m2_gated_recurrence_args;
+size_t m2_gated_recurrence_workspace_size(const m2_gated_recurrence_args* a);
 int m2_gated_recurrence(const m2_gated_recurrence_args* a, void* stream);
 
 /* ---------------------------------------------------------------------------

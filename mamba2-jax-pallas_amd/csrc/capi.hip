@@ -106,6 +106,9 @@ extern "C" size_t m2_linear_cross_entropy_grad_workspace_size(
 extern "C" size_t m2_clip_grad_norm_workspace_size(const m2_clip_grad_norm_args* a) {
     return a ? m2::clip_grad_norm_workspace(*a) : 0;
 }
+extern "C" size_t m2_gated_recurrence_workspace_size(const m2_gated_recurrence_args* a) {
+    return a ? m2::gated_recurrence_workspace(*a) : 0;
+}
 extern "C" size_t m2_gated_recurrence_grad_workspace_size(const m2_gated_recurrence_grad_args* a) {
     return a ? m2::gated_recurrence_grad_workspace(*a) : 0;
 }

@@ -12,7 +12,7 @@
 // consecutive steps of V channels; a run of steps is an affine map h -> P h + H, and the maps of the
 // threads of a wavefront (by lane shifts) and then of the wavefronts (by LDS, one barrier a tile)
 // are joined to the state that each thread's run begins with.  The forward leaves the state
-// that enters every span of 64 steps (float32, 1/64 of a stream); the backward goes through
+// that enters every span of 32 steps (float32, a sixteenth of a bf16 stream); the backward goes through
 // the tiles from the last to the first, computes the states of a tile again from there and both joins at
 // once (a run's map backward, m -> P m + M, has the same P).
 //
@@ -23,6 +23,8 @@
 // Where seq_idx changes the state is cleared: P = -1 marks a run that holds such a step, so that what
 // came before (a NaN, say) is selected away and not multiplied by zero.  Negative seq_idx is
 // padding: a = 1, nothing added, 0 stored; so are the steps past the end of the row.
+#include <type_traits>
+
 #include "m2_internal.h"
 
 namespace {
@@ -30,62 +32,93 @@ namespace {
 constexpr float LOG2E = 1.4426950408889634f;
 constexpr int SPAN = M2_RECURRENCE_SPAN;
 
-// V consecutive channels of a row, as loaded; rows need be aligned as their elements only
-template <typename T, int V> struct Raw;
-template <> struct Raw<bf16, 4> {
-    typedef uint32_t any __attribute__((ext_vector_type(2), aligned(2)));
-    any v;
-    M2_DEV void load(const bf16* p) { v = *reinterpret_cast<const any*>(p); }
-    M2_DEV float get(int i) const { return i & 1 ? bf16_hi(v[i >> 1]) : bf16_lo(v[i >> 1]); }
-    static M2_DEV void store(bf16* p, const float (&f)[4]) {
-        *reinterpret_cast<any*>(p) = any{pk_bf16(f[0], f[1]), pk_bf16(f[2], f[3])};
-    }
-};
-template <> struct Raw<float, 4> {
-    typedef uint32_t any __attribute__((ext_vector_type(4), aligned(4)));
-    any v;
-    M2_DEV void load(const float* p) { v = *reinterpret_cast<const any*>(p); }
-    M2_DEV float get(int i) const { return __uint_as_float(v[i]); }
-    static M2_DEV void store(float* p, const float (&f)[4]) {
-        *reinterpret_cast<any*>(p) = any{__float_as_uint(f[0]), __float_as_uint(f[1]), __float_as_uint(f[2]),
-                                         __float_as_uint(f[3])};
-    }
-};
-template <typename T> struct Raw<T, 1> {
-    T v;
-    M2_DEV void load(const T* p) { v = *p; }
-    M2_DEV float get(int) const { return to_f32(v); }
-    static M2_DEV void store(T* p, const float (&f)[1]) { *p = from_f32<T>(f[0]); }
-};
-// the values from `skip` on
-template <typename T, int V> M2_DEV void put(T* p, const float (&f)[V], int skip) {
-    if (skip == 0) {
-        Raw<T, V>::store(p, f);
-    } else {
-#pragma unroll
-        for (int v = 1; v < V; ++v)
-            if (v >= skip) p[v] = from_f32<T>(f[v]);
-    }
-}
+// Buffer accesses: a scalar descriptor of what may be touched (from a base on, so many bytes), a 32-bit
+// offset of the lane, one of the wavefront.  A step's address takes no vector instruction, and
+// what lies past the end reads 0 and is not stored.  Addresses need be aligned as elements only.
+typedef __amdgpu_buffer_rsrc_t Rsrc;
+M2_DEV Rsrc rsrc(const void* p, uint32_t bytes) { return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(p), 0, bytes, 0x00027000); }
+constexpr uint32_t NOWHERE = 0xfffffff0u;      // an offset past every end
 
-M2_DEV float sigmoid(float v) { return __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(v * -LOG2E)); }
-// 1 - sigmoid(v), which keeps its bits where the sigmoid is near 1
-M2_DEV float co_sigmoid(float v, float s) { return v > 0.f ? s * __builtin_amdgcn_exp2f(v * -LOG2E) : 1.f - s; }
-// 1 - exp(L): the series to L^7 / 7! (its rest is below 2^-25 of it) where 1 - exp would cancel
-M2_DEV float decay(float L) {
-    float p = fmaf(L, 1.f / 7, 1.f);
-    p = fmaf(L * p, 1.f / 6, 1.f);
-    p = fmaf(L * p, 1.f / 5, 1.f);
-    p = fmaf(L * p, 1.f / 4, 1.f);
-    p = fmaf(L * p, 1.f / 3, 1.f);
-    p = fmaf(L * p, 1.f / 2, 1.f);
-    return L < -0.35f ? 1.f - __builtin_amdgcn_exp2f(L * LOG2E) : -L * p;
+// V consecutive channels of a row, as loaded
+template <typename T, int V> struct Raw;
+template <> struct Raw<bf16, 2> {
+    uint32_t v;
+    M2_DEV void load(Rsrc r, uint32_t off, uint32_t soff) { v = __builtin_amdgcn_raw_buffer_load_b32(r, off, soff, 0); }
+    M2_DEV void fill(float f) { v = pk_bf16(f, f); }
+    M2_DEV float get(int i) const { return i ? bf16_hi(v) : bf16_lo(v); }
+    template <int AUX> static M2_DEV void store(Rsrc r, uint32_t off, uint32_t soff, const float (&f)[2]) {
+        __builtin_amdgcn_raw_buffer_store_b32(pk_bf16(f[0], f[1]), r, off, soff, AUX);
+    }
+};
+template <> struct Raw<float, 2> {
+    typedef uint32_t pair __attribute__((ext_vector_type(2)));
+    pair v;
+    M2_DEV void load(Rsrc r, uint32_t off, uint32_t soff) { v = __builtin_amdgcn_raw_buffer_load_b64(r, off, soff, 0); }
+    M2_DEV void fill(float f) { v[0] = v[1] = __float_as_uint(f); }
+    M2_DEV float get(int i) const { return __uint_as_float(v[i]); }
+    template <int AUX> static M2_DEV void store(Rsrc r, uint32_t off, uint32_t soff, const float (&f)[2]) {
+        __builtin_amdgcn_raw_buffer_store_b64(pair{__float_as_uint(f[0]), __float_as_uint(f[1])}, r, off, soff, AUX);
+    }
+};
+template <> struct Raw<bf16, 1> {
+    uint32_t v;
+    M2_DEV void load(Rsrc r, uint32_t off, uint32_t soff) {
+        v = (uint32_t)(uint16_t)__builtin_amdgcn_raw_buffer_load_b16(r, off, soff, 0) << 16;
+    }
+    M2_DEV void fill(float f) { v = __float_as_uint(f); }
+    M2_DEV float get(int) const { return __uint_as_float(v); }
+    template <int AUX> static M2_DEV void store(Rsrc r, uint32_t off, uint32_t soff, const float (&f)[1]) {
+        __builtin_amdgcn_raw_buffer_store_b16((uint16_t)pk_bf16(f[0], f[0]), r, off, soff, AUX);
+    }
+};
+template <> struct Raw<float, 1> {
+    uint32_t v;
+    M2_DEV void load(Rsrc r, uint32_t off, uint32_t soff) { v = __builtin_amdgcn_raw_buffer_load_b32(r, off, soff, 0); }
+    M2_DEV void fill(float f) { v = __float_as_uint(f); }
+    M2_DEV float get(int) const { return __uint_as_float(v); }
+    template <int AUX> static M2_DEV void store(Rsrc r, uint32_t off, uint32_t soff, const float (&f)[1]) {
+        __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(f[0]), r, off, soff, AUX);
+    }
+};
+
+constexpr float INF = __builtin_inff();
+
+// exp(-v), sigmoid(v) from it, and 1 - sigmoid(v), which keeps its bits where the sigmoid is near 1
+M2_DEV float exp_neg(float v) { return __builtin_amdgcn_exp2f(v * -LOG2E); }
+M2_DEV float sigmoid_of(float e) { return __builtin_amdgcn_rcpf(1.f + e); }
+M2_DEV float co_sigmoid(float e, float s) { return e <= 1.f ? e * s : 1.f - s; }
+// 1 - exp(L) for L <= 0: the series to L^8 / 8! where 1 - exp would cancel (from NEAR on its rest is below
+// 2^-26 of it), the exponential below
+constexpr float NEAR = -0.5f;
+M2_DEV float decay_near(float L) {
+    float p = 1.f / 40320;
+    p = fmaf(p, L, 1.f / 5040);
+    p = fmaf(p, L, 1.f / 720);
+    p = fmaf(p, L, 1.f / 120);
+    p = fmaf(p, L, 1.f / 24);
+    p = fmaf(p, L, 1.f / 6);
+    p = fmaf(p, L, 1.f / 2);
+    p = fmaf(p, L, 1.f);
+    return p * -L;
 }
-// a p + b.  (The product's operand is bounded: an infinite p stays what it is and is not inf - inf.)
-M2_DEV float step(float alpha, float p, float b) {
+M2_DEV float decay(float L, float near) { return L < NEAR ? 1.f - __builtin_amdgcn_exp2f(L * LOG2E) : near; }
+// far: some channel of the wavefront may have an L below NEAR
+template <int TS, int V> M2_DEV void decay_far(float (&al)[TS][V], const float (&L)[TS][V], bool far) {
+    if (!far) return;
+    asm volatile("");        // (a branch, not selects: the exponentials cost the others an eighth of their time)
+#pragma unroll
+    for (int j = 0; j < TS; ++j)
+#pragma unroll
+        for (int v = 0; v < V; ++v) al[j][v] = decay(L[j][v], al[j][v]);
+}
+// alpha p, of an infinite p the largest number (p - alpha p is then p, not inf - inf)
+M2_DEV float bounded(float p) {
     constexpr float MAX = 3.402823466e38f;
-    return fmaf(-alpha, __builtin_amdgcn_fmed3f(p, -MAX, MAX), p + b);
+    return __builtin_amdgcn_fmed3f(p, -MAX, MAX);
 }
+// a p + b
+M2_DEV float step(float alpha, float p, float b) { return fmaf(-alpha, bounded(p), p + b); }
+M2_DEV float step(float alpha, float p) { return fmaf(-alpha, bounded(p), p); }
 // 1 / sqrt(1 - a^2), 0 where a is 1 (below 1e-37 the hardware's root has no argument left)
 M2_DEV float inv_beta(float alpha, float& y) {
     y = alpha * (2.f - alpha);
@@ -112,8 +145,10 @@ struct RecArgs {
     const int32_t* seq;
     int64_t xb, xt, rb, rt, ib, it;      // strides of batch and time
     float* ck;                           // [batch][spans][dim]
+    float2* agg;                         // [batch][segments][dim]: (P, H) of each, or (P, M) back
     int64_t L, spans;
-    int dim, slabs;
+    int dim, slabs, segments;
+    int64_t seg;                         // steps of a segment: whole tiles
     // forward
     void* out;
     float* last;
@@ -122,333 +157,546 @@ struct RecArgs {
     int64_t gb, gt;
     const float* glast;
     void *dx, *dr, *di;
-    float* dA;                           // [batch][dim]
+    float* dA;                           // [batch][segments][dim]
     float* dh0;
 };
 
 // Which channels and steps of a tile a thread has
 template <int V, int LC, int TS, int W> struct Place {
     static constexpr int G = 64 / LC, TILE = G * W * TS, C = V * LC;
-    int b, c, col, tg, w, step;          // col: place in the slab
-    int skip;                            // the lane's first channels that another one stores
+    int b, segment, c, col, tg, w, step, lane;       // col: place in the slab
+    int64_t t0, end;                     // of the segment
+    // A lane that would reach past the last channel has the last V, and stores of them those that no other lane
+    // has: all (whole), the second alone (half, of an odd number of channels), none
+    bool whole, half;
     M2_DEV Place(const RecArgs& a) {
-        const int lane = threadIdx.x & 63;
+        lane = threadIdx.x & 63;
         const int id = xcd_remap(blockIdx.x, gridDim.x);
-        b = id / a.slabs;
+        const int of = __builtin_amdgcn_readfirstlane(id / a.slabs);
+        b = __builtin_amdgcn_readfirstlane(of / a.segments);
+        segment = of - b * a.segments;
+        t0 = segment * a.seg;
+        end = min(t0 + a.seg, a.L);
         w = wave_id();
         col = (lane % LC) * V;
         tg = lane / LC;
-        // (a lane that reaches past the last channel has the last V, and those past it V that others store)
-        const int from = (id - b * a.slabs) * C + col;
+        const int from = (id - of * a.slabs) * C + col;
         c = min(from, a.dim - V);
-        skip = from - c;
+        whole = from == c;
+        half = V == 2 && from == c + 1;
         step = (w * G + tg) * TS;
+    }
+    template <typename E, int N> M2_DEV void put(E* p, const E (&f)[N]) const {
+#pragma unroll
+        for (int v = 0; v < N; ++v)
+            if (whole || (half && v == N - 1)) p[v] = f[v];
+    }
+    M2_DEV int64_t agg(const RecArgs& a, int s) const { return ((int64_t)b * a.segments + s) * a.dim + c; }
+};
+
+// The tile of one input or output that the walk is at
+template <typename T, int V> struct Stream {
+    const char* base;        // of the tile's first step
+    uint32_t st, row;        // bytes between steps, of a row
+    uint32_t off;            // of the lane's first step
+    template <class P> M2_DEV Stream(const void* p, int64_t offset, int64_t stride, const RecArgs& a, const P& at)
+        : base(static_cast<const char*>(p) + offset * (int64_t)sizeof(T)), st((uint32_t)(stride * sizeof(T))),
+          row(a.dim * (uint32_t)sizeof(T)), off(at.step * st + at.c * (uint32_t)sizeof(T)) {}
+    M2_DEV void move(int64_t steps) { base += steps * st; }
+    // last: the row's last step, counted from the tile's first
+    M2_DEV Rsrc tile(int last) const { return rsrc(base, last * st + row); }
+    template <int TS> M2_DEV void load(Raw<T, V> (&r)[TS], int last) const {
+        const Rsrc t = tile(last);
+#pragma unroll
+        for (int j = 0; j < TS; ++j) r[j].load(t, off, j * st);
+    }
+};
+// NT: non-temporal stores
+template <typename T, int V, bool NT> struct Output : Stream<T, V> {
+    static constexpr int AUX = NT ? 2 : 0;
+    uint32_t whole, half;    // where this lane stores all of its channels, or the last alone
+    bool odd;
+    template <class P> M2_DEV Output(const void* p, int64_t offset, const RecArgs& a, const P& at)
+        : Stream<T, V>(p, offset, a.dim, a, at), whole(at.whole ? this->off : NOWHERE),
+          half(at.half ? this->off + (uint32_t)sizeof(T) : NOWHERE), odd(V == 2 && (a.dim & 1)) {}
+    M2_DEV void store(Rsrc t, int j, const float (&f)[V]) const {
+        Raw<T, V>::template store<AUX>(t, whole, j * this->st, f);
+        if (odd) {
+            const float one[1] = {f[V - 1]};
+            Raw<T, 1>::template store<AUX>(t, half, j * this->st, one);
+        }
     }
 };
 
 // The steps of a tile that a thread has: bit j of live: inside the row and no padding; of clear: the
-// state is cleared before it
-template <int TS, bool SEQ> struct Steps {
-    int sq[SEQ ? TS + 1 : 1];
+// state is cleared before it.  Lane l holds seq_idx of the wavefront's step l - 1 (one load for all its
+// steps); ballots make the bits of them.
+template <int TS, int G, bool SEQ> struct Steps {
+    static constexpr int N = G * TS;     // of a wavefront
+    static_assert(!SEQ || N < 16, "a row of lanes");
+    int sq;
     uint32_t live, clear;
-    M2_DEV void load(const int32_t* row, int64_t t, int64_t L) {
+    // row: of the tile's first step; begins: that is the row's first
+    template <class P> M2_DEV void load(const int32_t* row, bool begins, const P& at, int last) {
         if constexpr (SEQ) {
-#pragma unroll
-            for (int j = 0; j <= TS; ++j) {
-                const int64_t at = t + j - 1;
-                sq[j] = row[at < 0 ? 0 : at < L ? at : L - 1];
-            }
+            const int more = begins ? 0 : 1;                 // the step before the tile is read too
+            const Rsrc t = rsrc(row - more, 4 * (last + 1 + more));
+            sq = __builtin_amdgcn_raw_buffer_load_b32(t, 4 * max(at.w * N + min(at.lane, N) - 1 + more, 0), 0, 0);
         }
     }
-    M2_DEV void set(int64_t t, int64_t L) {
-        live = clear = 0;
-#pragma unroll
-        for (int j = 0; j < TS; ++j) {
-            const bool in = t + j < L;
-            if constexpr (SEQ) {
-                live |= (uint32_t)(in && sq[j + 1] >= 0) << j;
-                clear |= (uint32_t)(in && sq[j + 1] >= 0 && sq[j + 1] != sq[j]) << j;
-            } else {
-                live |= (uint32_t)in << j;
-            }
+    // -> whether all steps of the wavefront are live
+    template <class P> M2_DEV bool set(bool begins, const P& at, int last) {
+        const int first = at.w * N, in = min(max(last + 1 - first, 0), N);       // the wavefront's steps inside the row
+        uint32_t l = (1u << in) - 1, c = 0;
+        if constexpr (SEQ) {
+            const int before = __builtin_amdgcn_update_dpp(0, sq, 0x111, 0xf, 0xf, true);      // row_shr:1
+            l &= (uint32_t)(__ballot(sq >= 0) >> 1);
+            c = l & (uint32_t)(__ballot(sq != before) >> 1);
+            if (begins && first == 0) c &= ~1u;
         }
+        live = l >> (at.tg * TS);
+        clear = (c >> (at.tg * TS)) & ((1u << TS) - 1);
+        return l == (1u << N) - 1;
     }
     M2_DEV bool is_live(int j) const { return live >> j & 1; }
     M2_DEV bool clears(int j) const { return SEQ && (clear >> j & 1); }
 };
 
-// the maps of the lanes of each channel, joined in the order of their steps: inclusive
-template <int LC, bool SEQ> M2_DEV Map<SEQ> scan_up(Map<SEQ> m, int lane) {
-#pragma unroll
-    for (int o = LC; o < 64; o <<= 1) {
-        const Map<SEQ> e{__shfl_up(m.P, o), __shfl_up(m.H, o)};
-        if (lane >= o) m = m.after(e);
-    }
-    return m;
+// The maps of the lanes of each channel, joined in the order of their steps: m becomes the inclusive one,
+// the exclusive one is returned.  D: 1 from the first step on, -1 from the last back.  (A lane's shift goes through the LDS pipe,
+// which is idle; lanes without another one read any.)
+template <int D, int O, bool SEQ> M2_DEV Map<SEQ> shifted(const Map<SEQ>& m, int lane) {
+    const int from = (lane - D * O) * 4;
+    return Map<SEQ>{__int_as_float(__builtin_amdgcn_ds_bpermute(from, __float_as_int(m.P))),
+                    __int_as_float(__builtin_amdgcn_ds_bpermute(from, __float_as_int(m.H)))};
 }
-template <int LC, bool SEQ> M2_DEV Map<SEQ> scan_down(Map<SEQ> m, int lane) {
-#pragma unroll
-    for (int o = LC; o < 64; o <<= 1) {
-        const Map<SEQ> e{__shfl_down(m.P, o), __shfl_down(m.H, o)};
-        if (lane + o < 64) m = m.after(e);
+template <int D, int LC, int O, bool SEQ> M2_DEV void join(Map<SEQ>& m, int lane) {
+    if constexpr (O < 64) {
+        const Map<SEQ> e = shifted<D, O, SEQ>(m, lane), j = m.after(e);
+        const bool has = D > 0 ? lane >= O : lane + O < 64;
+        m.P = has ? j.P : m.P;
+        m.H = has ? j.H : m.H;
+        join<D, LC, 2 * O, SEQ>(m, lane);
     }
-    return m;
+}
+template <int D, int LC, bool SEQ> M2_DEV Map<SEQ> scan(Map<SEQ>& m, int lane) {
+    join<D, LC, LC, SEQ>(m, lane);
+    if constexpr (LC == 64) return Map<SEQ>{1.f, 0.f};
+    const Map<SEQ> e = shifted<D, LC, SEQ>(m, lane);
+    const bool has = D > 0 ? lane >= LC : lane + LC < 64;
+    return Map<SEQ>{has ? e.P : 1.f, has ? e.H : 0.f};
 }
 
-template <typename T, int V, int LC, int TS, int W, bool SEQ>
-__global__ void __launch_bounds__(W * 64) k_rec_forward(RecArgs a) {
+// AGG: only the map of the segment is wanted (a.agg)
+template <typename T, int V, int LC, int TS, int W, bool SEQ, bool AGG, bool NT>
+__global__ void __launch_bounds__(W * 64, 4) k_rec_forward(RecArgs a) {
     typedef Place<V, LC, TS, W> P;
-    __shared__ float2 tot[2][W][P::C];
+    __shared__ float2 tot[3][W][P::C];
     const P at(a);
-    const int lane = threadIdx.x & 63;
-    const T* x = static_cast<const T*>(a.x) + at.b * a.xb + at.c;
-    const T* r = static_cast<const T*>(a.r) + at.b * a.rb + at.c;
-    const T* i = static_cast<const T*>(a.i) + at.b * a.ib + at.c;
-    T* out = static_cast<T*>(a.out) + at.b * a.L * a.dim + at.c;
+    if (AGG && at.segment == a.segments - 1) return;     // (nothing follows it)
+    Stream<T, V> sx(a.x, at.b * a.xb + at.t0 * a.xt, a.xt, a, at), sr(a.r, at.b * a.rb + at.t0 * a.rt, a.rt, a, at),
+        si(a.i, at.b * a.ib + at.t0 * a.it, a.it, a, at);
+    Output<T, V, NT> so(a.out, (at.b * a.L + at.t0) * a.dim, a, at);
     const int32_t* seq = SEQ ? a.seq + at.b * a.L : nullptr;
-    float A[V], h[V];
+    float A[V];
+    Map<SEQ> h[V];               // from the segment's start on; but for AGG its H is the state
+    bool far = false;
 #pragma unroll
     for (int v = 0; v < V; ++v) {
         A[v] = a.A[at.c + v];
-        h[v] = a.h0 ? a.h0[(int64_t)at.b * a.dim + at.c + v] : 0.f;
+        far |= !(A[v] >= NEAR);
+        h[v] = Map<SEQ>{1.f, 0.f};
+        if (!AGG && a.h0) h[v].H = a.h0[(int64_t)at.b * a.dim + at.c + v];
     }
-    Raw<T, V> nx[TS], nr[TS], ni[TS];
-    Steps<TS, SEQ> ns, cs;
-    auto load = [&](int64_t t0) {
-        const int64_t t = t0 + at.step;
+    far = __any(far);
+    if (!AGG) {
+#pragma unroll 4
+        for (int u = 0; u < at.segment; ++u)
 #pragma unroll
-        for (int j = 0; j < TS; ++j) {
-            const int64_t u = min(t + j, a.L - 1);
-            nx[j].load(x + u * a.xt);
-            nr[j].load(r + u * a.rt);
-            ni[j].load(i + u * a.it);
-        }
-        ns.load(seq, t, a.L);
-    };
-    load(0);
-    int buf = 0;
-    for (int64_t t0 = 0; t0 < a.L; t0 += P::TILE, buf ^= 1) {
-        const int64_t t = t0 + at.step;
-        Raw<T, V> cx[TS], cr[TS], ci[TS];
-#pragma unroll
-        for (int j = 0; j < TS; ++j) { cx[j] = nx[j]; cr[j] = nr[j]; ci[j] = ni[j]; }
-        cs = ns;
-        if (t0 + P::TILE < a.L) load(t0 + P::TILE);
-        cs.set(t, a.L);
-        const bool masked = SEQ || t0 + P::TILE > a.L;
-        // the gates, and the map of this thread's steps
-        float al[TS][V], add[TS][V];
-        Map<SEQ> m[V];
-#pragma unroll
-        for (int v = 0; v < V; ++v) {
-            float S = 0.f, H = 0.f;
-#pragma unroll
-            for (int j = 0; j < TS; ++j) {
-                float q = sigmoid(cr[j].get(v)), s = sigmoid(ci[j].get(v)), xv = cx[j].get(v);
-                if (masked && !cs.is_live(j)) q = s = xv = 0.f;
-                const float L = A[v] * q;
-                al[j][v] = decay(L);
-                float y;
-                const float ib = inv_beta(al[j][v], y);
-                add[j][v] = y * ib * s * xv;
-                S += L;
-                const float e = cs.clears(j) ? 0.f : H;
-                H = step(al[j][v], e, add[j][v]);
+            for (int v = 0; v < V; ++v) {
+                const float2 p = a.agg[at.agg(a, u) + v];
+                h[v].H = Map<SEQ>{p.x, p.y}.of(h[v].H);
             }
-            m[v].P = SEQ && cs.clear ? -1.f : __builtin_amdgcn_exp2f(S * LOG2E);
-            m[v].H = H;
+    }
+    auto last_of = [&](int64_t t0) { return (int)min(at.end - 1 - t0, (int64_t)P::TILE - 1); };
+    struct Tile {
+        Raw<T, V> x[TS], r[TS], i[TS];
+        Steps<TS, P::G, SEQ> s;
+    } one, two, three;
+    auto load = [&](Tile& n, int64_t t0) {
+        const int last = last_of(t0);
+        sx.load(n.x, last);
+        sr.load(n.r, last);
+        si.load(n.i, last);
+        n.s.load(seq + t0, t0 == 0, at, last);
+        sx.move(P::TILE);
+        sr.move(P::TILE);
+        si.move(P::TILE);
+    };
+    // tile c, while the next one is loaded into n
+    auto tile = [&](Tile& c, Tile& n, int64_t t0, int buf) {
+        const int last = last_of(t0);
+        if (t0 + 2 * P::TILE < at.end) load(n, t0 + 2 * P::TILE);
+        if ((SEQ || last != P::TILE - 1) && !c.s.set(t0 == 0, at, last)) {
+#pragma unroll
+            for (int j = 0; j < TS; ++j)
+                if (!c.s.is_live(j)) {           // a = 1, nothing added
+                    c.x[j].fill(0.f);
+                    c.r[j].fill(-INF);
+                    c.i[j].fill(0.f);
+                }
         }
-        Map<SEQ> ex[V];
+        // the gates, and the map of this thread's steps
+        float al[TS][V], add[TS][V], L[TS][V];
+#pragma unroll
+        for (int j = 0; j < TS; ++j)
+#pragma unroll
+            for (int v = 0; v < V; ++v) {
+                const float q = sigmoid_of(exp_neg(c.r[j].get(v))), s = sigmoid_of(exp_neg(c.i[j].get(v)));
+                L[j][v] = A[v] * q;
+                al[j][v] = decay_near(L[j][v]);
+                add[j][v] = s * c.x[j].get(v);
+            }
+        decay_far<TS, V>(al, L, far);
+#pragma unroll
+        for (int j = 0; j < TS; ++j)
+#pragma unroll
+            for (int v = 0; v < V; ++v) add[j][v] *= __builtin_amdgcn_sqrtf(al[j][v] * (2.f - al[j][v]));
+        Map<SEQ> m[V], ex[V];
 #pragma unroll
         for (int v = 0; v < V; ++v) {
-            const Map<SEQ> in = scan_up<LC, SEQ>(m[v], lane);
-            ex[v] = Map<SEQ>{__shfl_up(in.P, LC), __shfl_up(in.H, LC)};
-            if (at.tg == 0) ex[v] = Map<SEQ>{1.f, 0.f};
-            if (at.tg == P::G - 1) tot[buf][at.w][at.col + v] = make_float2(in.P, in.H);
+            m[v] = Map<SEQ>{1.f - al[0][v], add[0][v]};
+#pragma unroll
+            for (int j = 1; j < TS; ++j) {
+                m[v].P = fmaf(-al[j][v], m[v].P, m[v].P);
+                m[v].H = step(al[j][v], c.s.clears(j) ? 0.f : m[v].H, add[j][v]);
+            }
+            if (SEQ && c.s.clear) m[v].P = -1.f;
+            ex[v] = scan<1, LC, SEQ>(m[v], at.lane);
+            if (at.tg == P::G - 1) tot[buf][at.w][at.col + v] = make_float2(m[v].P, m[v].H);
         }
         lds_barrier();
         float e[V];
 #pragma unroll
         for (int u = 0; u < W; ++u) {
+            if (!AGG && u == at.w) {
+                asm volatile("");                // (a branch: it is the wavefront's)
+#pragma unroll
+                for (int v = 0; v < V; ++v) e[v] = h[v].H;
+            }
 #pragma unroll
             for (int v = 0; v < V; ++v) {
                 const float2 p = tot[buf][u][at.col + v];
-                if (u == at.w) e[v] = h[v];
-                h[v] = Map<SEQ>{p.x, p.y}.of(h[v]);
+                const Map<SEQ> t{p.x, p.y};
+                if (AGG) h[v] = t.after(h[v]);
+                else h[v].H = t.of(h[v].H);
             }
         }
+        if constexpr (!AGG) {
 #pragma unroll
-        for (int v = 0; v < V; ++v) e[v] = ex[v].of(e[v]);
-        if (a.ck && t < a.L && t % SPAN == 0) {
-            float* ck = a.ck + (at.b * a.spans + t / SPAN) * a.dim + at.c;
-            put<float, V>(ck, e, at.skip);
-        }
+            for (int v = 0; v < V; ++v) e[v] = ex[v].of(e[v]);
+            if (a.ck && at.step % SPAN == 0 && at.step <= last)
+                at.put(a.ck + (at.b * a.spans + (t0 + at.step) / SPAN) * a.dim + at.c, e);
+            const Rsrc to = so.tile(last);
 #pragma unroll
-        for (int j = 0; j < TS; ++j) {
-            float o[V];
+            for (int j = 0; j < TS; ++j) {
+                float o[V];
 #pragma unroll
-            for (int v = 0; v < V; ++v) {
-                const float p = cs.clears(j) ? 0.f : e[v];
-                e[v] = step(al[j][v], p, add[j][v]);
-                o[v] = masked && !cs.is_live(j) ? 0.f : e[v];
+                for (int v = 0; v < V; ++v) {
+                    e[v] = step(al[j][v], c.s.clears(j) ? 0.f : e[v], add[j][v]);
+                    o[v] = SEQ && !c.s.is_live(j) ? 0.f : e[v];
+                }
+                so.store(to, j, o);
             }
-            if (t + j < a.L) put<T, V>(out + (t + j) * a.dim, o, at.skip);
+            so.move(P::TILE);
         }
+    };
+    load(one, at.t0);
+    if (at.t0 + P::TILE < at.end) load(two, at.t0 + P::TILE);
+    for (int64_t t0 = at.t0; t0 < at.end; t0 += 3 * P::TILE) {
+        tile(one, three, t0, 0);
+        if (t0 + P::TILE >= at.end) break;
+        tile(two, one, t0 + P::TILE, 1);
+        if (t0 + 2 * P::TILE >= at.end) break;
+        tile(three, two, t0 + 2 * P::TILE, 2);
     }
-    if (a.last && at.w == 0 && at.tg == 0) put<float, V>(a.last + (int64_t)at.b * a.dim + at.c, h, at.skip);
+    if (at.w != 0 || at.tg != 0) return;
+    if constexpr (AGG) {
+        float2 o[V];
+#pragma unroll
+        for (int v = 0; v < V; ++v) o[v] = make_float2(h[v].P, h[v].H);
+        at.put(a.agg + at.agg(a, at.segment), o);
+    } else if (a.last && at.segment == a.segments - 1) {
+        float o[V];
+#pragma unroll
+        for (int v = 0; v < V; ++v) o[v] = h[v].H;
+        at.put(a.last + (int64_t)at.b * a.dim + at.c, o);
+    }
 }
 
+// The map of each segment but the first from its end back: of r and the upstream gradient alone
 template <typename T, int V, int LC, int TS, int W, bool SEQ>
-__global__ void __launch_bounds__(W * 64) k_rec_backward(RecArgs a) {
+__global__ void __launch_bounds__(W * 64, 4) k_rec_back_agg(RecArgs a) {
     typedef Place<V, LC, TS, W> P;
-    static_assert(P::TILE % SPAN == 0, "");
-    __shared__ float tot[2][3][W][P::C];
+    __shared__ float2 tot[3][W][P::C];
     const P at(a);
-    const int lane = threadIdx.x & 63;
-    const T* x = static_cast<const T*>(a.x) + at.b * a.xb + at.c;
-    const T* r = static_cast<const T*>(a.r) + at.b * a.rb + at.c;
-    const T* i = static_cast<const T*>(a.i) + at.b * a.ib + at.c;
-    const T* g = static_cast<const T*>(a.g) + at.b * a.gb + at.c;
-    const int64_t o0 = at.b * a.L * a.dim + at.c;
-    T* dx = static_cast<T*>(a.dx) + o0;
-    T* dr = static_cast<T*>(a.dr) + o0;
-    T* di = static_cast<T*>(a.di) + o0;
+    if (at.segment == 0) return;
+    const int64_t end = at.t0 + (at.end - 1 - at.t0) / P::TILE * P::TILE;
+    Stream<T, V> sr(a.r, at.b * a.rb + end * a.rt, a.rt, a, at), sg(a.g, at.b * a.gb + end * a.gt, a.gt, a, at);
     const int32_t* seq = SEQ ? a.seq + at.b * a.L : nullptr;
-    const float* ck = a.ck + at.b * a.spans * a.dim + at.c;
-    float A[V], mu[V], dA[V];
+    float A[V];
+    Map<SEQ> mu[V];
+    bool far = false;
 #pragma unroll
     for (int v = 0; v < V; ++v) {
         A[v] = a.A[at.c + v];
+        far |= !(A[v] >= NEAR);
+        mu[v] = Map<SEQ>{1.f, 0.f};
+    }
+    far = __any(far);
+    auto last_of = [&](int64_t t0) { return (int)min(at.end - 1 - t0, (int64_t)P::TILE - 1); };
+    struct Tile {
+        Raw<T, V> r[TS], g[TS];
+        Steps<TS, P::G, SEQ> s;
+    } one, two, three;
+    auto load = [&](Tile& n, int64_t t0) {
+        const int last = last_of(t0);
+        sr.load(n.r, last);
+        sg.load(n.g, last);
+        n.s.load(seq + t0, t0 == 0, at, last);
+        sr.move(-P::TILE);
+        sg.move(-P::TILE);
+    };
+    auto tile = [&](Tile& c, Tile& n, int64_t t0, int buf) {
+        const int last = last_of(t0);
+        if (t0 - 2 * P::TILE >= at.t0) load(n, t0 - 2 * P::TILE);
+        if ((SEQ || last != P::TILE - 1) && !c.s.set(t0 == 0, at, last)) {
+#pragma unroll
+            for (int j = 0; j < TS; ++j)
+                if (!c.s.is_live(j)) {
+                    c.r[j].fill(-INF);
+                    c.g[j].fill(0.f);
+                }
+        }
+        float al[TS][V], L[TS][V];
+#pragma unroll
+        for (int j = 0; j < TS; ++j)
+#pragma unroll
+            for (int v = 0; v < V; ++v) {
+                L[j][v] = A[v] * sigmoid_of(exp_neg(c.r[j].get(v)));
+                al[j][v] = decay_near(L[j][v]);
+            }
+        decay_far<TS, V>(al, L, far);
+#pragma unroll
+        for (int v = 0; v < V; ++v) {
+            Map<SEQ> k{1.f - al[TS - 1][v], step(al[TS - 1][v], c.g[TS - 1].get(v))};
+            if (c.s.clears(TS - 1)) k.H = 0.f;
+#pragma unroll
+            for (int j = TS - 2; j >= 0; --j) {
+                k.P = fmaf(-al[j][v], k.P, k.P);
+                k.H = step(al[j][v], c.g[j].get(v) + k.H);
+                if (c.s.clears(j)) k.H = 0.f;
+            }
+            if (SEQ && c.s.clear) k.P = -1.f;
+            join<-1, LC, LC, SEQ>(k, at.lane);
+            if (at.tg == 0) tot[buf][at.w][at.col + v] = make_float2(k.P, k.H);
+        }
+        lds_barrier();
+#pragma unroll
+        for (int u = W - 1; u >= 0; --u)
+#pragma unroll
+            for (int v = 0; v < V; ++v) {
+                const float2 p = tot[buf][u][at.col + v];
+                mu[v] = Map<SEQ>{p.x, p.y}.after(mu[v]);
+            }
+    };
+    load(one, end);
+    if (end - P::TILE >= at.t0) load(two, end - P::TILE);
+    for (int64_t t0 = end; t0 >= at.t0; t0 -= 3 * P::TILE) {
+        tile(one, three, t0, 0);
+        if (t0 - P::TILE < at.t0) break;
+        tile(two, one, t0 - P::TILE, 1);
+        if (t0 - 2 * P::TILE < at.t0) break;
+        tile(three, two, t0 - 2 * P::TILE, 2);
+    }
+    if (at.w != 0 || at.tg != 0) return;
+    float2 o[V];
+#pragma unroll
+    for (int v = 0; v < V; ++v) o[v] = make_float2(mu[v].P, mu[v].H);
+    at.put(a.agg + at.agg(a, at.segment), o);
+}
+
+template <typename T, int V, int LC, int TS, int W, bool SEQ, bool NT>
+__global__ void __launch_bounds__(W * 64, 2) k_rec_backward(RecArgs a) {
+    typedef Place<V, LC, TS, W> P;
+    static_assert(P::TILE % SPAN == 0, "");
+    __shared__ float tot[3][3][W][P::C];
+    const P at(a);
+    const int64_t end = at.t0 + (at.end - 1 - at.t0) / P::TILE * P::TILE;
+    Stream<T, V> sx(a.x, at.b * a.xb + end * a.xt, a.xt, a, at), sr(a.r, at.b * a.rb + end * a.rt, a.rt, a, at),
+        si(a.i, at.b * a.ib + end * a.it, a.it, a, at), sg(a.g, at.b * a.gb + end * a.gt, a.gt, a, at);
+    const int64_t o0 = (at.b * a.L + end) * a.dim;
+    Output<T, V, NT> ox(a.dx, o0, a, at), orr(a.dr, o0, a, at), oi(a.di, o0, a, at);
+    const int32_t* seq = SEQ ? a.seq + at.b * a.L : nullptr;
+    const float* ck = a.ck + at.b * a.spans * a.dim + at.c;
+    float A[V], mu[V], dA[V];
+    bool far = false;
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+        A[v] = a.A[at.c + v];
+        far |= !(A[v] >= NEAR);
         mu[v] = a.glast ? a.glast[(int64_t)at.b * a.dim + at.c + v] : 0.f;
         dA[v] = 0.f;
     }
-    Raw<T, V> nx[TS], nr[TS], ni[TS], ng[TS];
-    Raw<float, V> nk;
-    Steps<TS, SEQ> ns, cs;
-    auto load = [&](int64_t t0) {
-        const int64_t t = t0 + at.step;
-#pragma unroll
-        for (int j = 0; j < TS; ++j) {
-            const int64_t u = min(t + j, a.L - 1);
-            nx[j].load(x + u * a.xt);
-            nr[j].load(r + u * a.rt);
-            ni[j].load(i + u * a.it);
-            ng[j].load(g + u * a.gt);
-        }
-        nk.load(ck + t0 / SPAN * a.dim);
-        ns.load(seq, t, a.L);
-    };
-    int64_t t0 = (a.L - 1) / P::TILE * P::TILE;
-    load(t0);
-    int buf = 0;
-    for (; t0 >= 0; t0 -= P::TILE, buf ^= 1) {
-        const int64_t t = t0 + at.step;
-        Raw<T, V> cx[TS], cr[TS], ci[TS], cg[TS];
-#pragma unroll
-        for (int j = 0; j < TS; ++j) { cx[j] = nx[j]; cr[j] = nr[j]; ci[j] = ni[j]; cg[j] = ng[j]; }
-        cs = ns;
-        float e[V];
-#pragma unroll
-        for (int v = 0; v < V; ++v) e[v] = nk.get(v);
-        if (t0 >= P::TILE) load(t0 - P::TILE);
-        cs.set(t, a.L);
-        const bool masked = SEQ || t0 + P::TILE > a.L;
-        auto dead = [&](int j) { return masked && !cs.is_live(j); };
-        float al[TS][V], q[TS][V], s[TS][V], ib[TS][V];
-        Map<SEQ> m[V];
-        float M[V];
+    far = __any(far);
+#pragma unroll 4
+    for (int u = a.segments - 1; u > at.segment; --u)
 #pragma unroll
         for (int v = 0; v < V; ++v) {
-            float S = 0.f, H = 0.f;
-#pragma unroll
-            for (int j = 0; j < TS; ++j) {
-                float xv = cx[j].get(v);
-                q[j][v] = sigmoid(cr[j].get(v));
-                s[j][v] = sigmoid(ci[j].get(v));
-                if (dead(j)) q[j][v] = s[j][v] = xv = 0.f;
-                const float L = A[v] * q[j][v];
-                al[j][v] = decay(L);
-                float y;
-                ib[j][v] = inv_beta(al[j][v], y);
-                S += L;
-                const float p = cs.clears(j) ? 0.f : H;
-                H = step(al[j][v], p, y * ib[j][v] * s[j][v] * xv);
-            }
-            m[v].P = SEQ && cs.clear ? -1.f : __builtin_amdgcn_exp2f(S * LOG2E);
-            m[v].H = H;
-            float k = 0.f;
-#pragma unroll
-            for (int j = TS - 1; j >= 0; --j) {
-                const float l = (dead(j) ? 0.f : cg[j].get(v)) + k;
-                k = cs.clears(j) ? 0.f : step(al[j][v], l, 0.f);
-            }
-            M[v] = k;
+            const float2 p = a.agg[at.agg(a, u) + v];
+            mu[v] = Map<SEQ>{p.x, p.y}.of(mu[v]);
         }
+    auto last_of = [&](int64_t t0) { return (int)min(at.end - 1 - t0, (int64_t)P::TILE - 1); };
+    struct Tile {
+        Raw<T, V> x[TS], r[TS], i[TS], g[TS];
+        float e[V];              // the state that enters the tile
+        Steps<TS, P::G, SEQ> s;
+    } one, two, three;
+    auto load = [&](Tile& n, int64_t t0) {
+        const int last = last_of(t0);
+        sx.load(n.x, last);
+        sr.load(n.r, last);
+        si.load(n.i, last);
+        sg.load(n.g, last);
+#pragma unroll
+        for (int v = 0; v < V; ++v) n.e[v] = ck[t0 / SPAN * a.dim + v];
+        n.s.load(seq + t0, t0 == 0, at, last);
+        sx.move(-P::TILE);
+        sr.move(-P::TILE);
+        si.move(-P::TILE);
+        sg.move(-P::TILE);
+    };
+    auto tile = [&](Tile& c, Tile& n, int64_t t0, int buf) {
+        const int last = last_of(t0);
+        if (t0 - 2 * P::TILE >= at.t0) load(n, t0 - 2 * P::TILE);
+        if ((SEQ || last != P::TILE - 1) && !c.s.set(t0 == 0, at, last)) {
+#pragma unroll
+            for (int j = 0; j < TS; ++j)
+                if (!c.s.is_live(j)) {           // a = 1, nothing added
+                    c.x[j].fill(0.f);
+                    c.r[j].fill(-INF);
+                    c.i[j].fill(0.f);
+                    c.g[j].fill(0.f);
+                }
+        }
+        float al[TS][V], q[TS][V], s[TS][V], cq[TS][V], cosg[TS][V], ib[TS][V], L[TS][V];
+#pragma unroll
+        for (int j = 0; j < TS; ++j)
+#pragma unroll
+            for (int v = 0; v < V; ++v) {
+                const float eq = exp_neg(c.r[j].get(v)), es = exp_neg(c.i[j].get(v));
+                q[j][v] = sigmoid_of(eq);
+                s[j][v] = sigmoid_of(es);
+                cq[j][v] = co_sigmoid(eq, q[j][v]);
+                cosg[j][v] = co_sigmoid(es, s[j][v]);
+                L[j][v] = A[v] * q[j][v];
+                al[j][v] = decay_near(L[j][v]);
+            }
+        decay_far<TS, V>(al, L, far);
+        // the maps of this thread's steps, forward and back (with the same P)
         Map<SEQ> up[V], down[V];
 #pragma unroll
         for (int v = 0; v < V; ++v) {
-            const Map<SEQ> f = scan_up<LC, SEQ>(m[v], lane), k = scan_down<LC, SEQ>(Map<SEQ>{m[v].P, M[v]}, lane);
-            up[v] = Map<SEQ>{__shfl_up(f.P, LC), __shfl_up(f.H, LC)};
-            down[v] = Map<SEQ>{__shfl_down(k.P, LC), __shfl_down(k.H, LC)};
+            Map<SEQ> f, k;
+#pragma unroll
+            for (int j = 0; j < TS; ++j) {
+                float y;
+                ib[j][v] = inv_beta(al[j][v], y);
+                const float add = y * ib[j][v] * s[j][v] * c.x[j].get(v);
+                f.P = j == 0 ? 1.f - al[j][v] : fmaf(-al[j][v], f.P, f.P);
+                f.H = j == 0 ? add : step(al[j][v], c.s.clears(j) ? 0.f : f.H, add);
+            }
+            if (SEQ && c.s.clear) f.P = -1.f;
+            k.P = f.P;
+#pragma unroll
+            for (int j = TS - 1; j >= 0; --j) {
+                k.H = step(al[j][v], j == TS - 1 ? c.g[j].get(v) : c.g[j].get(v) + k.H);
+                if (c.s.clears(j)) k.H = 0.f;
+            }
+            up[v] = scan<1, LC, SEQ>(f, at.lane);
+            down[v] = scan<-1, LC, SEQ>(k, at.lane);
             if (at.tg == 0) {
-                up[v] = Map<SEQ>{1.f, 0.f};
                 tot[buf][0][at.w][at.col + v] = k.P;
                 tot[buf][2][at.w][at.col + v] = k.H;
             }
-            if (at.tg == P::G - 1) {
-                down[v] = Map<SEQ>{1.f, 0.f};
-                tot[buf][1][at.w][at.col + v] = f.H;
-            }
+            if (at.tg == P::G - 1) tot[buf][1][at.w][at.col + v] = f.H;
         }
         lds_barrier();
         float k[V];
 #pragma unroll
         for (int u = 0; u < W; ++u) {
+            const int d = W - 1 - u;
+            if (u < at.w) {
+                asm volatile("");                // (branches: they are the wavefront's)
 #pragma unroll
-            for (int v = 0; v < V; ++v) {
-                const int f = u, d = W - 1 - u;
-                if (f < at.w) e[v] = Map<SEQ>{tot[buf][0][f][at.col + v], tot[buf][1][f][at.col + v]}.of(e[v]);
-                if (d == at.w) k[v] = mu[v];
-                mu[v] = Map<SEQ>{tot[buf][0][d][at.col + v], tot[buf][2][d][at.col + v]}.of(mu[v]);
+                for (int v = 0; v < V; ++v) c.e[v] = Map<SEQ>{tot[buf][0][u][at.col + v], tot[buf][1][u][at.col + v]}.of(c.e[v]);
             }
+            if (d == at.w) {
+                asm volatile("");
+#pragma unroll
+                for (int v = 0; v < V; ++v) k[v] = mu[v];
+            }
+#pragma unroll
+            for (int v = 0; v < V; ++v) mu[v] = Map<SEQ>{tot[buf][0][d][at.col + v], tot[buf][2][d][at.col + v]}.of(mu[v]);
         }
         float lam[TS][V];
 #pragma unroll
         for (int v = 0; v < V; ++v) {
-            e[v] = up[v].of(e[v]);
+            c.e[v] = up[v].of(c.e[v]);
             k[v] = down[v].of(k[v]);
 #pragma unroll
             for (int j = TS - 1; j >= 0; --j) {
-                lam[j][v] = (dead(j) ? 0.f : cg[j].get(v)) + k[v];
-                k[v] = cs.clears(j) ? 0.f : step(al[j][v], lam[j][v], 0.f);
+                lam[j][v] = c.g[j].get(v) + k[v];
+                k[v] = step(al[j][v], lam[j][v]);
+                if (c.s.clears(j)) k[v] = 0.f;
             }
         }
+        const Rsrc tx = ox.tile(last), tr = orr.tile(last), ti = oi.tile(last);
 #pragma unroll
         for (int j = 0; j < TS; ++j) {
-            float ox[V], orr[V], oi[V];
+            float dx[V], dr[V], di[V];
 #pragma unroll
             for (int v = 0; v < V; ++v) {
-                const bool off = dead(j);
-                const float xv = off ? 0.f : cx[j].get(v), p = cs.clears(j) ? 0.f : e[v];
-                const float av = 1.f - al[j][v], beta = al[j][v] * (2.f - al[j][v]) * ib[j][v];
-                const float sx = s[j][v] * xv;
-                e[v] = step(al[j][v], p, beta * sx);
-                ox[v] = lam[j][v] * beta * s[j][v];
-                const float dL = lam[j][v] * av * (p - av * ib[j][v] * sx);
-                oi[v] = off ? 0.f : ox[v] * xv * co_sigmoid(ci[j].get(v), s[j][v]);
-                orr[v] = off ? 0.f : dL * (A[v] * q[j][v]) * co_sigmoid(cr[j].get(v), q[j][v]);
-                dA[v] = fmaf(dL, q[j][v], dA[v]);
+                const float xv = c.x[j].get(v), p = c.s.clears(j) ? 0.f : c.e[v];
+                const float av = 1.f - al[j][v], sxv = s[j][v] * xv;
+                const float beta = al[j][v] * (2.f - al[j][v]) * ib[j][v];
+                c.e[v] = step(al[j][v], p, beta * sxv);
+                dx[v] = lam[j][v] * beta * s[j][v];
+                di[v] = dx[v] * xv * cosg[j][v];
+                const float dLq = lam[j][v] * av * fmaf(-av * ib[j][v], sxv, p) * q[j][v];
+                dr[v] = dLq * A[v] * cq[j][v];
+                dA[v] += dLq;
+                if (SEQ && !c.s.is_live(j)) dx[v] = dr[v] = di[v] = 0.f;
             }
-            if (t + j < a.L) {
-                put<T, V>(dx + (t + j) * a.dim, ox, at.skip);
-                put<T, V>(dr + (t + j) * a.dim, orr, at.skip);
-                put<T, V>(di + (t + j) * a.dim, oi, at.skip);
-            }
+            ox.store(tx, j, dx);
+            orr.store(tr, j, dr);
+            oi.store(ti, j, di);
         }
+        ox.move(-P::TILE);
+        orr.move(-P::TILE);
+        oi.move(-P::TILE);
+    };
+    load(one, end);
+    if (end - P::TILE >= at.t0) load(two, end - P::TILE);
+    for (int64_t t0 = end; t0 >= at.t0; t0 -= 3 * P::TILE) {
+        tile(one, three, t0, 0);
+        if (t0 - P::TILE < at.t0) break;
+        tile(two, one, t0 - P::TILE, 1);
+        if (t0 - 2 * P::TILE < at.t0) break;
+        tile(three, two, t0 - 2 * P::TILE, 2);
     }
-    const int64_t row = (int64_t)at.b * a.dim + at.c;
-    if (a.dh0 && at.w == 0 && at.tg == 0) put<float, V>(a.dh0 + row, mu, at.skip);
-    // dA of this row: of the lanes of a channel, then of the wavefronts in their order
+    if (a.dh0 && at.segment == 0 && at.w == 0 && at.tg == 0) at.put(a.dh0 + (int64_t)at.b * a.dim + at.c, mu);
+    // dA of this segment: of the lanes of a channel, then of the wavefronts in their order
     lds_barrier();
 #pragma unroll
     for (int v = 0; v < V; ++v) {
@@ -464,17 +712,17 @@ __global__ void __launch_bounds__(W * 64) k_rec_backward(RecArgs a) {
 #pragma unroll
             for (int u = 0; u < W; ++u) dA[v] += tot[0][0][u][at.col + v];
         }
-        put<float, V>(a.dA + row, dA, at.skip);
+        at.put(a.dA + at.agg(a, at.segment), dA);
     }
 }
 
-// dA of the batch rows, in their order
-__global__ void __launch_bounds__(64) k_rec_join(const float* part, float* dA, int64_t batch, int64_t dim) {
+// dA of the segments of all rows, in their order
+__global__ void __launch_bounds__(64) k_rec_join(const float* part, float* dA, int64_t parts, int64_t dim) {
     const int64_t c = (int64_t)blockIdx.x * 64 + threadIdx.x;
     if (c >= dim) return;
     double s = 0;
 #pragma unroll 8
-    for (int64_t b = 0; b < batch; ++b) s += part[b * dim + c];
+    for (int64_t b = 0; b < parts; ++b) s += part[b * dim + c];
     dA[c] = (float)s;
 }
 
@@ -497,13 +745,11 @@ template <typename T> __global__ void __launch_bounds__(64) k_rec_step(StepArgs 
     const int64_t b = blockIdx.y;
     const int c = blockIdx.x * 64 + threadIdx.x;
     if (c >= a.dim) return;
-    const float q = sigmoid(to_f32(static_cast<const T*>(a.r)[b * a.rb + c]));
-    const float s = sigmoid(to_f32(static_cast<const T*>(a.i)[b * a.ib + c]));
+    const float q = sigmoid_of(exp_neg(to_f32(static_cast<const T*>(a.r)[b * a.rb + c])));
+    const float s = sigmoid_of(exp_neg(to_f32(static_cast<const T*>(a.i)[b * a.ib + c])));
     const float xv = to_f32(static_cast<const T*>(a.x)[b * a.xb + c]), e = a.state[b * a.dim + c];
-    const float al = decay(a.A[c] * q);
-    float y;
-    const float ib = inv_beta(al, y);
-    const float h = step(al, e, y * ib * s * xv);
+    const float L = a.A[c] * q, al = decay(L, decay_near(L));
+    const float h = step(al, e, __builtin_amdgcn_sqrtf(al * (2.f - al)) * s * xv);
     a.next[b * a.dim + c] = h;
     static_cast<T*>(a.out)[b * a.dim + c] = from_f32<T>(h);
 }
@@ -511,37 +757,76 @@ template <typename T> __global__ void __launch_bounds__(64) k_rec_step(StepArgs 
 // ---------------------------------------------------------------------------
 // launches
 // ---------------------------------------------------------------------------
-template <typename T, int V, int LC, int TS, int W> void launch(RecArgs a, int64_t batch, bool back, hipStream_t s) {
+constexpr int LC = 32, TS = 4;
+// Segments of a row's length, and their steps.
+int segments(int64_t batch, int64_t L, int64_t dim, int64_t& seg) {
+    constexpr int64_t UNIT = 128;
+    const int64_t units = L > 0 ? (L + UNIT - 1) / UNIT : 1, slabs = batch * ((dim + 2 * LC - 1) / (2 * LC));
+    int64_t s = 1;
+    if (slabs < 400) s = slabs > 0 ? (1280 + slabs - 1) / slabs : 1;
+    if (s > units) s = units;
+    const int64_t per = (units + s - 1) / s;
+    seg = per * UNIT;
+    return (int)((units + per - 1) / per);
+}
+
+template <typename T, int V, bool SEQ, bool NT> void launch(RecArgs a, int64_t batch, bool back, hipStream_t s) {
     a.slabs = (a.dim + V * LC - 1) / (V * LC);
-    const dim3 grid((unsigned)(batch * a.slabs)), block(W * 64);
-    auto go = [&](auto k) { hipLaunchKernelGGL(k, grid, block, 0, s, a); };
+    const dim3 grid((unsigned)(batch * a.segments * a.slabs));
+    auto go = [&](auto k, int w) { hipLaunchKernelGGL(k, grid, dim3(w * 64), 0, s, a); };
     if (back) {
-        if (a.seq) go(k_rec_backward<T, V, LC, TS, W, true>);
-        else go(k_rec_backward<T, V, LC, TS, W, false>);
+        if (a.segments > 1) go(k_rec_back_agg<T, V, LC, TS, 4, SEQ>, 4);
+        go(k_rec_backward<T, V, LC, TS, 4, SEQ, NT>, 4);
+    } else if (a.segments > 1) {
+        go(k_rec_forward<T, V, LC, TS, 4, SEQ, true, false>, 4);
+        go(k_rec_forward<T, V, LC, TS, 4, SEQ, false, NT>, 4);
     } else {
-        if (a.seq) go(k_rec_forward<T, V, LC, TS, W, true>);
-        else go(k_rec_forward<T, V, LC, TS, W, false>);
+        go(k_rec_forward<T, V, LC, TS, 8, SEQ, false, NT>, 8);
     }
 }
 template <typename T> void run(const RecArgs& a, int64_t batch, bool back, hipStream_t s) {
-    if (a.dim < 4) launch<T, 1, 4, 4, 4>(a, batch, back, s);
-    else launch<T, 4, 16, 4, 4>(a, batch, back, s);
+    // Non-temporal stores where what is read and written does not fit the last-level cache (256 MB): results would take the
+    // place of what is read again (the second pass over a segment) or next.
+    const bool nt = batch * a.L * a.dim * (int64_t)sizeof(T) * (back ? 7 : 4) > (256ll << 20);
+    auto go = [&](auto seq, auto many) {
+        if (a.dim == 1) launch<T, 1, decltype(seq)::value, false>(a, batch, back, s);
+        else launch<T, 2, decltype(seq)::value, decltype(many)::value>(a, batch, back, s);
+    };
+    if (a.seq) {
+        if (nt) go(std::true_type(), std::true_type());
+        else go(std::true_type(), std::false_type());
+    } else {
+        if (nt) go(std::false_type(), std::true_type());
+        else go(std::false_type(), std::false_type());
+    }
 }
+
+// (a tile's offsets have 32 bits: at most 512 steps of 4 bytes)
+constexpr int64_t MAX_STRIDE = 1 << 20;
+// rows of a step that are one, or behind each other
+bool stride_ok(int64_t st, int64_t dim) { return st == 0 || (st >= dim && st <= MAX_STRIDE); }
 
 // what a call may ask for, whichever it is
 int check_sizes(const char* who, int64_t batch, int64_t seqlen, int64_t dim, int dtype) {
-    M2_REQUIRE(batch >= 0 && seqlen >= 0 && dim > 0 && dim < (1 << 30) && seqlen < (1ll << 40), M2_ERR_INVALID,
+    M2_REQUIRE(batch >= 0 && seqlen >= 0 && dim > 0 && dim <= MAX_STRIDE && seqlen < (1ll << 40), M2_ERR_INVALID,
                "%s: bad sizes (batch %lld, seqlen %lld, dim %lld)", who, (long long)batch, (long long)seqlen,
                (long long)dim);
     M2_REQUIRE(dtype == M2_F32 || dtype == M2_BF16, M2_ERR_UNSUPPORTED, "%s: dtype %d", who, dtype);
-    // (workgroups of the narrowest slabs)
-    M2_REQUIRE(batch < (1ll << 30) && batch * ((dim + 3) / 4) < (1ll << 31), M2_ERR_UNSUPPORTED, "%s: too many rows", who);
+    // (counts of workgroups)
+    M2_REQUIRE(batch < (1ll << 30) && batch * ((dim + 63) / 64) < (1ll << 24), M2_ERR_UNSUPPORTED, "%s: too many rows", who);
     return M2_OK;
 }
 
 }  // namespace
 
 namespace m2 {
+
+size_t gated_recurrence_workspace(const m2_gated_recurrence_args& a) {
+    if (check_sizes("gated_linear_recurrence", a.batch, a.seqlen, a.dim, a.dtype)) return 0;
+    int64_t seg;
+    const int n = segments(a.batch, a.seqlen, a.dim, seg);
+    return n > 1 ? 8 * (size_t)a.batch * n * a.dim : 256;
+}
 
 int launch_gated_recurrence(const m2_gated_recurrence_args& a, hipStream_t s) {
     const char* who = "gated_linear_recurrence";
@@ -555,6 +840,8 @@ int launch_gated_recurrence(const m2_gated_recurrence_args& a, hipStream_t s) {
                                a.initial_states, a.final_states, n);
         return check_launch(who);
     }
+    M2_REQUIRE(stride_ok(a.x_stride_time, a.dim) && stride_ok(a.r_stride_time, a.dim) && stride_ok(a.i_stride_time, a.dim),
+               M2_ERR_INVALID, "%s: strides of time (0, or dim to %lld)", who, (long long)MAX_STRIDE);
     RecArgs k{};
     k.x = a.x; k.r = a.r; k.i = a.i; k.A = a.A; k.h0 = a.initial_states; k.seq = a.seq_idx;
     k.xb = a.x_stride_batch; k.xt = a.x_stride_time;
@@ -562,6 +849,11 @@ int launch_gated_recurrence(const m2_gated_recurrence_args& a, hipStream_t s) {
     k.ib = a.i_stride_batch; k.it = a.i_stride_time;
     k.ck = a.span_states; k.L = a.seqlen; k.spans = (a.seqlen + SPAN - 1) / SPAN; k.dim = (int)a.dim;
     k.out = a.out; k.last = a.final_states;
+    k.segments = segments(a.batch, a.seqlen, a.dim, k.seg);
+    const size_t need = gated_recurrence_workspace(a);
+    M2_REQUIRE(k.segments == 1 || (a.workspace && a.workspace_bytes >= need), M2_ERR_WORKSPACE,
+               "%s: workspace of %zu bytes needed, %zu given", who, need, a.workspace_bytes);
+    k.agg = static_cast<float2*>(a.workspace);
     if (a.dtype == M2_F32) run<float>(k, a.batch, false, s);
     else run<bf16>(k, a.batch, false, s);
     return check_launch(who);
@@ -569,7 +861,9 @@ int launch_gated_recurrence(const m2_gated_recurrence_args& a, hipStream_t s) {
 
 size_t gated_recurrence_grad_workspace(const m2_gated_recurrence_grad_args& a) {
     if (check_sizes("gated_linear_recurrence_grad", a.batch, a.seqlen, a.dim, a.dtype)) return 0;
-    return 4 * (size_t)(a.batch > 1 ? a.batch : 1) * a.dim;
+    int64_t seg;
+    const size_t n = segments(a.batch, a.seqlen, a.dim, seg) * (size_t)(a.batch > 1 ? a.batch : 1);
+    return 12 * n * a.dim;
 }
 
 int launch_gated_recurrence_grad(const m2_gated_recurrence_grad_args& a, hipStream_t s) {
@@ -578,6 +872,9 @@ int launch_gated_recurrence_grad(const m2_gated_recurrence_grad_args& a, hipStre
     M2_REQUIRE(a.batch > 0 && a.seqlen > 0, M2_ERR_INVALID, "%s: no steps", who);
     M2_REQUIRE(a.x && a.r && a.i && a.A && a.span_states && a.grad_out && a.grad_x && a.grad_r && a.grad_i && a.grad_A,
                M2_ERR_INVALID, "%s: x, r, i, A, span_states, grad_out and the gradients are required", who);
+    M2_REQUIRE(stride_ok(a.x_stride_time, a.dim) && stride_ok(a.r_stride_time, a.dim) && stride_ok(a.i_stride_time, a.dim) &&
+                   stride_ok(a.grad_out_stride_time, a.dim),
+               M2_ERR_INVALID, "%s: strides of time (0, or dim to %lld)", who, (long long)MAX_STRIDE);
     const size_t need = gated_recurrence_grad_workspace(a);
     M2_REQUIRE(a.workspace && a.workspace_bytes >= need, M2_ERR_WORKSPACE,
                "%s: workspace of %zu bytes needed, %zu given", who, need, a.workspace_bytes);
@@ -591,11 +888,14 @@ int launch_gated_recurrence_grad(const m2_gated_recurrence_grad_args& a, hipStre
     k.g = a.grad_out; k.gb = a.grad_out_stride_batch; k.gt = a.grad_out_stride_time;
     k.glast = a.grad_final_states;
     k.dx = a.grad_x; k.dr = a.grad_r; k.di = a.grad_i; k.dh0 = a.grad_initial_states;
-    k.dA = a.batch == 1 ? a.grad_A : static_cast<float*>(a.workspace);
+    k.segments = segments(a.batch, a.seqlen, a.dim, k.seg);
+    const int64_t parts = a.batch * k.segments;
+    k.agg = static_cast<float2*>(a.workspace);
+    k.dA = parts == 1 ? a.grad_A : static_cast<float*>(a.workspace) + 2 * parts * a.dim;
     if (a.dtype == M2_F32) run<float>(k, a.batch, true, s);
     else run<bf16>(k, a.batch, true, s);
-    if (a.batch > 1)
-        hipLaunchKernelGGL(k_rec_join, dim3((unsigned)((a.dim + 63) / 64)), dim3(64), 0, s, k.dA, a.grad_A, a.batch, a.dim);
+    if (parts > 1)
+        hipLaunchKernelGGL(k_rec_join, dim3((unsigned)((a.dim + 63) / 64)), dim3(64), 0, s, k.dA, a.grad_A, parts, a.dim);
     return check_launch(who);
 }
 

@@ -65,6 +65,7 @@ size_t clip_grad_norm_workspace(const m2_clip_grad_norm_args& a);
 
 // the gated linear recurrence (gated_recurrence.hip)
 int launch_gated_recurrence(const m2_gated_recurrence_args& a, hipStream_t stream);
+size_t gated_recurrence_workspace(const m2_gated_recurrence_args& a);
 int launch_gated_recurrence_grad(const m2_gated_recurrence_grad_args& a, hipStream_t stream);
 size_t gated_recurrence_grad_workspace(const m2_gated_recurrence_grad_args& a);
 int launch_gated_recurrence_update(const m2_gated_recurrence_update_args& a, hipStream_t stream);

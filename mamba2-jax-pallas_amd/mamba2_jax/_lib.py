@@ -191,7 +191,8 @@ class GatedRecurrenceArgs(ctypes.Structure):
                 ("seq_idx", _c_p), ("out", _c_p), ("final_states", _c_p), ("span_states", _c_p),
                 ("batch", _i64), ("seqlen", _i64), ("dim", _i64), ("x_stride_batch", _i64),
                 ("x_stride_time", _i64), ("r_stride_batch", _i64), ("r_stride_time", _i64),
-                ("i_stride_batch", _i64), ("i_stride_time", _i64), ("dtype", _i32)]
+                ("i_stride_batch", _i64), ("i_stride_time", _i64), ("dtype", _i32),
+                ("workspace", _c_p), ("workspace_bytes", ctypes.c_size_t)]
 
 
 class GatedRecurrenceGradArgs(ctypes.Structure):
@@ -261,6 +262,7 @@ WORKSPACE_SIZES = {
     "m2_linear_cross_entropy_saved_size": LinearCrossEntropyArgs,
     "m2_linear_cross_entropy_grad_workspace_size": LinearCrossEntropyGradArgs,
     "m2_clip_grad_norm_workspace_size": ClipGradNormArgs,
+    "m2_gated_recurrence_workspace_size": GatedRecurrenceArgs,
     "m2_gated_recurrence_grad_workspace_size": GatedRecurrenceGradArgs,
     "m2_gated_linear_saved_size": GatedLinearArgs,
     "m2_gated_linear_workspace_size": GatedLinearArgs,
@@ -269,7 +271,7 @@ WORKSPACE_SIZES = {
 # activations of the gated feed-forward product (M2_SILU, M2_GELU)
 ACTIVATIONS = {"silu": 0, "gelu": 1}
 # positions between two of the states that the recurrence leaves its gradient (M2_RECURRENCE_SPAN)
-RECURRENCE_SPAN = 64
+RECURRENCE_SPAN = 32
 OTHER_SYMBOLS = ("m2_ssd_combined_workspace_size", "m2_ssd_combined_plan", "m2_last_error", "m2_abi_version",
                  "m2_set_dispatch_override", "m2_ssd_combined_noalloc_prepare",
                  *WORKSPACE_SIZES)

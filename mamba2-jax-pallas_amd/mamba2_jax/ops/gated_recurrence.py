@@ -19,9 +19,22 @@ from torch.autograd.function import once_differentiable
 from .. import _lib as L
 
 
-def _strided(t):
-    """t with contiguous channels (a copy where they are not)."""
+def _rows(t):
+    """t (batch, dim) with contiguous channels (a copy where they are not)."""
     return t if t.stride(-1) == 1 or t.shape[-1] == 1 else t.contiguous()
+
+
+MAX_STRIDE = 2 ** 20
+
+
+def _strided(t):
+    """t (batch, seqlen, dim) as the kernels read it in place: contiguous channels, positions that are one, or
+    behind each other and at most MAX_STRIDE elements apart; a copy where it is not so."""
+    dim = t.shape[2]
+    st = t.stride(1)
+    if (t.stride(2) == 1 or dim == 1) and (st == 0 or dim <= st <= MAX_STRIDE):
+        return t
+    return t.contiguous() if not t.is_contiguous() else t
 
 
 def _f32(t):
@@ -47,8 +60,7 @@ def _forward(x, r, i, A, initial_states, seq_idx, want_final, save):
         x.data_ptr(), r.data_ptr(), i.data_ptr(), A.data_ptr(), L.ptr(h0), L.ptr(seq_idx),
         out.data_ptr(), L.ptr(final), L.ptr(spans), batch, seqlen, dim, x.stride(0), x.stride(1),
         r.stride(0), r.stride(1), i.stride(0), i.stride(1), L.dtype_code(x, "x"))
-    with L.on_device(dev):
-        L.call("m2_gated_recurrence", args, L.stream_of(dev))
+    L.call_with_workspace("m2_gated_recurrence", args, dev)
     return out, final, (x, r, i, A, seq_idx, spans)
 
 
@@ -131,12 +143,13 @@ def gated_linear_recurrence(x, r, i, A, initial_states=None, seq_idx=None, retur
 
     Gates, states and sums are float32 (a state and the gradient that comes back to it never
     leave it between two positions); h and the gradients are rounded once.  Between the two the graph holds x, r, i and
-    the states that enter every 64 positions.  Where a_t is 1 the root has no slope, and its part
+    the states that enter every 32 positions.  Where a_t is 1 the root has no slope, and its part
     of the gradient is taken as 0.  Equal inputs give equal bits."""
     dev = L.device_of(x, r, i, A, initial_states, seq_idx)
     shape = x.shape
     L.require(len(shape) == 3, lambda: f"x.shape={tuple(shape)}: expected (batch, seqlen, dim)")
     _check_gates(x, r, i, A, shape)
+    L.require(shape[2] <= MAX_STRIDE, lambda: f"x.shape={tuple(shape)}: more than {MAX_STRIDE} channels")
     if initial_states is not None:
         L.require(initial_states.shape == (shape[0], shape[2]),
                   lambda: f"initial_states.shape={tuple(initial_states.shape)}: expected {(shape[0], shape[2])}")
@@ -170,7 +183,7 @@ def gated_linear_recurrence_update(state, x, r, i, A, *, inplace=False):
     L.dtype_code(state, "state")
     src = _f32(state)
     new = src if inplace and src is state else torch.empty(shape, dtype=torch.float32, device=dev)
-    x, r, i, A = _strided(x), _strided(r), _strided(i), _f32(A)
+    x, r, i, A = _rows(x), _rows(r), _rows(i), _f32(A)
     out = torch.empty(shape, dtype=x.dtype, device=dev)
     args = L.GatedRecurrenceUpdateArgs(
         x.data_ptr(), r.data_ptr(), i.data_ptr(), A.data_ptr(), src.data_ptr(), new.data_ptr(),

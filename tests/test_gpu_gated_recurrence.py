@@ -91,10 +91,14 @@ class Reference:
         if g is None:
             return
         g = torch.where(live, g.detach().double(), zero)
-        g = torch.cat([g[:, :-1], g[:, -1:] + (0 if glast is None else glast.detach().double()[:, None])], 1)
+        # the last position's gradient is a sum, whose terms a kernel may pass on apart from each other (a g and
+        # a glast, each rounded): of magnitude |g| + |glast|, however much of it cancels
+        gl = torch.zeros_like(g[:, 0]) if glast is None else glast.detach().double()
+        gmag = torch.cat([g[:, :-1].abs(), g[:, -1:].abs() + gl.abs()[:, None]], 1)
+        g = torch.cat([g[:, :-1], g[:, -1:] + gl[:, None]], 1)
         later = torch.cat([a[:, 1:], zero[:, :1]], 1)
         lam = scan(later.flip(1), g.flip(1)).flip(1)
-        lmag = scan(later.flip(1), g.abs().flip(1)).flip(1)
+        lmag = scan(later.flip(1), gmag.flip(1)).flip(1)
         passed = (alpha_live * ea * lmag + 3 * F * lmag)
         passed = torch.cat([passed[:, 1:], zero[:, :1]], 1)
         el = scan(later.flip(1), (passed + 2 * F * lmag).flip(1)).flip(1) + 24 * F * lmag
@@ -180,11 +184,23 @@ def test_recurrence(batch, seqlen, dim, dtype, fused, packed, carried):
     check(*inputs(batch, seqlen, dim, dtype, fused, packed, carried))
 
 
-@pytest.mark.parametrize("batch,seqlen,dim", [(8, 300, 640), (1, 2100, 700), (2, 900, 2560), (16, 70, 5120)])
+# rows of one segment and of many, of one and of several tiles, ended inside a tile
+LARGE = [(8, 300, 640), (1, 2100, 700), (2, 900, 2560), (16, 70, 5120), (6, 333, 4500), (1, 5000, 2560)]
+
+
+@pytest.mark.parametrize("batch,seqlen,dim", LARGE)
 @pytest.mark.parametrize("dtype", ["bf16", "f32"])
-def test_recurrence_large(batch, seqlen, dim, dtype):
-    announce("recurrence large", batch, seqlen, dim, dtype)
-    check(*inputs(batch, seqlen, dim, dtype, True, 100, True))
+@pytest.mark.parametrize("packed", [0, 100])
+def test_recurrence_large(batch, seqlen, dim, dtype, packed):
+    announce("recurrence large", batch, seqlen, dim, dtype, packed)
+    check(*inputs(batch, seqlen, dim, dtype, True, packed, True))
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+def test_recurrence_past_the_cache(dtype):
+    """More than the last-level cache holds."""
+    announce("past the cache", dtype)
+    check(*inputs(7, 1200, 4160, dtype, carried=True))
 
 
 @pytest.mark.parametrize("low,high", [(1e-6, 1e-5), (1e-4, 1e-3), (0.3, 0.4), (5.0, 60.0)])

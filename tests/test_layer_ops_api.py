@@ -49,12 +49,15 @@ def test_gated_recurrence_refusals():
               r_stride_batch=72, r_stride_time=8, i_stride_batch=72, i_stride_time=8, dtype=L.M2_BF16)
     mk = lambda **k: L.GatedRecurrenceArgs(**{**ok, **k})
     name = "m2_gated_recurrence"
-    for bad in (dict(batch=-1), dict(seqlen=-1), dict(dim=0), dict(dim=1 << 30), dict(seqlen=1 << 40)):
+    for bad in (dict(batch=-1), dict(seqlen=-1), dict(dim=0), dict(dim=(1 << 20) + 1), dict(seqlen=1 << 40)):
         refused(name, mk(**bad), -1, "bad sizes")
     refused(name, mk(dtype=L.M2_I32), -2, "dtype")
     refused(name, mk(batch=1 << 31, dim=64), -2, "too many rows")
     for p in ("x", "r", "i", "A", "out"):
         refused(name, mk(**{p: None}), -1, "required")
+    for p in "xri":
+        for st in (-8, 7, (1 << 20) + 1):
+            refused(name, mk(**{p + "_stride_time": st}), -1, "strides of time")
     okg = {k: v for k, v in ok.items() if k != "out"} | dict(
         span_states=4096, grad_out=4096, grad_x=4096, grad_r=4096, grad_i=4096, grad_A=4096,
         grad_out_stride_batch=72, grad_out_stride_time=8)
@@ -69,6 +72,7 @@ def test_gated_recurrence_refusals():
     refused(name, mg(dtype=7), -2, "dtype")
     for p in ("x", "r", "i", "A", "span_states", "grad_out", "grad_x", "grad_r", "grad_i", "grad_A"):
         refused(name, mg(**{p: None}), -1, "required")
+    refused(name, mg(grad_out_stride_time=7), -1, "strides of time")
     refused(name, mg(workspace=4096, workspace_bytes=need - 1), -4, "workspace")
     refused(name, mg(workspace_bytes=need), -4, "workspace")
 

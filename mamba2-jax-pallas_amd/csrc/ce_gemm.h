@@ -287,9 +287,11 @@ struct Shape {
     static constexpr int SLOT = LA::BYTES + LB::BYTES;
     static constexpr int LDS = SLOT * ST;
     static constexpr int LOADS = LA::J + LB::J;
-    // what deal() goes by: 1.4 us a step of 256 x 256 (as measured), 0.85 us of 256 x 128; six
-    // products 4.5 us of 256 x 128, 1.5 us of 128 x 64; a segment of 256 KB 0.11 us
-    static constexpr int STEP = TERMS == 1 ? (BN == 256 ? 280 : 170) : BN == 128 ? 900 : BN == 64 ? 300 : 100;
+    // what deal() and the choices of shapes go by: 1.4 us a step of 256 x 256 (as measured), 0.85 us of 256 x 128,
+    // 0.5 us of 128 x 64; six products 4.5 us of 256 x 128, 2.4 us of 128 x 128, 1.5 us of 128 x 64; a segment of
+    // 256 KB 0.11 us
+    static constexpr int STEP = TERMS == 1 ? (BN == 256 ? 280 : BN == 64 ? 100 : 170)
+                                : BN == 128 ? (BM == 128 ? 480 : 900) : BN == 64 ? 300 : 100;
     static constexpr int SEG = BM * BN * 22 / 65536 + 1;
 };
 

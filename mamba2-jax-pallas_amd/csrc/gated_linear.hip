@@ -7,16 +7,21 @@
 //
 // Forward: the product runs in the tiles of ce_gemm.h, whose rows are 16 of the gate and
 // the same 16 of the values in turn (PAIR): a lane's accumulators hold g and v of the same place, and
-// the epilogue stores h alone (and, for a gradient, g and v in the operands' type: to compute them again
-// would take a third of the gradient's operations, to keep them costs their bytes twice).  Up to 64 tokens
+// the epilogue stores h alone (and, for a gradient, act(g) and v act'(g), by which dh is multiplied, in
+// the operands' type: to compute them again would take a third of the gradient's operations, to keep
+// them costs their bytes twice; g and v themselves would be rounded before the activation's slope
+// and not after it).  Up to 64 tokens
 // whose rows a lane can load in 16-byte pieces run k_glu_few, bound by reading W once.
-// Backward: k_glu_dz makes dz = [dg | dv] (bf16, or three planes of it for float32), then two
+// Backward: k_glu_dz makes dz = [dg | dv] = [dh v act'(g) | dh act(g)] (bf16, or three planes of it for float32), then two
 // products read it: dx with K over W's rows, dW with K over the tokens.  Tiles that would leave CUs idle in the
 // last round are cut along K into float32 parts (deal), which k_glu_join adds up.
 //
 // Operands that direct loads cannot take in place (float32, widths that 64 does not divide, unaligned
 // rows) are packed first: rows padded with zeros, the gate's and the values' to whole 64s.
 #include "ce_gemm.h"
+#ifdef TUNE
+#include <cstdlib>
+#endif
 
 namespace {
 
@@ -24,16 +29,15 @@ using namespace m2ce;
 
 constexpr float LOG2E = 1.4426950408889634f;
 
-// act(g) and, for SLOPE, its derivative
-template <bool SLOPE> M2_DEV float act(float g, int gelu, float& slope) {
-    constexpr float C2 = 1.5957691216057308f, K = 0.044715f;
-    // (bounded: past +-100, +-20 of gelu, the sigmoid is 0 or 1 and its slope 0, not 0 inf)
-    const float lim = gelu ? 20.f : 100.f, b = __builtin_amdgcn_fmed3f(g, -lim, lim);
-    const float u = gelu ? C2 * b * fmaf(K * b, b, 1.f) : b;
+// act(g) and, for SLOPE, its derivative.  (Past +-100, +-20 of gelu, the sigmoid is 0 or 1 and its slope 0: g is bounded
+// where that multiplies it, so that no 0 inf comes of it.)
+template <bool GELU, bool SLOPE> M2_DEV float act(float g, float& slope) {
+    constexpr float C2 = 1.5957691216057308f, K = 0.044715f, LIM = GELU ? 20.f : 100.f;
+    const float u = GELU ? C2 * g * fmaf(K * g, g, 1.f) : g;
     const float s = __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(u * -LOG2E));
     if constexpr (SLOPE) {
-        const float du = gelu ? C2 * fmaf(3.f * K * b, b, 1.f) : 1.f;
-        slope = g != g ? g : fmaf(b * s * (1.f - s), du, s);
+        const float b = __builtin_amdgcn_fmed3f(g, -LIM, LIM), bs = b * s;
+        slope = fmaf(GELU ? bs * (C2 * fmaf(3.f * K * b, b, 1.f)) : bs, 1.f - s, s);
     }
     return g * s;
 }
@@ -57,16 +61,21 @@ template <typename T> M2_DEV void store_quad(T* row, int m, int64_t dim, const f
 // ---------------------------------------------------------------------------
 // forward
 // ---------------------------------------------------------------------------
-// m: pairs of the hidden size, n: token -> h, and z = [g | v] with rows of 2 fp
-template <typename T> struct EpiGlu {
+// m: pairs of the hidden size, n: token -> h, and for a gradient rows of 2 fp of v act'(g) and act(g)
+template <typename T, bool SAVE> struct EpiGlu {
     static constexpr bool SEG = false;
     T* h;
-    T* z;                    // or NULL
+    T* z;
     int64_t hidden, fp;
     int gelu;
 
     template <class S>
     M2_DEV void run(f32x4 (&acc)[S::FM][S::FN], int m0, int n0, int wm, int wn, int lane, int count, int, int) const {
+        if (gelu) with<S, true>(acc, m0, n0, wm, wn, lane, count);
+        else with<S, false>(acc, m0, n0, wm, wn, lane, count);
+    }
+    template <class S, bool GELU>
+    M2_DEV void with(f32x4 (&acc)[S::FM][S::FN], int m0, int n0, int wm, int wn, int lane, int count) const {
         static_assert(S::FM % 2 == 0, "");
         constexpr bool WIDE = S::FM % 4 == 0;
         const int f0 = m0 / 2 + wm * S::FM * 8;
@@ -79,26 +88,30 @@ template <typename T> struct EpiGlu {
 #pragma unroll
             for (int i = 0; i < S::FM; i += WIDE ? 4 : 2) {
                 const int f = f0 + 8 * i;
-                f32x4 o[WIDE ? 2 : 1];
+                constexpr int E = WIDE ? 2 : 1;
+                f32x4 o[E], by[E], at[E];
 #pragma unroll
-                for (int e = 0; e < (WIDE ? 2 : 1); ++e)
+                for (int e = 0; e < E; ++e)
 #pragma unroll
                     for (int r = 0; r < 4; ++r) {
+                        const float v = acc[i + 2 * e + 1][j][r];
                         float slope;
-                        o[e][r] = act<false>(acc[i + 2 * e][j][r], gelu, slope) * acc[i + 2 * e + 1][j][r];
+                        at[e][r] = act<GELU, SAVE>(acc[i + 2 * e][j][r], slope);
+                        o[e][r] = at[e][r] * v;
+                        if constexpr (SAVE) by[e][r] = slope * v;
                     }
                 if constexpr (WIDE) {
                     store_row(to, f, hidden, lane, o[0], o[1]);
-                    if (z) {
-                        store_row(gr, f, hidden, lane, acc[i][j], acc[i + 2][j]);
-                        store_row(gr + fp, f, hidden, lane, acc[i + 1][j], acc[i + 3][j]);
+                    if constexpr (SAVE) {
+                        store_row(gr, f, hidden, lane, by[0], by[1]);
+                        store_row(gr + fp, f, hidden, lane, at[0], at[1]);
                     }
                 } else {
                     const int q = f + 4 * (lane >> 4);
                     store_quad(to, q, hidden, o[0]);
-                    if (z) {
-                        store_quad(gr, q, hidden, acc[i][j]);
-                        store_quad(gr + fp, q, hidden, acc[i + 1][j]);
+                    if constexpr (SAVE) {
+                        store_quad(gr, q, hidden, by[0]);
+                        store_quad(gr + fp, q, hidden, at[0]);
                     }
                 }
             }
@@ -110,9 +123,9 @@ template <typename T> struct EpiGlu {
 template <typename T> struct Few;
 template <> struct Few<bf16> {
     bf16x8 v;
-    M2_DEV void load(const bf16* p, bool in) {
+    M2_DEV void load(const bf16* p) { v = *reinterpret_cast<const bf16x8*>(p); }
+    M2_DEV void keep(bool in) {
         const bf16x8 zero = {};
-        v = *reinterpret_cast<const bf16x8*>(p);
         if (!in) v = zero;
     }
     static M2_DEV f32x4 mma(const Few& a, const Few& b, f32x4 c) {
@@ -121,10 +134,12 @@ template <> struct Few<bf16> {
 };
 template <> struct Few<float> {
     u32x4 lo, hi;
-    M2_DEV void load(const float* p, bool in) {
-        const u32x4 zero = {};
+    M2_DEV void load(const float* p) {
         lo = reinterpret_cast<const u32x4*>(p)[0];
         hi = reinterpret_cast<const u32x4*>(p)[1];
+    }
+    M2_DEV void keep(bool in) {
+        const u32x4 zero = {};
         if (!in) lo = hi = zero;
     }
     M2_DEV void planes(bf16x8 (&p)[3]) const {
@@ -153,63 +168,83 @@ struct FewArgs {
     int64_t ldx, ldw, fp;
     int n, dim, hidden, gelu;
 };
-// Up to 16 MT tokens: a workgroup takes 8 of the hidden size, its NW wavefronts split K and meet in LDS.
-// The 16 rows of a matrix operand are the 8 of the gate and the 8 of the values, so that lanes
+// Up to 16 MT tokens: a workgroup takes 8 FT of the hidden size, its NW wavefronts split K and meet in LDS.
+// The 16 rows of a matrix operand are 8 of the gate and the 8 of the values, so that lanes
 // l and l + 32 hold g and v of the same place; every weight is read once, x comes from the cache.
-template <typename T, int MT, int NW>
+// U steps of 32 of K are in flight: a step's operands are loaded again, U steps on, right behind its products.
+template <typename T, int MT, int FT, int NW, int U>
 __global__ void __launch_bounds__(NW * 64) k_glu_few(FewArgs a) {
-    constexpr int U = sizeof(T) == 2 ? (MT > 2 ? 4 : 8) : MT > 2 ? 2 : 4;    // steps of 32 whose loads are issued together
-    __shared__ f32x4 red[NW][MT][64];
+    __shared__ f32x4 red[NW][FT * MT][64];
     const int lane = threadIdx.x & 63, w = wave_id();
-    const int f0 = blockIdx.x * 8, row = lane & 15, kq = (lane >> 4) * 8;
-    const T* wr = static_cast<const T*>(a.w) +
-                  ((int64_t)(row >> 3) * a.hidden + min(f0 + (row & 7), a.hidden - 1)) * a.ldw;
-    const T* xr[MT];
+    const int f0 = blockIdx.x * 8 * FT, row = lane & 15, kq = (lane >> 4) * 8;
+    const T *wr[FT], *xr[MT];
+#pragma unroll
+    for (int i = 0; i < FT; ++i)
+        wr[i] = static_cast<const T*>(a.w) +
+                ((int64_t)(row >> 3) * a.hidden + min(f0 + 8 * i + (row & 7), a.hidden - 1)) * a.ldw;
 #pragma unroll
     for (int t = 0; t < MT; ++t) xr[t] = static_cast<const T*>(a.x) + (int64_t)min(16 * t + row, a.n - 1) * a.ldx;
     const int steps = (a.dim + 31) / 32, per = (steps + NW - 1) / NW;
-    const int s1 = min(steps, (w + 1) * per);
-    f32x4 acc[MT];
+    const int s0 = w * per, s1 = min(steps, s0 + per);
+    f32x4 acc[FT][MT];
 #pragma unroll
-    for (int t = 0; t < MT; ++t) acc[t] = zero4();
-    for (int s = w * per; s < s1; s += U) {
-        Few<T> fw[U], fx[U][MT];
+    for (int i = 0; i < FT; ++i)
+#pragma unroll
+        for (int t = 0; t < MT; ++t) acc[i][t] = zero4();
+    Few<T> fw[U][FT], fx[U][MT];
+    auto load = [&](int q, int s) {
+        const int k = min(s * 32 + kq, a.dim - 8);         // (past the end of a row: its last piece, not used)
+#pragma unroll
+        for (int i = 0; i < FT; ++i) fw[q][i].load(wr[i] + k);
+#pragma unroll
+        for (int t = 0; t < MT; ++t) fx[q][t].load(xr[t] + k);
+    };
+#pragma unroll
+    for (int q = 0; q < U; ++q)
+        if (s0 + q < s1) load(q, s0 + q);
+    for (int s = s0; s < s1; s += U) {
 #pragma unroll
         for (int q = 0; q < U; ++q) {
-            const int k = (s + q) * 32 + kq;
-            const bool in = s + q < s1 && k < a.dim;
-            const int at = in ? k : 0;
-            fw[q].load(wr + at, in);
+            if (s + q >= s1) break;
+            if ((s + q) * 32 + 32 > a.dim) {               // a last step that is not whole
+                const bool in = (s + q) * 32 + kq < a.dim;
 #pragma unroll
-            for (int t = 0; t < MT; ++t) fx[q][t].load(xr[t] + at, in);
+                for (int i = 0; i < FT; ++i) fw[q][i].keep(in);
+#pragma unroll
+                for (int t = 0; t < MT; ++t) fx[q][t].keep(in);
+            }
+#pragma unroll
+            for (int i = 0; i < FT; ++i)
+#pragma unroll
+                for (int t = 0; t < MT; ++t) acc[i][t] = Few<T>::mma(fw[q][i], fx[q][t], acc[i][t]);
+            if (s + q + U < s1) load(q, s + q + U);
         }
-#pragma unroll
-        for (int q = 0; q < U; ++q)
-#pragma unroll
-            for (int t = 0; t < MT; ++t) acc[t] = Few<T>::mma(fw[q], fx[q][t], acc[t]);
     }
 #pragma unroll
-    for (int t = 0; t < MT; ++t) red[w][t][lane] = acc[t];
+    for (int i = 0; i < FT; ++i)
+#pragma unroll
+        for (int t = 0; t < MT; ++t) red[w][i * MT + t][lane] = acc[i][t];
     __syncthreads();
+    for (int p = w; p < FT * MT; p += NW) {
+        f32x4 v = red[0][p][lane];
 #pragma unroll
-    for (int t = w; t < MT; t += NW) {
-        f32x4 v = red[0][t][lane];
-#pragma unroll
-        for (int u = 1; u < NW; ++u) v += red[u][t][lane];
-        f32x4 o, other;
+        for (int u = 1; u < NW; ++u) v += red[u][p][lane];
+        f32x4 o, by, at;
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-            other[r] = __shfl_xor(v[r], 32);
+            const float other = __shfl_xor(v[r], 32);
             float slope;
-            o[r] = act<false>(v[r], a.gelu, slope) * other[r];
+            at[r] = a.gelu ? act<true, true>(v[r], slope) : act<false, true>(v[r], slope);
+            o[r] = at[r] * other;
+            by[r] = slope * other;
         }
-        const int n = 16 * t + (lane & 15), f = f0 + 4 * ((lane >> 4) & 1);
+        const int n = 16 * (p % MT) + (lane & 15), f = f0 + 8 * (p / MT) + 4 * ((lane >> 4) & 1);
         if (lane >= 32 || n >= a.n) continue;
         store_quad(static_cast<T*>(a.h) + (int64_t)n * a.hidden, f, a.hidden, o);
         if (a.z) {
             T* z = static_cast<T*>(a.z) + (int64_t)n * 2 * a.fp;
-            store_quad(z, f, a.hidden, v);
-            store_quad(z + a.fp, f, a.hidden, other);
+            store_quad(z, f, a.hidden, by);
+            store_quad(z + a.fp, f, a.hidden, at);
         }
     }
 }
@@ -240,10 +275,9 @@ template <typename T> __global__ void __launch_bounds__(256) k_glu_pack(PackArgs
 }
 
 struct DzArgs {
-    const void *z, *dh;
+    const void *z, *dh;      // as EpiGlu left it
     bf16* dz;                // [np][2 fp], zeros past n and past hidden
     int64_t n, np, hidden, fp, ldg, plane;
-    int gelu;
 };
 template <typename T> __global__ void __launch_bounds__(256) k_glu_dz(DzArgs a) {
     const int64_t per = a.fp / 8, id = (int64_t)blockIdx.x * 256 + threadIdx.x;
@@ -251,18 +285,16 @@ template <typename T> __global__ void __launch_bounds__(256) k_glu_dz(DzArgs a) 
     if (n >= a.np) return;
     float dg[8] = {0, 0, 0, 0, 0, 0, 0, 0}, dv[8] = {0, 0, 0, 0, 0, 0, 0, 0};
     if (n < a.n && c < a.hidden) {
-        float g[8], v[8], up[8];
+        float by[8], at[8], up[8];
         const T* z = static_cast<const T*>(a.z) + n * 2 * a.fp;
-        load8(z, c, a.fp, g);
-        load8(z + a.fp, c, a.fp, v);
+        load8(z, c, a.fp, by);
+        load8(z + a.fp, c, a.fp, at);
         load8(static_cast<const T*>(a.dh) + n * a.ldg, c, a.hidden, up);
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-            float slope;
-            const float s = act<true>(g[i], a.gelu, slope);
             // (past the hidden size z holds anything)
-            dv[i] = c + i < a.hidden ? up[i] * s : 0.f;
-            dg[i] = c + i < a.hidden ? up[i] * v[i] * slope : 0.f;
+            dg[i] = c + i < a.hidden ? up[i] * by[i] : 0.f;
+            dv[i] = c + i < a.hidden ? up[i] * at[i] : 0.f;
         }
     }
     bf16* to = a.dz + n * 2 * a.fp + c;
@@ -378,43 +410,48 @@ __global__ void __launch_bounds__(64) k_glu_sum(const float* part, bf16* dx, int
 // ---------------------------------------------------------------------------
 // plans
 // ---------------------------------------------------------------------------
+// Tiles of the forward's product (Z), of dx (X) and of dW (W): large, middle, small; few tokens
 template <bool F32> struct Shapes {
-    typedef Shape<256, 256, 2, 4, 2, 64, false, false, 1, true> Z256;
-    typedef Shape<128, 64, 4, 1, 3, 64, false, false, 1, true> Z64;
+    typedef Shape<256, 256, 2, 4, 2, 64, false, false, 1, true> ZL;
+    typedef Shape<256, 128, 2, 4, 2, 64, false, false, 1, true> ZM;
+    typedef Shape<128, 64, 4, 1, 3, 64, false, false, 1, true> ZS;
     typedef Shape<128, 16, 4, 1, 4, 64, false, false, 1, true> Z16;
-    typedef Shape<256, 256, 2, 4, 2, 64, true, false, 1> X256;
-    typedef Shape<256, 128, 2, 4, 2, 64, true, false, 1> X128;
+    typedef Shape<256, 256, 2, 4, 2, 64, true, false, 1> XL;
+    typedef Shape<256, 128, 2, 4, 2, 64, true, false, 1> XM;
+    typedef XM XS;
     typedef Shape<256, 64, 4, 1, 3, 64, true, false, 1> X64;
     typedef Shape<256, 16, 4, 1, 3, 64, true, false, 1> X16;
-    typedef Shape<256, 256, 2, 4, 2, 64, true, true, 1> W256;
-    typedef Shape<256, 128, 2, 4, 2, 64, true, true, 1> W128;
+    typedef Shape<256, 256, 2, 4, 2, 64, true, true, 1> WL;
+    typedef Shape<256, 128, 2, 4, 2, 64, true, true, 1> WM;
+    typedef WM WS;
 };
 template <> struct Shapes<true> {
-    typedef Shape<256, 128, 4, 2, 2, 32, false, false, 6, true> Z256;
-    typedef Shape<128, 64, 4, 2, 4, 32, false, false, 6, true> Z64;
+    typedef Shape<256, 128, 4, 2, 2, 32, false, false, 6, true> ZL;
+    typedef Shape<128, 128, 2, 4, 3, 32, false, false, 6, true> ZM;
+    typedef Shape<128, 64, 4, 2, 4, 32, false, false, 6, true> ZS;
     typedef Shape<128, 16, 4, 1, 4, 32, false, false, 6, true> Z16;
-    typedef Shape<256, 128, 4, 2, 2, 32, true, false, 6> X256;
-    typedef Shape<128, 64, 4, 2, 4, 32, true, false, 6> X128;
-    typedef Shape<256, 128, 4, 2, 2, 32, true, true, 6> W256;
-    typedef Shape<128, 64, 4, 2, 4, 32, true, true, 6> W128;
+    typedef Shape<256, 128, 4, 2, 2, 32, true, false, 6> XL;
+    typedef Shape<128, 128, 2, 4, 3, 32, true, false, 6> XM;
+    typedef Shape<128, 64, 4, 2, 4, 32, true, false, 6> XS;
+    typedef Shape<256, 128, 4, 2, 2, 32, true, true, 6> WL;
+    typedef Shape<128, 128, 2, 4, 3, 32, true, true, 6> WM;
+    typedef Shape<128, 64, 4, 2, 4, 32, true, true, 6> WS;
 };
 
-// The rounds of tiles over the CUs that a shape takes, in 5 ns: the small shapes are slower a step, but
-// fewer of the CUs stay without a tile
+// The time of a step of K, in 5 ns, of all rounds of tiles over the CUs
 template <class S> int64_t rounds(int64_t m, int64_t n) {
     const int64_t ncu = m2::cu_count();
     return S::STEP * (((int64_t)tiles(m, S::BM) * tiles(n, S::BN) + ncu - 1) / ncu);
 }
-
 // What both entry points share: how the operands are read
 struct Common {
     int64_t n, np, dim, hidden, dp, fp;
     bool f32, pack_x, pack_w;
-    size_t x, w, at;
+    size_t z, x, w, at;
 };
-// rows: K runs along the rows of both (the gradients) or along dim only
+// save: with what a gradient reads, whose K runs along the rows of both operands too, and not along dim only
 Common common(int64_t n, int64_t dim, int64_t hidden, int64_t ldx, int64_t ldw, const void* x, const void* w, int dtype,
-              bool rows) {
+              bool save) {
     Common c{};
     c.n = n; c.dim = dim; c.hidden = hidden;
     c.np = (n + 63) / 64 * 64;
@@ -426,26 +463,28 @@ Common common(int64_t n, int64_t dim, int64_t hidden, int64_t ldx, int64_t ldw, 
         return !c.f32 && dim % 64 == 0 && ld % 8 == 0 && al16(p) && ld <= (1 << 22) && ld * (apart + 256) < (1ll << 31);
     };
     c.pack_x = !direct(x, ldx, 0);
-    c.pack_w = !direct(w, ldw, hidden) || (rows && hidden % 64);
+    c.pack_w = !direct(w, ldw, hidden) || (save && hidden % 64);
     auto take = [&](size_t b) { const size_t r = c.at; c.at += align256(b); return r; };
     const size_t planes = c.f32 ? 3 : 1;
+    c.z = save ? take((size_t)(c.f32 ? 4 : 2) * n * 2 * c.fp) : 0;
     c.x = c.pack_x ? take(2 * planes * (size_t)c.np * c.dp) : c.at;
     c.w = c.pack_w ? take(2 * planes * (size_t)2 * c.fp * c.dp) : c.at;
     return c;
 }
 
-template <typename T> Operand operand_x(char* ws, const Common& c, const void* x, int64_t ldx, hipStream_t s) {
+// (pack: they are not there yet)
+template <typename T> Operand operand_x(char* ws, const Common& c, const void* x, int64_t ldx, bool pack, hipStream_t s) {
     if (!c.pack_x) return Operand{static_cast<const bf16*>(x), ldx, 0, (int)c.n, (int)c.dim};
     bf16* to = reinterpret_cast<bf16*>(ws + c.x);
     const PackArgs a{x, to, c.np, c.dim, ldx, c.dp, c.np * c.dp, 0, c.n};
-    hipLaunchKernelGGL(k_glu_pack<T>, dim3((unsigned)((c.np + 3) / 4)), dim3(256), 0, s, a);
+    if (pack) hipLaunchKernelGGL(k_glu_pack<T>, dim3((unsigned)((c.np + 3) / 4)), dim3(256), 0, s, a);
     return Operand{to, c.dp, c.np * c.dp, (int)c.np, (int)c.dp};
 }
-template <typename T> Operand operand_w(char* ws, const Common& c, const void* w, int64_t ldw, hipStream_t s) {
+template <typename T> Operand operand_w(char* ws, const Common& c, const void* w, int64_t ldw, bool pack, hipStream_t s) {
     if (!c.pack_w) return Operand{static_cast<const bf16*>(w), ldw, 0, (int)c.hidden, (int)c.dim, (int)c.hidden};
     bf16* to = reinterpret_cast<bf16*>(ws + c.w);
     const PackArgs a{w, to, 2 * c.fp, c.dim, ldw, c.dp, 2 * c.fp * c.dp, c.fp, c.hidden};
-    hipLaunchKernelGGL(k_glu_pack<T>, dim3((unsigned)(2 * c.fp / 4)), dim3(256), 0, s, a);
+    if (pack) hipLaunchKernelGGL(k_glu_pack<T>, dim3((unsigned)(2 * c.fp / 4)), dim3(256), 0, s, a);
     return Operand{to, c.dp, 2 * c.fp * c.dp, (int)c.fp, (int)c.dp, (int)c.fp};
 }
 
@@ -464,52 +503,86 @@ int check_sizes(const char* who, int64_t n, int64_t dim, int64_t hidden, int64_t
 }
 
 // 16-byte pieces along K that a lane loads by itself
-bool few(const m2_gated_linear_args& a) {
-    const int64_t e = 8, es = a.dtype == M2_F32 ? 4 : 2;
-    return a.n <= 64 && a.dim % e == 0 && a.ldx * es % 16 == 0 && a.ldw * es % 16 == 0 && al16(a.x) && al16(a.weight);
+template <class A> bool few(const A& a) {
+    const int64_t es = a.dtype == M2_F32 ? 4 : 2;
+    return a.n <= 64 && a.dim % 8 == 0 && a.ldx * es % 16 == 0 && a.ldw * es % 16 == 0 && al16(a.x) && al16(a.weight);
+}
+template <class A> Common common_of(const A& a, bool save) {
+    return common(a.n, a.dim, a.hidden, a.ldx, a.ldw, a.x, a.weight, a.dtype, save);
 }
 
 template <typename T> void run_few(const m2_gated_linear_args& a, hipStream_t s) {
     const FewArgs k{a.x, a.weight, a.out, a.saved, a.ldx, a.ldw, (a.hidden + 63) / 64 * 64,
                     (int)a.n, (int)a.dim, (int)a.hidden, a.activation == M2_GELU};
-    const unsigned wgs = (unsigned)((a.hidden + 7) / 8);
     auto go = [&](auto mt) {
         constexpr int MT = decltype(mt)::value;
-        // enough wavefronts for ~2048 over the chip
-        if (wgs >= 512) hipLaunchKernelGGL((k_glu_few<T, MT, 4>), dim3(wgs), dim3(256), 0, s, k);
-        else hipLaunchKernelGGL((k_glu_few<T, MT, 8>), dim3(wgs), dim3(512), 0, s, k);
+        auto with = [&](auto ft, auto nw, auto u) {
+            constexpr int FT = decltype(ft)::value, NW = decltype(nw)::value, U = decltype(u)::value;
+            hipLaunchKernelGGL((k_glu_few<T, MT, FT, NW, U>), dim3((unsigned)((a.hidden + 8 * FT - 1) / (8 * FT))), dim3(NW * 64), 0, s, k);
+        };
+        typedef std::integral_constant<int, 1> one;
+        typedef std::integral_constant<int, 2> two;
+        typedef std::integral_constant<int, 4> four;
+        typedef std::integral_constant<int, 8> eight;
+#ifdef TUNE
+        const int e = getenv("FEW") ? atoi(getenv("FEW")) : 0;
+        switch (e) {
+            case 0: with(one(), four(), eight()); break;
+            case 1: with(one(), eight(), four()); break;
+            case 2: with(two(), four(), four()); break;
+            case 3: with(two(), eight(), four()); break;
+            case 4: with(four(), four(), four()); break;
+            case 5: with(four(), eight(), two()); break;
+            case 6: with(four(), four(), two()); break;
+            case 7: with(two(), four(), eight()); break;
+            case 8: with(four(), eight(), four()); break;
+            case 9: with(two(), eight(), two()); break;
+        }
+#else
+        // More of the hidden size for each workgroup reads x less often, as long as there are workgroups for most
+        // CUs: 16 tokens x 2560 x 6912 by 8, 16, 32: 29, 24, 22 us, 2048 x 1024: 6.6, 8.0, 11.7.
+        const int64_t wgs = (a.hidden + 7) / 8;
+        if (wgs < 2 * 192) with(one(), eight(), four());
+        else if (wgs < 4 * 192) with(two(), eight(), two());
+        else if constexpr (sizeof(T) == 4 && MT < 4) with(four(), eight(), two());
+        else with(four(), four(), two());
+#endif
     };
     if (a.n <= 16) go(std::integral_constant<int, 1>());
     else if (a.n <= 32) go(std::integral_constant<int, 2>());
     else go(std::integral_constant<int, 4>());
 }
 
-template <bool F32> int run_fwd(const m2_gated_linear_args& a, const Common& c, hipStream_t s) {
+template <bool F32, bool SAVE> int run_fwd(const m2_gated_linear_args& a, const Common& c, hipStream_t s) {
     typedef typename std::conditional<F32, float, bf16>::type T;
     typedef Shapes<F32> P;
-    char* ws = static_cast<char*>(a.workspace);
+    char* ws = static_cast<char*>(SAVE ? a.saved : a.workspace);
     Gemm g{};
     g.n = (int)c.n; g.splits = 1;
     g.nk = (int)(c.dp / 64);
-    g.b = operand_x<T>(ws, c, a.x, a.ldx, s);
-    g.a = operand_w<T>(ws, c, a.weight, a.ldw, s);
-    const EpiGlu<T> e{static_cast<T*>(a.out), static_cast<T*>(a.saved), c.hidden, c.fp, a.activation == M2_GELU};
+    g.b = operand_x<T>(ws, c, a.x, a.ldx, true, s);
+    g.a = operand_w<T>(ws, c, a.weight, a.ldw, true, s);
+    const EpiGlu<T, SAVE> e{static_cast<T*>(a.out), reinterpret_cast<T*>(ws + c.z), c.hidden, c.fp, a.activation == M2_GELU};
+    const int64_t m = 2 * ((c.hidden + 15) / 16 * 16);
     auto go = [&](auto shape) {
         typedef decltype(shape) S;
-        g.tm = tiles(2 * ((c.hidden + 15) / 16 * 16), S::BM);
+        g.tm = tiles(m, S::BM);
         g.tn = tiles(c.n, S::BN);
         launch<S>(g, e, s);
     };
+    const int64_t l = rounds<typename P::ZL>(m, c.n), md = rounds<typename P::ZM>(m, c.n), sm = rounds<typename P::ZS>(m, c.n);
     if (c.n <= 16) go(typename P::Z16());
-    else if (c.n <= 64 || rounds<typename P::Z64>(2 * c.hidden, c.n) < rounds<typename P::Z256>(2 * c.hidden, c.n)) go(typename P::Z64());
-    else go(typename P::Z256());
+    else if (c.n <= 64 || (sm < md && sm < l)) go(typename P::ZS());
+    else if (md < l) go(typename P::ZM());
+    else go(typename P::ZL());
     return m2::check_launch("gated_linear");
 }
 
 struct BwdPlan {
     Common c;
     size_t dz, part, total;
-    int x;                   // dx: 0 the large tiles, 1 the small, 64 / 16 k_ce_stream's
+    bool pack;               // the operands are packed here, in the workspace; else they are in saved
+    int x;                   // dx: 0 the large tiles, 1 the middle, 2 the small, 64 / 16 k_ce_stream's
     int w;                   // dW: the same
     int splits;
 };
@@ -519,9 +592,11 @@ template <class S> Deal deal_of(int64_t m, int64_t n, int64_t k) {
 template <bool F32> BwdPlan plan_bwd(const m2_gated_linear_grad_args& a) {
     typedef Shapes<F32> P;
     BwdPlan p{};
-    p.c = common(a.n, a.dim, a.hidden, a.ldx, a.ldw, a.x, a.weight, a.dtype, true);
+    p.c = common_of(a, true);
     const Common& c = p.c;
-    size_t at = c.at;
+    // (the forward of few tokens packs nothing)
+    p.pack = few(a);
+    size_t at = p.pack ? c.at : 0;
     auto take = [&](size_t b) { const size_t r = at; at += align256(b); return r; };
     p.dz = take(2 * (size_t)(F32 ? 3 : 1) * c.np * 2 * c.fp);
     // (the two products run one after the other and share the parts' buffer)
@@ -530,13 +605,15 @@ template <bool F32> BwdPlan plan_bwd(const m2_gated_linear_grad_args& a) {
         const size_t b = d.s > 1 ? 4 * tile * d.rest * d.s : 0;
         if (b > need) need = b;
     };
-    auto choose = [&](auto large, auto small, int64_t m, int64_t n, int64_t k) {
+    auto choose = [&](auto large, auto middle, auto small, int64_t m, int64_t n, int64_t k) {
         typedef decltype(large) A;
-        typedef decltype(small) B;
-        const Deal da = deal_of<A>(m, n, k), db = deal_of<B>(m, n, k);
-        if (da.cost <= db.cost) { parts(da, (size_t)A::BM * A::BN); return 0; }
-        parts(db, (size_t)B::BM * B::BN);
-        return 1;
+        typedef decltype(middle) B;
+        typedef decltype(small) S;
+        const Deal da = deal_of<A>(m, n, k), db = deal_of<B>(m, n, k), ds = deal_of<S>(m, n, k);
+        if (da.cost <= db.cost && da.cost <= ds.cost) { parts(da, (size_t)A::BM * A::BN); return 0; }
+        if (db.cost <= ds.cost) { parts(db, (size_t)B::BM * B::BN); return 1; }
+        parts(ds, (size_t)S::BM * S::BN);
+        return 2;
     };
     if (a.grad_x) {
         if (!F32 && c.n <= 64) {
@@ -551,10 +628,10 @@ template <bool F32> BwdPlan plan_bwd(const m2_gated_linear_grad_args& a) {
             }
             need = 4 * (size_t)p.splits * c.np * c.dp;
         } else {
-            p.x = choose(typename P::X256(), typename P::X128(), c.dim, c.n, 2 * c.fp);
+            p.x = choose(typename P::XL(), typename P::XM(), typename P::XS(), c.dim, c.n, 2 * c.fp);
         }
     }
-    if (a.grad_weight) p.w = choose(typename P::W256(), typename P::W128(), c.dim, 2 * c.fp, c.np);
+    if (a.grad_weight) p.w = choose(typename P::WL(), typename P::WM(), typename P::WS(), c.dim, 2 * c.fp, c.np);
     p.part = take(need);
     p.total = at;
     return p;
@@ -564,11 +641,12 @@ template <bool F32> int run_bwd(const m2_gated_linear_grad_args& a, const BwdPla
     typedef typename std::conditional<F32, float, bf16>::type T;
     typedef Shapes<F32> P;
     char* ws = static_cast<char*>(a.workspace);
+    char* packed = p.pack ? ws : static_cast<char*>(const_cast<void*>(a.saved));
     const Common& c = p.c;
     bf16* dz = reinterpret_cast<bf16*>(ws + p.dz);
     float* part = reinterpret_cast<float*>(ws + p.part);
     const int64_t plane = c.np * 2 * c.fp;
-    const DzArgs d{a.saved, a.grad_out, dz, c.n, c.np, c.hidden, c.fp, a.ldg, plane, a.activation == M2_GELU};
+    const DzArgs d{a.saved, a.grad_out, dz, c.n, c.np, c.hidden, c.fp, a.ldg, plane};
     hipLaunchKernelGGL(k_glu_dz<T>, dim3((unsigned)((c.np * (c.fp / 8) + 255) / 256)), dim3(256), 0, s, d);
     auto product = [&](auto shape, Gemm g, int64_t m, int64_t n, int64_t k, const Out<T>& out) {
         typedef decltype(shape) S;
@@ -588,12 +666,12 @@ template <bool F32> int run_bwd(const m2_gated_linear_grad_args& a, const BwdPla
     if (a.grad_x) {
         Gemm g{};
         g.n = (int)c.n;
-        g.a = operand_w<T>(ws, c, a.weight, a.ldw, s);
+        g.a = operand_w<T>(packed, c, a.weight, a.ldw, p.pack, s);
         g.a.lim = g.a.klim;                  // read by columns
         g.a.klim = (int)(2 * c.fp);
         g.b = Operand{dz, 2 * c.fp, plane, (int)c.np, (int)(2 * c.fp)};
         const Out<T> out{static_cast<T*>(a.grad_x), c.dim, 0, (int)c.n};
-        if (p.x > 1) {
+        if (p.x > 2) {
             if constexpr (!F32) {
                 g.tm = tiles(c.dim, 256);
                 g.tn = 1;
@@ -606,21 +684,24 @@ template <bool F32> int run_bwd(const m2_gated_linear_grad_args& a, const BwdPla
                                    static_cast<bf16*>(a.grad_x), c.np, c.dp, c.dim, p.splits);
             }
         } else if (p.x == 0) {
-            product(typename P::X256(), g, c.dim, c.n, 2 * c.fp, out);
-        } else {
-            product(typename P::X128(), g, c.dim, c.n, 2 * c.fp, out);
+            product(typename P::XL(), g, c.dim, c.n, 2 * c.fp, out);
+        } else if (p.x == 1) {
+            product(typename P::XM(), g, c.dim, c.n, 2 * c.fp, out);
+        } else if constexpr (F32) {
+            product(typename P::XS(), g, c.dim, c.n, 2 * c.fp, out);
         }
     }
     if (a.grad_weight) {
         Gemm g{};
         g.n = (int)(2 * c.fp);
-        g.a = operand_x<T>(ws, c, a.x, a.ldx, s);
+        g.a = operand_x<T>(packed, c, a.x, a.ldx, p.pack, s);
         g.a.klim = g.a.lim;                  // read by columns; zero rows of dz stand against the repeated last row
         g.a.lim = (int)c.dp;
         g.b = Operand{dz, 2 * c.fp, plane, (int)(2 * c.fp), (int)c.np};
         const Out<T> out{static_cast<T*>(a.grad_weight), c.dim, (int)c.fp, (int)c.hidden};
-        if (p.w == 0) product(typename P::W256(), g, c.dim, 2 * c.fp, c.np, out);
-        else product(typename P::W128(), g, c.dim, 2 * c.fp, c.np, out);
+        if (p.w == 0) product(typename P::WL(), g, c.dim, 2 * c.fp, c.np, out);
+        else if (p.w == 1) product(typename P::WM(), g, c.dim, 2 * c.fp, c.np, out);
+        else if constexpr (F32) product(typename P::WS(), g, c.dim, 2 * c.fp, c.np, out);
     }
     return m2::check_launch("gated_linear_grad");
 }
@@ -631,14 +712,14 @@ namespace m2 {
 
 size_t gated_linear_saved(const m2_gated_linear_args& a) {
     if (check_sizes("gated_linear", a.n, a.dim, a.hidden, a.ldx, a.ldw, a.dtype, a.activation)) return 0;
-    const size_t b = m2_dtype_size(a.dtype) * (size_t)a.n * 2 * ((a.hidden + 63) / 64 * 64);
+    const Common c = common_of(a, true);
+    const size_t b = few(a) ? c.x : c.at;      // z stands first
     return b ? b : 256;
 }
 
 size_t gated_linear_workspace(const m2_gated_linear_args& a) {
     if (check_sizes("gated_linear", a.n, a.dim, a.hidden, a.ldx, a.ldw, a.dtype, a.activation)) return 0;
-    if (few(a)) return 256;
-    const size_t b = common(a.n, a.dim, a.hidden, a.ldx, a.ldw, a.x, a.weight, a.dtype, false).at;
+    const size_t b = a.saved || few(a) ? 0 : common_of(a, false).at;
     return b ? b : 256;
 }
 
@@ -654,10 +735,11 @@ int launch_gated_linear(const m2_gated_linear_args& a, hipStream_t s) {
         else run_few<bf16>(a, s);
         return check_launch(who);
     }
-    const Common c = common(a.n, a.dim, a.hidden, a.ldx, a.ldw, a.x, a.weight, a.dtype, false);
+    const Common c = common_of(a, a.saved != nullptr);
+    if (a.saved) return c.f32 ? run_fwd<true, true>(a, c, s) : run_fwd<false, true>(a, c, s);
     M2_REQUIRE(c.at == 0 || (a.workspace && a.workspace_bytes >= c.at), M2_ERR_WORKSPACE,
                "%s: workspace of %zu bytes needed, %zu given", who, c.at, a.workspace_bytes);
-    return c.f32 ? run_fwd<true>(a, c, s) : run_fwd<false>(a, c, s);
+    return c.f32 ? run_fwd<true, false>(a, c, s) : run_fwd<false, false>(a, c, s);
 }
 
 static BwdPlan plan(const m2_gated_linear_grad_args& a) {
@@ -678,6 +760,8 @@ int launch_gated_linear_grad(const m2_gated_linear_grad_args& a, hipStream_t s) 
     M2_REQUIRE(a.x && a.weight && a.saved && a.grad_out && (a.grad_x || a.grad_weight), M2_ERR_INVALID,
                "%s: x, weight, saved, grad_out and an output are required", who);
     const BwdPlan p = plan(a);
+    M2_REQUIRE(a.saved_bytes >= (p.pack ? p.c.x : p.c.at), M2_ERR_WORKSPACE, "%s: saved of %zu bytes needed, %zu given",
+               who, p.pack ? p.c.x : p.c.at, a.saved_bytes);
     M2_REQUIRE(a.workspace && a.workspace_bytes >= p.total, M2_ERR_WORKSPACE,
                "%s: workspace of %zu bytes needed, %zu given", who, p.total, a.workspace_bytes);
     return a.dtype == M2_F32 ? run_bwd<true>(a, p, s) : run_bwd<false>(a, p, s);

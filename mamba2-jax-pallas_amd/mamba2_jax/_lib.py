@@ -221,7 +221,8 @@ class GatedLinearArgs(ctypes.Structure):
 
 
 class GatedLinearGradArgs(ctypes.Structure):
-    _fields_ = [("x", _c_p), ("weight", _c_p), ("saved", _c_p), ("grad_out", _c_p),
+    _fields_ = [("x", _c_p), ("weight", _c_p), ("saved", _c_p),
+                ("saved_bytes", ctypes.c_size_t), ("grad_out", _c_p),
                 ("grad_x", _c_p), ("grad_weight", _c_p), ("n", _i64), ("dim", _i64),
                 ("hidden", _i64), ("ldx", _i64), ("ldw", _i64), ("ldg", _i64), ("dtype", _i32),
                 ("activation", _i32), ("workspace", _c_p), ("workspace_bytes", ctypes.c_size_t)]

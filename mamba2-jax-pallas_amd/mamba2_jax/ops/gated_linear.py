@@ -16,14 +16,14 @@ from .embedding import _rows, _stride
 
 
 def _forward(x, weight, activation, save):
-    """-> (h, what the gradient reads or None)"""
+    """-> (h, x and weight as they are read, what else the gradient reads or None)"""
     dev, dim = weight.device, weight.shape[1]
     hidden = weight.shape[0] // 2
     xr, w = _rows(x, dim), _rows(weight, dim)
     n = xr.shape[0]
     h = torch.empty((*x.shape[:-1], hidden), dtype=x.dtype, device=dev)
     if n == 0:
-        return h, None
+        return h, xr, w, None
     args = L.GatedLinearArgs(xr.data_ptr(), w.data_ptr(), h.data_ptr(), n, dim, hidden,
                              _stride(xr, dim), _stride(w, dim), L.dtype_code(w, "weight"), activation)
     saved = None
@@ -32,26 +32,24 @@ def _forward(x, weight, activation, save):
         saved = torch.empty(size, dtype=torch.uint8, device=dev)
         args.saved, args.saved_bytes = saved.data_ptr(), size
     L.call_with_workspace("m2_gated_linear", args, dev)
-    return h, saved
+    return h, xr, w, saved
 
 
 def _backward(ctx, grad):
-    x, weight, saved = ctx.saved_tensors
+    xr, w, saved = ctx.saved_tensors
     want_x, want_w = ctx.needs_input_grad[:2]
-    dim = weight.shape[1]
-    hidden = weight.shape[0] // 2
-    dx = torch.empty(x.shape, dtype=x.dtype, device=x.device) if want_x else None
-    dw = torch.empty(weight.shape, dtype=weight.dtype, device=x.device) if want_w else None
-    xr, w = _rows(x, dim), _rows(weight, dim)
+    dim, hidden = w.shape[1], w.shape[0] // 2
+    dx = torch.empty(ctx.shape, dtype=w.dtype, device=w.device) if want_x else None
+    dw = torch.empty(w.shape, dtype=w.dtype, device=w.device) if want_w else None
     n = xr.shape[0]
     if n == 0:
         return dx, None if dw is None else dw.zero_(), None
     g = _rows(grad, hidden)
     args = L.GatedLinearGradArgs(
-        xr.data_ptr(), w.data_ptr(), saved.data_ptr(), g.data_ptr(), L.ptr(dx), L.ptr(dw), n, dim,
+        xr.data_ptr(), w.data_ptr(), saved.data_ptr(), saved.numel(), g.data_ptr(), L.ptr(dx), L.ptr(dw), n, dim,
         hidden, _stride(xr, dim), _stride(w, dim), _stride(g, hidden), L.dtype_code(w, "weight"),
         ctx.activation)
-    L.call_with_workspace("m2_gated_linear_grad", args, weight.device)
+    L.call_with_workspace("m2_gated_linear_grad", args, w.device)
     return dx, dw, None
 
 
@@ -61,9 +59,10 @@ _backward_once = once_differentiable(_backward)
 class _GatedLinear(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, activation):
-        h, saved = _forward(x, weight, activation, True)
-        ctx.save_for_backward(x, weight, saved)
-        ctx.activation = activation
+        h, xr, w, saved = _forward(x, weight, activation, True)
+        # (the rows that were read: the same strides and alignment decide what lies in `saved`)
+        ctx.save_for_backward(xr, w, saved)
+        ctx.shape, ctx.activation = x.shape, activation
         return h
 
     @staticmethod
@@ -81,8 +80,10 @@ def gated_linear(x, weight, activation="silu"):
 
     Sums and the activation are float32, h is rounded once; float32 operands are multiplied as three
     bfloat16 parts each, accurate to about 2^-24 of each product (an infinity among them gives
-    NaN).  Between the two the graph holds x, weight and both products in their dtype; the gradient of
-    bfloat16 operands is taken through those, and rounds the gradients of the products to bfloat16 once.
+    NaN).  Between the two the graph holds x, weight, act(g) and v act'(g) of the two products g and v in
+    their dtype, and a packed copy of the operands that the kernels cannot read in place (float32, as three bfloat16
+    parts: 1.5 times each; a dim or hidden that 64 does not divide); the gradient of bfloat16 operands
+    rounds its products with those to bfloat16 once more.
     Equal inputs give equal bits."""
     dev = L.device_of_two(x, weight)
     shape = x.shape

@@ -98,7 +98,7 @@ def test_gated_linear_refusals():
     name = "m2_gated_linear"
     need = lib.m2_gated_linear_workspace_size(ctypes.byref(mk()))
     saved = lib.m2_gated_linear_saved_size(ctypes.byref(mk()))
-    assert need > 0 and saved == 100 * 2 * 64 * 2
+    assert need > 0 and saved >= 100 * 2 * 64 * 2
     far = dict(ldx=1 << 22, ldw=1 << 22)
     for bad in (dict(n=-1), dict(n=1 << 30), dict(dim=0), dict(dim=1 << 21), dict(hidden=0), dict(hidden=1 << 28)):
         assert lib.m2_gated_linear_workspace_size(ctypes.byref(mk(**{**far, **bad}))) == 0
@@ -115,8 +115,8 @@ def test_gated_linear_refusals():
     refused(name, mk(workspace_bytes=need), -4, "workspace")
     refused(name, mk(workspace=4096, workspace_bytes=need, saved=4096, saved_bytes=saved - 1), -4, "saved")
     assert lib.m2_gated_linear(ctypes.byref(mk(n=0, x=None)), None) == 0
-    okg = {k: v for k, v in ok.items() if k != "out"} | dict(saved=4096, grad_out=4096, grad_x=4096, grad_weight=4096,
-                                                            ldg=30)
+    okg = {k: v for k, v in ok.items() if k != "out"} | dict(saved=4096, saved_bytes=saved, grad_out=4096, grad_x=4096,
+                                                            grad_weight=4096, ldg=30)
     mg = lambda **k: L.GatedLinearGradArgs(**{**okg, **k})
     name = "m2_gated_linear_grad"
     need = lib.m2_gated_linear_grad_workspace_size(ctypes.byref(mg()))
@@ -126,6 +126,7 @@ def test_gated_linear_refusals():
     for p in ("x", "weight", "saved", "grad_out"):
         refused(name, mg(**{p: None}), -1, "required")
     refused(name, mg(grad_x=None, grad_weight=None), -1, "required")
+    refused(name, mg(workspace=4096, workspace_bytes=need, saved_bytes=saved - 1), -4, "saved")
     refused(name, mg(workspace=4096, workspace_bytes=need - 1), -4, "workspace")
 
 

@@ -43,7 +43,7 @@ constexpr uint32_t NOWHERE = 0xfffffff0u;      // an offset past every end
 template <typename T, int V> struct Raw;
 template <> struct Raw<bf16, 2> {
     uint32_t v;
-    M2_DEV void load(Rsrc r, uint32_t off, uint32_t soff) { v = __builtin_amdgcn_raw_buffer_load_b32(r, off, soff, 0); }
+    template <int AUX> M2_DEV void load(Rsrc r, uint32_t off, uint32_t soff) { v = __builtin_amdgcn_raw_buffer_load_b32(r, off, soff, AUX); }
     M2_DEV void fill(float f) { v = pk_bf16(f, f); }
     M2_DEV float get(int i) const { return i ? bf16_hi(v) : bf16_lo(v); }
     template <int AUX> static M2_DEV void store(Rsrc r, uint32_t off, uint32_t soff, const float (&f)[2]) {
@@ -53,7 +53,7 @@ template <> struct Raw<bf16, 2> {
 template <> struct Raw<float, 2> {
     typedef uint32_t pair __attribute__((ext_vector_type(2)));
     pair v;
-    M2_DEV void load(Rsrc r, uint32_t off, uint32_t soff) { v = __builtin_amdgcn_raw_buffer_load_b64(r, off, soff, 0); }
+    template <int AUX> M2_DEV void load(Rsrc r, uint32_t off, uint32_t soff) { v = __builtin_amdgcn_raw_buffer_load_b64(r, off, soff, AUX); }
     M2_DEV void fill(float f) { v[0] = v[1] = __float_as_uint(f); }
     M2_DEV float get(int i) const { return __uint_as_float(v[i]); }
     template <int AUX> static M2_DEV void store(Rsrc r, uint32_t off, uint32_t soff, const float (&f)[2]) {
@@ -62,8 +62,8 @@ template <> struct Raw<float, 2> {
 };
 template <> struct Raw<bf16, 1> {
     uint32_t v;
-    M2_DEV void load(Rsrc r, uint32_t off, uint32_t soff) {
-        v = (uint32_t)(uint16_t)__builtin_amdgcn_raw_buffer_load_b16(r, off, soff, 0) << 16;
+    template <int AUX> M2_DEV void load(Rsrc r, uint32_t off, uint32_t soff) {
+        v = (uint32_t)(uint16_t)__builtin_amdgcn_raw_buffer_load_b16(r, off, soff, AUX) << 16;
     }
     M2_DEV void fill(float f) { v = __float_as_uint(f); }
     M2_DEV float get(int) const { return __uint_as_float(v); }
@@ -73,7 +73,7 @@ template <> struct Raw<bf16, 1> {
 };
 template <> struct Raw<float, 1> {
     uint32_t v;
-    M2_DEV void load(Rsrc r, uint32_t off, uint32_t soff) { v = __builtin_amdgcn_raw_buffer_load_b32(r, off, soff, 0); }
+    template <int AUX> M2_DEV void load(Rsrc r, uint32_t off, uint32_t soff) { v = __builtin_amdgcn_raw_buffer_load_b32(r, off, soff, AUX); }
     M2_DEV void fill(float f) { v = __float_as_uint(f); }
     M2_DEV float get(int) const { return __uint_as_float(v); }
     template <int AUX> static M2_DEV void store(Rsrc r, uint32_t off, uint32_t soff, const float (&f)[1]) {
@@ -171,7 +171,9 @@ template <int V, int LC, int TS, int W> struct Place {
     bool whole, half;
     M2_DEV Place(const RecArgs& a) {
         lane = threadIdx.x & 63;
-        const int id = xcd_remap(blockIdx.x, gridDim.x);
+        // Neighbouring slabs to one XCD where there is one pass; to all in turn where there are segments (8 x 2048 x 5120
+        // forward 176 us so, 191 in turn; 16384 x 2560 127 so, 120 in turn)
+        const int id = a.segments == 1 ? xcd_remap(blockIdx.x, gridDim.x) : blockIdx.x;
         const int of = __builtin_amdgcn_readfirstlane(id / a.slabs);
         b = __builtin_amdgcn_readfirstlane(of / a.segments);
         segment = of - b * a.segments;
@@ -205,15 +207,17 @@ template <typename T, int V> struct Stream {
     M2_DEV void move(int64_t steps) { base += steps * st; }
     // last: the row's last step, counted from the tile's first
     M2_DEV Rsrc tile(int last) const { return rsrc(base, last * st + row); }
-    template <int TS> M2_DEV void load(Raw<T, V> (&r)[TS], int last) const {
+    template <int AUX, int TS> M2_DEV void load(Raw<T, V> (&r)[TS], int last) const {
         const Rsrc t = tile(last);
 #pragma unroll
-        for (int j = 0; j < TS; ++j) r[j].load(t, off, j * st);
+        for (int j = 0; j < TS; ++j) r[j].template load<AUX>(t, off, j * st);
     }
 };
-// NT: non-temporal stores
-template <typename T, int V, bool NT> struct Output : Stream<T, V> {
-    static constexpr int AUX = NT ? 2 : 0;
+// how a walk goes past the caches: not at all, its stores, its loads too (buffer accesses' nt bit)
+enum { CACHED, STORES_NT, ALL_NT };
+constexpr int NT_BIT = 2;
+template <typename T, int V, int NT> struct Output : Stream<T, V> {
+    static constexpr int AUX = NT != CACHED ? NT_BIT : 0;
     uint32_t whole, half;    // where this lane stores all of its channels, or the last alone
     bool odd;
     template <class P> M2_DEV Output(const void* p, int64_t offset, const RecArgs& a, const P& at)
@@ -288,9 +292,10 @@ template <int D, int LC, bool SEQ> M2_DEV Map<SEQ> scan(Map<SEQ>& m, int lane) {
 }
 
 // AGG: only the map of the segment is wanted (a.agg)
-template <typename T, int V, int LC, int TS, int W, bool SEQ, bool AGG, bool NT>
+template <typename T, int V, int LC, int TS, int W, bool SEQ, bool AGG, int NT>
 __global__ void __launch_bounds__(W * 64, 4) k_rec_forward(RecArgs a) {
     typedef Place<V, LC, TS, W> P;
+    constexpr int LD = NT == ALL_NT ? NT_BIT : 0;
     __shared__ float2 tot[3][W][P::C];
     const P at(a);
     if (AGG && at.segment == a.segments - 1) return;     // (nothing follows it)
@@ -325,9 +330,9 @@ __global__ void __launch_bounds__(W * 64, 4) k_rec_forward(RecArgs a) {
     } one, two, three;
     auto load = [&](Tile& n, int64_t t0) {
         const int last = last_of(t0);
-        sx.load(n.x, last);
-        sr.load(n.r, last);
-        si.load(n.i, last);
+        sx.template load<LD>(n.x, last);
+        sr.template load<LD>(n.r, last);
+        si.template load<LD>(n.i, last);
         n.s.load(seq + t0, t0 == 0, at, last);
         sx.move(P::TILE);
         sr.move(P::TILE);
@@ -461,8 +466,8 @@ __global__ void __launch_bounds__(W * 64, 4) k_rec_back_agg(RecArgs a) {
     } one, two, three;
     auto load = [&](Tile& n, int64_t t0) {
         const int last = last_of(t0);
-        sr.load(n.r, last);
-        sg.load(n.g, last);
+        sr.template load<0>(n.r, last);
+        sg.template load<0>(n.g, last);
         n.s.load(seq + t0, t0 == 0, at, last);
         sr.move(-P::TILE);
         sg.move(-P::TILE);
@@ -526,9 +531,10 @@ __global__ void __launch_bounds__(W * 64, 4) k_rec_back_agg(RecArgs a) {
     at.put(a.agg + at.agg(a, at.segment), o);
 }
 
-template <typename T, int V, int LC, int TS, int W, bool SEQ, bool NT>
+template <typename T, int V, int LC, int TS, int W, bool SEQ, int NT>
 __global__ void __launch_bounds__(W * 64, 2) k_rec_backward(RecArgs a) {
     typedef Place<V, LC, TS, W> P;
+    constexpr int LD = NT == ALL_NT ? NT_BIT : 0;
     static_assert(P::TILE % SPAN == 0, "");
     __shared__ float tot[3][3][W][P::C];
     const P at(a);
@@ -564,10 +570,10 @@ __global__ void __launch_bounds__(W * 64, 2) k_rec_backward(RecArgs a) {
     } one, two, three;
     auto load = [&](Tile& n, int64_t t0) {
         const int last = last_of(t0);
-        sx.load(n.x, last);
-        sr.load(n.r, last);
-        si.load(n.i, last);
-        sg.load(n.g, last);
+        sx.template load<LD>(n.x, last);
+        sr.template load<LD>(n.r, last);
+        si.template load<LD>(n.i, last);
+        sg.template load<LD>(n.g, last);
 #pragma unroll
         for (int v = 0; v < V; ++v) n.e[v] = ck[t0 / SPAN * a.dim + v];
         n.s.load(seq + t0, t0 == 0, at, last);
@@ -758,12 +764,17 @@ template <typename T> __global__ void __launch_bounds__(64) k_rec_step(StepArgs 
 // launches
 // ---------------------------------------------------------------------------
 constexpr int LC = 32, TS = 4;
-// Segments of a row's length, and their steps.
-int segments(int64_t batch, int64_t L, int64_t dim, int64_t& seg) {
+// Segments of a row's length, and their steps: where the slabs alone leave CUs idle, as many as make five workgroups a CU,
+// of 128 steps at least; a pass more over the inputs then finds what enters each.  One segment
+// against many, us: 40 slabs x 16384 forward 580 and 122; 160 x 4096 131 and 119, backward 298 and 196; 240 149 and
+// 234, 309 and 306; 320 221 and 273, 432 and 367; 480 x 2048 132 and 204, 246 and 271 (the backward's pass reads two
+// inputs of four, the forward's all three).
+int segments(int64_t batch, int64_t L, int64_t dim, bool back, int64_t& seg) {
     constexpr int64_t UNIT = 128;
     const int64_t units = L > 0 ? (L + UNIT - 1) / UNIT : 1, slabs = batch * ((dim + 2 * LC - 1) / (2 * LC));
+    const int64_t ncu = m2::cu_count();
     int64_t s = 1;
-    if (slabs < 400) s = slabs > 0 ? (1280 + slabs - 1) / slabs : 1;
+    if (slabs > 0 && slabs < (back ? ncu * 3 / 2 : ncu * 3 / 4)) s = (5 * ncu + slabs - 1) / slabs;
     if (s > units) s = units;
     const int64_t per = (units + s - 1) / s;
     seg = per * UNIT;
@@ -774,19 +785,25 @@ template <typename T, int V, bool SEQ, bool NT> void launch(RecArgs a, int64_t b
     a.slabs = (a.dim + V * LC - 1) / (V * LC);
     const dim3 grid((unsigned)(batch * a.segments * a.slabs));
     auto go = [&](auto k, int w) { hipLaunchKernelGGL(k, grid, dim3(w * 64), 0, s, a); };
+    constexpr int ALL = NT ? ALL_NT : CACHED, STORES = NT ? STORES_NT : CACHED;
     if (back) {
-        if (a.segments > 1) go(k_rec_back_agg<T, V, LC, TS, 4, SEQ>, 4);
-        go(k_rec_backward<T, V, LC, TS, 4, SEQ, NT>, 4);
+        if (a.segments > 1) {
+            go(k_rec_back_agg<T, V, LC, TS, 4, SEQ>, 4);
+            go(k_rec_backward<T, V, LC, TS, 4, SEQ, STORES>, 4);
+        } else {
+            go(k_rec_backward<T, V, LC, TS, 4, SEQ, ALL>, 4);
+        }
     } else if (a.segments > 1) {
-        go(k_rec_forward<T, V, LC, TS, 4, SEQ, true, false>, 4);
-        go(k_rec_forward<T, V, LC, TS, 4, SEQ, false, NT>, 4);
+        go(k_rec_forward<T, V, LC, TS, 4, SEQ, true, CACHED>, 4);
+        go(k_rec_forward<T, V, LC, TS, 4, SEQ, false, STORES>, 4);
     } else {
-        go(k_rec_forward<T, V, LC, TS, 8, SEQ, false, NT>, 8);
+        go(k_rec_forward<T, V, LC, TS, 8, SEQ, false, ALL>, 8);
     }
 }
 template <typename T> void run(const RecArgs& a, int64_t batch, bool back, hipStream_t s) {
-    // Non-temporal stores where what is read and written does not fit the last-level cache (256 MB): results would take the
-    // place of what is read again (the second pass over a segment) or next.
+    // Past the caches where what is read and written does not fit the last of them (256 MB): results would take the place of
+    // what is read again (the second pass over a segment) or next.  16384 x 2560 forward 136 us so, 122 with
+    // the results past them; 8 x 2048 x 5120, one pass, 188 and 171 with the inputs past them too.
     const bool nt = batch * a.L * a.dim * (int64_t)sizeof(T) * (back ? 7 : 4) > (256ll << 20);
     auto go = [&](auto seq, auto many) {
         if (a.dim == 1) launch<T, 1, decltype(seq)::value, false>(a, batch, back, s);
@@ -824,7 +841,7 @@ namespace m2 {
 size_t gated_recurrence_workspace(const m2_gated_recurrence_args& a) {
     if (check_sizes("gated_linear_recurrence", a.batch, a.seqlen, a.dim, a.dtype)) return 0;
     int64_t seg;
-    const int n = segments(a.batch, a.seqlen, a.dim, seg);
+    const int n = segments(a.batch, a.seqlen, a.dim, false, seg);
     return n > 1 ? 8 * (size_t)a.batch * n * a.dim : 256;
 }
 
@@ -849,7 +866,7 @@ int launch_gated_recurrence(const m2_gated_recurrence_args& a, hipStream_t s) {
     k.ib = a.i_stride_batch; k.it = a.i_stride_time;
     k.ck = a.span_states; k.L = a.seqlen; k.spans = (a.seqlen + SPAN - 1) / SPAN; k.dim = (int)a.dim;
     k.out = a.out; k.last = a.final_states;
-    k.segments = segments(a.batch, a.seqlen, a.dim, k.seg);
+    k.segments = segments(a.batch, a.seqlen, a.dim, false, k.seg);
     const size_t need = gated_recurrence_workspace(a);
     M2_REQUIRE(k.segments == 1 || (a.workspace && a.workspace_bytes >= need), M2_ERR_WORKSPACE,
                "%s: workspace of %zu bytes needed, %zu given", who, need, a.workspace_bytes);
@@ -862,7 +879,7 @@ int launch_gated_recurrence(const m2_gated_recurrence_args& a, hipStream_t s) {
 size_t gated_recurrence_grad_workspace(const m2_gated_recurrence_grad_args& a) {
     if (check_sizes("gated_linear_recurrence_grad", a.batch, a.seqlen, a.dim, a.dtype)) return 0;
     int64_t seg;
-    const size_t n = segments(a.batch, a.seqlen, a.dim, seg) * (size_t)(a.batch > 1 ? a.batch : 1);
+    const size_t n = segments(a.batch, a.seqlen, a.dim, true, seg) * (size_t)(a.batch > 1 ? a.batch : 1);
     return 12 * n * a.dim;
 }
 
@@ -888,7 +905,7 @@ int launch_gated_recurrence_grad(const m2_gated_recurrence_grad_args& a, hipStre
     k.g = a.grad_out; k.gb = a.grad_out_stride_batch; k.gt = a.grad_out_stride_time;
     k.glast = a.grad_final_states;
     k.dx = a.grad_x; k.dr = a.grad_r; k.di = a.grad_i; k.dh0 = a.grad_initial_states;
-    k.segments = segments(a.batch, a.seqlen, a.dim, k.seg);
+    k.segments = segments(a.batch, a.seqlen, a.dim, true, k.seg);
     const int64_t parts = a.batch * k.segments;
     k.agg = static_cast<float2*>(a.workspace);
     k.dA = parts == 1 ? a.grad_A : static_cast<float*>(a.workspace) + 2 * parts * a.dim;

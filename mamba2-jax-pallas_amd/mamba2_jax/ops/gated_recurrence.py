@@ -112,14 +112,31 @@ class _GatedRecurrence(torch.autograd.Function):
         return (_backward_once if torch.is_grad_enabled() else _backward)(ctx, grad, grad_final)
 
 
+def _device(*tensors):
+    """L.device_of(*tensors), without its cost where all is well."""
+    try:
+        at = tensors[0].get_device()
+        if at >= 0:
+            for t in tensors:
+                if t is not None and t.get_device() != at:
+                    break
+            else:
+                return tensors[0].device
+    except AttributeError:
+        pass
+    return L.device_of(*tensors)          # says what is wrong
+
+
 def _check_gates(x, r, i, A, shape):
-    L.require(shape[-1] > 0, lambda: f"x.shape={tuple(shape)}: no channels")
-    L.require(r.shape == shape and i.shape == shape,
-              lambda: f"r.shape={tuple(r.shape)}, i.shape={tuple(i.shape)}: expected x's {tuple(shape)}")
-    L.require(A.shape == shape[-1:], lambda: f"A.shape={tuple(A.shape)}: expected ({shape[-1]},)")
+    """-> x's type code"""
+    if not (r.shape == shape and i.shape == shape and shape[-1] > 0 and A.shape == shape[-1:]):
+        L.require(shape[-1] > 0, f"x.shape={tuple(shape)}: no channels")
+        raise L.M2ShapeError(f"r.shape={tuple(r.shape)}, i.shape={tuple(i.shape)}, A.shape={tuple(A.shape)}: "
+                             f"expected x's {tuple(shape)} and ({shape[-1]},)")
+    dtype = x.dtype
     code = L.dtype_code(x, "x")
-    if r.dtype != x.dtype or i.dtype != x.dtype:
-        raise TypeError(f"x is {x.dtype}, r {r.dtype} and i {i.dtype}: they must be the same")
+    if r.dtype != dtype or i.dtype != dtype:
+        raise TypeError(f"x is {dtype}, r {r.dtype} and i {i.dtype}: they must be the same")
     L.dtype_code(A, "A")
     return code
 
@@ -145,7 +162,7 @@ def gated_linear_recurrence(x, r, i, A, initial_states=None, seq_idx=None, retur
     leave it between two positions); h and the gradients are rounded once.  Between the two the graph holds x, r, i and
     the states that enter every 32 positions.  Where a_t is 1 the root has no slope, and its part
     of the gradient is taken as 0.  Equal inputs give equal bits."""
-    dev = L.device_of(x, r, i, A, initial_states, seq_idx)
+    dev = _device(x, r, i, A, initial_states, seq_idx)
     shape = x.shape
     L.require(len(shape) == 3, lambda: f"x.shape={tuple(shape)}: expected (batch, seqlen, dim)")
     _check_gates(x, r, i, A, shape)
@@ -175,15 +192,17 @@ def gated_linear_recurrence_update(state, x, r, i, A, *, inplace=False):
     channels read in place; A (dim,).  The caller's state is left untouched, unless inplace=True (keyword
     only) and it is float32 and contiguous: it is then updated and returned.
     Takes no gradients."""
-    dev = L.device_of(state, x, r, i, A)
+    dev = _device(state, x, r, i, A)
     shape = x.shape
-    L.require(len(shape) == 2, lambda: f"x.shape={tuple(shape)}: expected (batch, dim)")
-    L.require(state.shape == shape, lambda: f"state.shape={tuple(state.shape)}: expected {tuple(shape)}")
+    if len(shape) != 2 or state.shape != shape:
+        raise L.M2ShapeError(f"x.shape={tuple(shape)}, state.shape={tuple(state.shape)}: expected (batch, dim)")
     code = _check_gates(x, r, i, A, shape)
     L.dtype_code(state, "state")
     src = _f32(state)
     new = src if inplace and src is state else torch.empty(shape, dtype=torch.float32, device=dev)
-    x, r, i, A = _rows(x), _rows(r), _rows(i), _f32(A)
+    if not (x.stride(1) == r.stride(1) == i.stride(1) == 1):
+        x, r, i = _rows(x), _rows(r), _rows(i)
+    A = _f32(A)
     out = torch.empty(shape, dtype=x.dtype, device=dev)
     args = L.GatedRecurrenceUpdateArgs(
         x.data_ptr(), r.data_ptr(), i.data_ptr(), A.data_ptr(), src.data_ptr(), new.data_ptr(),

@@ -653,7 +653,7 @@ int m2_gated_recurrence_update(const m2_gated_recurrence_update_args* a, void* s
  * float32 sums, rounded once; act(g) = g sigmoid(g) (M2_SILU) or gelu's tanh form (M2_GELU).  float32
  * operands are multiplied as three bf16 parts each (six products, about 2^-24 of each; an infinity
  * among them gives NaN).  With saved (m2_gated_linear_saved_size bytes, 256-byte aligned) what the gradient
- * reads is left there: act(g) and v act'(g) in dtype, and the operands where the kernels do not read them in
+ * reads is left there: act(g) and v act'(g) (of bf16 operands their upper 24 bits), and the operands where the kernels do not read them in
  * place (float32, as three bf16 parts; a dim or, of weight, a hidden that 64 does not divide).  n < 2^30, hidden dim < 2^30.
  * No counterpart in the reference, whose blocks have a mixer alone (models/mamba2_lm.py:196-211).
  * ------------------------------------------------------------------------- */
@@ -675,8 +675,8 @@ size_t m2_gated_linear_workspace_size(const m2_gated_linear_args* a);
 int m2_gated_linear(const m2_gated_linear_args* a, void* stream);
 
 /* ---------------------------------------------------------------------------
- * gated_linear_grad: with d = grad_out, dv = d act(g), dg = d v act'(g) (bf16 operands: from what was
- * saved, rounded to bf16 once more),
+ * gated_linear_grad: with d = grad_out, dv = d act(g), dg = d v act'(g) (bf16 operands: rounded to
+ * bf16 once),
  *   grad_x = dg weight[:hidden] + dv weight[hidden:],  grad_weight = [dg | dv]^T x
  * from what the forward left in saved for the same arguments.  Either output may be NULL.
  * ------------------------------------------------------------------------- */

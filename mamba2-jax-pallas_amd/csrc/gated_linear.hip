@@ -7,10 +7,10 @@
 //
 // Forward: the product runs in the tiles of ce_gemm.h, whose rows are 16 of the gate and
 // the same 16 of the values in turn (PAIR): a lane's accumulators hold g and v of the same place, and
-// the epilogue stores h alone (and, for a gradient, act(g) and v act'(g), by which dh is multiplied, in
-// the operands' type: to compute them again would take a third of the gradient's operations, to keep
-// them costs their bytes twice; g and v themselves would be rounded before the activation's slope
-// and not after it).  Up to 64 tokens
+// the epilogue stores h alone (and, for a gradient, act(g) and v act'(g), by which dh is multiplied: to
+// compute them again would take a third of the gradient's operations, to keep them costs their bytes
+// twice.  bf16 operands: in 24 bits, so that dz alone is rounded to bf16; dx and dW of 8192 x 2560 x 6912 are
+// then 2.4e-3 off instead of 2.9e-3, 1.7e-3 of it their own rounding).  Up to 64 tokens
 // whose rows a lane can load in 16-byte pieces run k_glu_few, bound by reading W once.
 // Backward: k_glu_dz makes dz = [dg | dv] = [dh v act'(g) | dh act(g)] (bf16, or three planes of it for float32), then two
 // products read it: dx with K over W's rows, dW with K over the tokens.  Tiles that would leave CUs idle in the
@@ -58,6 +58,68 @@ template <typename T> M2_DEV void store_quad(T* row, int m, int64_t dim, const f
     }
 }
 
+// The factors of dh, rows of 2 fp: float32 as they are; of bf16 operands the upper 24 bits of a float32 (cut off: off by
+// 2^-15 at most, dz's own rounding is 2^-9), the upper 16 in one array, 8 more in another.
+template <typename T> struct Factors;
+template <> struct Factors<float> {
+    float* p;
+    static size_t bytes(int64_t n, int64_t fp) { return align256(4 * (size_t)n * 2 * fp); }
+    __host__ __device__ Factors(char* at, int64_t, int64_t) : p(reinterpret_cast<float*>(at)) {}
+    // four values from place m of row n (whole: a row ends at a multiple of 64, 8)
+    M2_DEV void quad(int64_t at, const f32x4& v) const { *reinterpret_cast<f32x4*>(p + at) = v; }
+    // 32 values from f on, as two fragments; the lane's own places are valid below fp
+    M2_DEV void pair(int64_t row, int f, int64_t fp, int lane, const f32x4& x, const f32x4& y) const {
+        const int m = f + 4 * (lane >> 4);
+        if (m < fp) quad(row + m, x);
+        if (m + 16 < fp) quad(row + m + 16, y);
+    }
+    M2_DEV void load(int64_t at, float (&v)[8]) const {
+        const f32x4 a = *reinterpret_cast<const f32x4*>(p + at), b = *reinterpret_cast<const f32x4*>(p + at + 4);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) { v[i] = a[i]; v[4 + i] = b[i]; }
+    }
+};
+template <> struct Factors<bf16> {
+    typedef uint32_t u2 __attribute__((ext_vector_type(2)));
+    uint16_t* hi;
+    uint8_t* lo;
+    static size_t bytes(int64_t n, int64_t fp) { return align256(2 * (size_t)n * 2 * fp) + align256((size_t)n * 2 * fp); }
+    __host__ __device__ Factors(char* at, int64_t n, int64_t fp)
+        : hi(reinterpret_cast<uint16_t*>(at)), lo(reinterpret_cast<uint8_t*>(at) + ((2 * n * 2 * fp + 255) & ~(int64_t)255)) {}
+    // the upper halves of two floats; the next bytes of four
+    static M2_DEV uint32_t high(float a, float b) { return __builtin_amdgcn_perm(__float_as_uint(b), __float_as_uint(a), 0x07060302); }
+    static M2_DEV uint32_t next(const f32x4& v) {
+        const uint32_t a = __builtin_amdgcn_perm(__float_as_uint(v[1]), __float_as_uint(v[0]), 0x0c0c0501);
+        const uint32_t b = __builtin_amdgcn_perm(__float_as_uint(v[3]), __float_as_uint(v[2]), 0x05010c0c);
+        return a | b;
+    }
+    M2_DEV void quad(int64_t at, const f32x4& v) const {
+        *reinterpret_cast<u2*>(hi + at) = u2{high(v[0], v[1]), high(v[2], v[3])};
+        *reinterpret_cast<uint32_t*>(lo + at) = next(v);
+    }
+    M2_DEV void pair(int64_t row, int f, int64_t fp, int lane, const f32x4& x, const f32x4& y) const {
+        uint32_t a = high(x[0], x[1]), b = high(x[2], x[3]), c = high(y[0], y[1]), d = high(y[2], y[3]);
+        uint32_t e = next(x), g = next(y);
+        pair_swap(a, c);
+        pair_swap(b, d);
+        pair_swap(e, g);
+        const int m = f + pair_m(lane);
+        if (m >= fp) return;
+        *reinterpret_cast<u32x4*>(hi + row + m) = u32x4{a, b, c, d};
+        *reinterpret_cast<u2*>(lo + row + m) = u2{e, g};
+    }
+    M2_DEV void load(int64_t at, float (&v)[8]) const {
+        const u32x4 h = *reinterpret_cast<const u32x4*>(hi + at);
+        const u2 l = *reinterpret_cast<const u2*>(lo + at);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            // bytes: 0, l's, h's two
+            const uint32_t sel = 0x000c | (uint32_t)(i & 3) << 8 | (uint32_t)(4 + 2 * (i & 1)) << 16 | (uint32_t)(5 + 2 * (i & 1)) << 24;
+            v[i] = __uint_as_float(__builtin_amdgcn_perm(h[i >> 1], l[i >> 2], sel));
+        }
+    }
+};
+
 // ---------------------------------------------------------------------------
 // forward
 // ---------------------------------------------------------------------------
@@ -65,7 +127,7 @@ template <typename T> M2_DEV void store_quad(T* row, int m, int64_t dim, const f
 template <typename T, bool SAVE> struct EpiGlu {
     static constexpr bool SEG = false;
     T* h;
-    T* z;
+    Factors<T> z;
     int64_t hidden, fp;
     int gelu;
 
@@ -84,7 +146,7 @@ template <typename T, bool SAVE> struct EpiGlu {
             const int n = n0 + (wn * S::FN + j) * 16 + (lane & 15);
             if (n >= count) continue;
             T* to = h + (int64_t)n * hidden;
-            T* gr = z + (int64_t)n * 2 * fp;
+            const int64_t row = (int64_t)n * 2 * fp;
 #pragma unroll
             for (int i = 0; i < S::FM; i += WIDE ? 4 : 2) {
                 const int f = f0 + 8 * i;
@@ -103,15 +165,15 @@ template <typename T, bool SAVE> struct EpiGlu {
                 if constexpr (WIDE) {
                     store_row(to, f, hidden, lane, o[0], o[1]);
                     if constexpr (SAVE) {
-                        store_row(gr, f, hidden, lane, by[0], by[1]);
-                        store_row(gr + fp, f, hidden, lane, at[0], at[1]);
+                        z.pair(row, f, fp, lane, by[0], by[1]);
+                        z.pair(row + fp, f, fp, lane, at[0], at[1]);
                     }
                 } else {
                     const int q = f + 4 * (lane >> 4);
                     store_quad(to, q, hidden, o[0]);
-                    if constexpr (SAVE) {
-                        store_quad(gr, q, hidden, by[0]);
-                        store_quad(gr + fp, q, hidden, at[0]);
+                    if (SAVE && q < fp) {
+                        z.quad(row + q, by[0]);
+                        z.quad(row + fp + q, at[0]);
                     }
                 }
             }
@@ -241,10 +303,10 @@ __global__ void __launch_bounds__(NW * 64) k_glu_few(FewArgs a) {
         const int n = 16 * (p % MT) + (lane & 15), f = f0 + 8 * (p / MT) + 4 * ((lane >> 4) & 1);
         if (lane >= 32 || n >= a.n) continue;
         store_quad(static_cast<T*>(a.h) + (int64_t)n * a.hidden, f, a.hidden, o);
-        if (a.z) {
-            T* z = static_cast<T*>(a.z) + (int64_t)n * 2 * a.fp;
-            store_quad(z, f, a.hidden, by);
-            store_quad(z + a.fp, f, a.hidden, at);
+        if (a.z && f < a.fp) {
+            const Factors<T> z(static_cast<char*>(a.z), a.n, a.fp);
+            z.quad((int64_t)n * 2 * a.fp + f, by);
+            z.quad((int64_t)n * 2 * a.fp + a.fp + f, at);
         }
     }
 }
@@ -286,9 +348,9 @@ template <typename T> __global__ void __launch_bounds__(256) k_glu_dz(DzArgs a) 
     float dg[8] = {0, 0, 0, 0, 0, 0, 0, 0}, dv[8] = {0, 0, 0, 0, 0, 0, 0, 0};
     if (n < a.n && c < a.hidden) {
         float by[8], at[8], up[8];
-        const T* z = static_cast<const T*>(a.z) + n * 2 * a.fp;
-        load8(z, c, a.fp, by);
-        load8(z + a.fp, c, a.fp, at);
+        const Factors<T> z(static_cast<char*>(const_cast<void*>(a.z)), a.n, a.fp);
+        z.load(n * 2 * a.fp + c, by);
+        z.load(n * 2 * a.fp + a.fp + c, at);
         load8(static_cast<const T*>(a.dh) + n * a.ldg, c, a.hidden, up);
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
@@ -466,7 +528,7 @@ Common common(int64_t n, int64_t dim, int64_t hidden, int64_t ldx, int64_t ldw, 
     c.pack_w = !direct(w, ldw, hidden) || (save && hidden % 64);
     auto take = [&](size_t b) { const size_t r = c.at; c.at += align256(b); return r; };
     const size_t planes = c.f32 ? 3 : 1;
-    c.z = save ? take((size_t)(c.f32 ? 4 : 2) * n * 2 * c.fp) : 0;
+    c.z = save ? take(c.f32 ? Factors<float>::bytes(n, c.fp) : Factors<bf16>::bytes(n, c.fp)) : 0;
     c.x = c.pack_x ? take(2 * planes * (size_t)c.np * c.dp) : c.at;
     c.w = c.pack_w ? take(2 * planes * (size_t)2 * c.fp * c.dp) : c.at;
     return c;
@@ -562,7 +624,7 @@ template <bool F32, bool SAVE> int run_fwd(const m2_gated_linear_args& a, const 
     g.nk = (int)(c.dp / 64);
     g.b = operand_x<T>(ws, c, a.x, a.ldx, true, s);
     g.a = operand_w<T>(ws, c, a.weight, a.ldw, true, s);
-    const EpiGlu<T, SAVE> e{static_cast<T*>(a.out), reinterpret_cast<T*>(ws + c.z), c.hidden, c.fp, a.activation == M2_GELU};
+    const EpiGlu<T, SAVE> e{static_cast<T*>(a.out), Factors<T>(ws + c.z, c.n, c.fp), c.hidden, c.fp, a.activation == M2_GELU};
     const int64_t m = 2 * ((c.hidden + 15) / 16 * 16);
     auto go = [&](auto shape) {
         typedef decltype(shape) S;

@@ -58,78 +58,74 @@ template <typename T> M2_DEV void store_quad(T* row, int m, int64_t dim, const f
     }
 }
 
-// The factors of dh, rows of 2 fp: float32 as they are; of bf16 operands the upper 24 bits of a float32 (cut off: off by
-// 2^-15 at most, dz's own rounding is 2^-9), the upper 16 in one array, 8 more in another.
+// The factors of dh, v act'(g) and act(g), as the lanes of the forward's product hold them: an entry is four places of
+// the hidden size of one token; entries of a wavefront's 64 lanes lie beside each other, so that they are written and read in
+// whole lines.  float32 as they are; of bf16 operands the upper 24 bits (cut off: off by 2^-15 at most, dz's own
+// rounding is 2^-9), the upper 16 in one array, 8 more in another.
 template <typename T> struct Factors;
 template <> struct Factors<float> {
-    float* p;
-    static size_t bytes(int64_t n, int64_t fp) { return align256(4 * (size_t)n * 2 * fp); }
-    __host__ __device__ Factors(char* at, int64_t, int64_t) : p(reinterpret_cast<float*>(at)) {}
-    // four values from place m of row n (whole: a row ends at a multiple of 64, 8)
-    M2_DEV void quad(int64_t at, const f32x4& v) const { *reinterpret_cast<f32x4*>(p + at) = v; }
-    // 32 values from f on, as two fragments; the lane's own places are valid below fp
-    M2_DEV void pair(int64_t row, int f, int64_t fp, int lane, const f32x4& x, const f32x4& y) const {
-        const int m = f + 4 * (lane >> 4);
-        if (m < fp) quad(row + m, x);
-        if (m + 16 < fp) quad(row + m + 16, y);
+    f32x4* p;
+    static size_t bytes(int64_t entries) { return 32 * (size_t)entries; }
+    __host__ __device__ Factors(const void* at, int64_t) : p(static_cast<f32x4*>(const_cast<void*>(at))) {}
+    // (entry e + lane: e is the wavefront's)
+    M2_DEV void put(int64_t e, uint32_t lane, const f32x4& by, const f32x4& at) const {
+        f32x4* d = p + 2 * e;
+        d[2 * lane] = by;
+        d[2 * lane + 1] = at;
     }
-    M2_DEV void load(int64_t at, float (&v)[8]) const {
-        const f32x4 a = *reinterpret_cast<const f32x4*>(p + at), b = *reinterpret_cast<const f32x4*>(p + at + 4);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) { v[i] = a[i]; v[4 + i] = b[i]; }
+    M2_DEV void get(int64_t e, f32x4& by, f32x4& at) const {
+        by = p[2 * e];
+        at = p[2 * e + 1];
     }
 };
 template <> struct Factors<bf16> {
     typedef uint32_t u2 __attribute__((ext_vector_type(2)));
-    uint16_t* hi;
-    uint8_t* lo;
-    static size_t bytes(int64_t n, int64_t fp) { return align256(2 * (size_t)n * 2 * fp) + align256((size_t)n * 2 * fp); }
-    __host__ __device__ Factors(char* at, int64_t n, int64_t fp)
-        : hi(reinterpret_cast<uint16_t*>(at)), lo(reinterpret_cast<uint8_t*>(at) + ((2 * n * 2 * fp + 255) & ~(int64_t)255)) {}
-    // the upper halves of two floats; the next bytes of four
+    u32x4* hi;
+    u2* lo;
+    static size_t bytes(int64_t entries) { return 24 * (size_t)entries; }
+    __host__ __device__ Factors(const void* at, int64_t entries)
+        : hi(static_cast<u32x4*>(const_cast<void*>(at))), lo(reinterpret_cast<u2*>(hi + entries)) {}
+    // the upper halves of two floats; the next bytes of four; a float of its half `k` of h and its byte `i` of l
     static M2_DEV uint32_t high(float a, float b) { return __builtin_amdgcn_perm(__float_as_uint(b), __float_as_uint(a), 0x07060302); }
     static M2_DEV uint32_t next(const f32x4& v) {
-        const uint32_t a = __builtin_amdgcn_perm(__float_as_uint(v[1]), __float_as_uint(v[0]), 0x0c0c0501);
-        const uint32_t b = __builtin_amdgcn_perm(__float_as_uint(v[3]), __float_as_uint(v[2]), 0x05010c0c);
-        return a | b;
+        return __builtin_amdgcn_perm(__float_as_uint(v[1]), __float_as_uint(v[0]), 0x0c0c0501) |
+               __builtin_amdgcn_perm(__float_as_uint(v[3]), __float_as_uint(v[2]), 0x05010c0c);
     }
-    M2_DEV void quad(int64_t at, const f32x4& v) const {
-        *reinterpret_cast<u2*>(hi + at) = u2{high(v[0], v[1]), high(v[2], v[3])};
-        *reinterpret_cast<uint32_t*>(lo + at) = next(v);
+    static M2_DEV float both(uint32_t h, int k, uint32_t l, int i) {
+        const uint32_t sel = 0x0000000c | (uint32_t)i << 8 | (uint32_t)(4 + 2 * k) << 16 | (uint32_t)(5 + 2 * k) << 24;
+        return __uint_as_float(__builtin_amdgcn_perm(h, l, sel));
     }
-    M2_DEV void pair(int64_t row, int f, int64_t fp, int lane, const f32x4& x, const f32x4& y) const {
-        uint32_t a = high(x[0], x[1]), b = high(x[2], x[3]), c = high(y[0], y[1]), d = high(y[2], y[3]);
-        uint32_t e = next(x), g = next(y);
-        pair_swap(a, c);
-        pair_swap(b, d);
-        pair_swap(e, g);
-        const int m = f + pair_m(lane);
-        if (m >= fp) return;
-        *reinterpret_cast<u32x4*>(hi + row + m) = u32x4{a, b, c, d};
-        *reinterpret_cast<u2*>(lo + row + m) = u2{e, g};
+    M2_DEV void put(int64_t e, uint32_t lane, const f32x4& by, const f32x4& at) const {
+        (hi + e)[lane] = u32x4{high(by[0], by[1]), high(by[2], by[3]), high(at[0], at[1]), high(at[2], at[3])};
+        (lo + e)[lane] = u2{next(by), next(at)};
     }
-    M2_DEV void load(int64_t at, float (&v)[8]) const {
-        const u32x4 h = *reinterpret_cast<const u32x4*>(hi + at);
-        const u2 l = *reinterpret_cast<const u2*>(lo + at);
+    M2_DEV void get(int64_t e, f32x4& by, f32x4& at) const {
+        const u32x4 h = hi[e];
+        const u2 l = lo[e];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            // bytes: 0, l's, h's two
-            const uint32_t sel = 0x000c | (uint32_t)(i & 3) << 8 | (uint32_t)(4 + 2 * (i & 1)) << 16 | (uint32_t)(5 + 2 * (i & 1)) << 24;
-            v[i] = __uint_as_float(__builtin_amdgcn_perm(h[i >> 1], l[i >> 2], sel));
+        for (int i = 0; i < 4; ++i) {
+            by[i] = both(h[i >> 1], i & 1, l[0], i);
+            at[i] = both(h[2 + (i >> 1)], i & 1, l[1], i);
         }
     }
 };
+// the first entry of a wavefront's (wm, wn) columns j and pairs of fragments p of the tile at (m0, n0); tn: tiles along n
+template <class S> M2_DEV int64_t entry(int m0, int n0, int tn, int wm, int wn, int j, int p) {
+    const int64_t tile = (int64_t)(m0 / S::BM) * tn + n0 / S::BN;
+    return (((tile * S::NW + wm * S::WN + wn) * S::FN + j) * (S::FM / 2) + p) * 64;
+}
+template <class S> int64_t entries(int64_t m, int64_t n) { return (int64_t)tiles(m, S::BM) * tiles(n, S::BN) * (S::BM * S::BN / 8); }
 
 // ---------------------------------------------------------------------------
 // forward
 // ---------------------------------------------------------------------------
-// m: pairs of the hidden size, n: token -> h, and for a gradient rows of 2 fp of v act'(g) and act(g)
+// m: pairs of the hidden size, n: token -> h, and for a gradient the factors
 template <typename T, bool SAVE> struct EpiGlu {
     static constexpr bool SEG = false;
     T* h;
     Factors<T> z;
-    int64_t hidden, fp;
-    int gelu;
+    int64_t hidden;
+    int tn, gelu;
 
     template <class S>
     M2_DEV void run(f32x4 (&acc)[S::FM][S::FN], int m0, int n0, int wm, int wn, int lane, int count, int, int) const {
@@ -146,36 +142,26 @@ template <typename T, bool SAVE> struct EpiGlu {
             const int n = n0 + (wn * S::FN + j) * 16 + (lane & 15);
             if (n >= count) continue;
             T* to = h + (int64_t)n * hidden;
-            const int64_t row = (int64_t)n * 2 * fp;
 #pragma unroll
             for (int i = 0; i < S::FM; i += WIDE ? 4 : 2) {
                 const int f = f0 + 8 * i;
                 constexpr int E = WIDE ? 2 : 1;
-                f32x4 o[E], by[E], at[E];
+                f32x4 o[E];
 #pragma unroll
-                for (int e = 0; e < E; ++e)
+                for (int e = 0; e < E; ++e) {
+                    f32x4 by, at;
 #pragma unroll
                     for (int r = 0; r < 4; ++r) {
                         const float v = acc[i + 2 * e + 1][j][r];
                         float slope;
-                        at[e][r] = act<GELU, SAVE>(acc[i + 2 * e][j][r], slope);
-                        o[e][r] = at[e][r] * v;
-                        if constexpr (SAVE) by[e][r] = slope * v;
+                        at[r] = act<GELU, SAVE>(acc[i + 2 * e][j][r], slope);
+                        o[e][r] = at[r] * v;
+                        if constexpr (SAVE) by[r] = slope * v;
                     }
-                if constexpr (WIDE) {
-                    store_row(to, f, hidden, lane, o[0], o[1]);
-                    if constexpr (SAVE) {
-                        z.pair(row, f, fp, lane, by[0], by[1]);
-                        z.pair(row + fp, f, fp, lane, at[0], at[1]);
-                    }
-                } else {
-                    const int q = f + 4 * (lane >> 4);
-                    store_quad(to, q, hidden, o[0]);
-                    if (SAVE && q < fp) {
-                        z.quad(row + q, by[0]);
-                        z.quad(row + fp + q, at[0]);
-                    }
+                    if constexpr (SAVE) z.put(entry<S>(m0, n0, tn, wm, wn, j, i / 2 + e), lane, by, at);
                 }
+                if constexpr (WIDE) store_row(to, f, hidden, lane, o[0], o[1]);
+                else store_quad(to, f + 4 * (lane >> 4), hidden, o[0]);
             }
         }
     }
@@ -227,14 +213,15 @@ template <> struct Few<float> {
 struct FewArgs {
     const void *x, *w;
     void *h, *z;
-    int64_t ldx, ldw, fp;
+    int64_t ldx, ldw, entries;
     int n, dim, hidden, gelu;
 };
 // Up to 16 MT tokens: a workgroup takes 8 FT of the hidden size, its NW wavefronts split K and meet in LDS.
 // The 16 rows of a matrix operand are 8 of the gate and the 8 of the values, so that lanes
 // l and l + 32 hold g and v of the same place; every weight is read once, x comes from the cache.
 // U steps of 32 of K are in flight: a step's operands are loaded again, U steps on, right behind its products.
-template <typename T, int MT, int FT, int NW, int U>
+// The factors lie as the shape S's lanes would hold them, whose tiles are of 64 tokens.
+template <typename T, class S, int MT, int FT, int NW, int U>
 __global__ void __launch_bounds__(NW * 64) k_glu_few(FewArgs a) {
     __shared__ f32x4 red[NW][FT * MT][64];
     const int lane = threadIdx.x & 63, w = wave_id();
@@ -303,10 +290,11 @@ __global__ void __launch_bounds__(NW * 64) k_glu_few(FewArgs a) {
         const int n = 16 * (p % MT) + (lane & 15), f = f0 + 8 * (p / MT) + 4 * ((lane >> 4) & 1);
         if (lane >= 32 || n >= a.n) continue;
         store_quad(static_cast<T*>(a.h) + (int64_t)n * a.hidden, f, a.hidden, o);
-        if (a.z && f < a.fp) {
-            const Factors<T> z(static_cast<char*>(a.z), a.n, a.fp);
-            z.quad((int64_t)n * 2 * a.fp + f, by);
-            z.quad((int64_t)n * 2 * a.fp + a.fp + f, at);
+        static_assert(S::BN == 64 && S::FM == 2, "");
+        if (a.z && f < a.hidden) {
+            const int m0 = f / (S::BM / 2) * S::BM, wm = f % (S::BM / 2) / 16, t = n / 16;
+            const int64_t e = entry<S>(m0, 0, 1, wm, t / S::FN, t % S::FN, 0);
+            Factors<T>(a.z, a.entries).put(e, (n & 15) + 16 * (f / 4 & 3), by, at);
         }
     }
 }
@@ -337,31 +325,88 @@ template <typename T> __global__ void __launch_bounds__(256) k_glu_pack(PackArgs
 }
 
 struct DzArgs {
-    const void *z, *dh;      // as EpiGlu left it
+    const void *z, *dh;
     bf16* dz;                // [np][2 fp], zeros past n and past hidden
-    int64_t n, np, hidden, fp, ldg, plane;
+    int64_t n, np, hidden, fp, ldg, plane, entries;
+    int tm, tn;              // of the forward's product
 };
-template <typename T> __global__ void __launch_bounds__(256) k_glu_dz(DzArgs a) {
-    const int64_t per = a.fp / 8, id = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    const int64_t n = id / per, c = (id - n * per) * 8;
-    if (n >= a.np) return;
-    float dg[8] = {0, 0, 0, 0, 0, 0, 0, 0}, dv[8] = {0, 0, 0, 0, 0, 0, 0, 0};
-    if (n < a.n && c < a.hidden) {
-        float by[8], at[8], up[8];
-        const Factors<T> z(static_cast<char*>(const_cast<void*>(a.z)), a.n, a.fp);
-        z.load(n * 2 * a.fp + c, by);
-        z.load(n * 2 * a.fp + a.fp + c, at);
-        load8(static_cast<const T*>(a.dh) + n * a.ldg, c, a.hidden, up);
+// dz from the factors as the forward's shape S left them: a wavefront for 16 tokens and 32 of the hidden size (16 where a
+// wavefront of S has no more)
+template <typename T, class S> __global__ void __launch_bounds__(256) k_glu_dz(DzArgs a) {
+    constexpr bool WIDE = S::FM % 4 == 0;
+    constexpr int E = WIDE ? 2 : 1, PER = S::FM / 2 / E, WAVES = S::NW * S::FN * PER;
+    const int lane = threadIdx.x & 63;
+    int64_t q = (int64_t)blockIdx.x * 4 + wave_id();
+    const int64_t tile = q / WAVES;
+    if (tile >= (int64_t)a.tm * a.tn) return;
+    const int in = (int)(q - tile * WAVES), p = in % PER * E, j = in / PER % S::FN, w = in / PER / S::FN;
+    const int m0 = (int)(tile / a.tn) * S::BM, n0 = (int)(tile % a.tn) * S::BN, wm = w / S::WN, wn = w % S::WN;
+    const int64_t n = n0 + (wn * S::FN + j) * 16 + (lane & 15);
+    const int64_t f0 = m0 / 2 + wm * S::FM * 8 + p * 16;
+    if (f0 >= a.fp) return;                  // (a row ends at a multiple of 64: of all lanes or of none)
+    const Factors<T> z(a.z, a.entries);
+    const bool on = n < a.n;
+    f32x4 by[E], at[E], up[E];
+    const T* dh = static_cast<const T*>(a.dh) + (on ? n : 0) * a.ldg;
+    if constexpr (WIDE && sizeof(T) == 2) {
+        // 8 consecutive values a lane, exchanged to the fragments' order
+        uint32_t v[4];
+        const int64_t f = f0 + pair_m(lane);
+        if (f + 8 <= a.hidden) {
+            const u32x4 r = load16(dh + f);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            // (past the hidden size z holds anything)
-            dg[i] = c + i < a.hidden ? up[i] * by[i] : 0.f;
-            dv[i] = c + i < a.hidden ? up[i] * at[i] : 0.f;
+            for (int i = 0; i < 4; ++i) v[i] = r[i];
+        } else {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const uint16_t* s = reinterpret_cast<const uint16_t*>(dh) + f + 2 * i;
+                v[i] = (f + 2 * i < a.hidden ? s[0] : 0) | (uint32_t)(f + 2 * i + 1 < a.hidden ? s[1] : 0) << 16;
+            }
         }
+        pair_swap(v[0], v[2]);
+        pair_swap(v[1], v[3]);
+#pragma unroll
+        for (int e = 0; e < 2; ++e) up[e] = f32x4{bf16_lo(v[2 * e]), bf16_hi(v[2 * e]), bf16_lo(v[2 * e + 1]), bf16_hi(v[2 * e + 1])};
+    } else {
+#pragma unroll
+        for (int e = 0; e < E; ++e)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                const int64_t f = f0 + 16 * e + 4 * (lane >> 4) + r;
+                up[e][r] = f < a.hidden ? to_f32(dh[f]) : 0.f;
+            }
     }
-    bf16* to = a.dz + n * 2 * a.fp + c;
-    store8<sizeof(T) == 4>(to, a.plane, dg);
-    store8<sizeof(T) == 4>(to + a.fp, a.plane, dv);
+#pragma unroll
+    for (int e = 0; e < E; ++e) z.get(entry<S>(m0, n0, a.tn, wm, wn, j, p + e) + lane, by[e], at[e]);
+    // (what the factors hold past the tokens and the hidden size is anything)
+#pragma unroll
+    for (int e = 0; e < E; ++e)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            const bool in = on && f0 + 16 * e + 4 * (lane >> 4) + r < a.hidden;
+            by[e][r] = in ? up[e][r] * by[e][r] : 0.f;
+            at[e][r] = in ? up[e][r] * at[e][r] : 0.f;
+        }
+    if (n >= a.np) return;                   // (np is a multiple of 16: all lanes or none)
+    auto put = [&](bf16* to, const f32x4 (&v)[E]) {
+        constexpr int PLANES = sizeof(T) == 4 ? 3 : 1;
+        float part[PLANES][E][4];
+#pragma unroll
+        for (int e = 0; e < E; ++e)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                if constexpr (PLANES == 3) split3(v[e][r], part[0][e][r], part[1][e][r], part[2][e][r]);
+                else part[0][e][r] = v[e][r];
+            }
+#pragma unroll
+        for (int k = 0; k < PLANES; ++k) {
+            if constexpr (WIDE) store_pair(to + k * a.plane + pair_m(lane), part[k][0], part[k][1]);
+            else store_quad(to + k * a.plane, 4 * (lane >> 4), 16, f32x4{part[k][0][0], part[k][0][1], part[k][0][2], part[k][0][3]});
+        }
+    };
+    bf16* row = a.dz + n * 2 * a.fp + f0;
+    put(row, by);
+    put(row + a.fp, at);
 }
 
 // ---------------------------------------------------------------------------
@@ -472,12 +517,11 @@ __global__ void __launch_bounds__(64) k_glu_sum(const float* part, bf16* dx, int
 // ---------------------------------------------------------------------------
 // plans
 // ---------------------------------------------------------------------------
-// Tiles of the forward's product (Z), of dx (X) and of dW (W): large, middle, small; few tokens
+// Tiles of the forward's product (Z), of dx (X) and of dW (W): large, middle, small; dx of few tokens (X64, X16)
 template <bool F32> struct Shapes {
     typedef Shape<256, 256, 2, 4, 2, 64, false, false, 1, true> ZL;
     typedef Shape<256, 128, 2, 4, 2, 64, false, false, 1, true> ZM;
     typedef Shape<128, 64, 4, 1, 3, 64, false, false, 1, true> ZS;
-    typedef Shape<128, 16, 4, 1, 4, 64, false, false, 1, true> Z16;
     typedef Shape<256, 256, 2, 4, 2, 64, true, false, 1> XL;
     typedef Shape<256, 128, 2, 4, 2, 64, true, false, 1> XM;
     typedef XM XS;
@@ -491,7 +535,6 @@ template <> struct Shapes<true> {
     typedef Shape<256, 128, 4, 2, 2, 32, false, false, 6, true> ZL;
     typedef Shape<128, 128, 2, 4, 3, 32, false, false, 6, true> ZM;
     typedef Shape<128, 64, 4, 2, 4, 32, false, false, 6, true> ZS;
-    typedef Shape<128, 16, 4, 1, 4, 32, false, false, 6, true> Z16;
     typedef Shape<256, 128, 4, 2, 2, 32, true, false, 6> XL;
     typedef Shape<128, 128, 2, 4, 3, 32, true, false, 6> XM;
     typedef Shape<128, 64, 4, 2, 4, 32, true, false, 6> XS;
@@ -509,8 +552,22 @@ template <class S> int64_t rounds(int64_t m, int64_t n) {
 struct Common {
     int64_t n, np, dim, hidden, dp, fp;
     bool f32, pack_x, pack_w;
+    int shape;               // of the forward's product: 0 large, 1 middle, 2 small
+    int tm, tn;              // its tiles
+    int64_t entries;         // of the factors
     size_t z, x, w, at;
 };
+template <class F> auto with_shape(bool f32, int shape, F&& f) {
+    typedef Shapes<false> B;
+    typedef Shapes<true> P;
+    if (f32) return shape == 0 ? f(P::ZL()) : shape == 1 ? f(P::ZM()) : f(P::ZS());
+    return shape == 0 ? f(B::ZL()) : shape == 1 ? f(B::ZM()) : f(B::ZS());
+}
+template <bool F32> int shape_of(int64_t m, int64_t n) {
+    typedef Shapes<F32> P;
+    const int64_t l = rounds<typename P::ZL>(m, n), md = rounds<typename P::ZM>(m, n), sm = rounds<typename P::ZS>(m, n);
+    return n <= 64 || (sm < md && sm < l) ? 2 : md < l ? 1 : 0;
+}
 // save: with what a gradient reads, whose K runs along the rows of both operands too, and not along dim only
 Common common(int64_t n, int64_t dim, int64_t hidden, int64_t ldx, int64_t ldw, const void* x, const void* w, int dtype,
               bool save) {
@@ -520,6 +577,14 @@ Common common(int64_t n, int64_t dim, int64_t hidden, int64_t ldx, int64_t ldw, 
     c.dp = (dim + 63) / 64 * 64;
     c.fp = (hidden + 63) / 64 * 64;
     c.f32 = dtype == M2_F32;
+    const int64_t m = 2 * ((hidden + 15) / 16 * 16);
+    c.shape = c.f32 ? shape_of<true>(m, n) : shape_of<false>(m, n);
+    with_shape(c.f32, c.shape, [&](auto shape) {
+        typedef decltype(shape) S;
+        c.tm = tiles(m, S::BM);
+        c.tn = tiles(n, S::BN);
+        c.entries = entries<S>(m, n);
+    });
     // in place: bf16 rows of whole 128-byte pieces, whose offsets within a tile fit 32 bits
     auto direct = [&](const void* p, int64_t ld, int64_t apart) {
         return !c.f32 && dim % 64 == 0 && ld % 8 == 0 && al16(p) && ld <= (1 << 22) && ld * (apart + 256) < (1ll << 31);
@@ -528,7 +593,7 @@ Common common(int64_t n, int64_t dim, int64_t hidden, int64_t ldx, int64_t ldw, 
     c.pack_w = !direct(w, ldw, hidden) || (save && hidden % 64);
     auto take = [&](size_t b) { const size_t r = c.at; c.at += align256(b); return r; };
     const size_t planes = c.f32 ? 3 : 1;
-    c.z = save ? take(c.f32 ? Factors<float>::bytes(n, c.fp) : Factors<bf16>::bytes(n, c.fp)) : 0;
+    c.z = save ? take(c.f32 ? Factors<float>::bytes(c.entries) : Factors<bf16>::bytes(c.entries)) : 0;
     c.x = c.pack_x ? take(2 * planes * (size_t)c.np * c.dp) : c.at;
     c.w = c.pack_w ? take(2 * planes * (size_t)2 * c.fp * c.dp) : c.at;
     return c;
@@ -574,13 +639,14 @@ template <class A> Common common_of(const A& a, bool save) {
 }
 
 template <typename T> void run_few(const m2_gated_linear_args& a, hipStream_t s) {
-    const FewArgs k{a.x, a.weight, a.out, a.saved, a.ldx, a.ldw, (a.hidden + 63) / 64 * 64,
+    typedef typename Shapes<sizeof(T) == 4>::ZS S;
+    const FewArgs k{a.x, a.weight, a.out, a.saved, a.ldx, a.ldw, entries<S>(2 * ((a.hidden + 15) / 16 * 16), a.n),
                     (int)a.n, (int)a.dim, (int)a.hidden, a.activation == M2_GELU};
     auto go = [&](auto mt) {
         constexpr int MT = decltype(mt)::value;
         auto with = [&](auto ft, auto nw, auto u) {
             constexpr int FT = decltype(ft)::value, NW = decltype(nw)::value, U = decltype(u)::value;
-            hipLaunchKernelGGL((k_glu_few<T, MT, FT, NW, U>), dim3((unsigned)((a.hidden + 8 * FT - 1) / (8 * FT))), dim3(NW * 64), 0, s, k);
+            hipLaunchKernelGGL((k_glu_few<T, S, MT, FT, NW, U>), dim3((unsigned)((a.hidden + 8 * FT - 1) / (8 * FT))), dim3(NW * 64), 0, s, k);
         };
         typedef std::integral_constant<int, 1> one;
         typedef std::integral_constant<int, 2> two;
@@ -624,19 +690,12 @@ template <bool F32, bool SAVE> int run_fwd(const m2_gated_linear_args& a, const 
     g.nk = (int)(c.dp / 64);
     g.b = operand_x<T>(ws, c, a.x, a.ldx, true, s);
     g.a = operand_w<T>(ws, c, a.weight, a.ldw, true, s);
-    const EpiGlu<T, SAVE> e{static_cast<T*>(a.out), Factors<T>(ws + c.z, c.n, c.fp), c.hidden, c.fp, a.activation == M2_GELU};
-    const int64_t m = 2 * ((c.hidden + 15) / 16 * 16);
-    auto go = [&](auto shape) {
-        typedef decltype(shape) S;
-        g.tm = tiles(m, S::BM);
-        g.tn = tiles(c.n, S::BN);
-        launch<S>(g, e, s);
-    };
-    const int64_t l = rounds<typename P::ZL>(m, c.n), md = rounds<typename P::ZM>(m, c.n), sm = rounds<typename P::ZS>(m, c.n);
-    if (c.n <= 16) go(typename P::Z16());
-    else if (c.n <= 64 || (sm < md && sm < l)) go(typename P::ZS());
-    else if (md < l) go(typename P::ZM());
-    else go(typename P::ZL());
+    const EpiGlu<T, SAVE> e{static_cast<T*>(a.out), Factors<T>(ws + c.z, c.entries), c.hidden, c.tn, a.activation == M2_GELU};
+    g.tm = c.tm;
+    g.tn = c.tn;
+    if (c.shape == 2) launch<typename P::ZS>(g, e, s);
+    else if (c.shape == 1) launch<typename P::ZM>(g, e, s);
+    else launch<typename P::ZL>(g, e, s);
     return m2::check_launch("gated_linear");
 }
 
@@ -708,8 +767,15 @@ template <bool F32> int run_bwd(const m2_gated_linear_grad_args& a, const BwdPla
     bf16* dz = reinterpret_cast<bf16*>(ws + p.dz);
     float* part = reinterpret_cast<float*>(ws + p.part);
     const int64_t plane = c.np * 2 * c.fp;
-    const DzArgs d{a.saved, a.grad_out, dz, c.n, c.np, c.hidden, c.fp, a.ldg, plane};
-    hipLaunchKernelGGL(k_glu_dz<T>, dim3((unsigned)((c.np * (c.fp / 8) + 255) / 256)), dim3(256), 0, s, d);
+    const DzArgs d{a.saved, a.grad_out, dz, c.n, c.np, c.hidden, c.fp, a.ldg, plane, c.entries, c.tm, c.tn};
+    auto make = [&](auto shape) {
+        typedef decltype(shape) S;
+        const int64_t waves = (int64_t)c.tm * c.tn * (S::BM * S::BN / 2 / 16 / (S::FM % 4 ? 16 : 32));
+        hipLaunchKernelGGL((k_glu_dz<T, S>), dim3((unsigned)((waves + 3) / 4)), dim3(256), 0, s, d);
+    };
+    if (c.shape == 2) make(typename P::ZS());
+    else if (c.shape == 1) make(typename P::ZM());
+    else make(typename P::ZL());
     auto product = [&](auto shape, Gemm g, int64_t m, int64_t n, int64_t k, const Out<T>& out) {
         typedef decltype(shape) S;
         g.tm = tiles(m, S::BM);

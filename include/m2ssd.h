@@ -574,7 +574,7 @@ int m2_clip_grad_norm(const m2_clip_grad_norm_args* a, void* stream);
  * unchanged, and what x, r and i hold there (they must be readable) reaches nothing.
  * final_states is the state behind the last position.  x, r and i are addressed through their strides of
  * batch and time (elements; channels are contiguous; of time 0, or dim to 2^20), e.g. as slices of one
- * projection's output.  dim <= 2^20.
+ * projection's output.  dim <= 2^20, batch ceil(dim / 64) < 2^22.
  * span_states (or NULL) takes the states that enter every M2_RECURRENCE_SPAN positions, which
  * the gradient reads.
  * No counterpart in the reference, whose only recurrence is the SSD's (ops/ssd_naive.py:220-322).
@@ -653,8 +653,9 @@ int m2_gated_recurrence_update(const m2_gated_recurrence_update_args* a, void* s
  * float32 sums, rounded once; act(g) = g sigmoid(g) (M2_SILU) or gelu's tanh form (M2_GELU).  float32
  * operands are multiplied as three bf16 parts each (six products, about 2^-24 of each; an infinity
  * among them gives NaN).  With saved (m2_gated_linear_saved_size bytes, 256-byte aligned) what the gradient
- * reads is left there: act(g) and v act'(g) (of bf16 operands their upper 24 bits), and the operands where the kernels do not read them in
- * place (float32, as three bf16 parts; a dim or, of weight, a hidden that 64 does not divide).  n < 2^30, hidden dim < 2^30.
+ * reads is left there: act(g) and v act'(g) (of bf16 operands their upper 24 bits), and the operands
+ * where the kernels do not read them in place (float32, as three bf16 parts; a dim or, of weight, a
+ * hidden that 64 does not divide).  n < 2^30, hidden <= 2^21, hidden dim < 2^30.
  * No counterpart in the reference, whose blocks have a mixer alone (models/mamba2_lm.py:196-211).
  * ------------------------------------------------------------------------- */
 #define M2_SILU 0
@@ -678,13 +679,14 @@ int m2_gated_linear(const m2_gated_linear_args* a, void* stream);
  * gated_linear_grad: with d = grad_out, dv = d act(g), dg = d v act'(g) (bf16 operands: rounded to
  * bf16 once),
  *   grad_x = dg weight[:hidden] + dv weight[hidden:],  grad_weight = [dg | dv]^T x
- * from what the forward left in saved for the same arguments.  Either output may be NULL.
+ * from what the forward left in saved for the same values; x and weight may lie elsewhere by now, with
+ * other strides and alignments.  Either output may be NULL.
  * ------------------------------------------------------------------------- */
 typedef struct {
     const void* x;
     const void* weight;
     const void* saved;             /* as the forward left it                    */
-    size_t      saved_bytes;
+    size_t      saved_bytes;       /* the forward's m2_gated_linear_saved_size: it tells what lies there */
     const void* grad_out;          /* [n, hidden] at ldg, dtype                 */
     void*       grad_x;            /* out [n, dim] contiguous, dtype, or NULL   */
     void*       grad_weight;       /* out [2 hidden, dim] contiguous, or NULL   */

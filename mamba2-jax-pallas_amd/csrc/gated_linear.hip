@@ -19,9 +19,6 @@
 // Operands that direct loads cannot take in place (float32, widths that 64 does not divide, unaligned
 // rows) are packed first: rows padded with zeros, the gate's and the values' to whole 64s.
 #include "ce_gemm.h"
-#ifdef TUNE
-#include <cstdlib>
-#endif
 
 namespace {
 
@@ -555,7 +552,7 @@ struct Common {
     int shape;               // of the forward's product: 0 large, 1 middle, 2 small
     int tm, tn;              // its tiles
     int64_t entries;         // of the factors
-    size_t z, x, w, at;
+    size_t z, x, w;          // bytes of the factors, and of x and weight where they are packed
 };
 template <class F> auto with_shape(bool f32, int shape, F&& f) {
     typedef Shapes<false> B;
@@ -591,25 +588,34 @@ Common common(int64_t n, int64_t dim, int64_t hidden, int64_t ldx, int64_t ldw, 
     };
     c.pack_x = !direct(x, ldx, 0);
     c.pack_w = !direct(w, ldw, hidden) || (save && hidden % 64);
-    auto take = [&](size_t b) { const size_t r = c.at; c.at += align256(b); return r; };
     const size_t planes = c.f32 ? 3 : 1;
-    c.z = save ? take(c.f32 ? Factors<float>::bytes(c.entries) : Factors<bf16>::bytes(c.entries)) : 0;
-    c.x = c.pack_x ? take(2 * planes * (size_t)c.np * c.dp) : c.at;
-    c.w = c.pack_w ? take(2 * planes * (size_t)2 * c.fp * c.dp) : c.at;
+    c.z = save ? align256(c.f32 ? Factors<float>::bytes(c.entries) : Factors<bf16>::bytes(c.entries)) : 0;
+    c.x = align256(2 * planes * (size_t)c.np * c.dp);
+    c.w = align256(2 * planes * (size_t)2 * c.fp * c.dp);
+    if (c.w == c.x) c.w += 256;              // (so that the size of `saved` tells what lies in it)
     return c;
 }
+// What the forward leaves for the gradient: the factors, then x and weight if it packed them.  The gradient goes by the size, for
+// x and weight may lie elsewhere by then, with other strides and another alignment.
+struct Kept {
+    bool x, w, known;
+};
+Kept kept(const Common& c, size_t bytes) {
+    if (bytes == c.z) return {false, false, true};
+    if (bytes == c.z + c.x) return {true, false, true};
+    if (bytes == c.z + c.w) return {false, true, true};
+    return {true, true, bytes == c.z + c.x + c.w};
+}
 
-// (pack: they are not there yet)
-template <typename T> Operand operand_x(char* ws, const Common& c, const void* x, int64_t ldx, bool pack, hipStream_t s) {
-    if (!c.pack_x) return Operand{static_cast<const bf16*>(x), ldx, 0, (int)c.n, (int)c.dim};
-    bf16* to = reinterpret_cast<bf16*>(ws + c.x);
+// An operand in place, or (to) packed there; pack: it is not there yet
+template <typename T> Operand operand_x(bf16* to, const Common& c, const void* x, int64_t ldx, bool pack, hipStream_t s) {
+    if (!to) return Operand{static_cast<const bf16*>(x), ldx, 0, (int)c.n, (int)c.dim};
     const PackArgs a{x, to, c.np, c.dim, ldx, c.dp, c.np * c.dp, 0, c.n};
     if (pack) hipLaunchKernelGGL(k_glu_pack<T>, dim3((unsigned)((c.np + 3) / 4)), dim3(256), 0, s, a);
     return Operand{to, c.dp, c.np * c.dp, (int)c.np, (int)c.dp};
 }
-template <typename T> Operand operand_w(char* ws, const Common& c, const void* w, int64_t ldw, bool pack, hipStream_t s) {
-    if (!c.pack_w) return Operand{static_cast<const bf16*>(w), ldw, 0, (int)c.hidden, (int)c.dim, (int)c.hidden};
-    bf16* to = reinterpret_cast<bf16*>(ws + c.w);
+template <typename T> Operand operand_w(bf16* to, const Common& c, const void* w, int64_t ldw, bool pack, hipStream_t s) {
+    if (!to) return Operand{static_cast<const bf16*>(w), ldw, 0, (int)c.hidden, (int)c.dim, (int)c.hidden};
     const PackArgs a{w, to, 2 * c.fp, c.dim, ldw, c.dp, 2 * c.fp * c.dp, c.fp, c.hidden};
     if (pack) hipLaunchKernelGGL(k_glu_pack<T>, dim3((unsigned)(2 * c.fp / 4)), dim3(256), 0, s, a);
     return Operand{to, c.dp, 2 * c.fp * c.dp, (int)c.fp, (int)c.dp, (int)c.fp};
@@ -622,8 +628,8 @@ int check_sizes(const char* who, int64_t n, int64_t dim, int64_t hidden, int64_t
     M2_REQUIRE(ldx >= dim && ldw >= dim, M2_ERR_INVALID, "%s: row strides", who);
     M2_REQUIRE(dtype == M2_F32 || dtype == M2_BF16, M2_ERR_UNSUPPORTED, "%s: dtype %d", who, dtype);
     M2_REQUIRE(activation == M2_SILU || activation == M2_GELU, M2_ERR_UNSUPPORTED, "%s: activation %d", who, activation);
-    // (offsets between the halves of a tile's rows; counts of tiles)
-    M2_REQUIRE((hidden + 64) * ((dim + 63) / 64 * 64) < (1ll << 30) &&
+    // (offsets between the halves of a tile's rows, and between 256 rows of dz; counts of tiles)
+    M2_REQUIRE(hidden <= (1 << 21) && (hidden + 64) * ((dim + 63) / 64 * 64) < (1ll << 30) &&
                    (int64_t)tiles(2 * hidden, 128) * tiles(n, 16) < (1ll << 30),
                M2_ERR_UNSUPPORTED, "%s: too large", who);
     return M2_OK;
@@ -652,21 +658,6 @@ template <typename T> void run_few(const m2_gated_linear_args& a, hipStream_t s)
         typedef std::integral_constant<int, 2> two;
         typedef std::integral_constant<int, 4> four;
         typedef std::integral_constant<int, 8> eight;
-#ifdef TUNE
-        const int e = getenv("FEW") ? atoi(getenv("FEW")) : 0;
-        switch (e) {
-            case 0: with(one(), four(), eight()); break;
-            case 1: with(one(), eight(), four()); break;
-            case 2: with(two(), four(), four()); break;
-            case 3: with(two(), eight(), four()); break;
-            case 4: with(four(), four(), four()); break;
-            case 5: with(four(), eight(), two()); break;
-            case 6: with(four(), four(), two()); break;
-            case 7: with(two(), four(), eight()); break;
-            case 8: with(four(), eight(), four()); break;
-            case 9: with(two(), eight(), two()); break;
-        }
-#else
         // More of the hidden size for each workgroup reads x less often, as long as there are workgroups for most
         // CUs: 16 tokens x 2560 x 6912 by 8, 16, 32: 29, 24, 22 us, 2048 x 1024: 6.6, 8.0, 11.7.
         const int64_t wgs = (a.hidden + 7) / 8;
@@ -674,7 +665,6 @@ template <typename T> void run_few(const m2_gated_linear_args& a, hipStream_t s)
         else if (wgs < 4 * 192) with(two(), eight(), two());
         else if constexpr (sizeof(T) == 4 && MT < 4) with(four(), eight(), two());
         else with(four(), four(), two());
-#endif
     };
     if (a.n <= 16) go(std::integral_constant<int, 1>());
     else if (a.n <= 32) go(std::integral_constant<int, 2>());
@@ -685,12 +675,14 @@ template <bool F32, bool SAVE> int run_fwd(const m2_gated_linear_args& a, const 
     typedef typename std::conditional<F32, float, bf16>::type T;
     typedef Shapes<F32> P;
     char* ws = static_cast<char*>(SAVE ? a.saved : a.workspace);
+    bf16* xp = c.pack_x ? reinterpret_cast<bf16*>(ws + c.z) : nullptr;
+    bf16* wp = c.pack_w ? reinterpret_cast<bf16*>(ws + c.z + (xp ? c.x : 0)) : nullptr;
     Gemm g{};
     g.n = (int)c.n; g.splits = 1;
     g.nk = (int)(c.dp / 64);
-    g.b = operand_x<T>(ws, c, a.x, a.ldx, true, s);
-    g.a = operand_w<T>(ws, c, a.weight, a.ldw, true, s);
-    const EpiGlu<T, SAVE> e{static_cast<T*>(a.out), Factors<T>(ws + c.z, c.entries), c.hidden, c.tn, a.activation == M2_GELU};
+    g.b = operand_x<T>(xp, c, a.x, a.ldx, true, s);
+    g.a = operand_w<T>(wp, c, a.weight, a.ldw, true, s);
+    const EpiGlu<T, SAVE> e{static_cast<T*>(a.out), Factors<T>(ws, c.entries), c.hidden, c.tn, a.activation == M2_GELU};
     g.tm = c.tm;
     g.tn = c.tn;
     if (c.shape == 2) launch<typename P::ZS>(g, e, s);
@@ -701,8 +693,9 @@ template <bool F32, bool SAVE> int run_fwd(const m2_gated_linear_args& a, const 
 
 struct BwdPlan {
     Common c;
-    size_t dz, part, total;
-    bool pack;               // the operands are packed here, in the workspace; else they are in saved
+    Kept kept;               // what lies in saved; what does not and cannot be read in place is packed into the workspace
+    bool pack_x, pack_w;
+    size_t xp, wp, dz, part, total;
     int x;                   // dx: 0 the large tiles, 1 the middle, 2 the small, 64 / 16 k_ce_stream's
     int w;                   // dW: the same
     int splits;
@@ -715,10 +708,13 @@ template <bool F32> BwdPlan plan_bwd(const m2_gated_linear_grad_args& a) {
     BwdPlan p{};
     p.c = common_of(a, true);
     const Common& c = p.c;
-    // (the forward of few tokens packs nothing)
-    p.pack = few(a);
-    size_t at = p.pack ? c.at : 0;
+    p.kept = kept(c, a.saved_bytes);
+    p.pack_x = a.grad_weight && c.pack_x && !p.kept.x;
+    p.pack_w = a.grad_x && c.pack_w && !p.kept.w;
+    size_t at = 0;
     auto take = [&](size_t b) { const size_t r = at; at += align256(b); return r; };
+    p.xp = take(p.pack_x ? c.x : 0);
+    p.wp = take(p.pack_w ? c.w : 0);
     p.dz = take(2 * (size_t)(F32 ? 3 : 1) * c.np * 2 * c.fp);
     // (the two products run one after the other and share the parts' buffer)
     size_t need = 0;
@@ -762,8 +758,10 @@ template <bool F32> int run_bwd(const m2_gated_linear_grad_args& a, const BwdPla
     typedef typename std::conditional<F32, float, bf16>::type T;
     typedef Shapes<F32> P;
     char* ws = static_cast<char*>(a.workspace);
-    char* packed = p.pack ? ws : static_cast<char*>(const_cast<void*>(a.saved));
     const Common& c = p.c;
+    auto at = [](const void* base, size_t off) { return reinterpret_cast<bf16*>(static_cast<char*>(const_cast<void*>(base)) + off); };
+    bf16* xp = p.kept.x ? at(a.saved, c.z) : p.pack_x ? at(ws, p.xp) : nullptr;
+    bf16* wp = p.kept.w ? at(a.saved, c.z + (p.kept.x ? c.x : 0)) : p.pack_w ? at(ws, p.wp) : nullptr;
     bf16* dz = reinterpret_cast<bf16*>(ws + p.dz);
     float* part = reinterpret_cast<float*>(ws + p.part);
     const int64_t plane = c.np * 2 * c.fp;
@@ -794,7 +792,7 @@ template <bool F32> int run_bwd(const m2_gated_linear_grad_args& a, const BwdPla
     if (a.grad_x) {
         Gemm g{};
         g.n = (int)c.n;
-        g.a = operand_w<T>(packed, c, a.weight, a.ldw, p.pack, s);
+        g.a = operand_w<T>(wp, c, a.weight, a.ldw, p.pack_w, s);
         g.a.lim = g.a.klim;                  // read by columns
         g.a.klim = (int)(2 * c.fp);
         g.b = Operand{dz, 2 * c.fp, plane, (int)c.np, (int)(2 * c.fp)};
@@ -822,7 +820,7 @@ template <bool F32> int run_bwd(const m2_gated_linear_grad_args& a, const BwdPla
     if (a.grad_weight) {
         Gemm g{};
         g.n = (int)(2 * c.fp);
-        g.a = operand_x<T>(packed, c, a.x, a.ldx, p.pack, s);
+        g.a = operand_x<T>(xp, c, a.x, a.ldx, p.pack_x, s);
         g.a.klim = g.a.lim;                  // read by columns; zero rows of dz stand against the repeated last row
         g.a.lim = (int)c.dp;
         g.b = Operand{dz, 2 * c.fp, plane, (int)(2 * c.fp), (int)c.np};
@@ -838,16 +836,19 @@ template <bool F32> int run_bwd(const m2_gated_linear_grad_args& a, const BwdPla
 
 namespace m2 {
 
+static size_t packed_bytes(const Common& c) { return (c.pack_x ? c.x : 0) + (c.pack_w ? c.w : 0); }
+
 size_t gated_linear_saved(const m2_gated_linear_args& a) {
     if (check_sizes("gated_linear", a.n, a.dim, a.hidden, a.ldx, a.ldw, a.dtype, a.activation)) return 0;
     const Common c = common_of(a, true);
-    const size_t b = few(a) ? c.x : c.at;      // z stands first
+    // (few tokens are packed for the gradient alone)
+    const size_t b = c.z + (few(a) ? 0 : packed_bytes(c));
     return b ? b : 256;
 }
 
 size_t gated_linear_workspace(const m2_gated_linear_args& a) {
     if (check_sizes("gated_linear", a.n, a.dim, a.hidden, a.ldx, a.ldw, a.dtype, a.activation)) return 0;
-    const size_t b = a.saved || few(a) ? 0 : common_of(a, false).at;
+    const size_t b = a.saved || few(a) ? 0 : packed_bytes(common_of(a, false));
     return b ? b : 256;
 }
 
@@ -865,8 +866,9 @@ int launch_gated_linear(const m2_gated_linear_args& a, hipStream_t s) {
     }
     const Common c = common_of(a, a.saved != nullptr);
     if (a.saved) return c.f32 ? run_fwd<true, true>(a, c, s) : run_fwd<false, true>(a, c, s);
-    M2_REQUIRE(c.at == 0 || (a.workspace && a.workspace_bytes >= c.at), M2_ERR_WORKSPACE,
-               "%s: workspace of %zu bytes needed, %zu given", who, c.at, a.workspace_bytes);
+    const size_t need = packed_bytes(c);
+    M2_REQUIRE(need == 0 || (a.workspace && a.workspace_bytes >= need), M2_ERR_WORKSPACE,
+               "%s: workspace of %zu bytes needed, %zu given", who, need, a.workspace_bytes);
     return c.f32 ? run_fwd<true, false>(a, c, s) : run_fwd<false, false>(a, c, s);
 }
 
@@ -888,8 +890,7 @@ int launch_gated_linear_grad(const m2_gated_linear_grad_args& a, hipStream_t s) 
     M2_REQUIRE(a.x && a.weight && a.saved && a.grad_out && (a.grad_x || a.grad_weight), M2_ERR_INVALID,
                "%s: x, weight, saved, grad_out and an output are required", who);
     const BwdPlan p = plan(a);
-    M2_REQUIRE(a.saved_bytes >= (p.pack ? p.c.x : p.c.at), M2_ERR_WORKSPACE, "%s: saved of %zu bytes needed, %zu given",
-               who, p.pack ? p.c.x : p.c.at, a.saved_bytes);
+    M2_REQUIRE(p.kept.known, M2_ERR_WORKSPACE, "%s: saved of %zu bytes is no forward's of these sizes", who, a.saved_bytes);
     M2_REQUIRE(a.workspace && a.workspace_bytes >= p.total, M2_ERR_WORKSPACE,
                "%s: workspace of %zu bytes needed, %zu given", who, p.total, a.workspace_bytes);
     return a.dtype == M2_F32 ? run_bwd<true>(a, p, s) : run_bwd<false>(a, p, s);

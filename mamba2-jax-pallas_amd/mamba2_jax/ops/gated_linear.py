@@ -80,7 +80,7 @@ def gated_linear(x, weight, activation="silu"):
 
     Sums and the activation are float32, h is rounded once; float32 operands are multiplied as three
     bfloat16 parts each, accurate to about 2^-24 of each product (an infinity among them gives
-NaN).  Between the two the graph holds x, weight, act(g) and v act'(g) of the two products g and v (for
+    NaN).  Between the two the graph holds x, weight, act(g) and v act'(g) of the two products g and v (for
     bfloat16 operands 24 bits of each), and a packed copy of the operands that the kernels cannot read in
     place (float32, as three bfloat16 parts: 1.5 times each; a dim or hidden that 64 does not divide); the
     gradient of bfloat16 operands rounds its products with those to bfloat16 once.

@@ -13,9 +13,11 @@ Tolerances are per element and derived from the arithmetic; F = 2^-24, u(T) half
 """
 
 import math
+import zlib
 
 import pytest
 import torch
+import torch.utils.checkpoint
 
 from gpu_util import announce
 from mamba2_jax import ops
@@ -33,7 +35,7 @@ def u(dtype):
 
 
 def gen(*key):
-    return torch.Generator(device=DEV).manual_seed(hash(key) % (2 ** 31))
+    return torch.Generator(device=DEV).manual_seed(zlib.crc32(repr(key).encode()))
 
 
 def within(got, want, tol, what):
@@ -218,6 +220,40 @@ def test_gated_linear_layouts(n, dim, hidden, dtype):
     assert torch.equal(ops.gated_linear(x[0], w), ops.gated_linear(x[:1], w)[0])
 
 
+@pytest.mark.parametrize("n,dim,hidden", [(40, 64, 64), (128, 128, 64), (90, 200, 77)])
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+def test_gated_linear_saved_elsewhere(n, dim, hidden, dtype):
+    """The graph's tensors put away and brought back at other places, strides and alignments (as hooks that keep them in host
+    memory do), and a pass that is computed again."""
+    announce("saved elsewhere", n, dim, hidden, dtype)
+    x, w, dh = inputs(n, dim, hidden, dtype)
+    want = Reference(x, w, "silu", dh)
+
+    def odd(t):
+        b = torch.empty((t.shape[0], t.shape[1] + 3), device=DEV, dtype=t.dtype)[:, 1:1 + t.shape[1]]
+        b.copy_(t.detach())
+        return b
+
+    bring = {"plain": lambda t: t.clone(), "odd": lambda t: odd(t) if t.dim() == 2 else t.clone()}
+    for x2 in (x, odd(x)):
+        for w2 in (w, odd(w)):
+            for name, unpack in bring.items():
+                xl, wl = x2.detach().requires_grad_(), w2.detach().requires_grad_()
+                with torch.autograd.graph.saved_tensors_hooks(lambda t: t, unpack):
+                    h = ops.gated_linear(xl, wl)
+                dx, dw = torch.autograd.grad(h, (xl, wl), dh)
+                within(dx, want.dx, want.edx, f"dx {name}")
+                within(dw, want.dw, want.edw, f"dw {name}")
+    xl, wl = x.detach().requires_grad_(), w.detach().requires_grad_()
+    with torch.autograd.graph.save_on_cpu():
+        h = ops.gated_linear(xl, wl)
+    moved = torch.autograd.grad(h, (xl, wl), dh)
+    again = torch.utils.checkpoint.checkpoint(ops.gated_linear, xl, wl, use_reentrant=False)
+    again = torch.autograd.grad(again, (xl, wl), dh)
+    for p, q, r in zip(moved, again, grads(x, w, dh)[1:]):
+        assert torch.equal(p, r) and torch.equal(q, r)
+
+
 def test_gated_linear_nothing():
     announce("nothing")
     x = torch.zeros((0, 64), device=DEV, dtype=torch.bfloat16).requires_grad_()
@@ -291,6 +327,18 @@ def test_gated_linear_far_rows():
     far.copy_(x)
     want = Reference(x, w, "silu", dh)
     h, dx, dw = grads(far, w, dh)
+    within(h, want.h, want.eh, "h")
+    within(dx, want.dx, want.edx, "dx")
+    within(dw, want.dw, want.edw, "dw")
+
+
+@pytest.mark.parametrize("n", [3, 70])
+def test_gated_linear_wide(n):
+    """The largest hidden size but a few: dz's rows lie 2^31 bytes apart within a tile."""
+    announce("wide", n)
+    x, w, dh = inputs(n, 64, 2 ** 21 - 5, "bf16")
+    want = Reference(x, w, "silu", dh)
+    h, dx, dw = grads(x, w, dh)
     within(h, want.h, want.eh, "h")
     within(dx, want.dx, want.edx, "dx")
     within(dw, want.dw, want.edw, "dw")

@@ -130,6 +130,34 @@ def test_gated_linear_refusals():
     refused(name, mg(workspace=4096, workspace_bytes=need - 1), -4, "workspace")
 
 
+def test_gated_linear_saved_layouts():
+    """What lies in `saved` follows from its size alone, wherever x and weight lie when the gradient is taken; a size that is no
+    forward's is refused."""
+    lib = L.load_library()
+    n, dim, hidden = 512, 256, 256              # (as many rows of x as weight has)
+    sizes = set()
+    for x in (4096, 4098):
+        for w in (4096, 4098):
+            a = L.GatedLinearArgs(x=x, weight=w, out=4096, n=n, dim=dim, hidden=hidden, ldx=dim, ldw=dim, dtype=L.M2_BF16)
+            sizes.add(lib.m2_gated_linear_saved_size(ctypes.byref(a)))
+    assert len(sizes) == 4
+    grad = lambda **k: L.GatedLinearGradArgs(**{**dict(
+        x=4096, weight=4096, saved=4096, grad_out=4096, grad_x=4096, grad_weight=4096, n=n, dim=dim, hidden=hidden, ldx=dim, ldw=dim,
+        ldg=hidden, dtype=L.M2_BF16), **k})
+    bare = min(sizes)
+    for size in sizes:
+        for x, w in ((4096, 4096), (4098, 4098)):
+            args = grad(x=x, weight=w, saved_bytes=size)
+            assert lib.m2_gated_linear_grad_workspace_size(ctypes.byref(args)) > 0
+            refused("m2_gated_linear_grad", args, -4, "workspace of")
+            args.saved_bytes += 1
+            refused("m2_gated_linear_grad", args, -4, "saved of")
+    # what is neither there nor readable in place is packed
+    ws = lambda **k: lib.m2_gated_linear_grad_workspace_size(ctypes.byref(grad(**k)))
+    assert ws(saved_bytes=bare, x=4098, weight=4098) >= ws(saved_bytes=bare) + 2 * 2 * n * dim
+    assert ws(saved_bytes=max(sizes), x=4098, weight=4098) == ws(saved_bytes=max(sizes)) == ws(saved_bytes=bare)
+
+
 def test_gated_linear_shape_refusals():
     x, w = _fake(3, 8), _fake(12, 8)
     for args in ((x[0, 0], w), (x, w[0]), (x, w[:, :7]), (x, w[:11]), (x, w[:0]), (x[:, :0], w[:, :0]), (x, w, "relu")):

@@ -829,8 +829,8 @@ int check_sizes(const char* who, int64_t batch, int64_t seqlen, int64_t dim, int
                "%s: bad sizes (batch %lld, seqlen %lld, dim %lld)", who, (long long)batch, (long long)seqlen,
                (long long)dim);
     M2_REQUIRE(dtype == M2_F32 || dtype == M2_BF16, M2_ERR_UNSUPPORTED, "%s: dtype %d", who, dtype);
-    // (counts of workgroups)
-    M2_REQUIRE(batch < (1ll << 30) && batch * ((dim + 63) / 64) < (1ll << 24), M2_ERR_UNSUPPORTED, "%s: too many rows", who);
+    // (counts of threads: 32 bits)
+    M2_REQUIRE(batch < (1ll << 22) && batch * ((dim + 63) / 64) < (1ll << 22), M2_ERR_UNSUPPORTED, "%s: too many rows", who);
     return M2_OK;
 }
 

@@ -30,11 +30,14 @@ MAX_STRIDE = 2 ** 20
 def _strided(t):
     """t (batch, seqlen, dim) as the kernels read it in place: contiguous channels, positions that are one, or
     behind each other and at most MAX_STRIDE elements apart; a copy where it is not so."""
-    dim = t.shape[2]
+    _, seqlen, dim = t.shape
     st = t.stride(1)
-    if (t.stride(2) == 1 or dim == 1) and (st == 0 or dim <= st <= MAX_STRIDE):
-        return t
-    return t.contiguous() if not t.is_contiguous() else t
+    if t.stride(2) == 1 or dim == 1:
+        if st == 0 or dim <= st <= MAX_STRIDE:
+            return t
+        if seqlen == 1:                   # (no next position: any stride)
+            return t.as_strided(t.shape, (t.stride(0), dim, 1))
+    return t.contiguous()
 
 
 def _f32(t):

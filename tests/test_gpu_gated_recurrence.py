@@ -15,6 +15,8 @@ Tolerances are per element and derived from the arithmetic; F = 2^-24, u(T) half
 * What is stored in bfloat16 is off by u of itself, gradients from a sum over n by n F of the magnitudes.
 """
 
+import zlib
+
 import pytest
 import torch
 
@@ -33,7 +35,7 @@ def u(dtype):
 
 
 def gen(*key):
-    return torch.Generator(device=DEV).manual_seed(hash(key) % (2 ** 31))
+    return torch.Generator(device=DEV).manual_seed(zlib.crc32(repr(key).encode()))
 
 
 def within(got, want, tol, what):
@@ -312,6 +314,26 @@ def test_recurrence_layouts(dtype):
     (p,) = torch.autograd.grad(ops.gated_linear_recurrence(xl, r, i, A, h0, seq).sum(), xl)
     (q,) = torch.autograd.grad(ops.gated_linear_recurrence(xl, r, i, A, h0, seq), xl, torch.ones_like(x))
     assert torch.equal(p, q)
+
+
+def test_recurrence_one_position():
+    """A single position has no next one: whatever its stride, forward and backward."""
+    announce("one position")
+    x, r, i, A, h0, _, go, _ = inputs(3, 1, 50, "bf16", carried=True)
+    views = []
+    for t in (x, r, i, go):
+        for stride in (2 ** 21 + 1, 7):
+            v = torch.empty(3 * 50, device=DEV, dtype=x.dtype).as_strided((3, 1, 50), (50, stride, 1))
+            v.copy_(t)
+            views.append(v)
+    want_in = [t.detach().requires_grad_() for t in (x, r, i)]
+    want = ops.gated_linear_recurrence(*want_in, A, h0)
+    for k in (0, 1):
+        leaves = [t.detach().requires_grad_() for t in views[k:6:2]]
+        got = ops.gated_linear_recurrence(*leaves, A, h0)
+        assert torch.equal(got, want)
+        for p, q in zip(torch.autograd.grad(got, leaves, views[6 + k]), torch.autograd.grad(want, want_in, go, retain_graph=True)):
+            assert torch.equal(p, q)
 
 
 def test_recurrence_parameter_types():

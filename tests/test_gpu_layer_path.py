@@ -131,6 +131,37 @@ def test_captured_step():
         assert all(torch.equal(p, q) for p, q in zip(grads, want))
 
 
+def test_two_streams_at_once():
+    """Training steps of two models that run beside each other on two streams, replayed from two graphs too: each as alone."""
+    announce("two streams")
+    sets = [(M.init(53, 64, 96, 2), text(53, 2, 150, 1)), (M.init(61, 128, 72, 1), text(61, 1, 700, 2))]
+    run = lambda p, ids: [*torch.autograd.grad(M.loss_of(p, ids[:, :-1], ids[:, 1:]), M.leaves(p))]
+    want = [run(*s) for s in sets]
+    streams = [torch.cuda.Stream() for _ in sets]
+    for s in streams:
+        s.wait_stream(torch.cuda.current_stream())
+    torch.cuda.synchronize()
+    got = [[], []]
+    for _ in range(5):
+        for k in (0, 1):
+            with torch.cuda.stream(streams[k]):
+                got[k].append(run(*sets[k]))
+    torch.cuda.synchronize()
+    graphs = []
+    for k in (0, 1):
+        graphs.append((torch.cuda.CUDAGraph(), []))
+        with torch.cuda.graph(graphs[k][0], stream=streams[k]):
+            graphs[k][1].extend(run(*sets[k]))
+    for _ in range(3):
+        for k in (0, 1):
+            with torch.cuda.stream(streams[k]):
+                graphs[k][0].replay()
+    torch.cuda.synchronize()
+    for k in (0, 1):
+        for one in (*got[k], graphs[k][1]):
+            assert all(torch.equal(p, q) for p, q in zip(one, want[k]))
+
+
 def test_prompt_then_tokens():
     """A prompt in one call and the tokens behind it one by one: the states and outputs of the whole in one call."""
     announce("prompt then tokens")

@@ -53,6 +53,8 @@ def test_gated_recurrence_refusals():
         refused(name, mk(**bad), -1, "bad sizes")
     refused(name, mk(dtype=L.M2_I32), -2, "dtype")
     refused(name, mk(batch=1 << 31, dim=64), -2, "too many rows")
+    refused(name, mk(batch=1 << 22, dim=1), -2, "too many rows")
+    refused(name, mk(batch=1 << 12, dim=1 << 16), -2, "too many rows")
     for p in ("x", "r", "i", "A", "out"):
         refused(name, mk(**{p: None}), -1, "required")
     for p in "xri":
@@ -109,6 +111,7 @@ def test_gated_linear_refusals():
     refused(name, mk(dtype=L.M2_I64), -2, "dtype")
     refused(name, mk(activation=2), -2, "activation")
     refused(name, mk(dim=1 << 16, ldx=1 << 16, ldw=1 << 16, hidden=1 << 14), -2, "too large")
+    refused(name, mk(hidden=(1 << 21) + 1), -2, "too large")
     for p in ("x", "weight", "out"):
         refused(name, mk(**{p: None}), -1, "required")
     refused(name, mk(workspace=4096, workspace_bytes=need - 1), -4, "workspace")

@@ -574,7 +574,8 @@ int m2_clip_grad_norm(const m2_clip_grad_norm_args* a, void* stream);
  * unchanged, and what x, r and i hold there (they must be readable) reaches nothing.
  * final_states is the state behind the last position.  x, r and i are addressed through their strides of
  * batch and time (elements; channels are contiguous; of time 0, or dim to 2^20), e.g. as slices of one
- * projection's output.  dim <= 2^20, batch ceil(dim / 64) < 2^22.
+ * projection's output.  dim <= 2^20, seqlen < 2^32,
+ * batch ceil(dim / 64) < 2^22.
  * span_states (or NULL) takes the states that enter every M2_RECURRENCE_SPAN positions, which
  * the gradient reads.
  * No counterpart in the reference, whose only recurrence is the SSD's (ops/ssd_naive.py:220-322).

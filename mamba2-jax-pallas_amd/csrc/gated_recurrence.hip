@@ -6,15 +6,22 @@
 //   dx = l beta s;  di = dx x (1 - s);  dL = l (a h[t-1] - a^2 / beta s x);  dr = dL A q (1 - q)
 //   dA = sum dL q;  dh0 = m[0]
 //
-// A workgroup owns the channels of a slab of one batch row and walks its whole length in
-// tiles, forward or backward; the state is carried from tile to tile in registers, so every
-// input is read once and nothing passes between workgroups.  Inside a tile each thread runs TS
-// consecutive steps of V channels; a run of steps is an affine map h -> P h + H, and the maps of the
-// threads of a wavefront (by lane shifts) and then of the wavefronts (by LDS, one barrier a tile)
-// are joined to the state that each thread's run begins with.  The forward leaves the state
-// that enters every span of 32 steps (float32, a sixteenth of a bf16 stream); the backward goes through
-// the tiles from the last to the first, computes the states of a tile again from there and both joins at
-// once (a run's map backward, m -> P m + M, has the same P).
+// A thread runs TS consecutive steps of V channels; a run of steps is an affine map h -> P h + H, and the maps of the
+// threads of a wavefront (by lane shifts) and then of the wavefronts (by LDS) are joined to the state that each thread's run
+// begins with.  A workgroup has 64 channels, so that a step of a bf16 stream is a whole line of 128 bytes.
+//
+// Forward: bound by bytes, three streams read and one written, and nearly by vector instructions (about 60 an element, five of
+// them exponentials, reciprocals and roots).  Workgroups take a segment each of a row's length, hold it in registers, and
+// pass the states on between them, so that every input is read and every gate computed once, with the whole chip
+// busy on a single row: 16384 x 2560 bf16 82-107 us (336 MB, 3.1 to 4.1 TB/s; with a pass of its own for the states 119, all
+// of a slab by one workgroup 580), 8 x 2048 x 5120 165-176 us (671 MB, 3.8 to 4.1 TB/s).
+// It leaves the state that enters every span of 32 steps (float32, a sixteenth of a bf16 stream) for the backward.
+//
+// Backward: a workgroup walks from the last tile to the first, three tiles in flight, computes the states of a tile again
+// from the span's and joins both directions at once (a run's map backward, m -> P m + M, has the same P).  Where there are few
+// slabs a first pass finds what enters the segments of each.  About 100 vector instructions and 14 bytes an
+// element; 8 x 2048 x 5120 332 us (1216 MB, 3.7 TB/s), no faster with the arithmetic taken out (335): the loads and stores of
+// seven streams in lines of 128 bytes.
 //
 // Everything is float32 but what is loaded and stored.  alpha = 1 - a is kept in place of a: near
 // 1, where memories are long, a itself has too few bits (beta^2 = alpha (2 - alpha) loses none,
@@ -43,7 +50,7 @@ constexpr uint32_t NOWHERE = 0xfffffff0u;      // an offset past every end
 template <typename T, int V> struct Raw;
 template <> struct Raw<bf16, 2> {
     uint32_t v;
-    template <int AUX> M2_DEV void load(Rsrc r, uint32_t off, uint32_t soff) { v = __builtin_amdgcn_raw_buffer_load_b32(r, off, soff, AUX); }
+    M2_DEV void load(Rsrc r, uint32_t off, uint32_t soff) { v = __builtin_amdgcn_raw_buffer_load_b32(r, off, soff, 0); }
     M2_DEV void fill(float f) { v = pk_bf16(f, f); }
     M2_DEV float get(int i) const { return i ? bf16_hi(v) : bf16_lo(v); }
     template <int AUX> static M2_DEV void store(Rsrc r, uint32_t off, uint32_t soff, const float (&f)[2]) {
@@ -53,7 +60,7 @@ template <> struct Raw<bf16, 2> {
 template <> struct Raw<float, 2> {
     typedef uint32_t pair __attribute__((ext_vector_type(2)));
     pair v;
-    template <int AUX> M2_DEV void load(Rsrc r, uint32_t off, uint32_t soff) { v = __builtin_amdgcn_raw_buffer_load_b64(r, off, soff, AUX); }
+    M2_DEV void load(Rsrc r, uint32_t off, uint32_t soff) { v = __builtin_amdgcn_raw_buffer_load_b64(r, off, soff, 0); }
     M2_DEV void fill(float f) { v[0] = v[1] = __float_as_uint(f); }
     M2_DEV float get(int i) const { return __uint_as_float(v[i]); }
     template <int AUX> static M2_DEV void store(Rsrc r, uint32_t off, uint32_t soff, const float (&f)[2]) {
@@ -62,8 +69,8 @@ template <> struct Raw<float, 2> {
 };
 template <> struct Raw<bf16, 1> {
     uint32_t v;
-    template <int AUX> M2_DEV void load(Rsrc r, uint32_t off, uint32_t soff) {
-        v = (uint32_t)(uint16_t)__builtin_amdgcn_raw_buffer_load_b16(r, off, soff, AUX) << 16;
+    M2_DEV void load(Rsrc r, uint32_t off, uint32_t soff) {
+        v = (uint32_t)(uint16_t)__builtin_amdgcn_raw_buffer_load_b16(r, off, soff, 0) << 16;
     }
     M2_DEV void fill(float f) { v = __float_as_uint(f); }
     M2_DEV float get(int) const { return __uint_as_float(v); }
@@ -73,7 +80,7 @@ template <> struct Raw<bf16, 1> {
 };
 template <> struct Raw<float, 1> {
     uint32_t v;
-    template <int AUX> M2_DEV void load(Rsrc r, uint32_t off, uint32_t soff) { v = __builtin_amdgcn_raw_buffer_load_b32(r, off, soff, AUX); }
+    M2_DEV void load(Rsrc r, uint32_t off, uint32_t soff) { v = __builtin_amdgcn_raw_buffer_load_b32(r, off, soff, 0); }
     M2_DEV void fill(float f) { v = __float_as_uint(f); }
     M2_DEV float get(int) const { return __uint_as_float(v); }
     template <int AUX> static M2_DEV void store(Rsrc r, uint32_t off, uint32_t soff, const float (&f)[1]) {
@@ -139,20 +146,25 @@ template <bool SEQ> struct Map {
     }
 };
 
+constexpr int TICKET = 32;       // a counter's line, in ints
 struct RecArgs {
     const void *x, *r, *i;
     const float *A, *h0;
     const int32_t* seq;
     int64_t xb, xt, rb, rt, ib, it;      // strides of batch and time
     float* ck;                           // [batch][spans][dim]
-    float2* agg;                         // [batch][segments][dim]: (P, H) of each, or (P, M) back
     int64_t L, spans;
     int dim, slabs, segments;
-    int64_t seg;                         // steps of a segment: whole tiles
     // forward
+    int chains;                          // slabs of all rows
+    int* tickets;                        // [chains] at TICKET: the segment that went out last
+    uint64_t* maps;                      // [batch][segments][dim]: (P, H) of each
+    uint32_t* states;                    // [batch][segments][dim]: behind each
     void* out;
     float* last;
     // backward
+    int64_t seg;                         // steps of a segment: whole tiles
+    float2* agg;                         // [batch][segments][dim]: (P, M) of each
     const void* g;
     int64_t gb, gt;
     const float* glast;
@@ -164,34 +176,41 @@ struct RecArgs {
 // Which channels and steps of a tile a thread has
 template <int V, int LC, int TS, int W> struct Place {
     static constexpr int G = 64 / LC, TILE = G * W * TS, C = V * LC;
-    int b, segment, c, col, tg, w, step, lane;       // col: place in the slab
+    int b, segment, c, col, tg, w, step, lane, slab;       // col: place in the slab, which begins at channel slab
     int64_t t0, end;                     // of the segment
     // A lane that would reach past the last channel has the last V, and stores of them those that no other lane
     // has: all (whole), the second alone (half, of an odd number of channels), none
     bool whole, half;
+    // segment `seg` of a chain: one tile
+    M2_DEV Place(const RecArgs& a, int chain, int seg) { init(a, chain, seg, TILE); }
+    // Of the backward's grid: neighbouring slabs to one XCD where there is one segment (8 x 2048 x 5120 332 us so, 355 in
+    // turn), to all in turn where there are more (3 x 4096 x 5120 310 and 292)
     M2_DEV Place(const RecArgs& a) {
-        lane = threadIdx.x & 63;
-        // Neighbouring slabs to one XCD where there is one pass; to all in turn where there are segments (8 x 2048 x 5120
-        // forward 176 us so, 191 in turn; 16384 x 2560 127 so, 120 in turn)
         const int id = a.segments == 1 ? xcd_remap(blockIdx.x, gridDim.x) : blockIdx.x;
-        const int of = __builtin_amdgcn_readfirstlane(id / a.slabs);
-        b = __builtin_amdgcn_readfirstlane(of / a.segments);
-        segment = of - b * a.segments;
-        t0 = segment * a.seg;
-        end = min(t0 + a.seg, a.L);
+        const int of = __builtin_amdgcn_readfirstlane(id / a.slabs), row = of / a.segments;
+        init(a, row * a.slabs + id - of * a.slabs, of - row * a.segments, a.seg);
+    }
+    M2_DEV void init(const RecArgs& a, int chain, int seg, int64_t steps) {
+        lane = threadIdx.x & 63;
+        b = __builtin_amdgcn_readfirstlane(chain / a.slabs);
+        segment = seg;
+        t0 = segment * steps;
+        end = min(t0 + steps, a.L);
         w = wave_id();
         col = (lane % LC) * V;
         tg = lane / LC;
-        const int from = (id - of * a.slabs) * C + col;
+        slab = (chain - b * a.slabs) * C;
+        const int from = slab + col;
         c = min(from, a.dim - V);
         whole = from == c;
         half = V == 2 && from == c + 1;
         step = (w * G + tg) * TS;
     }
-    template <typename E, int N> M2_DEV void put(E* p, const E (&f)[N]) const {
+    M2_DEV bool owns(int v) const { return whole || (half && v == V - 1); }
+    template <typename E> M2_DEV void put(E* p, const E (&f)[V]) const {
 #pragma unroll
-        for (int v = 0; v < N; ++v)
-            if (whole || (half && v == N - 1)) p[v] = f[v];
+        for (int v = 0; v < V; ++v)
+            if (owns(v)) p[v] = f[v];
     }
     M2_DEV int64_t agg(const RecArgs& a, int s) const { return ((int64_t)b * a.segments + s) * a.dim + c; }
 };
@@ -207,17 +226,15 @@ template <typename T, int V> struct Stream {
     M2_DEV void move(int64_t steps) { base += steps * st; }
     // last: the row's last step, counted from the tile's first
     M2_DEV Rsrc tile(int last) const { return rsrc(base, last * st + row); }
-    template <int AUX, int TS> M2_DEV void load(Raw<T, V> (&r)[TS], int last) const {
+    template <int TS> M2_DEV void load(Raw<T, V> (&r)[TS], int last) const {
         const Rsrc t = tile(last);
 #pragma unroll
-        for (int j = 0; j < TS; ++j) r[j].template load<AUX>(t, off, j * st);
+        for (int j = 0; j < TS; ++j) r[j].load(t, off, j * st);
     }
 };
-// how a walk goes past the caches: not at all, its stores, its loads too (buffer accesses' nt bit)
-enum { CACHED, STORES_NT, ALL_NT };
-constexpr int NT_BIT = 2;
-template <typename T, int V, int NT> struct Output : Stream<T, V> {
-    static constexpr int AUX = NT != CACHED ? NT_BIT : 0;
+// NT: past the caches (buffer accesses' nt bit)
+template <typename T, int V, bool NT> struct Output : Stream<T, V> {
+    static constexpr int AUX = NT ? 2 : 0;
     uint32_t whole, half;    // where this lane stores all of its channels, or the last alone
     bool odd;
     template <class P> M2_DEV Output(const void* p, int64_t offset, const RecArgs& a, const P& at)
@@ -237,7 +254,7 @@ template <typename T, int V, int NT> struct Output : Stream<T, V> {
 // steps); ballots make the bits of them.
 template <int TS, int G, bool SEQ> struct Steps {
     static constexpr int N = G * TS;     // of a wavefront
-    static_assert(!SEQ || N < 16, "a row of lanes");
+    static_assert(!SEQ || N < 32, "");
     int sq;
     uint32_t live, clear;
     // row: of the tile's first step; begins: that is the row's first
@@ -253,7 +270,9 @@ template <int TS, int G, bool SEQ> struct Steps {
         const int first = at.w * N, in = min(max(last + 1 - first, 0), N);       // the wavefront's steps inside the row
         uint32_t l = (1u << in) - 1, c = 0;
         if constexpr (SEQ) {
-            const int before = __builtin_amdgcn_update_dpp(0, sq, 0x111, 0xf, 0xf, true);      // row_shr:1
+            int before;
+            if constexpr (N < 16) before = __builtin_amdgcn_update_dpp(0, sq, 0x111, 0xf, 0xf, true);      // row_shr:1
+            else before = __shfl_up(sq, 1);
             l &= (uint32_t)(__ballot(sq >= 0) >> 1);
             c = l & (uint32_t)(__ballot(sq != before) >> 1);
             if (begins && first == 0) c &= ~1u;
@@ -291,154 +310,212 @@ template <int D, int LC, bool SEQ> M2_DEV Map<SEQ> scan(Map<SEQ>& m, int lane) {
     return Map<SEQ>{has ? e.P : 1.f, has ? e.H : 0.f};
 }
 
-// AGG: only the map of the segment is wanted (a.agg)
-template <typename T, int V, int LC, int TS, int W, bool SEQ, bool AGG, int NT>
+// ---------------------------------------------------------------------------
+// forward
+// ---------------------------------------------------------------------------
+// A workgroup's segment is one tile, held in registers.  A segment's map needs its own inputs alone; the state that enters it
+// is the one of an earlier segment of the chain (a row's slab of channels), carried on by the maps between.  Both are
+// published, and a segment waits until the states and maps of the W segments before it reach its start.
+//
+// Every wait ends: segments are given out by the chain's counter, so whoever waits for a segment knows that its workgroup
+// is running, and of those that run the first in its chain waits for nobody.  Equal inputs give equal bits: from whichever
+// state it starts, a segment applies the same maps to it in the same order.
+constexpr uint32_t UNKNOWN = 0xffffffffu;    // a NaN's bits; what is published has NaNs of one other kind
+M2_DEV uint32_t known(float f) { return f != f ? 0x7fc00000u : __float_as_uint(f); }
+template <typename E> M2_DEV E peek(const E* p) { return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
+template <typename E> M2_DEV void publish(E* p, E v) { __hip_atomic_store(p, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
+
+// everything unknown, every counter at -1
+__global__ void __launch_bounds__(256) k_rec_clear(u32x4* p, int64_t n) {
+    for (int64_t k = (int64_t)blockIdx.x * 256 + threadIdx.x; k < n; k += (int64_t)gridDim.x * 256)
+        p[k] = u32x4{UNKNOWN, UNKNOWN, UNKNOWN, UNKNOWN};
+}
+
+// The state that enters a segment.  Lanes stand for the slab's channels here, a wavefront w for the segment w + 1 before.
+template <int V, bool SEQ, class P, int W> struct Enter {
+    struct Shared {
+        float2 map[2][W][P::C];
+        uint32_t state[2][W][P::C];
+        uint32_t near[P::C];             // the state behind the segment before, if it was known at the start
+    };
+    int l, ch;
+    uint32_t early;
+    M2_DEV int64_t index(const RecArgs& a, const P& at, int seg) const { return ((int64_t)at.b * a.segments + seg) * a.dim + ch; }
+    M2_DEV uint32_t initial(const RecArgs& a, const P& at) const { return a.h0 ? known(a.h0[(int64_t)at.b * a.dim + ch]) : 0; }
+    M2_DEV void begin(const RecArgs& a, const P& at) {
+        l = at.lane % P::C;
+        ch = min(at.slab + l, a.dim - 1);
+        if (at.w == 0) early = at.segment > 0 ? peek(a.states + index(a, at, at.segment - 1)) : initial(a, at);
+    }
+    // before a barrier
+    M2_DEV void meet(const P& at, Shared& s) const {
+        if (at.w == 0) s.near[l] = early;
+    }
+    // behind it, in all wavefronts
+    M2_DEV void end(const RecArgs& a, const P& at, Shared& s, float (&h)[V]) const {
+        auto place = [&](int v) { return max(at.c - at.slab + v, 0); };      // (below 0: of a lane that stores nothing there)
+        if (__all(s.near[l] != UNKNOWN)) {
+#pragma unroll
+            for (int v = 0; v < V; ++v) h[v] = __uint_as_float(s.near[place(v)]);
+            return;
+        }
+        const int seg = at.segment - 1 - at.w;
+        uint64_t m = ~0ull;
+        uint32_t st = seg < 0 ? initial(a, at) : UNKNOWN;      // (before the row's start: nobody gets that far)
+        int buf = 0;
+        for (;; buf ^= 1) {
+            if (seg >= 0) {
+                st = peek(a.states + index(a, at, seg));
+                m = peek(a.maps + index(a, at, seg));
+            }
+            s.map[buf][at.w][l] = make_float2(__uint_as_float((uint32_t)m), __uint_as_float((uint32_t)(m >> 32)));
+            s.state[buf][at.w][l] = st;
+            lds_barrier();
+            // a state, and maps from there on
+            bool found = false, gap = false;
+#pragma unroll
+            for (int k = 0; k < W; ++k) {
+                const bool is = s.state[buf][k][l] != UNKNOWN;
+                found |= is && !gap;
+                gap |= !is && __float_as_uint(s.map[buf][k][l].x) == UNKNOWN;
+            }
+            if (__all(found)) break;             // (all wavefronts have read the same)
+            __builtin_amdgcn_s_sleep(4);
+        }
+#pragma unroll
+        for (int v = 0; v < V; ++v) {
+            h[v] = 0.f;
+#pragma unroll
+            for (int k = W - 1; k >= 0; --k) {
+                const uint32_t is = s.state[buf][k][place(v)];
+                const float2 p = s.map[buf][k][place(v)];
+                h[v] = is != UNKNOWN ? __uint_as_float(is) : Map<SEQ>{p.x, p.y}.of(h[v]);
+            }
+        }
+    }
+};
+
+template <typename T, int V, int LC, int TS, int W, bool SEQ, bool NT>
 __global__ void __launch_bounds__(W * 64, 4) k_rec_forward(RecArgs a) {
     typedef Place<V, LC, TS, W> P;
-    constexpr int LD = NT == ALL_NT ? NT_BIT : 0;
-    __shared__ float2 tot[3][W][P::C];
-    const P at(a);
-    if (AGG && at.segment == a.segments - 1) return;     // (nothing follows it)
-    Stream<T, V> sx(a.x, at.b * a.xb + at.t0 * a.xt, a.xt, a, at), sr(a.r, at.b * a.rb + at.t0 * a.rt, a.rt, a, at),
+    typedef Enter<V, SEQ, P, W> E;
+    __shared__ float2 tot[W][P::C];
+    __shared__ typename E::Shared look;
+    __shared__ int next;
+    const int chain = blockIdx.x % a.chains;
+    int segment = 0;
+    if (a.segments > 1) {
+        if (threadIdx.x == 0)
+            next = __hip_atomic_fetch_add(a.tickets + chain * TICKET, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) + 1;
+        lds_barrier();
+        segment = __builtin_amdgcn_readfirstlane(next);
+    }
+    const P at(a, chain, segment);
+    const bool ends = segment == a.segments - 1;
+    E en;
+    en.begin(a, at);
+    const Stream<T, V> sx(a.x, at.b * a.xb + at.t0 * a.xt, a.xt, a, at), sr(a.r, at.b * a.rb + at.t0 * a.rt, a.rt, a, at),
         si(a.i, at.b * a.ib + at.t0 * a.it, a.it, a, at);
-    Output<T, V, NT> so(a.out, (at.b * a.L + at.t0) * a.dim, a, at);
-    const int32_t* seq = SEQ ? a.seq + at.b * a.L : nullptr;
+    const Output<T, V, NT> so(a.out, (at.b * a.L + at.t0) * a.dim, a, at);
+    const int last = (int)(at.end - 1 - at.t0);
+    Raw<T, V> x[TS], r[TS], i[TS];
+    Steps<TS, P::G, SEQ> s;
+    sr.load(r, last);
+    sx.load(x, last);
+    si.load(i, last);
+    s.load(SEQ ? a.seq + at.b * a.L + at.t0 : nullptr, segment == 0, at, last);
     float A[V];
-    Map<SEQ> h[V];               // from the segment's start on; but for AGG its H is the state
     bool far = false;
 #pragma unroll
     for (int v = 0; v < V; ++v) {
         A[v] = a.A[at.c + v];
         far |= !(A[v] >= NEAR);
-        h[v] = Map<SEQ>{1.f, 0.f};
-        if (!AGG && a.h0) h[v].H = a.h0[(int64_t)at.b * a.dim + at.c + v];
     }
     far = __any(far);
-    if (!AGG) {
-#pragma unroll 4
-        for (int u = 0; u < at.segment; ++u)
+    if ((SEQ || last != P::TILE - 1) && !s.set(segment == 0, at, last)) {
 #pragma unroll
-            for (int v = 0; v < V; ++v) {
-                const float2 p = a.agg[at.agg(a, u) + v];
-                h[v].H = Map<SEQ>{p.x, p.y}.of(h[v].H);
+        for (int j = 0; j < TS; ++j)
+            if (!s.is_live(j)) {             // a = 1, nothing added
+                x[j].fill(0.f);
+                r[j].fill(-INF);
+                i[j].fill(0.f);
             }
     }
-    auto last_of = [&](int64_t t0) { return (int)min(at.end - 1 - t0, (int64_t)P::TILE - 1); };
-    struct Tile {
-        Raw<T, V> x[TS], r[TS], i[TS];
-        Steps<TS, P::G, SEQ> s;
-    } one, two, three;
-    auto load = [&](Tile& n, int64_t t0) {
-        const int last = last_of(t0);
-        sx.template load<LD>(n.x, last);
-        sr.template load<LD>(n.r, last);
-        si.template load<LD>(n.i, last);
-        n.s.load(seq + t0, t0 == 0, at, last);
-        sx.move(P::TILE);
-        sr.move(P::TILE);
-        si.move(P::TILE);
-    };
-    // tile c, while the next one is loaded into n
-    auto tile = [&](Tile& c, Tile& n, int64_t t0, int buf) {
-        const int last = last_of(t0);
-        if (t0 + 2 * P::TILE < at.end) load(n, t0 + 2 * P::TILE);
-        if ((SEQ || last != P::TILE - 1) && !c.s.set(t0 == 0, at, last)) {
+    // the gates, and the map of this thread's steps
+    float al[TS][V], add[TS][V], L[TS][V];
 #pragma unroll
-            for (int j = 0; j < TS; ++j)
-                if (!c.s.is_live(j)) {           // a = 1, nothing added
-                    c.x[j].fill(0.f);
-                    c.r[j].fill(-INF);
-                    c.i[j].fill(0.f);
-                }
-        }
-        // the gates, and the map of this thread's steps
-        float al[TS][V], add[TS][V], L[TS][V];
-#pragma unroll
-        for (int j = 0; j < TS; ++j)
-#pragma unroll
-            for (int v = 0; v < V; ++v) {
-                const float q = sigmoid_of(exp_neg(c.r[j].get(v))), s = sigmoid_of(exp_neg(c.i[j].get(v)));
-                L[j][v] = A[v] * q;
-                al[j][v] = decay_near(L[j][v]);
-                add[j][v] = s * c.x[j].get(v);
-            }
-        decay_far<TS, V>(al, L, far);
-#pragma unroll
-        for (int j = 0; j < TS; ++j)
-#pragma unroll
-            for (int v = 0; v < V; ++v) add[j][v] *= __builtin_amdgcn_sqrtf(al[j][v] * (2.f - al[j][v]));
-        Map<SEQ> m[V], ex[V];
+    for (int j = 0; j < TS; ++j)
 #pragma unroll
         for (int v = 0; v < V; ++v) {
-            m[v] = Map<SEQ>{1.f - al[0][v], add[0][v]};
-#pragma unroll
-            for (int j = 1; j < TS; ++j) {
-                m[v].P = fmaf(-al[j][v], m[v].P, m[v].P);
-                m[v].H = step(al[j][v], c.s.clears(j) ? 0.f : m[v].H, add[j][v]);
-            }
-            if (SEQ && c.s.clear) m[v].P = -1.f;
-            ex[v] = scan<1, LC, SEQ>(m[v], at.lane);
-            if (at.tg == P::G - 1) tot[buf][at.w][at.col + v] = make_float2(m[v].P, m[v].H);
+            L[j][v] = A[v] * sigmoid_of(exp_neg(r[j].get(v)));
+            al[j][v] = decay_near(L[j][v]);
         }
-        lds_barrier();
-        float e[V];
+    decay_far<TS, V>(al, L, far);
+    Map<SEQ> m[V], ex[V];
 #pragma unroll
-        for (int u = 0; u < W; ++u) {
-            if (!AGG && u == at.w) {
-                asm volatile("");                // (a branch: it is the wavefront's)
+    for (int v = 0; v < V; ++v) {
 #pragma unroll
-                for (int v = 0; v < V; ++v) e[v] = h[v].H;
-            }
-#pragma unroll
-            for (int v = 0; v < V; ++v) {
-                const float2 p = tot[buf][u][at.col + v];
-                const Map<SEQ> t{p.x, p.y};
-                if (AGG) h[v] = t.after(h[v]);
-                else h[v].H = t.of(h[v].H);
-            }
+        for (int j = 0; j < TS; ++j) {
+            add[j][v] = sigmoid_of(exp_neg(i[j].get(v))) * x[j].get(v) * __builtin_amdgcn_sqrtf(al[j][v] * (2.f - al[j][v]));
+            m[v].P = j == 0 ? 1.f - al[j][v] : fmaf(-al[j][v], m[v].P, m[v].P);
+            m[v].H = j == 0 ? add[j][v] : step(al[j][v], s.clears(j) ? 0.f : m[v].H, add[j][v]);
         }
-        if constexpr (!AGG) {
-#pragma unroll
-            for (int v = 0; v < V; ++v) e[v] = ex[v].of(e[v]);
-            if (a.ck && at.step % SPAN == 0 && at.step <= last)
-                at.put(a.ck + (at.b * a.spans + (t0 + at.step) / SPAN) * a.dim + at.c, e);
-            const Rsrc to = so.tile(last);
-#pragma unroll
-            for (int j = 0; j < TS; ++j) {
-                float o[V];
-#pragma unroll
-                for (int v = 0; v < V; ++v) {
-                    e[v] = step(al[j][v], c.s.clears(j) ? 0.f : e[v], add[j][v]);
-                    o[v] = SEQ && !c.s.is_live(j) ? 0.f : e[v];
-                }
-                so.store(to, j, o);
-            }
-            so.move(P::TILE);
-        }
-    };
-    load(one, at.t0);
-    if (at.t0 + P::TILE < at.end) load(two, at.t0 + P::TILE);
-    for (int64_t t0 = at.t0; t0 < at.end; t0 += 3 * P::TILE) {
-        tile(one, three, t0, 0);
-        if (t0 + P::TILE >= at.end) break;
-        tile(two, one, t0 + P::TILE, 1);
-        if (t0 + 2 * P::TILE >= at.end) break;
-        tile(three, two, t0 + 2 * P::TILE, 2);
+        if (SEQ && s.clear) m[v].P = -1.f;
+        ex[v] = scan<1, LC, SEQ>(m[v], at.lane);
+        if (at.tg == P::G - 1) tot[at.w][at.col + v] = make_float2(m[v].P, m[v].H);
     }
-    if (at.w != 0 || at.tg != 0) return;
-    if constexpr (AGG) {
-        float2 o[V];
+    en.meet(at, look);
+    lds_barrier();
+    auto of_wave = [&](int u, int v) {
+        const float2 p = tot[u][at.col + v];
+        return Map<SEQ>{p.x, p.y};
+    };
+    const bool one = at.w == 0 && at.tg == 0;
+    Map<SEQ> all[V];             // of the segment
+    if (one) {
 #pragma unroll
-        for (int v = 0; v < V; ++v) o[v] = make_float2(h[v].P, h[v].H);
-        at.put(a.agg + at.agg(a, at.segment), o);
-    } else if (a.last && at.segment == a.segments - 1) {
+        for (int v = 0; v < V; ++v) {
+            all[v] = of_wave(0, v);
+#pragma unroll
+            for (int u = 1; u < W; ++u) all[v] = of_wave(u, v).after(all[v]);
+            if (!ends && at.owns(v))
+                publish(a.maps + at.agg(a, segment) + v, (uint64_t)known(all[v].P) | (uint64_t)__float_as_uint(all[v].H) << 32);
+        }
+    }
+    float h[V];
+    en.end(a, at, look, h);
+    if (one) {
         float o[V];
 #pragma unroll
-        for (int v = 0; v < V; ++v) o[v] = h[v].H;
-        at.put(a.last + (int64_t)at.b * a.dim + at.c, o);
+        for (int v = 0; v < V; ++v) {
+            o[v] = all[v].of(h[v]);
+            if (!ends && at.owns(v)) publish(a.states + at.agg(a, segment) + v, known(o[v]));
+        }
+        if (ends && a.last) at.put(a.last + (int64_t)at.b * a.dim + at.c, o);
+    }
+    for (int u = 0; u < at.w; ++u)
+#pragma unroll
+        for (int v = 0; v < V; ++v) h[v] = of_wave(u, v).of(h[v]);
+#pragma unroll
+    for (int v = 0; v < V; ++v) h[v] = ex[v].of(h[v]);
+    if (a.ck && at.step % SPAN == 0 && at.step <= last)
+        at.put(a.ck + (at.b * a.spans + (at.t0 + at.step) / SPAN) * a.dim + at.c, h);
+    const Rsrc to = so.tile(last);
+#pragma unroll
+    for (int j = 0; j < TS; ++j) {
+        float o[V];
+#pragma unroll
+        for (int v = 0; v < V; ++v) {
+            h[v] = step(al[j][v], s.clears(j) ? 0.f : h[v], add[j][v]);
+            o[v] = SEQ && !s.is_live(j) ? 0.f : h[v];
+        }
+        so.store(to, j, o);
     }
 }
 
+// ---------------------------------------------------------------------------
+// backward
+// ---------------------------------------------------------------------------
 // The map of each segment but the first from its end back: of r and the upstream gradient alone
 template <typename T, int V, int LC, int TS, int W, bool SEQ>
 __global__ void __launch_bounds__(W * 64, 4) k_rec_back_agg(RecArgs a) {
@@ -466,8 +543,8 @@ __global__ void __launch_bounds__(W * 64, 4) k_rec_back_agg(RecArgs a) {
     } one, two, three;
     auto load = [&](Tile& n, int64_t t0) {
         const int last = last_of(t0);
-        sr.template load<0>(n.r, last);
-        sg.template load<0>(n.g, last);
+        sr.load(n.r, last);
+        sg.load(n.g, last);
         n.s.load(seq + t0, t0 == 0, at, last);
         sr.move(-P::TILE);
         sg.move(-P::TILE);
@@ -531,10 +608,9 @@ __global__ void __launch_bounds__(W * 64, 4) k_rec_back_agg(RecArgs a) {
     at.put(a.agg + at.agg(a, at.segment), o);
 }
 
-template <typename T, int V, int LC, int TS, int W, bool SEQ, int NT>
+template <typename T, int V, int LC, int TS, int W, bool SEQ, bool NT>
 __global__ void __launch_bounds__(W * 64, 2) k_rec_backward(RecArgs a) {
     typedef Place<V, LC, TS, W> P;
-    constexpr int LD = NT == ALL_NT ? NT_BIT : 0;
     static_assert(P::TILE % SPAN == 0, "");
     __shared__ float tot[3][3][W][P::C];
     const P at(a);
@@ -570,10 +646,10 @@ __global__ void __launch_bounds__(W * 64, 2) k_rec_backward(RecArgs a) {
     } one, two, three;
     auto load = [&](Tile& n, int64_t t0) {
         const int last = last_of(t0);
-        sx.template load<LD>(n.x, last);
-        sr.template load<LD>(n.r, last);
-        si.template load<LD>(n.i, last);
-        sg.template load<LD>(n.g, last);
+        sx.load(n.x, last);
+        sr.load(n.r, last);
+        si.load(n.i, last);
+        sg.load(n.g, last);
 #pragma unroll
         for (int v = 0; v < V; ++v) n.e[v] = ck[t0 / SPAN * a.dim + v];
         n.s.load(seq + t0, t0 == 0, at, last);
@@ -763,51 +839,76 @@ template <typename T> __global__ void __launch_bounds__(64) k_rec_step(StepArgs 
 // ---------------------------------------------------------------------------
 // launches
 // ---------------------------------------------------------------------------
-constexpr int LC = 32, TS = 4;
-// Segments of a row's length, and their steps: where the slabs alone leave CUs idle, as many as make five workgroups a CU,
-// of 128 steps at least; a pass more over the inputs then finds what enters each.  One segment
-// against many, us: 40 slabs x 16384 forward 580 and 122; 160 x 4096 131 and 119, backward 298 and 196; 240 149 and
-// 234, 309 and 306; 320 221 and 273, 432 and 367; 480 x 2048 132 and 204, 246 and 271 (the backward's pass reads two
-// inputs of four, the forward's all three).
-int segments(int64_t batch, int64_t L, int64_t dim, bool back, int64_t& seg) {
+constexpr int LC = 32;
+// Steps of a forward segment, 16 for each wavefront.  us for 64, 128, 256 of them: 160 chains x 4096 74, 86, 112; 240 131, 144,
+// 145; 640 x 2048 165, 177, 180.  A chain's counter gives out a segment every 0.43 us, which bounds few chains: 40 x 16384
+// 128, 95, 121; 16 x 16384 119, 60, 62; 8 x 16384 119, 58, 44.  One segment needs no counter: 2560 x 100 steps 38, 34, 69.
+int forward_steps(int64_t batch, int64_t L, int64_t dim) {
+    const int64_t chains = batch * ((dim + 2 * LC - 1) / (2 * LC));
+    return L <= 128 || (chains >= 16 && chains < m2::cu_count() / 2) ? 128 : chains < 16 ? 256 : 64;
+}
+// counters, maps, states
+struct ForwardPlan {
+    int64_t segments;
+    size_t maps, states, total;
+};
+ForwardPlan forward_plan(int64_t batch, int64_t L, int64_t dim) {
+    const int steps = forward_steps(batch, L, dim);
+    ForwardPlan p{(L + steps - 1) / steps};
+    if (p.segments <= 1) return p;
+    const size_t n = (size_t)batch * p.segments * dim;
+    p.maps = 4 * TICKET * (size_t)batch * ((dim + 2 * LC - 1) / (2 * LC));
+    p.states = p.maps + 8 * n;
+    p.total = (p.states + 4 * n + 15) / 16 * 16;
+    return p;
+}
+// Segments of the backward, and their steps: where the slabs alone leave CUs idle, as many as make five workgroups a CU,
+// of 128 steps at least; a pass more over two of the inputs then finds what enters each.  One segment
+// against many, us: 160 slabs x 4096 298 and 196; 240 309 and 306; 320 432 and 367; 480 x 2048 246 and 271.
+// (The forward's way, each segment waiting for others, takes 222 for 40 slabs x 16384, 191 so; 640 x 2048 362 and 327: a
+// segment's four inputs and its factors leave registers for two workgroups a CU, and none of them loads ahead.)
+int segments(int64_t batch, int64_t L, int64_t dim, int64_t& seg) {
     constexpr int64_t UNIT = 128;
     const int64_t units = L > 0 ? (L + UNIT - 1) / UNIT : 1, slabs = batch * ((dim + 2 * LC - 1) / (2 * LC));
     const int64_t ncu = m2::cu_count();
     int64_t s = 1;
-    if (slabs > 0 && slabs < (back ? ncu * 3 / 2 : ncu * 3 / 4)) s = (5 * ncu + slabs - 1) / slabs;
+    if (slabs > 0 && slabs < ncu * 3 / 2) s = (5 * ncu + slabs - 1) / slabs;
     if (s > units) s = units;
     const int64_t per = (units + s - 1) / s;
     seg = per * UNIT;
     return (int)((units + per - 1) / per);
 }
 
-template <typename T, int V, bool SEQ, bool NT> void launch(RecArgs a, int64_t batch, bool back, hipStream_t s) {
-    a.slabs = (a.dim + V * LC - 1) / (V * LC);
-    const dim3 grid((unsigned)(batch * a.segments * a.slabs));
+template <typename T, int V, bool SEQ, bool NT> void launch_forward(const RecArgs& a, int steps, hipStream_t s) {
+    const dim3 grid((unsigned)((int64_t)a.chains * a.segments));
     auto go = [&](auto k, int w) { hipLaunchKernelGGL(k, grid, dim3(w * 64), 0, s, a); };
-    constexpr int ALL = NT ? ALL_NT : CACHED, STORES = NT ? STORES_NT : CACHED;
-    if (back) {
-        if (a.segments > 1) {
-            go(k_rec_back_agg<T, V, LC, TS, 4, SEQ>, 4);
-            go(k_rec_backward<T, V, LC, TS, 4, SEQ, STORES>, 4);
-        } else {
-            go(k_rec_backward<T, V, LC, TS, 4, SEQ, ALL>, 4);
-        }
-    } else if (a.segments > 1) {
-        go(k_rec_forward<T, V, LC, TS, 4, SEQ, true, CACHED>, 4);
-        go(k_rec_forward<T, V, LC, TS, 4, SEQ, false, STORES>, 4);
-    } else {
-        go(k_rec_forward<T, V, LC, TS, 8, SEQ, false, ALL>, 8);
-    }
+    if (steps == 64) go(k_rec_forward<T, V, LC, 8, 4, SEQ, NT>, 4);
+    else if (steps == 128) go(k_rec_forward<T, V, LC, 8, 8, SEQ, NT>, 8);
+    else go(k_rec_forward<T, V, LC, 8, 16, SEQ, NT>, 16);
 }
-template <typename T> void run(const RecArgs& a, int64_t batch, bool back, hipStream_t s) {
-    // Past the caches where what is read and written does not fit the last of them (256 MB): results would take the place of
-    // what is read again (the second pass over a segment) or next.  16384 x 2560 forward 136 us so, 122 with
-    // the results past them; 8 x 2048 x 5120, one pass, 188 and 171 with the inputs past them too.
-    const bool nt = batch * a.L * a.dim * (int64_t)sizeof(T) * (back ? 7 : 4) > (256ll << 20);
+template <typename T, int V, bool SEQ, bool NT> void launch_backward(const RecArgs& a, hipStream_t s) {
+    const dim3 grid((unsigned)((int64_t)a.chains * a.segments));
+    auto go = [&](auto k) { hipLaunchKernelGGL(k, grid, dim3(256), 0, s, a); };
+    if (a.segments > 1) go(k_rec_back_agg<T, V, LC, 4, 4, SEQ>);
+    go(k_rec_backward<T, V, LC, 4, 4, SEQ, NT>);
+}
+// steps: of a forward segment, or 0: backward
+template <typename T> void run(RecArgs a, int64_t batch, int steps, hipStream_t s) {
+    a.slabs = a.dim == 1 ? 1 : (a.dim + 2 * LC - 1) / (2 * LC);
+    a.chains = (int)batch * a.slabs;
+    // Results go past the caches where what is read and written does not fit the last of them (256 MB): they would take
+    // the place of what is read next, or again.  us with and without: 16384 x 2560 forward 107 and 109, backward 197 and 211;
+    // 8 x 2048 x 5120 176 and 181, 332 and 341.
+    const bool nt = batch * a.L * a.dim * (int64_t)sizeof(T) * (steps ? 4 : 7) > (256ll << 20);
     auto go = [&](auto seq, auto many) {
-        if (a.dim == 1) launch<T, 1, decltype(seq)::value, false>(a, batch, back, s);
-        else launch<T, 2, decltype(seq)::value, decltype(many)::value>(a, batch, back, s);
+        constexpr bool SEQ = decltype(seq)::value, NT = decltype(many)::value;
+        if (steps) {
+            if (a.dim == 1) launch_forward<T, 1, SEQ, false>(a, steps, s);
+            else launch_forward<T, 2, SEQ, NT>(a, steps, s);
+        } else {
+            if (a.dim == 1) launch_backward<T, 1, SEQ, false>(a, s);
+            else launch_backward<T, 2, SEQ, NT>(a, s);
+        }
     };
     if (a.seq) {
         if (nt) go(std::true_type(), std::true_type());
@@ -825,7 +926,7 @@ bool stride_ok(int64_t st, int64_t dim) { return st == 0 || (st >= dim && st <= 
 
 // what a call may ask for, whichever it is
 int check_sizes(const char* who, int64_t batch, int64_t seqlen, int64_t dim, int dtype) {
-    M2_REQUIRE(batch >= 0 && seqlen >= 0 && dim > 0 && dim <= MAX_STRIDE && seqlen < (1ll << 40), M2_ERR_INVALID,
+    M2_REQUIRE(batch >= 0 && seqlen >= 0 && dim > 0 && dim <= MAX_STRIDE && seqlen < (1ll << 32), M2_ERR_INVALID,
                "%s: bad sizes (batch %lld, seqlen %lld, dim %lld)", who, (long long)batch, (long long)seqlen,
                (long long)dim);
     M2_REQUIRE(dtype == M2_F32 || dtype == M2_BF16, M2_ERR_UNSUPPORTED, "%s: dtype %d", who, dtype);
@@ -840,9 +941,8 @@ namespace m2 {
 
 size_t gated_recurrence_workspace(const m2_gated_recurrence_args& a) {
     if (check_sizes("gated_linear_recurrence", a.batch, a.seqlen, a.dim, a.dtype)) return 0;
-    int64_t seg;
-    const int n = segments(a.batch, a.seqlen, a.dim, false, seg);
-    return n > 1 ? 8 * (size_t)a.batch * n * a.dim : 256;
+    const size_t b = forward_plan(a.batch, a.seqlen, a.dim).total;
+    return b ? b : 256;
 }
 
 int launch_gated_recurrence(const m2_gated_recurrence_args& a, hipStream_t s) {
@@ -866,20 +966,30 @@ int launch_gated_recurrence(const m2_gated_recurrence_args& a, hipStream_t s) {
     k.ib = a.i_stride_batch; k.it = a.i_stride_time;
     k.ck = a.span_states; k.L = a.seqlen; k.spans = (a.seqlen + SPAN - 1) / SPAN; k.dim = (int)a.dim;
     k.out = a.out; k.last = a.final_states;
-    k.segments = segments(a.batch, a.seqlen, a.dim, false, k.seg);
-    const size_t need = gated_recurrence_workspace(a);
-    M2_REQUIRE(k.segments == 1 || (a.workspace && a.workspace_bytes >= need), M2_ERR_WORKSPACE,
-               "%s: workspace of %zu bytes needed, %zu given", who, need, a.workspace_bytes);
-    k.agg = static_cast<float2*>(a.workspace);
-    if (a.dtype == M2_F32) run<float>(k, a.batch, false, s);
-    else run<bf16>(k, a.batch, false, s);
+    const int steps = forward_steps(a.batch, a.seqlen, a.dim);
+    const ForwardPlan p = forward_plan(a.batch, a.seqlen, a.dim);
+    M2_REQUIRE(a.batch * ((a.dim + 63) / 64) * p.segments * (4 * steps) < (1ll << 32), M2_ERR_UNSUPPORTED, "%s: too many steps", who);
+    M2_REQUIRE(p.total == 0 || (a.workspace && a.workspace_bytes >= p.total), M2_ERR_WORKSPACE,
+               "%s: workspace of %zu bytes needed, %zu given", who, p.total, a.workspace_bytes);
+    k.segments = (int)p.segments;
+    if (p.segments > 1) {
+        char* ws = static_cast<char*>(a.workspace);
+        k.tickets = reinterpret_cast<int*>(ws);
+        k.maps = reinterpret_cast<uint64_t*>(ws + p.maps);
+        k.states = reinterpret_cast<uint32_t*>(ws + p.states);
+        const int64_t n = (int64_t)(p.total / 16);
+        hipLaunchKernelGGL(k_rec_clear, dim3((unsigned)(n < (1 << 18) ? (n + 255) / 256 : 1024)), dim3(256), 0, s,
+                           reinterpret_cast<u32x4*>(ws), n);
+    }
+    if (a.dtype == M2_F32) run<float>(k, a.batch, steps, s);
+    else run<bf16>(k, a.batch, steps, s);
     return check_launch(who);
 }
 
 size_t gated_recurrence_grad_workspace(const m2_gated_recurrence_grad_args& a) {
     if (check_sizes("gated_linear_recurrence_grad", a.batch, a.seqlen, a.dim, a.dtype)) return 0;
     int64_t seg;
-    const size_t n = segments(a.batch, a.seqlen, a.dim, true, seg) * (size_t)(a.batch > 1 ? a.batch : 1);
+    const size_t n = segments(a.batch, a.seqlen, a.dim, seg) * (size_t)(a.batch > 1 ? a.batch : 1);
     return 12 * n * a.dim;
 }
 
@@ -905,12 +1015,12 @@ int launch_gated_recurrence_grad(const m2_gated_recurrence_grad_args& a, hipStre
     k.g = a.grad_out; k.gb = a.grad_out_stride_batch; k.gt = a.grad_out_stride_time;
     k.glast = a.grad_final_states;
     k.dx = a.grad_x; k.dr = a.grad_r; k.di = a.grad_i; k.dh0 = a.grad_initial_states;
-    k.segments = segments(a.batch, a.seqlen, a.dim, true, k.seg);
+    k.segments = segments(a.batch, a.seqlen, a.dim, k.seg);
     const int64_t parts = a.batch * k.segments;
     k.agg = static_cast<float2*>(a.workspace);
     k.dA = parts == 1 ? a.grad_A : static_cast<float*>(a.workspace) + 2 * parts * a.dim;
-    if (a.dtype == M2_F32) run<float>(k, a.batch, true, s);
-    else run<bf16>(k, a.batch, true, s);
+    if (a.dtype == M2_F32) run<float>(k, a.batch, 0, s);
+    else run<bf16>(k, a.batch, 0, s);
     if (parts > 1)
         hipLaunchKernelGGL(k_rec_join, dim3((unsigned)((a.dim + 63) / 64)), dim3(64), 0, s, k.dA, a.grad_A, parts, a.dim);
     return check_launch(who);

@@ -336,6 +336,42 @@ def test_recurrence_one_position():
             assert torch.equal(p, q)
 
 
+@pytest.mark.parametrize("batch,seqlen,dim", [(1, 3001, 65), (1, 2999, 1409), (3, 1025, 4161), (130, 129, 1), (3, 128, 130), (3, 129, 130)])
+@pytest.mark.parametrize("packed", [0, 400])
+def test_recurrence_segments(batch, seqlen, dim, packed):
+    """Segments of every length, of few and of many chains, whose last slab has a single channel; and the same bits
+    every time, with other work beside it."""
+    announce("segments", batch, seqlen, dim, packed)
+    x, r, i, A, h0, seq, go, gl = sets = inputs(batch, seqlen, dim, "f32", packed=packed, carried=True)
+    check(*sets)
+    want = ops.gated_linear_recurrence(x, r, i, A, h0, seq, True)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    for _ in range(4):
+        with torch.cuda.stream(side):
+            other = ops.gated_linear_recurrence(x, r, i, A, h0, seq, True)
+        got = ops.gated_linear_recurrence(x, r, i, A, h0, seq, True)
+        torch.cuda.synchronize()
+        assert all(torch.equal(p, q) for p, q in zip(got, want)) and all(torch.equal(p, q) for p, q in zip(other, want))
+
+
+def test_recurrence_any_not_a_number():
+    """NaNs of all bits (and of all ones, which stand for what is not known yet) go on like any value."""
+    announce("any NaN")
+    x, r, i, A, h0, _, _, _ = inputs(2, 1500, 70, "f32", carried=True)
+    for bits in (-1, 0x7fc00000, 0x7f800001):
+        for where in (x, r, i, h0):
+            t = where.clone()
+            place = (0, 5) if where is h0 else (0, 300, 5)
+            t.view(torch.int32)[place] = bits
+            assert bool(t[place].isnan())
+            h = ops.gated_linear_recurrence(*(t if where is q else q for q in (x, r, i)), A, t if where is h0 else h0)
+            after = 0 if where is h0 else 300
+            assert bool(h[0, after:, 5].isnan().all())
+            h[0, after:, 5] = 0
+            assert bool(h.isfinite().all())
+
+
 def test_recurrence_parameter_types():
     """A and the states in bfloat16: their gradients come back in it."""
     announce("parameter types")

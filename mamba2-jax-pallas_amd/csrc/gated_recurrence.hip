@@ -19,9 +19,9 @@
 //
 // Backward: a workgroup walks from the last tile to the first, three tiles in flight, computes the states of a tile again
 // from the span's and joins both directions at once (a run's map backward, m -> P m + M, has the same P).  Where there are few
-// slabs a first pass finds what enters the segments of each.  About 100 vector instructions and 14 bytes an
-// element; 8 x 2048 x 5120 332 us (1216 MB, 3.7 TB/s), no faster with the arithmetic taken out (335): the loads and stores of
-// seven streams in lines of 128 bytes.
+// slabs a first pass finds what enters the segments of each; where there are more than run at once, segments pass it on.
+// About 100 vector instructions and 14 bytes an element: 8 x 2048 x 5120 294 us (1216 MB, 4.1 TB/s), 8 x 2048 x 4096, whose
+// 512 slabs run at once, 218-235 (973 MB, 4.1 to 4.5 TB/s).
 //
 // Everything is float32 but what is loaded and stored.  alpha = 1 - a is kept in place of a: near
 // 1, where memories are long, a itself has too few bits (beta^2 = alpha (2 - alpha) loses none,
@@ -155,11 +155,11 @@ struct RecArgs {
     float* ck;                           // [batch][spans][dim]
     int64_t L, spans;
     int dim, slabs, segments;
-    // forward
     int chains;                          // slabs of all rows
-    int* tickets;                        // [chains] at TICKET: the segment that went out last
+    int* tickets;                        // [chains] at TICKET: how many segments went out, less one
+    uint32_t* states;                    // [batch][segments][dim]: what each passes on
+    // forward
     uint64_t* maps;                      // [batch][segments][dim]: (P, H) of each
-    uint32_t* states;                    // [batch][segments][dim]: behind each
     void* out;
     float* last;
     // backward
@@ -183,8 +183,9 @@ template <int V, int LC, int TS, int W> struct Place {
     bool whole, half;
     // segment `seg` of a chain: one tile
     M2_DEV Place(const RecArgs& a, int chain, int seg) { init(a, chain, seg, TILE); }
-    // Of the backward's grid: neighbouring slabs to one XCD where there is one segment (8 x 2048 x 5120 332 us so, 355 in
-    // turn), to all in turn where there are more (3 x 4096 x 5120 310 and 292)
+    M2_DEV Place(const RecArgs& a, int chain, int seg, int64_t steps) { init(a, chain, seg, steps); }
+    // Of the grid of segments that are independent: neighbouring slabs to one XCD where there is one segment (8 x 2048 x 5120
+    // 332 us so, 355 in turn), to all in turn where there are more (3 x 4096 x 5120 310 and 292)
     M2_DEV Place(const RecArgs& a) {
         const int id = a.segments == 1 ? xcd_remap(blockIdx.x, gridDim.x) : blockIdx.x;
         const int of = __builtin_amdgcn_readfirstlane(id / a.slabs), row = of / a.segments;
@@ -325,6 +326,14 @@ M2_DEV uint32_t known(float f) { return f != f ? 0x7fc00000u : __float_as_uint(f
 template <typename E> M2_DEV E peek(const E* p) { return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
 template <typename E> M2_DEV void publish(E* p, E v) { __hip_atomic_store(p, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
 
+// How many segments of the chain went out before; `next` is shared
+M2_DEV int take(const RecArgs& a, int chain, int& next) {
+    if (threadIdx.x == 0)
+        next = __hip_atomic_fetch_add(a.tickets + chain * TICKET, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) + 1;
+    lds_barrier();
+    return __builtin_amdgcn_readfirstlane(next);
+}
+
 // everything unknown, every counter at -1
 __global__ void __launch_bounds__(256) k_rec_clear(u32x4* p, int64_t n) {
     for (int64_t k = (int64_t)blockIdx.x * 256 + threadIdx.x; k < n; k += (int64_t)gridDim.x * 256)
@@ -403,13 +412,7 @@ __global__ void __launch_bounds__(W * 64, 4) k_rec_forward(RecArgs a) {
     __shared__ typename E::Shared look;
     __shared__ int next;
     const int chain = blockIdx.x % a.chains;
-    int segment = 0;
-    if (a.segments > 1) {
-        if (threadIdx.x == 0)
-            next = __hip_atomic_fetch_add(a.tickets + chain * TICKET, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) + 1;
-        lds_barrier();
-        segment = __builtin_amdgcn_readfirstlane(next);
-    }
+    const int segment = a.segments > 1 ? take(a, chain, next) : 0;
     const P at(a, chain, segment);
     const bool ends = segment == a.segments - 1;
     E en;
@@ -613,7 +616,10 @@ __global__ void __launch_bounds__(W * 64, 2) k_rec_backward(RecArgs a) {
     typedef Place<V, LC, TS, W> P;
     static_assert(P::TILE % SPAN == 0, "");
     __shared__ float tot[3][3][W][P::C];
-    const P at(a);
+    __shared__ int next;
+    const bool passed = a.tickets != nullptr;            // from segment to segment, else a.agg tells what enters each
+    const int chain = xcd_remap(blockIdx.x % a.chains, a.chains);
+    const P at = passed ? P(a, chain, a.segments - 1 - take(a, chain, next), a.seg) : P(a);
     const int64_t end = at.t0 + (at.end - 1 - at.t0) / P::TILE * P::TILE;
     Stream<T, V> sx(a.x, at.b * a.xb + end * a.xt, a.xt, a, at), sr(a.r, at.b * a.rb + end * a.rt, a.rt, a, at),
         si(a.i, at.b * a.ib + end * a.it, a.it, a, at), sg(a.g, at.b * a.gb + end * a.gt, a.gt, a, at);
@@ -631,6 +637,7 @@ __global__ void __launch_bounds__(W * 64, 2) k_rec_backward(RecArgs a) {
         dA[v] = 0.f;
     }
     far = __any(far);
+    if (!passed)
 #pragma unroll 4
     for (int u = a.segments - 1; u > at.segment; --u)
 #pragma unroll
@@ -770,6 +777,15 @@ __global__ void __launch_bounds__(W * 64, 2) k_rec_backward(RecArgs a) {
     };
     load(one, end);
     if (end - P::TILE >= at.t0) load(two, end - P::TILE);
+    if (passed && at.segment < a.segments - 1) {
+#pragma unroll
+        for (int v = 0; v < V; ++v) {
+            const uint32_t* p = a.states + at.agg(a, at.segment + 1) + v;
+            uint32_t m = 0;                  // (of what is stored by another lane, or chain: any)
+            while (__any(at.owns(v) && (m = peek(p)) == UNKNOWN)) __builtin_amdgcn_s_sleep(8);
+            mu[v] = __uint_as_float(m);
+        }
+    }
     for (int64_t t0 = end; t0 >= at.t0; t0 -= 3 * P::TILE) {
         tile(one, three, t0, 0);
         if (t0 - P::TILE < at.t0) break;
@@ -777,6 +793,10 @@ __global__ void __launch_bounds__(W * 64, 2) k_rec_backward(RecArgs a) {
         if (t0 - 2 * P::TILE < at.t0) break;
         tile(three, two, t0 - 2 * P::TILE, 2);
     }
+    if (passed && at.segment > 0 && at.w == 0 && at.tg == 0)
+#pragma unroll
+        for (int v = 0; v < V; ++v)
+            if (at.owns(v)) publish(a.states + at.agg(a, at.segment) + v, known(mu[v]));
     if (a.dh0 && at.segment == 0 && at.w == 0 && at.tg == 0) at.put(a.dh0 + (int64_t)at.b * a.dim + at.c, mu);
     // dA of this segment: of the lanes of a channel, then of the wavefronts in their order
     lds_barrier();
@@ -862,21 +882,47 @@ ForwardPlan forward_plan(int64_t batch, int64_t L, int64_t dim) {
     p.total = (p.states + 4 * n + 15) / 16 * 16;
     return p;
 }
-// Segments of the backward, and their steps: where the slabs alone leave CUs idle, as many as make five workgroups a CU,
+// Segments of the backward, and their steps.  Where the slabs alone leave CUs idle, as many as make five workgroups a CU,
 // of 128 steps at least; a pass more over two of the inputs then finds what enters each.  One segment
 // against many, us: 160 slabs x 4096 298 and 196; 240 309 and 306; 320 432 and 367; 480 x 2048 246 and 271.
 // (The forward's way, each segment waiting for others, takes 222 for 40 slabs x 16384, 191 so; 640 x 2048 362 and 327: a
 // segment's four inputs and its factors leave registers for two workgroups a CU, and none of them loads ahead.)
-int segments(int64_t batch, int64_t L, int64_t dim, int64_t& seg) {
+// Two workgroups a CU run at once.  Where the slabs are a few times as many, the last round of whole rows would leave CUs idle:
+// up to four segments of 512 steps at least then pass on what goes from one to the next, given out like the forward's
+// (a slab's next segment is due when all slabs' last ones went out, so hardly anybody waits).  One, two, four of them, us:
+// 520 slabs x 1024 163, 143, 135; 640 x 2048 332, 308, 294; 800 x 1600 321, 299, 295; 1280 x 1024 301, 293, 302; 2560 x 512
+// 281, 299, 335; 748 x 301 78, 85, 87.
+struct BackPlan {
+    int64_t seg;
+    int segments;
+    bool passed;
+    size_t states, dA, total;                // counters or maps first
+};
+BackPlan back_plan(int64_t batch, int64_t L, int64_t dim) {
     constexpr int64_t UNIT = 128;
     const int64_t units = L > 0 ? (L + UNIT - 1) / UNIT : 1, slabs = batch * ((dim + 2 * LC - 1) / (2 * LC));
     const int64_t ncu = m2::cu_count();
+    BackPlan p{};
     int64_t s = 1;
     if (slabs > 0 && slabs < ncu * 3 / 2) s = (5 * ncu + slabs - 1) / slabs;
+    else if (slabs > 2 * ncu && slabs <= 8 * ncu) s = units / 4 < 4 ? units / 4 : 4;
     if (s > units) s = units;
+    if (s < 1) s = 1;
     const int64_t per = (units + s - 1) / s;
-    seg = per * UNIT;
-    return (int)((units + per - 1) / per);
+    p.seg = per * UNIT;
+    p.segments = (int)((units + per - 1) / per);
+    p.passed = p.segments > 1 && slabs >= ncu * 3 / 2;
+    const size_t n = (size_t)(batch > 1 ? batch : 1) * p.segments * dim;
+    p.states = p.passed ? 4 * TICKET * (size_t)slabs : 0;
+    p.dA = p.passed ? (p.states + 4 * n + 15) / 16 * 16 : 8 * n;
+    p.total = p.dA + 4 * n;
+    return p;
+}
+// counters and states of `bytes`, unknown
+void clear(void* ws, size_t bytes, hipStream_t s) {
+    const int64_t n = (int64_t)(bytes / 16);
+    hipLaunchKernelGGL(k_rec_clear, dim3((unsigned)(n < (1 << 18) ? (n + 255) / 256 : 1024)), dim3(256), 0, s,
+                       static_cast<u32x4*>(ws), n);
 }
 
 template <typename T, int V, bool SEQ, bool NT> void launch_forward(const RecArgs& a, int steps, hipStream_t s) {
@@ -889,7 +935,7 @@ template <typename T, int V, bool SEQ, bool NT> void launch_forward(const RecArg
 template <typename T, int V, bool SEQ, bool NT> void launch_backward(const RecArgs& a, hipStream_t s) {
     const dim3 grid((unsigned)((int64_t)a.chains * a.segments));
     auto go = [&](auto k) { hipLaunchKernelGGL(k, grid, dim3(256), 0, s, a); };
-    if (a.segments > 1) go(k_rec_back_agg<T, V, LC, 4, 4, SEQ>);
+    if (a.segments > 1 && !a.tickets) go(k_rec_back_agg<T, V, LC, 4, 4, SEQ>);
     go(k_rec_backward<T, V, LC, 4, 4, SEQ, NT>);
 }
 // steps: of a forward segment, or 0: backward
@@ -977,9 +1023,7 @@ int launch_gated_recurrence(const m2_gated_recurrence_args& a, hipStream_t s) {
         k.tickets = reinterpret_cast<int*>(ws);
         k.maps = reinterpret_cast<uint64_t*>(ws + p.maps);
         k.states = reinterpret_cast<uint32_t*>(ws + p.states);
-        const int64_t n = (int64_t)(p.total / 16);
-        hipLaunchKernelGGL(k_rec_clear, dim3((unsigned)(n < (1 << 18) ? (n + 255) / 256 : 1024)), dim3(256), 0, s,
-                           reinterpret_cast<u32x4*>(ws), n);
+        clear(ws, p.total, s);
     }
     if (a.dtype == M2_F32) run<float>(k, a.batch, steps, s);
     else run<bf16>(k, a.batch, steps, s);
@@ -988,9 +1032,7 @@ int launch_gated_recurrence(const m2_gated_recurrence_args& a, hipStream_t s) {
 
 size_t gated_recurrence_grad_workspace(const m2_gated_recurrence_grad_args& a) {
     if (check_sizes("gated_linear_recurrence_grad", a.batch, a.seqlen, a.dim, a.dtype)) return 0;
-    int64_t seg;
-    const size_t n = segments(a.batch, a.seqlen, a.dim, seg) * (size_t)(a.batch > 1 ? a.batch : 1);
-    return 12 * n * a.dim;
+    return back_plan(a.batch, a.seqlen, a.dim).total;
 }
 
 int launch_gated_recurrence_grad(const m2_gated_recurrence_grad_args& a, hipStream_t s) {
@@ -1015,10 +1057,19 @@ int launch_gated_recurrence_grad(const m2_gated_recurrence_grad_args& a, hipStre
     k.g = a.grad_out; k.gb = a.grad_out_stride_batch; k.gt = a.grad_out_stride_time;
     k.glast = a.grad_final_states;
     k.dx = a.grad_x; k.dr = a.grad_r; k.di = a.grad_i; k.dh0 = a.grad_initial_states;
-    k.segments = segments(a.batch, a.seqlen, a.dim, k.seg);
+    const BackPlan p = back_plan(a.batch, a.seqlen, a.dim);
+    k.segments = p.segments;
+    k.seg = p.seg;
     const int64_t parts = a.batch * k.segments;
-    k.agg = static_cast<float2*>(a.workspace);
-    k.dA = parts == 1 ? a.grad_A : static_cast<float*>(a.workspace) + 2 * parts * a.dim;
+    char* ws = static_cast<char*>(a.workspace);
+    if (p.passed) {
+        k.tickets = reinterpret_cast<int*>(ws);
+        k.states = reinterpret_cast<uint32_t*>(ws + p.states);
+        clear(ws, p.dA, s);
+    } else {
+        k.agg = reinterpret_cast<float2*>(ws);
+    }
+    k.dA = parts == 1 ? a.grad_A : reinterpret_cast<float*>(ws + p.dA);
     if (a.dtype == M2_F32) run<float>(k, a.batch, 0, s);
     else run<bf16>(k, a.batch, 0, s);
     if (parts > 1)

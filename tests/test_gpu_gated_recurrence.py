@@ -355,6 +355,30 @@ def test_recurrence_segments(batch, seqlen, dim, packed):
         assert all(torch.equal(p, q) for p, q in zip(got, want)) and all(torch.equal(p, q) for p, q in zip(other, want))
 
 
+@pytest.mark.parametrize("packed", [0, 300])
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+def test_recurrence_more_rows_than_run_at_once(dtype, packed):
+    """Rows that are cut so that no CU idles at the end: what goes back from segment to segment, and the same bits every time."""
+    announce("more rows", dtype, packed)
+    sets = inputs(9, 1100, 3713, dtype, packed=packed, carried=True)
+    check(*sets)
+    x, r, i, A, h0, seq, go, gl = sets
+
+    def run():
+        leaves = [t.detach().requires_grad_() for t in (x, r, i, A, h0)]
+        return torch.autograd.grad(ops.gated_linear_recurrence(*leaves, seq, True), leaves, (go, gl))
+
+    want = run()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    for _ in range(3):
+        with torch.cuda.stream(side):
+            other = run()
+        got = run()
+        torch.cuda.synchronize()
+        assert all(torch.equal(p, q) for p, q in zip(got, want)) and all(torch.equal(p, q) for p, q in zip(other, want))
+
+
 def test_recurrence_any_not_a_number():
     """NaNs of all bits (and of all ones, which stand for what is not known yet) go on like any value."""
     announce("any NaN")

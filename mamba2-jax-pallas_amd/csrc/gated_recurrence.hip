@@ -638,7 +638,7 @@ __global__ void __launch_bounds__(W * 64, 2) k_rec_backward(RecArgs a) {
     }
     far = __any(far);
     if (!passed)
-#pragma unroll 4
+#pragma unroll 16
     for (int u = a.segments - 1; u > at.segment; --u)
 #pragma unroll
         for (int v = 0; v < V; ++v) {

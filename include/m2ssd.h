@@ -575,7 +575,7 @@ int m2_clip_grad_norm(const m2_clip_grad_norm_args* a, void* stream);
  * final_states is the state behind the last position.  x, r and i are addressed through their strides of
  * batch and time (elements; channels are contiguous; of time 0, or dim to 2^20), e.g. as slices of one
  * projection's output.  dim <= 2^20, seqlen < 2^32,
- * batch ceil(dim / 64) < 2^22.
+ * batch ceil(dim / 64) < 2^22.  Workspaces are 16-byte aligned.
  * span_states (or NULL) takes the states that enter every M2_RECURRENCE_SPAN positions, which
  * the gradient reads.
  * No counterpart in the reference, whose only recurrence is the SSD's (ops/ssd_naive.py:220-322).
@@ -632,7 +632,7 @@ int m2_gated_recurrence_grad(const m2_gated_recurrence_grad_args* a, void* strea
 
 /* ---------------------------------------------------------------------------
  * gated_linear_recurrence_update: one position of every batch row, new_state = h, out = h
- * rounded once; new_state may be state.
+ * rounded once; new_state may be state.  batch <= 65535.
  * ------------------------------------------------------------------------- */
 typedef struct {
     const void*  x;                /* [b, d] at x_stride_batch, dtype           */
@@ -653,7 +653,7 @@ int m2_gated_recurrence_update(const m2_gated_recurrence_update_args* a, void* s
  *   g[n, f] = x[n] . weight[f],  v[n, f] = x[n] . weight[hidden + f],  out = act(g) v,
  * float32 sums, rounded once; act(g) = g sigmoid(g) (M2_SILU) or gelu's tanh form (M2_GELU).  float32
  * operands are multiplied as three bf16 parts each (six products, about 2^-24 of each; an infinity
- * among them gives NaN).  With saved (m2_gated_linear_saved_size bytes, 256-byte aligned) what the gradient
+ * among them gives NaN).  With saved (m2_gated_linear_saved_size bytes, 16-byte aligned, as the workspaces) what the gradient
  * reads is left there: act(g) and v act'(g) (of bf16 operands their upper 24 bits), and the operands
  * where the kernels do not read them in place (float32, as three bf16 parts; a dim or, of weight, a
  * hidden that 64 does not divide).  n < 2^30, hidden <= 2^21, hidden dim < 2^30.

@@ -862,6 +862,7 @@ int launch_gated_linear(const m2_gated_linear_args& a, hipStream_t s) {
     const char* who = "gated_linear";
     if (int rc = check_sizes(who, a.n, a.dim, a.hidden, a.ldx, a.ldw, a.dtype, a.activation)) return rc;
     M2_REQUIRE(a.n == 0 || (a.x && a.weight && a.out), M2_ERR_INVALID, "%s: x, weight and out are required", who);
+    M2_REQUIRE(al16(a.saved) && al16(a.workspace), M2_ERR_WORKSPACE, "%s: saved and workspace of 16-byte alignment needed", who);
     M2_REQUIRE(!a.saved || a.saved_bytes >= gated_linear_saved(a), M2_ERR_WORKSPACE,
                "%s: saved of %zu bytes needed, %zu given", who, gated_linear_saved(a), a.saved_bytes);
     if (a.n == 0) return M2_OK;
@@ -895,6 +896,7 @@ int launch_gated_linear_grad(const m2_gated_linear_grad_args& a, hipStream_t s) 
     M2_REQUIRE(a.ldg >= a.hidden, M2_ERR_INVALID, "%s: row strides", who);
     M2_REQUIRE(a.x && a.weight && a.saved && a.grad_out && (a.grad_x || a.grad_weight), M2_ERR_INVALID,
                "%s: x, weight, saved, grad_out and an output are required", who);
+    M2_REQUIRE(al16(a.saved) && al16(a.workspace), M2_ERR_WORKSPACE, "%s: saved and workspace of 16-byte alignment needed", who);
     const BwdPlan p = plan(a);
     M2_REQUIRE(p.kept.known, M2_ERR_WORKSPACE, "%s: saved of %zu bytes is no forward's of these sizes", who, a.saved_bytes);
     M2_REQUIRE(a.workspace && a.workspace_bytes >= p.total, M2_ERR_WORKSPACE,

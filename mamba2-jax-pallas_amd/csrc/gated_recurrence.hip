@@ -181,8 +181,7 @@ template <int V, int LC, int TS, int W> struct Place {
     // A lane that would reach past the last channel has the last V, and stores of them those that no other lane
     // has: all (whole), the second alone (half, of an odd number of channels), none
     bool whole, half;
-    // segment `seg` of a chain: one tile
-    M2_DEV Place(const RecArgs& a, int chain, int seg) { init(a, chain, seg, TILE); }
+    // segment `seg` of a chain, of so many steps
     M2_DEV Place(const RecArgs& a, int chain, int seg, int64_t steps) { init(a, chain, seg, steps); }
     // Of the grid of segments that are independent: neighbouring slabs to one XCD where there is one segment (8 x 2048 x 5120
     // 332 us so, 355 in turn), to all in turn where there are more (3 x 4096 x 5120 310 and 292)
@@ -305,7 +304,6 @@ template <int D, int LC, int O, bool SEQ> M2_DEV void join(Map<SEQ>& m, int lane
 }
 template <int D, int LC, bool SEQ> M2_DEV Map<SEQ> scan(Map<SEQ>& m, int lane) {
     join<D, LC, LC, SEQ>(m, lane);
-    if constexpr (LC == 64) return Map<SEQ>{1.f, 0.f};
     const Map<SEQ> e = shifted<D, LC, SEQ>(m, lane);
     const bool has = D > 0 ? lane >= LC : lane + LC < 64;
     return Map<SEQ>{has ? e.P : 1.f, has ? e.H : 0.f};
@@ -413,7 +411,7 @@ __global__ void __launch_bounds__(W * 64, 4) k_rec_forward(RecArgs a) {
     __shared__ int next;
     const int chain = blockIdx.x % a.chains;
     const int segment = a.segments > 1 ? take(a, chain, next) : 0;
-    const P at(a, chain, segment);
+    const P at(a, chain, segment, P::TILE);
     const bool ends = segment == a.segments - 1;
     E en;
     en.begin(a, at);
@@ -965,8 +963,9 @@ template <typename T> void run(RecArgs a, int64_t batch, int steps, hipStream_t 
     }
 }
 
-// (a tile's offsets have 32 bits: at most 512 steps of 4 bytes)
+// (a tile's offsets have 32 bits: at most 256 steps of 4 bytes)
 constexpr int64_t MAX_STRIDE = 1 << 20;
+bool al16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 // rows of a step that are one, or behind each other
 bool stride_ok(int64_t st, int64_t dim) { return st == 0 || (st >= dim && st <= MAX_STRIDE); }
 
@@ -1017,6 +1016,7 @@ int launch_gated_recurrence(const m2_gated_recurrence_args& a, hipStream_t s) {
     M2_REQUIRE(a.batch * ((a.dim + 63) / 64) * p.segments * (4 * steps) < (1ll << 32), M2_ERR_UNSUPPORTED, "%s: too many steps", who);
     M2_REQUIRE(p.total == 0 || (a.workspace && a.workspace_bytes >= p.total), M2_ERR_WORKSPACE,
                "%s: workspace of %zu bytes needed, %zu given", who, p.total, a.workspace_bytes);
+    M2_REQUIRE(p.total == 0 || al16(a.workspace), M2_ERR_WORKSPACE, "%s: workspace of 16-byte alignment needed", who);
     k.segments = (int)p.segments;
     if (p.segments > 1) {
         char* ws = static_cast<char*>(a.workspace);
@@ -1044,9 +1044,10 @@ int launch_gated_recurrence_grad(const m2_gated_recurrence_grad_args& a, hipStre
     M2_REQUIRE(stride_ok(a.x_stride_time, a.dim) && stride_ok(a.r_stride_time, a.dim) && stride_ok(a.i_stride_time, a.dim) &&
                    stride_ok(a.grad_out_stride_time, a.dim),
                M2_ERR_INVALID, "%s: strides of time (0, or dim to %lld)", who, (long long)MAX_STRIDE);
-    const size_t need = gated_recurrence_grad_workspace(a);
-    M2_REQUIRE(a.workspace && a.workspace_bytes >= need, M2_ERR_WORKSPACE,
-               "%s: workspace of %zu bytes needed, %zu given", who, need, a.workspace_bytes);
+    const BackPlan p = back_plan(a.batch, a.seqlen, a.dim);
+    M2_REQUIRE(a.workspace && a.workspace_bytes >= p.total, M2_ERR_WORKSPACE,
+               "%s: workspace of %zu bytes needed, %zu given", who, p.total, a.workspace_bytes);
+    M2_REQUIRE(al16(a.workspace), M2_ERR_WORKSPACE, "%s: workspace of 16-byte alignment needed", who);
     RecArgs k{};
     k.x = a.x; k.r = a.r; k.i = a.i; k.A = a.A; k.seq = a.seq_idx;
     k.xb = a.x_stride_batch; k.xt = a.x_stride_time;
@@ -1057,7 +1058,6 @@ int launch_gated_recurrence_grad(const m2_gated_recurrence_grad_args& a, hipStre
     k.g = a.grad_out; k.gb = a.grad_out_stride_batch; k.gt = a.grad_out_stride_time;
     k.glast = a.grad_final_states;
     k.dx = a.grad_x; k.dr = a.grad_r; k.di = a.grad_i; k.dh0 = a.grad_initial_states;
-    const BackPlan p = back_plan(a.batch, a.seqlen, a.dim);
     k.segments = p.segments;
     k.seg = p.seg;
     const int64_t parts = a.batch * k.segments;

@@ -191,7 +191,7 @@ def gated_linear_recurrence_update(state, x, r, i, A, *, inplace=False):
     """One step of ``gated_linear_recurrence`` -> (new_state (batch, dim) float32, h (batch, dim),
     x's dtype).
 
-    state (batch, dim); x, r, i (batch, dim), all bfloat16 or all float32, rows with contiguous
+    state (batch, dim), batch at most 65535; x, r, i (batch, dim), all bfloat16 or all float32, rows with contiguous
     channels read in place; A (dim,).  The caller's state is left untouched, unless inplace=True (keyword
     only) and it is float32 and contiguous: it is then updated and returned.
     Takes no gradients."""

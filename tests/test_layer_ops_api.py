@@ -57,6 +57,7 @@ def test_gated_recurrence_refusals():
     refused(name, mk(batch=1 << 12, dim=1 << 16), -2, "too many rows")
     refused(name, mk(batch=1 << 21, seqlen=1 << 12, dim=1), -2, "too many steps")
     refused(name, mk(seqlen=65536), -4, "workspace")
+    refused(name, mk(seqlen=65536, workspace=4104, workspace_bytes=1 << 30), -4, "alignment")
     assert L.load_library().m2_gated_recurrence_workspace_size(ctypes.byref(mk(seqlen=65536))) > 0
     for p in ("x", "r", "i", "A", "out"):
         refused(name, mk(**{p: None}), -1, "required")
@@ -79,6 +80,7 @@ def test_gated_recurrence_refusals():
         refused(name, mg(**{p: None}), -1, "required")
     refused(name, mg(grad_out_stride_time=7), -1, "strides of time")
     refused(name, mg(workspace=4096, workspace_bytes=need - 1), -4, "workspace")
+    refused(name, mg(workspace=4104, workspace_bytes=need), -4, "alignment")
     refused(name, mg(workspace_bytes=need), -4, "workspace")
 
 
@@ -120,6 +122,8 @@ def test_gated_linear_refusals():
     refused(name, mk(workspace=4096, workspace_bytes=need - 1), -4, "workspace")
     refused(name, mk(workspace_bytes=need), -4, "workspace")
     refused(name, mk(workspace=4096, workspace_bytes=need, saved=4096, saved_bytes=saved - 1), -4, "saved")
+    refused(name, mk(workspace=4096, workspace_bytes=need, saved=4104, saved_bytes=saved), -4, "alignment")
+    refused(name, mk(workspace=4104, workspace_bytes=need), -4, "alignment")
     assert lib.m2_gated_linear(ctypes.byref(mk(n=0, x=None)), None) == 0
     okg = {k: v for k, v in ok.items() if k != "out"} | dict(saved=4096, saved_bytes=saved, grad_out=4096, grad_x=4096,
                                                             grad_weight=4096, ldg=30)

@@ -4,7 +4,7 @@ Tolerances are per element and derived from the arithmetic; F = 2^-24, u(T) half
 
 * A gate q = sigmoid(r) is off by (6 + 2 |r|) F of itself: the argument's product rounds by |r| F, the
   exponential and the reciprocal by two steps each, the sum by half a one.
-* L = A q by F more; alpha = 1 - exp(L) by 12 F more (the series' seven roundings; below -0.35 the
+* L = A q by F more; alpha = 1 - exp(L) by 12 F more (the polynomial's seven roundings; below -0.35 the
   exponential's 2 F over alpha > 0.29, with the argument's |L| F a where a is its weight); beta by half of
   alpha's and 5 F, and so is 1 / beta; what is added, b = beta s x, by the sum of its factors' and 2 F.
 * A step passes its state's error on by a and adds alpha's error times the state, b's and two roundings of

@@ -23,9 +23,11 @@
 // About 100 vector instructions and 14 bytes an element: 8 x 2048 x 5120 294 us (1216 MB, 4.1 TB/s), 8 x 2048 x 4096, whose
 // 512 slabs run at once, 218-235 (973 MB, 4.1 to 4.5 TB/s).
 //
-// Everything is float32 but what is loaded and stored.  alpha = 1 - a is kept in place of a: near
+// Everything is float32 but what is loaded and stored.  Where log a >= NEAR alpha = 1 - a is kept in place of a: near
 // 1, where memories are long, a itself has too few bits (beta^2 = alpha (2 - alpha) loses none,
-// and h - alpha h + b rounds by the step's own size only).
+// and h - alpha h + b rounds by the step's own size only).  Below NEAR a itself is, for there 1 - a has lost its bits, and
+// h + b would round what is added at the size of a state that is about to go.  Wavefronts with a channel whose A is below
+// NEAR (FAR) take either form step by step; the others need the first alone.
 //
 // Where seq_idx changes the state is cleared: P = -1 marks a run that holds such a step, so that what
 // came before (a NaN, say) is selected away and not multiplied by zero.  Negative seq_idx is
@@ -107,29 +109,58 @@ M2_DEV float decay_near(float L) {
     p = fmaf(p, L, 1.f);
     return p * -L;
 }
-M2_DEV float decay(float L, float near) { return L < NEAR ? 1.f - __builtin_amdgcn_exp2f(L * LOG2E) : near; }
-// far: some channel of the wavefront may have an L below NEAR
-template <int TS, int V> M2_DEV void decay_far(float (&al)[TS][V], const float (&L)[TS][V], bool far) {
+constexpr float LEAST = 0x1p-149f;           // (what a is at least: never 0, whose sign would tell nothing)
+// What is kept of a step's decay a = exp(L): k = alpha = 1 - a >= 0, or (of FAR, where L < NEAR) -a < 0; and y = 1 - a^2
+M2_DEV void decay(float L, float& k, float& y) {
+    k = decay_near(L);
+    y = k * (2.f - k);
+}
+M2_DEV void decay_far(float L, float& k, float& y) {
+    const float a = __builtin_amdgcn_fmed3f(__builtin_amdgcn_exp2f(L * LOG2E), LEAST, 1.f);
+    k = L < NEAR ? -a : k;
+    y = L < NEAR ? fmaf(-a, a, 1.f) : y;
+}
+// of the steps of a thread; far: of some channel of the wavefront an L may be below NEAR
+template <int TS, int V> M2_DEV void decays(const float (&L)[TS][V], bool far, float (&k)[TS][V], float (&y)[TS][V]) {
+#pragma unroll
+    for (int j = 0; j < TS; ++j)
+#pragma unroll
+        for (int v = 0; v < V; ++v) decay(L[j][v], k[j][v], y[j][v]);
     if (!far) return;
     asm volatile("");        // (a branch, not selects: the exponentials cost the others an eighth of their time)
 #pragma unroll
     for (int j = 0; j < TS; ++j)
 #pragma unroll
-        for (int v = 0; v < V; ++v) al[j][v] = decay(L[j][v], al[j][v]);
+        for (int v = 0; v < V; ++v) decay_far(L[j][v], k[j][v], y[j][v]);
 }
+// f of either kind of steps: what the wavefronts without the second compute stays without selects (8 x 2048 x 5120: forward 161
+// and, with selects, 170 us, backward 304 and 326; both ways of the whole kernels instead of these parts of them hold 123
+// registers for 78)
+template <class F> M2_DEV void by_decay(bool far, F&& f) {
+    if (far) {
+        asm volatile("; far");
+        f(std::true_type());
+    } else {
+        asm volatile("; near");
+        f(std::false_type());
+    }
+}
+// A channel's A: one above 0 is no decay, and makes NaNs
+M2_DEV float decay_rate(float A) { return A > 0.f ? __builtin_nanf("") : A; }
 // alpha p, of an infinite p the largest number (p - alpha p is then p, not inf - inf)
 M2_DEV float bounded(float p) {
     constexpr float MAX = 3.402823466e38f;
     return __builtin_amdgcn_fmed3f(p, -MAX, MAX);
 }
-// a p + b
-M2_DEV float step(float alpha, float p, float b) { return fmaf(-alpha, bounded(p), p + b); }
-M2_DEV float step(float alpha, float p) { return fmaf(-alpha, bounded(p), p); }
-// 1 / sqrt(1 - a^2), 0 where a is 1 (below 1e-37 the hardware's root has no argument left)
-M2_DEV float inv_beta(float alpha, float& y) {
-    y = alpha * (2.f - alpha);
-    return fabsf(y) <= 1e-37f ? 0.f : __builtin_amdgcn_rsqf(y);
+// Of what is kept, k: a; a p; a p + b; a P of a map, whose P is finite
+template <bool FAR> M2_DEV float factor(float k) { return FAR && k < 0.f ? -k : 1.f - k; }
+template <bool FAR> M2_DEV float step(float k, float p) { return FAR && k < 0.f ? -k * p : fmaf(-k, bounded(p), p); }
+template <bool FAR> M2_DEV float step(float k, float p, float b) {
+    return FAR && k < 0.f ? fmaf(-k, p, b) : fmaf(-k, bounded(p), p + b);
 }
+template <bool FAR> M2_DEV float shrunk(float k, float P) { return FAR && k < 0.f ? -k * P : fmaf(-k, P, P); }
+// 1 / sqrt(y), y = 1 - a^2; 0 where a is 1 (below 1e-37 the hardware's root has no argument left)
+M2_DEV float inv_beta(float y) { return fabsf(y) <= 1e-37f ? 0.f : __builtin_amdgcn_rsqf(y); }
 
 // an affine map v -> P v + H; P = -1: the state is cleared in it, v -> H
 template <bool SEQ> struct Map {
@@ -213,6 +244,17 @@ template <int V, int LC, int TS, int W> struct Place {
     }
     M2_DEV int64_t agg(const RecArgs& a, int s) const { return ((int64_t)b * a.segments + s) * a.dim + c; }
 };
+
+// A of a thread's channels -> whether some channel of the wavefront has one below NEAR (or a NaN)
+template <int V, class P> M2_DEV bool decay_rates(const RecArgs& a, const P& at, float (&A)[V]) {
+    bool far = false;
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+        A[v] = decay_rate(a.A[at.c + v]);
+        far |= !(A[v] >= NEAR);
+    }
+    return __any(far);
+}
 
 // The tile of one input or output that the walk is at
 template <typename T, int V> struct Stream {
@@ -425,13 +467,7 @@ __global__ void __launch_bounds__(W * 64, 4) k_rec_forward(RecArgs a) {
     si.load(i, last);
     s.load(SEQ ? a.seq + at.b * a.L + at.t0 : nullptr, segment == 0, at, last);
     float A[V];
-    bool far = false;
-#pragma unroll
-    for (int v = 0; v < V; ++v) {
-        A[v] = a.A[at.c + v];
-        far |= !(A[v] >= NEAR);
-    }
-    far = __any(far);
+    const bool far = decay_rates<V>(a, at, A);
     if ((SEQ || last != P::TILE - 1) && !s.set(segment == 0, at, last)) {
 #pragma unroll
         for (int j = 0; j < TS; ++j)
@@ -442,24 +478,29 @@ __global__ void __launch_bounds__(W * 64, 4) k_rec_forward(RecArgs a) {
             }
     }
     // the gates, and the map of this thread's steps
-    float al[TS][V], add[TS][V], L[TS][V];
+    float k[TS][V], add[TS][V], L[TS][V];
 #pragma unroll
     for (int j = 0; j < TS; ++j)
 #pragma unroll
-        for (int v = 0; v < V; ++v) {
-            L[j][v] = A[v] * sigmoid_of(exp_neg(r[j].get(v)));
-            al[j][v] = decay_near(L[j][v]);
-        }
-    decay_far<TS, V>(al, L, far);
+        for (int v = 0; v < V; ++v) L[j][v] = A[v] * sigmoid_of(exp_neg(r[j].get(v)));
+    decays<TS, V>(L, far, k, add);
     Map<SEQ> m[V], ex[V];
 #pragma unroll
-    for (int v = 0; v < V; ++v) {
+    for (int j = 0; j < TS; ++j)
 #pragma unroll
-        for (int j = 0; j < TS; ++j) {
-            add[j][v] = sigmoid_of(exp_neg(i[j].get(v))) * x[j].get(v) * __builtin_amdgcn_sqrtf(al[j][v] * (2.f - al[j][v]));
-            m[v].P = j == 0 ? 1.f - al[j][v] : fmaf(-al[j][v], m[v].P, m[v].P);
-            m[v].H = j == 0 ? add[j][v] : step(al[j][v], s.clears(j) ? 0.f : m[v].H, add[j][v]);
-        }
+        for (int v = 0; v < V; ++v) add[j][v] = sigmoid_of(exp_neg(i[j].get(v))) * x[j].get(v) * __builtin_amdgcn_sqrtf(add[j][v]);
+    by_decay(far, [&](auto is_far) {
+        constexpr bool FAR = decltype(is_far)::value;
+#pragma unroll
+        for (int v = 0; v < V; ++v)
+#pragma unroll
+            for (int j = 0; j < TS; ++j) {
+                m[v].P = j == 0 ? factor<FAR>(k[j][v]) : shrunk<FAR>(k[j][v], m[v].P);
+                m[v].H = j == 0 ? add[j][v] : step<FAR>(k[j][v], s.clears(j) ? 0.f : m[v].H, add[j][v]);
+            }
+    });
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
         if (SEQ && s.clear) m[v].P = -1.f;
         ex[v] = scan<1, LC, SEQ>(m[v], at.lane);
         if (at.tg == P::G - 1) tot[at.w][at.col + v] = make_float2(m[v].P, m[v].H);
@@ -501,16 +542,19 @@ __global__ void __launch_bounds__(W * 64, 4) k_rec_forward(RecArgs a) {
     if (a.ck && at.step % SPAN == 0 && at.step <= last)
         at.put(a.ck + (at.b * a.spans + (at.t0 + at.step) / SPAN) * a.dim + at.c, h);
     const Rsrc to = so.tile(last);
+    by_decay(far, [&](auto is_far) {
+        constexpr bool FAR = decltype(is_far)::value;
 #pragma unroll
-    for (int j = 0; j < TS; ++j) {
-        float o[V];
+        for (int j = 0; j < TS; ++j) {
+            float o[V];
 #pragma unroll
-        for (int v = 0; v < V; ++v) {
-            h[v] = step(al[j][v], s.clears(j) ? 0.f : h[v], add[j][v]);
-            o[v] = SEQ && !s.is_live(j) ? 0.f : h[v];
+            for (int v = 0; v < V; ++v) {
+                h[v] = step<FAR>(k[j][v], s.clears(j) ? 0.f : h[v], add[j][v]);
+                o[v] = SEQ && !s.is_live(j) ? 0.f : h[v];
+            }
+            so.store(to, j, o);
         }
-        so.store(to, j, o);
-    }
+    });
 }
 
 // ---------------------------------------------------------------------------
@@ -528,14 +572,9 @@ __global__ void __launch_bounds__(W * 64, 4) k_rec_back_agg(RecArgs a) {
     const int32_t* seq = SEQ ? a.seq + at.b * a.L : nullptr;
     float A[V];
     Map<SEQ> mu[V];
-    bool far = false;
 #pragma unroll
-    for (int v = 0; v < V; ++v) {
-        A[v] = a.A[at.c + v];
-        far |= !(A[v] >= NEAR);
-        mu[v] = Map<SEQ>{1.f, 0.f};
-    }
-    far = __any(far);
+    for (int v = 0; v < V; ++v) mu[v] = Map<SEQ>{1.f, 0.f};
+    const bool far = decay_rates<V>(a, at, A);
     auto last_of = [&](int64_t t0) { return (int)min(at.end - 1 - t0, (int64_t)P::TILE - 1); };
     struct Tile {
         Raw<T, V> r[TS], g[TS];
@@ -560,28 +599,29 @@ __global__ void __launch_bounds__(W * 64, 4) k_rec_back_agg(RecArgs a) {
                     c.g[j].fill(0.f);
                 }
         }
-        float al[TS][V], L[TS][V];
+        float kept[TS][V], y[TS][V], L[TS][V];
 #pragma unroll
         for (int j = 0; j < TS; ++j)
 #pragma unroll
-            for (int v = 0; v < V; ++v) {
-                L[j][v] = A[v] * sigmoid_of(exp_neg(c.r[j].get(v)));
-                al[j][v] = decay_near(L[j][v]);
-            }
-        decay_far<TS, V>(al, L, far);
+            for (int v = 0; v < V; ++v) L[j][v] = A[v] * sigmoid_of(exp_neg(c.r[j].get(v)));
+        decays<TS, V>(L, far, kept, y);
+        Map<SEQ> k[V];
+        by_decay(far, [&](auto is_far) {
+            constexpr bool FAR = decltype(is_far)::value;
+#pragma unroll
+            for (int v = 0; v < V; ++v)
+#pragma unroll
+                for (int j = TS - 1; j >= 0; --j) {
+                    k[v].P = j == TS - 1 ? factor<FAR>(kept[j][v]) : shrunk<FAR>(kept[j][v], k[v].P);
+                    k[v].H = step<FAR>(kept[j][v], j == TS - 1 ? c.g[j].get(v) : c.g[j].get(v) + k[v].H);
+                    if (c.s.clears(j)) k[v].H = 0.f;
+                }
+        });
 #pragma unroll
         for (int v = 0; v < V; ++v) {
-            Map<SEQ> k{1.f - al[TS - 1][v], step(al[TS - 1][v], c.g[TS - 1].get(v))};
-            if (c.s.clears(TS - 1)) k.H = 0.f;
-#pragma unroll
-            for (int j = TS - 2; j >= 0; --j) {
-                k.P = fmaf(-al[j][v], k.P, k.P);
-                k.H = step(al[j][v], c.g[j].get(v) + k.H);
-                if (c.s.clears(j)) k.H = 0.f;
-            }
-            if (SEQ && c.s.clear) k.P = -1.f;
-            join<-1, LC, LC, SEQ>(k, at.lane);
-            if (at.tg == 0) tot[buf][at.w][at.col + v] = make_float2(k.P, k.H);
+            if (SEQ && c.s.clear) k[v].P = -1.f;
+            join<-1, LC, LC, SEQ>(k[v], at.lane);
+            if (at.tg == 0) tot[buf][at.w][at.col + v] = make_float2(k[v].P, k[v].H);
         }
         lds_barrier();
 #pragma unroll
@@ -625,15 +665,12 @@ __global__ void __launch_bounds__(W * 64, 2) k_rec_backward(RecArgs a) {
     const int32_t* seq = SEQ ? a.seq + at.b * a.L : nullptr;
     const float* ck = a.ck + at.b * a.spans * a.dim + at.c;
     float A[V], mu[V], dA[V];
-    bool far = false;
+    const bool far = decay_rates<V>(a, at, A);
 #pragma unroll
     for (int v = 0; v < V; ++v) {
-        A[v] = a.A[at.c + v];
-        far |= !(A[v] >= NEAR);
         mu[v] = a.glast ? a.glast[(int64_t)at.b * a.dim + at.c + v] : 0.f;
         dA[v] = 0.f;
     }
-    far = __any(far);
     if (!passed)
 #pragma unroll 16
     for (int u = a.segments - 1; u > at.segment; --u)
@@ -675,7 +712,7 @@ __global__ void __launch_bounds__(W * 64, 2) k_rec_backward(RecArgs a) {
                     c.g[j].fill(0.f);
                 }
         }
-        float al[TS][V], q[TS][V], s[TS][V], cq[TS][V], cosg[TS][V], ib[TS][V], L[TS][V];
+        float kept[TS][V], q[TS][V], s[TS][V], cq[TS][V], cosg[TS][V], ib[TS][V], beta[TS][V], L[TS][V];
 #pragma unroll
         for (int j = 0; j < TS; ++j)
 #pragma unroll
@@ -686,36 +723,45 @@ __global__ void __launch_bounds__(W * 64, 2) k_rec_backward(RecArgs a) {
                 cq[j][v] = co_sigmoid(eq, q[j][v]);
                 cosg[j][v] = co_sigmoid(es, s[j][v]);
                 L[j][v] = A[v] * q[j][v];
-                al[j][v] = decay_near(L[j][v]);
             }
-        decay_far<TS, V>(al, L, far);
+        decays<TS, V>(L, far, kept, beta);
+#pragma unroll
+        for (int j = 0; j < TS; ++j)
+#pragma unroll
+            for (int v = 0; v < V; ++v) {
+                ib[j][v] = inv_beta(beta[j][v]);
+                beta[j][v] *= ib[j][v];
+            }
         // the maps of this thread's steps, forward and back (with the same P)
-        Map<SEQ> up[V], down[V];
+        Map<SEQ> up[V], down[V], f[V], b[V];
+        by_decay(far, [&](auto is_far) {
+            constexpr bool FAR = decltype(is_far)::value;
+#pragma unroll
+            for (int v = 0; v < V; ++v) {
+#pragma unroll
+                for (int j = 0; j < TS; ++j) {
+                    const float add = beta[j][v] * s[j][v] * c.x[j].get(v);
+                    f[v].P = j == 0 ? factor<FAR>(kept[j][v]) : shrunk<FAR>(kept[j][v], f[v].P);
+                    f[v].H = j == 0 ? add : step<FAR>(kept[j][v], c.s.clears(j) ? 0.f : f[v].H, add);
+                }
+#pragma unroll
+                for (int j = TS - 1; j >= 0; --j) {
+                    b[v].H = step<FAR>(kept[j][v], j == TS - 1 ? c.g[j].get(v) : c.g[j].get(v) + b[v].H);
+                    if (c.s.clears(j)) b[v].H = 0.f;
+                }
+            }
+        });
 #pragma unroll
         for (int v = 0; v < V; ++v) {
-            Map<SEQ> f, k;
-#pragma unroll
-            for (int j = 0; j < TS; ++j) {
-                float y;
-                ib[j][v] = inv_beta(al[j][v], y);
-                const float add = y * ib[j][v] * s[j][v] * c.x[j].get(v);
-                f.P = j == 0 ? 1.f - al[j][v] : fmaf(-al[j][v], f.P, f.P);
-                f.H = j == 0 ? add : step(al[j][v], c.s.clears(j) ? 0.f : f.H, add);
-            }
-            if (SEQ && c.s.clear) f.P = -1.f;
-            k.P = f.P;
-#pragma unroll
-            for (int j = TS - 1; j >= 0; --j) {
-                k.H = step(al[j][v], j == TS - 1 ? c.g[j].get(v) : c.g[j].get(v) + k.H);
-                if (c.s.clears(j)) k.H = 0.f;
-            }
-            up[v] = scan<1, LC, SEQ>(f, at.lane);
-            down[v] = scan<-1, LC, SEQ>(k, at.lane);
+            if (SEQ && c.s.clear) f[v].P = -1.f;
+            b[v].P = f[v].P;
+            up[v] = scan<1, LC, SEQ>(f[v], at.lane);
+            down[v] = scan<-1, LC, SEQ>(b[v], at.lane);
             if (at.tg == 0) {
-                tot[buf][0][at.w][at.col + v] = k.P;
-                tot[buf][2][at.w][at.col + v] = k.H;
+                tot[buf][0][at.w][at.col + v] = b[v].P;
+                tot[buf][2][at.w][at.col + v] = b[v].H;
             }
-            if (at.tg == P::G - 1) tot[buf][1][at.w][at.col + v] = f.H;
+            if (at.tg == P::G - 1) tot[buf][1][at.w][at.col + v] = f[v].H;
         }
         lds_barrier();
         float k[V];
@@ -735,39 +781,41 @@ __global__ void __launch_bounds__(W * 64, 2) k_rec_backward(RecArgs a) {
 #pragma unroll
             for (int v = 0; v < V; ++v) mu[v] = Map<SEQ>{tot[buf][0][d][at.col + v], tot[buf][2][d][at.col + v]}.of(mu[v]);
         }
-        float lam[TS][V];
-#pragma unroll
-        for (int v = 0; v < V; ++v) {
-            c.e[v] = up[v].of(c.e[v]);
-            k[v] = down[v].of(k[v]);
-#pragma unroll
-            for (int j = TS - 1; j >= 0; --j) {
-                lam[j][v] = c.g[j].get(v) + k[v];
-                k[v] = step(al[j][v], lam[j][v]);
-                if (c.s.clears(j)) k[v] = 0.f;
-            }
-        }
         const Rsrc tx = ox.tile(last), tr = orr.tile(last), ti = oi.tile(last);
-#pragma unroll
-        for (int j = 0; j < TS; ++j) {
-            float dx[V], dr[V], di[V];
+        by_decay(far, [&](auto is_far) {
+            constexpr bool FAR = decltype(is_far)::value;
+            float lam[TS][V];
 #pragma unroll
             for (int v = 0; v < V; ++v) {
-                const float xv = c.x[j].get(v), p = c.s.clears(j) ? 0.f : c.e[v];
-                const float av = 1.f - al[j][v], sxv = s[j][v] * xv;
-                const float beta = al[j][v] * (2.f - al[j][v]) * ib[j][v];
-                c.e[v] = step(al[j][v], p, beta * sxv);
-                dx[v] = lam[j][v] * beta * s[j][v];
-                di[v] = dx[v] * xv * cosg[j][v];
-                const float dLq = lam[j][v] * av * fmaf(-av * ib[j][v], sxv, p) * q[j][v];
-                dr[v] = dLq * A[v] * cq[j][v];
-                dA[v] += dLq;
-                if (SEQ && !c.s.is_live(j)) dx[v] = dr[v] = di[v] = 0.f;
+                c.e[v] = up[v].of(c.e[v]);
+                k[v] = down[v].of(k[v]);
+#pragma unroll
+                for (int j = TS - 1; j >= 0; --j) {
+                    lam[j][v] = c.g[j].get(v) + k[v];
+                    k[v] = step<FAR>(kept[j][v], lam[j][v]);
+                    if (c.s.clears(j)) k[v] = 0.f;
+                }
             }
-            ox.store(tx, j, dx);
-            orr.store(tr, j, dr);
-            oi.store(ti, j, di);
-        }
+#pragma unroll
+            for (int j = 0; j < TS; ++j) {
+                float dx[V], dr[V], di[V];
+#pragma unroll
+                for (int v = 0; v < V; ++v) {
+                    const float xv = c.x[j].get(v), p = c.s.clears(j) ? 0.f : c.e[v];
+                    const float av = factor<FAR>(kept[j][v]), sxv = s[j][v] * xv;
+                    c.e[v] = step<FAR>(kept[j][v], p, beta[j][v] * sxv);
+                    dx[v] = lam[j][v] * beta[j][v] * s[j][v];
+                    di[v] = dx[v] * xv * cosg[j][v];
+                    const float dLq = lam[j][v] * av * fmaf(-av * ib[j][v], sxv, p) * q[j][v];
+                    dr[v] = dLq * A[v] * cq[j][v];
+                    dA[v] += dLq;
+                    if (SEQ && !c.s.is_live(j)) dx[v] = dr[v] = di[v] = 0.f;
+                }
+                ox.store(tx, j, dx);
+                orr.store(tr, j, dr);
+                oi.store(ti, j, di);
+            }
+        });
         ox.move(-P::TILE);
         orr.move(-P::TILE);
         oi.move(-P::TILE);
@@ -847,8 +895,11 @@ template <typename T> __global__ void __launch_bounds__(64) k_rec_step(StepArgs 
     const float q = sigmoid_of(exp_neg(to_f32(static_cast<const T*>(a.r)[b * a.rb + c])));
     const float s = sigmoid_of(exp_neg(to_f32(static_cast<const T*>(a.i)[b * a.ib + c])));
     const float xv = to_f32(static_cast<const T*>(a.x)[b * a.xb + c]), e = a.state[b * a.dim + c];
-    const float L = a.A[c] * q, al = decay(L, decay_near(L));
-    const float h = step(al, e, __builtin_amdgcn_sqrtf(al * (2.f - al)) * s * xv);
+    const float L = decay_rate(a.A[c]) * q;
+    float k, y;
+    decay(L, k, y);
+    decay_far(L, k, y);
+    const float h = step<true>(k, e, __builtin_amdgcn_sqrtf(y) * s * xv);
     a.next[b * a.dim + c] = h;
     static_cast<T*>(a.out)[b * a.dim + c] = from_f32<T>(h);
 }

@@ -1,0 +1,162 @@
+"""The gated linear recurrence where its arithmetic ends: infinite states, decays that leave nothing of a large state,
+padding around them, offsets past 32 bits; against the formulas in 64 bits.
+
+Tolerances are per element and derived from the arithmetic; F = 2^-24, u(T) half a step of T.
+
+* A gate is off by (6 + 2 |r|) F of itself, L = A q by F more.
+* a: where L is below -0.5 it is an exponential, off by |L| (L's own error and 2 F of its product) and 3 F of itself
+  (and 2^-126 flushed); above, alpha = 1 - a is off by L's error and 12 F of itself, a by as much of alpha.
+  (Between -0.5 and -0.5001 either form may be taken, of which the second allows more.)
+* beta = sqrt(1 - a^2), by half of what 1 - a^2 is off by, and 5 F.
+* A step rounds what it multiplies and adds at their own sizes: 6 F (a |h| + |b|), a being at least 0.6 where
+  h itself is added to b first.  So a state's error decays as the state does, and the error obeys the
+  recurrence itself, run here on magnitudes; the joins of maps add 24 F of the sum of the magnitudes.
+* A gradient is a product: its factors' errors, times the other factors' magnitudes.
+"""
+
+import math
+
+import pytest
+import torch
+
+from gpu_util import announce
+from mamba2_jax import ops
+from mamba2_jax.ops import gated_recurrence as R
+from test_gpu_gated_recurrence import DEV, DT, F, gen, inputs, scan, u, within
+
+pytestmark = pytest.mark.gpu
+
+INF, NAN = float("inf"), float("nan")
+
+
+class Sharp:
+    """Results in 64 bits, and what a kernel may be off by that keeps the bits of every decay."""
+
+    def __init__(self, x, r, i, A, h0, seq, g=None, glast=None):
+        x, r, i, A = (t.detach().double() for t in (x, r, i, A))
+        b, n, d = x.shape
+        live = torch.ones((b, n, 1), dtype=torch.bool, device=x.device)
+        clear = torch.zeros_like(live)
+        if seq is not None:
+            live = (seq >= 0)[..., None]
+            clear[:, 1:, 0] = (seq[:, 1:] != seq[:, :-1]) & (seq[:, 1:] >= 0)
+        zero = torch.zeros_like(x)
+        x, r, i = (torch.where(live, t, zero) for t in (x, r, i))
+        q, s = torch.sigmoid(r), torch.sigmoid(i)
+        eq, es = (6 + 2 * r.abs()) * F, (6 + 2 * i.abs()) * F
+        la = A * q
+        eL = eq + F
+        ea = torch.exp(la)
+        alpha, y = -torch.expm1(la), -torch.expm1(2 * la)
+        far = la < -0.5001
+        aerr = torch.where(far, ea * (la.abs() * (eL + 2 * F) + 3 * F) + 2.0 ** -126, alpha * (eL + 12 * F) + F * alpha)
+        beta = torch.sqrt(y)
+        eb = torch.where(far, (2 * ea * aerr + F) / y.clamp_min(0.5) / 2, 0.65 * (eL + 12 * F)) + 5 * F
+        add = torch.where(live, beta * s * x, zero)
+        a = torch.where(clear, zero, torch.where(live, ea, zero + 1))
+        aerr_h = torch.where(live & ~clear, aerr, zero)          # of what the state is multiplied by
+        eadd = (eb + es + 2 * F) * add.abs()
+        h0 = zero[:, 0] if h0 is None else h0.detach().double()
+        first = lambda t, v: torch.cat([t[:, :1] + a[:, :1] * v[:, None], t[:, 1:]], 1)
+        before = lambda t, v: torch.where(clear, zero, torch.cat([v[:, None], t[:, :-1]], 1))
+        h = scan(a, first(add, h0))
+        mag = scan(a, first(add.abs(), h0.abs()))
+        mb = before(mag, h0.abs())
+        eh = scan(a, aerr_h * mb + eadd + 6 * F * (a * mb + add.abs())) + 24 * F * mag
+        self.h, self.last = torch.where(live, h, zero), h[:, -1]
+        self.eh, self.elast = torch.where(live, eh, zero), eh[:, -1]
+        if g is None:
+            return
+        g = torch.where(live, g.detach().double(), zero)
+        gl = torch.zeros_like(g[:, 0]) if glast is None else glast.detach().double()
+        gmag = torch.cat([g[:, :-1].abs(), g[:, -1:].abs() + gl.abs()[:, None]], 1)
+        g = torch.cat([g[:, :-1], g[:, -1:] + gl[:, None]], 1)
+        later = torch.cat([a[:, 1:], zero[:, :1]], 1)
+        lam = scan(later.flip(1), g.flip(1)).flip(1)
+        lmag = scan(later.flip(1), gmag.flip(1)).flip(1)
+        passed = aerr_h * lmag + 4 * F * a * lmag
+        el = scan(later.flip(1), (torch.cat([passed[:, 1:], zero[:, :1]], 1) + 2 * F * lmag).flip(1)).flip(1) + 24 * F * lmag
+        self.dh0 = a[:, 0] * lam[:, 0]
+        self.edh0 = (a * el + passed)[:, 0]
+        lam, lmag, el = (torch.where(live, t, zero) for t in (lam, lmag, el))
+        p, ep = before(h, h0), before(eh, zero[:, 0])
+        rise = ea * ea / beta.clamp_min(1e-300) * s * x
+        self.dx = lam * beta * s
+        self.edx = el * beta * s + lmag * beta * s * (eb + es + 3 * F)
+        self.di = self.dx * x * (1 - s)
+        self.edi = (self.edx + lmag * beta * s * (2 * es + 5 * F)) * x.abs() * (1 - s)
+        dL = lam * (ea * p - rise)
+        edL = el * (ea * p - rise).abs() + lmag * (
+            ea * ep + aerr * mb + rise.abs() * (2 * aerr / ea.clamp_min(1e-300) + eb + es + 8 * F)
+            + 4 * F * (ea * mb + rise.abs()))
+        edL = torch.where(live, edL, zero)
+        slope = (la * (1 - q)).abs()
+        self.dr, self.edr = dL * la * (1 - q), (edL + dL.abs() * (3 * eq + 6 * F)) * slope
+        self.dr, self.edr = (torch.where(live, t, zero) for t in (self.dr, self.edr))
+        terms = torch.where(live, dL * q, zero)
+        self.dA = terms.sum((0, 1))
+        self.edA = (edL * q + terms.abs() * (eq + 2 * F)).sum((0, 1)) + b * n * F * terms.abs().sum((0, 1))
+
+
+def spikes(t, g, big):
+    """Every tenth entry or so `big` times the others."""
+    return torch.where(torch.rand(t.shape, generator=g, device=DEV) < 0.1, t * big, t)
+
+
+def sharp_check(x, r, i, A, h0, seq, go, gl):
+    want = Sharp(x, r, i, A, h0, seq, go, gl)
+    leaves = [t.detach().clone().requires_grad_() for t in (x, r, i, A, h0)]
+    h, last = ops.gated_linear_recurrence(*leaves, seq, True)
+    within(h, want.h, want.eh + u(h.dtype) * want.h.abs() * (h.dtype == torch.bfloat16) + 1e-37, "h")
+    within(last, want.last, want.elast + 1e-37, "last")
+    for name, got in zip(("dx", "dr", "di", "dA", "dh0"), torch.autograd.grad((h, last), leaves, (go, gl))):
+        ref = getattr(want, name)
+        tol = getattr(want, "e" + name) + (u(got.dtype) * ref.abs() if got.dtype == torch.bfloat16 else 0) + 1e-36
+        within(got, ref, tol, name)
+
+
+# from decays that no step takes below -0.5 to ones that leave nothing, and all of them in neighbouring channels
+DECAYS = [(0.3, 2.0), (16.0, 60.0), (1e-3, 200.0)]
+
+
+@pytest.mark.parametrize("low,high", DECAYS)
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("batch,seqlen,dim,packed", [(2, 300, 40, 0), (1, 1100, 70, 0), (3, 333, 65, 40), (9, 1100, 3713, 0)])
+def test_recurrence_keeps_small_inputs_behind_large_states(batch, seqlen, dim, packed, dtype, low, high):
+    """What a strong decay leaves of a state, however large, does not round what comes in, forward or backward."""
+    announce("strong decay", batch, seqlen, dim, packed, dtype, low, high)
+    if dim > 1000 and high != 60.0:
+        pytest.skip("the sizes whose backward passes segments on, once")
+    x, r, i, A, h0, seq, go, gl = inputs(batch, seqlen, dim, dtype, packed=packed, carried=True, low=low, high=high)
+    g = gen("spikes", batch, seqlen, dim, low)
+    x, go = (spikes(t * 2.0 ** -10, g, 2.0 ** 24) for t in (x, go))
+    sharp_check(x, r, i, A, h0 * 2.0 ** 20, seq, go, gl * 2.0 ** 20)
+
+
+@pytest.mark.parametrize("low,high", DECAYS)
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_update_keeps_small_inputs_behind_large_states(dtype, low, high):
+    announce("strong decay, steps", dtype, low, high)
+    x, r, i, A, h0, _, _, _ = inputs(3, 12, 70, dtype, fused=True, carried=True, low=low, high=high)
+    x, h0 = x * 2.0 ** -10, h0 * 2.0 ** 20
+    want = Sharp(x, r, i, A, h0, None)
+    state = h0
+    for t in range(12):
+        state, y = ops.gated_linear_recurrence_update(state, x[:, t], r[:, t], i[:, t], A)
+        tol = want.eh[:, t] + 1e-37
+        within(state, want.h[:, t], tol, f"state {t}")
+        within(y, want.h[:, t], tol + u(y.dtype) * want.h[:, t].abs(), f"step {t}")
+
+
+def test_recurrence_positive_decay():
+    """A above 0 is not a decay: NaN in its channel, whatever its neighbours' are."""
+    announce("positive A")
+    x, r, i, A, h0, _, _, _ = inputs(2, 40, 8, "f32", carried=True)
+    for other in (-0.1, -30.0):
+        A = torch.full_like(A, other)
+        A[3] = 0.2
+        h = ops.gated_linear_recurrence(x, r, i, A, h0)
+        state, y = ops.gated_linear_recurrence_update(h0, x[:, 0], r[:, 0], i[:, 0], A)
+        for t in (h, state[:, None], y[:, None]):
+            bad = t.isnan()
+            assert bool(bad[..., 3].all()) and not bool(bad[..., [0, 1, 2, 4, 5, 6, 7]].any())

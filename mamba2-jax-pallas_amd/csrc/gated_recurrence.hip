@@ -109,14 +109,17 @@ M2_DEV float decay_near(float L) {
     p = fmaf(p, L, 1.f);
     return p * -L;
 }
-constexpr float LEAST = 0x1p-149f;           // (what a is at least: never 0, whose sign would tell nothing)
+// What a, and a product of them, is at least: never 0, whose sign would tell nothing, and of which an infinite state would make
+// a NaN
+constexpr float LEAST = 0x1p-149f;
+M2_DEV float at_least(float p) { return __builtin_amdgcn_fmed3f(p, LEAST, 1.f); }
 // What is kept of a step's decay a = exp(L): k = alpha = 1 - a >= 0, or (of FAR, where L < NEAR) -a < 0; and y = 1 - a^2
 M2_DEV void decay(float L, float& k, float& y) {
     k = decay_near(L);
     y = k * (2.f - k);
 }
 M2_DEV void decay_far(float L, float& k, float& y) {
-    const float a = __builtin_amdgcn_fmed3f(__builtin_amdgcn_exp2f(L * LOG2E), LEAST, 1.f);
+    const float a = at_least(__builtin_amdgcn_exp2f(L * LOG2E));
     k = L < NEAR ? -a : k;
     y = L < NEAR ? fmaf(-a, a, 1.f) : y;
 }
@@ -158,11 +161,13 @@ template <bool FAR> M2_DEV float step(float k, float p) { return FAR && k < 0.f 
 template <bool FAR> M2_DEV float step(float k, float p, float b) {
     return FAR && k < 0.f ? fmaf(-k, p, b) : fmaf(-k, bounded(p), p + b);
 }
-template <bool FAR> M2_DEV float shrunk(float k, float P) { return FAR && k < 0.f ? -k * P : fmaf(-k, P, P); }
+// (the runs of steps with k > 0 are too short to end at 0)
+template <bool FAR> M2_DEV float shrunk(float k, float P) { return FAR && k < 0.f ? at_least(-k * P) : fmaf(-k, P, P); }
 // 1 / sqrt(y), y = 1 - a^2; 0 where a is 1 (below 1e-37 the hardware's root has no argument left)
 M2_DEV float inv_beta(float y) { return fabsf(y) <= 1e-37f ? 0.f : __builtin_amdgcn_rsqf(y); }
 
-// an affine map v -> P v + H; P = -1: the state is cleared in it, v -> H
+// an affine map v -> P v + H; P = -1: the state is cleared in it, v -> H.  A product of many a's would end at 0,
+// of which an infinite v makes a NaN: no P is less than LEAST (which adds 5e-7 at most, of the largest v).
 template <bool SEQ> struct Map {
     float P, H;
     M2_DEV float of(float v) const { return SEQ && P < 0.f ? H : fmaf(P, v, H); }
@@ -170,7 +175,7 @@ template <bool SEQ> struct Map {
     M2_DEV Map after(const Map& first) const {
         Map m;
         m.H = of(first.H);
-        m.P = P * first.P;
+        m.P = at_least(P * first.P);
         if constexpr (SEQ) m.P = P < 0.f || first.P < 0.f ? -1.f : m.P;
         return m;
     }

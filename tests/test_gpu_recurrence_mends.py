@@ -148,6 +148,52 @@ def test_update_keeps_small_inputs_behind_large_states(dtype, low, high):
         within(y, want.h[:, t], tol + u(y.dtype) * want.h[:, t].abs(), f"step {t}")
 
 
+@pytest.mark.parametrize("decay", [-1e-3, -0.4, -5.0, -40.0, -200.0, -2000.0])
+@pytest.mark.parametrize("batch,seqlen,dim", [(1, 5, 3), (2, 900, 66), (9, 1100, 3713)])
+def test_recurrence_infinite_states_stay(decay, batch, seqlen, dim):
+    """a is never 0: an infinite state, or gradient of one, stays what it is until a sequence ends, and no
+    neighbour sees it."""
+    announce("infinite states", decay, batch, seqlen, dim)
+    if dim > 1000 and decay != -40.0:
+        pytest.skip("the sizes whose backward passes segments on, once")
+    x, r, i, A, h0, _, go, gl = inputs(batch, seqlen, dim, "f32", carried=True)
+    A = torch.full_like(A, decay)
+    bad_h, bad_g, bad_x = h0.clone(), gl.clone(), x.clone()
+    bad_h[0, 0], bad_g[0, 1], bad_x[0, 2, 2] = INF, -INF, -INF
+
+    def run(x, h0, gl):
+        leaves = [t.clone().requires_grad_() for t in (x, r, i, A, h0)]
+        out = ops.gated_linear_recurrence(*leaves, None, True)
+        return [t.detach() for t in out], torch.autograd.grad(out, leaves, (go, gl))
+
+    (h, last), _ = run(bad_x, bad_h, gl)
+    assert bool((h[0, :, 0] == INF).all()) and float(last[0, 0]) == INF
+    assert bool((h[0, 2:, 2] == -INF).all()) and float(last[0, 2]) == -INF
+    (clean, clean_last), grads = run(x, h0, gl)
+    for p, q in ((h, clean), (last, clean_last)):
+        q = q.clone()
+        q[0, ..., 0], q[0, ..., 2] = p[0, ..., 0], p[0, ..., 2]
+        assert torch.equal(p, q)
+    assert torch.equal(h[0, :2, 2], clean[0, :2, 2])
+    _, (dx, dr, di, dA, dh0) = run(x, h0, bad_g)
+    assert float(dh0[0, 1]) == -INF and bool((dx[0, :, 1] == -INF).all())
+    for p, q in zip((dx, dr, di, dA, dh0), grads):
+        p, q = p.clone(), q.clone()
+        p[..., 1], q[..., 1] = 0, 0
+        assert torch.equal(p, q)
+    # one token at a time
+    state = bad_h
+    for t in range(min(seqlen, 12)):
+        state, y = ops.gated_linear_recurrence_update(state, bad_x[:, t], r[:, t], i[:, t], A)
+        assert torch.equal(state[0, 0], last[0, 0]) and float(y[0, 0]) == INF
+    assert float(state[0, 2]) == -INF
+    # until a sequence ends
+    seq = torch.zeros((batch, seqlen), dtype=torch.int32, device=DEV)
+    seq[:, 3:] = 1
+    h = ops.gated_linear_recurrence(bad_x, r, i, A, bad_h, seq)
+    assert bool((h[0, :3, 0] == INF).all()) and bool(h[:, 3:].isfinite().all())
+
+
 def test_recurrence_positive_decay():
     """A above 0 is not a decay: NaN in its channel, whatever its neighbours' are."""
     announce("positive A")

@@ -811,10 +811,11 @@ __global__ void __launch_bounds__(W * 64, 2) k_rec_backward(RecArgs a) {
                     c.e[v] = step<FAR>(kept[j][v], p, beta[j][v] * sxv);
                     dx[v] = lam[j][v] * beta[j][v] * s[j][v];
                     di[v] = dx[v] * xv * cosg[j][v];
-                    const float dLq = lam[j][v] * av * fmaf(-av * ib[j][v], sxv, p) * q[j][v];
+                    float dLq = lam[j][v] * av * fmaf(-av * ib[j][v], sxv, p) * q[j][v];
                     dr[v] = dLq * A[v] * cq[j][v];
+                    // (what a padded row carries through may be no number)
+                    if (SEQ && !c.s.is_live(j)) dx[v] = dr[v] = di[v] = dLq = 0.f;
                     dA[v] += dLq;
-                    if (SEQ && !c.s.is_live(j)) dx[v] = dr[v] = di[v] = 0.f;
                 }
                 ox.store(tx, j, dx);
                 orr.store(tr, j, dr);

@@ -119,14 +119,16 @@ def sharp_check(x, r, i, A, h0, seq, go, gl):
 DECAYS = [(0.3, 2.0), (16.0, 60.0), (1e-3, 200.0)]
 
 
-@pytest.mark.parametrize("low,high", DECAYS)
+# (the last of the sizes: rows whose backward passes segments on)
+STRONG = [(*size, *decay) for size in [(2, 300, 40, 0), (1, 1100, 70, 0), (3, 333, 65, 40)] for decay in DECAYS] + [
+    (9, 1100, 3713, 0, 16.0, 60.0)]
+
+
 @pytest.mark.parametrize("dtype", ["f32", "bf16"])
-@pytest.mark.parametrize("batch,seqlen,dim,packed", [(2, 300, 40, 0), (1, 1100, 70, 0), (3, 333, 65, 40), (9, 1100, 3713, 0)])
+@pytest.mark.parametrize("batch,seqlen,dim,packed,low,high", STRONG)
 def test_recurrence_keeps_small_inputs_behind_large_states(batch, seqlen, dim, packed, dtype, low, high):
     """What a strong decay leaves of a state, however large, does not round what comes in, forward or backward."""
     announce("strong decay", batch, seqlen, dim, packed, dtype, low, high)
-    if dim > 1000 and high != 60.0:
-        pytest.skip("the sizes whose backward passes segments on, once")
     x, r, i, A, h0, seq, go, gl = inputs(batch, seqlen, dim, dtype, packed=packed, carried=True, low=low, high=high)
     g = gen("spikes", batch, seqlen, dim, low)
     x, go = (spikes(t * 2.0 ** -10, g, 2.0 ** 24) for t in (x, go))
@@ -148,14 +150,15 @@ def test_update_keeps_small_inputs_behind_large_states(dtype, low, high):
         within(y, want.h[:, t], tol + u(y.dtype) * want.h[:, t].abs(), f"step {t}")
 
 
-@pytest.mark.parametrize("decay", [-1e-3, -0.4, -5.0, -40.0, -200.0, -2000.0])
-@pytest.mark.parametrize("batch,seqlen,dim", [(1, 5, 3), (2, 900, 66), (9, 1100, 3713)])
-def test_recurrence_infinite_states_stay(decay, batch, seqlen, dim):
+INFINITE = [(*size, decay) for size in [(1, 5, 3), (2, 900, 66)] for decay in (-1e-3, -0.4, -5.0, -40.0, -200.0, -2000.0)] + [
+    (9, 1100, 3713, -40.0)]
+
+
+@pytest.mark.parametrize("batch,seqlen,dim,decay", INFINITE)
+def test_recurrence_infinite_states_stay(batch, seqlen, dim, decay):
     """a is never 0: an infinite state, or gradient of one, stays what it is until a sequence ends, and no
     neighbour sees it."""
     announce("infinite states", decay, batch, seqlen, dim)
-    if dim > 1000 and decay != -40.0:
-        pytest.skip("the sizes whose backward passes segments on, once")
     x, r, i, A, h0, _, go, gl = inputs(batch, seqlen, dim, "f32", carried=True)
     A = torch.full_like(A, decay)
     bad_h, bad_g, bad_x = h0.clone(), gl.clone(), x.clone()
@@ -192,6 +195,32 @@ def test_recurrence_infinite_states_stay(decay, batch, seqlen, dim):
     seq[:, 3:] = 1
     h = ops.gated_linear_recurrence(bad_x, r, i, A, bad_h, seq)
     assert bool((h[0, :3, 0] == INF).all()) and bool(h[:, 3:].isfinite().all())
+
+
+@pytest.mark.parametrize("value", [INF, -INF, NAN])
+@pytest.mark.parametrize("seqlen", [7, 300])
+def test_recurrence_states_that_pass_padding_alone(value, seqlen):
+    """A row of padding hands its state on, whatever it is, and takes no part in any gradient but that state's."""
+    announce("padding alone", value, seqlen)
+    x, r, i, A, h0, _, go, gl = inputs(3, seqlen, 37, "f32", carried=True)
+    seq = torch.zeros((3, seqlen), dtype=torch.int32, device=DEV)
+    seq[1] = -1
+    seq[2, seqlen - 3:] = -1
+
+    def run(h0, gl):
+        leaves = [t.clone().requires_grad_() for t in (x, r, i, A, h0)]
+        out = ops.gated_linear_recurrence(*leaves, seq, True)
+        return [t.detach() for t in out], torch.autograd.grad(out, leaves, (go, gl))
+
+    (h, last), grads = run(h0, gl)
+    bad_h, bad_g = h0.clone(), gl.clone()
+    bad_h[1, 5], bad_g[1, 9] = value, value
+    (h2, last2), grads2 = run(bad_h, bad_g)
+    assert torch.equal(h, h2) and torch.equal(last2.view(torch.int32)[1], bad_h.view(torch.int32)[1])
+    for name, p, q in zip(("dx", "dr", "di", "dA"), grads, grads2):
+        assert torch.equal(p, q), name
+    got = grads2[4][1]
+    assert bool(((got == bad_g[1]) | (got.isnan() & bad_g[1].isnan())).all())
 
 
 def test_recurrence_positive_decay():

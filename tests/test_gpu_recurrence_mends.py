@@ -235,3 +235,80 @@ def test_recurrence_positive_decay():
         for t in (h, state[:, None], y[:, None]):
             bad = t.isnan()
             assert bool(bad[..., 3].all()) and not bool(bad[..., [0, 1, 2, 4, 5, 6, 7]].any())
+
+
+@pytest.mark.parametrize("batch,seqlen,dim,strides", [(3, 40, 16, (2 ** 31 + 8, 16, 1)), (1, 4200, 16, (0, 2 ** 20, 1))])
+def test_recurrence_in_place_past_32_bits(batch, seqlen, dim, strides):
+    """Views read in place whose rows, or positions, lie more than 2^32 bytes apart, forward and backward."""
+    announce("in place past 32 bits", batch, seqlen, dim, strides)
+    x, r, i, A, h0, _, go, gl = inputs(batch, seqlen, dim, "bf16", carried=True)
+    apart = dim if strides[1] > dim else seqlen * dim + 24           # of the four streams
+    base = torch.empty((batch - 1) * strides[0] + (seqlen - 1) * strides[1] + 4 * apart, device=DEV, dtype=torch.bfloat16)
+    assert 2 * base.numel() > 2 ** 32
+    views = [base.as_strided((batch, seqlen, dim), strides, k * apart).copy_(t) for k, t in enumerate((x, r, i, go))]
+    for v in views:
+        assert R._strided(v) is v
+
+    def run(x, r, i, go):
+        leaves = [t.detach().requires_grad_() for t in (x, r, i)] + [t.clone().requires_grad_() for t in (A, h0)]
+        out = ops.gated_linear_recurrence(*leaves, None, True)
+        return [*out, *torch.autograd.grad(out, leaves, (go, gl))]
+
+    for p, q in zip(run(*views), run(x, r, i, go)):
+        assert torch.equal(p, q)
+
+
+def test_recurrence_results_past_32_bits():
+    """Outputs, the states between them and gradients of more than 2^31 elements: the row's end against a row of its own."""
+    announce("results past 32 bits")
+    n, d, tail = 2 ** 21 + 261, 1032, 700
+    g = gen("huge")
+    x, r, i, go = (torch.empty((1, n, d), device=DEV, dtype=torch.bfloat16).normal_(generator=g) for _ in range(4))
+    assert x.numel() > 2 ** 31
+    A = -torch.rand(d, generator=g, device=DEV) - 1e-3
+    seq = torch.zeros((1, n), dtype=torch.int32, device=DEV)
+    seq[:, n - tail:] = 1
+    leaves = [t.requires_grad_() for t in (x, r, i)]
+    h, last = ops.gated_linear_recurrence(*leaves, A, None, seq, True)
+    grads = torch.autograd.grad(h, leaves, go)
+    cut = [t.detach()[:, n - tail:].contiguous() for t in (x, r, i)]
+    want = Sharp(*cut, A, None, None, go[:, n - tail:])
+    within(h[:, n - tail:], want.h, want.eh + u(h.dtype) * want.h.abs() + 1e-37, "h")
+    within(last, want.last, want.elast + 1e-37, "last")
+    for name, got in zip(("dx", "dr", "di"), grads):
+        ref = getattr(want, name)
+        within(got[:, n - tail:], ref, getattr(want, "e" + name) + u(got.dtype) * ref.abs() + 1e-36, name)
+
+
+def test_recurrence_differences_by_the_formula():
+    """The gradients against differences of the operator: what a central difference of step e is off by is taken
+    from the formula in 64 bits at the same points, and the sums' errors over e from their bounds."""
+    announce("differences by the formula")
+    for low, high in ((0.05, 0.5), (0.2, 6.0)):
+        x, r, i, A, h0, seq, go, gl = inputs(2, 120, 9, "f32", packed=50, carried=True, low=low, high=high)
+        leaves = [t.clone().requires_grad_() for t in (x, r, i, A, h0)]
+        run = lambda ts: ops.gated_linear_recurrence(*ts, seq, True)
+        dot = lambda h, last: float((h.double() * go.double()).sum() + (last.double() * gl.double()).sum())
+        grads = torch.autograd.grad(run(leaves), leaves, (go, gl))
+        want = Sharp(x, r, i, A, h0, seq, go, gl)
+        g = gen("differences by the formula", low)
+        e = 2.0 ** -4
+        for k, name in enumerate(("dx", "dr", "di", "dA", "dh0")):
+            t = (x, r, i, A, h0)[k]
+            d = torch.randn(t.shape, generator=g, device=DEV)
+            if name == "dA":
+                d = d * A.abs()
+            at = [[*(x, r, i, A, h0)] for _ in range(2)]
+            at[0][k], at[1][k] = t + e * d, t - e * d
+            refs = [Sharp(*ts, seq) for ts in at]
+            step = (at[0][k].double() - at[1][k].double()) / (2 * e)       # (as float32 has it)
+            exact = (dot(refs[0].h, refs[0].last) - dot(refs[1].h, refs[1].last)) / (2 * e)
+            slope = float((getattr(want, name) * step).sum())
+            noise = sum(float((q.eh * go.double().abs()).sum() + (q.elast * gl.double().abs()).sum()) for q in refs)
+            diff = (dot(*run(at[0])) - dot(*run(at[1]))) / (2 * e)
+            got = float((grads[k].double() * step).sum())
+            own = float((getattr(want, "e" + name) * step.abs()).sum())
+            tol = noise / (2 * e) + own + abs(exact - slope)
+            print(f"  {name}: {got:.6f} {diff:.6f} tolerance {tol:.2e}, of it the difference's own {abs(exact - slope):.2e}", flush=True)
+            assert abs(got - diff) <= tol
+            assert math.isfinite(tol) and tol < 0.05 * float((getattr(want, name).abs() * step.abs()).sum())

@@ -15,6 +15,7 @@ import os
 import threading
 
 import torch
+import torch.autograd.forward_ad as _forward_ad
 
 LIB_PATH = os.path.join(os.path.dirname(os.path.abspath(__file__)), "libm2ssd.so")
 
@@ -489,6 +490,16 @@ def device_of_two(a, b):
     except AttributeError:
         pass
     return device_of(a, b)              # says what is wrong
+
+
+def refuse_tangents(*tensors):
+    """Raise NotImplementedError where a tensor carries a forward-mode derivative (None entries ignored): a
+    result without one would read as a derivative of zero."""
+    if _forward_ad._current_level < 0:
+        return
+    for t in tensors:
+        if t is not None and _forward_ad.unpack_dual(t).tangent is not None:
+            raise NotImplementedError("no forward-mode derivatives: the kernels have backward passes only")
 
 
 def dev_contig(t, dtype=None):

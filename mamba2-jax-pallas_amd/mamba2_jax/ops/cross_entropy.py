@@ -121,6 +121,7 @@ def linear_cross_entropy(x, weight, targets, ignore_index=-100, reduction="mean"
     ignore_index = int(ignore_index)
     if (x.requires_grad or weight.requires_grad) and torch.is_grad_enabled():
         return _LinearCrossEntropy.apply(x, weight, targets, ignore_index, reduction)
+    L.refuse_tangents(x, weight)
     return _forward(x, weight, targets, ignore_index, reduction, False)[0]
 
 

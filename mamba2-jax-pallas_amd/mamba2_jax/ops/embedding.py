@@ -89,6 +89,7 @@ def embedding(ids, weight, scale=1.0, padding_idx=None):
     scale = float(scale)
     if weight.requires_grad and torch.is_grad_enabled():
         return _Embedding.apply(ids, weight, scale, padding_idx)
+    L.refuse_tangents(weight)
     return _lookup(dev, ids, weight, scale)
 
 

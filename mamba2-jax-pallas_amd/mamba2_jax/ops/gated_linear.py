@@ -99,6 +99,7 @@ def gated_linear(x, weight, activation="silu"):
     code = L.ACTIVATIONS[activation]
     if (x.requires_grad or weight.requires_grad) and torch.is_grad_enabled():
         return _GatedLinear.apply(x, weight, code)
+    L.refuse_tangents(x, weight)
     return _forward(x, weight, code, False)[0]
 
 

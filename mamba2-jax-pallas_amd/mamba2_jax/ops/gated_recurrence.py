@@ -183,6 +183,7 @@ def gated_linear_recurrence(x, r, i, A, initial_states=None, seq_idx=None, retur
     if torch.is_grad_enabled() and (x.requires_grad or r.requires_grad or i.requires_grad or A.requires_grad
                                     or (initial_states is not None and initial_states.requires_grad)):
         return _GatedRecurrence.apply(x, r, i, A, initial_states, seq_idx, want_final)
+    L.refuse_tangents(x, r, i, A, initial_states)
     out, final, _ = _forward(x, r, i, A, initial_states, seq_idx, want_final, False)
     return (out, final) if want_final else out
 
@@ -201,6 +202,7 @@ def gated_linear_recurrence_update(state, x, r, i, A, *, inplace=False):
         raise L.M2ShapeError(f"x.shape={tuple(shape)}, state.shape={tuple(state.shape)}: expected (batch, dim)")
     code = _check_gates(x, r, i, A, shape)
     L.dtype_code(state, "state")
+    L.refuse_tangents(state, x, r, i, A)
     src = _f32(state)
     new = src if inplace and src is state else torch.empty(shape, dtype=torch.float32, device=dev)
     if not (x.stride(1) == r.stride(1) == i.stride(1) == 1):

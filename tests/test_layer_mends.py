@@ -1,0 +1,31 @@
+"""What the operators of a trained layer, and the vocabulary's, refuse rather than answer without a derivative or past their
+launches' counts, without a GPU."""
+
+import ctypes
+
+import pytest
+import torch
+import torch.autograd.forward_ad as fwAD
+
+from mamba2_jax import _lib as L
+from mamba2_jax import ops
+from test_layer_ops_api import _fake, refused
+
+
+def test_forward_mode_derivatives_are_refused():
+    """An output without a tangent would read as a derivative of zero."""
+    x3, x2, A, w = _fake(2, 4, 8), _fake(3, 8), _fake(8), _fake(12, 8)
+    ids = torch.zeros(3, dtype=torch.int64).as_subclass(type(x3))
+    calls = [
+        (ops.gated_linear_recurrence, (x3, x3, x3, A, x3[:, 0].clone()), range(5)),
+        (ops.gated_linear_recurrence_update, (x2, x2, x2, x2, A), range(5)),
+        (ops.gated_linear, (x2, w), range(2)),
+        (ops.linear_cross_entropy, (x2, w, ids), range(2)),
+        (ops.embedding, (ids, w), [1]),
+    ]
+    with fwAD.dual_level():
+        for fn, args, at in calls:
+            for k in at:
+                dual = fwAD.make_dual(args[k].clone(), torch.ones_like(args[k]))
+                with pytest.raises(NotImplementedError, match="forward"):
+                    fn(*args[:k], dual, *args[k + 1:])

@@ -54,7 +54,7 @@ def layer(u, b, states=None, seq_idx=None):
 
 
 def layer_step(u, b, state):
-    """One token: u (batch, dim), state updated in place -> u behind the layer"""
+    """One token, under torch.no_grad(): u (batch, dim), state updated in place -> u behind the layer"""
     x, r, i = (u @ b["w_in"]).chunk(3, dim=-1)
     _, h = ops.gated_linear_recurrence_update(state, x, r, i, -torch.exp(b["A_log"]), inplace=True)
     u = u + h @ b["w_out"]

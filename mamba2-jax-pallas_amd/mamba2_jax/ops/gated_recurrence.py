@@ -195,7 +195,7 @@ def gated_linear_recurrence_update(state, x, r, i, A, *, inplace=False):
     state (batch, dim), batch at most 65535; x, r, i (batch, dim), all bfloat16 or all float32, rows with contiguous
     channels read in place; A (dim,).  The caller's state is left untouched, unless inplace=True (keyword
     only) and it is float32 and contiguous: it is then updated and returned.
-    Takes no gradients."""
+    Takes no gradients: an input that requires one is refused where they are recorded."""
     dev = _device(state, x, r, i, A)
     shape = x.shape
     if len(shape) != 2 or state.shape != shape:
@@ -203,6 +203,9 @@ def gated_linear_recurrence_update(state, x, r, i, A, *, inplace=False):
     code = _check_gates(x, r, i, A, shape)
     L.dtype_code(state, "state")
     L.refuse_tangents(state, x, r, i, A)
+    if torch.is_grad_enabled() and (state.requires_grad or x.requires_grad or r.requires_grad or i.requires_grad
+                                    or A.requires_grad):
+        raise L.M2ShapeError("a single step takes no gradients: call it under torch.no_grad(), or gated_linear_recurrence")
     src = _f32(state)
     new = src if inplace and src is state else torch.empty(shape, dtype=torch.float32, device=dev)
     if not (x.stride(1) == r.stride(1) == i.stride(1) == 1):

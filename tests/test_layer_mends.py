@@ -29,3 +29,13 @@ def test_forward_mode_derivatives_are_refused():
                 dual = fwAD.make_dual(args[k].clone(), torch.ones_like(args[k]))
                 with pytest.raises(NotImplementedError, match="forward"):
                     fn(*args[:k], dual, *args[k + 1:])
+
+
+def test_update_refuses_inputs_that_require_gradients():
+    """It takes no gradients: results without a graph would train nothing, and say nothing."""
+    x, A = _fake(3, 8), _fake(8)
+    for k in range(5):
+        args = [x.clone() for _ in range(4)] + [A.clone()]
+        args[k].requires_grad_()
+        with pytest.raises(L.M2ShapeError, match="no gradients"):
+            ops.gated_linear_recurrence_update(*args)

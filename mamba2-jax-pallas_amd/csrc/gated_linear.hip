@@ -312,19 +312,24 @@ struct PackArgs {
     bf16* dst;
     int64_t rows, dim, ld, dp, plane, half, valid;
 };
+constexpr int64_t PACK_ROWS = 1 << 24;       // of a launch, a wavefront each (a launch counts its threads in 32 bits)
 template <typename T> __global__ void __launch_bounds__(256) k_glu_pack(PackArgs a) {
-    const int64_t r = (int64_t)blockIdx.x * 4 + wave_id();
-    if (r >= a.rows) return;
     const int lane = threadIdx.x & 63;
-    const int second = a.half && r >= a.half;
-    const int64_t j = second ? r - a.half : r;
-    const bool in = j < a.valid;
-    const T* src = static_cast<const T*>(a.src) + (in ? j + (second ? a.valid : 0) : 0) * a.ld;
-    for (int64_t c = lane * 8; c < a.dp; c += 512) {
-        float v[8] = {0, 0, 0, 0, 0, 0, 0, 0};
-        if (in) load8(src, c, a.dim, v);
-        store8<sizeof(T) == 4>(a.dst + r * a.dp + c, a.plane, v);
+    for (int64_t r = (int64_t)blockIdx.x * 4 + wave_id(); r < a.rows; r += PACK_ROWS) {
+        const int second = a.half && r >= a.half;
+        const int64_t j = second ? r - a.half : r;
+        const bool in = j < a.valid;
+        const T* src = static_cast<const T*>(a.src) + (in ? j + (second ? a.valid : 0) : 0) * a.ld;
+        for (int64_t c = lane * 8; c < a.dp; c += 512) {
+            float v[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+            if (in) load8(src, c, a.dim, v);
+            store8<sizeof(T) == 4>(a.dst + r * a.dp + c, a.plane, v);
+        }
     }
+}
+template <typename T> void pack_rows(const PackArgs& a, hipStream_t s) {
+    const int64_t rows = a.rows < PACK_ROWS ? a.rows : PACK_ROWS;
+    hipLaunchKernelGGL(k_glu_pack<T>, dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, s, a);
 }
 
 struct DzArgs {
@@ -617,13 +622,13 @@ Kept kept(const Common& c, size_t bytes) {
 template <typename T> Operand operand_x(bf16* to, const Common& c, const void* x, int64_t ldx, bool pack, hipStream_t s) {
     if (!to) return Operand{static_cast<const bf16*>(x), ldx, 0, (int)c.n, (int)c.dim};
     const PackArgs a{x, to, c.np, c.dim, ldx, c.dp, c.np * c.dp, 0, c.n};
-    if (pack) hipLaunchKernelGGL(k_glu_pack<T>, dim3((unsigned)((c.np + 3) / 4)), dim3(256), 0, s, a);
+    if (pack) pack_rows<T>(a, s);
     return Operand{to, c.dp, c.np * c.dp, (int)c.np, (int)c.dp};
 }
 template <typename T> Operand operand_w(bf16* to, const Common& c, const void* w, int64_t ldw, bool pack, hipStream_t s) {
     if (!to) return Operand{static_cast<const bf16*>(w), ldw, 0, (int)c.hidden, (int)c.dim, (int)c.hidden};
     const PackArgs a{w, to, 2 * c.fp, c.dim, ldw, c.dp, 2 * c.fp * c.dp, c.fp, c.hidden};
-    if (pack) hipLaunchKernelGGL(k_glu_pack<T>, dim3((unsigned)(2 * c.fp / 4)), dim3(256), 0, s, a);
+    if (pack) pack_rows<T>(a, s);
     return Operand{to, c.dp, 2 * c.fp * c.dp, (int)c.fp, (int)c.dp, (int)c.fp};
 }
 
@@ -760,6 +765,11 @@ template <bool F32> BwdPlan plan_bwd(const m2_gated_linear_grad_args& a) {
     return p;
 }
 
+// wavefronts of k_glu_dz
+template <class S> int64_t dz_waves(const Common& c) {
+    return (int64_t)c.tm * c.tn * (S::BM * S::BN / 2 / 16 / (S::FM % 4 ? 16 : 32));
+}
+
 template <bool F32> int run_bwd(const m2_gated_linear_grad_args& a, const BwdPlan& p, hipStream_t s) {
     typedef typename std::conditional<F32, float, bf16>::type T;
     typedef Shapes<F32> P;
@@ -774,8 +784,7 @@ template <bool F32> int run_bwd(const m2_gated_linear_grad_args& a, const BwdPla
     const DzArgs d{a.saved, a.grad_out, dz, c.n, c.np, c.hidden, c.fp, a.ldg, plane, c.entries, c.tm, c.tn};
     auto make = [&](auto shape) {
         typedef decltype(shape) S;
-        const int64_t waves = (int64_t)c.tm * c.tn * (S::BM * S::BN / 2 / 16 / (S::FM % 4 ? 16 : 32));
-        hipLaunchKernelGGL((k_glu_dz<T, S>), dim3((unsigned)((waves + 3) / 4)), dim3(256), 0, s, d);
+        hipLaunchKernelGGL((k_glu_dz<T, S>), dim3((unsigned)((dz_waves<S>(c) + 3) / 4)), dim3(256), 0, s, d);
     };
     if (c.shape == 2) make(typename P::ZS());
     else if (c.shape == 1) make(typename P::ZM());
@@ -898,6 +907,9 @@ int launch_gated_linear_grad(const m2_gated_linear_grad_args& a, hipStream_t s) 
                "%s: x, weight, saved, grad_out and an output are required", who);
     M2_REQUIRE(al16(a.saved) && al16(a.workspace), M2_ERR_WORKSPACE, "%s: saved and workspace of 16-byte alignment needed", who);
     const BwdPlan p = plan(a);
+    int64_t waves = 0;
+    with_shape(p.c.f32, p.c.shape, [&](auto shape) { waves = dz_waves<decltype(shape)>(p.c); });
+    M2_REQUIRE(waves < (1 << 26) - 4, M2_ERR_UNSUPPORTED, "%s: too many tokens (a launch counts its threads in 32 bits)", who);
     M2_REQUIRE(p.kept.known, M2_ERR_WORKSPACE, "%s: saved of %zu bytes is no forward's of these sizes", who, a.saved_bytes);
     M2_REQUIRE(a.workspace && a.workspace_bytes >= p.total, M2_ERR_WORKSPACE,
                "%s: workspace of %zu bytes needed, %zu given", who, p.total, a.workspace_bytes);

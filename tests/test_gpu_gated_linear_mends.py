@@ -1,0 +1,59 @@
+"""The gated feed-forward product by the norms of its errors, which tell a lost part of an operand that bounds on single
+elements let pass, and at sizes past its launches' counts; against the formulas in 64 bits.
+
+F = 2^-24.  Of normal operands, float32:
+
+* A product over K adds up 6 K / 32 instructions' results with up to eight roundings each, at most F of a sum that grows
+  as the root of its length: of the result's norm (0.5 sqrt(K) + 1) F at most.  Without one of the three small products (of a high
+  and a low part, or of both middle ones) h, dx and dw would be off by 58 to 70 F of their norms (a part's rounding to
+  bfloat16 leaves 2^-9.2 of it, so each is about 2^-18.4 of its product's), without all three by 110.
+* h = act(g) v: errors of g and v as above reach h with the weights E act'^2 v^2 / E h^2 and 1, 1.44 together of normal g and
+  v (of either activation less than 1.5), act itself 6 F.  The factors of the gradient likewise.
+
+bfloat16: what the result is off by is the rounding of dz and its own, both of which the formulas in 64 bits show when
+they round at the same two places.  Factors cut to 24 bits (2^-15) add nothing to that; of 16 bits they would add a
+quarter.
+"""
+
+import math
+
+import pytest
+import torch
+
+from gpu_util import announce
+from mamba2_jax import ops
+from test_gpu_gated_linear import DEV, F, act, grads, inputs
+
+pytestmark = pytest.mark.gpu
+
+
+def formula(x, w, dh, activation, rounded=lambda t: t):
+    """(h, dx, dw) in 64 bits, dz and the results rounded by `rounded`"""
+    x, w, dh = (t.detach().double() for t in (x, w, dh))
+    g, v = (x @ w.t()).chunk(2, 1)
+    a, slope, _ = act(g, activation)
+    dz = rounded(torch.cat([dh * v * slope, dh * a], 1))
+    return rounded(a * v), rounded(dz @ w), rounded(dz.t().contiguous() @ x)
+
+
+def off(got, want):
+    return float((got.detach().double() - want).norm() / want.norm())
+
+
+# 1 to 64 tokens, then the small, middle and large tiles of the forward product
+TILES = [(1, 256, 256), (16, 256, 256), (64, 256, 2048), (64, 264, 40), (333, 250, 365), (2000, 256, 1000), (300, 256, 6912),
+         (1500, 256, 256)]
+
+
+def test_more_rows_than_a_launch_counts():
+    """Packing of more tokens than 2^32 threads would take a wavefront each."""
+    announce("many rows")
+    n = 2 ** 26 + 5
+    g = torch.Generator(device=DEV).manual_seed(3)
+    x = torch.randn((n, 1), generator=g, device=DEV).bfloat16()
+    w = torch.tensor([[0.75], [-1.5]], device=DEV).bfloat16()
+    h = ops.gated_linear(x, w)
+    for part in (slice(0, 1000), slice(2 ** 25 - 500, 2 ** 25 + 500), slice(n - 1000, n)):
+        t = x[part].double()
+        want = 0.75 * t * torch.sigmoid(0.75 * t) * (-1.5 * t)
+        assert bool(((h[part].double() - want).abs() <= (2.0 ** -8 + 40 * F) * want.abs() + 1e-37).all())

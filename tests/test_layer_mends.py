@@ -39,3 +39,13 @@ def test_update_refuses_inputs_that_require_gradients():
         args[k].requires_grad_()
         with pytest.raises(L.M2ShapeError, match="no gradients"):
             ops.gated_linear_recurrence_update(*args)
+
+
+def test_gated_linear_grad_refuses_more_rows_than_a_launch_counts():
+    lib = L.load_library()
+    for n, code, text in (((1 << 28) - 300, -4, "workspace of"), (1 << 28, -2, "too many tokens"), (1 << 29, -2, "too many tokens")):
+        a = L.GatedLinearArgs(x=4096, weight=4096, out=4096, n=n, dim=1, hidden=1, ldx=1, ldw=1, dtype=L.M2_BF16)
+        saved = lib.m2_gated_linear_saved_size(ctypes.byref(a))
+        refused("m2_gated_linear_grad", L.GatedLinearGradArgs(
+            x=4096, weight=4096, saved=4096, saved_bytes=saved, grad_out=4096, grad_x=4096, grad_weight=4096, n=n, dim=1, hidden=1,
+            ldx=1, ldw=1, ldg=1, dtype=L.M2_BF16), code, text)

@@ -483,7 +483,8 @@ int m2_embedding_grad(const m2_embedding_grad_args* a, void* stream);
  * that are left out reaches nothing (the rows must be readable).  A target outside [0, vocab)
  * that is not ignore_index makes its loss NaN, and so does a logit of +inf or NaN.  total (or NULL) takes the sum of the losses, over
  * max(1, the number of rows kept) with mean.  float32 operands are multiplied as three bf16
- * parts each (six products, about 2^-24 of each).  vocab, n < 2^30.
+ * parts each (six products, about 2^-24 of each).  vocab < 2^30, or 2^26 where weight is packed (float32, a dim that 64 does
+ * not divide), n / 4 + vocab / 2048 < 2^24.
  * No counterpart in the reference, whose models answer with logits
  * (models/mamba2_lm.py:213-216).
  * ------------------------------------------------------------------------- */

@@ -952,6 +952,13 @@ int check_sizes(const char* who, int64_t n, int64_t vocab, int64_t dim, int64_t 
     M2_REQUIRE((int64_t)tiles(vocab, 128) * tiles(n, 16) < (1ll << 28) || n > 64, M2_ERR_UNSUPPORTED,
                "%s: too large", who);
     M2_REQUIRE((int64_t)tiles(vocab, 256) * tiles(n, 256) < (1ll << 30), M2_ERR_UNSUPPORTED, "%s: too large", who);
+    // (a launch counts its threads in 32 bits: a wavefront for each token, and a workgroup for CLEAR rows of the vocabulary)
+    M2_REQUIRE((n + 67) / 4 + tiles(vocab, CLEAR) < (1 << 24), M2_ERR_UNSUPPORTED, "%s: too many rows", who);
+    return M2_OK;
+}
+// the same of weight's rows, where they are packed
+int check_packed(const char* who, const Common& c) {
+    M2_REQUIRE(!c.pack_w || (c.vocab + 3) / 4 < (1 << 24), M2_ERR_UNSUPPORTED, "%s: too many rows to pack", who);
     return M2_OK;
 }
 
@@ -1259,12 +1266,14 @@ namespace m2 {
 
 size_t linear_ce_saved(const m2_linear_cross_entropy_args& a) {
     if (check_sizes("linear_cross_entropy", a.n, a.vocab, a.dim, a.ldx, a.ldw, a.dtype, a.target_dtype)) return 0;
-    return common(a.n, a.vocab, a.dim, a.ldw, a.weight, a.dtype, true).at;
+    const Common c = common(a.n, a.vocab, a.dim, a.ldw, a.weight, a.dtype, true);
+    return check_packed("linear_cross_entropy", c) ? 0 : c.at;
 }
 
 size_t linear_ce_workspace(const m2_linear_cross_entropy_args& a) {
     if (check_sizes("linear_cross_entropy", a.n, a.vocab, a.dim, a.ldx, a.ldw, a.dtype, a.target_dtype)) return 0;
-    return fwd_plan(a).total;
+    const FwdPlan p = fwd_plan(a);
+    return check_packed("linear_cross_entropy", p.c) ? 0 : p.total;
 }
 
 int launch_linear_ce(const m2_linear_cross_entropy_args& a, hipStream_t s) {
@@ -1273,6 +1282,7 @@ int launch_linear_ce(const m2_linear_cross_entropy_args& a, hipStream_t s) {
     M2_REQUIRE(a.weight && (a.n == 0 || (a.x && a.targets)) && (a.loss || a.total), M2_ERR_INVALID,
                "%s: x, weight, targets and loss or total are required", who);
     const FwdPlan p = fwd_plan(a);
+    if (int rc = check_packed(who, p.c)) return rc;
     M2_REQUIRE(a.workspace && a.workspace_bytes >= p.total, M2_ERR_WORKSPACE,
                "%s: workspace of %zu bytes needed, %zu given", who, p.total, a.workspace_bytes);
     M2_REQUIRE(!a.saved || a.saved_bytes >= p.c.at, M2_ERR_WORKSPACE, "%s: saved of %zu bytes needed, %zu given",
@@ -1287,7 +1297,8 @@ int launch_linear_ce(const m2_linear_cross_entropy_args& a, hipStream_t s) {
 size_t linear_ce_grad_workspace(const m2_linear_cross_entropy_grad_args& a) {
     if (check_sizes("linear_cross_entropy_grad", a.n, a.vocab, a.dim, a.ldx, a.ldw, a.dtype, a.target_dtype))
         return 0;
-    return bwd_plan(a).total;
+    const BwdPlan p = bwd_plan(a);
+    return check_packed("linear_cross_entropy_grad", p.c) ? 0 : p.total;
 }
 
 int launch_linear_ce_grad(const m2_linear_cross_entropy_grad_args& a, hipStream_t s) {
@@ -1300,6 +1311,7 @@ int launch_linear_ce_grad(const m2_linear_cross_entropy_grad_args& a, hipStream_
                "%s: saved, or x, targets, loss and lse are required", who);
     M2_REQUIRE(a.grad_loss_stride >= 0, M2_ERR_INVALID, "%s: grad_loss stride", who);
     const BwdPlan p = bwd_plan(a);
+    if (int rc = check_packed(who, p.c)) return rc;
     M2_REQUIRE(!a.saved || a.saved_bytes >= p.c.at, M2_ERR_WORKSPACE, "%s: saved of %zu bytes needed, %zu given",
                who, p.c.at, a.saved_bytes);
     M2_REQUIRE(a.workspace && a.workspace_bytes >= p.total, M2_ERR_WORKSPACE,

@@ -41,6 +41,18 @@ def test_update_refuses_inputs_that_require_gradients():
             ops.gated_linear_recurrence_update(*args)
 
 
+def test_cross_entropy_refuses_more_rows_than_a_launch_counts():
+    """Packing takes a wavefront a row: 2^32 threads are not launched, and no kernel reads what none filled."""
+    ok = dict(x=4096, weight=4096, targets=4096, loss=4096, n=100, vocab=70, dim=60, ldx=60, ldw=60, dtype=L.M2_BF16,
+              target_dtype=L.M2_I32)
+    mk = lambda **k: L.LinearCrossEntropyArgs(**{**ok, **k})
+    lib = L.load_library()
+    for bad in (dict(n=1 << 26), dict(vocab=1 << 26), dict(n=1 << 29)):
+        refused("m2_linear_cross_entropy", mk(**bad), -2, "too many rows")
+        assert lib.m2_linear_cross_entropy_workspace_size(ctypes.byref(mk(**bad))) == 0
+    assert lib.m2_linear_cross_entropy_workspace_size(ctypes.byref(mk(n=(1 << 26) - 4096))) > 0
+
+
 def test_gated_linear_grad_refuses_more_rows_than_a_launch_counts():
     lib = L.load_library()
     for n, code, text in (((1 << 28) - 300, -4, "workspace of"), (1 << 28, -2, "too many tokens"), (1 << 29, -2, "too many tokens")):

@@ -45,6 +45,35 @@ TILES = [(1, 256, 256), (16, 256, 256), (64, 256, 2048), (64, 264, 40), (333, 25
          (1500, 256, 256)]
 
 
+@pytest.mark.parametrize("n,dim,hidden", TILES)
+@pytest.mark.parametrize("activation", ["silu", "gelu"])
+def test_float32_products_keep_every_part(n, dim, hidden, activation):
+    announce("every part", n, dim, hidden, activation)
+    x, w, dh = inputs(n, dim, hidden, "f32")
+    want = formula(x, w, dh, activation)
+    product = lambda k: (0.5 * math.sqrt(k) + 1) * F
+    h = 1.5 * product(dim) + 6 * F
+    for name, got, ref, tol in zip(("h", "dx", "dw"), grads(x, w, dh, activation), want,
+                                   (h, h + product(2 * hidden), h + product(n))):
+        e = off(got, ref)
+        print(f"  {name}: {e / F:.2f} F of {tol / F:.2f} F", flush=True)
+        assert e <= tol, name
+
+
+@pytest.mark.parametrize("n,dim,hidden", [(16, 512, 700), (64, 256, 2048), (333, 1001, 1365), (2000, 512, 1000), (300, 2560, 6912),
+                                          (3000, 640, 1024)])
+@pytest.mark.parametrize("activation", ["silu", "gelu"])
+def test_bfloat16_gradient_is_off_by_its_two_roundings(n, dim, hidden, activation):
+    announce("two roundings", n, dim, hidden, activation)
+    x, w, dh = inputs(n, dim, hidden, "bf16")
+    want = formula(x, w, dh, activation)
+    model = formula(x, w, dh, activation, lambda t: t.bfloat16().double())
+    for name, got, ref, m in zip(("h", "dx", "dw"), grads(x, w, dh, activation), want, model):
+        e, by = off(got, ref), off(m, ref)
+        print(f"  {name}: {e:.3e}, by the roundings {by:.3e}", flush=True)
+        assert e <= 1.08 * by, name
+
+
 def test_more_rows_than_a_launch_counts():
     """Packing of more tokens than 2^32 threads would take a wavefront each."""
     announce("many rows")

@@ -571,8 +571,10 @@ int m2_clip_grad_norm(const m2_clip_grad_norm_args* a, void* stream);
  *   log a[t] = A sigmoid(r[t]),  h[t] = a[t] h[t-1] + sqrt(1 - a[t]^2) sigmoid(i[t]) x[t]
  * with h[-1] = initial_states (0 without), A <= 0 and finite; float32, out = h rounded once.
  * With seq_idx the state is cleared before a position whose entry is not negative and differs from the
- * one before it; a position with a negative entry is padding: out is 0 there, the state passes it
- * unchanged, and what x, r and i hold there (they must be readable) reaches nothing.
+ * one before it (also where that one is padding, and so behind padding at a row's start); a position with a negative
+ * entry is padding: out is 0 there, the state passes it
+ * unchanged, and what x, r and i hold there (they must be readable) reaches nothing.  a is never 0: an infinite
+ * state, or gradient of one, stays infinite until its sequence ends.
  * final_states is the state behind the last position.  x, r and i are addressed through their strides of
  * batch and time (elements; channels are contiguous; of time 0, or dim to 2^20), e.g. as slices of one
  * projection's output.  dim <= 2^20, seqlen < 2^32,
@@ -657,7 +659,8 @@ int m2_gated_recurrence_update(const m2_gated_recurrence_update_args* a, void* s
  * among them gives NaN).  With saved (m2_gated_linear_saved_size bytes, 16-byte aligned, as the workspaces) what the gradient
  * reads is left there: act(g) and v act'(g) (of bf16 operands their upper 24 bits), and the operands
  * where the kernels do not read them in place (float32, as three bf16 parts; a dim or, of weight, a
- * hidden that 64 does not divide).  n < 2^30, hidden <= 2^21, hidden dim < 2^30.
+ * hidden that 64 does not divide).  n < 2^30, hidden <= 2^21, hidden + 64 times dim (rounded up to 64) < 2^30; the gradient
+ * of n hidden < 2^34, both rounded up to tiles of 256 and 128.
  * No counterpart in the reference, whose blocks have a mixer alone (models/mamba2_lm.py:196-211).
  * ------------------------------------------------------------------------- */
 #define M2_SILU 0

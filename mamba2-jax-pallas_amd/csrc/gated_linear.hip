@@ -219,7 +219,9 @@ struct FewArgs {
     int n, dim, hidden, gelu;
 };
 // Up to 16 MT tokens: a workgroup takes 8 FT of the hidden size, its NW wavefronts split K and meet in LDS.  Bound by W's
-// bytes: 1 token x 2560 x 6912 bf16 13.7 us, 16 tokens 15.4 (71 MB, 5.2 and 4.6 TB/s).
+// bytes: 1 token x 2560 x 6912 bf16 18.9 us, 16 tokens 23.8 (71 MB, 3.7 and 3.0 TB/s; 13.7 and 15.4 where a part of the weights
+// is in the last-level cache), float32 33, 35 and 64 tokens 61 (142 MB, 4.3, 4.0 and 2.3 TB/s: every pair of fragments splits
+// both of them in three anew).
 // The 16 rows of a matrix operand are 8 of the gate and the 8 of the values, so that lanes
 // l and l + 32 hold g and v of the same place; every weight is read once, x comes from the cache.
 // U steps of 32 of K are in flight: a step's operands are loaded again, U steps on, right behind its products.
@@ -670,7 +672,8 @@ template <typename T> void run_few(const m2_gated_linear_args& a, hipStream_t s)
         typedef std::integral_constant<int, 4> four;
         typedef std::integral_constant<int, 8> eight;
         // More of the hidden size for each workgroup reads x less often, as long as there are workgroups for most
-        // CUs: 16 tokens x 2560 x 6912 by 8, 16, 32: 29, 24, 22 us, 2048 x 1024: 6.6, 8.0, 11.7.
+        // CUs: 16 tokens x 2560 x 6912 by 8, 16, 32, of weights that no cache holds: 29, 25, 24 us, 2048 x 1024: 6.6, 8.0, 11.6;
+        // float32 45, 38, 35 and 12.6, 15.8, 24.
         const int64_t wgs = (a.hidden + 7) / 8;
         if (wgs < 2 * 192) with(one(), eight(), four());
         else if (wgs < 4 * 192) with(two(), eight(), two());

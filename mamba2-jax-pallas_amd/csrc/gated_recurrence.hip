@@ -10,18 +10,18 @@
 // threads of a wavefront (by lane shifts) and then of the wavefronts (by LDS) are joined to the state that each thread's run
 // begins with.  A workgroup has 64 channels, so that a step of a bf16 stream is a whole line of 128 bytes.
 //
-// Forward: bound by bytes, three streams read and one written, and nearly by vector instructions (about 60 an element, five of
+// Forward: bound by bytes, three streams read and one written, and nearly by vector instructions (41 to 45 an element, five of
 // them exponentials, reciprocals and roots).  Workgroups take a segment each of a row's length, hold it in registers, and
 // pass the states on between them, so that every input is read and every gate computed once, with the whole chip
-// busy on a single row: 16384 x 2560 bf16 82-107 us (336 MB, 3.1 to 4.1 TB/s; with a pass of its own for the states 119, all
-// of a slab by one workgroup 580), 8 x 2048 x 5120 165-176 us (671 MB, 3.8 to 4.1 TB/s).
+// busy on a single row: 16384 x 2560 bf16 77 us (336 MB, 4.4 TB/s; 85-94 with the clearing before it, where a pass of its own
+// for the states takes 119, and all of a slab by one workgroup 580), 8 x 2048 x 5120 147-161 us (671 MB, 4.2 to 4.6 TB/s).
 // It leaves the state that enters every span of 32 steps (float32, a sixteenth of a bf16 stream) for the backward.
 //
 // Backward: a workgroup walks from the last tile to the first, three tiles in flight, computes the states of a tile again
 // from the span's and joins both directions at once (a run's map backward, m -> P m + M, has the same P).  Where there are few
 // slabs a first pass finds what enters the segments of each; where there are more than run at once, segments pass it on.
-// About 100 vector instructions and 14 bytes an element: 8 x 2048 x 5120 294 us (1216 MB, 4.1 TB/s), 8 x 2048 x 4096, whose
-// 512 slabs run at once, 218-235 (973 MB, 4.1 to 4.5 TB/s).
+// 74 vector instructions and 14 bytes an element: 8 x 2048 x 5120 296-337 us (1216 MB, 3.6 to 4.1 TB/s: the kernel of one call
+// after the other under a trace), 8 x 2048 x 4096, whose 512 slabs run at once, 255 with its join (973 MB, 3.8 TB/s).
 //
 // Everything is float32 but what is loaded and stored.  Where log a >= NEAR alpha = 1 - a is kept in place of a: near
 // 1, where memories are long, a itself has too few bits (beta^2 = alpha (2 - alpha) loses none,
@@ -96,9 +96,9 @@ constexpr float INF = __builtin_inff();
 M2_DEV float exp_neg(float v) { return __builtin_amdgcn_exp2f(v * -LOG2E); }
 M2_DEV float sigmoid_of(float e) { return __builtin_amdgcn_rcpf(1.f + e); }
 M2_DEV float co_sigmoid(float e, float s) { return e <= 1.f ? e * s : 1.f - s; }
-// 1 - exp(L) for L <= 0: from NEAR on, where 1 - exp would cancel, -L times the polynomial of degree 5 with the smallest
-// largest relative error there (by Remez's exchange: 2^-29.4; with float32's roundings as far off as the series to L^8 / 8!,
-// 2^-23.3, in two instructions less), the exponential below
+// 1 - exp(L) from NEAR on, where 1 - exp would cancel: -L times a polynomial of degree 5, found by Remez's exchange and rounded
+// to float32 with its constant at 1.  As it stands its relative error is 2^-27.1 at most (at NEAR), and 2^-23.3 with the
+// roundings of its evaluation, as the series to L^8 / 8! has in two instructions more.
 constexpr float NEAR = -0.5f;
 M2_DEV float decay_near(float L) {
     float p = 0x1.2607a4p-10f;

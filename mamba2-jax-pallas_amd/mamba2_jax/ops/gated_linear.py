@@ -84,7 +84,7 @@ def gated_linear(x, weight, activation="silu"):
     bfloat16 operands 24 bits of each), and a packed copy of the operands that the kernels cannot read in
     place (float32, as three bfloat16 parts: 1.5 times each; a dim or hidden that 64 does not divide); the
     gradient of bfloat16 operands rounds its products with those to bfloat16 once.
-    Equal inputs give equal bits."""
+    Inputs that carry forward-mode derivatives are refused.  Equal inputs give equal bits."""
     dev = L.device_of_two(x, weight)
     shape = x.shape
     L.require(weight.dim() == 2 and shape and shape[-1] == weight.shape[1],

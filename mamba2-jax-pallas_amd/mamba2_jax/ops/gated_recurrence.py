@@ -156,15 +156,18 @@ def gated_linear_recurrence(x, r, i, A, initial_states=None, seq_idx=None, retur
     contiguous (slices of one projection's output, say) are read in place.  A (dim,), finite and <= 0 (a
     positive one gives NaN), float32 or bfloat16.  initial_states (batch, dim): h_{-1}, zeros by
     default.  seq_idx (batch, seqlen) int32 or int64 (of int32's range): where an entry differs from the one before it a new
-    sequence begins, with a state of zero (the first goes on from initial_states); a negative
+    sequence begins, with a state of zero (the one at a row's first position goes on from initial_states); a negative
     entry is padding: h is 0 there, the state passes it unchanged, its
-    gradients are 0 and what the inputs hold there (a NaN, say) reaches nothing.  The final
+    gradients are 0 and what the inputs hold there (a NaN, say) reaches nothing.  An entry behind padding differs from
+    it and begins a sequence: a row that begins with padding has no use for initial_states but as final states of
+    padding alone.  The final
     states are those behind the last position.
 
     Gates, states and sums are float32 (a state and the gradient that comes back to it never
     leave it between two positions); h and the gradients are rounded once.  Between the two the graph holds x, r, i and
     the states that enter every 32 positions.  Where a_t is 1 the root has no slope, and its part
-    of the gradient is taken as 0.  Equal inputs give equal bits."""
+    of the gradient is taken as 0.  a_t is never 0: an infinite state (or gradient of one) stays infinite until its sequence
+    ends.  Inputs that carry forward-mode derivatives are refused.  Equal inputs give equal bits."""
     dev = _device(x, r, i, A, initial_states, seq_idx)
     shape = x.shape
     L.require(len(shape) == 3, lambda: f"x.shape={tuple(shape)}: expected (batch, seqlen, dim)")

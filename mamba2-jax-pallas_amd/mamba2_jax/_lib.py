@@ -492,6 +492,12 @@ def device_of_two(a, b):
     return device_of(a, b)              # says what is wrong
 
 
+def require_saved(t, shape, dtype, what):
+    """Raise unless t, as autograd's saved-tensor hooks gave it back, is what was saved."""
+    if t.shape != shape or t.dtype != dtype:
+        raise M2ShapeError(f"{what}: saved as {tuple(shape)} {dtype}, given back as {tuple(t.shape)} {t.dtype}")
+
+
 def refuse_tangents(*tensors):
     """Raise NotImplementedError where a tensor carries a forward-mode derivative (None entries ignored): a
     result without one would read as a derivative of zero."""

@@ -43,14 +43,18 @@ def _forward(x, weight, targets, ignore_index, reduction, save):
 
 def _backward(ctx, grad):
     weight, saved = ctx.saved_tensors
-    shape, n, ignore_index, reduction, index_code = ctx.args
+    shape, n, ignore_index, reduction, index_code, weight_shape, dtype, size = ctx.args
+    # (hooks may have given them back at other places and strides)
+    L.device_of(weight, saved)
+    L.require_saved(weight, weight_shape, dtype, "weight")
     want_x, want_w = ctx.needs_input_grad[:2]
     dev, dim = weight.device, weight.shape[1]
     dx = weight.new_empty(shape) if want_x else None
     dw = weight.new_empty(weight.shape) if want_w else None
     if n == 0:
         return dx, None if dw is None else dw.zero_(), None, None, None
-    w = _rows(weight, dim)
+    L.require_saved(saved, (size,), torch.uint8, "the loss's kept rows")
+    w, saved = _rows(weight, dim), L.dev_contig(saved)
     g = grad.reshape(-1) if grad.dim() != 1 else grad
     if g.dtype != torch.float32:
         g = g.float()
@@ -72,7 +76,8 @@ class _LinearCrossEntropy(torch.autograd.Function):
         out, saved = _forward(x, weight, targets, ignore_index, reduction, True)
         # (x is not read again: its kept rows are in `saved`)
         ctx.save_for_backward(weight, saved)
-        ctx.args = x.shape, targets.numel(), ignore_index, reduction, L.index_code(targets, "targets")
+        ctx.args = (x.shape, targets.numel(), ignore_index, reduction, L.index_code(targets, "targets"), weight.shape,
+                    weight.dtype, 0 if saved is None else saved.numel())
         return out
 
     @staticmethod

@@ -38,15 +38,25 @@ def _forward(x, weight, activation, save):
 def _backward(ctx, grad):
     xr, w, saved = ctx.saved_tensors
     want_x, want_w = ctx.needs_input_grad[:2]
-    dim, hidden = w.shape[1], w.shape[0] // 2
+    x_shape, w_shape, size, dtype = ctx.saved_as
+    (n, dim), hidden = x_shape, w_shape[0] // 2
+    # (hooks may have given them back at other places and strides)
+    at = w.get_device()
+    if at < 0 or xr.get_device() != at or (n and saved.get_device() != at):
+        L.device_of(xr, w, saved)
+    if not (xr.shape == x_shape and w.shape == w_shape and xr.dtype == w.dtype == dtype):
+        L.require_saved(xr, x_shape, dtype, "x")
+        L.require_saved(w, w_shape, dtype, "weight")
+    xr, w = _rows(xr, dim), _rows(w, dim)
     dx = torch.empty(ctx.shape, dtype=w.dtype, device=w.device) if want_x else None
     dw = torch.empty(w.shape, dtype=w.dtype, device=w.device) if want_w else None
-    n = xr.shape[0]
     if n == 0:
         return dx, None if dw is None else dw.zero_(), None
+    L.require_saved(saved, size, torch.uint8, "the product's factors")
+    saved = L.dev_contig(saved)
     g = _rows(grad, hidden)
     args = L.GatedLinearGradArgs(
-        xr.data_ptr(), w.data_ptr(), saved.data_ptr(), saved.numel(), g.data_ptr(), L.ptr(dx), L.ptr(dw), n, dim,
+        xr.data_ptr(), w.data_ptr(), saved.data_ptr(), size[0], g.data_ptr(), L.ptr(dx), L.ptr(dw), n, dim,
         hidden, _stride(xr, dim), _stride(w, dim), _stride(g, hidden), L.dtype_code(w, "weight"),
         ctx.activation)
     L.call_with_workspace("m2_gated_linear_grad", args, w.device)
@@ -63,6 +73,7 @@ class _GatedLinear(torch.autograd.Function):
         # (the rows that were read: the same strides and alignment decide what lies in `saved`)
         ctx.save_for_backward(xr, w, saved)
         ctx.shape, ctx.activation = x.shape, activation
+        ctx.saved_as = xr.shape, w.shape, None if saved is None else saved.shape, w.dtype
         return h
 
     @staticmethod

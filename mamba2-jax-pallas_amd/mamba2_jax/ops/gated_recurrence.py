@@ -50,7 +50,7 @@ def _f32(t):
 
 
 def _forward(x, r, i, A, initial_states, seq_idx, want_final, save):
-    """-> (out, the final states or None, what the gradient reads)"""
+    """-> (out, the final states or None, what the gradient reads, x's, r's and i's strides in it)"""
     dev = x.device
     batch, seqlen, dim = x.shape
     x, r, i = _strided(x), _strided(r), _strided(i)
@@ -59,16 +59,38 @@ def _forward(x, r, i, A, initial_states, seq_idx, want_final, save):
     final = torch.empty((batch, dim), dtype=torch.float32, device=dev) if want_final else None
     spans = torch.empty((batch, -(-seqlen // L.RECURRENCE_SPAN), dim), dtype=torch.float32, device=dev) \
         if save else None
+    strides = sx, sr, si = x.stride(), r.stride(), i.stride()
     args = L.GatedRecurrenceArgs(
         x.data_ptr(), r.data_ptr(), i.data_ptr(), A.data_ptr(), L.ptr(h0), L.ptr(seq_idx),
-        out.data_ptr(), L.ptr(final), L.ptr(spans), batch, seqlen, dim, x.stride(0), x.stride(1),
-        r.stride(0), r.stride(1), i.stride(0), i.stride(1), L.dtype_code(x, "x"))
+        out.data_ptr(), L.ptr(final), L.ptr(spans), batch, seqlen, dim, sx[0], sx[1], sr[0], sr[1], si[0], si[1],
+        L.dtype_code(x, "x"))
     L.call_with_workspace("m2_gated_recurrence", args, dev)
-    return out, final, (x, r, i, A, seq_idx, spans)
+    return out, final, (x, r, i, A, seq_idx, spans), strides
+
+
+def _saved(ctx):
+    """What the forward saved, as the kernels read it: hooks may have given it back at other places and strides."""
+    x, r, i, A, seq_idx, spans = saved = ctx.saved_tensors
+    shape, dtype, spans_shape, strides = ctx.saved_as
+    _device(*saved)
+    if not (x.shape == r.shape == i.shape == shape and x.dtype == r.dtype == i.dtype == dtype and A.dtype == torch.float32
+            and A.shape == shape[2:] and spans.shape == spans_shape and spans.dtype == torch.float32
+            and (seq_idx is None or (seq_idx.shape == shape[:2] and seq_idx.dtype == torch.int32))):
+        for t in (x, r, i):
+            L.require_saved(t, shape, dtype, "x, r or i")
+        L.require_saved(A, shape[2:], torch.float32, "A")
+        L.require_saved(spans, spans_shape, torch.float32, "span states")
+        L.require_saved(seq_idx, shape[:2], torch.int32, "seq_idx")
+    if seq_idx is not None:
+        seq_idx = seq_idx.contiguous()
+    if (x.stride(), r.stride(), i.stride()) != strides:
+        x, r, i = _strided(x), _strided(r), _strided(i)
+        strides = x.stride(), r.stride(), i.stride()
+    return x, r, i, A.contiguous(), seq_idx, spans.contiguous(), strides
 
 
 def _backward(ctx, grad, grad_final=None):
-    x, r, i, A, seq_idx, spans = ctx.saved_tensors
+    x, r, i, A, seq_idx, spans, (sx, sr, si) = _saved(ctx)
     a_dtype, h0_dtype = ctx.dtypes
     batch, seqlen, dim = x.shape
     dev = x.device
@@ -88,8 +110,8 @@ def _backward(ctx, grad, grad_final=None):
     args = L.GatedRecurrenceGradArgs(
         x.data_ptr(), r.data_ptr(), i.data_ptr(), A.data_ptr(), L.ptr(seq_idx), spans.data_ptr(),
         g.data_ptr(), L.ptr(gf), dx.data_ptr(), dr.data_ptr(), di.data_ptr(), dA.data_ptr(),
-        L.ptr(dh0), batch, seqlen, dim, x.stride(0), x.stride(1), r.stride(0), r.stride(1),
-        i.stride(0), i.stride(1), g.stride(0), g.stride(1), L.dtype_code(x, "x"))
+        L.ptr(dh0), batch, seqlen, dim, sx[0], sx[1], sr[0], sr[1], si[0], si[1], g.stride(0), g.stride(1),
+        L.dtype_code(x, "x"))
     L.call_with_workspace("m2_gated_recurrence_grad", args, dev)
     if a_dtype != torch.float32:
         dA = dA.to(a_dtype)
@@ -105,8 +127,9 @@ class _GatedRecurrence(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, r, i, A, initial_states, seq_idx, want_final):
         ctx.set_materialize_grads(False)
-        out, final, saved = _forward(x, r, i, A, initial_states, seq_idx, want_final, True)
+        out, final, saved, strides = _forward(x, r, i, A, initial_states, seq_idx, want_final, True)
         ctx.save_for_backward(*saved)
+        ctx.saved_as = x.shape, x.dtype, saved[5].shape, strides
         ctx.dtypes = A.dtype, None if initial_states is None else initial_states.dtype
         return (out, final) if want_final else out
 
@@ -187,7 +210,7 @@ def gated_linear_recurrence(x, r, i, A, initial_states=None, seq_idx=None, retur
                                     or (initial_states is not None and initial_states.requires_grad)):
         return _GatedRecurrence.apply(x, r, i, A, initial_states, seq_idx, want_final)
     L.refuse_tangents(x, r, i, A, initial_states)
-    out, final, _ = _forward(x, r, i, A, initial_states, seq_idx, want_final, False)
+    out, final, _, _ = _forward(x, r, i, A, initial_states, seq_idx, want_final, False)
     return (out, final) if want_final else out
 
 

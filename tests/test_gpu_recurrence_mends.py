@@ -312,3 +312,45 @@ def test_recurrence_differences_by_the_formula():
             print(f"  {name}: {got:.6f} {diff:.6f} tolerance {tol:.2e}, of it the difference's own {abs(exact - slope):.2e}", flush=True)
             assert abs(got - diff) <= tol
             assert math.isfinite(tol) and tol < 0.05 * float((getattr(want, name).abs() * step.abs()).sum())
+
+
+def turned(t):
+    """t's values with its last dimension's stride the largest."""
+    return t.detach().movedim(-1, 0).contiguous().movedim(0, -1) if t.dim() > 1 else t.detach().clone()
+
+
+@pytest.mark.parametrize("bring", ["plain", "turned", "odd"])
+def test_saved_tensors_elsewhere(bring):
+    """What the graphs saved, given back at other places, strides and alignments: the same gradients."""
+    announce("saved elsewhere", bring)
+
+    def odd(t):
+        b = torch.empty(t.numel() + 1, device=t.device, dtype=t.dtype)[1:].view(t.shape)
+        return b.copy_(t.detach())
+
+    unpack = {"plain": lambda t: t.detach().clone(), "turned": turned, "odd": odd}[bring]
+    x, r, i, A, h0, seq, go, gl = inputs(2, 150, 24, "bf16", packed=40, carried=True)
+    g = gen("saved elsewhere")
+    rows, w = (torch.randn(s, generator=g, device=DEV) for s in ((70, 40), (96, 40)))
+    up = torch.randn((70, 48), generator=g, device=DEV)
+    targets = torch.randint(0, 96, (70,), generator=g, device=DEV)
+    calls = [
+        (lambda *t: ops.gated_linear_recurrence(*t, seq, True), (x, r, i, A, h0), (go, gl)),
+        (lambda *t: ops.gated_linear(*t), (rows, w), (up,)),
+        (lambda *t: ops.linear_cross_entropy(*t, targets), (rows, w), (torch.ones((), device=DEV),)),
+        (lambda t: ops.embedding(targets, t), (w,), (torch.randn((70, 40), generator=g, device=DEV),)),
+    ]
+    for fn, args, ups in calls:
+        def run(hooks):
+            leaves = [t.detach().clone().requires_grad_() for t in args]
+            if hooks is None:
+                out = fn(*leaves)
+            else:
+                with hooks:
+                    out = fn(*leaves)
+            return torch.autograd.grad(out, leaves, ups)
+
+        want = run(None)
+        for hooks in (torch.autograd.graph.saved_tensors_hooks(lambda t: t, unpack), torch.autograd.graph.save_on_cpu()):
+            for p, q in zip(run(hooks), want):
+                assert torch.equal(p, q)

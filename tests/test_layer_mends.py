@@ -61,3 +61,75 @@ def test_gated_linear_grad_refuses_more_rows_than_a_launch_counts():
         refused("m2_gated_linear_grad", L.GatedLinearGradArgs(
             x=4096, weight=4096, saved=4096, saved_bytes=saved, grad_out=4096, grad_x=4096, grad_weight=4096, n=n, dim=1, hidden=1,
             ldx=1, ldw=1, ldg=1, dtype=L.M2_BF16), code, text)
+
+
+@pytest.fixture
+def recorded(monkeypatch):
+    """The arguments of every launch, none of which takes place."""
+    calls = []
+    monkeypatch.setattr(L, "call_with_workspace", lambda name, args, device: calls.append((name, args)))
+    monkeypatch.setattr(L, "size_of", lambda name, args: 4096)
+    return calls
+
+
+def _turned(t):
+    """t's values with its last dimension's stride the largest."""
+    return t.movedim(-1, 0).contiguous().movedim(0, -1) if t.dim() > 1 else t
+
+
+def _operators():
+    x, g, w = _fake(3, 40, 8), _fake(5, 8), _fake(12, 8)
+    ids = torch.zeros(5, dtype=torch.int64).as_subclass(type(x))
+    seq = torch.zeros((3, 40), dtype=torch.int32).as_subclass(type(x))
+    return {
+        "recurrence": (lambda a: ops.gated_linear_recurrence(a, x, x, _fake(8), None, seq), x.clone()),
+        "gated linear": (lambda a: ops.gated_linear(a, w), g.clone()),
+        "loss": (lambda a: ops.linear_cross_entropy(g, a, ids), w.clone()),
+    }
+
+
+@pytest.mark.parametrize("name", list(_operators()))
+def test_saved_tensors_at_other_strides_are_read_as_they_lie(recorded, monkeypatch, name):
+    """Hooks that give back what a graph saved with other strides, or one element for all: the kernels are given rows that they
+    can read, and none reads past what there is."""
+    fn, leaf = _operators()[name]
+    leaf.requires_grad_()
+    monkeypatch.setattr(L, "device_of", lambda *ts: ts[0].device)         # (a hook's results are no fakes)
+    given = []
+
+    def one_for_all(t):
+        given.append(torch.zeros((), dtype=t.dtype).expand(t.shape))
+        return given[-1]
+
+    def turned(t):
+        given.append(_turned(t.detach()))
+        return given[-1]
+
+    for unpack in (one_for_all, turned):
+        given.clear()
+        with torch.autograd.graph.saved_tensors_hooks(lambda t: t, unpack):
+            out = fn(leaf)
+        recorded.clear()
+        torch.autograd.grad(out, leaf, torch.ones_like(out))
+        bad = {t.data_ptr() for t in given if t.numel() > 1 and not t.is_contiguous()}
+        assert bad and len(recorded) == 1
+        args = recorded[0][1]
+        pointers = {getattr(args, f) for f, kind in args._fields_ if kind is ctypes.c_void_p}
+        assert not pointers & bad
+
+
+@pytest.mark.parametrize("name", list(_operators()))
+@pytest.mark.parametrize("what", ["host", "shape", "type"])
+def test_saved_tensors_that_changed_are_refused(recorded, monkeypatch, name, what):
+    fn, leaf = _operators()[name]
+    leaf.requires_grad_()
+    if what != "host":
+        monkeypatch.setattr(L, "device_of", lambda *ts: ts[0].device)
+    change = {"host": lambda t: t.detach().clone(), "shape": lambda t: t.detach()[..., :-1],
+              "type": lambda t: t.detach().double() if t.is_floating_point() else t.detach().short()}[what]
+    with torch.autograd.graph.saved_tensors_hooks(lambda t: t, change):
+        out = fn(leaf)
+    recorded.clear()
+    with pytest.raises(ValueError, match="GPU tensors" if what == "host" else "given back as"):
+        torch.autograd.grad(out, leaf, torch.ones_like(out))
+    assert not recorded

@@ -22,7 +22,7 @@ import torch
 
 from gpu_util import announce
 from mamba2_jax import ops
-from test_gpu_gated_linear import DEV, F, act, grads, inputs
+from test_gpu_gated_linear import DEV, F, Reference, act, grads, inputs
 
 pytestmark = pytest.mark.gpu
 
@@ -86,3 +86,34 @@ def test_more_rows_than_a_launch_counts():
         t = x[part].double()
         want = 0.75 * t * torch.sigmoid(0.75 * t) * (-1.5 * t)
         assert bool(((h[part].double() - want).abs() <= (2.0 ** -8 + 40 * F) * want.abs() + 1e-37).all())
+
+
+@pytest.mark.parametrize("activation", ["silu", "gelu"])
+def test_gated_linear_differences_by_the_formula(activation):
+    """The gradients against differences of the operator: what a central difference of step e is off by is taken from
+    the formula in 64 bits at the same points, and the products' errors over e from their bounds."""
+    announce("differences by the formula", activation)
+    x, w, dh = inputs(90, 48, 40, "f32")
+    want = Reference(x, w, activation, dh)
+    got = grads(x, w, dh, activation)[1:]
+    g = torch.Generator(device=DEV).manual_seed(11)
+    e = 2.0 ** -4
+    up = dh.double()
+    for k, name in enumerate(("dx", "dw")):
+        t = (x, w)[k]
+        d = torch.randn(t.shape, generator=g, device=DEV) * (1.0 if k == 0 else 1 / math.sqrt(48))
+        at = [[x, w] for _ in range(2)]
+        at[0][k], at[1][k] = t + e * d, t - e * d
+        refs = [Reference(*p, activation) for p in at]
+        step = (at[0][k].double() - at[1][k].double()) / (2 * e)              # (as float32 has it)
+        exact = float(((refs[0].h - refs[1].h) * up).sum()) / (2 * e)
+        slope = float((getattr(want, name) * step).sum())
+        noise = sum(float((r.eh * up.abs()).sum()) for r in refs) / (2 * e)
+        own = float((getattr(want, "e" + name) * step.abs()).sum())
+        one = [ops.gated_linear(*p, activation).double() for p in at]
+        diff = float(((one[0] - one[1]) * up).sum()) / (2 * e)
+        mine = float((got[k].double() * step).sum())
+        tol = noise + own + abs(exact - slope)
+        print(f"  {name}: {mine:.5f} {diff:.5f} tolerance {tol:.2e}, of it the difference's own {abs(exact - slope):.2e}", flush=True)
+        assert abs(mine - diff) <= tol
+        assert tol < 0.05 * float((getattr(want, name).abs() * step.abs()).sum())
